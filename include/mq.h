@@ -49,7 +49,8 @@ extern "C" {
 /* Activation dtypes. */
 #define MQ_F32 0
 #define MQ_F16 1
-#define MQ_BF16 2 /* weights for the packers only */
+#define MQ_BF16 2 /* the packers' weights; activations of the int8, norm and beam operators */
+#define MQ_S8 3   /* int8 rows with an fp32 scale per row: an output of the norms */
 
 /* Quantisation methods of mq_quantize_q4. */
 #define MQ_Q4_MAX7 0   /* scale = fp16(max|w| / 7) */
@@ -340,6 +341,76 @@ MQ_API int mq_ep_expert_step(const uint16_t *rows, const int32_t *ids, const uin
  * (mq_moe_combine over the plan's slot_of). */
 MQ_API int mq_ep_combine(const float *ret, const int32_t *slot_of, const float *weights, int64_t tokens, int topk,
                          int64_t d, int add, float *y, const int *flags, int world, const int *epoch, void *stream);
+
+/* ---- int8 products: a scale per token and per output channel -------------------------------------------
+ * No counterpart kernel in the reference's hot path (its weights have at most 4 bits). An int8 matrix is
+ * rows of int8 values, 16-byte aligned, each row `ld` bytes after the last (ld % 16 == 0, ld >= k; k itself
+ * may be any number), with one fp32 scale per row. Activations of these operators are fp32, fp16 or bf16. */
+
+/* q[r][c] = rint(x[r][c] * (127 / a)), s[r] = a / 127 with a = max |x[r]|: quantises tokens, and weights
+ * once. A row of zeros gives q = 0, s = 0; a row with a NaN or an infinity q = 0, s = NaN (so the products
+ * of that row are NaN). x rows ldx elements apart; any cols up to 32768. rows == 0 does nothing. */
+MQ_API int mq_quantize_s8(const void *x, int x_dtype, int64_t ldx, int8_t *q, int64_t ldq, float *s, int64_t rows,
+                          int64_t cols, void *stream);
+
+/* y[t][r] (+)= xs[t] * ws[r] * sum_k xq[t][k] * wq[r][k] + bias[r] for t < m, r < n on the tcgen05 tensor
+ * cores: sums exact in int32 (k <= 131071), then fp32, rounded once to y's type. bias (may be NULL): fp32
+ * [n]. y: fp32, fp16 or bf16, rows ldy elements apart. Reproducible bit for bit. m == 0 does nothing. */
+MQ_API int mq_gemm_w8a8(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw, const float *ws,
+                        const float *bias, void *y, int y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, int add,
+                        void *stream);
+
+/* a[t][j] = silu(g) * u with g, u the products of rows j and f + j of the fused [2f][k] gate|up matrix,
+ * as mq_gemm_w8a8 computes them. */
+MQ_API int mq_gate_up_w8a8(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw, const float *ws,
+                           void *a, int a_dtype, int64_t lda, int64_t m, int64_t f, int64_t k, void *stream);
+
+/* ---- norms around a block ---------------------------------------------------------------------------------
+ * RMS norms with the gate, the residual and the quantisation beside them in one pass (rmsnorm and
+ * rmsnorm_pack of the reference run them as kernels of their own, qwen3/kernels/qwen3k.mojo:17-57). Rows of
+ * up to 32768 columns; every tensor has its own type and row stride (in elements). Statistics are fp32 (the
+ * squares of a row must not overflow it). */
+
+/* h[r] = x[r] / sqrt(mean(x[r]^2) + eps) * w. h_dtype MQ_S8: h is quantised as mq_quantize_s8 does, its
+ * scales in hs (fp32 [rows]); else hs is not used. rows == 0 does nothing. */
+MQ_API int mq_pre_norm(const void *x, int x_dtype, int64_t ldx, const void *w, int w_dtype, float eps, void *h,
+                       int h_dtype, int64_t ldh, float *hs, int64_t rows, int64_t cols, void *stream);
+
+/* out = residual + scale * gate * norm(y; w, eps), then h = mq_pre_norm(out; next_w, next_eps) from the
+ * sum before it is rounded to out's type. w NULL: y itself in the place of its norm. gate NULL: 1; else row
+ * r takes gate row r / rows_per_gate. h NULL: no norm follows. out has residual's type and may be the
+ * residual's own buffer. */
+MQ_API int mq_post_norm(const void *y, int y_dtype, int64_t ldy, const void *w, int w_dtype, float eps,
+                        const void *residual, int r_dtype, int64_t ldr, const void *gate, int gate_dtype, int64_t ldg,
+                        int64_t rows_per_gate, float scale, void *out, int64_t ldo, const void *next_w,
+                        int next_w_dtype, float next_eps, void *h, int h_dtype, int64_t ldh, float *hs, int64_t rows,
+                        int64_t cols, void *stream);
+
+/* ---- beam search -------------------------------------------------------------------------------------------
+ * mq_head_argmax's place when more than one hypothesis is kept. Token v of beam i of a request scores
+ * scores[i] + (logits[i][v] - log(sum exp(logits[i]))) in fp32; of a finished beam, eos scores scores[i]
+ * and every other token -inf. So does every token of a beam whose score is -inf or NaN, or whose logits are
+ * all -inf or hold a NaN or +inf (this last is reported through mq_device_status, 15). The `beams` best
+ * tokens of each request are taken in order, the lowest i * vocab + v among equal scores: next_scores,
+ * tokens, parents (the beam i), and next_finished (may be NULL): the parent was finished or the token is
+ * eos. logits: [batch * beams] rows of vocab, ld elements apart, fp32 / fp16 / bf16 (-inf masks a token).
+ * finished: bytes [batch][beams] or NULL; eos: a token, or -1 where finished is NULL. next_scores and
+ * next_finished may be the input buffers. beams <= 32. workspace: mq_beam_workspace_size() bytes, 16-byte
+ * aligned. batch == 0 does nothing. */
+MQ_API size_t mq_beam_workspace_size(int64_t batch, int beams, int64_t vocab);
+MQ_API int mq_beam_select(const void *logits, int dtype, int64_t ld, const float *scores, const uint8_t *finished,
+                          int eos, float *next_scores, int32_t *tokens, int32_t *parents, uint8_t *next_finished,
+                          int64_t batch, int beams, int64_t vocab, void *workspace, size_t workspace_bytes,
+                          void *stream);
+
+/* state[b][i] <- state[b][parents[b][i]] for every request b and beam i, in place, in each of nstates device
+ * tensors of one layout: row b * beams + i starts row_stride bytes after the last and holds outer[0] x
+ * outer[1] x outer[2] pieces of inner_bytes, outer_stride[] bytes apart. Only beams that change their parent
+ * are read and written. `states`, `outer` and `outer_stride` are host arrays, read before the call returns.
+ * A parent outside [0, beams) is reported (16) and its beam keeps its state. beams <= 32, batch <= 65535. */
+MQ_API int mq_beam_reorder(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
+                           int64_t row_stride, const int64_t *outer, const int64_t *outer_stride, int64_t inner_bytes,
+                           void *stream);
 
 /* ---- weight files -------------------------------------------------------------------------------- */
 

@@ -1,0 +1,561 @@
+// Beam search's selection over beams x vocabulary, and the states that follow their beams
+// (mq_beam_select, mq_beam_reorder).
+//
+// Candidate (beam i, token v) of a request scores c = score[i] + (logit[i][v] - lse[i]) with
+// lse = log(sum exp(logit[i])); of a finished beam the eos token scores score[i] and every other token
+// -inf; so does every token of a beam whose score is -inf or NaN or whose lse is not finite. The `beams`
+// largest are taken in order, the lowest flat index i * vocab + v among equal ones.
+//
+// beam_scan_kernel reads every logit once: `splits` CTAs per row, each thread keeps a running maximum and
+// sum of exponentials, the CTA the best kp = beams + 1 (logit, token) pairs of its part. Within a row the
+// score grows with the logit, so no other token can be among the `beams` best -- except where rounding
+// gives unequal logits equal scores; the pair beyond the `beams` best shows whether that can matter.
+// beam_merge_kernel, one CTA per request, joins the sums, scores the kept pairs and picks the best.
+// Bound by the bytes of the logits when there are many, by latency for one request.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+
+namespace mq {
+namespace beam {
+
+constexpr int kThreads = 256;
+constexpr int kMaxBeams = 32;
+constexpr int kMaxLists = 256;  // (beam, split) lists of a request: one per thread of the merge
+constexpr int kElems = 16;      // logits per thread and chunk
+constexpr int kChunk = kThreads * kElems;
+constexpr int kTargetCtas = 148 * 8;
+constexpr float kNegInf = -INFINITY;
+
+__host__ __device__ constexpr int splits_for(int64_t rows, int beams, int64_t vocab) {
+  const int64_t chunks = (vocab + kChunk - 1) / kChunk;
+  int64_t s = kTargetCtas / rows;
+  if (s > kMaxLists / beams) s = kMaxLists / beams;
+  if (s > chunks) s = chunks;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+// What one CTA leaves for the merge, followed by kp keys (best first, 0 = none).
+struct Part {
+  float top, sum;
+  int bad, count;
+};
+
+// Order-preserving bits of a float; -0 counts as +0.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+// Larger is better: the value, then the lower index.
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+  return static_cast<uint64_t>(order_of(v)) << 32 | (0xFFFFFFFFu - index);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
+__device__ __forceinline__ float value_of_key(uint64_t key) { return value_of(static_cast<uint32_t>(key >> 32)); }
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+struct ScanParams {
+  const void *logits;
+  const float *scores;
+  const uint8_t *finished;
+  uint8_t *parts;
+  int64_t ld;
+  int beams, vocab, splits, part_bytes;
+};
+
+__device__ __forceinline__ bool live_beam(const float *scores, const uint8_t *finished, int64_t row) {
+  return scores[row] > kNegInf && !(finished && finished[row]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) beam_scan_kernel(const ScanParams p) {
+  constexpr int V = 16 / sizeof(T), U = kElems / V;  // elements of a 16-byte vector, vectors per chunk
+  __shared__ uint64_t list[2][kMaxBeams + 1];
+  __shared__ uint64_t fresh[(kMaxBeams + 1) * kElems];
+  __shared__ uint64_t best_of[kThreads];
+  __shared__ uint64_t raised;
+  __shared__ int nfresh;
+  __shared__ float red[2][kThreads / 32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int64_t row = blockIdx.x / p.splits;
+  const int split = blockIdx.x % p.splits, tid = threadIdx.x, kp = p.beams + 1;
+  if (!live_beam(p.scores, p.finished, row)) return;
+  const T *x = static_cast<const T *>(p.logits) + row * p.ld;
+  // 16-byte vectors from the aligned address at or below x: vector g holds columns g * V - lead ...
+  const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  const int nvec = (p.vocab + lead + V - 1) / V;
+  const int chunks = (nvec + kThreads * U - 1) / (kThreads * U);
+  const int c_begin = static_cast<int>(static_cast<int64_t>(chunks) * split / p.splits);
+  const int c_end = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / p.splits);
+  if (tid == 0) nfresh = 0;
+  __syncthreads();
+
+  float m = -3.402823466e38f, s = 0.f;
+  int bad = 0, cur = 0, have = 0;
+  uint64_t bar = 0;  // a pair enters the list only above this key
+  for (int c = c_begin; c < c_end; ++c) {
+    float v[kElems];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int g = (c * U + u) * kThreads + tid, col = g * V - lead;
+      if (col >= 0 && col + V <= p.vocab) {
+        const uint4 q = ldg_stream_v4(x + col);
+        const T *e = reinterpret_cast<const T *>(&q);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[u * V + i] = to_float(e[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[u * V + i] = col + i >= 0 && col + i < p.vocab ? to_float(x[col + i]) : kNegInf;
+      }
+    }
+    float big = kNegInf;
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) {
+      bad |= !(v[i] < INFINITY);  // NaN or +infinity
+      big = fmaxf(big, v[i]);
+    }
+    if (big > m) {
+      s *= expf(m - big);
+      m = big;
+    }
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) s += expf(v[i] - m);
+    // The best pairs: threads whose largest key passes the bar offer theirs.
+    uint64_t mine = 0;
+    auto key_at = [&](int i) -> uint64_t {
+      const int col = ((c * U + i / V) * kThreads + tid) * V - lead + i % V;
+      return col >= 0 && col < p.vocab ? key_of(v[i], col) : 0;
+    };
+    if (bar == 0 || big >= value_of_key(bar)) {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) mine = max(mine, key_at(i));
+    }
+    const int offers = __syncthreads_count(mine > bar);
+    if (offers == 0) continue;
+    uint64_t limit = bar;
+    if (offers > kp) {
+      // kp threads' largest pairs are enough: no pair below the smallest of those kp can be kept. So at
+      // most kp * kElems pairs are written, whatever the order of the logits.
+      best_of[tid] = mine > bar ? mine : 0;
+      __syncthreads();
+      int rank = 0;
+      for (int j = 0; j < kThreads; ++j) rank += best_of[j] > mine;
+      if (mine > bar && rank == kp - 1) raised = mine - 1;
+      __syncthreads();
+      limit = raised;
+    }
+    if (mine > limit) {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) {
+        const uint64_t key = key_at(i);
+        if (key > limit) fresh[atomicAdd(&nfresh, 1)] = key;
+      }
+    }
+    __syncthreads();
+    const int n = have + nfresh, old = have;
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t key = i < old ? list[cur][i] : fresh[i - old];
+      int rank = 0;
+      for (int j = 0; j < old; ++j) rank += list[cur][j] > key;
+      for (int j = 0; j < n - old; ++j) rank += fresh[j] > key;
+      if (rank < kp) list[cur ^ 1][rank] = key;
+    }
+    __syncthreads();
+    if (tid == 0) nfresh = 0;
+    cur ^= 1;
+    have = min(n, kp);
+    bar = have == kp ? list[cur][kp - 1] : 0;
+    __syncthreads();
+  }
+
+  // Join the threads' maxima and sums, in one fixed order.
+  float top = m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (tid % 32 == 0) red[0][tid / 32] = top;
+  bad = __syncthreads_or(bad);
+  top = red[0][0];
+  for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, red[0][w]);
+  s *= expf(m - top);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (tid % 32 == 0) red[1][tid / 32] = s;
+  __syncthreads();
+  uint8_t *out = p.parts + static_cast<int64_t>(blockIdx.x) * p.part_bytes;
+  if (tid == 0) {
+    s = 0.f;
+    for (int w = 0; w < kThreads / 32; ++w) s += red[1][w];
+    *reinterpret_cast<Part *>(out) = Part{top, s, bad, have};
+  }
+  uint64_t *keys = reinterpret_cast<uint64_t *>(out + sizeof(Part));
+  for (int i = tid; i < have; i += kThreads) keys[i] = list[cur][i];
+}
+
+struct MergeParams {
+  const void *logits;
+  const float *scores;
+  const uint8_t *finished;
+  const uint8_t *parts;
+  float *next_scores;
+  int32_t *tokens, *parents;
+  uint8_t *next_finished;
+  int64_t ld;
+  int dtype, beams, vocab, splits, part_bytes, eos;
+};
+
+enum : int { kLive = 0, kFinished = 1, kDead = 2 };
+
+__device__ __forceinline__ float read_logit(const MergeParams &p, int64_t row, int v) {
+  const int64_t at = row * p.ld + v;
+  if (p.dtype == MQ_F32) return static_cast<const float *>(p.logits)[at];
+  if (p.dtype == MQ_F16) return __half2float(static_cast<const __half *>(p.logits)[at]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p.logits)[at]);
+}
+
+// The next value of the logits' type below v (finite, or -inf): its bit pattern one step down.
+__device__ __forceinline__ float next_below(float v, int dtype) {
+  if (!(v > kNegInf)) return kNegInf;
+  if (dtype == MQ_F32) {
+    const uint32_t b = __float_as_uint(v);
+    return __uint_as_float(v > 0.f ? b - 1 : v < 0.f ? b + 1 : 0x80000001u);
+  }
+  const uint16_t b = dtype == MQ_F16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  const uint16_t d = v > 0.f ? b - 1 : v < 0.f ? b + 1 : 0x8001;
+  return dtype == MQ_F16 ? __half2float(__ushort_as_half(d)) : __bfloat162float(__ushort_as_bfloat16(d));
+}
+
+__device__ __forceinline__ float score_of(float score, float logit, float lse) {
+  const float c = score + (logit - lse);
+  return c == c ? c : kNegInf;
+}
+
+// One CTA per request. Dynamic shared memory: kp keys per (beam, split) list.
+__global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams p) {
+  extern __shared__ uint64_t cand[];
+  __shared__ float lse[kMaxBeams], score[kMaxBeams];
+  __shared__ int kind[kMaxBeams];
+  __shared__ uint64_t red[kThreads / 32];
+  __shared__ uint64_t chosen[kMaxBeams];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, kp = p.beams + 1, lists = p.beams * p.splits;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.beams;
+  const uint8_t *parts = p.parts + row0 * p.splits * p.part_bytes;
+  auto part_of = [&](int l) { return reinterpret_cast<const Part *>(parts + static_cast<int64_t>(l) * p.part_bytes); };
+
+  for (int i = warp; i < p.beams; i += kThreads / 32) {
+    const float sc = p.scores[row0 + i];
+    int k = p.finished && p.finished[row0 + i] ? kFinished : sc > kNegInf ? kLive : kDead;
+    float total = 0.f;
+    if (k == kLive) {
+      float top = -3.402823466e38f;
+      int bad = 0;
+      for (int j = lane; j < p.splits; j += 32) {
+        top = fmaxf(top, part_of(i * p.splits + j)->top);
+        bad |= part_of(i * p.splits + j)->bad;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int j = lane; j < p.splits; j += 32) {
+        const Part *q = part_of(i * p.splits + j);
+        total += q->sum * expf(q->top - top);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      total = top + logf(total);
+      bad = __any_sync(0xffffffffu, bad);
+      if (bad || !(fabsf(total) < INFINITY)) k = kDead;
+      if (bad && lane == 0) raise_status(kStatusBeamNonFinite);
+    }
+    if (lane == 0) lse[i] = total, score[i] = sc == sc ? sc : kNegInf, kind[i] = k;
+  }
+  __syncthreads();
+
+  // List `tid`: its pairs as (score, flat index) keys, and the best of them.
+  uint64_t *own = cand + tid * kp;
+  uint64_t best = 0;
+  uint64_t last = 0;  // the logit key of a full list's last pair
+  if (tid < lists) {
+    const int i = tid / p.splits;
+    const uint32_t flat0 = static_cast<uint32_t>(i) * p.vocab;
+    int count = 0;
+    if (kind[i] == kLive) {
+      const Part *q = part_of(tid);
+      const uint64_t *keys = reinterpret_cast<const uint64_t *>(q + 1);
+      count = q->count;
+      for (int j = 0; j < count; ++j)
+        own[j] = key_of(score_of(score[i], value_of_key(keys[j]), lse[i]), flat0 + index_of(keys[j]));
+      if (count == kp) last = keys[kp - 1];
+    } else if (tid % p.splits == 0) {
+      const int at = kind[i] == kFinished ? p.eos : -1;
+      if (at >= 0) own[count++] = key_of(score[i], flat0 + at);
+      for (int v = 0; v < p.vocab && count < kp; ++v)
+        if (v != at) own[count++] = key_of(kNegInf, flat0 + v);
+    }
+    for (int j = count; j < kp; ++j) own[j] = 0;
+    for (int j = 0; j < kp; ++j) best = max(best, own[j]);
+  }
+  for (int k = 0; k < p.beams; ++k) {
+    uint64_t top = best;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    top = red[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) top = max(top, red[w]);
+    if (top == best && top) {  // keys are unique: one thread
+      chosen[k] = top;
+      best = 0;
+      for (int j = 0; j < kp; ++j) {
+        if (own[j] == top) own[j] = 0;
+        best = max(best, own[j]);
+      }
+    }
+    __syncthreads();
+  }
+
+  // Unequal logits with equal scores: a token that was not kept could tie with the last chosen one and
+  // have a lower index, where a full list's last pair ties with it and so would the next lower logit.
+  const uint32_t edge = static_cast<uint32_t>(chosen[p.beams - 1] >> 32);
+  bool open = false;
+  if (last) {
+    const int i = tid / p.splits;
+    const float l = value_of_key(last);
+    open = order_of(score_of(score[i], l, lse[i])) == edge &&
+           order_of(score_of(score[i], next_below(l, p.dtype), lse[i])) == edge;
+  }
+  if (__syncthreads_or(open)) {
+    // Take the ties from the logits themselves, in the order of their flat index.
+    __shared__ int warp_count[kThreads / 32];
+    int k = 0;
+    while (static_cast<uint32_t>(chosen[k] >> 32) != edge) ++k;  // the ones above the ties stay
+    __syncthreads();
+    for (int i = 0; i < p.beams && k < p.beams; ++i) {
+      for (int v0 = 0; v0 < p.vocab && k < p.beams; v0 += kThreads) {
+        const int v = v0 + tid;
+        bool tie = false;
+        if (v < p.vocab) {
+          float c = kNegInf;
+          if (kind[i] == kLive)
+            c = score_of(score[i], read_logit(p, row0 + i, v), lse[i]);
+          else if (kind[i] == kFinished && v == p.eos)
+            c = score[i];
+          tie = order_of(c) == edge;
+        }
+        const unsigned vote = __ballot_sync(0xffffffffu, tie);
+        if (lane == 0) warp_count[warp] = __popc(vote);
+        __syncthreads();
+        int at = k, all = 0;
+        for (int w = 0; w < kThreads / 32; ++w) {
+          if (w < warp) at += warp_count[w];
+          all += warp_count[w];
+        }
+        at += __popc(vote & ((1u << lane) - 1));
+        if (tie && at < p.beams) chosen[at] = static_cast<uint64_t>(edge) << 32 | (0xFFFFFFFFu - (static_cast<uint32_t>(i) * p.vocab + v));
+        k = min(p.beams, k + all);
+        __syncthreads();
+      }
+    }
+  }
+  if (tid < p.beams) {
+    const uint32_t flat = index_of(chosen[tid]);
+    const int parent = static_cast<int>(flat / static_cast<uint32_t>(p.vocab)), token = static_cast<int>(flat % static_cast<uint32_t>(p.vocab));
+    p.next_scores[row0 + tid] = value_of_key(chosen[tid]);
+    p.parents[row0 + tid] = parent;
+    p.tokens[row0 + tid] = token;
+    if (p.next_finished) p.next_finished[row0 + tid] = kind[parent] == kFinished || token == p.eos;
+  }
+}
+
+// ---- states ---------------------------------------------------------------------------------------
+
+constexpr int kMaxStates = 64;  // tensors of one launch
+struct ReorderParams {
+  void *states[kMaxStates];
+  const int32_t *parents;
+  int64_t row_stride;               // bytes from one beam's state to the next
+  int64_t outer_stride[3];          // bytes; outer dimensions, the last one fastest
+  uint32_t outer1, outer2;          // sizes of the last two outer dimensions
+  uint32_t vecs;                    // vectors of the contiguous inner part
+  int64_t items;                    // vectors of one beam's state
+  int beams;
+};
+
+// state[b][i] <- state[b][parent[i]] in place: a thread owns one vector position of a request, loads
+// what the moving beams need and then stores it, so no other thread touches what it reads or writes.
+template <typename V, int B>
+__global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
+  griddep_wait();
+  const int32_t *par = p.parents + static_cast<int64_t>(blockIdx.y) * p.beams;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (item >= p.items) return;
+  const int64_t o = item / p.vecs;
+  const uint32_t c = static_cast<uint32_t>(item - o * p.vecs);
+  const int64_t o12 = static_cast<int64_t>(p.outer1) * p.outer2;
+  const int64_t o0 = o / o12;
+  const uint32_t rest = static_cast<uint32_t>(o - o0 * o12);
+  uint8_t *base = static_cast<uint8_t *>(p.states[blockIdx.z]) + static_cast<int64_t>(blockIdx.y) * p.beams * p.row_stride +
+                  o0 * p.outer_stride[0] + rest / p.outer2 * p.outer_stride[1] + rest % p.outer2 * p.outer_stride[2] +
+                  static_cast<int64_t>(c) * sizeof(V);
+  V v[B];
+  uint32_t moves = 0;
+#pragma unroll
+  for (int i = 0; i < B; ++i) {
+    if (i < p.beams) {
+      const int from = par[i];
+      if (from < 0 || from >= p.beams) {
+        if (item == 0 && blockIdx.z == 0) raise_status(kStatusBeamBadParent);
+      } else if (from != i) {
+        v[i] = *reinterpret_cast<const V *>(base + from * p.row_stride);
+        moves |= 1u << i;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < B; ++i)
+    if (moves >> i & 1) *reinterpret_cast<V *>(base + i * p.row_stride) = v[i];
+}
+
+template <typename V>
+int reorder_launch(const ReorderParams &p, int batch, int nstates, cudaStream_t s) {
+  const int64_t blocks = (p.items + 255) / 256;
+  MQ_REQUIRE(blocks < (1LL << 31), MQ_EUNSUPPORTED, "mq_beam_reorder: a state is too large");
+  const dim3 grid(static_cast<unsigned>(blocks), batch, nstates);
+  const char *what = "mq_beam_reorder";
+  if (p.beams <= 4) return launch_overlapped(beam_reorder_kernel<V, 4>, grid, dim3(256), 0, s, what, p);
+  if (p.beams <= 8) return launch_overlapped(beam_reorder_kernel<V, 8>, grid, dim3(256), 0, s, what, p);
+  if (p.beams <= 16) return launch_overlapped(beam_reorder_kernel<V, 16>, grid, dim3(256), 0, s, what, p);
+  return launch_overlapped(beam_reorder_kernel<V, 32>, grid, dim3(256), 0, s, what, p);
+}
+
+}  // namespace beam
+}  // namespace mq
+
+extern "C" size_t mq_beam_workspace_size(int64_t batch, int beams, int64_t vocab) {
+  if (batch <= 0 || beams <= 0 || beams > mq::beam::kMaxBeams || vocab <= 0) return 0;
+  const int64_t rows = batch * beams;
+  return static_cast<size_t>(rows) * mq::beam::splits_for(rows, beams, vocab) * (sizeof(mq::beam::Part) + 8 * (beams + 1));
+}
+
+extern "C" int mq_beam_select(const void *logits, int dtype, int64_t ld, const float *scores, const uint8_t *finished,
+                              int eos, float *next_scores, int32_t *tokens, int32_t *parents, uint8_t *next_finished,
+                              int64_t batch, int beams, int64_t vocab, void *workspace, size_t workspace_bytes,
+                              void *stream) {
+  using namespace mq::beam;
+  const char *what = "mq_beam_select";
+  MQ_REQUIRE(batch >= 0 && beams > 0 && vocab > 0, MQ_EINVAL, "%s: bad shape", what);
+  MQ_REQUIRE(beams <= kMaxBeams, MQ_EUNSUPPORTED, "%s: beams is above %d", what, kMaxBeams);
+  MQ_REQUIRE(vocab * beams < (1LL << 31) - kChunk && batch * beams < (1LL << 22), MQ_EUNSUPPORTED,
+             "%s: beams * vocab or batch * beams is too large", what);
+  MQ_REQUIRE(dtype == MQ_F32 || dtype == MQ_F16 || dtype == MQ_BF16, MQ_EINVAL,
+             "%s: the logits' type must be MQ_F32, MQ_F16 or MQ_BF16", what);
+  MQ_REQUIRE(ld >= vocab, MQ_EINVAL, "%s: the logits' row stride is less than vocab", what);
+  MQ_REQUIRE(eos >= -1 && eos < vocab && !(finished && eos < 0), MQ_EINVAL,
+             "%s: eos must be a token (-1 only without finished)", what);
+  if (batch == 0) return MQ_OK;
+  MQ_REQUIRE(logits && scores && next_scores && tokens && parents && workspace, MQ_EINVAL, "%s: null pointer", what);
+  MQ_REQUIRE(mq::aligned(logits, dtype == MQ_F32 ? 4 : 2) && mq::aligned(scores, 4) && mq::aligned(next_scores, 4) &&
+                 mq::aligned(tokens, 4) && mq::aligned(parents, 4) && mq::aligned(workspace, 16),
+             MQ_EALIGN, "%s: the workspace must be 16-byte aligned, the others aligned to their elements", what);
+  MQ_REQUIRE(workspace_bytes >= mq_beam_workspace_size(batch, beams, vocab), MQ_EINVAL, "%s: the workspace is too small",
+             what);
+  mq::DeviceInfo dev;
+  if (int rc = mq::device_info(&dev)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t rows = batch * beams;
+  const int splits = splits_for(rows, beams, vocab), part = static_cast<int>(sizeof(Part)) + 8 * (beams + 1);
+  ScanParams sp{logits, scores, finished, static_cast<uint8_t *>(workspace), ld, beams, static_cast<int>(vocab), splits, part};
+  const dim3 grid(static_cast<unsigned>(rows * splits));
+  int rc;
+  if (dtype == MQ_F32)
+    rc = mq::launch_overlapped(beam_scan_kernel<float>, grid, dim3(kThreads), 0, s, what, sp);
+  else if (dtype == MQ_F16)
+    rc = mq::launch_overlapped(beam_scan_kernel<__half>, grid, dim3(kThreads), 0, s, what, sp);
+  else
+    rc = mq::launch_overlapped(beam_scan_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, s, what, sp);
+  if (rc) return rc;
+  MergeParams mp{logits, scores, finished, static_cast<const uint8_t *>(workspace), next_scores, tokens, parents, next_finished, ld, dtype,
+                 beams, static_cast<int>(vocab), splits, part, eos};
+  const size_t smem = static_cast<size_t>(kThreads) * (beams + 1) * 8;
+  static size_t configured[64] = {};
+  if (int rc2 = mq::ensure_smem(beam_merge_kernel, smem, configured, what)) return rc2;
+  return mq::launch_overlapped(beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(kThreads), smem, s, what, mp);
+}
+
+extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
+                               int64_t row_stride, const int64_t *outer, const int64_t *outer_stride, int64_t inner_bytes,
+                               void *stream) {
+  using namespace mq::beam;
+  const char *what = "mq_beam_reorder";
+  MQ_REQUIRE(nstates >= 0 && batch >= 0 && beams > 0 && inner_bytes >= 0, MQ_EINVAL, "%s: bad shape", what);
+  MQ_REQUIRE(beams <= kMaxBeams && batch <= 65535, MQ_EUNSUPPORTED, "%s: beams is above %d or batch above 65535", what,
+             kMaxBeams);
+  if (nstates == 0 || batch == 0 || inner_bytes == 0) return MQ_OK;
+  MQ_REQUIRE(states && parents && outer && outer_stride, MQ_EINVAL, "%s: null pointer", what);
+  // Every (row, outer index) must have bytes of its own: sorted by stride, each dimension has to step
+  // over all that the faster ones cover.
+  int64_t count = 1;
+  int align = 16;
+  auto divides = [&](int64_t v) { while (align > 1 && v % align) align /= 2; };
+  struct Dim { int64_t stride, size; };
+  Dim dims[4] = {{outer_stride[0], outer[0]}, {outer_stride[1], outer[1]}, {outer_stride[2], outer[2]},
+                 {row_stride, batch * beams}};
+  std::sort(dims, dims + 4, [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
+  int64_t extent = inner_bytes;
+  for (const Dim &d : dims) {
+    MQ_REQUIRE(d.size >= 0 && d.size < (1LL << 31), MQ_EINVAL, "%s: bad outer dimension", what);
+    if (d.size == 0) return MQ_OK;
+    if (d.size == 1) continue;
+    MQ_REQUIRE(d.stride >= extent, MQ_EINVAL, "%s: states overlap (a stride is less than what it steps over)", what);
+    divides(d.stride);
+    extent += d.stride * (d.size - 1);
+  }
+  for (int d = 0; d < 3; ++d) count *= outer[d];
+  MQ_REQUIRE(outer[1] * outer[2] < (1LL << 31), MQ_EUNSUPPORTED, "%s: the outer dimensions are too large", what);
+  divides(inner_bytes);
+  for (int i = 0; i < nstates; ++i) {
+    MQ_REQUIRE(states[i], MQ_EINVAL, "%s: null state", what);
+    divides(static_cast<int64_t>(reinterpret_cast<uintptr_t>(states[i]) % 16));
+  }
+  mq::DeviceInfo dev;
+  if (int rc = mq::device_info(&dev)) return rc;
+  ReorderParams p{};
+  p.parents = parents, p.row_stride = row_stride, p.beams = beams;
+  for (int d = 0; d < 3; ++d) p.outer_stride[d] = outer_stride[d];
+  p.outer1 = static_cast<uint32_t>(outer[1]), p.outer2 = static_cast<uint32_t>(outer[2]);
+  const int width = align == 16 ? 16 : align >= 4 ? 4 : align;
+  MQ_REQUIRE(inner_bytes / width < (1LL << 31), MQ_EUNSUPPORTED, "%s: the inner part is too large", what);
+  p.vecs = static_cast<uint32_t>(inner_bytes / width);
+  p.items = count * p.vecs;
+  for (int first = 0; first < nstates; first += kMaxStates) {
+    const int n = std::min(kMaxStates, nstates - first);
+    for (int i = 0; i < n; ++i) p.states[i] = states[first + i];
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int rc;
+    if (width == 16)
+      rc = reorder_launch<uint4>(p, static_cast<int>(batch), n, s);
+    else if (width == 4)
+      rc = reorder_launch<uint32_t>(p, static_cast<int>(batch), n, s);
+    else if (width == 2)
+      rc = reorder_launch<uint16_t>(p, static_cast<int>(batch), n, s);
+    else
+      rc = reorder_launch<uint8_t>(p, static_cast<int>(batch), n, s);
+    if (rc) return rc;
+  }
+  return MQ_OK;
+}

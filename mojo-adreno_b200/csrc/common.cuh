@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -122,6 +123,11 @@ enum : int {
   kStatusEpOverflow = 9,      // more pairs for one rank than the plan's capacity: the excess was left out
   kStatusEpDispatchWait = 10,  // an expert-parallel rank's rows did not arrive in time (the layer went on without them)
   kStatusEpReturnWait = 11,    // an owner's expert outputs did not come back in time
+  kStatusW8TmaWait = 12,
+  kStatusW8MmaWait = 13,
+  kStatusW8EpiWait = 14,
+  kStatusBeamNonFinite = 15,  // a beam's logits hold a NaN or +infinity: none of its tokens was selected
+  kStatusBeamBadParent = 16,  // a parent outside [0, beams): its beam kept its own state
 };
 
 // Waits until the kernels this grid depends on (earlier work on its stream) have completed and

@@ -11,3 +11,6 @@
 #include "pack.cu"
 #include "io.cu"
 #include "ep.cu"
+#include "gemm_w8a8.cu"
+#include "norm.cu"
+#include "beam.cu"

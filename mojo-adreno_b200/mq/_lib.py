@@ -6,6 +6,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 library_path = os.path.join(_HERE, "libmq.so")
 
 c_int, c_i64, c_vp, c_char_p, c_size = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t
+c_f32 = ctypes.c_float
 
 # name -> (restype, argtypes), in include/mq.h order.
 SIGNATURES = {
@@ -54,6 +55,17 @@ SIGNATURES = {
     "mq_ep_expert_step": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_i64, c_int, c_int, c_int,
                                   c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
     "mq_ep_combine": (c_int, [c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_vp, c_vp, c_int, c_vp, c_vp]),
+    "mq_quantize_s8": (c_int, [c_vp, c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp]),
+    "mq_gemm_w8a8": (c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_int,
+                             c_vp]),
+    "mq_gate_up_w8a8": (c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "mq_pre_norm": (c_int, [c_vp, c_int, c_i64, c_vp, c_int, c_f32, c_vp, c_int, c_i64, c_vp, c_i64, c_i64, c_vp]),
+    "mq_post_norm": (c_int, [c_vp, c_int, c_i64, c_vp, c_int, c_f32, c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_i64, c_f32,
+                             c_vp, c_i64, c_vp, c_int, c_f32, c_vp, c_int, c_i64, c_vp, c_i64, c_i64, c_vp]),
+    "mq_beam_workspace_size": (c_size, [c_i64, c_int, c_i64]),
+    "mq_beam_select": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_vp,
+                               c_size, c_vp]),
+    "mq_beam_reorder": (c_int, [c_vp, c_int, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_i64, c_vp]),
     "mq_read_file_to_device": (c_int, [c_vp, c_i64, c_char_p, c_i64, c_vp]),
     "mq_pack_half": (c_int, [c_vp, c_vp, c_i64, c_vp]),
 }

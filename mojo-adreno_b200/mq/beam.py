@@ -1,0 +1,100 @@
+"""Beam search over libmq: the selection over beams and vocabulary, and the states that follow their beams
+(head_argmax's place when more than one hypothesis is kept).
+"""
+import ctypes
+
+import torch
+
+from ._lib import MQError, lib
+from .int8 import _rows
+from .kernels import _need, _p, _stream
+from .pack import _DT
+
+__all__ = ["beam_select", "beam_reorder"]
+
+_FLAGS = (torch.uint8, torch.bool)
+
+
+def beam_select(logits, scores, finished=None, eos=-1, next_scores=None, tokens=None, parents=None, next_finished=None,
+                workspace=None):
+    """The `beams` best continuations of each request by scores[b, i] + log_softmax(logits[b, i])[v], the lowest
+    i * vocab + v among equal ones. logits fp32 / fp16 / bf16 [batch * beams, vocab] (-inf masks a token);
+    scores fp32 [batch, beams] (-inf: a beam not in use); finished uint8 / bool [batch, beams]: such a beam
+    goes on with `eos` alone, its score unchanged. Returns (next_scores, tokens, parents, next_finished), fp32, int32,
+    int32 and uint8 [batch, beams]; the parent is the beam's index within its request. A beam whose logits
+    hold a NaN or +inf is dropped and reported by device_status() (15)."""
+    if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
+        raise MQError(-1, "scores: expected a [batch, beams] tensor")
+    batch, beams = scores.shape
+    _need(scores, "scores", (torch.float32,))
+    rows, vocab, ld = _rows(logits, "logits", _DT, None, batch * beams)
+    if finished is not None:
+        _need(finished, "finished", _FLAGS, rows)
+    shape, dev = (batch, beams), logits.device
+    next_scores = torch.empty(shape, dtype=torch.float32, device=dev) if next_scores is None else next_scores
+    tokens = torch.empty(shape, dtype=torch.int32, device=dev) if tokens is None else tokens
+    parents = torch.empty(shape, dtype=torch.int32, device=dev) if parents is None else parents
+    next_finished = torch.empty(shape, dtype=torch.uint8, device=dev) if next_finished is None else next_finished
+    _need(next_scores, "next_scores", (torch.float32,), rows)
+    _need(tokens, "tokens", (torch.int32,), rows)
+    _need(parents, "parents", (torch.int32,), rows)
+    _need(next_finished, "next_finished", _FLAGS, rows)
+    nbytes = lib.mq_beam_workspace_size(batch, beams, vocab)
+    if workspace is None:
+        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    else:
+        _need(workspace, "workspace", (torch.uint8,))
+    lib.call("mq_beam_select", _p(logits), _DT[logits.dtype], ld, _p(scores), None if finished is None else _p(finished), eos,
+             _p(next_scores), _p(tokens), _p(parents), _p(next_finished), batch, beams, vocab, _p(workspace),
+             workspace.numel(), _stream())
+    return next_scores, tokens, parents, next_finished
+
+
+def _layout(t):
+    """(row stride, outer sizes, outer strides, inner bytes) of a state [rows, ..] in bytes: its dimensions
+    after the first, those without a gap between them merged, the innermost one contiguous."""
+    size = t.element_size()
+    inner, outer = size, []  # outer: (size, stride), fastest first
+    for n, st in sorted(zip(t.shape[1:], t.stride()[1:]), key=lambda d: d[1]):
+        st *= size
+        if n == 1:
+            continue
+        if not outer and st == inner:
+            inner *= n
+        elif outer and st == outer[-1][0] * outer[-1][1]:
+            outer[-1] = (outer[-1][0] * n, outer[-1][1])
+        else:
+            outer.append((n, st))
+    if len(outer) > 3:
+        raise MQError(-1, "states: at most three gaps between a state's dimensions")
+    outer = [(1, 0)] * (3 - len(outer)) + outer[::-1]
+    return t.stride(0) * size, [n for n, _ in outer], [st for _, st in outer], inner
+
+
+def beam_reorder(states, parents):
+    """state[b * beams + i] <- state[b * beams + parents[b, i]] in place for each tensor of `states` (one tensor or
+    a list, e.g. every layer's keys and values): [batch * beams, ..] of any type, their other dimensions
+    in any order, sliced or not (a cache's filled part: cache[:, :, :length]). parents int32 [batch,
+    beams], as beam_select gives them. Only beams that change their parent are copied. Returns states."""
+    each = [states] if isinstance(states, torch.Tensor) else list(states)
+    if not isinstance(parents, torch.Tensor) or parents.dim() != 2:
+        raise MQError(-1, "parents: expected a [batch, beams] tensor")
+    _need(parents, "parents", (torch.int32,))
+    batch, beams = parents.shape
+    groups = {}
+    for t in each:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise MQError(-1, "states: expected CUDA tensors (there is no CPU path)")
+        if t.dim() < 2 or t.shape[0] != batch * beams:
+            raise MQError(-1, f"states: shape {tuple(t.shape)} is not [{batch * beams}, ..]")
+        if t.numel():
+            groups.setdefault((t.shape, t.stride(), t.dtype), []).append(t)
+    if batch == 0 or beams == 0:
+        return states
+    stream = _stream()
+    for same in groups.values():  # one launch for all states of one layout
+        row, outer, strides, inner = _layout(same[0])
+        n = len(same)
+        lib.call("mq_beam_reorder", (ctypes.c_void_p * n)(*[t.data_ptr() for t in same]), n, _p(parents), batch, beams, row,
+                 (ctypes.c_int64 * 3)(*outer), (ctypes.c_int64 * 3)(*strides), inner, stream)
+    return states
