@@ -83,16 +83,9 @@ thread_local CUtensorMap t_maps[kTmapCache];
 thread_local int t_nkeys = 0, t_next = 0;
 }  // namespace
 
-int encode_tmap_2d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,
-                   uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
-                   CUtensorMapSwizzle swizzle, const char *what) {
-  const TmapKey key{base, cols, rows, row_stride_bytes, box_cols, box_rows, static_cast<int>(dtype),
-                    static_cast<int>(swizzle)};
-  for (int i = 0; i < t_nkeys; ++i)
-    if (t_keys[i] == key) {
-      *map = t_maps[i];
-      return MQ_OK;
-    }
+int encode_tmap_2d_now(CUtensorMap *map, const void *base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,
+                       uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
+                       CUtensorMapSwizzle swizzle, const char *what) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(MQ_ECUDA, "%s: cuTensorMapEncodeTiled is not available from the driver", what);
   if (reinterpret_cast<uintptr_t>(base) % 16 || row_stride_bytes % 16 || (box_cols * elem_bytes) % 16)
@@ -104,6 +97,22 @@ int encode_tmap_2d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype
   CUresult r = fn(map, dtype, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MQ_ECUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, static_cast<int>(r));
+  return MQ_OK;
+}
+
+int encode_tmap_2d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,
+                   uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
+                   CUtensorMapSwizzle swizzle, const char *what) {
+  const TmapKey key{base, cols, rows, row_stride_bytes, box_cols, box_rows, static_cast<int>(dtype),
+                    static_cast<int>(swizzle)};
+  for (int i = 0; i < t_nkeys; ++i)
+    if (t_keys[i] == key) {
+      *map = t_maps[i];
+      return MQ_OK;
+    }
+  if (int rc = encode_tmap_2d_now(map, base, dtype, elem_bytes, cols, rows, row_stride_bytes, box_cols, box_rows, swizzle,
+                                  what))
+    return rc;
   t_keys[t_next] = key;
   t_maps[t_next] = *map;
   t_next = (t_next + 1) % kTmapCache;

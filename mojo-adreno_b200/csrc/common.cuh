@@ -34,22 +34,32 @@ int device_info(DeviceInfo *out);
 // (programmatic dependent launch). Such a kernel runs only set-up that touches no global memory
 // (barriers, TMEM, descriptor prefetch) before griddep_wait(); after it, every write of earlier
 // work on the stream is visible, exactly as with an ordinary launch.
+// cluster > 1: in clusters of that many CTAs along x.
 template <typename... KArgs, typename... Args>
-int launch_overlapped(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const char *what,
-                      Args... args) {
+int launch_overlapped_clusters(void (*kern)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem,
+                               cudaStream_t stream, const char *what, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
   if (e != cudaSuccess) return fail(MQ_ECUDA, "%s: launch: %s", what, cudaGetErrorString(e));
   return check_launch(what);
+}
+
+template <typename... KArgs, typename... Args>
+int launch_overlapped(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const char *what,
+                      Args... args) {
+  return launch_overlapped_clusters(kern, grid, block, 1, smem, stream, what, args...);
 }
 
 namespace gemv {
@@ -76,6 +86,10 @@ int gemm_q4_run(const uint32_t *wq, const uint16_t *ws, const void *x, int x_dty
 int encode_tmap_2d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,
                    uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
                    CUtensorMapSwizzle swizzle, const char *what);
+// The same, encoded at every call (62 ns on the host) instead of kept with the thread's last maps.
+int encode_tmap_2d_now(CUtensorMap *map, const void *base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,
+                       uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows,
+                       CUtensorMapSwizzle swizzle, const char *what);
 // A 3-D map: `planes` copies of a [rows][cols] matrix, plane_stride_bytes apart (two row blocks of
 // one matrix, fetched by one box).
 int encode_tmap_3d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype, int elem_bytes, uint64_t cols,

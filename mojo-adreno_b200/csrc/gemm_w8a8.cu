@@ -231,11 +231,11 @@ int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params 
   p.stages = static_cast<int>(std::min<size_t>(kMaxStages, (dev.smem_optin - 4096) / slot));
   const size_t smem = static_cast<size_t>(p.stages) * slot + 1024;
   CUtensorMap wmap, xmap;
-  if (int rc = encode_tmap_2d(&wmap, wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, static_cast<uint64_t>(P) * p.n, ldw, kBK,
-                              kRows, CU_TENSOR_MAP_SWIZZLE_128B, what))
+  if (int rc = encode_tmap_2d_now(&wmap, wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, static_cast<uint64_t>(P) * p.n, ldw,
+                                  kBK, kRows, CU_TENSOR_MAP_SWIZZLE_128B, what))
     return rc;
-  if (int rc = encode_tmap_2d(&xmap, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, p.m, ldx, kBK, p.bn,
-                              CU_TENSOR_MAP_SWIZZLE_128B, what))
+  if (int rc = encode_tmap_2d_now(&xmap, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, p.m, ldx, kBK, p.bn,
+                                  CU_TENSOR_MAP_SWIZZLE_128B, what))
     return rc;
   auto kern = w8a8_kernel<P>;
   static size_t configured[64] = {};
@@ -263,6 +263,23 @@ int check(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int6
 }  // namespace w8
 }  // namespace mq
 
+#include "gemm_w8a8_tile.cu"
+
+namespace mq {
+namespace w8 {
+
+template <int P>
+int run(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, const Params &p, cudaStream_t stream,
+        const char *what) {
+  DeviceInfo dev;
+  if (int rc = device_info(&dev)) return rc;
+  if (p.m > 256) return launch_tile<P>(xq, ldx, wq, ldw, p, stream, dev, what);
+  return launch<P>(xq, ldx, wq, ldw, p, stream, dev, what);
+}
+
+}  // namespace w8
+}  // namespace mq
+
 extern "C" int mq_gemm_w8a8(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw,
                             const float *ws, const float *bias, void *y, int y_dtype, int64_t ldy, int64_t m, int64_t n,
                             int64_t k, int add, void *stream) {
@@ -270,12 +287,10 @@ extern "C" int mq_gemm_w8a8(const int8_t *xq, int64_t ldx, const float *xs, cons
   if (int rc = mq::w8::check(xq, ldx, xs, wq, ldw, ws, y, y_dtype, ldy, m, n, n, k, what)) return rc;
   MQ_REQUIRE(mq::aligned(bias, 4), MQ_EALIGN, "%s: bias must be 4-byte aligned", what);
   if (m == 0) return MQ_OK;
-  mq::DeviceInfo dev;
-  if (int rc = mq::device_info(&dev)) return rc;
   mq::w8::Params p{};
   p.xs = xs, p.ws = ws, p.bias = bias, p.y = y, p.ldy = ldy, p.y_dtype = y_dtype, p.add = add != 0;
   p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.k = static_cast<int>(k);
-  return mq::w8::launch<1>(xq, ldx, wq, ldw, p, static_cast<cudaStream_t>(stream), dev, what);
+  return mq::w8::run<1>(xq, ldx, wq, ldw, p, static_cast<cudaStream_t>(stream), what);
 }
 
 extern "C" int mq_gate_up_w8a8(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw,
@@ -284,10 +299,8 @@ extern "C" int mq_gate_up_w8a8(const int8_t *xq, int64_t ldx, const float *xs, c
   const char *what = "mq_gate_up_w8a8";
   if (int rc = mq::w8::check(xq, ldx, xs, wq, ldw, ws, a, a_dtype, lda, m, f, 2 * f, k, what)) return rc;
   if (m == 0) return MQ_OK;
-  mq::DeviceInfo dev;
-  if (int rc = mq::device_info(&dev)) return rc;
   mq::w8::Params p{};
   p.xs = xs, p.ws = ws, p.y = a, p.ldy = lda, p.y_dtype = a_dtype;
   p.m = static_cast<int>(m), p.n = static_cast<int>(f), p.k = static_cast<int>(k);
-  return mq::w8::launch<2>(xq, ldx, wq, ldw, p, static_cast<cudaStream_t>(stream), dev, what);
+  return mq::w8::run<2>(xq, ldx, wq, ldw, p, static_cast<cudaStream_t>(stream), what);
 }
