@@ -23,9 +23,14 @@ namespace w8 {
 constexpr int kRows = 128;      // weight rows of a tile (the MMA's M)
 constexpr int kBK = 128;        // k per stage: one 128-byte swizzled row
 constexpr int kMaxStages = 12;
-constexpr int kThreads = 192;   // warp 0 TMA, warp 1 MMA + TMEM, warps 2-5 epilogue
+constexpr int kEpiWarps = 4;    // one per TMEM lane quarter; eight measured slower (4.4 -> 5.8 us for 1x2048x2048)
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // warp 0 TMA, warp 1 MMA + TMEM, then the epilogue
 constexpr int kWBytes = kRows * kBK;
+constexpr int kMaxSplits = 4;   // clusters of 8 with this much shared memory did not all fit at once (4.9 -> 8.3 us)
 constexpr int64_t kMaxK = 131071;  // 128 * 128 * k stays below 2^31
+// 128-k blocks per stage: eight MMAs for each wait and commit of the issuing thread, which cost it about
+// 0.17 us together (four 128 x 16 MMAs take 0.1 us).
+__host__ __device__ constexpr int sub_blocks(int planes) { return planes == 1 ? 2 : 1; }
 
 struct Params {
   const float *xs, *ws, *bias;
@@ -34,6 +39,7 @@ struct Params {
   int y_dtype, add;
   int m, n, k;      // n: output columns (f of the gate|up form)
   int bn, tiles_m, tiles;
+  int splits;       // CTAs of a cluster that share a tile's k (1: persistent CTAs, each tile's k whole)
   int stages, buf_cols, tmem_cols;  // TMEM columns of one accumulator buffer (all planes), allocated
 };
 
@@ -53,32 +59,71 @@ __host__ __device__ constexpr uint32_t umma_idesc_i8(int m, int n) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void store_out(void *y, int dtype, int64_t at, float v, int add) {
-  if (dtype == MQ_F32) {
-    float *p = static_cast<float *>(y) + at;
-    *p = add ? *p + v : v;
-  } else if (dtype == MQ_F16) {
-    __half *p = static_cast<__half *>(y) + at;
-    *p = __float2half_rn(add ? __half2float(*p) + v : v);
-  } else {
-    __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(y) + at;
-    *p = __float2bfloat16_rn(add ? __bfloat162float(*p) + v : v);
-  }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of the same shared variable in the CTA of the given rank of this cluster.
+__device__ __forceinline__ uint32_t map_shared(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_remote_v4(uint32_t cluster_addr, int4 v) {
+  asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
 }
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+
+// y[at] (+)= v in y's type. `put` is instantiated per type so that a loop over it holds no branch on the type.
+template <typename T>
+__device__ __forceinline__ void put(void *y, int64_t at, float v, int add) {
+  T *p = static_cast<T *>(y) + at;
+  *p = from_float<T>(add ? static_cast<float>(*p) + v : v);
+}
+template <typename F>
+__device__ __forceinline__ void by_type(int dtype, F f) {
+  if (dtype == MQ_F32)
+    f(float());
+  else if (dtype == MQ_F16)
+    f(__half());
+  else
+    f(__nv_bfloat16());
+}
+
+// silu(g) * u with the fast exponential and quotient: their errors, (2 + 1.2 |g|) and 2 ulp, are below what
+// one rounding of g does to silu for large |g|; the accurate forms cost the epilogue several times as much.
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
 template <int P>  // weight planes of a tile: 1, or 2 (gate and up)
 __global__ void __launch_bounds__(kThreads, 1)
     w8a8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Params p) {
+  constexpr int SUB = sub_blocks(P);
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2];
+  __shared__ __align__(16) float token_scale[kEpiWarps][256];  // a copy for each epilogue warp
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int S = p.stages, slot_bytes = P * kWBytes + p.bn * kBK;
-  const int nkb = (p.k + kBK - 1) / kBK;
+  const int S = p.stages, sub_bytes = P * kWBytes + p.bn * kBK, slot_bytes = SUB * sub_bytes;
+  const int nst_all = (p.k + SUB * kBK - 1) / (SUB * kBK);
+  const int split = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int st0 = nst_all * split / p.splits, nst = nst_all * (split + 1) / p.splits - st0;
+  const int first = blockIdx.x / p.splits, step = gridDim.x / p.splits;
 
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
@@ -88,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 128);
+      mbar_init(&tempty[i], 32 * kEpiWarps);
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -98,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  bool live = false;  // an epilogue warp of a split tile whose sums are in TMEM
   griddep_wait();
 
   if (warp == 0) {
@@ -107,10 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     int s = 0, round = 0;
     int64_t issued = 0;
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+    bool ok = true;
+    for (int t = first; ok && t < p.tiles; t += step) {
       const int m0 = t % p.tiles_m * p.bn, n0 = t / p.tiles_m * kRows;
-      bool ok = true;
-      for (int kb = 0; kb < nkb; ++kb) {
+      for (int st = 0; st < nst; ++st) {
         if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[s], (round - 1) & 1))) {
           if (lane == 0) {
             raise_status(kStatusW8TmaWait);
@@ -121,15 +167,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (lane == 0) mbar_expect_tx(&full[s], slot_bytes);
         __syncwarp();
-        if (lane <= P) {  // lanes 0 .. P - 1: the weight planes; lane P: the tokens
-          const bool w = lane < P;
-          tma_load_2d(ring + s * slot_bytes + lane * kWBytes, w ? &wmap : &xmap, &full[s], kb * kBK,
-                      w ? n0 + lane * p.n : m0);
+        if (lane < SUB * (P + 1)) {  // per 128 k: P weight planes, then the tokens; one instruction for all
+          const int j = lane / (P + 1), q = lane % (P + 1);
+          tma_load_2d(ring + s * slot_bytes + j * sub_bytes + q * kWBytes, q < P ? &wmap : &xmap, &full[s],
+                      ((st0 + st) * SUB + j) * kBK, q < P ? n0 + q * p.n : m0);
         }
         ++issued;
         if (++s == S) s = 0, ++round;
       }
-      if (!ok) break;
     }
     // Leave no copy in flight: the last load issued into each slot has landed before the CTA ends.
     if (lane == 0)
@@ -139,24 +184,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t idesc = umma_idesc_i8(kRows, p.bn);
       int s = 0, it = 0;
       uint32_t ph = 0;
-      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
+      for (int t = first; t < p.tiles; t += step, ++it) {
         const int b = it & 1;
         bool ok = mbar_wait(&tempty[b], ((it >> 1) & 1) ^ 1);
         tc_fence_after();
-        for (int kb = 0; ok && kb < nkb; ++kb) {
+        for (int st = 0; ok && st < nst; ++st) {
           if (!mbar_wait(&full[s], ph)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t base = smem_u32(ring + s * slot_bytes);
-          const uint64_t db = umma_desc_sw128(base + P * kWBytes);
 #pragma unroll
-          for (int q = 0; q < P; ++q) {
-            const uint64_t da = umma_desc_sw128(base + q * kWBytes);
-            const uint32_t d = tmem + b * p.buf_cols + q * (p.buf_cols / P);
+          for (int u = 0; u < SUB; ++u) {
+            const uint64_t db = umma_desc_sw128(base + u * sub_bytes + P * kWBytes);
 #pragma unroll
-            for (int j = 0; j < kBK / 32; ++j) umma_i8(d, da + 2 * j, db + 2 * j, idesc, kb != 0 || j != 0);
+            for (int q = 0; q < P; ++q) {
+              const uint64_t da = umma_desc_sw128(base + u * sub_bytes + q * kWBytes);
+              const uint32_t d = tmem + b * p.buf_cols + q * (p.buf_cols / P);
+#pragma unroll
+              for (int j = 0; j < kBK / 32; ++j) umma_i8(d, da + 2 * j, db + 2 * j, idesc, st != 0 || u != 0 || j != 0);
+            }
           }
           umma_commit(&empty[s]);
           if (++s == S) s = 0, ph ^= 1;
@@ -173,9 +221,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    float *sx = token_scale[warp - 2];
     int it = 0;
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
+    for (int t = first; t < p.tiles; t += step, ++it) {
       const int b = it & 1;
+      // The scales are fetched while the tile is still being multiplied.
+      const int m0 = t % p.tiles_m * p.bn, toks = min(p.bn, p.m - m0), r = t / p.tiles_m * kRows + row;
+      const bool in = r < p.n;
+      const float sw = in ? p.ws[r] : 0.f, su = in && P == 2 ? p.ws[p.n + r] : 0.f;
+      const float bias = in && P == 1 && p.bias ? p.bias[r] : 0.f;
+      __syncwarp();
+      for (int i = lane; i < toks; i += 32) sx[i] = p.xs[m0 + i];
+      __syncwarp();
       const bool ok = !abort_flag && mbar_wait(&tfull[b], (it >> 1) & 1);
       if (!__all_sync(0xffffffffu, ok && !abort_flag)) {
         if (lane == 0 && !abort_flag) {
@@ -185,28 +242,107 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
-      const int m0 = t % p.tiles_m * p.bn, r = t / p.tiles_m * kRows + row;
-      const bool live = r < p.n;
-      const float sw = live ? p.ws[r] : 0.f, su = live && P == 2 ? p.ws[p.n + r] : 0.f;
-      const float bias = live && P == 1 && p.bias ? p.bias[r] : 0.f;
-      for (int c0 = 0; c0 < p.bn; c0 += 32) {
+      if (p.splits > 1) {  // the one tile of this cluster: joined below
+        live = true;
+        break;
+      }
+      for (int c0 = 0; c0 < toks; c0 += 32) {
         float v[32], u[32];
         tmem_ld32(tmem + b * p.buf_cols + lanes + c0, v);
         if (P == 2) tmem_ld32(tmem + b * p.buf_cols + p.buf_cols / P + lanes + c0, u);
-        if (live) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int tok = m0 + c0 + j;
-            if (c0 + j >= p.bn || tok >= p.m) break;
-            const float sx = p.xs[tok];
-            float out = static_cast<float>(__float_as_int(v[j])) * sx * sw + bias;
-            if (P == 2) out = silu_mul(out, static_cast<float>(__float_as_int(u[j])) * sx * su);
-            store_out(p.y, p.y_dtype, tok * p.ldy + r, out, p.add);
+        for (int j = 0; j < 32; j += 4) {
+          if (c0 + j >= toks) break;
+          const float4 s4 = *reinterpret_cast<const float4 *>(sx + c0 + j);
+          const float sj[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float &o = v[j + i];
+            o = static_cast<float>(__float_as_int(o)) * sj[i] * sw + bias;
+            if (P == 2) o = silu_mul(o, static_cast<float>(__float_as_int(u[j + i])) * sj[i] * su);
           }
         }
+        if (in)
+          by_type(p.y_dtype, [&](auto type) {
+            using T = decltype(type);
+            T *const y = static_cast<T *>(p.y) + (m0 + c0) * p.ldy + r;
+            if (p.add) {
+              const T *from = y;
+#pragma unroll
+              for (int j = 0; j < 32; ++j, from += p.ldy)
+                if (c0 + j < toks) v[j] += static_cast<float>(*from);
+            }
+            T *to = y;
+#pragma unroll
+            for (int j = 0; j < 32; ++j, to += p.ldy)
+              if (c0 + j < toks) *to = from_float<T>(v[j]);
+          });
       }
       tc_fence_before();
       mbar_arrive(&tempty[b]);
+    }
+  }
+  if (p.splits > 1) {
+    // Join the splits' int32 sums through distributed shared memory: CTA s finishes rows s * rs .. of the
+    // tile. The parts land in its ring, [split][plane][4 tokens][row] of int4, once every CTA's MMAs are
+    // done with theirs.
+    cluster_sync_all();
+    const int rs = kRows / p.splits;  // 64 or 32
+    const int m0 = first % p.tiles_m * p.bn, toks = min(p.bn, p.m - m0), quads = p.bn / 4;
+    if (live) {
+      const int row = (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t dst = map_shared(smem_u32(ring), row / rs) + (split * P * quads * rs + row % rs) * 16;
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+        for (int c0 = 0; c0 < toks; c0 += 32) {
+          float v[32];
+          tmem_ld32(tmem + q * (p.buf_cols / P) + lanes + c0, v);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            if (c0 + j < toks)
+              st_remote_v4(dst + (q * quads + (c0 + j) / 4) * rs * 16,
+                           make_int4(__float_as_int(v[j]), __float_as_int(v[j + 1]), __float_as_int(v[j + 2]),
+                                     __float_as_int(v[j + 3])));
+        }
+    }
+    cluster_sync_all();
+    // kThreads is a multiple of rs: a thread keeps its row and takes every kThreads / rs-th group of 4 tokens.
+    const int row = threadIdx.x % rs, r = first / p.tiles_m * kRows + split * rs + row;
+    if (r < p.n && !abort_flag) {
+      const int4 *parts = reinterpret_cast<const int4 *>(ring) + row;
+      const float sw = p.ws[r], su = P == 2 ? p.ws[p.n + r] : 0.f, bias = P == 1 && p.bias ? p.bias[r] : 0.f;
+      by_type(p.y_dtype, [&](auto type) {
+        using T = decltype(type);
+        T *y = static_cast<T *>(p.y) + m0 * p.ldy + r;
+        for (int g = threadIdx.x / rs; 4 * g < toks; g += kThreads / rs) {
+          int4 sum[P];
+#pragma unroll
+          for (int q = 0; q < P; ++q) {
+            sum[q] = parts[(q * quads + g) * rs];
+#pragma unroll
+            for (int z = 1; z < kMaxSplits; ++z)
+              if (z < p.splits) {
+                const int4 o = parts[((z * P + q) * quads + g) * rs];
+                sum[q].x += o.x, sum[q].y += o.y, sum[q].z += o.z, sum[q].w += o.w;
+              }
+          }
+          const float4 s4 = *reinterpret_cast<const float4 *>(&token_scale[0][4 * g]);
+          const float sx[4] = {s4.x, s4.y, s4.z, s4.w};
+          const int a[4] = {sum[0].x, sum[0].y, sum[0].z, sum[0].w};
+          const int c[4] = {sum[P - 1].x, sum[P - 1].y, sum[P - 1].z, sum[P - 1].w};
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i] = static_cast<float>(a[i]) * sx[i] * sw + bias;
+            if (P == 2) v[i] = silu_mul(v[i], static_cast<float>(c[i]) * sx[i] * su);
+            if (p.add && 4 * g + i < toks) v[i] += static_cast<float>(y[(4 * g + i) * p.ldy]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (4 * g + i < toks) y[(4 * g + i) * p.ldy] = from_float<T>(v[i]);
+        }
+      });
     }
   }
   tc_fence_before();
@@ -219,17 +355,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int P>
 int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params p, cudaStream_t stream,
-           const DeviceInfo &dev, const char *what) {
-  constexpr int kMaxBn = 256 / P;  // two buffers of P accumulators in the 512 columns of TMEM
+           const DeviceInfo &dev, const char *what, int force = 0) {
+  constexpr int kMaxBn = 256 / P, SUB = sub_blocks(P);  // two buffers of P accumulators in the 512 columns of TMEM
   p.tiles_m = (p.m + kMaxBn - 1) / kMaxBn;
   p.bn = ((p.m + p.tiles_m - 1) / p.tiles_m + 15) / 16 * 16;
   p.tiles = p.tiles_m * ((p.n + kRows - 1) / kRows);
   p.buf_cols = P * std::max(32, p.bn);  // the epilogue reads 32 columns at a time
   p.tmem_cols = 64;
   while (p.tmem_cols < 2 * p.buf_cols) p.tmem_cols *= 2;
-  const int slot = P * kWBytes + p.bn * kBK;
-  p.stages = static_cast<int>(std::min<size_t>(kMaxStages, (dev.smem_optin - 4096) / slot));
+  const int slot = SUB * (P * kWBytes + p.bn * kBK);
+  p.stages = static_cast<int>(std::min<size_t>(kMaxStages, (dev.smem_optin - 1024 - 5120) / slot));
   const size_t smem = static_cast<size_t>(p.stages) * slot + 1024;
+  const int nst = (p.k + SUB * kBK - 1) / (SUB * kBK);
+  p.splits = 1;
+  while (p.splits < kMaxSplits && 2 * p.splits * p.tiles <= dev.sms && 2 * p.splits <= nst) p.splits *= 2;
+  if (force) p.splits = force;
   CUtensorMap wmap, xmap;
   if (int rc = encode_tmap_2d_now(&wmap, wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, static_cast<uint64_t>(P) * p.n, ldw,
                                   kBK, kRows, CU_TENSOR_MAP_SWIZZLE_128B, what))
@@ -240,7 +380,8 @@ int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params 
   auto kern = w8a8_kernel<P>;
   static size_t configured[64] = {};
   if (int rc = ensure_smem(kern, smem, configured, what)) return rc;
-  return launch_overlapped(kern, dim3(std::min(p.tiles, dev.sms)), dim3(kThreads), smem, stream, what, wmap, xmap, p);
+  const int grid = p.splits > 1 ? p.tiles * p.splits : std::min(p.tiles, dev.sms);
+  return launch_overlapped_clusters(kern, dim3(grid), dim3(kThreads), p.splits, smem, stream, what, wmap, xmap, p);
 }
 
 int check(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw, const float *ws, const void *y,

@@ -34,20 +34,6 @@ struct TileParams {
   int tiles_m, tiles_n, tiles;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// The address of the same shared variable in the CTA of the given rank of this cluster.
-__device__ __forceinline__ uint32_t map_shared(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -192,10 +178,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint8_t *mine = out_stage + (warp - 2) * 2 * kStageOutBytes;
     const uint32_t tempty_leader[2] = {map_shared(smem_u32(&tempty[0]), 0), map_shared(smem_u32(&tempty[1]), 0)};
     const bool f32 = p.y_dtype == MQ_F32;
-    const int width = 128 / P;  // output columns of this half of the warps
+    constexpr int width = 128 / P, kChunks = width / 32;  // output columns of this half of the warps
     int it = 0, buf = 0;
     for (int t = blockIdx.x / 2; t < p.tiles; t += step, ++it) {
       const int b = it & 1;
+      const TileAt at = tile_at<P>(p, t);
+      const int row0 = at.m0 + 128 * rank + 32 * quarter, row = row0 + lane;
+      // Scales and biases come while the tile is still being multiplied: fetched at their use they cost the
+      // epilogue an L2 latency per 32 columns (2.4 instead of 1 us a tile). Lane l holds column c + l's.
+      const float sx = row < p.m ? p.xs[row] : 0.f;
+      float sw[kChunks], more[kChunks];  // more: the up scales, or the bias
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int col = at.n0 + half * width + 32 * i + lane;
+        sw[i] = col < p.n ? p.ws[col] : 0.f;
+        more[i] = col >= p.n ? 0.f : P == 2 ? p.ws[p.n + col] : p.bias ? p.bias[col] : 0.f;
+      }
       const bool ok = !abort_flag && mbar_wait(&tfull[b], (it >> 1) & 1);
       if (!__all_sync(0xffffffffu, ok && !abort_flag)) {
         if (lane == 0 && !abort_flag) {
@@ -205,30 +203,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         break;
       }
       tc_fence_after();
-      const TileAt at = tile_at<P>(p, t);
-      const int row0 = at.m0 + 128 * rank + 32 * quarter, row = row0 + lane;
-      const float sx = row < p.m ? p.xs[row] : 0.f;
       const uint32_t acc = tmem + b * 256 + lanes + half * width;
-#pragma unroll 1
-      for (int c = 0; c < width; c += 32) {
-        const int col0 = at.n0 + half * width + c, col = col0 + lane;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = 32 * i, col0 = at.n0 + half * width + c;
         float v[32];
-        const float sw = col < p.n ? p.ws[col] : 0.f;
         tmem_ld32(acc + c, v);
         if (P == 2) {
-          const float su = col < p.n ? p.ws[p.n + col] : 0.f;
           float u[32];
           tmem_ld32(acc + 128 + c, u);
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            v[j] = silu_mul(static_cast<float>(__float_as_int(v[j])) * sx * __shfl_sync(0xffffffffu, sw, j),
-                            static_cast<float>(__float_as_int(u[j])) * sx * __shfl_sync(0xffffffffu, su, j));
+            v[j] = silu_mul(static_cast<float>(__float_as_int(v[j])) * sx * __shfl_sync(0xffffffffu, sw[i], j),
+                            static_cast<float>(__float_as_int(u[j])) * sx * __shfl_sync(0xffffffffu, more[i], j));
         } else {
-          const float bias = p.bias && col < p.n ? p.bias[col] : 0.f;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            v[j] = static_cast<float>(__float_as_int(v[j])) * sx * __shfl_sync(0xffffffffu, sw, j) +
-                   __shfl_sync(0xffffffffu, bias, j);
+            v[j] = static_cast<float>(__float_as_int(v[j])) * sx * __shfl_sync(0xffffffffu, sw[i], j);
+          if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xffffffffu, more[i], j);
+          }
         }
         if (c + 32 >= width) {  // the last read of this accumulator
           tc_fence_before();
@@ -239,7 +234,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (row < p.m) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.n) store_out(p.y, p.y_dtype, row * p.ldy + col0 + j, v[j], p.add);
+              if (col0 + j < p.n)
+                by_type(p.y_dtype, [&](auto type) { put<decltype(type)>(p.y, row * p.ldy + col0 + j, v[j], p.add); });
           }
           continue;
         }
@@ -259,13 +255,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int u = 0; u < 4; ++u) {
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float lo = v[8 * u + 2 * i], hi = v[8 * u + 2 * i + 1];
+            for (int h = 0; h < 4; ++h) {
+              const float lo = v[8 * u + 2 * h], hi = v[8 * u + 2 * h + 1];
               if (p.y_dtype == MQ_F16) {
-                w[i] = pack_half2(lo, hi);
+                w[h] = pack_half2(lo, hi);
               } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(lo, hi);
+                w[h] = *reinterpret_cast<const uint32_t *>(&b2);
               }
             }
             *reinterpret_cast<uint4 *>(dst + ((4 * part + u) ^ (lane & 7)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
