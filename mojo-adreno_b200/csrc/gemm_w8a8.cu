@@ -26,10 +26,16 @@ constexpr int kMaxStages = 12;
 constexpr int kEpiWarps = 4;    // one per TMEM lane quarter; eight measured slower (4.4 -> 5.8 us for 1x2048x2048)
 constexpr int kThreads = 64 + 32 * kEpiWarps;  // warp 0 TMA, warp 1 MMA + TMEM, then the epilogue
 constexpr int kWBytes = kRows * kBK;
-constexpr int kMaxSplits = 4;   // clusters of 8 with this much shared memory did not all fit at once (4.9 -> 8.3 us)
+constexpr int kMaxSplits = 8;
+// Clusters of 1 .. 8 CTAs, one CTA per SM, that run at once on a B200 (cudaOccupancyMaxActiveClusters; the
+// SMs of a cluster share a GPC): a split whose clusters do not all fit takes twice as long (16 clusters
+// of 8: 4.9 -> 8.3 us for 1x2048x2048).
+__host__ __device__ constexpr int clusters_at_once(int size) {
+  return size == 1 ? 148 : size == 2 ? 74 : size == 3 ? 45 : size == 4 ? 33 : size == 5 ? 26 : size == 6 ? 22 : 15;
+}
 constexpr int64_t kMaxK = 131071;  // 128 * 128 * k stays below 2^31
-// 128-k blocks per stage: eight MMAs for each wait and commit of the issuing thread, which cost it about
-// 0.17 us together (four 128 x 16 MMAs take 0.1 us).
+// 128-k blocks per stage: eight MMAs for each wait and commit of the issuing thread, which cost it about 0.17 us
+// together (four 128 x 16 MMAs take 0.1 us): 16x2048x8192 on 16 CTAs 21.8 -> 16.2 us.
 __host__ __device__ constexpr int sub_blocks(int planes) { return planes == 1 ? 2 : 1; }
 
 struct Params {
@@ -144,6 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   bool live = false;  // an epilogue warp of a split tile whose sums are in TMEM
+  float sw = 0.f, su = 0.f, bias = 0.f;  // of an epilogue thread's weight row
   griddep_wait();
 
   if (warp == 0) {
@@ -228,8 +235,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // The scales are fetched while the tile is still being multiplied.
       const int m0 = t % p.tiles_m * p.bn, toks = min(p.bn, p.m - m0), r = t / p.tiles_m * kRows + row;
       const bool in = r < p.n;
-      const float sw = in ? p.ws[r] : 0.f, su = in && P == 2 ? p.ws[p.n + r] : 0.f;
-      const float bias = in && P == 1 && p.bias ? p.bias[r] : 0.f;
+      sw = in ? p.ws[r] : 0.f, su = in && P == 2 ? p.ws[p.n + r] : 0.f;
+      bias = in && P == 1 && p.bias ? p.bias[r] : 0.f;
       __syncwarp();
       for (int i = lane; i < toks; i += 32) sx[i] = p.xs[m0 + i];
       __syncwarp();
@@ -283,64 +290,67 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (p.splits > 1) {
-    // Join the splits' int32 sums through distributed shared memory: CTA s finishes rows s * rs .. of the
-    // tile. The parts land in its ring, [split][plane][4 tokens][row] of int4, once every CTA's MMAs are
-    // done with theirs.
+    // Join the splits' int32 sums through distributed shared memory: groups of 4 tokens are dealt to the
+    // cluster's CTAs in turn. The parts land in their owner's ring, [split][plane][group][row] of int4,
+    // once every CTA's MMAs are done with theirs.
     cluster_sync_all();
-    const int rs = kRows / p.splits;  // 64 or 32
-    const int m0 = first % p.tiles_m * p.bn, toks = min(p.bn, p.m - m0), quads = p.bn / 4;
+    const int m0 = first % p.tiles_m * p.bn, toks = min(p.bn, p.m - m0);
+    const int owned = (p.bn / 4 + p.splits - 1) / p.splits;  // groups of one CTA
+    const int row = (warp & 3) * 32 + lane;
     if (live) {
-      const int row = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t dst = map_shared(smem_u32(ring), row / rs) + (split * P * quads * rs + row % rs) * 16;
+      const uint32_t part = smem_u32(ring) + (split * P * owned * kRows + row) * 16;
 #pragma unroll
-      for (int q = 0; q < P; ++q)
+      for (int q = 0; q < P; ++q) {
+        int owner = 0, at = 0;
         for (int c0 = 0; c0 < toks; c0 += 32) {
           float v[32];
           tmem_ld32(tmem + q * (p.buf_cols / P) + lanes + c0, v);
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
-            if (c0 + j < toks)
-              st_remote_v4(dst + (q * quads + (c0 + j) / 4) * rs * 16,
+            if (c0 + j < toks) {
+              st_remote_v4(map_shared(part + (q * owned + at) * kRows * 16, owner),
                            make_int4(__float_as_int(v[j]), __float_as_int(v[j + 1]), __float_as_int(v[j + 2]),
                                      __float_as_int(v[j + 3])));
+              if (++owner == p.splits) owner = 0, ++at;
+            }
         }
+      }
     }
     cluster_sync_all();
-    // kThreads is a multiple of rs: a thread keeps its row and takes every kThreads / rs-th group of 4 tokens.
-    const int row = threadIdx.x % rs, r = first / p.tiles_m * kRows + split * rs + row;
-    if (r < p.n && !abort_flag) {
+    const int r = first / p.tiles_m * kRows + row;
+    if (live && r < p.n && !abort_flag) {
       const int4 *parts = reinterpret_cast<const int4 *>(ring) + row;
-      const float sw = p.ws[r], su = P == 2 ? p.ws[p.n + r] : 0.f, bias = P == 1 && p.bias ? p.bias[r] : 0.f;
       by_type(p.y_dtype, [&](auto type) {
         using T = decltype(type);
-        T *y = static_cast<T *>(p.y) + m0 * p.ldy + r;
-        for (int g = threadIdx.x / rs; 4 * g < toks; g += kThreads / rs) {
+        for (int at = 0; 4 * (at * p.splits + split) < toks; ++at) {
+          const int tok = 4 * (at * p.splits + split);
           int4 sum[P];
 #pragma unroll
           for (int q = 0; q < P; ++q) {
-            sum[q] = parts[(q * quads + g) * rs];
+            sum[q] = parts[(q * owned + at) * kRows];
 #pragma unroll
             for (int z = 1; z < kMaxSplits; ++z)
               if (z < p.splits) {
-                const int4 o = parts[((z * P + q) * quads + g) * rs];
+                const int4 o = parts[((z * P + q) * owned + at) * kRows];
                 sum[q].x += o.x, sum[q].y += o.y, sum[q].z += o.z, sum[q].w += o.w;
               }
           }
-          const float4 s4 = *reinterpret_cast<const float4 *>(&token_scale[0][4 * g]);
+          const float4 s4 = *reinterpret_cast<const float4 *>(&token_scale[warp - 2][tok]);
           const float sx[4] = {s4.x, s4.y, s4.z, s4.w};
           const int a[4] = {sum[0].x, sum[0].y, sum[0].z, sum[0].w};
           const int c[4] = {sum[P - 1].x, sum[P - 1].y, sum[P - 1].z, sum[P - 1].w};
+          T *const y = static_cast<T *>(p.y) + (m0 + tok) * p.ldy + r;
           float v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             v[i] = static_cast<float>(a[i]) * sx[i] * sw + bias;
             if (P == 2) v[i] = silu_mul(v[i], static_cast<float>(c[i]) * sx[i] * su);
-            if (p.add && 4 * g + i < toks) v[i] += static_cast<float>(y[(4 * g + i) * p.ldy]);
+            if (p.add && tok + i < toks) v[i] += static_cast<float>(y[i * p.ldy]);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (4 * g + i < toks) y[(4 * g + i) * p.ldy] = from_float<T>(v[i]);
+            if (tok + i < toks) y[i * p.ldy] = from_float<T>(v[i]);
         }
       });
     }
@@ -353,23 +363,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// The token tiles (of bn, at most 256 / P: two buffers of P accumulators in the 512 columns of TMEM) and
+// the tiles of the streaming kernel.
+struct Shape {
+  int tiles_m, bn, tiles;
+};
+inline Shape shape_of(int planes, int m, int n) {
+  Shape s;
+  s.tiles_m = (m + 256 / planes - 1) / (256 / planes);
+  s.bn = ((m + s.tiles_m - 1) / s.tiles_m + 15) / 16 * 16;
+  s.tiles = s.tiles_m * ((n + kRows - 1) / kRows);
+  return s;
+}
+
 template <int P>
 int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params p, cudaStream_t stream,
-           const DeviceInfo &dev, const char *what, int force = 0) {
-  constexpr int kMaxBn = 256 / P, SUB = sub_blocks(P);  // two buffers of P accumulators in the 512 columns of TMEM
-  p.tiles_m = (p.m + kMaxBn - 1) / kMaxBn;
-  p.bn = ((p.m + p.tiles_m - 1) / p.tiles_m + 15) / 16 * 16;
-  p.tiles = p.tiles_m * ((p.n + kRows - 1) / kRows);
+           const DeviceInfo &dev, const char *what, int splits) {
+  constexpr int SUB = sub_blocks(P);
+  const Shape sh = shape_of(P, p.m, p.n);
+  p.tiles_m = sh.tiles_m, p.bn = sh.bn, p.tiles = sh.tiles, p.splits = splits;
   p.buf_cols = P * std::max(32, p.bn);  // the epilogue reads 32 columns at a time
   p.tmem_cols = 64;
   while (p.tmem_cols < 2 * p.buf_cols) p.tmem_cols *= 2;
-  const int slot = SUB * (P * kWBytes + p.bn * kBK);
-  p.stages = static_cast<int>(std::min<size_t>(kMaxStages, (dev.smem_optin - 1024 - 5120) / slot));
-  const size_t smem = static_cast<size_t>(p.stages) * slot + 1024;
-  const int nst = (p.k + SUB * kBK - 1) / (SUB * kBK);
-  p.splits = 1;
-  while (p.splits < kMaxSplits && 2 * p.splits * p.tiles <= dev.sms && 2 * p.splits <= nst) p.splits *= 2;
-  if (force) p.splits = force;
+  // As many slots as shared memory holds, and no more than a CTA fills: the next kernel's CTAs can then
+  // come in beside these.
+  const int slot = SUB * (P * kWBytes + p.bn * kBK), nst = (p.k + SUB * kBK - 1) / (SUB * kBK);
+  const int grid = splits > 1 ? p.tiles * splits : std::min(p.tiles, dev.sms);
+  const int64_t fills = splits > 1 ? (nst + splits - 1) / splits : static_cast<int64_t>(nst) * ((p.tiles + grid - 1) / grid);
+  p.stages = static_cast<int>(std::min<int64_t>({kMaxStages, fills, static_cast<int64_t>(dev.smem_optin - 1024 - 5120) / slot}));
+  const size_t parts = splits > 1 ? static_cast<size_t>(splits) * P * ((p.bn / 4 + splits - 1) / splits) * kRows * 16 : 0;
+  const size_t smem = std::max(static_cast<size_t>(p.stages) * slot, parts) + 1024;
   CUtensorMap wmap, xmap;
   if (int rc = encode_tmap_2d_now(&wmap, wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, static_cast<uint64_t>(P) * p.n, ldw,
                                   kBK, kRows, CU_TENSOR_MAP_SWIZZLE_128B, what))
@@ -380,7 +403,6 @@ int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params 
   auto kern = w8a8_kernel<P>;
   static size_t configured[64] = {};
   if (int rc = ensure_smem(kern, smem, configured, what)) return rc;
-  const int grid = p.splits > 1 ? p.tiles * p.splits : std::min(p.tiles, dev.sms);
   return launch_overlapped_clusters(kern, dim3(grid), dim3(kThreads), p.splits, smem, stream, what, wmap, xmap, p);
 }
 
@@ -409,13 +431,45 @@ int check(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int6
 namespace mq {
 namespace w8 {
 
+// Which kernel, and how many CTAs (pairs of CTAs) share a tile's k: the least of the times below, in us,
+// fitted to measurements on a B200 with weights from HBM. Streaming kernel: 0.2 us per 128 k and wave of tiles up
+// to about 150 tokens per tile (the issue of the MMAs), 0.33 at 256 (its operands' way into shared memory),
+// for gate|up 0.3 and 0.45 at 128; 2.2 us and 0.015 per token and plane outside the loop, 3 and 0.028 with the
+// parts of a split to join. Pairs: 0.285 us per 128 k and wave of 256 x 256 tiles, 5.2 us outside, 9.8 with
+// parts. Measured, streaming against pairs: 128x4096x4096 8.8 / 13.8, 431x2048x8192 14.2 / 17.0,
+// 512x4096x4096 16.9 / 15.2, 1024x4096x4096 18.0 / 16.5, gate|up 64x8192x2048 11.9 / 13.0, 400x8192x2048 20.5 / 17.7.
+struct Plan {
+  bool pairs;
+  int splits;
+};
+inline Plan plan_of(int planes, int m, int n, int k) {
+  Plan best{false, 1};
+  float least = 1e30f;
+  auto consider = [&](bool pairs, int splits, float us) {
+    if (us < least) least = us, best = Plan{pairs, splits};
+  };
+  const Shape sh = shape_of(planes, m, n);
+  const float block = planes == 1 ? std::max(0.2f, 0.33f / 256 * sh.bn) : std::max(0.3f, 0.45f / 128 * sh.bn);
+  const int blocks = (k + kBK - 1) / kBK, stages = (blocks + sub_blocks(planes) - 1) / sub_blocks(planes);
+  consider(false, 1, 2.2f + 0.015f * planes * sh.bn + ((sh.tiles + 147) / 148) * blocks * block);
+  for (int z = 2; z <= std::min(kMaxSplits, stages); ++z)
+    if (sh.tiles <= clusters_at_once(z))
+      consider(false, z, 3.f + 0.028f * planes * sh.bn + (stages + z - 1) / z * sub_blocks(planes) * block);
+  const int tiles = ((m + kTileM - 1) / kTileM) * ((n + kTileB / planes - 1) / (kTileB / planes));
+  consider(true, 1, 5.2f + ((tiles + 73) / 74) * blocks * 0.285f);
+  for (int z = 2; z <= std::min(kTileMaxSplits, blocks); ++z)
+    if (tiles <= clusters_at_once(2 * z)) consider(true, z, 9.8f + (blocks + z - 1) / z * 0.285f);
+  return best;
+}
+
 template <int P>
 int run(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, const Params &p, cudaStream_t stream,
         const char *what) {
   DeviceInfo dev;
   if (int rc = device_info(&dev)) return rc;
-  if (p.m > 256) return launch_tile<P>(xq, ldx, wq, ldw, p, stream, dev, what);
-  return launch<P>(xq, ldx, wq, ldw, p, stream, dev, what);
+  const Plan plan = plan_of(P, p.m, p.n, p.k);
+  if (plan.pairs) return launch_tile<P>(xq, ldx, wq, ldw, p, stream, dev, what, plan.splits);
+  return launch<P>(xq, ldx, wq, ldw, p, stream, dev, what, plan.splits);
 }
 
 }  // namespace w8

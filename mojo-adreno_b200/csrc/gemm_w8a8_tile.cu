@@ -11,8 +11,8 @@
 //    through stay in L2), accumulators double-buffered (2 x 256 columns of TMEM): eight warps of each
 //    CTA scale, convert and store one tile while the next one is multiplied.
 //  * The epilogue stages 32 rows x 128 bytes per warp in the swizzled layout and writes it with one TMA
-//    store, which clips the last rows and columns; y whose rows are not 16-byte aligned, and add, take
-//    plain stores.
+//    store, which clips the last rows and columns. y whose rows are not 16-byte aligned, and add, are
+//    written from the staged rows by plain stores, consecutive lanes on consecutive outputs.
 #include "common.cuh"
 
 namespace mq {
@@ -23,7 +23,7 @@ constexpr int kTileStages = 5, kTileStageBytes = 2 * 128 * kBK;
 constexpr int kTileEpiWarps = 8, kTileThreads = 64 + 32 * kTileEpiWarps;
 constexpr int kStageOutBytes = 4096;        // 32 rows x 128 bytes
 constexpr int kTileSmem = kTileStages * kTileStageBytes + kTileEpiWarps * 2 * kStageOutBytes + 1024;
-constexpr int kBand = 8;
+constexpr int kBand = 8, kTileMaxSplits = 4;
 
 struct TileParams {
   const float *xs, *ws, *bias;
@@ -32,6 +32,7 @@ struct TileParams {
   int y_dtype, add, y_tma;
   int m, n, k;  // n: output columns
   int tiles_m, tiles_n, tiles;
+  int splits;  // pairs of a cluster that share a tile's k (1: persistent pairs, each tile's k whole)
 };
 
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
@@ -82,8 +83,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ volatile int abort_flag;
   constexpr int S = kTileStages;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t rank = cluster_rank();
-  const int nkb = (p.k + kBK - 1) / kBK, step = gridDim.x / 2;
+  const uint32_t crank = cluster_rank(), rank = crank & 1, leader = crank & ~1u;  // rank: within the pair
+  const int split = crank / 2, nkb_all = (p.k + kBK - 1) / kBK;
+  const int kb0 = nkb_all * split / p.splits, nkb = nkb_all * (split + 1) / p.splits - kb0;
+  const int first = blockIdx.x / (2 * p.splits), step = gridDim.x / (2 * p.splits);
 
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
@@ -107,6 +110,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   cluster_sync_all();  // the pair's barriers exist before anything completes on them
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  bool live = false;  // an epilogue warp of a split tile whose sums are in TMEM
   griddep_wait();
 
   if (warp == 0) {
@@ -117,7 +121,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     int s = 0, round = 0;
     int64_t issued = 0;
     bool ok = true;
-    for (int t = blockIdx.x / 2; ok && t < p.tiles; t += step) {
+    for (int t = first; ok && t < p.tiles; t += step) {
       const TileAt at = tile_at<P>(p, t);
       const int m0 = at.m0 + 128 * rank, n0 = at.n0 + (P == 1 ? 128 : p.n) * rank;
       for (int kb = 0; kb < nkb; ++kb) {
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncwarp();
         if (lane < 2)  // lane 0: the tokens, lane 1: the weights
           tma_load_2d_pair(ring + s * kTileStageBytes + lane * 128 * kBK, lane ? &wmap : &xmap,
-                           map_shared(smem_u32(&full[s]), 0), kb * kBK, lane ? n0 : m0);
+                           map_shared(smem_u32(&full[s]), leader), (kb0 + kb) * kBK, lane ? n0 : m0);
         ++issued;
         if (++s == S) s = 0, ++round;
       }
@@ -144,9 +148,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = umma_idesc_i8(256, 256);
+      const uint16_t both = static_cast<uint16_t>(3u << leader);
       int s = 0, it = 0;
       uint32_t ph = 0;
-      for (int t = blockIdx.x / 2; t < p.tiles; t += step, ++it) {
+      for (int t = first; t < p.tiles; t += step, ++it) {
         const int b = it & 1;
         bool ok = mbar_wait(&tempty[b], ((it >> 1) & 1) ^ 1);
         tc_fence_after();
@@ -160,10 +165,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const uint64_t da = umma_desc_sw128(base), db = umma_desc_sw128(base + 128 * kBK);
 #pragma unroll
           for (int j = 0; j < kBK / 32; ++j) umma_i8_pair(tmem + b * 256, da + 2 * j, db + 2 * j, idesc, kb != 0 || j != 0);
-          umma_commit_pair(&empty[s], 3);
+          umma_commit_pair(&empty[s], both);
           if (++s == S) s = 0, ph ^= 1;
         }
-        umma_commit_pair(&tfull[b], 3);
+        umma_commit_pair(&tfull[b], both);
         if (!ok) {
           raise_status(kStatusW8MmaWait);
           abort_flag = 1;
@@ -176,11 +181,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     uint8_t *mine = out_stage + (warp - 2) * 2 * kStageOutBytes;
-    const uint32_t tempty_leader[2] = {map_shared(smem_u32(&tempty[0]), 0), map_shared(smem_u32(&tempty[1]), 0)};
-    const bool f32 = p.y_dtype == MQ_F32;
+    const uint32_t tempty_leader[2] = {map_shared(smem_u32(&tempty[0]), leader), map_shared(smem_u32(&tempty[1]), leader)};
+    const bool f32 = p.y_dtype == MQ_F32 || p.add;  // staged as fp32: y is added before the one rounding
     constexpr int width = 128 / P, kChunks = width / 32;  // output columns of this half of the warps
     int it = 0, buf = 0;
-    for (int t = blockIdx.x / 2; t < p.tiles; t += step, ++it) {
+    for (int t = first; t < p.tiles; t += step, ++it) {
       const int b = it & 1;
       const TileAt at = tile_at<P>(p, t);
       const int row0 = at.m0 + 128 * rank + 32 * quarter, row = row0 + lane;
@@ -203,6 +208,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         break;
       }
       tc_fence_after();
+      if (p.splits > 1) {  // the one tile of this cluster: joined below
+        live = true;
+        break;
+      }
       const uint32_t acc = tmem + b * 256 + lanes + half * width;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
@@ -229,15 +238,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_remote(tempty_leader[b]);
-        }
-        if (!p.y_tma) {
-          if (row < p.m) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.n)
-                by_type(p.y_dtype, [&](auto type) { put<decltype(type)>(p.y, row * p.ldy + col0 + j, v[j], p.add); });
-          }
-          continue;
         }
         // fp32: a staged row of 128 bytes is these 32 columns; 16-bit types: two such steps fill it.
         const int part = f32 ? 0 : c / 32 & 1;
@@ -268,18 +268,118 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         if (f32 || part == 1) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            const int x = f32 ? col0 : col0 - 32;
-            if (x < p.n && row0 < p.m) tma_store_2d(&ymap, mine + buf * kStageOutBytes, x, row0, false);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          const int x = f32 ? col0 : col0 - 32;
+          if (p.y_tma) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (x < p.n && row0 < p.m) tma_store_2d(&ymap, mine + buf * kStageOutBytes, x, row0, false);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {  // a row at a time, consecutive lanes on consecutive outputs
+            __syncwarp();
+            by_type(p.y_dtype, [&](auto type) {
+              using T = decltype(type);
+              const uint8_t *const staged = mine + buf * kStageOutBytes;
+              const int cols = p.n - x;
+              T *y = static_cast<T *>(p.y) + row0 * p.ldy + x;
+#pragma unroll 4
+              for (int r = 0; r < min(32, p.m - row0); ++r, y += p.ldy) {
+                if (f32) {
+                  float o = *reinterpret_cast<const float *>(staged + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4);
+                  if (lane < cols) y[lane] = from_float<T>(p.add ? o + static_cast<float>(y[lane]) : o);
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 64; e += 32) {
+                    const int at = e + lane;
+                    const T o = *reinterpret_cast<const T *>(staged + r * 128 + ((at / 8) ^ (r & 7)) * 16 + at % 8 * 2);
+                    if (at < cols) y[at] = o;
+                  }
+                }
+              }
+            });
           }
           buf ^= 1;
         }
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory stays until it is read
+  }
+  if (p.splits > 1) {
+    // Join the splits' int32 sums through distributed shared memory: groups of 32 columns are dealt to the
+    // cluster's pairs in turn; a pair's even CTA joins its own rows, the odd one its. The parts land in the
+    // ring and the staging area, [split][plane][group][4 columns][row] of int4, once the MMAs are done.
+    cluster_sync_all();
+    constexpr int kGroups = 256 / P / 32;
+    const int owned = (kGroups + p.splits - 1) / p.splits, quarter = warp & 3, half = (warp - 2) >> 2;
+    if (live) {
+      const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t row_at = smem_u32(ring) + (quarter * 32 + lane) * 16;
+      for (int g = half; g < kGroups; g += 2) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          float v[32];
+          tmem_ld32(acc + q * 128 + 32 * g, v);
+          const uint32_t dst = map_shared(row_at + ((split * P + q) * owned + g / p.splits) * 8 * 128 * 16,
+                                          2 * (g % p.splits) + rank);
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            st_remote_v4(dst + u * 128 * 16, make_int4(__float_as_int(v[4 * u]), __float_as_int(v[4 * u + 1]),
+                                                       __float_as_int(v[4 * u + 2]), __float_as_int(v[4 * u + 3])));
+        }
+      }
+    }
+    cluster_sync_all();
+    const TileAt at = tile_at<P>(p, first);
+    const int row = at.m0 + 128 * rank + quarter * 32 + lane;
+    if (live && !abort_flag) {
+      const float sx = row < p.m ? p.xs[row] : 0.f;
+      for (int o = 0; split + o * p.splits < kGroups; ++o) {  // 16 columns of each group for this warp
+        const int col0 = at.n0 + (split + o * p.splits) * 32 + half * 16, col = col0 + lane % 16;
+        const float sw = col < p.n ? p.ws[col] : 0.f;
+        const float more = col >= p.n ? 0.f : P == 2 ? p.ws[p.n + col] : p.bias ? p.bias[col] : 0.f;
+        int a[P][16] = {};
+#pragma unroll
+        for (int z = 0; z < kTileMaxSplits; ++z)
+          if (z < p.splits)
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int4 v = *reinterpret_cast<const int4 *>(
+                    ring + ((((z * P + q) * owned + o) * 8 + half * 4 + u) * 128 + quarter * 32 + lane) * 16);
+                a[q][4 * u] += v.x, a[q][4 * u + 1] += v.y, a[q][4 * u + 2] += v.z, a[q][4 * u + 3] += v.w;
+              }
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float wj = __shfl_sync(0xffffffffu, sw, j), mj = __shfl_sync(0xffffffffu, more, j);
+          v[j] = static_cast<float>(a[0][j]) * sx * wj;
+          v[j] = P == 2 ? silu_mul(v[j], static_cast<float>(a[P - 1][j]) * sx * mj) : v[j] + mj;
+        }
+        if (row < p.m)
+          by_type(p.y_dtype, [&](auto type) {
+            using T = decltype(type);
+            T *const y = static_cast<T *>(p.y) + row * p.ldy + col0;
+            if (p.y_tma && col0 + 16 <= p.n) {  // 16-byte aligned rows
+              struct alignas(16) Vec {
+                T t[16 / sizeof(T)];
+              };
+#pragma unroll
+              for (int j = 0; j < 16; j += 16 / sizeof(T)) {
+                Vec o16;
+#pragma unroll
+                for (int i = 0; i < 16 / sizeof(T); ++i) o16.t[i] = from_float<T>(v[j + i]);
+                *reinterpret_cast<Vec *>(y + j) = o16;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (col0 + j < p.n) y[j] = from_float<T>(p.add ? v[j] + static_cast<float>(y[j]) : v[j]);
+            }
+          });
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -292,13 +392,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
 template <int P>
 int launch_tile(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, const Params &q, cudaStream_t stream,
-                const DeviceInfo &dev, const char *what) {
+                const DeviceInfo &dev, const char *what, int splits) {
   TileParams p{};
   p.xs = q.xs, p.ws = q.ws, p.bias = q.bias, p.y = q.y, p.ldy = q.ldy, p.y_dtype = q.y_dtype, p.add = q.add;
   p.m = q.m, p.n = q.n, p.k = q.k;
   p.tiles_m = (p.m + kTileM - 1) / kTileM;
   p.tiles_n = (p.n + kTileB / P - 1) / (kTileB / P);
   p.tiles = p.tiles_m * p.tiles_n;
+  p.splits = splits;
   const int es = p.y_dtype == MQ_F32 ? 4 : 2;
   p.y_tma = !p.add && aligned(p.y, 16) && p.ldy * es % 16 == 0;
   CUtensorMap xmap, wmap, ymap;
@@ -318,8 +419,9 @@ int launch_tile(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, co
   auto kern = w8a8_tile_kernel<P>;
   static size_t configured[64] = {};
   if (int rc = ensure_smem(kern, kTileSmem, configured, what)) return rc;
-  return launch_overlapped_clusters(kern, dim3(2 * std::min(p.tiles, dev.sms / 2)), dim3(kTileThreads), 2, kTileSmem, stream,
-                                    what, xmap, wmap, ymap, p);
+  const int grid = 2 * (p.splits > 1 ? p.tiles * p.splits : std::min(p.tiles, dev.sms / 2));
+  return launch_overlapped_clusters(kern, dim3(grid), dim3(kTileThreads), 2 * p.splits, kTileSmem, stream, what, xmap, wmap,
+                                    ymap, p);
 }
 
 }  // namespace w8
