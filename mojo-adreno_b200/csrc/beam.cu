@@ -23,24 +23,36 @@ namespace beam {
 constexpr int kThreads = 256;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 256;  // (beam, split) lists of a request: one per thread of the merge
-constexpr int kElems = 16;      // logits per thread and chunk
-constexpr int kChunk = kThreads * kElems;
-constexpr int kTargetCtas = 148 * 8;
-constexpr float kNegInf = -INFINITY;
+constexpr int kVecs = 4;        // 16-byte vectors per thread and chunk
+constexpr int kChunkBytes = kThreads * kVecs * 16;
+constexpr int kFresh = 1280;    // pairs that may wait to be merged into the list: at least (kMaxBeams + 1) * 32
+constexpr int kStages = 2;      // chunks on their way into shared memory: 32 KB for each of four CTAs per SM
+constexpr float kNegInf = -INFINITY, kLowest = -3.402823466e38f, kLog2e = 1.44269504088896340736f;
 
+// (Counted in fp32 chunks for every type, so that the workspace's size does not depend on it.)
+// The least (CTAs of an SM) x (chunks of a CTA + 6 for its start and end); at most one list per thread of the
+// merge.
 __host__ __device__ constexpr int splits_for(int64_t rows, int beams, int64_t vocab) {
-  const int64_t chunks = (vocab + kChunk - 1) / kChunk;
-  int64_t s = kTargetCtas / rows;
-  if (s > kMaxLists / beams) s = kMaxLists / beams;
-  if (s > chunks) s = chunks;
-  return s < 1 ? 1 : static_cast<int>(s);
+  const int64_t chunks = (vocab * 4 + kChunkBytes - 1) / kChunkBytes;
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t s = 1; s <= kMaxLists / beams && s <= chunks; ++s) {
+    const int64_t cost = (rows * s + 147) / 148 * ((chunks + s - 1) / s + 6);
+    if (cost < least) least = cost, best = s;
+  }
+  return static_cast<int>(best);
 }
 
-// What one CTA leaves for the merge, followed by kp keys (best first, 0 = none).
-struct Part {
-  float top, sum;
-  int bad, count;
+// What the CTAs leave for the merge: a base and the sum of 2^(v log2 e - base) each (NaN where a logit is NaN
+// or +infinity), then kp keys each, best first, 0 = none.
+struct Parts {
+  float2 *sums;    // [rows * splits]
+  uint64_t *keys;  // [rows * splits][kp]
 };
+inline size_t parts_bytes(int64_t lists, int kp) { return static_cast<size_t>(lists) * (sizeof(float2) + 8 * kp); }
+inline Parts parts_at(void *workspace, int64_t lists) {
+  float2 *sums = static_cast<float2 *>(workspace);
+  return {sums, reinterpret_cast<uint64_t *>(sums + lists)};
+}
 
 // Order-preserving bits of a float; -0 counts as +0.
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -57,6 +69,12 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
 __device__ __forceinline__ float value_of_key(uint64_t key) { return value_of(static_cast<uint32_t>(key >> 32)); }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <typename T>
 __device__ __forceinline__ float to_float(T v);
 template <>
@@ -70,9 +88,9 @@ struct ScanParams {
   const void *logits;
   const float *scores;
   const uint8_t *finished;
-  uint8_t *parts;
+  Parts parts;
   int64_t ld;
-  int beams, vocab, splits, part_bytes;
+  int beams, vocab, splits;
 };
 
 __device__ __forceinline__ bool live_beam(const float *scores, const uint8_t *finished, int64_t row) {
@@ -80,92 +98,55 @@ __device__ __forceinline__ bool live_beam(const float *scores, const uint8_t *fi
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_scan_kernel(const ScanParams p) {
-  constexpr int V = 16 / sizeof(T), U = kElems / V;  // elements of a 16-byte vector, vectors per chunk
+__global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams p) {
+  constexpr int V = 16 / sizeof(T), U = kVecs, kElems = V * U;  // elements of a vector; vectors, elements per chunk
+  constexpr int kChunk = kThreads * kElems;
+  extern __shared__ __align__(16) uint8_t slots[];   // kStages chunks
+  __shared__ uint64_t full[kStages];
   __shared__ uint64_t list[2][kMaxBeams + 1];
-  __shared__ uint64_t fresh[(kMaxBeams + 1) * kElems];
+  __shared__ uint64_t fresh[kFresh];
   __shared__ uint64_t best_of[kThreads];
   __shared__ uint64_t raised;
   __shared__ int nfresh;
   __shared__ float red[2][kThreads / 32];
+  const int tid = threadIdx.x, kp = p.beams + 1;
   griddep_launch_dependents();
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+    nfresh = 0;
+  }
+  __syncthreads();
   griddep_wait();
   const int64_t row = blockIdx.x / p.splits;
-  const int split = blockIdx.x % p.splits, tid = threadIdx.x, kp = p.beams + 1;
+  const int split = blockIdx.x % p.splits;
   if (!live_beam(p.scores, p.finished, row)) return;
   const T *x = static_cast<const T *>(p.logits) + row * p.ld;
-  // 16-byte vectors from the aligned address at or below x: vector g holds columns g * V - lead ...
-  const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
-  const int nvec = (p.vocab + lead + V - 1) / V;
+  // The row's 16-byte aligned vectors come in chunks; the elements before the first and after the last
+  // (at most V - 1 each) are one more step of the first split's CTA.
+  const int head = min(p.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+  const int nvec = (p.vocab - head) / V, body_end = head + nvec * V, edges = head + p.vocab - body_end;
   const int chunks = (nvec + kThreads * U - 1) / (kThreads * U);
   const int c_begin = static_cast<int>(static_cast<int64_t>(chunks) * split / p.splits);
   const int c_end = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / p.splits);
-  if (tid == 0) nfresh = 0;
-  __syncthreads();
+  const int c_last = c_end + (split == 0 && edges > 0);
+  auto fetch = [&](int c) {  // by thread 0
+    const int slot = (c - c_begin) % kStages;
+    const uint32_t bytes = min(nvec - c * kThreads * U, kThreads * U) * 16;
+    mbar_expect_tx(&full[slot], bytes);
+    bulk_load(slots + slot * kChunkBytes, x + head + static_cast<int64_t>(c) * kChunk, bytes, &full[slot]);
+  };
+  if (tid == 0)
+    for (int c = c_begin; c < min(c_end, c_begin + kStages); ++c) fetch(c);
 
-  float m = -3.402823466e38f, s = 0.f;
-  int bad = 0, cur = 0, have = 0;
-  uint64_t bar = 0;  // a pair enters the list only above this key
-  for (int c = c_begin; c < c_end; ++c) {
-    float v[kElems];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int g = (c * U + u) * kThreads + tid, col = g * V - lead;
-      if (col >= 0 && col + V <= p.vocab) {
-        const uint4 q = ldg_stream_v4(x + col);
-        const T *e = reinterpret_cast<const T *>(&q);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[u * V + i] = to_float(e[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          v[u * V + i] = col + i >= 0 && col + i < p.vocab ? to_float(x[col + i]) : kNegInf;
-      }
-    }
-    float big = kNegInf;
-#pragma unroll
-    for (int i = 0; i < kElems; ++i) {
-      bad |= !(v[i] < INFINITY);  // NaN or +infinity
-      big = fmaxf(big, v[i]);
-    }
-    if (big > m) {
-      s *= expf(m - big);
-      m = big;
-    }
-#pragma unroll
-    for (int i = 0; i < kElems; ++i) s += expf(v[i] - m);
-    // The best pairs: threads whose largest key passes the bar offer theirs.
-    uint64_t mine = 0;
-    auto key_at = [&](int i) -> uint64_t {
-      const int col = ((c * U + i / V) * kThreads + tid) * V - lead + i % V;
-      return col >= 0 && col < p.vocab ? key_of(v[i], col) : 0;
-    };
-    if (bar == 0 || big >= value_of_key(bar)) {
-#pragma unroll
-      for (int i = 0; i < kElems; ++i) mine = max(mine, key_at(i));
-    }
-    const int offers = __syncthreads_count(mine > bar);
-    if (offers == 0) continue;
-    uint64_t limit = bar;
-    if (offers > kp) {
-      // kp threads' largest pairs are enough: no pair below the smallest of those kp can be kept. So at
-      // most kp * kElems pairs are written, whatever the order of the logits.
-      best_of[tid] = mine > bar ? mine : 0;
-      __syncthreads();
-      int rank = 0;
-      for (int j = 0; j < kThreads; ++j) rank += best_of[j] > mine;
-      if (mine > bar && rank == kp - 1) raised = mine - 1;
-      __syncthreads();
-      limit = raised;
-    }
-    if (mine > limit) {
-#pragma unroll
-      for (int i = 0; i < kElems; ++i) {
-        const uint64_t key = key_at(i);
-        if (key > limit) fresh[atomicAdd(&nfresh, 1)] = key;
-      }
-    }
-    __syncthreads();
+  float m = kLowest, base = kLowest, s = 0.f;  // the largest logit, log2(e) times it, sum of 2^(v log2 e - base)
+  int cur = 0, have = 0;
+  int bound = 0;     // at least as many pairs as wait in `fresh`; the same in every thread
+  uint64_t bar = 0;  // a pair is offered only above this key
+  float bar_value = kNegInf;
+  // Merges `fresh` into the list by counting, for each pair, the better ones. Called by the whole CTA, after
+  // a barrier behind the last append; the next append comes behind a barrier too.
+  auto merge = [&]() {
     const int n = have + nfresh, old = have;
     for (int i = tid; i < n; i += kThreads) {
       const uint64_t key = i < old ? list[cur][i] : fresh[i - old];
@@ -178,43 +159,152 @@ __global__ void __launch_bounds__(kThreads) beam_scan_kernel(const ScanParams p)
     if (tid == 0) nfresh = 0;
     cur ^= 1;
     have = min(n, kp);
-    bar = have == kp ? list[cur][kp - 1] : 0;
-    __syncthreads();
+    if (have == kp) bar = list[cur][kp - 1], bar_value = value_of_key(bar);
+  };
+  bool arrived = true;  // false once a wait ran out: the rest counts as -inf
+  for (int c = c_begin; c < c_last; ++c) {
+    const bool edge = c == c_end;
+    const int edge_col = tid < head ? tid : body_end + tid - head;
+    const int slot = (c - c_begin) % kStages;
+    float v[kElems];
+    if (!edge && arrived && !mbar_wait(&full[slot], (c - c_begin) / kStages & 1)) {
+      raise_status(kStatusBeamLoadWait);
+      arrived = false;
+    }
+    const uint8_t *mine_at = slots + slot * kChunkBytes + tid * 16;
+    auto take = [&](int u) {
+      const uint4 q = *reinterpret_cast<const uint4 *>(mine_at + u * kThreads * 16);
+      const T *e = reinterpret_cast<const T *>(&q);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[u * V + i] = to_float(e[i]);
+    };
+    if (!edge && arrived && (c + 1) * kThreads * U <= nvec) {  // a whole chunk
+#pragma unroll
+      for (int u = 0; u < U; ++u) take(u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) v[i] = kNegInf;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (!edge && arrived && (c * U + u) * kThreads + tid < nvec) take(u);
+    }
+    if (edge && tid < edges) v[0] = to_float(x[edge_col]);
+    float big = v[0];
+#pragma unroll
+    for (int i = 1; i < kElems; ++i) big = fmaxf(big, v[i]);
+    if (big > m) {
+      m = big;
+      const float to = m * kLog2e;
+      s *= exp2_fast(base - to);
+      base = to;
+    }
+    // 2^(v log2 e - base): one rounding of the exponent, none from base, which the sum is relative to. A NaN or
+    // +infinity (base infinite: inf - inf) makes s NaN.
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) s += exp2_fast(fmaf(v[i], kLog2e, -base));
+    // The best pairs. A logit below the bar's is never offered, and after a few chunks hardly any thread has one
+    // that is not: the keys are formed only there.
+    auto key_at = [&](int i) -> uint64_t {
+      if (edge) return i == 0 && tid < edges ? key_of(v[0], edge_col) : 0;
+      const int g = (c * U + i / V) * kThreads + tid;
+      return g < nvec ? key_of(v[i], head + g * V + i % V) : 0;
+    };
+    const int offers = __syncthreads_count(big >= bar_value);
+    if (tid == 0 && c + kStages < c_end) fetch(c + kStages);  // every thread has read this slot
+    if (offers == 0) continue;
+    bound += offers * kElems;
+    uint64_t limit = bar;
+    const int done = c - c_begin;
+    // No room for all that might be offered, or chunk 0, 1, 2, 4, 8 ..: merge what waits, which raises the bar. With
+    // a bar as old as half the chunks, each of them offers about kp pairs.
+    const bool full = bound > kFresh || (done & (done - 1)) == 0;
+    if (full) {
+      merge();
+      __syncthreads();
+      limit = bar;
+      uint64_t mine = 0;
+      if (big >= bar_value)
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) mine = max(mine, key_at(i));
+      if (__syncthreads_count(mine > bar) * kElems > kFresh) {
+        // Still none (the first chunk, rising logits): kp threads' largest pairs are enough, no pair below the
+        // smallest of those kp can be kept. Of the first 64 threads, which is quick and does for logits in no
+        // order; else of all, so that at most kp * kElems pairs come in, whatever the order.
+        best_of[tid] = mine > bar ? mine : 0;
+        if (tid == 0) raised = bar;
+        __syncthreads();
+        for (int n = 64; n <= kThreads; n *= 4) {
+          if (tid < n && mine > bar) {
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) rank += best_of[j] > mine;
+            if (rank == kp - 1) raised = mine - 1;
+          }
+          __syncthreads();
+          limit = raised;
+          if (__syncthreads_count(mine > limit) * kElems <= kFresh) break;
+        }
+      }
+    }
+    const float limit_value = limit ? value_of_key(limit) : kNegInf;
+    if (big >= limit_value) {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i)
+        if (v[i] >= limit_value) {
+          const uint64_t key = key_at(i);
+          if (key > limit) fresh[atomicAdd(&nfresh, 1)] = key;
+        }
+    }
+    if (full) {
+      __syncthreads();
+      merge();
+      __syncthreads();
+      bound = 0;
+    }
   }
+  __syncthreads();
+  merge();
 
-  // Join the threads' maxima and sums, in one fixed order.
-  float top = m;
+  // Join the threads' sums, in one fixed order.
+  float top = base;
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (tid % 32 == 0) red[0][tid / 32] = top;
-  bad = __syncthreads_or(bad);
+  __syncthreads();
   top = red[0][0];
   for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, red[0][w]);
-  s *= expf(m - top);
+  s *= exp2_fast(base - top);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (tid % 32 == 0) red[1][tid / 32] = s;
   __syncthreads();
-  uint8_t *out = p.parts + static_cast<int64_t>(blockIdx.x) * p.part_bytes;
   if (tid == 0) {
     s = 0.f;
     for (int w = 0; w < kThreads / 32; ++w) s += red[1][w];
-    *reinterpret_cast<Part *>(out) = Part{top, s, bad, have};
+    p.parts.sums[blockIdx.x] = make_float2(top, s);
   }
-  uint64_t *keys = reinterpret_cast<uint64_t *>(out + sizeof(Part));
-  for (int i = tid; i < have; i += kThreads) keys[i] = list[cur][i];
+  uint64_t *keys = p.parts.keys + static_cast<int64_t>(blockIdx.x) * kp;
+  if (tid < kp) keys[tid] = tid < have ? list[cur][tid] : 0;
+}
+
+template <typename T>
+int scan_launch(const ScanParams &p, dim3 grid, cudaStream_t s, const char *what) {
+  const size_t smem = kStages * kChunkBytes;
+  static size_t configured[64] = {};
+  if (int rc = ensure_smem(beam_scan_kernel<T>, smem, configured, what)) return rc;
+  return launch_overlapped(beam_scan_kernel<T>, grid, dim3(kThreads), smem, s, what, p);
 }
 
 struct MergeParams {
   const void *logits;
   const float *scores;
   const uint8_t *finished;
-  const uint8_t *parts;
+  Parts parts;
   float *next_scores;
   int32_t *tokens, *parents;
   uint8_t *next_finished;
   int64_t ld;
-  int dtype, beams, vocab, splits, part_bytes, eos;
+  int dtype, beams, vocab, splits, eos;
 };
 
 enum : int { kLive = 0, kFinished = 1, kDead = 2 };
@@ -243,91 +333,100 @@ __device__ __forceinline__ float score_of(float score, float logit, float lse) {
   return c == c ? c : kNegInf;
 }
 
-// One CTA per request. Dynamic shared memory: kp keys per (beam, split) list.
+// One CTA per request. Dynamic shared memory: kp keys per (beam, split) list, then a position in each.
 __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams p) {
   extern __shared__ uint64_t cand[];
+  __shared__ float2 sums[kMaxLists];
   __shared__ float lse[kMaxBeams], score[kMaxBeams];
   __shared__ int kind[kMaxBeams];
-  __shared__ uint64_t red[kThreads / 32];
   __shared__ uint64_t chosen[kMaxBeams];
   griddep_launch_dependents();
   griddep_wait();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, kp = p.beams + 1, lists = p.beams * p.splits;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.beams;
-  const uint8_t *parts = p.parts + row0 * p.splits * p.part_bytes;
-  auto part_of = [&](int l) { return reinterpret_cast<const Part *>(parts + static_cast<int64_t>(l) * p.part_bytes); };
+  const uint64_t *keys = p.parts.keys + row0 * p.splits * kp;
+  uint8_t *position = reinterpret_cast<uint8_t *>(cand + lists * kp);
 
-  for (int i = warp; i < p.beams; i += kThreads / 32) {
-    const float sc = p.scores[row0 + i];
-    int k = p.finished && p.finished[row0 + i] ? kFinished : sc > kNegInf ? kLive : kDead;
-    float total = 0.f;
-    if (k == kLive) {
-      float top = -3.402823466e38f;
-      int bad = 0;
-      for (int j = lane; j < p.splits; j += 32) {
-        top = fmaxf(top, part_of(i * p.splits + j)->top);
-        bad |= part_of(i * p.splits + j)->bad;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      for (int j = lane; j < p.splits; j += 32) {
-        const Part *q = part_of(i * p.splits + j);
-        total += q->sum * expf(q->top - top);
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      total = top + logf(total);
-      bad = __any_sync(0xffffffffu, bad);
-      if (bad || !(fabsf(total) < INFINITY)) k = kDead;
-      if (bad && lane == 0) raise_status(kStatusBeamNonFinite);
-    }
-    if (lane == 0) lse[i] = total, score[i] = sc == sc ? sc : kNegInf, kind[i] = k;
+  // Everything is fetched at once; the lists of beams that are not live hold nothing and are replaced below.
+  for (int e = tid; e < lists * kp; e += kThreads) cand[e] = keys[e];
+  if (tid < lists) sums[tid] = p.parts.sums[row0 * p.splits + tid], position[tid] = 0;
+  if (tid < p.beams) {
+    const float sc = p.scores[row0 + tid];
+    score[tid] = sc == sc ? sc : kNegInf;
+    kind[tid] = p.finished && p.finished[row0 + tid] ? kFinished : sc > kNegInf ? kLive : kDead;
   }
   __syncthreads();
-
-  // List `tid`: its pairs as (score, flat index) keys, and the best of them.
-  uint64_t *own = cand + tid * kp;
-  uint64_t best = 0;
-  uint64_t last = 0;  // the logit key of a full list's last pair
-  if (tid < lists) {
-    const int i = tid / p.splits;
-    const uint32_t flat0 = static_cast<uint32_t>(i) * p.vocab;
-    int count = 0;
-    if (kind[i] == kLive) {
-      const Part *q = part_of(tid);
-      const uint64_t *keys = reinterpret_cast<const uint64_t *>(q + 1);
-      count = q->count;
-      for (int j = 0; j < count; ++j)
-        own[j] = key_of(score_of(score[i], value_of_key(keys[j]), lse[i]), flat0 + index_of(keys[j]));
-      if (count == kp) last = keys[kp - 1];
-    } else if (tid % p.splits == 0) {
-      const int at = kind[i] == kFinished ? p.eos : -1;
-      if (at >= 0) own[count++] = key_of(score[i], flat0 + at);
-      for (int v = 0; v < p.vocab && count < kp; ++v)
-        if (v != at) own[count++] = key_of(kNegInf, flat0 + v);
+  for (int i = warp; i < p.beams; i += kThreads / 32) {
+    if (kind[i] != kLive) continue;
+    float top = kLowest, total = 0.f;
+    for (int j = lane; j < p.splits; j += 32) top = fmaxf(top, sums[i * p.splits + j].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int j = lane; j < p.splits; j += 32) total += sums[i * p.splits + j].y * exp2_fast(sums[i * p.splits + j].x - top);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) {
+      if (total != total) raise_status(kStatusBeamNonFinite);
+      total = static_cast<float>((top + log2(static_cast<double>(total))) * 0.69314718055994530942);
+      lse[i] = total;
+      if (!(fabsf(total) < INFINITY)) kind[i] = kDead;
     }
-    for (int j = count; j < kp; ++j) own[j] = 0;
-    for (int j = 0; j < kp; ++j) best = max(best, own[j]);
   }
-  for (int k = 0; k < p.beams; ++k) {
-    uint64_t top = best;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
-    top = red[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) top = max(top, red[w]);
-    if (top == best && top) {  // keys are unique: one thread
-      chosen[k] = top;
+  __syncthreads();
+  uint64_t last = 0;  // the logit key that ends list `tid` if it is full
+  if (tid < lists && kind[tid / p.splits] == kLive) last = cand[tid * kp + kp - 1];
+  __syncthreads();
+  for (int e = tid; e < lists * kp; e += kThreads) {  // (logit, token) -> (score, flat index)
+    const int l = e / kp, j = e % kp, i = l / p.splits;
+    const uint32_t flat0 = static_cast<uint32_t>(i) * p.vocab;
+    uint64_t key = 0;
+    if (kind[i] == kLive) {
+      key = cand[e];
+      if (key) key = key_of(score_of(score[i], value_of_key(key), lse[i]), flat0 + index_of(key));
+    } else if (l % p.splits == 0 && j < p.vocab) {
+      // eos first if it scores, then the others from token 0 on, all -inf
+      const int at = kind[i] == kFinished ? p.eos : p.vocab;
+      key = j == 0 && at < p.vocab ? key_of(score[i], flat0 + at)
+                                   : key_of(kNegInf, flat0 + (at == p.vocab ? j : j - 1 < at ? j - 1 : j));
+    }
+    cand[e] = key;
+  }
+  __syncthreads();
+  // The lists are in order of their logits; where rounding makes scores equal, the index decides.
+  if (tid < lists) {
+    uint64_t *own = cand + tid * kp;
+    for (int j = 1; j < kp; ++j) {
+      const uint64_t key = own[j];
+      int at = j;
+      for (; at > 0 && own[at - 1] < key; --at) own[at] = own[at - 1];
+      if (at < j) own[at] = key;
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {  // one warp takes the best head of the lists, `beams` times: a lane has every 32nd list
+    uint64_t best = 0;
+    int from = 0;
+    auto look = [&]() {
       best = 0;
-      for (int j = 0; j < kp; ++j) {
-        if (own[j] == top) own[j] = 0;
-        best = max(best, own[j]);
+      for (int l = lane; l < lists; l += 32) {
+        const int at = position[l];
+        const uint64_t key = at < kp ? cand[l * kp + at] : 0;
+        if (key > best) best = key, from = l;
+      }
+    };
+    look();
+    for (int k = 0; k < p.beams; ++k) {
+      const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(best >> 32));
+      const bool in = static_cast<uint32_t>(best >> 32) == hi;
+      const uint32_t lo = __reduce_max_sync(0xffffffffu, in ? static_cast<uint32_t>(best) : 0u);
+      if (in && static_cast<uint32_t>(best) == lo) {  // keys are unique: one lane
+        chosen[k] = best;
+        ++position[from];
+        look();
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
 
   // Unequal logits with equal scores: a token that was not kept could tie with the last chosen one and
   // have a lower index, where a full list's last pair ties with it and so would the next lower logit.
@@ -449,7 +548,7 @@ int reorder_launch(const ReorderParams &p, int batch, int nstates, cudaStream_t 
 extern "C" size_t mq_beam_workspace_size(int64_t batch, int beams, int64_t vocab) {
   if (batch <= 0 || beams <= 0 || beams > mq::beam::kMaxBeams || vocab <= 0) return 0;
   const int64_t rows = batch * beams;
-  return static_cast<size_t>(rows) * mq::beam::splits_for(rows, beams, vocab) * (sizeof(mq::beam::Part) + 8 * (beams + 1));
+  return mq::beam::parts_bytes(rows * mq::beam::splits_for(rows, beams, vocab), beams + 1);
 }
 
 extern "C" int mq_beam_select(const void *logits, int dtype, int64_t ld, const float *scores, const uint8_t *finished,
@@ -460,7 +559,7 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t ld, const f
   const char *what = "mq_beam_select";
   MQ_REQUIRE(batch >= 0 && beams > 0 && vocab > 0, MQ_EINVAL, "%s: bad shape", what);
   MQ_REQUIRE(beams <= kMaxBeams, MQ_EUNSUPPORTED, "%s: beams is above %d", what, kMaxBeams);
-  MQ_REQUIRE(vocab * beams < (1LL << 31) - kChunk && batch * beams < (1LL << 22), MQ_EUNSUPPORTED,
+  MQ_REQUIRE(vocab * beams < (1LL << 31) - kChunkBytes && batch * beams < (1LL << 22), MQ_EUNSUPPORTED,
              "%s: beams * vocab or batch * beams is too large", what);
   MQ_REQUIRE(dtype == MQ_F32 || dtype == MQ_F16 || dtype == MQ_BF16, MQ_EINVAL,
              "%s: the logits' type must be MQ_F32, MQ_F16 or MQ_BF16", what);
@@ -478,20 +577,21 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t ld, const f
   if (int rc = mq::device_info(&dev)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t rows = batch * beams;
-  const int splits = splits_for(rows, beams, vocab), part = static_cast<int>(sizeof(Part)) + 8 * (beams + 1);
-  ScanParams sp{logits, scores, finished, static_cast<uint8_t *>(workspace), ld, beams, static_cast<int>(vocab), splits, part};
+  const int splits = splits_for(rows, beams, vocab);
+  const Parts parts = parts_at(workspace, rows * splits);
+  ScanParams sp{logits, scores, finished, parts, ld, beams, static_cast<int>(vocab), splits};
   const dim3 grid(static_cast<unsigned>(rows * splits));
   int rc;
   if (dtype == MQ_F32)
-    rc = mq::launch_overlapped(beam_scan_kernel<float>, grid, dim3(kThreads), 0, s, what, sp);
+    rc = scan_launch<float>(sp, grid, s, what);
   else if (dtype == MQ_F16)
-    rc = mq::launch_overlapped(beam_scan_kernel<__half>, grid, dim3(kThreads), 0, s, what, sp);
+    rc = scan_launch<__half>(sp, grid, s, what);
   else
-    rc = mq::launch_overlapped(beam_scan_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, s, what, sp);
+    rc = scan_launch<__nv_bfloat16>(sp, grid, s, what);
   if (rc) return rc;
-  MergeParams mp{logits, scores, finished, static_cast<const uint8_t *>(workspace), next_scores, tokens, parents, next_finished, ld, dtype,
-                 beams, static_cast<int>(vocab), splits, part, eos};
-  const size_t smem = static_cast<size_t>(kThreads) * (beams + 1) * 8;
+  MergeParams mp{logits, scores, finished, parts, next_scores, tokens, parents, next_finished, ld, dtype, beams,
+                 static_cast<int>(vocab), splits, eos};
+  const size_t smem = static_cast<size_t>(beams) * splits * (beams + 1) * 8 + kMaxLists;
   static size_t configured[64] = {};
   if (int rc2 = mq::ensure_smem(beam_merge_kernel, smem, configured, what)) return rc2;
   return mq::launch_overlapped(beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(kThreads), smem, s, what, mp);

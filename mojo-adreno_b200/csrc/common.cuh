@@ -141,6 +141,7 @@ enum : int {
   kStatusW8MmaWait = 13,
   kStatusW8EpiWait = 14,
   kStatusBeamNonFinite = 15,  // a beam's logits hold a NaN or +infinity: none of its tokens was selected
+  kStatusBeamLoadWait = 17,
   kStatusBeamBadParent = 16,  // a parent outside [0, beams): its beam kept its own state
 };
 
@@ -287,6 +288,14 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void 
 __device__ __forceinline__ void bulk_commit_and_wait() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// Untiled copy of `bytes` (a multiple of 16) of global memory into shared memory, completing on `bar`; both
+// addresses 16-byte aligned.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 // Warms L2 with `bytes` (a multiple of 16) of global memory from a 16-byte aligned address.
