@@ -24,22 +24,21 @@ constexpr int kThreads = 256;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 256;  // (beam, split) lists of a request: one per thread of the merge
 constexpr int kVecs = 4;        // 16-byte vectors per thread and chunk
-constexpr int kChunkBytes = kThreads * kVecs * 16;
+constexpr int kScan = 128, kScanCtas = 8;  // threads of a scan CTA, CTAs per SM
+constexpr int kChunkBytes = kScan * kVecs * 16;
 constexpr int kFresh = 1280;    // pairs that may wait to be merged into the list: at least (kMaxBeams + 1) * 32
 constexpr int kStages = 2;      // chunks on their way into shared memory: 32 KB for each of four CTAs per SM
 constexpr float kNegInf = -INFINITY, kLowest = -3.402823466e38f, kLog2e = 1.44269504088896340736f;
 
 // (Counted in fp32 chunks for every type, so that the workspace's size does not depend on it.)
-// The least (CTAs of an SM) x (chunks of a CTA + 6 for its start and end); at most one list per thread of the
-// merge.
+// As many CTAs as run at once (64x8x128256: 2 splits, 63 us; 1: 88, 3: 80; 16x4x50257: 16 splits, 16 us; 8: 19, 24:
+// 17.5); at most one list per thread of the merge.
 __host__ __device__ constexpr int splits_for(int64_t rows, int beams, int64_t vocab) {
   const int64_t chunks = (vocab * 4 + kChunkBytes - 1) / kChunkBytes;
-  int64_t best = 1, least = INT64_MAX;
-  for (int64_t s = 1; s <= kMaxLists / beams && s <= chunks; ++s) {
-    const int64_t cost = (rows * s + 147) / 148 * ((chunks + s - 1) / s + 6);
-    if (cost < least) least = cost, best = s;
-  }
-  return static_cast<int>(best);
+  int64_t s = 148 * kScanCtas / rows;
+  if (s > kMaxLists / beams) s = kMaxLists / beams;
+  if (s > chunks) s = chunks;
+  return s < 1 ? 1 : static_cast<int>(s);
 }
 
 // What the CTAs leave for the merge: a base and the sum of 2^(v log2 e - base) each (NaN where a logit is NaN
@@ -98,17 +97,17 @@ __device__ __forceinline__ bool live_beam(const float *scores, const uint8_t *fi
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScan, kScanCtas) beam_scan_kernel(const ScanParams p) {
   constexpr int V = 16 / sizeof(T), U = kVecs, kElems = V * U;  // elements of a vector; vectors, elements per chunk
-  constexpr int kChunk = kThreads * kElems;
+  constexpr int kChunk = kScan * kElems;
   extern __shared__ __align__(16) uint8_t slots[];   // kStages chunks
   __shared__ uint64_t full[kStages];
   __shared__ uint64_t list[2][kMaxBeams + 1];
   __shared__ uint64_t fresh[kFresh];
-  __shared__ uint64_t best_of[kThreads];
+  __shared__ uint64_t best_of[kScan];
   __shared__ uint64_t raised;
   __shared__ int nfresh;
-  __shared__ float red[2][kThreads / 32];
+  __shared__ float red[2][kScan / 32];
   const int tid = threadIdx.x, kp = p.beams + 1;
   griddep_launch_dependents();
   if (tid == 0) {
@@ -126,13 +125,13 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
   // (at most V - 1 each) are one more step of the first split's CTA.
   const int head = min(p.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
   const int nvec = (p.vocab - head) / V, body_end = head + nvec * V, edges = head + p.vocab - body_end;
-  const int chunks = (nvec + kThreads * U - 1) / (kThreads * U);
+  const int chunks = (nvec + kScan * U - 1) / (kScan * U);
   const int c_begin = static_cast<int>(static_cast<int64_t>(chunks) * split / p.splits);
   const int c_end = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / p.splits);
   const int c_last = c_end + (split == 0 && edges > 0);
   auto fetch = [&](int c) {  // by thread 0
     const int slot = (c - c_begin) % kStages;
-    const uint32_t bytes = min(nvec - c * kThreads * U, kThreads * U) * 16;
+    const uint32_t bytes = min(nvec - c * kScan * U, kScan * U) * 16;
     mbar_expect_tx(&full[slot], bytes);
     bulk_load(slots + slot * kChunkBytes, x + head + static_cast<int64_t>(c) * kChunk, bytes, &full[slot]);
   };
@@ -148,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
   // a barrier behind the last append; the next append comes behind a barrier too.
   auto merge = [&]() {
     const int n = have + nfresh, old = have;
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid; i < n; i += kScan) {
       const uint64_t key = i < old ? list[cur][i] : fresh[i - old];
       int rank = 0;
       for (int j = 0; j < old; ++j) rank += list[cur][j] > key;
@@ -173,12 +172,12 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
     }
     const uint8_t *mine_at = slots + slot * kChunkBytes + tid * 16;
     auto take = [&](int u) {
-      const uint4 q = *reinterpret_cast<const uint4 *>(mine_at + u * kThreads * 16);
+      const uint4 q = *reinterpret_cast<const uint4 *>(mine_at + u * kScan * 16);
       const T *e = reinterpret_cast<const T *>(&q);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[u * V + i] = to_float(e[i]);
     };
-    if (!edge && arrived && (c + 1) * kThreads * U <= nvec) {  // a whole chunk
+    if (!edge && arrived && (c + 1) * kScan * U <= nvec) {  // a whole chunk
 #pragma unroll
       for (int u = 0; u < U; ++u) take(u);
     } else {
@@ -186,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
       for (int i = 0; i < kElems; ++i) v[i] = kNegInf;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (!edge && arrived && (c * U + u) * kThreads + tid < nvec) take(u);
+        if (!edge && arrived && (c * U + u) * kScan + tid < nvec) take(u);
     }
     if (edge && tid < edges) v[0] = to_float(x[edge_col]);
     float big = v[0];
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
     // that is not: the keys are formed only there.
     auto key_at = [&](int i) -> uint64_t {
       if (edge) return i == 0 && tid < edges ? key_of(v[0], edge_col) : 0;
-      const int g = (c * U + i / V) * kThreads + tid;
+      const int g = (c * U + i / V) * kScan + tid;
       return g < nvec ? key_of(v[i], head + g * V + i % V) : 0;
     };
     const int offers = __syncthreads_count(big >= bar_value);
@@ -214,13 +213,12 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
     if (offers == 0) continue;
     bound += offers * kElems;
     uint64_t limit = bar;
-    const int done = c - c_begin;
-    // No room for all that might be offered, or chunk 0, 1, 2, 4, 8 ..: merge what waits, which raises the bar. With
-    // a bar as old as half the chunks, each of them offers about kp pairs.
-    const bool full = bound > kFresh || (done & (done - 1)) == 0;
-    if (full) {
-      merge();
-      __syncthreads();
+    const bool full = bound > kFresh;
+    if (full) {  // no room for all that might be offered: merge what waits, which raises the bar
+      if (bound > offers * kElems) {
+        merge();
+        __syncthreads();
+      }
       limit = bar;
       uint64_t mine = 0;
       if (big >= bar_value)
@@ -233,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
         best_of[tid] = mine > bar ? mine : 0;
         if (tid == 0) raised = bar;
         __syncthreads();
-        for (int n = 64; n <= kThreads; n *= 4) {
+        for (int n = 64; n <= kScan; n *= kScan / 64) {
           if (tid < n && mine > bar) {
             int rank = 0;
 #pragma unroll 8
@@ -255,7 +253,9 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
           if (key > limit) fresh[atomicAdd(&nfresh, 1)] = key;
         }
     }
-    if (full) {
+    // Chunks 0, 1, 2, 4, 8 ..: with a bar at most half as old as the row, each chunk offers about kp pairs.
+    const int done = c - c_begin;
+    if (full || (done & (done - 1)) == 0) {
       __syncthreads();
       merge();
       __syncthreads();
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
   if (tid % 32 == 0) red[0][tid / 32] = top;
   __syncthreads();
   top = red[0][0];
-  for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, red[0][w]);
+  for (int w = 1; w < kScan / 32; ++w) top = fmaxf(top, red[0][w]);
   s *= exp2_fast(base - top);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_scan_kernel(const ScanParams
   __syncthreads();
   if (tid == 0) {
     s = 0.f;
-    for (int w = 0; w < kThreads / 32; ++w) s += red[1][w];
+    for (int w = 0; w < kScan / 32; ++w) s += red[1][w];
     p.parts.sums[blockIdx.x] = make_float2(top, s);
   }
   uint64_t *keys = p.parts.keys + static_cast<int64_t>(blockIdx.x) * kp;
@@ -292,7 +292,7 @@ int scan_launch(const ScanParams &p, dim3 grid, cudaStream_t s, const char *what
   const size_t smem = kStages * kChunkBytes;
   static size_t configured[64] = {};
   if (int rc = ensure_smem(beam_scan_kernel<T>, smem, configured, what)) return rc;
-  return launch_overlapped(beam_scan_kernel<T>, grid, dim3(kThreads), smem, s, what, p);
+  return launch_overlapped(beam_scan_kernel<T>, grid, dim3(kScan), smem, s, what, p);
 }
 
 struct MergeParams {
@@ -333,7 +333,39 @@ __device__ __forceinline__ float score_of(float score, float logit, float lse) {
   return c == c ? c : kNegInf;
 }
 
-// One CTA per request. Dynamic shared memory: kp keys per (beam, split) list, then a position in each.
+// One warp takes the best head of the sorted lists `count` times: a lane has lists lane, lane + 32 .. (N of them).
+template <int N>
+__device__ __forceinline__ void take_best(const uint64_t *cand, int lists, int kp, int count, int lane, uint64_t *chosen) {
+  uint64_t head[N], best = 0;
+  int at[N];  // where each list's head is
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    at[n] = (lane + 32 * n) * kp;
+    head[n] = lane + 32 * n < lists ? cand[at[n]] : 0;
+    best = max(best, head[n]);
+  }
+  for (int k = 0; k < count; ++k) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(best >> 32));
+    const bool in = static_cast<uint32_t>(best >> 32) == hi;
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, in ? static_cast<uint32_t>(best) : 0u);
+    if (in && static_cast<uint32_t>(best) == lo) {  // keys are unique: one lane, one of its lists
+      chosen[k] = best;
+      int list = 0, next_at = 0;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (head[n] == best) list = n, next_at = at[n] + 1;
+      const uint64_t next = next_at < (lane + 32 * list + 1) * kp ? cand[next_at] : 0;
+      best = 0;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (n == list) head[n] = next, at[n] = next_at;
+        best = max(best, head[n]);
+      }
+    }
+  }
+}
+
+// One CTA per request. Dynamic shared memory: kp keys per (beam, split) list.
 __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams p) {
   extern __shared__ uint64_t cand[];
   __shared__ float2 sums[kMaxLists];
@@ -345,11 +377,10 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, kp = p.beams + 1, lists = p.beams * p.splits;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.beams;
   const uint64_t *keys = p.parts.keys + row0 * p.splits * kp;
-  uint8_t *position = reinterpret_cast<uint8_t *>(cand + lists * kp);
 
   // Everything is fetched at once; the lists of beams that are not live hold nothing and are replaced below.
   for (int e = tid; e < lists * kp; e += kThreads) cand[e] = keys[e];
-  if (tid < lists) sums[tid] = p.parts.sums[row0 * p.splits + tid], position[tid] = 0;
+  if (tid < lists) sums[tid] = p.parts.sums[row0 * p.splits + tid];
   if (tid < p.beams) {
     const float sc = p.scores[row0 + tid];
     score[tid] = sc == sc ? sc : kNegInf;
@@ -376,14 +407,16 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
   uint64_t last = 0;  // the logit key that ends list `tid` if it is full
   if (tid < lists && kind[tid / p.splits] == kLive) last = cand[tid * kp + kp - 1];
   __syncthreads();
+  // e / kp and l / splits by multiplication: exact for e < kMaxLists * kp, l < kMaxLists.
+  const uint32_t per_kp = ((1u << 22) + kp - 1) / kp, per_split = ((1u << 16) + p.splits - 1) / p.splits;
   for (int e = tid; e < lists * kp; e += kThreads) {  // (logit, token) -> (score, flat index)
-    const int l = e / kp, j = e % kp, i = l / p.splits;
+    const int l = e * per_kp >> 22, j = e - l * kp, i = l * per_split >> 16;
     const uint32_t flat0 = static_cast<uint32_t>(i) * p.vocab;
     uint64_t key = 0;
     if (kind[i] == kLive) {
       key = cand[e];
       if (key) key = key_of(score_of(score[i], value_of_key(key), lse[i]), flat0 + index_of(key));
-    } else if (l % p.splits == 0 && j < p.vocab) {
+    } else if (l == i * p.splits && j < p.vocab) {
       // eos first if it scores, then the others from token 0 on, all -inf
       const int at = kind[i] == kFinished ? p.eos : p.vocab;
       key = j == 0 && at < p.vocab ? key_of(score[i], flat0 + at)
@@ -392,8 +425,13 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
     cand[e] = key;
   }
   __syncthreads();
-  // The lists are in order of their logits; where rounding makes scores equal, the index decides.
-  if (tid < lists) {
+  bool inverted = false;
+  for (int e = tid; e < lists * kp - 1; e += kThreads) {
+    const int l = e * per_kp >> 22;
+    inverted |= e - l * kp < kp - 1 && cand[e] < cand[e + 1];
+  }
+  // The lists are in order of their logits; where rounding made scores equal, the index decides.
+  if (__syncthreads_or(inverted) && tid < lists) {
     uint64_t *own = cand + tid * kp;
     for (int j = 1; j < kp; ++j) {
       const uint64_t key = own[j];
@@ -403,28 +441,11 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
     }
   }
   __syncthreads();
-  if (warp == 0) {  // one warp takes the best head of the lists, `beams` times: a lane has every 32nd list
-    uint64_t best = 0;
-    int from = 0;
-    auto look = [&]() {
-      best = 0;
-      for (int l = lane; l < lists; l += 32) {
-        const int at = position[l];
-        const uint64_t key = at < kp ? cand[l * kp + at] : 0;
-        if (key > best) best = key, from = l;
-      }
-    };
-    look();
-    for (int k = 0; k < p.beams; ++k) {
-      const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(best >> 32));
-      const bool in = static_cast<uint32_t>(best >> 32) == hi;
-      const uint32_t lo = __reduce_max_sync(0xffffffffu, in ? static_cast<uint32_t>(best) : 0u);
-      if (in && static_cast<uint32_t>(best) == lo) {  // keys are unique: one lane
-        chosen[k] = best;
-        ++position[from];
-        look();
-      }
-    }
+  if (warp == 0) {
+    if (lists <= 32)
+      take_best<1>(cand, lists, kp, p.beams, lane, chosen);
+    else
+      take_best<kMaxLists / 32>(cand, lists, kp, p.beams, lane, chosen);
   }
   __syncthreads();
 
@@ -591,7 +612,7 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t ld, const f
   if (rc) return rc;
   MergeParams mp{logits, scores, finished, parts, next_scores, tokens, parents, next_finished, ld, dtype, beams,
                  static_cast<int>(vocab), splits, eos};
-  const size_t smem = static_cast<size_t>(beams) * splits * (beams + 1) * 8 + kMaxLists;
+  const size_t smem = static_cast<size_t>(beams) * splits * (beams + 1) * 8;
   static size_t configured[64] = {};
   if (int rc2 = mq::ensure_smem(beam_merge_kernel, smem, configured, what)) return rc2;
   return mq::launch_overlapped(beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(kThreads), smem, s, what, mp);
