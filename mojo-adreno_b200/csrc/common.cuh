@@ -118,6 +118,17 @@ int ensure_smem(Kern kern, size_t smem, size_t (&seen)[64], const char *what) {
     if (!(cond)) return ::mq::fail(code, __VA_ARGS__); \
   } while (0)
 
+// f(T()) with the C++ type of an activation dtype: a loop inside f then holds no branch on it.
+template <typename F>
+__device__ __forceinline__ void by_type(int dtype, F f) {
+  if (dtype == MQ_F32)
+    f(float());
+  else if (dtype == MQ_F16)
+    f(__half());
+  else
+    f(__nv_bfloat16());
+}
+
 // ---- device: status word ----------------------------------------------------------------------
 
 // Set (first writer wins) by a kernel whose bounded wait ran out; read by mq_device_status().
@@ -142,6 +153,7 @@ enum : int {
   kStatusW8EpiWait = 14,
   kStatusBeamNonFinite = 15,  // a beam's logits hold a NaN or +infinity: none of its tokens was selected
   kStatusBeamLoadWait = 17,
+  kStatusNormLoadWait = 18,
   kStatusBeamBadParent = 16,  // a parent outside [0, beams): its beam kept its own state
 };
 

@@ -100,16 +100,6 @@ __device__ __forceinline__ void put(void *y, int64_t at, float v, int add) {
   T *p = static_cast<T *>(y) + at;
   *p = from_float<T>(add ? static_cast<float>(*p) + v : v);
 }
-template <typename F>
-__device__ __forceinline__ void by_type(int dtype, F f) {
-  if (dtype == MQ_F32)
-    f(float());
-  else if (dtype == MQ_F16)
-    f(__half());
-  else
-    f(__nv_bfloat16());
-}
-
 // silu(g) * u with the fast exponential and quotient: their errors, (2 + 1.2 |g|) and 2 ulp, are below what
 // one rounding of g does to silu for large |g|; the accurate forms cost the epilogue several times as much.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }

@@ -11,6 +11,7 @@
 // (warp shuffles, then shared memory), in one fixed order. Sums and r' are fp32; r' is rounded only where
 // it is stored, the norm that follows reads the unrounded value.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -27,60 +28,82 @@ struct Params {
   int64_t rows_per_gate;
   int y_dt, w_dt, r_dt, g_dt, nw_dt, h_dt;  // out has residual's type
   int cols, tpr;
-  float scale, eps, next_eps;
+  float scale, eps, next_eps, inv_cols;
 };
 
-template <int VEC>
-__device__ __forceinline__ void load_vec(const void *p, int dt, int64_t at, float *v) {
-  if (VEC == 1) {
-    v[0] = dt == MQ_F32   ? static_cast<const float *>(p)[at]
-           : dt == MQ_F16 ? __half2float(static_cast<const __half *>(p)[at])
-                          : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[at]);
-  } else if (dt == MQ_F32) {
-    const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at);
+template <typename T, int VEC>
+struct alignas(VEC == 1 ? sizeof(T) : 16) Raw {
+  T v[VEC];
+};
+// Values of a vector as fp32 and back: two at a time for the 16-bit types (a bf16 is the upper half of its fp32).
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Raw<T, VEC> &raw, float *v) {
+  if constexpr (VEC == 1 || std::is_same<T, float>::value) {
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) {
-      const float4 f = q[i];
-      v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
-    }
+    for (int i = 0; i < VEC; ++i) v[i] = static_cast<float>(raw.v[i]);
   } else {
-    const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
-    const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+    const uint4 q = *reinterpret_cast<const uint4 *>(&raw);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (dt == MQ_F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r[i]));
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
         v[2 * i] = f.x, v[2 * i + 1] = f.y;
-      } else {  // a bf16 is the upper half of its fp32
-        v[2 * i] = __uint_as_float(r[i] << 16), v[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
       }
     }
   }
 }
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, int dt) {
-  if (dt == MQ_F16) return pack_half2(lo, hi);
-  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&b);
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T *p, const float *v) {
+  if constexpr (std::is_same<T, float>::value && VEC == 8) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else if constexpr (VEC == 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        w[i] = pack_half2(v[2 * i], v[2 * i + 1]);
+      } else {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&b);
+      }
+    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    if constexpr (std::is_same<T, float>::value) *p = v[0];
+    if constexpr (std::is_same<T, __half>::value) *p = __float2half_rn(v[0]);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) *p = __float2bfloat16_rn(v[0]);
+  }
 }
 
-template <int VEC>
-__device__ __forceinline__ void store_vec(void *p, int dt, int64_t at, const float *v) {
-  if (VEC == 1) {
-    if (dt == MQ_F32)
-      static_cast<float *>(p)[at] = v[0];
-    else if (dt == MQ_F16)
-      static_cast<__half *>(p)[at] = __float2half_rn(v[0]);
-    else
-      static_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v[0]);
-  } else if (dt == MQ_F32) {
-    float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
+// This thread's E vectors of a row: f(e, values) for each inside it. All loads are on their way before the first
+// is used.
+template <typename T, int VEC, int E, typename F>
+__device__ __forceinline__ void each_vec_of(const T *row, int cols, int tpr, F f) {
+  Raw<T, VEC> raw[E];
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) q[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else {
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) =
-        make_uint4(pack2(v[0], v[1], dt), pack2(v[2], v[3], dt), pack2(v[4], v[5], dt), pack2(v[6], v[7], dt));
+  for (int e = 0; e < E; ++e) {
+    const int c = (e * tpr + threadIdx.x) * VEC;
+    if (c < cols) raw[e] = *reinterpret_cast<const Raw<T, VEC> *>(row + c);
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if ((e * tpr + threadIdx.x) * VEC >= cols) continue;
+    float v[VEC];
+    unpack<T, VEC>(raw[e], v);
+    f(e, v);
+  }
+}
+// The same for a row that starts at element `at` of an array of a type known at run time.
+template <int VEC, int E, typename F>
+__device__ __forceinline__ void each_vec(const void *base, int dt, int64_t at, int cols, int tpr, F f) {
+  by_type(dt, [&](auto type) {
+    using T = decltype(type);
+    each_vec_of<T, VEC, E>(static_cast<const T *>(base) + at, cols, tpr, f);
+  });
 }
 
 template <int VEC>
@@ -97,100 +120,71 @@ __device__ __forceinline__ void store_s8(int8_t *p, const int *q) {
   }
 }
 
-// Sum and largest bit pattern of |v| over the threads of a row (every thread gets both). The
-// patterns of non-negative floats are ordered as the values, with infinity and NaN above all.
-__device__ __forceinline__ void row_reduce(float &sum, uint32_t &top, int tpr, float *ssum, uint32_t *stop) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (tpr == 32) return;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = tpr / 32;
-  if (lane == 0) ssum[warp] = sum, stop[warp] = top;
-  __syncthreads();
-  sum = lane < warps ? ssum[lane] : 0.f;
-  top = lane < warps ? stop[lane] : 0u;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  top = __reduce_max_sync(0xffffffffu, top);
-}
-
-// E vectors of VEC values per thread; a row has p.tpr threads (threadIdx.x), a CTA blockDim.y rows.
-// EARLY: the dependents may start before this grid ends (not when it may be writing weights).
-template <int VEC, int E, bool POST, bool EARLY>
-__global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const Params p) {
-  __shared__ float ssum[2][16];
-  __shared__ uint32_t stop[2][16];
-  if (EARLY) griddep_launch_dependents();
-  griddep_wait();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  if (row >= p.rows) return;  // rows of one warp each where blockDim.y > 1: no barrier is skipped
-  float z[E * VEC];
-  float sum = 0.f;
+// The largest bit pattern of |v|: the patterns of non-negative floats are ordered as the values, with infinity
+// and NaN above all.
+template <int N>
+__device__ __forceinline__ uint32_t top_of(const float *z) {
   uint32_t top = 0u;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = (e * p.tpr + threadIdx.x) * VEC;
+  for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(z[i]) & 0x7FFFFFFFu);
+  return top;
+}
+
+struct Scratch {  // of one reduction: a value per warp, 0 where there is no warp
+  float sum[16];
+  uint32_t top[16];
+};
+
+// Sum of the squares and (with_top) largest |v| of a row over its `tpr` threads; every thread gets both, in one
+// fixed order. With more than one warp the threads pass one barrier.
+template <int N>
+__device__ __forceinline__ void row_reduce(const float *z, float &sum, uint32_t &top, bool with_top, int tpr, Scratch &s) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) z[e * VEC + i] = 0.f;
-    if (c < p.cols) load_vec<VEC>(p.y, p.y_dt, row * p.ldy + c, z + e * VEC);
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (with_top) top = __reduce_max_sync(0xffffffffu, top_of<N>(z));
+  if (tpr == 32) return;
+  const int warp = threadIdx.x / 32, warps = tpr / 32;
+  if (threadIdx.x % 32 == 0) {
+    s.sum[warp] = sum;
+    if (with_top) s.top[warp] = top;
   }
-  if (POST) {
-    float inv = 1.f;
-    if (p.w) {
+  __syncthreads();
+  sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < E * VEC; ++e) sum += z[e] * z[e];
-      row_reduce(sum, top, p.tpr, ssum[0], stop[0]);
-      inv = rsqrtf(sum / p.cols + p.eps);
-    }
-    inv *= p.scale;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = (e * p.tpr + threadIdx.x) * VEC;
-      if (c >= p.cols) continue;
-      float r[VEC], g[VEC];
-      load_vec<VEC>(p.residual, p.r_dt, row * p.ldr + c, r);
-      if (p.w) {
-        load_vec<VEC>(p.w, p.w_dt, c, g);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= g[i];
-      }
-      if (p.gate) {
-        load_vec<VEC>(p.gate, p.g_dt, row / p.rows_per_gate * p.ldg + c, g);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= g[i];
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) z[e * VEC + i] = fmaf(z[e * VEC + i], inv, r[i]);
-      store_vec<VEC>(p.out, p.r_dt, row * p.ldo + c, z + e * VEC);
-    }
-    if (!p.h) return;
+  for (int w = 0; w < 16; w += 4) {
+    if (w >= warps) break;
+    const float4 f = *reinterpret_cast<const float4 *>(&s.sum[w]);
+    sum += f.x + (w + 1 < warps ? f.y : 0.f) + ((w + 2 < warps ? f.z : 0.f) + (w + 3 < warps ? f.w : 0.f));
   }
-  sum = 0.f, top = 0u;
+  if (with_top)
+    for (int w = 0; w < warps; ++w) top = max(top, s.top[w]);
+}
+
+template <int N>
+__device__ __forceinline__ float squares(const float *z) {
+  float part[4] = {};
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = (e * p.tpr + threadIdx.x) * VEC;
-    if (c >= p.cols) continue;
-    float w[VEC];
-    if (p.next_w) load_vec<VEC>(p.next_w, p.nw_dt, c, w);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float &v = z[e * VEC + i];
-      sum += v * v;
-      if (p.next_w) v *= w[i];
-      top = max(top, __float_as_uint(v) & 0x7FFFFFFFu);
-    }
-  }
-  row_reduce(sum, top, p.tpr, ssum[1], stop[1]);
-  const float inv = p.next_w ? rsqrtf(sum / p.cols + p.next_eps) : 1.f;
+  for (int i = 0; i < N; ++i) part[i % 4] = fmaf(z[i], z[i], part[i % 4]);
+  return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// h from v = z * next_w (z itself without next_w) and the row's sum of squares and largest |v|.
+template <int VEC, int E>
+__device__ __forceinline__ void write_h(const Params &p, int64_t row, float *z, float sum, uint32_t top) {
+  const float inv = p.next_w ? rsqrtf(fmaf(sum, p.inv_cols, p.next_eps)) : 1.f;
   if (p.h_dt != MQ_S8) {
+    by_type(p.h_dt, [&](auto type) {
+      using T = decltype(type);
+      T *h = static_cast<T *>(p.h) + row * p.ldh;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = (e * p.tpr + threadIdx.x) * VEC;
-      if (c >= p.cols) continue;
+      for (int e = 0; e < E; ++e) {
+        const int c = (e * p.tpr + threadIdx.x) * VEC;
+        if (c >= p.cols) continue;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= inv;
-      store_vec<VEC>(p.h, p.h_dt, row * p.ldh + c, z + e * VEC);
-    }
+        for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= inv;
+        store_vec<T, VEC>(h + c, z + e * VEC);
+      }
+    });
     return;
   }
   // A maximum below 1e-30 is lifted by 2^80 (exact) first, so 127 / a stays finite.
@@ -198,6 +192,7 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const Params p)
   const bool bad = top >= 0x7F800000u || !(inv < INFINITY);
   const float f = bad || top == 0u ? 0.f : 127.f / (a * lift);
   if (threadIdx.x == 0) p.hs[row] = bad ? NAN : a / 127.f * inv;
+  int8_t *h = static_cast<int8_t *>(p.h) + row * p.ldh;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = (e * p.tpr + threadIdx.x) * VEC;
@@ -205,7 +200,179 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const Params p)
     int q[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) q[i] = bad ? 0 : __float2int_rn(z[e * VEC + i] * lift * f);
-    store_s8<VEC>(static_cast<int8_t *>(p.h) + row * p.ldh + c, q);
+    store_s8<VEC>(h + c, q);
+  }
+}
+
+// E vectors of VEC values per thread; a row has p.tpr threads (threadIdx.x), a CTA blockDim.y rows.
+// EARLY: the dependents may start before this grid ends (not when it may be writing weights).
+template <int VEC, int E, bool POST, bool EARLY>
+__global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const Params p) {
+  __shared__ __align__(16) Scratch scratch[2];
+  if (EARLY) griddep_launch_dependents();
+  griddep_wait();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (row >= p.rows) return;  // rows of one warp each where blockDim.y > 1: no barrier is skipped
+  const int cols = p.cols, tpr = p.tpr;
+  float z[E * VEC];
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < E * VEC; ++i) z[i] = 0.f;
+  each_vec<VEC, E>(p.y, p.y_dt, row * p.ldy, cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) z[e * VEC + i] = v[i];
+  });
+  if (POST) {
+    float r[E * VEC];  // fetched before the reduction, which hides its latency
+    each_vec<VEC, E>(p.residual, p.r_dt, row * p.ldr, cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) r[e * VEC + i] = v[i];
+    });
+    float inv = p.scale;
+    if (p.w) {
+      float sum = squares<E * VEC>(z);
+      row_reduce<E * VEC>(z, sum, top, false, tpr, scratch[0]);
+      inv *= rsqrtf(fmaf(sum, p.inv_cols, p.eps));
+      each_vec<VEC, E>(p.w, p.w_dt, 0, cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= v[i];
+      });
+    }
+    if (p.gate)
+      each_vec<VEC, E>(p.gate, p.g_dt, row / p.rows_per_gate * p.ldg, cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= v[i];
+      });
+    by_type(p.r_dt, [&](auto type) {
+      using T = decltype(type);
+      T *out = static_cast<T *>(p.out) + row * p.ldo;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = (e * tpr + threadIdx.x) * VEC;
+        if (c >= cols) continue;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[e * VEC + i] = fmaf(z[e * VEC + i], inv, r[e * VEC + i]);
+        store_vec<T, VEC>(out + c, z + e * VEC);
+      }
+    });
+    if (!p.h) return;
+  }
+  float sum = squares<E * VEC>(z);
+  if (p.next_w)
+    each_vec<VEC, E>(p.next_w, p.nw_dt, 0, cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= v[i];
+    });
+  row_reduce<E * VEC>(z, sum, top, p.h_dt == MQ_S8, tpr, scratch[1]);
+  write_h<VEC, E>(p, row, z, sum, top);
+}
+
+// The same for many rows: persistent CTAs of one row at a time, whose next rows (y, residual, gate) are on their
+// way into a ring in shared memory while one is worked on, and which fetch the weights once. Against one CTA per
+// row, which loads, reduces and stores in turn, with its weights from L2 each time: PLACEHOLDER
+constexpr int kRingMax = 8, kStreamThreads = 512;
+struct Ring {
+  int stages, streams;       // rows on their way; 1 (y) or 2, 3 (y, residual, gate) streams each
+  int row_bytes[3], at[3];   // of a stream, and where it is in a stage
+  int stage_bytes, w_at, next_w_at, total;  // bytes; the weights lie behind the ring
+};
+
+// TY, TR, TW: the types of y, of the residual, and of w, next_w and the gate (a branch on a type inside would
+// have the loads of all three from shared memory speculated, and spilled).
+template <typename TY, typename TR, typename TW, int E, bool POST, bool EARLY>
+__global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params p, const Ring g) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kRingMax + 1];  // the last one: the weights
+  __shared__ __align__(16) Scratch scratch[2][2];
+  constexpr int VEC = 8;
+  if (EARLY) griddep_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
+    mbar_init(&full[kRingMax], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  griddep_wait();
+  const int cols = p.cols, tpr = p.tpr;
+  const int step = gridDim.x;
+  auto fetch = [&](int64_t row, int slot) {  // by thread 0
+    uint8_t *at = smem + slot * g.stage_bytes;
+    mbar_expect_tx(&full[slot], g.stage_bytes);
+    bulk_load(at, static_cast<const uint8_t *>(p.y) + row * p.ldy * sizeof(TY), g.row_bytes[0], &full[slot]);
+    if (POST) {
+      bulk_load(at + g.at[1], static_cast<const uint8_t *>(p.residual) + row * p.ldr * sizeof(TR), g.row_bytes[1], &full[slot]);
+      if (p.gate)
+        bulk_load(at + g.at[2], static_cast<const uint8_t *>(p.gate) + row / p.rows_per_gate * p.ldg * sizeof(TW),
+                  g.row_bytes[2], &full[slot]);
+    }
+  };
+  bool arrived = true;
+  if (threadIdx.x == 0) {
+    const int w_bytes = POST && p.w ? cols * static_cast<int>(sizeof(TW)) : 0;
+    const int nw_bytes = p.next_w ? cols * static_cast<int>(sizeof(TW)) : 0;
+    mbar_expect_tx(&full[kRingMax], w_bytes + nw_bytes);
+    if (w_bytes) bulk_load(smem + g.w_at, p.w, w_bytes, &full[kRingMax]);
+    if (nw_bytes) bulk_load(smem + g.next_w_at, p.next_w, nw_bytes, &full[kRingMax]);
+    int64_t row = blockIdx.x;
+    for (int i = 0; i < g.stages && row < p.rows; ++i, row += step) fetch(row, i);
+  }
+  if (!mbar_wait(&full[kRingMax], 0)) {
+    raise_status(kStatusNormLoadWait);
+    arrived = false;
+  }
+  int slot = 0, parity = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += step, parity ^= 1) {
+    if (arrived && !mbar_wait(&full[slot], phase)) {
+      raise_status(kStatusNormLoadWait);  // what there is goes on; the status says that it may be wrong
+      arrived = false;
+    }
+    const uint8_t *at = smem + slot * g.stage_bytes;
+    float z[E * VEC], sum = 0.f;
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < E * VEC; ++i) z[i] = 0.f;
+    each_vec_of<TY, VEC, E>(reinterpret_cast<const TY *>(at), cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[e * VEC + i] = v[i];
+    });
+    if (POST) {
+      float inv = p.scale;
+      if (p.w) {
+        sum = squares<E * VEC>(z);
+        row_reduce<E * VEC>(z, sum, top, false, tpr, scratch[parity][0]);
+        inv *= rsqrtf(fmaf(sum, p.inv_cols, p.eps));
+        each_vec_of<TW, VEC, E>(reinterpret_cast<const TW *>(smem + g.w_at), cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= v[i];
+        });
+      }
+      if (p.gate)
+        each_vec_of<TW, VEC, E>(reinterpret_cast<const TW *>(at + g.at[2]), cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= v[i];
+        });
+      TR *out = static_cast<TR *>(p.out) + row * p.ldo;
+      each_vec_of<TR, VEC, E>(reinterpret_cast<const TR *>(at + g.at[1]), cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[e * VEC + i] = fmaf(z[e * VEC + i], inv, v[i]);
+        store_vec<TR, VEC>(out + (e * tpr + threadIdx.x) * VEC, z + e * VEC);
+      });
+    }
+    if (!POST || p.h) {
+      sum = squares<E * VEC>(z);
+      if (EARLY || p.next_w)
+        each_vec_of<TW, VEC, E>(reinterpret_cast<const TW *>(smem + g.next_w_at), cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= v[i];
+        });
+      row_reduce<E * VEC>(z, sum, top, p.h_dt == MQ_S8, tpr, scratch[parity][1]);
+    }
+    if (tpr == 32 || (POST && !p.h)) __syncthreads();  // else row_reduce's barrier: every thread has read the slot
+    if (threadIdx.x == 0 && row + static_cast<int64_t>(g.stages) * step < p.rows)
+      fetch(row + static_cast<int64_t>(g.stages) * step, slot);
+    if (++slot == g.stages) slot = 0, phase ^= 1;
+    if (!POST || p.h) write_h<VEC, E>(p, row, z, sum, top);
   }
 }
 
@@ -219,20 +386,99 @@ int launch_e(const Params &p, int threads, int rows_per_cta, cudaStream_t s, con
 
 constexpr int kMaxCols = 64 * kMaxThreads;
 
+inline int bytes_of(int dt) { return dt == MQ_F32 ? 4 : 2; }
+
+// The ring for this row size with `per_sm` CTAs on an SM; stages < 2: it does not fit.
+template <bool POST>
+Ring ring_of(const Params &p, int per_sm) {
+  Ring g{};
+  const int dts[3] = {p.y_dt, p.r_dt, p.g_dt};
+  g.streams = POST ? p.gate ? 3 : 2 : 1;
+  for (int i = 0; i < g.streams; ++i) {
+    g.at[i] = g.stage_bytes;
+    g.row_bytes[i] = p.cols * bytes_of(dts[i]);
+    g.stage_bytes += g.row_bytes[i];
+  }
+  const int w = POST && p.w ? p.cols * bytes_of(p.w_dt) : 0, nw = p.next_w ? p.cols * bytes_of(p.nw_dt) : 0;
+  g.stages = std::min(kRingMax, (200 * 1024 / per_sm - 1536 - w - nw) / g.stage_bytes);
+  g.w_at = g.stages * g.stage_bytes;
+  g.next_w_at = g.w_at + w;
+  g.total = g.next_w_at + nw;
+  return g;
+}
+
+// CTAs per SM of the streaming kernel, 0 where it does not apply: 32 values a thread, about 640 threads per SM, fewer
+// where the ring would have less than three stages. The residual has y's type or fp32; w, next_w and the gate one
+// type, y's or fp32.
+template <bool POST>
+int plan_ring(Params &p) {
+  if (POST && p.r_dt != p.y_dt && p.r_dt != MQ_F32) return 0;
+  const int dts[3] = {POST && p.w ? p.w_dt : -1, POST && p.gate ? p.g_dt : -1, p.next_w ? p.nw_dt : -1};
+  int one = -1;
+  for (int dt : dts) {
+    if (dt < 0) continue;
+    if ((dt != p.y_dt && dt != MQ_F32) || (one >= 0 && dt != one)) return 0;
+    one = dt;
+  }
+  p.w_dt = p.g_dt = p.nw_dt = one < 0 ? p.y_dt : one;
+  p.tpr = (p.cols + 511) / 512 * 32;
+  if (p.cols < 1024 || p.tpr > kStreamThreads) return 0;
+  for (int per_sm = std::min(16, 1024 / p.tpr); per_sm >= 1; per_sm = per_sm > 1 ? per_sm / 2 : 0)
+    if (ring_of<POST>(p, per_sm).stages >= (per_sm > 1 ? 3 : 2)) return per_sm;
+  return 0;
+}
+
+template <typename TY, typename TR, typename TW, int E, bool POST, bool EARLY>
+int launch_ring_e(const Params &p, int per_sm, cudaStream_t s, const char *what) {
+  const Ring g = ring_of<POST>(p, per_sm);
+  auto kern = row_stream_kernel<TY, TR, TW, E, POST, EARLY>;
+  static size_t configured[64] = {};
+  if (int rc = ensure_smem(kern, g.total, configured, what)) return rc;
+  const int64_t grid = std::min<int64_t>(p.rows, 148 * per_sm);
+  return launch_overlapped(kern, dim3(static_cast<unsigned>(grid)), dim3(p.tpr), g.total, s, what, p, g);
+}
+
+template <typename TY, bool POST, bool EARLY>
+int launch_ring_y(const Params &p, int per_sm, cudaStream_t s, const char *what) {
+  auto wide = [&](auto r, auto w) {
+    using TR = decltype(r);
+    using TW = decltype(w);
+    return launch_ring_e<TY, TR, TW, 2, POST, EARLY>(p, per_sm, s, what);
+  };
+  auto with_r = [&](auto r) {
+    if constexpr (EARLY && !std::is_same<TY, float>::value)  // (the quantiser has no weights)
+      if (p.nw_dt != p.y_dt) return wide(r, float());
+    return wide(r, TY());
+  };
+  if constexpr (POST && !std::is_same<TY, float>::value)
+    if (p.r_dt != p.y_dt) return with_r(float());
+  return with_r(TY());
+}
+
+template <bool POST, bool EARLY>
+int launch_ring(const Params &p, int per_sm, cudaStream_t s, const char *what) {
+  if (p.y_dt == MQ_F32) return launch_ring_y<float, POST, EARLY>(p, per_sm, s, what);
+  if (p.y_dt == MQ_F16) return launch_ring_y<__half, POST, EARLY>(p, per_sm, s, what);
+  return launch_ring_y<__nv_bfloat16, POST, EARLY>(p, per_sm, s, what);
+}
+
 template <bool POST, bool EARLY>
 int launch(Params p, bool vec, cudaStream_t s, const char *what) {
   MQ_REQUIRE(p.cols <= kMaxCols, MQ_EUNSUPPORTED, "%s: cols is above %d", what, kMaxCols);
+  if (vec && p.rows >= 4 * 148)
+    if (const int per_sm = plan_ring<POST>(p)) return launch_ring<POST, EARLY>(p, per_sm, s, what);
+  // As many threads of a row as there are vectors (8 values each), for the least latency.
+  const int per = vec ? 8 : 4;
+  p.tpr = std::min(kMaxThreads, (p.cols + 32 * per - 1) / (32 * per) * 32);
+  const int rows_per_cta = p.tpr == 32 ? 4 : 1, each = (p.cols + p.tpr - 1) / p.tpr;
   if (vec) {
-    // 8 values per thread (one warp up to 256 columns), 16 to 64 only where a row is too long for that
-    p.tpr = std::min(kMaxThreads, (p.cols + 255) / 256 * 32);
-    if (p.cols <= 8 * p.tpr) return launch_e<8, 1, POST, EARLY>(p, p.tpr, p.tpr == 32 ? 4 : 1, s, what);
-    if (p.cols <= 16 * p.tpr) return launch_e<8, 2, POST, EARLY>(p, p.tpr, 1, s, what);
-    if (p.cols <= 32 * p.tpr) return launch_e<8, 4, POST, EARLY>(p, p.tpr, 1, s, what);
+    if (each <= 8) return launch_e<8, 1, POST, EARLY>(p, p.tpr, rows_per_cta, s, what);
+    if (each <= 16) return launch_e<8, 2, POST, EARLY>(p, p.tpr, rows_per_cta, s, what);
+    if (each <= 32) return launch_e<8, 4, POST, EARLY>(p, p.tpr, rows_per_cta, s, what);
     return launch_e<8, 8, POST, EARLY>(p, p.tpr, 1, s, what);
   }
-  p.tpr = std::min(kMaxThreads, (p.cols + 127) / 128 * 32);
-  if (p.cols <= 4 * p.tpr) return launch_e<1, 4, POST, EARLY>(p, p.tpr, p.tpr == 32 ? 4 : 1, s, what);
-  if (p.cols <= 16 * p.tpr) return launch_e<1, 16, POST, EARLY>(p, p.tpr, 1, s, what);
+  if (each <= 4) return launch_e<1, 4, POST, EARLY>(p, p.tpr, rows_per_cta, s, what);
+  if (each <= 16) return launch_e<1, 16, POST, EARLY>(p, p.tpr, rows_per_cta, s, what);
   return launch_e<1, 64, POST, EARLY>(p, p.tpr, 1, s, what);
 }
 
@@ -280,7 +526,7 @@ extern "C" int mq_quantize_s8(const void *x, int x_dtype, int64_t ldx, int8_t *q
   if (int rc = mq::device_info(&dev)) return rc;
   mq::norm::Params p{};
   p.y = x, p.y_dt = x_dtype, p.ldy = ldx, p.h = q, p.h_dt = MQ_S8, p.ldh = ldq, p.hs = s;
-  p.rows = rows, p.cols = static_cast<int>(cols);
+  p.rows = rows, p.cols = static_cast<int>(cols), p.inv_cols = 1.f / static_cast<float>(cols);
   const bool vec = cols % 8 == 0 && mq::norm::vec_ok(x, x_dtype, ldx, rows) && mq::norm::vec_ok(q, MQ_S8, ldq, rows);
   // No early start of the dependents: q may be a weight matrix, which a product may read ahead.
   return mq::norm::launch<false, false>(p, vec, static_cast<cudaStream_t>(stream), what);
@@ -300,7 +546,7 @@ extern "C" int mq_pre_norm(const void *x, int x_dtype, int64_t ldx, const void *
   mq::norm::Params p{};
   p.y = x, p.y_dt = x_dtype, p.ldy = ldx, p.next_w = w, p.nw_dt = w_dtype, p.next_eps = eps;
   p.h = h, p.h_dt = h_dtype, p.ldh = ldh, p.hs = hs;
-  p.rows = rows, p.cols = static_cast<int>(cols);
+  p.rows = rows, p.cols = static_cast<int>(cols), p.inv_cols = 1.f / static_cast<float>(cols);
   using mq::norm::vec_ok;
   const bool vec = cols % 8 == 0 && vec_ok(x, x_dtype, ldx, rows) && vec_ok(w, w_dtype, cols, 1) &&
                    vec_ok(h, h_dtype, ldh, rows);
@@ -338,7 +584,7 @@ extern "C" int mq_post_norm(const void *y, int y_dtype, int64_t ldy, const void 
   p.gate = gate, p.g_dt = gate_dtype, p.ldg = ldg, p.rows_per_gate = rows_per_gate;
   p.next_w = next_w, p.nw_dt = next_w_dtype, p.next_eps = next_eps;
   p.h = h, p.h_dt = h_dtype, p.ldh = ldh, p.hs = hs;
-  p.rows = rows, p.cols = static_cast<int>(cols);
+  p.rows = rows, p.cols = static_cast<int>(cols), p.inv_cols = 1.f / static_cast<float>(cols);
   using mq::norm::vec_ok;
   const bool vec = cols % 8 == 0 && vec_ok(y, y_dtype, ldy, rows) && vec_ok(residual, r_dtype, ldr, rows) &&
                    vec_ok(out, r_dtype, ldo, rows) && vec_ok(w, w_dtype, cols, 1) &&
