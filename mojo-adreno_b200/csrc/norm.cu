@@ -79,19 +79,19 @@ __device__ __forceinline__ void store_vec(T *p, const float *v) {
   }
 }
 
-// This thread's E vectors of a row: f(e, values) for each inside it. All loads are on their way before the first
-// is used.
+// This thread's E vectors of a row: f(e, values) for each, zeros outside the row. All loads are on their way before
+// the first is used.
 template <typename T, int VEC, int E, typename F>
 __device__ __forceinline__ void each_vec_of(const T *row, int cols, int tpr, F f) {
   Raw<T, VEC> raw[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = (e * tpr + threadIdx.x) * VEC;
+    raw[e] = Raw<T, VEC>{};
     if (c < cols) raw[e] = *reinterpret_cast<const Raw<T, VEC> *>(row + c);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if ((e * tpr + threadIdx.x) * VEC >= cols) continue;
     float v[VEC];
     unpack<T, VEC>(raw[e], v);
     f(e, v);
@@ -106,34 +106,41 @@ __device__ __forceinline__ void each_vec(const void *base, int dt, int64_t at, i
   });
 }
 
+// rint(v * f) as int8, |v * f| <= 127: the sum with 1.5 * 2^23 has the integer in its low bits, rounded to nearest,
+// ties to even. (Conversion instructions run at an eighth of the rate.)
 template <int VEC>
-__device__ __forceinline__ void store_s8(int8_t *p, const int *q) {
-  if (VEC == 1) {
-    *p = static_cast<int8_t>(q[0]);
-  } else {
-    uint32_t r[2];
+__device__ __forceinline__ void store_s8(int8_t *p, const float *v, float f) {
+  uint32_t b[VEC];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      r[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 |
-             static_cast<uint32_t>(q[4 * i + 3]) << 24;
-    *reinterpret_cast<uint2 *>(p) = make_uint2(r[0], r[1]);
-  }
+  for (int i = 0; i < VEC; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], f), 12582912.f));
+  if constexpr (VEC == 1)
+    *p = static_cast<int8_t>(b[0]);
+  else
+    *reinterpret_cast<uint2 *>(p) =
+        make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                   __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
-// The largest bit pattern of |v|: the patterns of non-negative floats are ordered as the values, with infinity
-// and NaN above all.
+// The bits of the largest |v|, a NaN where there is one. The patterns of non-negative floats are ordered as the
+// values, with infinity and NaN above all.
 template <int N>
 __device__ __forceinline__ uint32_t top_of(const float *z) {
-  uint32_t top = 0u;
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(z[i]) & 0x7FFFFFFFu);
-  return top;
+  for (int i = 0; i < N; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(z[i])));
+  return __float_as_uint(top);
 }
 
-struct Scratch {  // of one reduction: a value per warp, 0 where there is no warp
+struct Scratch {  // of one reduction: a value per warp, the sums 0 where there is no warp (clear_scratch)
   float sum[16];
   uint32_t top[16];
 };
+
+// Before the first reduction, behind which there is a barrier.
+__device__ __forceinline__ void clear_scratch(Scratch *s, int n, int warps) {
+  for (int i = threadIdx.x; i < 16 * n; i += blockDim.x)
+    if (i % 16 >= warps) s[i / 16].sum[i % 16] = 0.f;
+}
 
 // Sum of the squares and (with_top) largest |v| of a row over its `tpr` threads; every thread gets both, in one
 // fixed order. With more than one warp the threads pass one barrier.
@@ -150,11 +157,9 @@ __device__ __forceinline__ void row_reduce(const float *z, float &sum, uint32_t 
   }
   __syncthreads();
   sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < 16; w += 4) {
-    if (w >= warps) break;
+  for (int w = 0; w < warps; w += 4) {
     const float4 f = *reinterpret_cast<const float4 *>(&s.sum[w]);
-    sum += f.x + (w + 1 < warps ? f.y : 0.f) + ((w + 2 < warps ? f.z : 0.f) + (w + 3 < warps ? f.w : 0.f));
+    sum += (f.x + f.y) + (f.z + f.w);
   }
   if (with_top)
     for (int w = 0; w < warps; ++w) top = max(top, s.top[w]);
@@ -169,8 +174,10 @@ __device__ __forceinline__ float squares(const float *z) {
 }
 
 // h from v = z * next_w (z itself without next_w) and the row's sum of squares and largest |v|.
-template <int VEC, int E>
+// TPR: p.tpr where it is known when compiling, else 0.
+template <int VEC, int E, int TPR = 0>
 __device__ __forceinline__ void write_h(const Params &p, int64_t row, float *z, float sum, uint32_t top) {
+  const int tpr = TPR ? TPR : p.tpr;
   const float inv = p.next_w ? rsqrtf(fmaf(sum, p.inv_cols, p.next_eps)) : 1.f;
   if (p.h_dt != MQ_S8) {
     by_type(p.h_dt, [&](auto type) {
@@ -178,7 +185,7 @@ __device__ __forceinline__ void write_h(const Params &p, int64_t row, float *z, 
       T *h = static_cast<T *>(p.h) + row * p.ldh;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int c = (e * p.tpr + threadIdx.x) * VEC;
+        const int c = (e * tpr + threadIdx.x) * VEC;
         if (c >= p.cols) continue;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= inv;
@@ -187,20 +194,21 @@ __device__ __forceinline__ void write_h(const Params &p, int64_t row, float *z, 
     });
     return;
   }
-  // A maximum below 1e-30 is lifted by 2^80 (exact) first, so 127 / a stays finite.
-  const float a = __uint_as_float(top), lift = a < 1e-30f ? 0x1p80f : 1.f;
-  const bool bad = top >= 0x7F800000u || !(inv < INFINITY);
-  const float f = bad || top == 0u ? 0.f : 127.f / (a * lift);
+  const float a = __uint_as_float(top);
+  const bool bad = !(a < INFINITY) || !(inv < INFINITY);
   if (threadIdx.x == 0) p.hs[row] = bad ? NAN : a / 127.f * inv;
+  float f = a > 0.f ? 127.f / a : 0.f;
+  if (bad || a < 1e-30f) {  // (the whole row)
+    // A maximum below 1e-30 is lifted by 2^80 (exact) first, so 127 / a stays finite.
+    f = bad || a == 0.f ? 0.f : 127.f / (a * 0x1p80f);
+#pragma unroll
+    for (int i = 0; i < E * VEC; ++i) z[i] = bad ? 0.f : z[i] * 0x1p80f;
+  }
   int8_t *h = static_cast<int8_t *>(p.h) + row * p.ldh;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int c = (e * p.tpr + threadIdx.x) * VEC;
-    if (c >= p.cols) continue;
-    int q[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) q[i] = bad ? 0 : __float2int_rn(z[e * VEC + i] * lift * f);
-    store_s8<VEC>(h + c, q);
+    const int c = (e * tpr + threadIdx.x) * VEC;
+    if (c < p.cols) store_s8<VEC>(h + c, z + e * VEC, f);
   }
 }
 
@@ -211,13 +219,12 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const Params p)
   __shared__ __align__(16) Scratch scratch[2];
   if (EARLY) griddep_launch_dependents();
   griddep_wait();
+  if (p.tpr > 32) clear_scratch(scratch, 2, p.tpr / 32);  // (read behind the reductions' barriers)
   const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if (row >= p.rows) return;  // rows of one warp each where blockDim.y > 1: no barrier is skipped
   const int cols = p.cols, tpr = p.tpr;
   float z[E * VEC];
   uint32_t top = 0u;
-#pragma unroll
-  for (int i = 0; i < E * VEC; ++i) z[i] = 0.f;
   each_vec<VEC, E>(p.y, p.y_dt, row * p.ldy, cols, tpr, [&](int e, const float *v) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) z[e * VEC + i] = v[i];
@@ -267,13 +274,13 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const Params p)
   write_h<VEC, E>(p, row, z, sum, top);
 }
 
-// The same for many rows: persistent CTAs of one row at a time, whose next rows (y, residual, gate) are on their
+// The same for many rows: persistent CTAs of one row at a time, whose next rows (y, residual) are on their
 // way into a ring in shared memory while one is worked on, and which fetch the weights once. Against one CTA per
 // row, which loads, reduces and stores in turn, with its weights from L2 each time: PLACEHOLDER
 constexpr int kRingMax = 8, kStreamThreads = 512;
 struct Ring {
-  int stages, streams;       // rows on their way; 1 (y) or 2, 3 (y, residual, gate) streams each
-  int row_bytes[3], at[3];   // of a stream, and where it is in a stage
+  int stages;                // rows on their way, each of y and, after a block, of the residual
+  int row_bytes[2], at[2];   // of the two, and where they are in a stage
   int stage_bytes, w_at, next_w_at, total;  // bytes; the weights lie behind the ring
 };
 
@@ -291,6 +298,7 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
     mbar_init(&full[kRingMax], 1);
     fence_mbar_init();
   }
+  clear_scratch(&scratch[0][0], 4, p.tpr / 32);
   __syncthreads();
   griddep_wait();
   const int cols = p.cols, tpr = p.tpr;
@@ -301,9 +309,6 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
     bulk_load(at, static_cast<const uint8_t *>(p.y) + row * p.ldy * sizeof(TY), g.row_bytes[0], &full[slot]);
     if (POST) {
       bulk_load(at + g.at[1], static_cast<const uint8_t *>(p.residual) + row * p.ldr * sizeof(TR), g.row_bytes[1], &full[slot]);
-      if (p.gate)
-        bulk_load(at + g.at[2], static_cast<const uint8_t *>(p.gate) + row / p.rows_per_gate * p.ldg * sizeof(TW),
-                  g.row_bytes[2], &full[slot]);
     }
   };
   bool arrived = true;
@@ -328,10 +333,18 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
       arrived = false;
     }
     const uint8_t *at = smem + slot * g.stage_bytes;
+    Raw<TW, VEC> gate[E];  // (a row of it serves many rows, or comes from memory while this one is reduced)
+    if (POST && p.gate) {
+      const TW *from = static_cast<const TW *>(p.gate) + row / p.rows_per_gate * p.ldg;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = (e * tpr + threadIdx.x) * VEC;
+        gate[e] = Raw<TW, VEC>{};
+        if (c < cols) gate[e] = *reinterpret_cast<const Raw<TW, VEC> *>(from + c);
+      }
+    }
     float z[E * VEC], sum = 0.f;
     uint32_t top = 0u;
-#pragma unroll
-    for (int i = 0; i < E * VEC; ++i) z[i] = 0.f;
     each_vec_of<TY, VEC, E>(reinterpret_cast<const TY *>(at), cols, tpr, [&](int e, const float *v) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) z[e * VEC + i] = v[i];
@@ -348,15 +361,19 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
         });
       }
       if (p.gate)
-        each_vec_of<TW, VEC, E>(reinterpret_cast<const TW *>(at + g.at[2]), cols, tpr, [&](int e, const float *v) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float v[VEC];
+          unpack<TW, VEC>(gate[e], v);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) z[e * VEC + i] *= v[i];
-        });
+        }
       TR *out = static_cast<TR *>(p.out) + row * p.ldo;
       each_vec_of<TR, VEC, E>(reinterpret_cast<const TR *>(at + g.at[1]), cols, tpr, [&](int e, const float *v) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) z[e * VEC + i] = fmaf(z[e * VEC + i], inv, v[i]);
-        store_vec<TR, VEC>(out + (e * tpr + threadIdx.x) * VEC, z + e * VEC);
+        const int c = (e * tpr + threadIdx.x) * VEC;
+        if (c < cols) store_vec<TR, VEC>(out + c, z + e * VEC);
       });
     }
     if (!POST || p.h) {
@@ -376,6 +393,178 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
   }
 }
 
+// Rows that are not 16-byte aligned, or not a multiple of 8 long: the 16-byte granules that lie inside a row come
+// through the ring, the few elements before and after them by plain loads one row ahead, each by the thread that
+// works on it, which puts them into their places. A thread has every tpr-th element, 16 at most; its weights
+// stay in registers.
+template <typename T>
+struct Edge {
+  T head, tail;
+};
+template <typename T>
+struct Span {
+  static constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements of a granule
+  int head, end;  // elements before the first granule, first element after the last one
+  __device__ __forceinline__ Span(const T *row, int cols) {
+    head = static_cast<int>((0 - reinterpret_cast<uintptr_t>(row)) % 16 / sizeof(T));
+    end = cols - ((cols - head) & (kPer - 1));
+  }
+  // This thread's elements outside the granules: element threadIdx.x of the first few, element `last` (its one column
+  // among the row's last tpr) of the last few.
+  __device__ __forceinline__ Edge<T> edge(const T *row, int last) const {
+    Edge<T> e{};
+    if (static_cast<int>(threadIdx.x) < head) e.head = row[threadIdx.x];
+    if (last >= end) e.tail = row[last];
+    return e;
+  }
+  // Element 0's place in a slot (the granules start at byte 16) with this thread's edge elements put in.
+  __device__ __forceinline__ const T *put(uint8_t *at, Edge<T> e, int last) const {
+    T *row = reinterpret_cast<T *>(at + 16) - head;
+    const bool first = static_cast<int>(threadIdx.x) < head, final = last >= end;
+    if (first) row[threadIdx.x] = e.head;
+    if (final) row[last] = e.tail;
+    if (first || final) fence_proxy_async_smem();  // before a later row's granules come to the same place
+    return row;
+  }
+};
+
+// TPR: the threads of a row, known so that its elements lie at fixed distances (with a distance known at run time
+// the addresses alone took most of the instructions: 1001 columns 42 us a 20000 rows, see below).
+template <typename TY, typename TR, int TPR, bool POST, bool EARLY>
+__global__ void __launch_bounds__(TPR) row_stream1_kernel(const Params p, const Ring g) {
+  constexpr int E = 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kRingMax];
+  __shared__ __align__(16) Scratch scratch[2][2];
+  if (EARLY) griddep_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  clear_scratch(&scratch[0][0], 4, TPR / 32);
+  __syncthreads();
+  griddep_wait();
+  constexpr int tpr = TPR;
+  const int cols = p.cols, step = gridDim.x;
+  const int last = cols - 1 - ((cols - 1) % tpr + tpr - static_cast<int>(threadIdx.x)) % tpr;
+  const TY *y = static_cast<const TY *>(p.y) + blockIdx.x * p.ldy;  // of this row; `step` rows further on:
+  const TR *r = POST ? static_cast<const TR *>(p.residual) + blockIdx.x * p.ldr : nullptr;
+  const int64_t y_step = step * p.ldy, r_step = step * p.ldr;
+  auto fetch = [&](int64_t row, int slot) {  // by thread 0
+    uint8_t *at = smem + slot * g.stage_bytes + 16;
+    const TY *yr = static_cast<const TY *>(p.y) + row * p.ldy;
+    const Span<TY> ys(yr, cols);
+    const uint32_t y_bytes = (ys.end - ys.head) * sizeof(TY);
+    if (POST) {
+      const TR *rr = static_cast<const TR *>(p.residual) + row * p.ldr;
+      const Span<TR> rs(rr, cols);
+      const uint32_t r_bytes = (rs.end - rs.head) * sizeof(TR);
+      mbar_expect_tx(&full[slot], y_bytes + r_bytes);
+      bulk_load(at + g.at[1], rr + rs.head, r_bytes, &full[slot]);
+    } else {
+      mbar_expect_tx(&full[slot], y_bytes);
+    }
+    bulk_load(at, yr + ys.head, y_bytes, &full[slot]);
+  };
+  if (threadIdx.x == 0) {
+    int64_t row = blockIdx.x;
+    for (int i = 0; i < g.stages && row < p.rows; ++i, row += step) fetch(row, i);
+  }
+  auto weights = [&](const void *base, int dt, float *w) {
+    by_type(dt, [&](auto type) {
+      using T = decltype(type);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = e * tpr + threadIdx.x;
+        w[e] = c < cols ? static_cast<float>((static_cast<const T *>(base) + threadIdx.x)[e * TPR]) : 0.f;
+      }
+    });
+  };
+  float w[E], next_w[E];
+  if (POST && p.w) weights(p.w, p.w_dt, w);
+  if (EARLY && p.next_w) weights(p.next_w, p.nw_dt, next_w);
+  Edge<TY> y_edge{};
+  Edge<TR> r_edge{};
+  if (blockIdx.x < p.rows) {
+    y_edge = Span<TY>(y, cols).edge(y, last);
+    if (POST) r_edge = Span<TR>(r, cols).edge(r, last);
+  }
+  bool arrived = true;
+  int slot = 0, parity = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += step, parity ^= 1) {
+    float gate[E];
+    if (POST && p.gate)
+      by_type(p.g_dt, [&](auto type) {
+        using T = decltype(type);
+        const T *from = static_cast<const T *>(p.gate) + row / p.rows_per_gate * p.ldg + threadIdx.x;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int c = e * tpr + threadIdx.x;
+          gate[e] = c < cols ? static_cast<float>(from[e * TPR]) : 0.f;
+        }
+      });
+    const Span<TY> ys(y, cols);
+    const Span<TR> rs(r, cols);
+    const Edge<TY> y_now = y_edge;
+    const Edge<TR> r_now = r_edge;
+    y += y_step;
+    if (POST) r += r_step;
+    if (row + step < p.rows) {
+      y_edge = Span<TY>(y, cols).edge(y, last);
+      if (POST) r_edge = Span<TR>(r, cols).edge(r, last);
+    }
+    if (arrived && !mbar_wait(&full[slot], phase)) {
+      raise_status(kStatusNormLoadWait);  // what there is goes on; the status says that it may be wrong
+      arrived = false;
+    }
+    uint8_t *at = smem + slot * g.stage_bytes;
+    float z[E], sum = 0.f;
+    uint32_t top = 0u;
+    const TY *from = ys.put(at, y_now, last) + threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = e * tpr + threadIdx.x;
+      z[e] = c < cols ? static_cast<float>(from[e * TPR]) : 0.f;
+    }
+    if (POST) {
+      float inv = p.scale;
+      if (p.w) {
+        sum = squares<E>(z);
+        row_reduce<E>(z, sum, top, false, tpr, scratch[parity][0]);
+        inv *= rsqrtf(fmaf(sum, p.inv_cols, p.eps));
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[e] *= w[e];
+      }
+      if (p.gate)
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[e] *= gate[e];
+      const TR *residual = rs.put(at + g.at[1], r_now, last) + threadIdx.x;
+      TR *out = static_cast<TR *>(p.out) + row * p.ldo + threadIdx.x;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = e * tpr + threadIdx.x;
+        if (c < cols) {
+          z[e] = fmaf(z[e], inv, static_cast<float>(residual[e * TPR]));
+          store_vec<TR, 1>(out + e * TPR, z + e);
+        }
+      }
+    }
+    if (!POST || p.h) {
+      sum = squares<E>(z);
+      if (EARLY && p.next_w)
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[e] *= next_w[e];
+      row_reduce<E>(z, sum, top, p.h_dt == MQ_S8, tpr, scratch[parity][1]);
+    }
+    if (tpr == 32 || (POST && !p.h)) __syncthreads();  // else row_reduce's barrier: every thread has read the slot
+    if (threadIdx.x == 0 && row + static_cast<int64_t>(g.stages) * step < p.rows)
+      fetch(row + static_cast<int64_t>(g.stages) * step, slot);
+    if (++slot == g.stages) slot = 0, phase ^= 1;
+    if (!POST || p.h) write_h<1, E, TPR>(p, row, z, sum, top);
+  }
+}
+
 template <int VEC, int E, bool POST, bool EARLY>
 int launch_e(const Params &p, int threads, int rows_per_cta, cudaStream_t s, const char *what) {
   const int64_t grid = (p.rows + rows_per_cta - 1) / rows_per_cta;
@@ -392,9 +581,8 @@ inline int bytes_of(int dt) { return dt == MQ_F32 ? 4 : 2; }
 template <bool POST>
 Ring ring_of(const Params &p, int per_sm) {
   Ring g{};
-  const int dts[3] = {p.y_dt, p.r_dt, p.g_dt};
-  g.streams = POST ? p.gate ? 3 : 2 : 1;
-  for (int i = 0; i < g.streams; ++i) {
+  const int dts[2] = {p.y_dt, p.r_dt};
+  for (int i = 0; i < (POST ? 2 : 1); ++i) {
     g.at[i] = g.stage_bytes;
     g.row_bytes[i] = p.cols * bytes_of(dts[i]);
     g.stage_bytes += g.row_bytes[i];
@@ -422,10 +610,20 @@ int plan_ring(Params &p) {
   }
   p.w_dt = p.g_dt = p.nw_dt = one < 0 ? p.y_dt : one;
   p.tpr = (p.cols + 511) / 512 * 32;
-  if (p.cols < 1024 || p.tpr > kStreamThreads) return 0;
-  for (int per_sm = std::min(16, 1024 / p.tpr); per_sm >= 1; per_sm = per_sm > 1 ? per_sm / 2 : 0)
+  if (p.cols < 768 || p.tpr > kStreamThreads) return 0;
+  for (int per_sm = std::min(16, 1024 / p.tpr); per_sm >= 1; --per_sm)
     if (ring_of<POST>(p, per_sm).stages >= (per_sm > 1 ? 3 : 2)) return per_sm;
   return 0;
+}
+
+// As many CTAs as run at once: those that had to wait would start their rows when the others are done.
+template <typename Kern>
+int launch_persistent(Kern kern, int per_sm, const Params &p, const Ring &g, cudaStream_t s, const char *what) {
+  int fit = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, p.tpr, g.total);
+  if (e != cudaSuccess || fit < 1) return fail(MQ_ECUDA, "%s: occupancy: %s", what, cudaGetErrorString(e));
+  const int64_t grid = std::min<int64_t>(p.rows, 148 * std::min(per_sm, fit));
+  return launch_overlapped(kern, dim3(static_cast<unsigned>(grid)), dim3(p.tpr), g.total, s, what, p, g);
 }
 
 template <typename TY, typename TR, typename TW, int E, bool POST, bool EARLY>
@@ -434,8 +632,7 @@ int launch_ring_e(const Params &p, int per_sm, cudaStream_t s, const char *what)
   auto kern = row_stream_kernel<TY, TR, TW, E, POST, EARLY>;
   static size_t configured[64] = {};
   if (int rc = ensure_smem(kern, g.total, configured, what)) return rc;
-  const int64_t grid = std::min<int64_t>(p.rows, 148 * per_sm);
-  return launch_overlapped(kern, dim3(static_cast<unsigned>(grid)), dim3(p.tpr), g.total, s, what, p, g);
+  return launch_persistent(kern, per_sm, p, g, s, what);
 }
 
 template <typename TY, bool POST, bool EARLY>
@@ -462,13 +659,58 @@ int launch_ring(const Params &p, int per_sm, cudaStream_t s, const char *what) {
   return launch_ring_y<__nv_bfloat16, POST, EARLY>(p, per_sm, s, what);
 }
 
+// The ring of the kernel for unaligned rows: the same without the weights.
+template <typename TY, typename TR, int TPR, bool POST, bool EARLY>
+int launch_ring1_e(const Params &p, const Ring &g, int per_sm, cudaStream_t s, const char *what) {
+  auto kern = row_stream1_kernel<TY, TR, TPR, POST, EARLY>;
+  static size_t configured[64] = {};
+  if (int rc = ensure_smem(kern, g.total, configured, what)) return rc;
+  return launch_persistent(kern, per_sm, p, g, s, what);
+}
+
+template <typename TY, typename TR, bool POST, bool EARLY>
+int launch_ring1_t(const Params &p, const Ring &g, int per_sm, cudaStream_t s, const char *what) {
+  if (p.tpr == 64) return launch_ring1_e<TY, TR, 64, POST, EARLY>(p, g, per_sm, s, what);
+  if (p.tpr == 128) return launch_ring1_e<TY, TR, 128, POST, EARLY>(p, g, per_sm, s, what);
+  if (p.tpr == 256) return launch_ring1_e<TY, TR, 256, POST, EARLY>(p, g, per_sm, s, what);
+  return launch_ring1_e<TY, TR, 512, POST, EARLY>(p, g, per_sm, s, what);
+}
+
+template <typename TY, bool POST, bool EARLY>
+int launch_ring1_y(const Params &p, const Ring &g, int per_sm, cudaStream_t s, const char *what) {
+  if constexpr (POST && !std::is_same<TY, float>::value)
+    if (p.r_dt == MQ_F32) return launch_ring1_t<TY, float, POST, EARLY>(p, g, per_sm, s, what);
+  return launch_ring1_t<TY, TY, POST, EARLY>(p, g, per_sm, s, what);
+}
+
+template <bool POST, bool EARLY>
+int launch_ring1(Params p, cudaStream_t s, const char *what) {
+  p.tpr = 64;
+  while (16 * p.tpr < p.cols) p.tpr *= 2;
+  const int per_sm = std::min(16, 1024 / p.tpr);
+  Ring g{};
+  const int dts[2] = {p.y_dt, p.r_dt};
+  for (int i = 0; i < (POST ? 2 : 1); ++i) {
+    g.at[i] = g.stage_bytes;
+    g.stage_bytes += 16 + (p.cols * bytes_of(dts[i]) + 15) / 16 * 16;
+  }
+  g.stages = std::max(2, std::min(kRingMax, (200 * 1024 / per_sm - 1536) / g.stage_bytes));
+  g.total = g.stages * g.stage_bytes;
+  if (p.y_dt == MQ_F32) return launch_ring1_y<float, POST, EARLY>(p, g, per_sm, s, what);
+  if (p.y_dt == MQ_F16) return launch_ring1_y<__half, POST, EARLY>(p, g, per_sm, s, what);
+  return launch_ring1_y<__nv_bfloat16, POST, EARLY>(p, g, per_sm, s, what);
+}
+
 template <bool POST, bool EARLY>
 int launch(Params p, bool vec, cudaStream_t s, const char *what) {
   MQ_REQUIRE(p.cols <= kMaxCols, MQ_EUNSUPPORTED, "%s: cols is above %d", what, kMaxCols);
   if (vec && p.rows >= 4 * 148)
     if (const int per_sm = plan_ring<POST>(p)) return launch_ring<POST, EARLY>(p, per_sm, s, what);
-  // As many threads of a row as there are vectors (8 values each), for the least latency.
-  const int per = vec ? 8 : 4;
+  if (!vec && p.rows >= 4 * 148 && p.cols >= 256 && p.cols <= 16 * kStreamThreads && (!POST || p.r_dt == p.y_dt || p.r_dt == MQ_F32))
+    return launch_ring1<POST, EARLY>(p, s, what);
+  // Few rows: a thread of a row for each 8 values, for the least latency. Many: 16, so that what a reduction costs
+  // each thread (as much as some 20 values) is spread over more of them. Without alignment 4 and 16 single values.
+  const int per = p.rows >= 4 * 148 ? 16 : vec ? 8 : 4;
   p.tpr = std::min(kMaxThreads, (p.cols + 32 * per - 1) / (32 * per) * 32);
   const int rows_per_cta = p.tpr == 32 ? 4 : 1, each = (p.cols + p.tpr - 1) / p.tpr;
   if (vec) {

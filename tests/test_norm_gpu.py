@@ -98,6 +98,62 @@ def test_post_norm(cuda, rows, cols, gates, normed, y_t, r_t, h_t):
     assert (np.abs(got - h_ref) <= step * (0.5 + 1e-4) + h_err + 128 * 60 * U * step).all()
 
 
+MANY = [(601, 256, 0), (1500, 264, 0), (700, 777, 0), (700, 1000, 0), (3001, 1001, 0), (640, 2048, 8), (1200, 4096, 0),
+        (600, 4096, 1), (640, 5003, 0), (600, 8191, 3), (620, 8192, 0), (600, 8200, 0)]
+
+
+@pytest.mark.parametrize("rows,cols,pad", MANY)
+@pytest.mark.parametrize("y_t,r_t,w_t,h_t", [(torch.bfloat16, torch.bfloat16, torch.bfloat16, torch.bfloat16),
+                                             (torch.float16, torch.float32, torch.float32, torch.float16),
+                                             (torch.float32, torch.float32, torch.float32, torch.bfloat16),
+                                             (torch.bfloat16, torch.float16, torch.float32, torch.float32)])
+def test_many_rows(cuda, rows, cols, pad, y_t, r_t, w_t, h_t):
+    """Row counts at which the rows stream through persistent CTAs, aligned and not, all outputs."""
+    rng = np.random.default_rng(rows + cols)
+    y, res = rand(rng, rows, cols, y_t, cuda, pad), rand(rng, rows, cols, r_t, cuda, pad)
+    w, nw = rand(rng, 1, cols, w_t, cuda)[0].contiguous(), rand(rng, 1, cols, w_t, cuda)[0].contiguous()
+    h_ref = serving.rms_norm(np64(y), np64(nw), 1e-6)
+    within(mq.pre_norm(y, nw, 1e-6, dtype=h_t), h_ref, 60 * U * np.abs(h_ref), h_t)
+    v = y.float().cpu().numpy() * nw.float().cpu().numpy()
+    q, s = mq.pre_norm_s8(y, nw, 1e-6)
+    np.testing.assert_array_equal(q.cpu().numpy(), serving.quantize_s8(v)[0])
+    q, s = mq.quantize_s8(y)
+    rq, rs = serving.quantize_s8(y.float().cpu().numpy())
+    np.testing.assert_array_equal(q.cpu().numpy(), rq)
+    np.testing.assert_array_equal(s.cpu().numpy(), rs)
+    groups = next(g for g in (7, 5, 3, 2, 1) if rows % g == 0)
+    gate = rand(rng, groups, cols, w_t, cuda)
+    ref, added = serving.post_norm(np64(y), np64(w), np64(res), np64(gate), 0.3, 1e-6)
+    err = 60 * U * added + U * np.abs(ref)
+    h_ref = serving.rms_norm(ref, np64(nw), 1e-6)
+    inv = 1 / np.sqrt((ref * ref).mean(-1, keepdims=True) + 1e-6)
+    share = np.sqrt((err * err).sum(-1, keepdims=True) / (ref * ref).sum(-1, keepdims=True))
+    h_err = np.abs(np64(nw)) * inv * err + np.abs(h_ref) * (60 * U + share)
+    out, h = mq.post_norm(y, w, res, nw, gate=gate, scale=0.3, eps=1e-6, dtype=h_t)
+    within(out, ref, err, r_t)
+    within(h, h_ref, h_err, h_t)
+    out8, q, s = mq.post_norm_s8(y, w, res, nw, gate=gate, scale=0.3, eps=1e-6)
+    assert torch.equal(out8, out)
+    got, step = np64(q) * np64(s)[:, None], np64(s)[:, None]
+    assert (np.abs(got - h_ref) <= step * (0.5 + 1e-4) + h_err + 128 * 60 * U * step).all()
+    same, _ = mq.post_norm(y, w, res, gate=gate, scale=0.3, eps=1e-6, out=res)  # in place, nothing behind it
+    assert same is res and torch.equal(res, out)
+    assert mq.device_status() == 0
+
+
+def test_many_rows_propagate_nan_in_its_row_alone(cuda):
+    for cols in (1001, 4096):
+        x, w = torch.randn(900, cols, device=cuda), torch.ones(cols, device=cuda)
+        x[700, cols - 1] = float("nan")
+        x[3, 0] = float("inf")
+        bad = torch.zeros(900, dtype=torch.bool, device=cuda)
+        bad[[3, 700]] = True
+        q, s = mq.pre_norm_s8(x, w)
+        assert s[bad].isnan().all() and s[~bad].isfinite().all() and (q[bad] == 0).all()
+        h = mq.pre_norm(x, w)
+        assert h[700].isnan().all() and h[~bad].isfinite().all()
+
+
 def test_post_norm_gate_of_one_row_is_a_vector(cuda):
     y, r, w = torch.randn(4, 64, device=cuda), torch.randn(4, 64, device=cuda), torch.rand(64, device=cuda)
     g = torch.randn(64, device=cuda)
