@@ -6,13 +6,14 @@ import ctypes
 import torch
 
 from ._lib import MQError, lib
-from .int8 import _rows
-from .kernels import _need, _p, _stream
+from .int8 import _F32, _flat, _rows
+from .kernels import _need, _stream
 from .pack import _DT
 
 __all__ = ["beam_select", "beam_reorder"]
 
-_FLAGS = (torch.uint8, torch.bool)
+_FLAGS = frozenset((torch.uint8, torch.bool))
+_I32 = frozenset((torch.int32,))
 
 
 def beam_select(logits, scores, finished=None, eos=-1, next_scores=None, tokens=None, parents=None, next_finished=None,
@@ -26,28 +27,30 @@ def beam_select(logits, scores, finished=None, eos=-1, next_scores=None, tokens=
     if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
         raise MQError(-1, "scores: expected a [batch, beams] tensor")
     batch, beams = scores.shape
-    _need(scores, "scores", (torch.float32,))
-    rows, vocab, ld = _rows(logits, "logits", _DT, None, batch * beams)
-    if finished is not None:
-        _need(finished, "finished", _FLAGS, rows)
-    shape, dev = (batch, beams), logits.device
-    next_scores = torch.empty(shape, dtype=torch.float32, device=dev) if next_scores is None else next_scores
-    tokens = torch.empty(shape, dtype=torch.int32, device=dev) if tokens is None else tokens
-    parents = torch.empty(shape, dtype=torch.int32, device=dev) if parents is None else parents
-    next_finished = torch.empty(shape, dtype=torch.uint8, device=dev) if next_finished is None else next_finished
-    _need(next_scores, "next_scores", (torch.float32,), rows)
-    _need(tokens, "tokens", (torch.int32,), rows)
-    _need(parents, "parents", (torch.int32,), rows)
-    _need(next_finished, "next_finished", _FLAGS, rows)
-    nbytes = lib.mq_beam_workspace_size(batch, beams, vocab)
+    n = batch * beams
+    _, vocab, ld = _rows(logits, "logits", _DT, None, n)
+    if next_scores is None:
+        next_scores = torch.empty_like(scores)
+    if tokens is None:
+        tokens = torch.empty(batch, beams, dtype=torch.int32, device=logits.device)
+    if parents is None:
+        parents = torch.empty(batch, beams, dtype=torch.int32, device=logits.device)
+    if next_finished is None:
+        next_finished = torch.empty(batch, beams, dtype=torch.uint8, device=logits.device)
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        workspace = torch.empty(max(lib.mq_beam_workspace_size(batch, beams, vocab), 16), dtype=torch.uint8,
+                                device=logits.device)
     else:
         _need(workspace, "workspace", (torch.uint8,))
-    lib.call("mq_beam_select", _p(logits), _DT[logits.dtype], ld, _p(scores), None if finished is None else _p(finished), eos,
-             _p(next_scores), _p(tokens), _p(parents), _p(next_finished), batch, beams, vocab, _p(workspace),
-             workspace.numel(), _stream())
+    lib.call("mq_beam_select", logits.data_ptr(), _DT[logits.dtype], ld, _flat(scores, "scores", _F32, n),
+             None if finished is None else _flat(finished, "finished", _FLAGS, n), eos,
+             _flat(next_scores, "next_scores", _F32, n), _flat(tokens, "tokens", _I32, n), _flat(parents, "parents", _I32, n),
+             _flat(next_finished, "next_finished", _FLAGS, n), batch, beams, vocab, workspace.data_ptr(), workspace.numel(),
+             _stream())
     return next_scores, tokens, parents, next_finished
+
+
+_Three = ctypes.c_int64 * 3
 
 
 def _layout(t):
@@ -79,22 +82,20 @@ def beam_reorder(states, parents):
     each = [states] if isinstance(states, torch.Tensor) else list(states)
     if not isinstance(parents, torch.Tensor) or parents.dim() != 2:
         raise MQError(-1, "parents: expected a [batch, beams] tensor")
-    _need(parents, "parents", (torch.int32,))
     batch, beams = parents.shape
+    parents_p = _flat(parents, "parents", _I32, batch * beams)
     groups = {}
     for t in each:
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise MQError(-1, "states: expected CUDA tensors (there is no CPU path)")
-        if t.dim() < 2 or t.shape[0] != batch * beams:
-            raise MQError(-1, f"states: shape {tuple(t.shape)} is not [{batch * beams}, ..]")
-        if t.numel():
-            groups.setdefault((t.shape, t.stride(), t.dtype), []).append(t)
-    if batch == 0 or beams == 0:
-        return states
-    stream = _stream()
-    for same in groups.values():  # one launch for all states of one layout
+        groups.setdefault((t.shape, t.stride(), t.dtype), []).append(t)
+    for (shape, _, _), same in groups.items():  # one launch for all states of one layout
+        if len(shape) < 2 or shape[0] != batch * beams:
+            raise MQError(-1, f"states: shape {tuple(shape)} is not [{batch * beams}, ..]")
+        if 0 in shape:
+            continue
         row, outer, strides, inner = _layout(same[0])
         n = len(same)
-        lib.call("mq_beam_reorder", (ctypes.c_void_p * n)(*[t.data_ptr() for t in same]), n, _p(parents), batch, beams, row,
-                 (ctypes.c_int64 * 3)(*outer), (ctypes.c_int64 * 3)(*strides), inner, stream)
+        lib.call("mq_beam_reorder", (ctypes.c_void_p * n)(*[t.data_ptr() for t in same]), n, parents_p, batch, beams, row,
+                 _Three(*outer), _Three(*strides), inner, _stream())
     return states

@@ -7,7 +7,7 @@ number), with one fp32 scale per row; quantize_s8 makes both, of tokens and, onc
 import torch
 
 from ._lib import MQError, lib
-from .kernels import _need, _p, _stream
+from .kernels import _need, _stream
 from .pack import _DT
 
 __all__ = ["MQ_S8", "int8_rows", "quantize_s8", "gemm_w8a8", "gate_up_w8a8"]
@@ -31,13 +31,13 @@ def _rows(t, name, dtypes, cols=None, rows=None):
         if step != 1 and c > 1:
             raise MQError(-1, f"{name}: the last dimension must be contiguous")
         if r <= 1:
-            ld = max(c, 1)
+            ld = c or 1
     else:
         if not shape or not t.is_contiguous():
             raise MQError(-1, f"{name}: must be two-dimensional or contiguous")
         c = shape[-1]
         r = t.numel() // c if c else 0
-        ld = max(c, 1)
+        ld = c or 1
     if cols is not None and c != cols:
         raise MQError(-1, f"{name}: has rows of {c} elements, expected {cols}")
     if rows is not None and r != rows:
@@ -45,9 +45,21 @@ def _rows(t, name, dtypes, cols=None, rows=None):
     return r, c, ld
 
 
+def _flat(t, name, dtypes, numel):
+    """The data pointer of a contiguous CUDA tensor of numel elements."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or t.numel() != numel or \
+            not t.is_contiguous():
+        _need(t, name, tuple(dtypes), numel)
+    return t.data_ptr()
+
+
+_F32 = frozenset((torch.float32,))
+_S8 = frozenset((torch.int8,))
+
+
 def _rows8(t, name, cols=None, rows=None):
     """_rows of an int8 matrix; the stride of a single row is never used and is rounded up to 16."""
-    r, c, ld = _rows(t, name, (torch.int8,), cols, rows)
+    r, c, ld = _rows(t, name, _S8, cols, rows)
     return r, c, -(-ld // 16) * 16 if r <= 1 else ld
 
 
@@ -62,9 +74,9 @@ def quantize_s8(x, q=None, s=None):
     rows, cols, ldx = _rows(x, "x", _DT)
     q = int8_rows(rows, cols, x.device) if q is None else q
     s = torch.empty(rows, dtype=torch.float32, device=x.device) if s is None else s
-    ldq = _rows(q, "q", (torch.int8,), cols, rows)[2]
-    _need(s, "s", (torch.float32,), rows)
-    lib.call("mq_quantize_s8", _p(x), _DT[x.dtype], ldx, _p(q), ldq, _p(s), rows, cols, _stream())
+    ldq = _rows(q, "q", _S8, cols, rows)[2]
+    lib.call("mq_quantize_s8", x.data_ptr(), _DT[x.dtype], ldx, q.data_ptr(), ldq, _flat(s, "s", _F32, rows), rows, cols,
+             _stream())
     return q, s
 
 
@@ -73,17 +85,14 @@ def gemm_w8a8(xq, xs, wq, ws, y=None, bias=None, add=False, dtype=torch.float16)
     aligned), xs fp32 [m], ws fp32 [n], bias fp32 [n]; y fp32 / fp16 / bf16 [m, n] (made of `dtype` if None)."""
     m, k, ldx = _rows8(xq, "xq")
     n, _, ldw = _rows8(wq, "wq", k)
-    _need(xs, "xs", (torch.float32,), m)
-    _need(ws, "ws", (torch.float32,), n)
-    if bias is not None:
-        _need(bias, "bias", (torch.float32,), n)
     if y is None:
         if add:
             raise MQError(-1, "y: add needs the tensor to add into")
         y = torch.empty(m, n, dtype=dtype, device=xq.device)
     ldy = _rows(y, "y", _DT, n, m)[2]
-    lib.call("mq_gemm_w8a8", _p(xq), ldx, _p(xs), _p(wq), ldw, _p(ws), None if bias is None else _p(bias), _p(y),
-             _DT[y.dtype], ldy, m, n, k, int(bool(add)), _stream())
+    lib.call("mq_gemm_w8a8", xq.data_ptr(), ldx, _flat(xs, "xs", _F32, m), wq.data_ptr(), ldw, _flat(ws, "ws", _F32, n),
+             None if bias is None else _flat(bias, "bias", _F32, n), y.data_ptr(), _DT[y.dtype], ldy, m, n, k,
+             1 if add else 0, _stream())
     return y
 
 
@@ -94,9 +103,8 @@ def gate_up_w8a8(xq, xs, wq, ws, a=None, dtype=torch.float16):
     n, _, ldw = _rows8(wq, "wq", k)
     if n % 2:
         raise MQError(-1, f"wq: {n} rows are not gate and up rows")
-    _need(xs, "xs", (torch.float32,), m)
-    _need(ws, "ws", (torch.float32,), n)
     a = torch.empty(m, n // 2, dtype=dtype, device=xq.device) if a is None else a
     lda = _rows(a, "a", _DT, n // 2, m)[2]
-    lib.call("mq_gate_up_w8a8", _p(xq), ldx, _p(xs), _p(wq), ldw, _p(ws), _p(a), _DT[a.dtype], lda, m, n // 2, k, _stream())
+    lib.call("mq_gate_up_w8a8", xq.data_ptr(), ldx, _flat(xs, "xs", _F32, m), wq.data_ptr(), ldw, _flat(ws, "ws", _F32, n),
+             a.data_ptr(), _DT[a.dtype], lda, m, n // 2, k, _stream())
     return a
