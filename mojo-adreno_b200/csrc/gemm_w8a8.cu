@@ -424,31 +424,38 @@ namespace w8 {
 // Which kernel, and how many CTAs (pairs of CTAs) share a tile's k: the least of the times below, in us,
 // fitted to measurements on a B200 with weights from HBM. Streaming kernel: 0.2 us per 128 k and wave of tiles up
 // to about 150 tokens per tile (the issue of the MMAs), 0.33 at 256 (its operands' way into shared memory),
-// for gate|up 0.3 and 0.45 at 128; 2.2 us and 0.015 per token and plane outside the loop, 3 and 0.028 with the
-// parts of a split to join. Pairs: 0.285 us per 128 k and wave of 256 x 256 tiles, 5.2 us outside, 9.8 with
-// parts. Measured, streaming against pairs: 128x4096x4096 8.8 / 13.8, 431x2048x8192 14.2 / 17.0,
-// 512x4096x4096 16.9 / 15.2, 1024x4096x4096 18.0 / 16.5, gate|up 64x8192x2048 11.9 / 13.0, 400x8192x2048 20.5 / 17.7.
+// for gate|up 0.3 and 0.45 at 128, but at least 0.0215 us per token to write a tile; 2.2 us and 0.015 per token and
+// plane outside the loop, 3 and 0.028 with the parts of a split to join. Pairs: 0.285 us per 128 k and wave of 256 x
+// 256 tiles, at least 3.5 us to write one (fp32 5), 5.5 where y's rows are not 16-byte aligned (fp32 8.5); 5.2 us
+// outside, 9.8 with parts to join and 12 more to write those to such rows. Measured, streaming against pairs:
+// 128x4096x4096 8.9 / 13.8, 431x2048x8192 14.5 / 17.0, 512x4096x4096 17.3 / 15.3, 1024x4096x4096 18.8 / 16.5,
+// 1609x21624x411 43.8 / 32.5, 459x2110x6087 (unaligned rows) 17.8 / 24.7, gate|up 64x8192x2048 12.0 / 13.1,
+// 400x8192x2048 20.5 / 17.7.
 struct Plan {
   bool pairs;
   int splits;
 };
-inline Plan plan_of(int planes, int m, int n, int k) {
+inline Plan plan_of(int planes, const Params &p) {
   Plan best{false, 1};
   float least = 1e30f;
   auto consider = [&](bool pairs, int splits, float us) {
     if (us < least) least = us, best = Plan{pairs, splits};
   };
-  const Shape sh = shape_of(planes, m, n);
+  const Shape sh = shape_of(planes, p.m, p.n);
   const float block = planes == 1 ? std::max(0.2f, 0.33f / 256 * sh.bn) : std::max(0.3f, 0.45f / 128 * sh.bn);
-  const int blocks = (k + kBK - 1) / kBK, stages = (blocks + sub_blocks(planes) - 1) / sub_blocks(planes);
-  consider(false, 1, 2.2f + 0.015f * planes * sh.bn + ((sh.tiles + 147) / 148) * blocks * block);
+  const int blocks = (p.k + kBK - 1) / kBK, stages = (blocks + sub_blocks(planes) - 1) / sub_blocks(planes);
+  consider(false, 1, 2.2f + 0.015f * planes * sh.bn + ((sh.tiles + 147) / 148) * std::max(blocks * block, 0.0215f * sh.bn));
   for (int z = 2; z <= std::min(kMaxSplits, stages); ++z)
     if (sh.tiles <= clusters_at_once(z))
       consider(false, z, 3.f + 0.028f * planes * sh.bn + (stages + z - 1) / z * sub_blocks(planes) * block);
-  const int tiles = ((m + kTileM - 1) / kTileM) * ((n + kTileB / planes - 1) / (kTileB / planes));
-  consider(true, 1, 5.2f + ((tiles + 73) / 74) * blocks * 0.285f);
+  const int es = p.y_dtype == MQ_F32 ? 4 : 2;
+  const bool rows_aligned = !p.add && aligned(p.y, 16) && p.ldy * es % 16 == 0;
+  const float write = rows_aligned ? (es == 2 ? 3.5f : 5.f) : (es == 2 ? 5.5f : 8.5f);
+  const int tiles = ((p.m + kTileM - 1) / kTileM) * ((p.n + kTileB / planes - 1) / (kTileB / planes));
+  consider(true, 1, 5.2f + ((tiles + 73) / 74 - 1) * std::max(blocks * 0.285f, write) + blocks * 0.285f + write - 3.5f);
   for (int z = 2; z <= std::min(kTileMaxSplits, blocks); ++z)
-    if (tiles <= clusters_at_once(2 * z)) consider(true, z, 9.8f + (blocks + z - 1) / z * 0.285f);
+    if (tiles <= clusters_at_once(2 * z))
+      consider(true, z, 9.8f + (blocks + z - 1) / z * 0.285f + (rows_aligned ? 0.f : 12.f));
   return best;
 }
 
@@ -457,7 +464,7 @@ int run(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, const Para
         const char *what) {
   DeviceInfo dev;
   if (int rc = device_info(&dev)) return rc;
-  const Plan plan = plan_of(P, p.m, p.n, p.k);
+  const Plan plan = plan_of(P, p);
   if (plan.pairs) return launch_tile<P>(xq, ldx, wq, ldw, p, stream, dev, what, plan.splits);
   return launch<P>(xq, ldx, wq, ldw, p, stream, dev, what, plan.splits);
 }

@@ -282,19 +282,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               using T = decltype(type);
               const uint8_t *const staged = mine + buf * kStageOutBytes;
               const int cols = p.n - x;
-              T *y = static_cast<T *>(p.y) + row0 * p.ldy + x;
-#pragma unroll 4
-              for (int r = 0; r < min(32, p.m - row0); ++r, y += p.ldy) {
+              T *y = static_cast<T *>(p.y) + row0 * p.ldy + x + lane;
+              const int rows = min(32, p.m - row0);
+              // Eight rows are read before any is written: the compiler may not move the reads across the writes.
+#pragma unroll 1
+              for (int r0 = 0; r0 < rows; r0 += 8, y += 8 * p.ldy) {
                 if (f32) {
-                  float o = *reinterpret_cast<const float *>(staged + r * 128 + ((lane / 4) ^ (r & 7)) * 16 + lane % 4 * 4);
-                  if (lane < cols) y[lane] = from_float<T>(p.add ? o + static_cast<float>(y[lane]) : o);
-                } else {
+                  float o[8];
 #pragma unroll
-                  for (int e = 0; e < 64; e += 32) {
-                    const int at = e + lane;
-                    const T o = *reinterpret_cast<const T *>(staged + r * 128 + ((at / 8) ^ (r & 7)) * 16 + at % 8 * 2);
-                    if (at < cols) y[at] = o;
+                  for (int i = 0; i < 8; ++i)
+                    o[i] = *reinterpret_cast<const float *>(staged + (r0 + i) * 128 + ((lane / 4) ^ i) * 16 + lane % 4 * 4);
+                  if (p.add) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                      if (r0 + i < rows && lane < cols) o[i] += static_cast<float>(y[i * p.ldy]);
                   }
+#pragma unroll
+                  for (int i = 0; i < 8; ++i)
+                    if (r0 + i < rows && lane < cols) y[i * p.ldy] = from_float<T>(o[i]);
+                } else {
+                  T o[8][2];
+#pragma unroll
+                  for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                      const int at = 32 * h + lane;
+                      o[i][h] = *reinterpret_cast<const T *>(staged + (r0 + i) * 128 + ((at / 8) ^ i) * 16 + at % 8 * 2);
+                    }
+#pragma unroll
+                  for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                      if (r0 + i < rows && 32 * h + lane < cols) y[i * p.ldy + 32 * h] = o[i][h];
                 }
               }
             });
