@@ -27,7 +27,7 @@ constexpr int kVecs = 4;        // 16-byte vectors per thread and chunk
 constexpr int kScan = 128, kScanCtas = 8;  // threads of a scan CTA, CTAs per SM
 constexpr int kChunkBytes = kScan * kVecs * 16;
 constexpr int kFresh = 1280;    // pairs that may wait to be merged into the list: at least (kMaxBeams + 1) * 32
-constexpr int kStages = 2;      // chunks on their way into shared memory: 32 KB for each of four CTAs per SM
+constexpr int kStages = 2;      // chunks on their way into shared memory: 16 KB for each of the CTAs of an SM
 constexpr float kNegInf = -INFINITY, kLowest = -3.402823466e38f, kLog2e = 1.44269504088896340736f;
 
 // (Counted in fp32 chunks for every type, so that the workspace's size does not depend on it.)
@@ -41,7 +41,7 @@ __host__ __device__ constexpr int splits_for(int64_t rows, int beams, int64_t vo
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
-// What the CTAs leave for the merge: a base and the sum of 2^(v log2 e - base) each (NaN where a logit is NaN
+// What the CTAs leave for the merge: the largest logit and the sum relative to it each (NaN where a logit is NaN
 // or +infinity), then kp keys each, best first, 0 = none.
 struct Parts {
   float2 *sums;    // [rows * splits]
@@ -72,6 +72,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// A sum s stands for s * 2^(unit(m)) with m the largest logit it has seen. unit(m) is the fp32 product m log2 e, so that
+// a term is one FMA, 2^(v log2 e - unit(m)), and no rounding of the unit enters the result; where that product
+// could overflow (a mask of the type's lowest value) terms are 2^((v - m) log2 e) and s stands for s * e^m.
+__device__ __forceinline__ bool moderate(float m) { return fabsf(m) < 1e37f; }
+// What takes a sum from m to another m that is not smaller.
+__device__ __forceinline__ float rescale(float from, float to) {
+  return exp2_fast(moderate(from) && moderate(to) ? from * kLog2e - to * kLog2e : (from - to) * kLog2e);
 }
 
 template <typename T>
@@ -138,7 +147,7 @@ __global__ void __launch_bounds__(kScan, kScanCtas) beam_scan_kernel(const ScanP
   if (tid == 0)
     for (int c = c_begin; c < min(c_end, c_begin + kStages); ++c) fetch(c);
 
-  float m = kLowest, base = kLowest, s = 0.f;  // the largest logit, log2(e) times it, sum of 2^(v log2 e - base)
+  float m = kLowest, s = 0.f;  // the largest logit, the sum of exponentials relative to it
   int cur = 0, have = 0;
   int bound = 0;     // at least as many pairs as wait in `fresh`; the same in every thread
   uint64_t bar = 0;  // a pair is offered only above this key
@@ -192,15 +201,18 @@ __global__ void __launch_bounds__(kScan, kScanCtas) beam_scan_kernel(const ScanP
 #pragma unroll
     for (int i = 1; i < kElems; ++i) big = fmaxf(big, v[i]);
     if (big > m) {
+      s *= rescale(m, big);
       m = big;
-      const float to = m * kLog2e;
-      s *= exp2_fast(base - to);
-      base = to;
     }
-    // 2^(v log2 e - base): one rounding of the exponent, none from base, which the sum is relative to. A NaN or
-    // +infinity (base infinite: inf - inf) makes s NaN.
+    // A NaN or +infinity (m infinite: inf - inf) makes s NaN.
+    if (moderate(m)) {
+      const float unit = m * kLog2e;
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) s += exp2_fast(fmaf(v[i], kLog2e, -base));
+      for (int i = 0; i < kElems; ++i) s += exp2_fast(fmaf(v[i], kLog2e, -unit));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) s += exp2_fast((v[i] - m) * kLog2e);
+    }
     // The best pairs. A logit below the bar's is never offered, and after a few chunks hardly any thread has one
     // that is not: the keys are formed only there.
     auto key_at = [&](int i) -> uint64_t {
@@ -266,14 +278,14 @@ __global__ void __launch_bounds__(kScan, kScanCtas) beam_scan_kernel(const ScanP
   merge();
 
   // Join the threads' sums, in one fixed order.
-  float top = base;
+  float top = m;
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (tid % 32 == 0) red[0][tid / 32] = top;
   __syncthreads();
   top = red[0][0];
   for (int w = 1; w < kScan / 32; ++w) top = fmaxf(top, red[0][w]);
-  s *= exp2_fast(base - top);
+  s *= rescale(m, top);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (tid % 32 == 0) red[1][tid / 32] = s;
@@ -393,12 +405,13 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
     for (int j = lane; j < p.splits; j += 32) top = fmaxf(top, sums[i * p.splits + j].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    for (int j = lane; j < p.splits; j += 32) total += sums[i * p.splits + j].y * exp2_fast(sums[i * p.splits + j].x - top);
+    for (int j = lane; j < p.splits; j += 32) total += sums[i * p.splits + j].y * rescale(sums[i * p.splits + j].x, top);
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) {
       if (total != total) raise_status(kStatusBeamNonFinite);
-      total = static_cast<float>((top + log2(static_cast<double>(total))) * 0.69314718055994530942);
+      total = static_cast<float>(moderate(top) ? (top * kLog2e + log2(static_cast<double>(total))) / static_cast<double>(kLog2e)
+                                               : top + log(static_cast<double>(total)));
       lse[i] = total;
       if (!(fabsf(total) < INFINITY)) kind[i] = kDead;
     }

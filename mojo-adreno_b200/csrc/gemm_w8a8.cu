@@ -94,12 +94,6 @@ __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-// y[at] (+)= v in y's type. `put` is instantiated per type so that a loop over it holds no branch on the type.
-template <typename T>
-__device__ __forceinline__ void put(void *y, int64_t at, float v, int add) {
-  T *p = static_cast<T *>(y) + at;
-  *p = from_float<T>(add ? static_cast<float>(*p) + v : v);
-}
 // silu(g) * u with the fast exponential and quotient: their errors, (2 + 1.2 |g|) and 2 ulp, are below what
 // one rounding of g does to silu for large |g|; the accurate forms cost the epilogue several times as much.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }

@@ -4,7 +4,8 @@
 //    N = 256, K = 32 per instruction) works on 256 tokens x 256 weight rows: each CTA loads 128 rows of
 //    each, its TMEM holds its 128 tokens x 256 int32 sums, and the instruction reads both CTAs' shared memory. Per
 //    stage of 128 k a CTA fetches 32 KB for 512 cycles of MMA, where one CTA alone on 128 x 256 would
-//    need 48 KB: the 1-CTA kernel ran at half the MMA's rate (1015 us for gate|up 8192x12288x4096).
+//    need 48 KB (gate|up 8192x12288x4096: 435 us against the streaming kernel's 570 with constant operands;
+//    with random ones power caps the clock and it takes 526-600 us, 2.7-3.1 POP/s).
 //  * gate|up: the even CTA loads 128 gate rows, the odd one the matching 128 up rows, so columns j and
 //    128 + j of the tile belong together and one thread holds both.
 //  * Persistent pairs over the tiles in bands of 8 token tiles (a band's tokens and the weights it walks
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     }
     // Leave no copy in flight: the MMAs that read the last copy into each slot have finished.
-    if (lane == 0 && ok)
+    if (lane == 0)
       for (int64_t i = issued > S ? issued - S : 0; i < issued; ++i) mbar_wait(&empty[i % S], (i / S) & 1);
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {

@@ -36,13 +36,14 @@ def grid(rng, batch, beams, vocab, steps=64):
     return z.astype(np.float32), (-20 - np.sort(rng.permutation(batch * beams * 4)[:batch * beams].reshape(batch, beams), -1) / 7.0).astype(np.float32)
 
 
-def check(got, cand, beams):
+def check(got, cand, beams, size=None):
+    """size: the largest |score| + |logit| + |lse| where it is above the 3 |score| of the other tests."""
     scores, tokens, parents, _ = got
     ref, rp, rt = serving.beam_select(cand)
     fin = np.isfinite(ref)
     np.testing.assert_array_equal(fin, np.isfinite(scores))
     # |logit|, |lse| <= 16 here (steps of 1/8 up to 8, vocabularies below e^8 times that)
-    np.testing.assert_allclose(scores[fin], ref[fin], atol=0, rtol=8 * U * (1 + 40 / 20))
+    np.testing.assert_allclose(scores[fin], ref[fin], atol=8 * U * size if size else 0, rtol=8 * U * (1 + 40 / 20))
     flat = cand.reshape(cand.shape[0], -1)
     for b in range(flat.shape[0]):  # the precondition: the best candidates of different beams are apart
         top = np.argsort(-flat[b], kind="stable")[:beams + 1]
@@ -89,6 +90,25 @@ def test_select_orders_and_masks(cuda, kind, vocab):
     scores[1, 1:] = -INF  # a first step: one beam in use
     got, cand = select(z, scores, cuda)
     check(got, cand, beams)
+    assert mq.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [3, 5000, 33000])
+def test_select_masks_of_the_lowest_value(cuda, dtype, vocab):
+    """Masks of the type's lowest finite value: they count as what they are, in a row that has nothing else too."""
+    rng = np.random.default_rng(vocab)
+    low = float(torch.finfo(dtype).min)
+    z = np.full((4, vocab), low)
+    z[0, rng.integers(0, vocab, 7)] = 1.5
+    z[1, : vocab // 2] = rng.integers(-16, 16, vocab // 2) / 8.0
+    z[2, vocab - 1] = low / 2  # (rows 2 and 3: nothing of a usual size)
+    for b, scores in enumerate(([-1, -2.37], [-3, -5.71], [-15.71, -3])):  # the third: row 3, all masked, is the best
+        rows = z[2 * min(b, 1):][:2].astype(np.float32)
+        scores = np.array([scores], np.float32)
+        got, _ = select(rows, scores, cuda, dtype=dtype)
+        # fp16's lowest value leaves lse some last bits; the others' swallows everything beside it
+        check(got, serving.beam_scores(rows, scores, None, -1), 2, 3 * abs(low) if b and dtype == torch.float16 else None)
     assert mq.device_status() == 0
 
 
