@@ -11,7 +11,11 @@
 // score grows with the logit, so no other token can be among the `beams` best -- except where rounding
 // gives unequal logits equal scores; the pair beyond the `beams` best shows whether that can matter.
 // beam_merge_kernel, one CTA per request, joins the sums, scores the kept pairs and picks the best.
-// Bound by the bytes of the logits when there are many, by latency for one request.
+//
+// Many rows: bound by the scan's instructions (14 per logit, 0.53 issued per cycle) before the bytes: 64x8x128256
+// 57 us in fp32 (4.6 TB/s), 58 in fp16; of that the merge is 5. One request (1x4x151669): 13 us, all
+// latency: 5 for a chunk, 5.5 for the merge, the launches. The states' reordering moves 6.6 TB/s (64x8 states of
+// 2 x 8 x 1001 x 64 fp16, five beams of eight moving: 159 us, the copy bandwidth).
 #include <algorithm>
 #include <cmath>
 
