@@ -14,7 +14,7 @@
 //  * Few tiles: a cluster of up to 8 CTAs shares a tile's k, each with its part of the sums, joined in
 //    distributed shared memory in int32: exact, so the result does not depend on the split.
 // Decode is bound by the weights' bytes once every SM has a tile, below that by latency; B200: head 128256x2048
-// for one token 43-45 us (6.1 TB/s, 0.93 of the copy bandwidth), 2048x2048 4.1 us, gate|up 64x8192x2048
+// for one token 42-44 us (6.2 TB/s, 0.96 of the copy bandwidth), 2048x2048 4.1 us, gate|up 64x8192x2048
 // 11.6 us (64 CTAs: 3.0 TB/s), 431x2048x8192 13.9 us (the join of 224 x 128 parts takes a third of it:
 // distributed shared memory moves 32 GB/s per SM, by stores as by bulk copies).
 // Many tokens go to pairs of CTAs (gemm_w8a8_tile.cu).
@@ -41,9 +41,11 @@ __host__ __device__ constexpr int clusters_at_once(int size) {
   return size == 1 ? 148 : size == 2 ? 74 : size == 3 ? 45 : size == 4 ? 33 : size == 5 ? 26 : size == 6 ? 22 : 15;
 }
 constexpr int64_t kMaxK = 131071;  // 128 * 128 * k stays below 2^31
-// 128-k blocks per stage: eight MMAs for each wait and commit of the issuing thread, which cost it about 0.17 us
-// together (four 128 x 16 MMAs take 0.1 us): 16x2048x8192 on 16 CTAs 21.8 -> 16.2 us.
-__host__ __device__ constexpr int sub_blocks(int planes) { return planes == 1 ? 2 : 1; }
+// 128-k blocks per stage: the issuing thread's wait and commit cost about 0.17 us together, four 128 x 16 MMAs 0.1 us,
+// so a stage has eight MMAs at least (16x2048x8192 on 16 CTAs 21.8 -> 15.5 us), and sixteen where that leaves the
+// ring slots small enough, up to 32 tokens (12.9 us; head for one token 43.7 -> 41.8, gate|up 1x8192x2048 10.1 -> 8.9;
+// with 64 tokens the fewer slots cost more: gate|up 64x12288x4096 20.8 -> 21.8).
+__host__ __device__ constexpr int sub_blocks(int planes, int bn) { return (planes == 1 ? 2 : 1) * (bn <= 32 ? 2 : 1); }
 
 struct Params {
   const float *xs, *ws, *bias;
@@ -105,10 +107,9 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bf
 // one rounding of g does to silu for large |g|; the accurate forms cost the epilogue several times as much.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
-template <int P>  // weight planes of a tile: 1, or 2 (gate and up)
+template <int P, int SUB>  // weight planes of a tile: 1, or 2 (gate and up); 128-k blocks per stage
 __global__ void __launch_bounds__(kThreads, 1)
     w8a8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Params p) {
-  constexpr int SUB = sub_blocks(P);
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2];
@@ -367,10 +368,9 @@ inline Shape shape_of(int planes, int m, int n) {
   return s;
 }
 
-template <int P>
-int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params p, cudaStream_t stream,
+template <int P, int SUB>
+int launch_sub(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params p, cudaStream_t stream,
            const DeviceInfo &dev, const char *what, int splits) {
-  constexpr int SUB = sub_blocks(P);
   const Shape sh = shape_of(P, p.m, p.n);
   p.tiles_m = sh.tiles_m, p.bn = sh.bn, p.tiles = sh.tiles, p.splits = splits;
   p.buf_cols = P * std::max(32, p.bn);  // the epilogue reads 32 columns at a time
@@ -391,10 +391,18 @@ int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Params 
   if (int rc = encode_tmap_2d_now(&xmap, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, p.m, ldx, kBK, p.bn,
                                   CU_TENSOR_MAP_SWIZZLE_128B, what))
     return rc;
-  auto kern = w8a8_kernel<P>;
+  auto kern = w8a8_kernel<P, SUB>;
   static size_t configured[64] = {};
   if (int rc = ensure_smem(kern, smem, configured, what)) return rc;
   return launch_overlapped_clusters(kern, dim3(grid), dim3(kThreads), p.splits, smem, stream, what, wmap, xmap, p);
+}
+
+template <int P>
+int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, const Params &p, cudaStream_t stream,
+           const DeviceInfo &dev, const char *what, int splits) {
+  constexpr int kFew = sub_blocks(P, 32), kMany = sub_blocks(P, 256);
+  if (shape_of(P, p.m, p.n).bn <= 32) return launch_sub<P, kFew>(xq, ldx, wq, ldw, p, stream, dev, what, splits);
+  return launch_sub<P, kMany>(xq, ldx, wq, ldw, p, stream, dev, what, splits);
 }
 
 int check(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw, const float *ws, const void *y,
@@ -424,7 +432,7 @@ namespace w8 {
 
 // Which kernel, and how many CTAs (pairs of CTAs) share a tile's k: the least of the times below, in us,
 // fitted to measurements on a B200 with weights from HBM. Streaming kernel: 0.2 us per 128 k and wave of tiles up
-// to about 150 tokens per tile (the issue of the MMAs), 0.33 at 256 (its operands' way into shared memory),
+// to about 150 tokens per tile (the issue of the MMAs; 0.8 of it up to 32), 0.33 at 256 (its operands' way into shared memory),
 // for gate|up 0.3 and 0.45 at 128, but at least 0.0215 us per token to write a tile; 2.2 us and 0.015 per token and
 // plane outside the loop, 3 and 0.028 with the parts of a split to join. Pairs: 0.285 us per 128 k and wave of 256 x
 // 256 tiles, at least 3.5 us to write one (fp32 5), 5.5 where y's rows are not 16-byte aligned (fp32 8.5); 5.2 us
@@ -443,12 +451,13 @@ inline Plan plan_of(int planes, const Params &p) {
     if (us < least) least = us, best = Plan{pairs, splits};
   };
   const Shape sh = shape_of(planes, p.m, p.n);
-  const float block = planes == 1 ? std::max(0.2f, 0.33f / 256 * sh.bn) : std::max(0.3f, 0.45f / 128 * sh.bn);
-  const int blocks = (p.k + kBK - 1) / kBK, stages = (blocks + sub_blocks(planes) - 1) / sub_blocks(planes);
+  const float few = sh.bn <= 32 ? 0.8f : 1.f;
+  const float block = planes == 1 ? std::max(0.2f * few, 0.33f / 256 * sh.bn) : std::max(0.3f * few, 0.45f / 128 * sh.bn);
+  const int sub = sub_blocks(planes, sh.bn), blocks = (p.k + kBK - 1) / kBK, stages = (blocks + sub - 1) / sub;
   consider(false, 1, 2.2f + 0.015f * planes * sh.bn + ((sh.tiles + 147) / 148) * std::max(blocks * block, 0.0215f * sh.bn));
   for (int z = 2; z <= std::min(kMaxSplits, stages); ++z)
     if (sh.tiles <= clusters_at_once(z))
-      consider(false, z, 3.f + 0.028f * planes * sh.bn + (stages + z - 1) / z * sub_blocks(planes) * block);
+      consider(false, z, 3.f + 0.028f * planes * sh.bn + (stages + z - 1) / z * sub * block);
   const int es = p.y_dtype == MQ_F32 ? 4 : 2;
   const bool rows_aligned = !p.add && aligned(p.y, 16) && p.ldy * es % 16 == 0;
   const float write = rows_aligned ? (es == 2 ? 3.5f : 5.f) : (es == 2 ? 5.5f : 8.5f);

@@ -84,18 +84,28 @@ def beam_reorder(states, parents):
         raise MQError(-1, "parents: expected a [batch, beams] tensor")
     batch, beams = parents.shape
     parents_p = _flat(parents, "parents", _I32, batch * beams)
-    groups = {}
-    for t in each:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    calls = []  # one launch for all states of one layout, none before all are checked
+    while each:
+        first = each[0]
+        if not isinstance(first, torch.Tensor):
             raise MQError(-1, "states: expected CUDA tensors (there is no CPU path)")
-        groups.setdefault((t.shape, t.stride(), t.dtype), []).append(t)
-    for (shape, _, _), same in groups.items():  # one launch for all states of one layout
+        shape, stride, dtype = first.shape, first.stride(), first.dtype
+        same, rest = [], []
+        for t in each:
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise MQError(-1, "states: expected CUDA tensors (there is no CPU path)")
+            if t.shape == shape and t.stride() == stride and t.dtype == dtype:
+                same.append(t.data_ptr())
+            else:
+                rest.append(t)
+        each = rest
         if len(shape) < 2 or shape[0] != batch * beams:
             raise MQError(-1, f"states: shape {tuple(shape)} is not [{batch * beams}, ..]")
-        if 0 in shape:
-            continue
-        row, outer, strides, inner = _layout(same[0])
+        if 0 not in shape:
+            calls.append((same, _layout(first)))
+    stream = _stream()
+    for same, (row, outer, strides, inner) in calls:
         n = len(same)
-        lib.call("mq_beam_reorder", (ctypes.c_void_p * n)(*[t.data_ptr() for t in same]), n, parents_p, batch, beams, row,
-                 _Three(*outer), _Three(*strides), inner, _stream())
+        lib.call("mq_beam_reorder", (ctypes.c_void_p * n)(*same), n, parents_p, batch, beams, row, _Three(*outer),
+                 _Three(*strides), inner, stream)
     return states

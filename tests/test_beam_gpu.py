@@ -259,6 +259,14 @@ def test_reorder_reports_a_bad_parent_and_keeps_its_beam(cuda):
     assert mq.device_status() == 16 and torch.equal(x, want)
 
 
+def test_reorder_refuses_before_it_moves_anything(cuda):
+    good, bad = torch.randn(8, 16, device=cuda), torch.randn(7, 16, device=cuda)
+    kept = good.clone()
+    with pytest.raises(mq.MQError, match="shape"):
+        mq.beam_reorder([good, bad], torch.tensor([[1, 0, 0, 0], [3, 3, 3, 3]], dtype=torch.int32, device=cuda))
+    assert torch.equal(good, kept)
+
+
 def test_reorder_refusals(cuda):
     x, p = torch.randn(8, 16, device=cuda), torch.zeros(2, 4, dtype=torch.int32, device=cuda)
     with pytest.raises(mq.MQError, match="shape"):
