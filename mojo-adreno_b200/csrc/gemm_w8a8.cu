@@ -14,8 +14,8 @@
 //  * Few tiles: a cluster of up to 8 CTAs shares a tile's k, each with its part of the sums, joined in
 //    distributed shared memory in int32: exact, so the result does not depend on the split.
 // Decode is bound by the weights' bytes once every SM has a tile, below that by latency; B200: head 128256x2048
-// for one token 42-44 us (6.2 TB/s, 0.96 of the copy bandwidth), 2048x2048 4.1 us, gate|up 64x8192x2048
-// 11.6 us (64 CTAs: 3.0 TB/s), 431x2048x8192 13.9 us (the join of 224 x 128 parts takes a third of it:
+// for one token 42-44 us (6.2 TB/s, 0.96 of the copy bandwidth), 2048x2048 4.2 us, gate|up 64x8192x2048
+// 11.9 us (64 CTAs: 2.9 TB/s), 431x2048x8192 14.0 us (the join of 224 x 128 parts takes a third of it:
 // distributed shared memory moves 32 GB/s per SM, by stores as by bulk copies).
 // Many tokens go to pairs of CTAs (gemm_w8a8_tile.cu).
 // Every wait on an mbarrier is bounded; on a time-out the kernel records a status code, stops issuing,
@@ -33,6 +33,7 @@ constexpr int kMaxStages = 12;
 constexpr int kEpiWarps = 4;    // one per TMEM lane quarter; eight measured slower (4.4 -> 5.8 us for 1x2048x2048)
 constexpr int kThreads = 64 + 32 * kEpiWarps;  // warp 0 TMA, warp 1 MMA + TMEM, then the epilogue
 constexpr int kWBytes = kRows * kBK;
+constexpr int kStaticShared = 4352;  // of w8a8_kernel (barriers, token scales), as ptxas reports it
 constexpr int kMaxSplits = 8;
 // Clusters of 1 .. 8 CTAs, one CTA per SM, that run at once on a B200 (cudaOccupancyMaxActiveClusters; the
 // SMs of a cluster share a GPC): a split whose clusters do not all fit takes twice as long (16 clusters
@@ -123,7 +124,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int st0 = nst_all * split / p.splits, nst = nst_all * (split + 1) / p.splits - st0;
   const int first = blockIdx.x / p.splits, step = gridDim.x / p.splits;
 
-  griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);
@@ -136,14 +136,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     abort_flag = 0;
     fence_mbar_init();
   }
+  // TMEM is taken when the kernels before this one have theirs back, and the kernels after it start when it has
+  // been taken: a grid that waits for another never holds TMEM that the other still needs.
+  griddep_wait();
   if (warp == 1) tmem_alloc(&tmem_slot, p.tmem_cols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  griddep_launch_dependents();
   const uint32_t tmem = tmem_slot;
   bool live = false;  // an epilogue warp of a split tile whose sums are in TMEM
   float sw = 0.f, su = 0.f, bias = 0.f;  // of an epilogue thread's weight row
-  griddep_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -374,8 +377,9 @@ int launch_sub(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Par
   const Shape sh = shape_of(P, p.m, p.n);
   p.tiles_m = sh.tiles_m, p.bn = sh.bn, p.tiles = sh.tiles, p.splits = splits;
   p.buf_cols = P * std::max(32, p.bn);  // the epilogue reads 32 columns at a time
-  p.tmem_cols = 64;
-  while (p.tmem_cols < 2 * p.buf_cols) p.tmem_cols *= 2;
+  const int used = splits > 1 ? p.buf_cols : 2 * p.buf_cols;  // (a split's CTA has one tile: no second buffer)
+  p.tmem_cols = 32;
+  while (p.tmem_cols < used) p.tmem_cols *= 2;
   // As many slots as shared memory holds, and no more than a CTA fills: the next kernel's CTAs can then
   // come in beside these.
   const int slot = SUB * (P * kWBytes + p.bn * kBK), nst = (p.k + SUB * kBK - 1) / (SUB * kBK);
@@ -383,7 +387,11 @@ int launch_sub(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, Par
   const int64_t fills = splits > 1 ? (nst + splits - 1) / splits : static_cast<int64_t>(nst) * ((p.tiles + grid - 1) / grid);
   p.stages = static_cast<int>(std::min<int64_t>({kMaxStages, fills, static_cast<int64_t>(dev.smem_optin - 1024 - 5120) / slot}));
   const size_t parts = splits > 1 ? static_cast<size_t>(splits) * P * ((p.bn / 4 + splits - 1) / splits) * kRows * 16 : 0;
-  const size_t smem = std::max(static_cast<size_t>(p.stages) * slot, parts) + 1024;
+  // At least the share of an SM's shared memory (228 KB) that the tile takes of its TMEM: CTAs that fit beside one
+  // another, of any stream, then never wait for TMEM, which those of two clusters could for good.
+  const size_t share = std::min<size_t>(static_cast<size_t>(p.tmem_cols) * (228 * 1024 / 512) - 1024 - kStaticShared,
+                                        dev.smem_optin - kStaticShared);
+  const size_t smem = std::max(std::max(static_cast<size_t>(p.stages) * slot, parts) + 1024, share);
   CUtensorMap wmap, xmap;
   if (int rc = encode_tmap_2d_now(&wmap, wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.k, static_cast<uint64_t>(P) * p.n, ldw,
                                   kBK, kRows, CU_TENSOR_MAP_SWIZZLE_128B, what))

@@ -89,7 +89,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int kb0 = nkb_all * split / p.splits, nkb = nkb_all * (split + 1) / p.splits - kb0;
   const int first = blockIdx.x / (2 * p.splits), step = gridDim.x / (2 * p.splits);
 
-  griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);   // the even CTA's: both CTAs' copies complete on it
@@ -102,6 +101,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     abort_flag = 0;
     fence_mbar_init();
   }
+  griddep_wait();  // (before TMEM is taken, as in the streaming kernel)
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -110,9 +110,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   cluster_sync_all();  // the pair's barriers exist before anything completes on them
   tc_fence_after();
+  griddep_launch_dependents();
   const uint32_t tmem = tmem_slot;
   bool live = false;  // an epilogue warp of a split tile whose sums are in TMEM
-  griddep_wait();
 
   if (warp == 0) {
     if (lane == 0) {
