@@ -6,8 +6,8 @@ import ctypes
 import torch
 
 from ._lib import MQError, lib
-from .int8 import _F32, _flat, _rows
-from .kernels import _need, _stream
+from .int8 import _F32, _flat, _rows, _stream
+from .kernels import _need
 from .pack import _DT
 
 __all__ = ["beam_select", "beam_reorder"]

@@ -7,12 +7,21 @@ number), with one fp32 scale per row; quantize_s8 makes both, of tokens and, onc
 import torch
 
 from ._lib import MQError, lib
-from .kernels import _need, _stream
+from .kernels import _need, _raw_stream
+from .kernels import _stream as _any_stream
 from .pack import _DT
 
 __all__ = ["MQ_S8", "int8_rows", "quantize_s8", "gemm_w8a8", "gate_up_w8a8"]
 
 MQ_S8 = 3
+
+
+_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def _stream():
+    """The current device's current stream, behind a check of a CUDA tensor (so CUDA is initialised)."""
+    return _any_stream() if _device is None or _raw_stream is None else _raw_stream(_device())
 
 
 def _rows(t, name, dtypes, cols=None, rows=None):

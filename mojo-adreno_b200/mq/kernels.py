@@ -18,14 +18,13 @@ __all__ = ["MQ_F32", "MQ_F16", "MQError", "gemv_q4", "gemv_add_q4", "gate_up_q4"
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream():
     """The current device's current CUDA stream as a raw handle (building a torch Stream object costs
     about 3 us per call, as much as the launch itself)."""
     if _raw_stream is not None:
-        return _raw_stream(_device())
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 

@@ -5,8 +5,8 @@ run the norm alone).
 import torch
 
 from ._lib import MQError, lib
-from .int8 import MQ_S8, _F32, _S8, _flat, _rows, int8_rows
-from .kernels import MQ_F32, _stream
+from .int8 import MQ_S8, _F32, _S8, _flat, _rows, _stream, int8_rows
+from .kernels import MQ_F32
 from .pack import _DT
 
 __all__ = ["pre_norm", "pre_norm_s8", "post_norm", "post_norm_s8"]
