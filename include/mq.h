@@ -378,7 +378,7 @@ MQ_API int mq_pre_norm(const void *x, int x_dtype, int64_t ldx, const void *w, i
 
 /* out = residual + scale * gate * norm(y; w, eps), then h = mq_pre_norm(out; next_w, next_eps) from the
  * sum before it is rounded to out's type. w NULL: y itself in the place of its norm. gate NULL: 1; else row
- * r takes gate row r / rows_per_gate. h NULL: no norm follows. out has residual's type and may be the
+ * r takes gate row r / rows_per_gate. h NULL: no norm follows and next_w is not read. out has residual's type and may be the
  * residual's own buffer. */
 MQ_API int mq_post_norm(const void *y, int y_dtype, int64_t ldy, const void *w, int w_dtype, float eps,
                         const void *residual, int r_dtype, int64_t ldr, const void *gate, int gate_dtype, int64_t ldg,

@@ -831,13 +831,13 @@ extern "C" int mq_post_norm(const void *y, int y_dtype, int64_t ldy, const void 
   p.y = y, p.y_dt = y_dtype, p.ldy = ldy, p.w = w, p.w_dt = w_dtype, p.eps = eps;
   p.residual = residual, p.r_dt = r_dtype, p.ldr = ldr, p.out = out, p.ldo = ldo, p.scale = scale;
   p.gate = gate, p.g_dt = gate_dtype, p.ldg = ldg, p.rows_per_gate = rows_per_gate;
-  p.next_w = next_w, p.nw_dt = next_w_dtype, p.next_eps = next_eps;
+  if (h) p.next_w = next_w, p.nw_dt = next_w_dtype, p.next_eps = next_eps;  // (unchecked, and not read, without h)
   p.h = h, p.h_dt = h_dtype, p.ldh = ldh, p.hs = hs;
   p.rows = rows, p.cols = static_cast<int>(cols), p.inv_cols = 1.f / static_cast<float>(cols);
   using mq::norm::vec_ok;
   const bool vec = cols % 8 == 0 && vec_ok(y, y_dtype, ldy, rows) && vec_ok(residual, r_dtype, ldr, rows) &&
                    vec_ok(out, r_dtype, ldo, rows) && vec_ok(w, w_dtype, cols, 1) &&
-                   vec_ok(gate, gate_dtype, ldg, rows) && vec_ok(h ? next_w : nullptr, next_w_dtype, cols, 1) &&
+                   vec_ok(gate, gate_dtype, ldg, rows) && vec_ok(p.next_w, next_w_dtype, cols, 1) &&
                    vec_ok(h, h_dtype, ldh, rows);
   return mq::norm::launch<true, true>(p, vec, static_cast<cudaStream_t>(stream), what);
 }

@@ -141,6 +141,24 @@ def test_many_rows(cuda, rows, cols, pad, y_t, r_t, w_t, h_t):
     assert mq.device_status() == 0
 
 
+@pytest.mark.parametrize("rows,cols", [(5, 264), (640, 2048), (640, 1001)])
+def test_post_norm_without_h_has_no_use_for_next_w(cuda, rows, cols):
+    """The C entry with h NULL writes the same, a next_w given or not, whatever type is said of it."""
+    y, r = torch.randn(rows, cols, device=cuda).bfloat16(), torch.randn(rows, cols, device=cuda).bfloat16()
+    w, next_w = torch.rand(cols, device=cuda).bfloat16(), torch.full((cols,), float("nan"), device=cuda)
+
+    def call(next_w, next_dtype):
+        out = torch.empty_like(r)
+        mq.lib.call("mq_post_norm", y.data_ptr(), 2, cols, w.data_ptr(), 2, 1e-6, r.data_ptr(), 2, cols, None, 0, cols, 1,
+                    0.7, out.data_ptr(), cols, next_w, next_dtype, 1e-6, None, 0, cols, None, rows, cols,
+                    torch.cuda.current_stream().cuda_stream)
+        return out
+
+    want = call(None, 0)
+    assert torch.equal(call(next_w.data_ptr(), 0), want) and torch.equal(call(next_w.data_ptr(), 77), want)
+    assert torch.equal(mq.post_norm(y, w, r, scale=0.7)[0], want) and mq.device_status() == 0
+
+
 def test_many_rows_propagate_nan_in_its_row_alone(cuda):
     for cols in (1001, 4096):
         x, w = torch.randn(900, cols, device=cuda), torch.ones(cols, device=cuda)
