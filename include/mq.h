@@ -407,6 +407,7 @@ MQ_API int mq_beam_select(const void *logits, int dtype, int64_t ld, const float
  * tensors of one layout: row b * beams + i starts row_stride bytes after the last and holds outer[0] x
  * outer[1] x outer[2] pieces of inner_bytes, outer_stride[] bytes apart. Only beams that change their parent
  * are read and written. `states`, `outer` and `outer_stride` are host arrays, read before the call returns.
+ * States may lie between one another's pieces, but two that share a byte are refused (MQ_EINVAL).
  * A parent outside [0, beams) is reported (16) and its beam keeps its state. beams <= 32, batch <= 65535. */
 MQ_API int mq_beam_reorder(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
                            int64_t row_stride, const int64_t *outer, const int64_t *outer_stride, int64_t inner_bytes,

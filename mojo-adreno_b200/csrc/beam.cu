@@ -18,6 +18,8 @@
 // 2 x 8 x 1001 x 64 fp16, five beams of eight moving: 159 us, the copy bandwidth).
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 #include "common.cuh"
 
@@ -533,6 +535,27 @@ struct ReorderParams {
   int beams;
 };
 
+// One dimension of a state's layout: bytes from one index to the next, indices.
+struct Dim {
+  int64_t stride, size;
+};
+
+// Whether two states of one layout, `delta` bytes apart, share a byte: some difference of their positions,
+// sum_d i_d stride_d with |i_d| < size_d, lies within inner_bytes of delta. `dims` goes from the largest
+// stride down, each at least the extent (extents[d + 1]) of what follows it, so that only the two multiples of a
+// stride around what is left of delta can lead there.
+inline bool share_bytes(const Dim *dims, const int64_t *extents, int n, int64_t delta) {
+  if (n == 0) return delta > -extents[0] && delta < extents[0];
+  const int64_t stride = dims[0].stride, top = dims[0].size - 1, rest = extents[1];
+  int64_t i = delta < 0 || delta >= stride ? delta / stride : 0;  // rounded towards 0
+  if (delta < i * stride) --i;
+  for (int k = 0; k < 2; ++k, ++i) {
+    const int64_t left = delta - i * stride;
+    if (i >= -top && i <= top && left > -rest && left < rest && share_bytes(dims + 1, extents + 1, n - 1, left)) return true;
+  }
+  return false;
+}
+
 // state[b][i] <- state[b][parent[i]] in place: a thread owns one vector position of a request, loads
 // what the moving beams need and then stores it, so no other thread touches what it reads or writes.
 template <typename V, int B>
@@ -650,11 +673,12 @@ extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *
   int64_t count = 1;
   int align = 16;
   auto divides = [&](int64_t v) { while (align > 1 && v % align) align /= 2; };
-  struct Dim { int64_t stride, size; };
   Dim dims[4] = {{outer_stride[0], outer[0]}, {outer_stride[1], outer[1]}, {outer_stride[2], outer[2]},
                  {row_stride, batch * beams}};
   std::sort(dims, dims + 4, [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
-  int64_t extent = inner_bytes;
+  int64_t extent = inner_bytes, extents[5] = {0, 0, 0, 0, inner_bytes};  // of the last n dimensions of `steps`
+  Dim steps[4];  // those with more than one index, from the largest stride down
+  int first_step = 4;
   for (const Dim &d : dims) {
     MQ_REQUIRE(d.size >= 0 && d.size < (1LL << 31), MQ_EINVAL, "%s: bad outer dimension", what);
     if (d.size == 0) return MQ_OK;
@@ -662,6 +686,7 @@ extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *
     MQ_REQUIRE(d.stride >= extent, MQ_EINVAL, "%s: states overlap (a stride is less than what it steps over)", what);
     divides(d.stride);
     extent += d.stride * (d.size - 1);
+    steps[--first_step] = d, extents[first_step] = extent;
   }
   for (int d = 0; d < 3; ++d) count *= outer[d];
   MQ_REQUIRE(outer[1] * outer[2] < (1LL << 31), MQ_EUNSUPPORTED, "%s: the outer dimensions are too large", what);
@@ -669,6 +694,16 @@ extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *
   for (int i = 0; i < nstates; ++i) {
     MQ_REQUIRE(states[i], MQ_EINVAL, "%s: null state", what);
     divides(static_cast<int64_t>(reinterpret_cast<uintptr_t>(states[i]) % 16));
+  }
+  if (nstates > 1) {  // two states of one launch that share memory would race
+    std::unique_ptr<uintptr_t[]> at(new (std::nothrow) uintptr_t[nstates]);
+    MQ_REQUIRE(at, MQ_EINVAL, "%s: no memory to compare %d states", what, nstates);
+    for (int i = 0; i < nstates; ++i) at[i] = reinterpret_cast<uintptr_t>(states[i]);
+    std::sort(at.get(), at.get() + nstates);
+    for (int i = 0; i < nstates; ++i)
+      for (int j = i + 1; j < nstates && at[j] - at[i] < static_cast<uintptr_t>(extent); ++j)
+        MQ_REQUIRE(!share_bytes(steps + first_step, extents + first_step, 4 - first_step, static_cast<int64_t>(at[j] - at[i])),
+                   MQ_EINVAL, "%s: states overlap one another", what);
   }
   mq::DeviceInfo dev;
   if (int rc = mq::device_info(&dev)) return rc;

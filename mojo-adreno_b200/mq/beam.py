@@ -78,7 +78,8 @@ def beam_reorder(states, parents):
     """state[b * beams + i] <- state[b * beams + parents[b, i]] in place for each tensor of `states` (one tensor or
     a list, e.g. every layer's keys and values): [batch * beams, ..] of any type, their other dimensions
     in any order, sliced or not (a cache's filled part: cache[:, :, :length]). parents int32 [batch,
-    beams], as beam_select gives them. Only beams that change their parent are copied. Returns states."""
+    beams], as beam_select gives them. Only beams that change their parent are copied. No two states may share memory
+    (refused where they have one layout). Returns states."""
     each = [states] if isinstance(states, torch.Tensor) else list(states)
     if not isinstance(parents, torch.Tensor) or parents.dim() != 2:
         raise MQError(-1, "parents: expected a [batch, beams] tensor")

@@ -235,6 +235,20 @@ def test_reorder_views(cuda, perm, cut):
     assert torch.equal(state, want)
 
 
+def test_reorder_of_states_beside_and_inside_one_another(cuda):
+    """Keys and values of all layers in one tensor are moved together; a tensor given twice is refused and stays."""
+    parents = torch.tensor([[1, 1, 0, 2], [3, 0, 0, 0]], dtype=torch.int32, device=cuda)
+    cache = torch.randn(8, 3, 2, 10, 4, 16, device=cuda)  # [rows, layers, keys and values, length, heads, dim]
+    want = cache.clone()
+    want[:, :, :, :7] = reordered(cache, parents.long())[:, :, :, :7]
+    mq.beam_reorder([cache[:, i, j, :7] for i in range(3) for j in range(2)], parents)
+    assert torch.equal(cache, want)
+    for pair in ([cache, cache], [cache[:, 0, 0, :7], cache[:, 1, 0, :7], cache[:, 0, 0, 2:9]]):
+        with pytest.raises(mq.MQError, match="one another"):
+            mq.beam_reorder(pair, parents)
+    assert torch.equal(cache, want) and mq.device_status() == 0
+
+
 def test_reorder_past_32_bits_and_many_tensors(cuda):
     """A request's state more than 4 GiB from the first one's, and more tensors than one launch takes."""
     big = torch.empty(4, 1400 << 20, dtype=torch.uint8, device=cuda)

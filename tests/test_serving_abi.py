@@ -98,6 +98,27 @@ def test_beams():
     assert _status("mq_beam_reorder", *args)[0] == 0
 
 
+def test_reorder_refuses_states_that_share_memory():
+    """Two states of one layout, any distance apart: refused exactly where their bytes meet."""
+    import itertools
+
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("what is not refused would be launched with made-up addresses")
+    layouts = (((1, 1, 1), (0, 0, 0), 2, 12), ((1, 1, 3), (0, 0, 8), 4, 32), ((1, 2, 3), (0, 64, 12), 8, 192),
+               ((2, 3, 2), (40, 12, 4), 3, 100), ((1, 2, 2), (0, 8, 64), 8, 16))
+    for sizes, strides, inner, row in layouts:
+        offsets = [sum(i * s for i, s in zip(at, strides + (row,))) for at in itertools.product(*map(range, sizes + (4,)))]
+        own = {o + b for o in offsets for b in range(inner)}
+        for delta in range(0, max(own) + 3):
+            states = (P * 3)(P((1 << 20) + delta), P(1 << 24), P(1 << 20))
+            rc, msg = _status("mq_beam_reorder", states, 3, OK, 2, 2, row, (ctypes.c_int64 * 3)(*sizes),
+                              (ctypes.c_int64 * 3)(*strides), inner, None)
+            meet = any(b + delta in own for b in own)
+            assert (rc == -1 and "one another" in msg) if meet else rc == -3, (sizes, strides, inner, row, delta, rc, msg)
+
+
 def test_python_refuses_cpu_tensors():
     import torch
 
