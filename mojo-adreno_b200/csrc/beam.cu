@@ -184,6 +184,8 @@ __global__ void __launch_bounds__(kScan, kScanCtas) beam_scan_kernel(const ScanP
     if (!edge && arrived && !mbar_wait(&full[slot], (c - c_begin) / kStages & 1)) {
       raise_status(kStatusBeamLoadWait);
       arrived = false;
+      if (tid == 0)  // fetches no more; what is on its way lands before the CTA ends
+        for (int d = c; d < min(c_end, c + kStages); ++d) mbar_wait(&full[(d - c_begin) % kStages], (d - c_begin) / kStages & 1);
     }
     const uint8_t *mine_at = slots + slot * kChunkBytes + tid * 16;
     auto take = [&](int u) {
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(kScan, kScanCtas) beam_scan_kernel(const ScanP
       return g < nvec ? key_of(v[i], head + g * V + i % V) : 0;
     };
     const int offers = __syncthreads_count(big >= bar_value);
-    if (tid == 0 && c + kStages < c_end) fetch(c + kStages);  // every thread has read this slot
+    if (tid == 0 && arrived && c + kStages < c_end) fetch(c + kStages);  // every thread has read this slot
     if (offers == 0) continue;
     bound += offers * kElems;
     uint64_t limit = bar;

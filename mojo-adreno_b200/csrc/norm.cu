@@ -291,6 +291,24 @@ struct Ring {
   int stage_bytes, w_at, next_w_at, total;  // bytes; the weights lie behind the ring
 };
 
+// Where the first wait ran out for the thread that fetches. It then fetches no more, and at the end (code inside the
+// row loop cost post_norm 12337x4096 77 -> 79.7 us) the rows that were on their way are waited for: they land before the CTA
+// ends.
+struct Lost {
+  int64_t row;
+  int slot;
+  uint32_t phase;
+};
+__device__ __forceinline__ void drain_ring(uint64_t *full, const Ring &g, int64_t rows, const Lost &lost) {
+  int slot = lost.slot;
+  uint32_t phase = lost.phase;
+  int64_t row = lost.row;
+  for (int i = 0; i < g.stages && row < rows; ++i, row += gridDim.x) {
+    mbar_wait(&full[slot], phase);
+    if (++slot == g.stages) slot = 0, phase ^= 1;
+  }
+}
+
 // TY, TR, TW: the types of y, of the residual, and of w, next_w and the gate (a branch on a type inside would
 // have the loads of all three from shared memory speculated, and spilled).
 template <typename TY, typename TR, typename TW, int E, bool POST, bool EARLY>
@@ -298,6 +316,7 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kRingMax + 1];  // the last one: the weights
   __shared__ __align__(16) Scratch scratch[2][2];
+  __shared__ Lost lost;  // by thread 0
   constexpr int VEC = 8;
   if (EARLY) griddep_launch_dependents();
   if (threadIdx.x == 0) {
@@ -331,6 +350,7 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
   if (!mbar_wait(&full[kRingMax], 0)) {
     raise_status(kStatusNormLoadWait);
     arrived = false;
+    if (threadIdx.x == 0) lost = Lost{blockIdx.x, 0, 0};
   }
   int slot = 0, parity = 0;
   uint32_t phase = 0;
@@ -338,6 +358,7 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
     if (arrived && !mbar_wait(&full[slot], phase)) {
       raise_status(kStatusNormLoadWait);  // what there is goes on; the status says that it may be wrong
       arrived = false;
+      if (threadIdx.x == 0) lost = Lost{row, slot, phase};
     }
     const uint8_t *at = smem + slot * g.stage_bytes;
     Raw<TW, VEC> gate[E];  // (a row of it serves many rows, or comes from memory while this one is reduced)
@@ -393,10 +414,14 @@ __global__ void __launch_bounds__(kStreamThreads) row_stream_kernel(const Params
       row_reduce<E * VEC>(z, sum, top, p.h_dt == MQ_S8, tpr, scratch[parity][1]);
     }
     if (tpr == 32 || (POST && !p.h)) __syncthreads();  // else row_reduce's barrier: every thread has read the slot
-    if (threadIdx.x == 0 && row + static_cast<int64_t>(g.stages) * step < p.rows)
+    if (threadIdx.x == 0 && arrived && row + static_cast<int64_t>(g.stages) * step < p.rows)
       fetch(row + static_cast<int64_t>(g.stages) * step, slot);
     if (++slot == g.stages) slot = 0, phase ^= 1;
     if (!POST || p.h) write_h<VEC, E>(p, row, z, sum, top);
+  }
+  if (threadIdx.x == 0 && !arrived) {
+    mbar_wait(&full[kRingMax], 0);  // the weights
+    drain_ring(full, g, p.rows, lost);
   }
 }
 
@@ -443,6 +468,7 @@ __global__ void __launch_bounds__(TPR) row_stream1_kernel(const Params p, const 
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kRingMax];
   __shared__ __align__(16) Scratch scratch[2][2];
+  __shared__ Lost lost;  // by thread 0
   if (EARLY) griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < g.stages; ++i) mbar_init(&full[i], 1);
@@ -524,6 +550,7 @@ __global__ void __launch_bounds__(TPR) row_stream1_kernel(const Params p, const 
     if (arrived && !mbar_wait(&full[slot], phase)) {
       raise_status(kStatusNormLoadWait);  // what there is goes on; the status says that it may be wrong
       arrived = false;
+      if (threadIdx.x == 0) lost = Lost{row, slot, phase};
     }
     uint8_t *at = smem + slot * g.stage_bytes;
     float z[E], sum = 0.f;
@@ -565,11 +592,12 @@ __global__ void __launch_bounds__(TPR) row_stream1_kernel(const Params p, const 
       row_reduce<E>(z, sum, top, p.h_dt == MQ_S8, tpr, scratch[parity][1]);
     }
     if (tpr == 32 || (POST && !p.h)) __syncthreads();  // else row_reduce's barrier: every thread has read the slot
-    if (threadIdx.x == 0 && row + static_cast<int64_t>(g.stages) * step < p.rows)
+    if (threadIdx.x == 0 && arrived && row + static_cast<int64_t>(g.stages) * step < p.rows)
       fetch(row + static_cast<int64_t>(g.stages) * step, slot);
     if (++slot == g.stages) slot = 0, phase ^= 1;
     if (!POST || p.h) write_h<1, E, TPR>(p, row, z, sum, top);
   }
+  if (threadIdx.x == 0 && !arrived) drain_ring(full, g, p.rows, lost);
 }
 
 template <int VEC, int E, bool POST, bool EARLY>
