@@ -80,13 +80,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// A sum s stands for s * 2^(unit(m)) with m the largest logit it has seen. unit(m) is the fp32 product m log2 e, so that
-// a term is one FMA, 2^(v log2 e - unit(m)), and no rounding of the unit enters the result; where that product
-// could overflow (a mask of the type's lowest value) terms are 2^((v - m) log2 e) and s stands for s * e^m.
-__device__ __forceinline__ bool moderate(float m) { return fabsf(m) < 1e37f; }
-// What takes a sum from m to another m that is not smaller.
+// A sum s stands for s * 2^(unit(m)) with m the largest logit it has seen. unit(m) is the rounded fp32 product m log2 e, so
+// that a term is one FMA, 2^(v log2 e - unit(m)), and the unit's rounding error does not enter the result, being in the
+// term and in the unit. It is in the term as a factor, though, of 2^128 and more where m is some 1e10 (a row masked with -1e10):
+// above 1e6, where it is 2^(1/16) at most, terms are 2^((v - m) log2 e) and s stands for s * e^m.
+__device__ __forceinline__ bool moderate(float m) { return fabsf(m) < 1e6f; }
+__device__ __forceinline__ float unit_of(float m) { return __fmul_rn(m, kLog2e); }  // (never part of an FMA)
+// What takes a sum from m to another m that is not smaller; 1 where they are equal.
 __device__ __forceinline__ float rescale(float from, float to) {
-  return exp2_fast(moderate(from) && moderate(to) ? from * kLog2e - to * kLog2e : (from - to) * kLog2e);
+  float e = __fsub_rn(unit_of(from), unit_of(to));
+  if (__builtin_expect(!moderate(fmaxf(fabsf(from), fabsf(to))), 0))
+    e = moderate(from) ? fmaf(-to, kLog2e, unit_of(from)) : moderate(to) ? fmaf(from, kLog2e, -unit_of(to)) : (from - to) * kLog2e;
+  return exp2_fast(e);
 }
 
 template <typename T>
@@ -214,7 +219,7 @@ __global__ void __launch_bounds__(kScan, kScanCtas) beam_scan_kernel(const ScanP
     }
     // A NaN or +infinity (m infinite: inf - inf) makes s NaN.
     if (moderate(m)) {
-      const float unit = m * kLog2e;
+      const float unit = unit_of(m);
 #pragma unroll
       for (int i = 0; i < kElems; ++i) s += exp2_fast(fmaf(v[i], kLog2e, -unit));
     } else {
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) {
       if (total != total) raise_status(kStatusBeamNonFinite);
-      total = static_cast<float>(moderate(top) ? (top * kLog2e + log2(static_cast<double>(total))) / static_cast<double>(kLog2e)
+      total = static_cast<float>(moderate(top) ? (unit_of(top) + log2(static_cast<double>(total))) / static_cast<double>(kLog2e)
                                                : top + log(static_cast<double>(total)));
       lse[i] = total;
       if (!(fabsf(total) < INFINITY)) kind[i] = kDead;

@@ -112,6 +112,27 @@ def test_select_masks_of_the_lowest_value(cuda, dtype, vocab):
     assert mq.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [3, 5000, 33000])
+@pytest.mark.parametrize("size", [1e5, 3e6, 1e9, 1e10, 1e30, 3e37])
+def test_select_rows_of_one_huge_magnitude(cuda, size, vocab, dtype):
+    """A row all of whose logits are far from zero, as masks of -1e9 or -1e30 make one, is a row like any other; so
+    is one where such values stand beside usual ones."""
+    rng = np.random.default_rng(vocab)
+    usual = (rng.integers(-16, 16, vocab) / 8.0).astype(np.float32)
+    for mask in (-size, size):
+        z = np.stack([usual, np.full(vocab, mask, np.float32)])
+        z[1] = t(z[1:], cuda, dtype).float().cpu().numpy()
+        # lse swallows what is beside it, so such a token scores between scores[1] - log(vocab) and scores[1]: best of all
+        got, cand = select(z, np.array([[-40, -3]], np.float32), cuda, dtype=dtype)
+        check(got, cand, 2, 3 * size)
+    z[1, : vocab // 2 + 1] = -abs(z[1, 0])  # a part that is masked, the rest is usual
+    z[1, vocab // 2 + 1:] = usual[vocab // 2 + 1:]
+    got, cand = select(z, np.array([[-40, -3.37]], np.float32), cuda, dtype=dtype)
+    check(got, cand, 2)
+    assert mq.device_status() == 0
+
+
 def test_select_takes_equal_scores_by_index(cuda):
     """Unequal logits far below the score's last bit: every token of the beam scores the same, so the first
     tokens win, wherever the largest logits are."""
