@@ -431,7 +431,12 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
   }
   __syncthreads();
   uint64_t last = 0;  // the logit key that ends list `tid` if it is full
-  if (tid < lists && kind[tid / p.splits] == kLive) last = cand[tid * kp + kp - 1];
+  int equal = 0;      // pairs of that logit at the list's end
+  if (tid < lists && kind[tid / p.splits] == kLive) {
+    last = cand[tid * kp + kp - 1];
+    do ++equal;
+    while (equal < kp && cand[tid * kp + kp - 1 - equal] >> 32 == last >> 32);
+  }
   __syncthreads();
   // e / kp and l / splits by multiplication: exact for e < kMaxLists * kp, l < kMaxLists.
   const uint32_t per_kp = ((1u << 22) + kp - 1) / kp, per_split = ((1u << 16) + p.splits - 1) / p.splits;
@@ -475,15 +480,17 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const MergeParams 
   }
   __syncthreads();
 
-  // Unequal logits with equal scores: a token that was not kept could tie with the last chosen one and
-  // have a lower index, where a full list's last pair ties with it and so would the next lower logit.
+  // Unequal logits with equal scores: a token that was not kept could tie with the last chosen one and have a lower
+  // index where a full list's last pair ties with it, and so does the next lower logit, or a pair of the list with
+  // a larger logit (the token may have the last pair's logit, and an index above that pair's but below the other's).
   const uint32_t edge = static_cast<uint32_t>(chosen[p.beams - 1] >> 32);
   bool open = false;
   if (last) {
     const int i = tid / p.splits;
     const float l = value_of_key(last);
     open = order_of(score_of(score[i], l, lse[i])) == edge &&
-           order_of(score_of(score[i], next_below(l, p.dtype), lse[i])) == edge;
+           ((equal < kp && static_cast<uint32_t>(cand[tid * kp + kp - 1 - equal] >> 32) == edge) ||
+            order_of(score_of(score[i], next_below(l, p.dtype), lse[i])) == edge);
   }
   if (__syncthreads_or(open)) {
     // Take the ties from the logits themselves, in the order of their flat index.

@@ -133,6 +133,30 @@ def test_select_rows_of_one_huge_magnitude(cuda, size, vocab, dtype):
     assert mq.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("vocab", [1000, 40000])
+def test_select_takes_equal_scores_of_dropped_tokens(cuda, vocab, dtype):
+    """Tokens 100 and 101 are one step of the type above tokens 10 and 20. Where the step is lost in the scores'
+    rounding the lower two win, else the upper two; one of each is never right. The logits start at one of eight
+    neighbouring values per request, so that the rounding falls differently."""
+    base, score = (5.0, -25.0) if dtype == torch.float32 else (0.2, -3000.0)
+    one = torch.tensor(base, dtype=dtype)
+    bits = one.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    ladder = torch.stack([(bits + j).view(dtype) for j in range(9)]).float().numpy()
+    for upper in ((100, 101), (vocab - 2, vocab - 1)):
+        z = np.full((8, 3, vocab), -2, np.float32)
+        z[:, 0, vocab // 2] = 8  # the best one, and most of lse
+        for j in range(8):
+            z[j, 0, [10, 20]] = ladder[j]
+            z[j, 0, list(upper)] = ladder[j + 1]
+        scores = np.full((8, 3), -INF, np.float32)
+        scores[:, 0] = score
+        (_, tokens, parents, _), _ = select(z.reshape(24, vocab), scores, cuda, dtype=dtype)
+        assert (tokens[:, 0] == vocab // 2).all() and (parents == 0).all()
+        pairs = [tuple(row) for row in tokens[:, 1:]]
+        assert set(pairs) == {(10, 20), upper}, pairs
+
+
 def test_select_takes_equal_scores_by_index(cuda):
     """Unequal logits far below the score's last bit: every token of the beam scores the same, so the first
     tokens win, wherever the largest logits are."""
