@@ -620,8 +620,13 @@ int reorder_launch(const ReorderParams &p, int batch, int nstates, cudaStream_t 
 }  // namespace beam
 }  // namespace mq
 
+// The sizes that mq_beam_select takes, beams being in range (by division: no product of them overflows).
+static bool beam_sizes_fit(int64_t batch, int beams, int64_t vocab) {
+  return vocab <= ((1LL << 31) - mq::beam::kChunkBytes - 1) / beams && batch <= ((1LL << 22) - 1) / beams;
+}
+
 extern "C" size_t mq_beam_workspace_size(int64_t batch, int beams, int64_t vocab) {
-  if (batch <= 0 || beams <= 0 || beams > mq::beam::kMaxBeams || vocab <= 0) return 0;
+  if (batch <= 0 || beams <= 0 || beams > mq::beam::kMaxBeams || vocab <= 0 || !beam_sizes_fit(batch, beams, vocab)) return 0;
   const int64_t rows = batch * beams;
   return mq::beam::parts_bytes(rows * mq::beam::splits_for(rows, beams, vocab), beams + 1);
 }
@@ -634,8 +639,7 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t ld, const f
   const char *what = "mq_beam_select";
   MQ_REQUIRE(batch >= 0 && beams > 0 && vocab > 0, MQ_EINVAL, "%s: bad shape", what);
   MQ_REQUIRE(beams <= kMaxBeams, MQ_EUNSUPPORTED, "%s: beams is above %d", what, kMaxBeams);
-  MQ_REQUIRE(vocab * beams < (1LL << 31) - kChunkBytes && batch * beams < (1LL << 22), MQ_EUNSUPPORTED,
-             "%s: beams * vocab or batch * beams is too large", what);
+  MQ_REQUIRE(beam_sizes_fit(batch, beams, vocab), MQ_EUNSUPPORTED, "%s: beams * vocab or batch * beams is too large", what);
   MQ_REQUIRE(dtype == MQ_F32 || dtype == MQ_F16 || dtype == MQ_BF16, MQ_EINVAL,
              "%s: the logits' type must be MQ_F32, MQ_F16 or MQ_BF16", what);
   MQ_REQUIRE(ld >= vocab, MQ_EINVAL, "%s: the logits' row stride is less than vocab", what);
@@ -681,6 +685,7 @@ extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *
   MQ_REQUIRE(beams <= kMaxBeams && batch <= 65535, MQ_EUNSUPPORTED, "%s: beams is above %d or batch above 65535", what,
              kMaxBeams);
   if (nstates == 0 || batch == 0 || inner_bytes == 0) return MQ_OK;
+  MQ_REQUIRE(inner_bytes < (1LL << 60), MQ_EUNSUPPORTED, "%s: a state is too large", what);
   MQ_REQUIRE(states && parents && outer && outer_stride, MQ_EINVAL, "%s: null pointer", what);
   // Every (row, outer index) must have bytes of its own: sorted by stride, each dimension has to step
   // over all that the faster ones cover.
@@ -698,6 +703,7 @@ extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *
     if (d.size == 0) return MQ_OK;
     if (d.size == 1) continue;
     MQ_REQUIRE(d.stride >= extent, MQ_EINVAL, "%s: states overlap (a stride is less than what it steps over)", what);
+    MQ_REQUIRE(d.stride < (1LL << 60) / d.size, MQ_EUNSUPPORTED, "%s: a state is too large", what);
     divides(d.stride);
     extent += d.stride * (d.size - 1);
     steps[--first_step] = d, extents[first_step] = extent;

@@ -414,13 +414,13 @@ int launch(const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, const P
 }
 
 int check(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw, const float *ws, const void *y,
-          int y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t wrows, int64_t k, const char *what) {
+          int y_dtype, int64_t ldy, int64_t m, int64_t n, int planes, int64_t k, const char *what) {
   MQ_REQUIRE(m >= 0 && n > 0 && k > 0, MQ_EINVAL, "%s: bad shape", what);
   MQ_REQUIRE(y_dtype == MQ_F32 || y_dtype == MQ_F16 || y_dtype == MQ_BF16, MQ_EINVAL,
              "%s: the output type must be MQ_F32, MQ_F16 or MQ_BF16", what);
   MQ_REQUIRE(ldx >= k && ldw >= k && ldy >= n, MQ_EINVAL, "%s: a row stride is less than the row", what);
   MQ_REQUIRE(k <= kMaxK, MQ_EUNSUPPORTED, "%s: k is above %lld (the int32 sums)", what, static_cast<long long>(kMaxK));
-  MQ_REQUIRE(m < (1LL << 30) && wrows < (1LL << 30), MQ_EUNSUPPORTED, "%s: m and n must be below 2^30", what);
+  MQ_REQUIRE(m < (1LL << 30) && n < (1LL << 30) / planes, MQ_EUNSUPPORTED, "%s: m and n must be below 2^30", what);
   if (m == 0) return MQ_OK;
   MQ_REQUIRE(xq && xs && wq && ws && y, MQ_EINVAL, "%s: null pointer", what);
   MQ_REQUIRE(aligned(xq, 16) && aligned(wq, 16) && ldx % 16 == 0 && ldw % 16 == 0, MQ_EALIGN,
@@ -494,7 +494,7 @@ extern "C" int mq_gemm_w8a8(const int8_t *xq, int64_t ldx, const float *xs, cons
                             const float *ws, const float *bias, void *y, int y_dtype, int64_t ldy, int64_t m, int64_t n,
                             int64_t k, int add, void *stream) {
   const char *what = "mq_gemm_w8a8";
-  if (int rc = mq::w8::check(xq, ldx, xs, wq, ldw, ws, y, y_dtype, ldy, m, n, n, k, what)) return rc;
+  if (int rc = mq::w8::check(xq, ldx, xs, wq, ldw, ws, y, y_dtype, ldy, m, n, 1, k, what)) return rc;
   MQ_REQUIRE(mq::aligned(bias, 4), MQ_EALIGN, "%s: bias must be 4-byte aligned", what);
   if (m == 0) return MQ_OK;
   mq::w8::Params p{};
@@ -507,7 +507,7 @@ extern "C" int mq_gate_up_w8a8(const int8_t *xq, int64_t ldx, const float *xs, c
                                const float *ws, void *a, int a_dtype, int64_t lda, int64_t m, int64_t f, int64_t k,
                                void *stream) {
   const char *what = "mq_gate_up_w8a8";
-  if (int rc = mq::w8::check(xq, ldx, xs, wq, ldw, ws, a, a_dtype, lda, m, f, 2 * f, k, what)) return rc;
+  if (int rc = mq::w8::check(xq, ldx, xs, wq, ldw, ws, a, a_dtype, lda, m, f, 2, k, what)) return rc;
   if (m == 0) return MQ_OK;
   mq::w8::Params p{};
   p.xs = xs, p.ws = ws, p.y = a, p.ldy = lda, p.y_dtype = a_dtype;

@@ -119,6 +119,28 @@ def test_reorder_refuses_states_that_share_memory():
             assert (rc == -1 and "one another" in msg) if meet else rc == -3, (sizes, strides, inner, row, delta, rc, msg)
 
 
+def test_sizes_whose_products_pass_64_bits():
+    """Refused as too large, not taken for what is left of them after an overflow."""
+    from mq._lib import lib
+
+    huge = 1 << 62
+    for batch, vocab in ((huge, 1000), (2, huge), (1 << 60, 1 << 60), ((1 << 22) // 4, 1000), (2, (1 << 31) // 4)):
+        assert lib.mq_beam_workspace_size(batch, 4, vocab) == 0
+        rc, msg = _status("mq_beam_select", OK, 0, vocab, OK, None, -1, OK, OK, OK, None, batch, 4, vocab, OK, 1 << 24, None)
+        assert rc == -4 and "large" in msg, (batch, vocab, rc, msg)
+    assert lib.mq_beam_workspace_size((1 << 20) - 1, 4, 1000) > 0 and lib.mq_beam_workspace_size(1, 4, 536868000) > 0
+    rc, msg = _status("mq_gate_up_w8a8", OK, 64, OK, OK, 64, OK, OK, 0, huge, 4, huge, 64, None)
+    assert rc == -4 and "2^30" in msg, (rc, msg)
+    rc, msg = _status("mq_gemm_w8a8", OK, 64, OK, OK, 64, OK, None, OK, 0, huge, 4, huge, 64, 0, None)
+    assert rc == -4 and "2^30" in msg, (rc, msg)
+    states = (P * 2)(OK, P(1 << 24))
+    for sizes, strides, row, inner in (((1, 1, 4), (0, 0, 1 << 61), huge, 64), ((1, 1, 1), (0, 0, 0), huge, 64),
+                                       ((1, 1, 1), (0, 0, 0), huge, 1 << 61)):
+        rc, msg = _status("mq_beam_reorder", states, 2, OK, 2, 4, row, (ctypes.c_int64 * 3)(*sizes),
+                          (ctypes.c_int64 * 3)(*strides), inner, None)
+        assert rc == -4 and "too large" in msg, (sizes, strides, row, inner, rc, msg)
+
+
 def test_python_refuses_cpu_tensors():
     import torch
 
