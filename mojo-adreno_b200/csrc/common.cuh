@@ -10,6 +10,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 #include "../../include/mq.h"
 
@@ -97,18 +98,22 @@ int encode_tmap_3d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype
                    uint32_t box_cols, uint32_t box_rows, uint32_t box_planes, CUtensorMapSwizzle swizzle,
                    const char *what);
 
-// Raises kern's dynamic shared-memory limit to at least `smem` on the current device, once per
-// device: the attribute belongs to the device's context, so a process that drives several GPUs sets
-// it on each. `seen` is the kernel's own table of the limits already set, by device.
+// Raises kern's dynamic shared-memory limit to at least `smem` on the current device: the attribute belongs to the
+// device's context, so a process that drives several GPUs sets it on each. `seen` is the kernel's own table of the
+// limits already set, by device. A call that raises the limit compares, sets and notes it under a lock, so that the
+// limit never falls below what `seen` says; one that has no need to takes none.
 template <typename Kern>
 int ensure_smem(Kern kern, size_t smem, size_t (&seen)[64], const char *what) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || dev < 0 || dev >= 64) return fail(MQ_ECUDA, "%s: cudaGetDevice failed", what);
+  if (smem <= __atomic_load_n(&seen[dev], __ATOMIC_ACQUIRE)) return MQ_OK;
+  static std::mutex raising;
+  std::lock_guard<std::mutex> lock(raising);
   if (smem > seen[dev]) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return fail(MQ_ECUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
-    seen[dev] = smem;
+    __atomic_store_n(&seen[dev], smem, __ATOMIC_RELEASE);
   }
   return MQ_OK;
 }
