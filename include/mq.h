@@ -361,7 +361,8 @@ MQ_API int mq_gemm_w8a8(const int8_t *xq, int64_t ldx, const float *xs, const in
                         void *stream);
 
 /* a[t][j] = silu(g) * u with g, u the products of rows j and f + j of the fused [2f][k] gate|up matrix,
- * as mq_gemm_w8a8 computes them. */
+ * as mq_gemm_w8a8 computes them. silu is within 6 * 2^-23 of its value, relative, before the one rounding
+ * to a's type, and 0 below g = -87.3 (where it is above -1.1e-36). */
 MQ_API int mq_gate_up_w8a8(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq, int64_t ldw, const float *ws,
                            void *a, int a_dtype, int64_t lda, int64_t m, int64_t f, int64_t k, void *stream);
 

@@ -104,9 +104,21 @@ __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-// silu(g) * u with the fast exponential and quotient: their errors, (2 + 1.2 |g|) and 2 ulp, are below what
-// one rounding of g does to silu for large |g|; the accurate forms cost the epilogue several times as much.
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// silu(g) * u = g / (1 + e^-g) * u through E = e^-|g|, at most 1: g / (1 + E) where g is positive, g E / (1 + E) where it
+// is not, so the divisor stays within 1 .. 2 and its reciprocal is good to an ulp. E = 2^t (1 + c) with t = -|g| log2 e
+// rounded and c = -|g| - t ln 2 what the rounding took (ln 2 in two parts): without c the error would grow with |g|, to some
+// 80 ulp. As it is the whole stays within 6 * 2^-23 (2^t two, the rest roundings), and E, so the result, is 0 below
+// g = -87.3, where silu is above -1.1e-36. gate|up 2048x8192x512 37.3 us, 400x8192x2048 18.6; with expf and a division
+// 41.1 and 18.8, with an E that keeps its subnormals 40.1 and 19.0, without c 37.3 and 18.0.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  const float a = fmaxf(-fabsf(g), -200.f), t = a * 1.44269504f;  // (of an infinite g, c would be NaN)
+  const float c = fmaf(t, 1.904654299e-9f, fmaf(t, -0.693147182f, a));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  e = fmaf(e, c, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * (g < 0.f ? e : 1.f) * r * u;
+}
 
 template <int P, int SUB>  // weight planes of a tile: 1, or 2 (gate and up); 128-k blocks per stage
 __global__ void __launch_bounds__(kThreads, 1)

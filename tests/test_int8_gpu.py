@@ -11,6 +11,7 @@ import mq
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
+INF = float("inf")
 # half an ulp relative, and half of the smallest step
 ROUND = {torch.float32: (U, 2.0 ** -150), torch.float16: (2.0 ** -11, 2.0 ** -25), torch.bfloat16: (2.0 ** -8, 2.0 ** -134)}
 TYPES = list(ROUND)
@@ -90,6 +91,35 @@ def test_gate_up(cuda, m, f, k):
         # a relative error e of g moves silu by at most (1 + |g|) e; exp, the sum and the division add a few ulp
         close(a, ref, np.abs(ref) * (3 + np.abs(y[:, :f])), dtype)
     assert mq.device_status() == 0
+
+
+@pytest.mark.parametrize("m", [1, 40, 2000])
+def test_gate_up_keeps_its_bits_at_large_gates(cuda, m):
+    """fp32 outputs with gates from -104 to 90: within six steps of 2^-23 (2^t two, the reciprocal one, the sum and the
+    products one half each), however large the gate; below -87.3, where e^g is no normal number, between 0 and the value."""
+    f, k = 777, 32
+    gate = np.linspace(-104, 90, f).astype(np.float32)
+    xq, wq = np.zeros((m, k), np.int8), np.zeros((2 * f, k), np.int8)
+    xq[:, 3], wq[:, 3] = 1, 1
+    ws = np.concatenate([gate, np.full(f, 1, np.float32)])
+    a = mq.gate_up_w8a8(*(torch.from_numpy(v).to(cuda) for v in (xq, np.ones(m, np.float32), wq, ws)), dtype=torch.float32)
+    ref = serving.silu_mul(ws.astype(np.float64))
+    high, low = gate >= -87.3, np64(a)[:, gate < -87.3]
+    ratio = np.abs(np64(a) - ref)[:, high] / np.maximum(6 * 2.0 ** -23 * np.abs(ref), 1e-300)[high]
+    assert ratio.max() <= 1, f"{ratio.max()} of the bound at a gate of {gate[high][ratio.max(0).argmax()]}"
+    assert (low <= 0).all() and (low >= 1.001 * ref[gate < -87.3]).all()
+
+
+def test_gate_up_of_infinite_gates(cuda):
+    """silu(+inf) u = inf u, silu(-inf) is 0 times infinity: NaN, as the formula; its neighbours stay."""
+    q = torch.ones(1, 16, dtype=torch.int8, device=cuda)
+    w = torch.ones(6, 16, dtype=torch.int8, device=cuda)
+    ws = torch.tensor([INF, 1e37, -1e37, 2, 2, 2], device=cuda)
+    for dtype in (torch.float32, torch.bfloat16):
+        a = mq.gate_up_w8a8(q, torch.ones(1, device=cuda), w, ws, dtype=dtype)
+        assert a[0].tolist() == [INF, INF, 0], a
+    ws[0] = -INF
+    assert mq.gate_up_w8a8(q, torch.ones(1, device=cuda), w, ws)[0, 0].isnan()
 
 
 def test_largest_sums(cuda):
