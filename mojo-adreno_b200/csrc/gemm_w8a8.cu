@@ -81,6 +81,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();  // the barrier is taken by whole warps; of some, one lane comes from a branch of its own
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The address of the same shared variable in the CTA of the given rank of this cluster.
