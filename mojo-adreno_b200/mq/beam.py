@@ -100,7 +100,7 @@ def beam_reorder(states, parents):
             else:
                 rest.append(t)
         each = rest
-        if len(shape) < 2 or shape[0] != batch * beams:
+        if not shape or shape[0] != batch * beams:
             raise MQError(-1, f"states: shape {tuple(shape)} is not [{batch * beams}, ..]")
         if 0 not in shape:
             calls.append((same, _layout(first)))

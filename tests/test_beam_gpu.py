@@ -280,6 +280,19 @@ def test_reorder_views(cuda, perm, cut):
     assert torch.equal(state, want)
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64, torch.uint8])
+def test_reorder_of_one_number_per_beam(cuda, dtype):
+    """States [batch * beams]: lengths, positions, flags; also a column of a table."""
+    parents = torch.tensor([[1, 1, 0, 2], [3, 0, 0, 0]], dtype=torch.int32, device=cuda)
+    x, table = torch.arange(8, device=cuda).to(dtype), torch.arange(24, device=cuda).to(dtype).view(8, 3)
+    want, column = reordered(x, parents.long()), reordered(table[:, 1], parents.long())
+    others = table[:, [0, 2]]
+    mq.beam_reorder([x, table[:, 1]], parents)
+    assert torch.equal(x, want) and torch.equal(table[:, 1], column) and torch.equal(table[:, [0, 2]], others)
+    with pytest.raises(mq.MQError, match="shape"):
+        mq.beam_reorder(x.sum(), parents)
+
+
 def test_reorder_of_states_beside_and_inside_one_another(cuda):
     """Keys and values of all layers in one tensor are moved together; a tensor given twice is refused and stays."""
     parents = torch.tensor([[1, 1, 0, 2], [3, 0, 0, 0]], dtype=torch.int32, device=cuda)
