@@ -413,6 +413,11 @@ MQ_API int mq_beam_select(const void *logits, int dtype, int64_t ld, const float
 MQ_API int mq_beam_reorder(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
                            int64_t row_stride, const int64_t *outer, const int64_t *outer_stride, int64_t inner_bytes,
                            void *stream);
+/* What mq_beam_reorder would answer to these arguments, without moving anything: for a caller with states of several
+ * layouts, who wants all of them moved or none. */
+MQ_API int mq_beam_reorder_check(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
+                                 int64_t row_stride, const int64_t *outer, const int64_t *outer_stride,
+                                 int64_t inner_bytes);
 
 /* ---- weight files -------------------------------------------------------------------------------- */
 

@@ -607,9 +607,7 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant
 
 template <typename V>
 int reorder_launch(const ReorderParams &p, int batch, int nstates, cudaStream_t s) {
-  const int64_t blocks = (p.items + 255) / 256;
-  MQ_REQUIRE(blocks < (1LL << 31), MQ_EUNSUPPORTED, "mq_beam_reorder: a state is too large");
-  const dim3 grid(static_cast<unsigned>(blocks), batch, nstates);
+  const dim3 grid(static_cast<unsigned>((p.items + 255) / 256), batch, nstates);
   const char *what = "mq_beam_reorder";
   if (p.beams <= 4) return launch_overlapped(beam_reorder_kernel<V, 4>, grid, dim3(256), 0, s, what, p);
   if (p.beams <= 8) return launch_overlapped(beam_reorder_kernel<V, 8>, grid, dim3(256), 0, s, what, p);
@@ -676,10 +674,13 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t ld, const f
   return mq::launch_overlapped(beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(kThreads), smem, s, what, mp);
 }
 
-extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
-                               int64_t row_stride, const int64_t *outer, const int64_t *outer_stride, int64_t inner_bytes,
-                               void *stream) {
-  using namespace mq::beam;
+namespace mq {
+namespace beam {
+
+// The checks of mq_beam_reorder, and its launches' parameters but for the states: p.items stays 0 where there is nothing
+// to move. width: bytes of a vector.
+int reorder_plan(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams, int64_t row_stride,
+                 const int64_t *outer, const int64_t *outer_stride, int64_t inner_bytes, ReorderParams &p, int &width) {
   const char *what = "mq_beam_reorder";
   MQ_REQUIRE(nstates >= 0 && batch >= 0 && beams > 0 && inner_bytes >= 0, MQ_EINVAL, "%s: bad shape", what);
   MQ_REQUIRE(beams <= kMaxBeams && batch <= 65535, MQ_EUNSUPPORTED, "%s: beams is above %d or batch above 65535", what,
@@ -725,16 +726,39 @@ extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *
         MQ_REQUIRE(!share_bytes(steps + first_step, extents + first_step, 4 - first_step, static_cast<int64_t>(at[j] - at[i])),
                    MQ_EINVAL, "%s: states overlap one another", what);
   }
-  mq::DeviceInfo dev;
-  if (int rc = mq::device_info(&dev)) return rc;
-  ReorderParams p{};
   p.parents = parents, p.row_stride = row_stride, p.beams = beams;
   for (int d = 0; d < 3; ++d) p.outer_stride[d] = outer_stride[d];
   p.outer1 = static_cast<uint32_t>(outer[1]), p.outer2 = static_cast<uint32_t>(outer[2]);
-  const int width = align == 16 ? 16 : align >= 4 ? 4 : align;
+  width = align == 16 ? 16 : align >= 4 ? 4 : align;
   MQ_REQUIRE(inner_bytes / width < (1LL << 31), MQ_EUNSUPPORTED, "%s: the inner part is too large", what);
   p.vecs = static_cast<uint32_t>(inner_bytes / width);
   p.items = count * p.vecs;
+  MQ_REQUIRE(p.items < (1LL << 31) * 256 - 256, MQ_EUNSUPPORTED, "%s: a state is too large", what);
+  return MQ_OK;
+}
+
+}  // namespace beam
+}  // namespace mq
+
+extern "C" int mq_beam_reorder_check(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
+                                     int64_t row_stride, const int64_t *outer, const int64_t *outer_stride,
+                                     int64_t inner_bytes) {
+  mq::beam::ReorderParams p{};
+  int width = 0;
+  return mq::beam::reorder_plan(states, nstates, parents, batch, beams, row_stride, outer, outer_stride, inner_bytes, p, width);
+}
+
+extern "C" int mq_beam_reorder(void *const *states, int nstates, const int32_t *parents, int64_t batch, int beams,
+                               int64_t row_stride, const int64_t *outer, const int64_t *outer_stride, int64_t inner_bytes,
+                               void *stream) {
+  using namespace mq::beam;
+  ReorderParams p{};
+  int width = 0;
+  if (int rc = reorder_plan(states, nstates, parents, batch, beams, row_stride, outer, outer_stride, inner_bytes, p, width))
+    return rc;
+  if (p.items == 0) return MQ_OK;
+  mq::DeviceInfo dev;
+  if (int rc = mq::device_info(&dev)) return rc;
   for (int first = 0; first < nstates; first += kMaxStates) {
     const int n = std::min(kMaxStates, nstates - first);
     for (int i = 0; i < n; ++i) p.states[i] = states[first + i];

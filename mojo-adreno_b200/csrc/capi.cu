@@ -145,7 +145,7 @@ extern "C" {
 
 const char *mq_last_error(void) { return mq::t_error; }
 
-int mq_version(void) { return 101; }
+int mq_version(void) { return 102; }
 
 int mq_device_status(int reset, void *stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -66,6 +66,7 @@ SIGNATURES = {
     "mq_beam_select": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_vp,
                                c_size, c_vp]),
     "mq_beam_reorder": (c_int, [c_vp, c_int, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_i64, c_vp]),
+    "mq_beam_reorder_check": (c_int, [c_vp, c_int, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_i64]),
     "mq_read_file_to_device": (c_int, [c_vp, c_i64, c_char_p, c_i64, c_vp]),
     "mq_pack_half": (c_int, [c_vp, c_vp, c_i64, c_vp]),
 }

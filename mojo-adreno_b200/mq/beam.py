@@ -85,7 +85,7 @@ def beam_reorder(states, parents):
         raise MQError(-1, "parents: expected a [batch, beams] tensor")
     batch, beams = parents.shape
     parents_p = _flat(parents, "parents", _I32, batch * beams)
-    calls = []  # one launch for all states of one layout, none before all are checked
+    calls = []  # one for all states of one layout, none before all are checked
     while each:
         first = each[0]
         if not isinstance(first, torch.Tensor):
@@ -103,10 +103,13 @@ def beam_reorder(states, parents):
         if not shape or shape[0] != batch * beams:
             raise MQError(-1, f"states: shape {tuple(shape)} is not [{batch * beams}, ..]")
         if 0 not in shape:
-            calls.append((same, _layout(first)))
+            row, outer, strides, inner = _layout(first)
+            n = len(same)
+            calls.append(((ctypes.c_void_p * n)(*same), n, parents_p, batch, beams, row, _Three(*outer), _Three(*strides), inner))
+    if len(calls) > 1:
+        for args in calls:
+            lib.call("mq_beam_reorder_check", *args)
     stream = _stream()
-    for same, (row, outer, strides, inner) in calls:
-        n = len(same)
-        lib.call("mq_beam_reorder", (ctypes.c_void_p * n)(*same), n, parents_p, batch, beams, row, _Three(*outer),
-                 _Three(*strides), inner, stream)
+    for args in calls:
+        lib.call("mq_beam_reorder", *args, stream)
     return states

@@ -339,6 +339,17 @@ def test_reorder_refuses_before_it_moves_anything(cuda):
     assert torch.equal(good, kept)
 
 
+@pytest.mark.parametrize("bad", ["expanded", "overlapping", "twice"])
+def test_reorder_moves_all_layouts_or_none(cuda, bad):
+    """A state of a second layout that only the library refuses: the first layout's states stay too."""
+    good, x = torch.randn(8, 16, device=cuda), torch.randn(9, 32, device=cuda)
+    second = {"expanded": [x[0].expand(8, 32)], "overlapping": [x.as_strided((8, 24), (16, 1))], "twice": [x[:8], x[:8]]}[bad]
+    kept, parents = (good.clone(), x.clone()), torch.tensor([[1, 0, 0, 0], [3, 3, 3, 3]], dtype=torch.int32, device=cuda)
+    with pytest.raises(mq.MQError, match="overlap"):
+        mq.beam_reorder([good, *second], parents)
+    assert torch.equal(good, kept[0]) and torch.equal(x, kept[1])
+
+
 def test_reorder_refusals(cuda):
     x, p = torch.randn(8, 16, device=cuda), torch.zeros(2, 4, dtype=torch.int32, device=cuda)
     with pytest.raises(mq.MQError, match="shape"):
