@@ -30,15 +30,18 @@ constexpr int kThreads = 256;
 constexpr int kMaxBeams = 32;
 constexpr int kMaxLists = 256;  // (beam, split) lists of a request: one per thread of the merge
 constexpr int kVecs = 4;        // 16-byte vectors per thread and chunk
-constexpr int kScan = 128, kScanCtas = 8;  // threads of a scan CTA, CTAs per SM
+constexpr int kScan = 128, kScanCtas = 7;  // threads of a scan CTA, CTAs per SM
 constexpr int kChunkBytes = kScan * kVecs * 16;
 constexpr int kFresh = 1280;    // pairs that may wait to be merged into the list: at least (kMaxBeams + 1) * 32
 constexpr int kStages = 2;      // chunks on their way into shared memory: 16 KB for each of the CTAs of an SM
+// So many CTAs fit in an SM's shared memory: their static and dynamic part, and 1 KB that the system takes.
+static_assert(kScanCtas * (1024 + kStages * kChunkBytes + (2 * (kMaxBeams + 1) + kFresh + kScan) * 8 + 128) <= 228 * 1024,
+              "the scan plans with more CTAs than run at once");
 constexpr float kNegInf = -INFINITY, kLowest = -3.402823466e38f, kLog2e = 1.44269504088896340736f;
 
 // (Counted in fp32 chunks for every type, so that the workspace's size does not depend on it.)
-// As many CTAs as run at once (64x8x128256: 2 splits, 63 us; 1: 88, 3: 80; 16x4x50257: 16 splits, 16 us; 8: 19, 24:
-// 17.5); at most one list per thread of the merge.
+// As many CTAs as run at once (a few more start a second wave: 32x4x151669 fp32 8 splits 28.1 us, 9 36.2; 16x4x50257 16 splits
+// 15.6 us, 18 18.5); at most one list per thread of the merge.
 __host__ __device__ constexpr int splits_for(int64_t rows, int beams, int64_t vocab) {
   const int64_t chunks = (vocab * 4 + kChunkBytes - 1) / kChunkBytes;
   int64_t s = 148 * kScanCtas / rows;
