@@ -64,7 +64,11 @@ MQ_API int mq_version(void);
 
 /* Reads the device-side status word that kernels with bounded waits set when a wait runs out
  * (0 = none, else the code of the first wait that gave up). Synchronises `stream`. When `reset`
- * is nonzero the word is cleared afterwards. Returns the word (>= 0) or a negative MQ_E* code. */
+ * is nonzero the word is cleared afterwards. Returns the word (>= 0) or a negative MQ_E* code.
+ * Waits: 1-4 int4 and ternary GEMM, 5-7 GEMVs, 10 and 11 a peer's rows or returns, 12-14 int8 products, 17 beam
+ * selection, 18 norms. Four codes report data instead: 8 an expert id out of range, 9 more pairs than a rank's capacity,
+ * 15 a beam with a NaN or +inf logit, 16 a parent out of range. The first code of either kind stays until it is reset,
+ * so a caller who expects such data resets the word to see what comes later. */
 MQ_API int mq_device_status(int reset, void *stream);
 
 /*
@@ -397,7 +401,8 @@ MQ_API int mq_post_norm(const void *y, int y_dtype, int64_t ldy, const void *w, 
  * eos. logits: [batch * beams] rows of vocab, ld elements apart, fp32 / fp16 / bf16 (-inf masks a token).
  * finished: bytes [batch][beams] or NULL; eos: a token, or -1 where finished is NULL. next_scores and
  * next_finished may be the input buffers. beams <= 32. workspace: mq_beam_workspace_size() bytes, 16-byte
- * aligned. batch == 0 does nothing. */
+ * aligned. batch == 0 does nothing. Scores are sums of log-probabilities, without a length normalisation: a caller who
+ * ranks hypotheses by one applies it outside. mq_beam_workspace_size is 0 for sizes that mq_beam_select refuses. */
 MQ_API size_t mq_beam_workspace_size(int64_t batch, int beams, int64_t vocab);
 MQ_API int mq_beam_select(const void *logits, int dtype, int64_t ld, const float *scores, const uint8_t *finished,
                           int eos, float *next_scores, int32_t *tokens, int32_t *parents, uint8_t *next_finished,

@@ -12,10 +12,12 @@
 // gives unequal logits equal scores; the pair beyond the `beams` best shows whether that can matter.
 // beam_merge_kernel, one CTA per request, joins the sums, scores the kept pairs and picks the best.
 //
-// Many rows: bound by the scan's instructions (14 per logit, 0.53 issued per cycle) before the bytes: 64x8x128256
-// 57 us in fp32 (4.6 TB/s), 58 in fp16; of that the merge is 5. One request (1x4x151669): 13 us, all
-// latency: 5 for a chunk, 5.5 for the merge, the launches. The states' reordering moves 6.6 TB/s (64x8 states of
-// 2 x 8 x 1001 x 64 fp16, five beams of eight moving: 159 us, the copy bandwidth).
+// Many rows: 64x8x128256 57 us in fp32 (4.6 TB/s), 57 in fp16 (2.3 TB/s), 58 in bf16; of that the merge is 5. Neither the bytes nor
+// the issue slots bound it (14 instructions per logit, 0.54 issued per cycle and scheduler): of the seven warps of a
+// scheduler most wait at the barrier of their chunk (a quarter of the stalls, a third in fp16) or for the
+// instruction before (a quarter). One request (1x4x151669): 13.6 us in a graph, latency: some 5 for a chunk, 5.5 for the merge, the
+// launches. The states' reordering moves 6.5 TB/s (64x8 states of 2 x 8 x 1001 x 64 fp16, five beams of eight
+// moving: 161 us, the copy bandwidth).
 #include <algorithm>
 #include <cmath>
 #include <memory>

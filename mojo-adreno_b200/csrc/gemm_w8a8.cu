@@ -109,8 +109,9 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bf
 // is not, so the divisor stays within 1 .. 2 and its reciprocal is good to an ulp. E = 2^t (1 + c) with t = -|g| log2 e
 // rounded and c = -|g| - t ln 2 what the rounding took (ln 2 in two parts): without c the error would grow with |g|, to some
 // 80 ulp. As it is the whole stays within 6 * 2^-23 (2^t two, the rest roundings), and E, so the result, is 0 below
-// g = -87.3, where silu is above -1.1e-36. gate|up 2048x8192x512 37.3 us, 400x8192x2048 18.6; with expf and a division
-// 41.1 and 18.8, with an E that keeps its subnormals 40.1 and 19.0, without c 37.3 and 18.0.
+// g = -87.3, where silu is above -1.1e-36. gate|up 2048x8192x512 fp16 37.2 us, fp32 37.2, 400x8192x2048 bf16 18.5; with expf
+// and a division 41.1, 40.9 and 18.8, with an E that keeps its subnormals 40.1, 40.5 and 19.0; c for fp32 outputs only, in
+// two copies of the loops, 35.6, 39.2 and 18.4: not kept for what it takes from fp32.
 __device__ __forceinline__ float silu_mul(float g, float u) {
   const float a = fmaxf(-fabsf(g), -200.f), t = a * 1.44269504f;  // (of an infinite g, c would be NaN)
   const float c = fmaf(t, 1.904654299e-9f, fmaf(t, -0.693147182f, a));

@@ -13,7 +13,8 @@
 // Three kernels: block_norm_kernel (a row per CTA or warp: few rows, rows below 768 or above 8192 columns),
 // row_stream_kernel (many aligned rows) and row_stream1_kernel (many rows without alignment).
 // B200: pre_norm 8192x4096 bf16 26.5 us (5.1 TB/s), to int8 28.3; post_norm 12337x4096 bf16 with its gate
-// and the next norm 70.8-73 us (5.6 TB/s, 0.87 of the copy bandwidth); one row of 4096: 2.4 and 3.6 us.
+// and the next norm 70.8-73 us (5.6 TB/s, 0.87 of the copy bandwidth); one row of 4096: 2.1 and 3.0-3.7 us. Rows below 768
+// columns do not stream, and a warp per short row does not fill the memory pipe: 262144x128 bf16 68 us, three floors.
 #include <algorithm>
 #include <type_traits>
 
@@ -630,7 +631,7 @@ Ring ring_of(const Params &p, int per_sm) {
   return g;
 }
 
-// CTAs per SM of the streaming kernel, 0 where it does not apply: 32 values a thread, about 640 threads per SM, fewer
+// CTAs per SM of the streaming kernel, 0 where it does not apply: 16 values a thread, 1024 threads per SM, fewer
 // where the ring would have less than three stages. The residual has y's type or fp32; w, next_w and the gate one
 // type, y's or fp32.
 template <bool POST>
