@@ -424,6 +424,77 @@ MQ_API int mq_beam_reorder_check(void *const *states, int nstates, const int32_t
                                  int64_t row_stride, const int64_t *outer, const int64_t *outer_stride,
                                  int64_t inner_bytes);
 
+/* ---- a paged cache of keys and values, and attention over it ----------------------------------------------
+ * No counterpart in the reference's hot path (its attention reads one contiguous cache of one sequence). A cache is a pool of
+ * pages of `page` positions for each of `heads` kv heads, keys and values apart. Sequence b keeps position p in
+ * page table[b][p / page] of the pool, at row p % page. */
+typedef struct mq_kv_pages {
+  void *k, *v;                     /* rows of dim elements: fp16, bf16, or int8 with a scale per row */
+  float *k_scale, *v_scale;        /* int8 only, else not read */
+  int64_t k_stride[3], v_stride[3];    /* elements from one page, head and position to the next; rows start 16-byte aligned */
+  int64_t ks_stride[3], vs_stride[3];  /* the same of the scales */
+  int64_t pages;
+  int32_t dtype;                   /* MQ_F16, MQ_BF16 or MQ_S8 */
+  int32_t heads, page, dim;        /* page: 16, 32, 64, 128 or 256; dim: a multiple of 16 up to 128 */
+} mq_kv_pages;
+
+/* The new tokens of a call, [tokens] rows, belong to `batch` sequences: sequence b has rows starts[b] .. starts[b + 1] - 1
+ * (starts: int32 [batch + 1], rising; NULL: row b, one each) and lengths[b] positions in the cache, the new ones among them, so
+ * that its row i of n is position lengths[b] - n + i. table: int32 [batch][width], ldt elements from row to row; only the
+ * entries of positions below lengths[b] are read. All of these are device memory, read when the kernels run. Rows before
+ * starts[0] and behind starts[batch] are left as they are. A table entry outside the pool is reported (mq_device_status 19): its
+ * rows are not written, and read as zeros. A length below 0 or above width * page is reported (20) and cut. A position below 0
+ * (more rows than positions) is not stored, loads as zeros and sees nothing. */
+
+/* k[t][h], v[t][h] -> the pages, rounded to their type; int8 as mq_quantize_s8 makes it, row by row (a row with a NaN or an
+ * infinity: zeros and scale NaN). k, v: fp32, fp16 or bf16 (dtype), [tokens][heads][dim] with strides in elements, rows
+ * 16-byte aligned. A position that two rows name gets either's values, or a mix of the two. Keys and values, and the rows that
+ * are read, must not share memory with one another's pages. */
+MQ_API int mq_kv_store(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
+                       int dtype, const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width,
+                       const int32_t *lengths, const int32_t *starts, int64_t batch, int64_t tokens, void *stream);
+/* The other way: what the pages hold of those positions -> k, v (an int8 row times its scale), rounded once. */
+MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width, const int32_t *lengths,
+                      const int32_t *starts, int64_t batch, int64_t tokens, void *k, int64_t k_token, int64_t k_head, void *v,
+                      int64_t v_token, int64_t v_head, int dtype, void *stream);
+
+/* out[t][h] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * q[t][h].k_j), over the positions j that row t sees: its own and
+ * those before it, the last `window` of them (0: all). Query head h uses kv head h / (heads / cache->heads). q and out: fp16
+ * or bf16 (q_dtype; a 16-bit cache's own type), [tokens][heads][dim] with strides in elements, rows 16-byte aligned; out may be
+ * q's own buffer with q's strides. A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
+ * row does not see have no influence on it, whatever they hold; one that it sees and whose row holds a NaN or an infinity (int8: whose scale is one) makes
+ * it NaN or infinite. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they
+ * meet the values; an int8 cache's scales must not be negative, and a value scale below 1e-30 counts as 1e-30.
+ * max_new: no sequence has more new tokens (0: unknown); one that has is reported (26) and its rows are left as they are.
+ * scale > 0. Reproducible bit for bit. workspace: mq_paged_attention_workspace_size() bytes, 16-byte aligned (0 for sizes that
+ * are refused); calls that may overlap in time need one each. tokens == 0 does nothing. */
+MQ_API size_t mq_paged_attention_workspace_size(const mq_kv_pages *cache, int64_t heads, int64_t batch, int64_t tokens,
+                                                int64_t max_new);
+MQ_API int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, int64_t q_head, const mq_kv_pages *cache,
+                              const int32_t *table, int64_t ldt, int64_t width, const int32_t *lengths, const int32_t *starts,
+                              int64_t batch, int64_t tokens, int64_t heads, float scale, int64_t window, int64_t max_new,
+                              void *out, int64_t o_token, int64_t o_head, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
+/* ---- drafted tokens ------------------------------------------------------------------------------------------
+ * Which of a request's drafted tokens stay, so that the tokens are distributed as the target's own samples. p_i and q_i:
+ * softmax(logits / temperature[b]) of row i of the request's target rows [drafts + 1] and draft rows [drafts] (draft NULL: q_i is
+ * all on the drafted token). Token i is kept while uniform[b][i] * q_i(token) < p_i(token). At the first that is not, i = n, a token is
+ * drawn from max(p_n - q_n, 0) (where all are kept, from p_n; where nothing is left of it, from p_n): the first v whose running sum
+ * exceeds uniform[b][drafts] times the whole (sums in fp64). A temperature below 1e-5 (or NaN): p_i is all on the largest logit, the
+ * lowest index among equal ones, and the draft's logits and the uniforms do not count.
+ * tokens[b]: the kept ones, the drawn one, then -1; accepted[b] = n; logprobs[b][i] = log p_i(tokens[b][i]), 0 behind.
+ * temperature: fp32 [batch] or NULL (1). counts: int32 [batch] or NULL, how many drafts request b has (<= drafts; outside
+ * [0, drafts] reported, 25, and cut); rows behind are not read. A drafted token outside the vocabulary is reported (25) and not kept. A target row that is
+ * no distribution (a NaN, +infinity, all -infinity) is reported (24), and its request ends there with token -1; such a draft row is
+ * reported, its token is not kept and q counts as 0. Logits: fp32, fp16 or bf16, rows ld elements apart. drafts <= 32.
+ * workspace: mq_verify_workspace_size() bytes, 16-byte aligned. batch == 0 does nothing. */
+MQ_API size_t mq_verify_workspace_size(int64_t batch, int64_t drafts, int64_t vocab);
+MQ_API int mq_verify_drafts(const void *target, int64_t ld_target, const void *draft, int64_t ld_draft, int dtype,
+                            const int32_t *drafted, const int32_t *counts, const float *uniform, const float *temperature,
+                            int32_t *tokens, int32_t *accepted, float *logprobs, int64_t batch, int64_t drafts, int64_t vocab,
+                            void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- weight files -------------------------------------------------------------------------------- */
 
 /* Reads nbytes at byte `offset` of the file at `path` into device memory at dst, through two pinned

@@ -1,0 +1,666 @@
+// Attention of new tokens over a paged cache, for sequences with few rows per kv head (mq_paged_attention; many rows:
+// attn_tile.cu).
+//
+//   o[i] = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale q_i.k_j),  j over the positions that row i sees:
+//   p - window < j <= p with p the row's own position.
+//
+// The group's query heads of all of a sequence's new tokens are the rows of one product with a kv head's keys, so a
+// key or value is read once for all of them. What bounds it is the stream of keys and values; arithmetic goes to the warp-level
+// mma.m16n8k16, which has the rate for it (64 keys x 128 dim x 16 rows: 128 of them, 280 cycles, against the 1400 that
+// an SM's share of the bandwidth needs for the 16-bit rows) and takes its operands without a detour through TMEM.
+//
+//  * A producer warp brings blocks of 64 keys and values through a ring, one tiled copy per page (or part of one) and
+//    128 (int8: 64) bytes of a row, a lane each; the ring's barriers are the only ones between producer and consumers.
+//  * Four consumer warps: MT of them take 16 rows each, the others share the block's keys. Each keeps its own
+//    running maximum, sum and accumulators, in fp32, and they meet once, when an item ends.
+//  * All CTAs take equal shares of all blocks (paged.cuh), so lengths need not be known on the host and a long
+//    sequence takes as many SMs as it has work for. Parts of cut items are joined by a kernel behind this one, in a fixed
+//    order: results do not vary from run to run.
+//  * int8: k_j = s_j * integers, v_j = t_j * integers. The integers go to fp16 exactly (a byte next to 0x64 is
+//    1024 + it), the rows' q to fp16 after a power of two that its largest |q| fixes (exact but below 2^-24 of that). s_j scales
+//    the scores; t_j goes into the exponent: w_j t_j = 2^(score + log2 t_j - m) with m the maximum of that, so the
+//    weights that meet the integers are at most 2^8 whatever the scales, and the sum of w is that of (w t) (1 / t).
+//  * The maximum may lag by 2^8 before accumulators are rescaled: weights up to 2^8 are as exact in fp16 and bf16.
+//  * Blocks that some row sees only in part: scores are replaced, not added to, so no masked key's value matters; a
+//    value that is no number is taken out of the product and makes the score of its key NaN for the rows that see it.
+#include "paged.cuh"
+
+namespace mq {
+namespace paged {
+
+constexpr int kFewKeys = 64, kFewRows = 64;  // keys of a block; the most rows of an item
+constexpr int kFewWarps = 4, kFewThreads = 32 * (kFewWarps + 1);
+constexpr int kPadCols = 72;                 // floats between rows of the joining buffer: no bank conflicts
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if (BF) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&b);
+  }
+  return pack_half2(lo, hi);
+}
+// Two bytes of x (biased by 128), which SEL puts beside 0x64 each, as fp16 integers in -128 .. 127.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t x) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0x64646464u), "n"(SEL));
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&r), __half2half2(__ushort_as_half(0x6480)));  // 1152
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 0xffff in each half of x that is infinite or no number.
+template <bool BF>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
+  constexpr uint32_t e = BF ? 0x7f807f80u : 0x7c007c00u;
+  return __vcmpeq2(x & e, e);
+}
+// V scales count as at least this: their inverses and the sums of those stay finite.
+constexpr float kLeastScale = 1e-30f;
+
+struct AttnParams {
+  Seqs seqs;
+  Shape shape;
+  const void *q;
+  int64_t q_token, q_head;  // strides in elements
+  int q_dtype;
+  const float *k_scale, *v_scale;
+  int64_t ks_stride[3], vs_stride[3];
+  Output o;
+  float scale;  // times log2(e)
+  Parts parts;
+};
+
+template <typename T>
+__device__ __forceinline__ void store4(void *out, int64_t at, float a, float b, float c, float d) {
+  struct alignas(4 * sizeof(T)) Four {
+    T t[4];
+  };
+  *reinterpret_cast<Four *>(static_cast<T *>(out) + at) = Four{{T(a), T(b), T(c), T(d)}};
+}
+__device__ __forceinline__ void store_out4(const Output &o, int64_t token, int64_t head, int col, float a, float b, float c, float d) {
+  const int64_t at = token * o.token_stride + head * o.head_stride + col;
+  if (o.dtype == MQ_F16)
+    store4<__half>(o.out, at, a, b, c, d);
+  else
+    store4<__nv_bfloat16>(o.out, at, a, b, c, d);
+}
+// What a row's accumulators are multiplied by: 0 for a row that sees nothing, NaN where its sum is.
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+template <int D, int MT, int KIND>
+struct Few {
+  static constexpr int kBytes = KIND == MQ_S8 ? 1 : 2;
+  static constexpr int kBox = KIND == MQ_S8 ? 64 : 128;                 // bytes of a row in a box
+  static constexpr int kBoxes = D * kBytes / kBox;
+  static constexpr int kTile = kFewKeys * D * kBytes;                   // of keys, or of values
+  static constexpr int kScales = KIND == MQ_S8 ? 2 * kFewKeys * 4 : 0;  // of keys and of values
+  static constexpr int kStageBytes = 2 * kTile + 1024 * (kScales > 0);
+  // Two CTAs on an SM where a stage has 32 KB or a warp works on 64 keys of 128 dim (204 registers), else three; as
+  // many stages, up to four, as fit beside the joining buffer.
+  static constexpr int kCtas = kTile == 16384 || (MT == 4 && D == 128) ? 2 : 3;
+  static constexpr int kJoin = kFewRows * kPadCols * 4;
+  static constexpr int kRoom = (227 * 1024 / kCtas - 1024 - kJoin - 2048) / kStageBytes;
+  static constexpr int kStages = kRoom > 4 ? 4 : kRoom;
+  static constexpr int kSmem = kStages * kStageBytes + kJoin + 1024;
+};
+
+template <int D, int MT, int KIND>
+__global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
+    attn_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
+  using F = Few<D, MT, KIND>;
+  constexpr bool BF = KIND == MQ_BF16, S8 = KIND == MQ_S8;
+  constexpr int WK = kFewWarps / MT, KW = kFewKeys / WK;  // warps that share a block's keys; keys of a warp
+  constexpr int NT = KW / 8, S = F::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float *join = reinterpret_cast<float *>(ring + S * F::kStageBytes);  // [WK][16 MT][kPadCols]
+  __shared__ uint64_t full[S], empty[S];
+  __shared__ ShareScratch<kFewThreads> scratch;
+  __shared__ float2 row_stats[WK][16 * MT];
+  __shared__ volatile int abort_flag;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  griddep_launch_dependents();
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], S8 ? 33 : 1);  // the copies' bytes; the lanes whose scales have come
+      mbar_init(&empty[i], kFewWarps);
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  griddep_wait();
+  const Share share = find_share<kFewThreads, kFewRows, kFewKeys>(p.seqs, p.shape, scratch);
+  if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = share.total, p.parts.counts[1] = share.parts;
+  if (static_cast<int>(blockIdx.x) >= share.parts) return;
+  Walk<kFewRows, kFewKeys> walk;
+  walk.start(p.seqs, p.shape, share);
+  Item item;
+
+  if (warp == kFewWarps) {
+    if (lane == 0) {
+      prefetch_tmap(&kmap);
+      prefetch_tmap(&vmap);
+    }
+    const int box_rows = min(kFewKeys, 1 << p.seqs.page_log2), per_block = kFewKeys / box_rows;
+    const int boxes = per_block * F::kBoxes;  // of keys, and as many of values
+    int s = 0, round = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    while (ok && walk.next(p.seqs, p.shape, item)) {
+      for (int i = 0; i < item.blocks; ++i) {
+        const int key0 = (item.block + i) * kFewKeys;
+        // Boxes behind the sequence's end are not fetched: their table entries may be anything.
+        const int live = max(0, min(per_block, (item.s.length - key0 + box_rows - 1) / box_rows));
+        int page = -1;  // lane l knows the page of box l of the block
+        if (lane < live) page = page_of(p.seqs, item.b, key0 + lane * box_rows);
+        float sk[2], sv[2];  // scales of keys lane and lane + 32
+        if (S8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = lane + 32 * h, of = __shfl_sync(0xffffffffu, page, key / box_rows);
+            sk[h] = 0.f, sv[h] = 0.f;
+            if (of >= 0 && key0 + key < item.s.length) {
+              const int row = (key0 + key) & ((1 << p.seqs.page_log2) - 1);
+              sk[h] = p.k_scale[of * p.ks_stride[0] + item.head * p.ks_stride[1] + row * p.ks_stride[2]];
+              sv[h] = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
+            }
+          }
+        }
+        if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[s], (round - 1) & 1))) {
+          if (lane == 0) raise_status(kStatusAttnLoadWait), abort_flag = 1;
+          ok = false;
+          break;
+        }
+        uint8_t *stage = ring + s * F::kStageBytes;
+        if (S8) {
+          float *sc = reinterpret_cast<float *>(stage + 2 * F::kTile);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) sc[lane + 32 * h] = sk[h], sc[kFewKeys + lane + 32 * h] = sv[h];
+        }
+        if (lane == 0) mbar_expect_tx(&full[s], 2 * live * F::kBoxes * box_rows * F::kBox);
+        __syncwarp();
+        for (int base = 0; base < 2 * boxes; base += 32) {
+          const int l = base + lane, which = l / boxes, box = l % boxes, part = box / per_block, at = box % per_block;
+          const int of = __shfl_sync(0xffffffffu, page, at);
+          if (l < 2 * boxes && at < live) {
+            const int row = (key0 + at * box_rows) & ((1 << p.seqs.page_log2) - 1);
+            uint8_t *dst = stage + which * F::kTile + part * kFewKeys * F::kBox + at * box_rows * F::kBox;
+            // (a page outside the pool lies outside the map: zeros)
+            asm volatile(
+                "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(which ? &vmap : &kmap)), "r"(smem_u32(&full[s])),
+                "r"(part * (F::kBox / F::kBytes)), "r"(row), "r"(item.head), "r"(of < 0 ? p.seqs.pages : of)
+                : "memory");
+          }
+        }
+        if (S8) mbar_arrive(&full[s]);
+        ++issued;
+        if (++s == S) s = 0, ++round;
+      }
+    }
+    // Leave no copy in flight.
+    if (lane == 0)
+      for (int64_t i = issued > S ? issued - S : 0; i < issued; ++i) mbar_wait(&full[i % S], (i / S) & 1);
+    return;
+  }
+
+  const int mt = warp % MT, wk = warp / MT, g = lane / 4, t = lane % 4;
+  const int heads = p.shape.group;
+  int s = 0;
+  uint32_t phase = 0;
+  bool first_item = true;
+  while (walk.next(p.seqs, p.shape, item)) {
+    const int rows = item.s.n * heads;
+    // A thread's rows are g and g + 8 of its warp's 16; q as the MMA's A, in registers.
+    uint32_t qa[D / 16][4];
+    float row_scale[2];
+    int lo[2], hi[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = mt * 16 + g + 8 * r, i = min(row, rows - 1) / heads;
+      const int pos = item.s.pos0 + i;
+      hi[r] = max(pos + 1, 0);
+      lo[r] = p.shape.window ? max(0, pos + 1 - p.shape.window) : 0;
+      row_scale[r] = p.scale;
+      const int64_t at = static_cast<int64_t>(item.s.first + i) * p.q_token + static_cast<int64_t>(item.head * heads + row % heads) * p.q_head;
+      const bool real = row < rows;
+      if constexpr (S8) {
+        float v[D / 4];  // d = 64 h + 16 t + 0 .. 15: bytes that a 16-byte load of the keys brings to this thread
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int d = 64 * h + 16 * t + 8 * u;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (real && d < p.o.dim) w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + at + d);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float2 f;
+              if (p.q_dtype == MQ_F16)
+                f = __half22float2(*reinterpret_cast<const __half2 *>(&ws[e]));
+              else
+                f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&ws[e]));
+              v[16 * h + 8 * u + 2 * e] = f.x, v[16 * h + 8 * u + 2 * e + 1] = f.y;
+            }
+          }
+        float big = 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 4; ++e) big = fmaxf(big, fabsf(v[e]));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // 2^e with 1 <= big / 2^e < 2, from the exponent's bits (an infinite row stays one; a tiny one counts as 2^-100's).
+        const uint32_t e = min(max(__float_as_uint(big) >> 23, 27u), 227u);
+        const float up = __uint_as_float(e << 23), down = __uint_as_float((254 - e) << 23);
+        row_scale[r] *= up;
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            qa[4 * h + i4][r] = pack_half2(v[16 * h + 4 * i4] * down, v[16 * h + 4 * i4 + 1] * down);
+            qa[4 * h + i4][r + 2] = pack_half2(v[16 * h + 4 * i4 + 2] * down, v[16 * h + 4 * i4 + 3] * down);
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int d = 16 * k + 8 * u + 2 * t;
+            qa[k][r + 2 * u] = real && d < p.o.dim ? *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(p.q) + at + d) : 0u;
+          }
+      }
+    }
+    // Blocks outside [most_lo, least_hi) are seen in part by some row (rows rise with their position).
+    const int least_hi = max(item.s.pos0 + 1, 0);
+    const int most_lo = p.shape.window ? max(0, item.s.pos0 + item.s.n - p.shape.window) : 0;
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // l: this thread's columns
+
+    for (int b = 0; b < item.blocks; ++b) {
+      const bool came = !abort_flag && mbar_wait(&full[s], phase);
+      if (!__all_sync(0xffffffffu, came)) {
+        if (lane == 0 && !abort_flag) raise_status(kStatusAttnSoftmaxWait), abort_flag = 1;
+        break;
+      }
+      const uint32_t stage = smem_u32(ring + s * F::kStageBytes);
+      const float *scales = reinterpret_cast<const float *>(ring + s * F::kStageBytes + 2 * F::kTile);
+      const int key0 = (item.block + b) * kFewKeys + wk * KW;  // of this warp
+      const bool edge = key0 + KW > least_hi || key0 < most_lo;
+      float c[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[j][e] = 0.f;
+      // Scores. int8: word w of a thread's 16 bytes is its k of one step, for keys and q alike.
+      if constexpr (S8) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int key = wk * KW + 8 * j + g;
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(stage + h * kFewKeys * 64 + key * 64 + ((t ^ ((key >> 1) & 3)) * 16)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t x = w[e] ^ 0x80808080u;
+              mma16<false>(c[j], qa[4 * h + e], bytes_to_half2<0x4140>(x), bytes_to_half2<0x4342>(x));
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < NT / 2; ++j) {
+            const int key = wk * KW + 16 * j + (lane & 7) + ((lane >> 4) & 1) * 8, chunk = 2 * k + ((lane >> 3) & 1);
+            uint32_t f[4];
+            ldsm4(f, stage + (chunk / 8) * kFewKeys * 128 + key * 128 + (((chunk & 7) ^ (key & 7)) * 16));
+            mma16<BF>(c[2 * j], qa[k], f[0], f[1]);
+            mma16<BF>(c[2 * j + 1], qa[k], f[2], f[3]);
+          }
+      }
+      const uint32_t values = stage + F::kTile;
+      // 16 keys (step kk) x 16 columns (16-bit) or 32 (int8) of the values, as the MMA's B of two or four column tiles.
+      auto value_at = [&](int kk, int j, uint32_t (&f)[4]) {
+        const int key = wk * KW + 16 * kk + (lane & 7) + ((lane >> 3) & 1) * 8, chunk = 2 * j + (lane >> 4);
+        if (S8)
+          ldsm4t(f, values + (chunk / 4) * kFewKeys * 64 + key * 64 + (((chunk & 3) ^ ((key >> 1) & 3)) * 16));
+        else
+          ldsm4t(f, values + (chunk / 8) * kFewKeys * 128 + key * 128 + (((chunk & 7) ^ (key & 7)) * 16));
+      };
+      // Scaled scores, log2: of columns 8 j + 2 t + (e & 1), rows g + 8 (e >> 1).
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if (S8) {
+          const float2 ks = *reinterpret_cast<const float2 *>(scales + wk * KW + 8 * j + 2 * t);
+          float2 vs = *reinterpret_cast<const float2 *>(scales + kFewKeys + wk * KW + 8 * j + 2 * t);
+          // (fmaxf would drop a NaN)
+          vs.x = vs.x < kLeastScale ? kLeastScale : vs.x, vs.y = vs.y < kLeastScale ? kLeastScale : vs.y;
+          const float lx = lg2(vs.x), ly = lg2(vs.y);
+          c[j][0] = fmaf(c[j][0] * row_scale[0], ks.x, lx), c[j][1] = fmaf(c[j][1] * row_scale[0], ks.y, ly);
+          c[j][2] = fmaf(c[j][2] * row_scale[1], ks.x, lx), c[j][3] = fmaf(c[j][3] * row_scale[1], ks.y, ly);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[j][e] *= p.scale;
+        }
+      }
+      if (edge) {
+        if constexpr (!S8) {
+#pragma unroll
+          for (int kk = 0; kk < KW / 16; ++kk) {
+            uint32_t bad[2] = {0, 0};  // keys 2 t, 2 t + 1 and 8 more of this step
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+              uint32_t f[4];
+              value_at(kk, j, f);
+              bad[0] |= not_finite2<BF>(f[0]) | not_finite2<BF>(f[2]);
+              bad[1] |= not_finite2<BF>(f[1]) | not_finite2<BF>(f[3]);
+            }
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) {
+              bad[0] |= __shfl_xor_sync(0xffffffffu, bad[0], x);
+              bad[1] |= __shfl_xor_sync(0xffffffffu, bad[1], x);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (bad[u] >> (e & 1 ? 16 : 0) & 1) c[2 * kk + u][e] = NAN;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 8 * j + 2 * t + (e & 1);
+            if (key >= hi[e >> 1] || key < lo[e >> 1]) c[j][e] = -INFINITY;
+          }
+      }
+      float ref[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float top = fmaxf(c[0][2 * r], c[0][2 * r + 1]);
+#pragma unroll
+        for (int j = 1; j < NT; ++j) top = fmaxf(top, fmaxf(c[j][2 * r], c[j][2 * r + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const bool grows = top > m[r] + 8.f;  // (-inf + 8 is -inf)
+        if (__any_sync(0xffffffffu, grows)) {
+          const float next = grows ? top : m[r];
+          const float a = m[r] == next ? 1.f : ex2(m[r] - next);
+          l[r] *= a;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) o[j][2 * r] *= a, o[j][2 * r + 1] *= a;
+          m[r] = next;
+        }
+        ref[r] = m[r] == -INFINITY ? 0.f : m[r];
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[j][e] = ex2(c[j][e] - ref[e >> 1]);
+      if (S8) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float2 vs = *reinterpret_cast<const float2 *>(scales + kFewKeys + wk * KW + 8 * j + 2 * t);
+          const float ix = __frcp_rn(vs.x < kLeastScale ? kLeastScale : vs.x), iy = __frcp_rn(vs.y < kLeastScale ? kLeastScale : vs.y);
+          // (a masked key's scale may be anything, its weight is 0)
+          l[0] += (c[j][0] == 0.f ? 0.f : c[j][0] * ix) + (c[j][1] == 0.f ? 0.f : c[j][1] * iy);
+          l[1] += (c[j][2] == 0.f ? 0.f : c[j][2] * ix) + (c[j][3] == 0.f ? 0.f : c[j][3] * iy);
+        }
+      }
+      // Weights become the MMA's A; 16-bit caches sum them as they were rounded, so that the two roundings cancel where
+      // one key has most of the weight.
+#pragma unroll
+      for (int kk = 0; kk < KW / 16; ++kk) {
+        const uint32_t a[4] = {pack16<BF>(c[2 * kk][0], c[2 * kk][1]), pack16<BF>(c[2 * kk][2], c[2 * kk][3]),
+                               pack16<BF>(c[2 * kk + 1][0], c[2 * kk + 1][1]), pack16<BF>(c[2 * kk + 1][2], c[2 * kk + 1][3])};
+        if (!S8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float2 f;
+            if (BF)
+              f = make_float2(__uint_as_float(a[e] << 16), __uint_as_float(a[e] & 0xffff0000u));
+            else
+              f = __half22float2(*reinterpret_cast<const __half2 *>(&a[e]));
+            l[e & 1] += f.x + f.y;
+          }
+        }
+        if constexpr (S8) {
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            uint32_t f[4];
+            value_at(kk, j, f);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t x0 = f[2 * u] ^ 0x80808080u, x1 = f[2 * u + 1] ^ 0x80808080u;
+              mma16<false>(o[4 * j + 2 * u], a, bytes_to_half2<0x4240>(x0), bytes_to_half2<0x4240>(x1));
+              mma16<false>(o[4 * j + 2 * u + 1], a, bytes_to_half2<0x4341>(x0), bytes_to_half2<0x4341>(x1));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            uint32_t f[4];
+            value_at(kk, j, f);
+            if (edge)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[e] &= ~not_finite2<BF>(f[e]);
+            mma16<BF>(o[2 * j], a, f[0], f[1]);
+            mma16<BF>(o[2 * j + 1], a, f[2], f[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+      if (++s == S) s = 0, phase ^= 1;
+    }
+
+    // The warps that shared the keys join.
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (t == 0) row_stats[wk][mt * 16 + g + 8 * r] = make_float2(m[r], l[r]);
+    }
+    named_bar_sync(1, 32 * kFewWarps);
+    if (abort_flag) break;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) top = fmaxf(top, row_stats[w][mt * 16 + g + 8 * r].x);
+      const float a = m[r] == top ? 1.f : ex2(m[r] - top);
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) o[j][2 * r] *= a, o[j][2 * r + 1] *= a;
+    }
+    const bool goes_on = item.before > 0, whole = !goes_on && item.blocks == item.whole;
+    if (first_item && tid == 0) {
+      Cut cut{item.b, item.head, item.tile, goes_on, share.begin - item.before, share.begin - item.before + item.whole};
+      p.parts.cuts[blockIdx.x] = cut;
+    }
+    first_item = false;
+    const int64_t part0 = (2 * static_cast<int64_t>(blockIdx.x) + (goes_on ? 0 : 1)) * (16 * MT);
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      float *mine = join + (wk * 16 * MT + mt * 16) * kPadCols;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float *at = mine + (g + 8 * r) * kPadCols;
+        if (S8) {  // columns 16 c + 4 t + 0 .. 3 of tiles 2 c (even ones) and 2 c + 1
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const auto &ev = o[8 * h + 2 * c], &od = o[8 * h + 2 * c + 1];
+            *reinterpret_cast<float4 *>(at + 16 * c + 4 * t) = make_float4(ev[2 * r], od[2 * r], ev[2 * r + 1], od[2 * r + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float2 *>(at + 8 * c + 2 * t) = make_float2(o[8 * h + c][2 * r], o[8 * h + c][2 * r + 1]);
+        }
+      }
+      named_bar_sync(1, 32 * kFewWarps);
+      for (int e = tid; e < 16 * MT * 16; e += 32 * kFewWarps) {
+        const int row = e / 16, col = e % 16 * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float4 x = *reinterpret_cast<const float4 *>(join + (w * 16 * MT + row) * kPadCols + col);
+          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+          top = fmaxf(top, row_stats[w][row].x);
+        }
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float2 st = row_stats[w][row];
+          sum += st.x == top ? st.y : st.y * ex2(st.x - top);
+        }
+        if (row < rows) {
+          if (whole) {
+            const float inv = inverse_sum(sum);
+            if (64 * h + col < p.o.dim)
+              store_out4(p.o, item.s.first + row / heads, item.head * heads + row % heads, 64 * h + col, v.x * inv, v.y * inv, v.z * inv,
+                         v.w * inv);
+          } else {
+            *reinterpret_cast<float4 *>(p.parts.sums + (part0 + row) * D + 64 * h + col) = v;
+            if (h == 0 && col == 0) p.parts.stats[part0 + row] = make_float2(top, sum);
+          }
+        }
+      }
+      named_bar_sync(1, 32 * kFewWarps);
+    }
+  }
+}
+
+// Joins the parts of the items that CTAs of the launch before shared. CTA c (of x) takes the item that c goes on with
+// where c is the first to do so; y: 16 rows each.
+struct JoinParams {
+  Seqs seqs;
+  Shape shape;
+  Output o;
+  Parts parts;
+  int rows;  // of an item's parts
+};
+template <int D, int TILE_ROWS>
+__global__ void __launch_bounds__(128) attn_join_kernel(const JoinParams p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int64_t total = p.parts.counts[0], ctas = p.parts.counts[1];
+  const int c = blockIdx.x;
+  if (c == 0 || c >= ctas) return;
+  const Cut cut = p.parts.cuts[c];
+  if (!cut.goes_on || total * (c - 1) / ctas > cut.first) return;
+  const Seq s = sequence(p.seqs, cut.b);
+  const int rows = min(TILE_ROWS, s.n * p.shape.group - cut.tile * TILE_ROWS);
+  const int row = blockIdx.y * 16 + threadIdx.x / 8, u = threadIdx.x % 8;
+  if (static_cast<int>(blockIdx.y) * 16 >= rows) return;
+  int last = c;  // the item's last CTA
+  while (last + 1 < ctas && total * (last + 1) / ctas < cut.end) ++last;
+  const int from = row < rows ? row : 0;
+  // Part 0 is CTA c - 1's, which began the item (its slot 1), the others what CTAs c .. last went on with (slot 0).
+  const int n = last - c + 2;
+  auto at = [&](int i) { return (2 * static_cast<int64_t>(c - 1 + i) + (i == 0 ? 1 : 0)) * p.rows + from; };
+  float top = -INFINITY;
+  for (int i = u; i < n; i += 8) top = fmaxf(top, p.parts.stats[at(i)].x);
+#pragma unroll
+  for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  float sum = 0.f;
+  float4 v[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const int64_t a = at(i);
+    const float2 st = p.parts.stats[a];
+    const float w = st.x == top ? 1.f : ex2(st.x - top);
+    sum += st.y * w;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      const float4 x = *reinterpret_cast<const float4 *>(p.parts.sums + a * D + (k * 8 + u) * 4);
+      v[k].x += x.x * w, v[k].y += x.y * w, v[k].z += x.z * w, v[k].w += x.w * w;
+    }
+  }
+  if (row >= rows) return;
+  const float inv = inverse_sum(sum);
+  const int r = cut.tile * TILE_ROWS + row;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k)
+    if ((k * 8 + u) * 4 < p.o.dim)
+      store_out4(p.o, s.first + r / p.shape.group, cut.head * p.shape.group + r % p.shape.group, (k * 8 + u) * 4, v[k].x * inv,
+                 v[k].y * inv, v[k].z * inv, v[k].w * inv);
+}
+
+// A map of a pool's rows: (dim, row of the page, head, page), boxes of `box_bytes` of `box_rows` rows.
+inline int encode_pages(CUtensorMap *map, void *base, int dtype, const mq_kv_pages *c, const int64_t *stride, int box_bytes,
+                        int box_rows, CUtensorMapSwizzle swizzle, const char *what) {
+  const int es = element_size(dtype);
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->dim), static_cast<cuuint64_t>(c->page), static_cast<cuuint64_t>(c->heads),
+                              static_cast<cuuint64_t>(c->pages)};
+  // (a stride is not used where its dimension has one index, and may then be anything)
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 16 : static_cast<cuuint64_t>(stride[2 - i]) * es;
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(box_bytes / es), static_cast<cuuint32_t>(box_rows), 1, 1};
+  return encode_tmap_4d(map, base, dtype == MQ_S8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : dtype == MQ_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        dims, strides, box, swizzle, what);
+}
+
+template <int D, int MT, int KIND>
+int launch_few(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, cudaStream_t stream, const char *what) {
+  using F = Few<D, MT, KIND>;
+  CUtensorMap kmap, vmap;
+  const int box_rows = std::min(kFewKeys, c->page);
+  const CUtensorMapSwizzle swizzle = KIND == MQ_S8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  if (int rc = encode_pages(&kmap, c->k, KIND, c, c->k_stride, F::kBox, box_rows, swizzle, what)) return rc;
+  if (int rc = encode_pages(&vmap, c->v, KIND, c, c->v_stride, F::kBox, box_rows, swizzle, what)) return rc;
+  p.parts = parts_at(workspace, ctas, 16 * MT);
+  static size_t configured[64] = {};
+  auto kern = attn_few_kernel<D, MT, KIND>;
+  if (int rc = ensure_smem(kern, F::kSmem, configured, what)) return rc;
+  if (int rc = launch_overlapped(kern, dim3(ctas), dim3(kFewThreads), F::kSmem, stream, what, kmap, vmap, p)) return rc;
+  JoinParams j{p.seqs, p.shape, p.o, p.parts, 16 * MT};
+  return launch_overlapped(attn_join_kernel<D, kFewRows>, dim3(ctas, MT), dim3(128), 0, stream, what, j);
+}
+
+}  // namespace paged
+}  // namespace mq

@@ -1,0 +1,660 @@
+// Attention of new tokens over a paged cache, for sequences with many rows per kv head: 256 rows of an item on one SM's
+// tensor core (see attn.cu for the operator, paged.cuh for items and shares).
+//
+//  * Two tiles of 128 rows take turns: while the softmax of one runs, the MMAs of the other do. S = Q K^T (M = 128 rows,
+//    N = 128 keys) lands in TMEM, a thread of the tile's softmax warps reads its row from there, writes the
+//    weights back over it as 16-bit values, and they are the A operand of O += P V from TMEM. O stays in TMEM, and is
+//    rescaled there only when a row's maximum has grown by 2^8 since the last time.
+//  * V is used as it lies, [keys][dim], as an MN-major B operand: nothing is transposed.
+//  * Warps 0-3 and 4-7: softmax and output of the two tiles. Warp 8: the copies of keys and values, a lane per page (or part
+//    of one) and 128 bytes of row. Warp 9: one thread issues the MMAs. Warps 10 and 11: bring q, and stand
+//    between the copies and the MMAs: of an int8 cache they make fp16 of every block; of a 16-bit one they take what is
+//    no number out of the values of the blocks that some row sees only in part, and say which keys had any.
+//  * One persistent CTA per SM, all of TMEM, equal shares of the blocks: causal or ragged, no SM waits for another.
+#include "paged.cuh"
+
+namespace mq {
+namespace paged {
+
+constexpr int kTileKeys = 128, kTileRows = 256;
+constexpr int kTileThreads = 384, kAuxWarps = 2;
+
+template <int D, int KIND>
+struct Tile {
+  static constexpr bool kS8 = KIND == MQ_S8;
+  static constexpr int kBlock = kTileKeys * D * 2;          // of keys or values, as operands
+  static constexpr int kSlots = kS8 ? 3 : 4;                // keys and values in turn
+  static constexpr int kRaw = kS8 ? kTileKeys * D : 0;      // int8 as it was copied, two of them
+  static constexpr int kQ = kTileRows * D * 2;
+  // All of shared memory, since it takes all of TMEM: no other CTA that wants TMEM then fits beside it.
+  static constexpr int kSmem = 220 * 1024;
+  static_assert(kQ + kSlots * kBlock + 2 * kRaw + 1024 <= kSmem, "shared memory");
+};
+
+// Row-major rows of 128 bytes, 128 of them to a 64-column part: where 16-byte chunk c of row r lies.
+__device__ __forceinline__ int swizzled(int r, int c) { return (c >> 3) * 16384 + r * 128 + ((c ^ r) & 7) * 16; }
+
+// The MN-major descriptor of a [keys][dim] block: 64 columns of 128 bytes, 8-key atoms 1024 bytes apart (stride
+// offset), the next 64 columns 16 KB on (leading offset).
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(16384 >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+constexpr uint32_t idesc_16(int m, int n, bool bf, bool b_mn) {
+  return umma_idesc_f16(m, n) | (bf ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+// 32 columns, without the wait; tmem_loaded() stands between the wait and their use.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_loaded(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 16)
+    asm volatile(""
+                 : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]),
+                   "+f"(v[i + 7]), "+f"(v[i + 8]), "+f"(v[i + 9]), "+f"(v[i + 10]), "+f"(v[i + 11]), "+f"(v[i + 12]),
+                   "+f"(v[i + 13]), "+f"(v[i + 14]), "+f"(v[i + 15]));
+}
+
+template <int D, int KIND>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    attn_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
+  using T = Tile<D, KIND>;
+  constexpr bool BF = KIND == MQ_BF16, S8 = T::kS8;
+  constexpr int NS = T::kSlots, NF = S8 ? 2 : NS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock;
+  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full, q_empty, drained, s_full[2], p_full[2], o_full[2];
+  __shared__ ShareScratch<kTileThreads> scratch;
+  __shared__ uint32_t bad_keys[NS][4];
+  __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  if (tid == 0) {
+    for (int i = 0; i < NF; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&raw_empty[i], kAuxWarps);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&ready[i], kAuxWarps);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&q_full, kAuxWarps);
+    mbar_init(&q_empty, 1);
+    mbar_init(&drained, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  griddep_wait();  // (before TMEM is taken: the kernels before this one have returned theirs)
+  if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_launch_dependents();
+  const uint32_t tmem = tmem_slot;
+  const Share share = find_share<kTileThreads, kTileRows, kTileKeys>(p.seqs, p.shape, scratch);
+  if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = share.total, p.parts.counts[1] = share.parts;
+  const bool works = static_cast<int>(blockIdx.x) < share.parts;
+  const int group = p.shape.group;
+  Walk<kTileRows, kTileKeys> walk;
+  Item item;
+  if (works) walk.start(p.seqs, p.shape, share);
+  // Waits that give up set the flag, and everybody leaves at the next wait.
+  auto wait = [&](uint64_t *bar, uint32_t parity, int code) -> bool {
+    if (!abort_flag && mbar_wait(bar, parity)) return true;
+    if (!abort_flag) raise_status(code), abort_flag = 1;
+    return false;
+  };
+  auto warp_wait = [&](uint64_t *bar, uint32_t parity, int code) -> bool {
+    return __all_sync(0xffffffffu, wait(bar, parity, code));
+  };
+  // Rows of an item's two tiles; whether some row of the item sees a block only in part.
+  auto rows_of = [&](const Item &it) { return min(kTileRows, it.s.n * group - it.tile * kTileRows); };
+  auto least_hi = [&](const Item &it) { return max(it.s.pos0 + it.tile * kTileRows / group + 1, 0); };
+  auto most_lo = [&](const Item &it) {
+    return p.shape.window ? max(0, it.s.pos0 + (it.tile * kTileRows + rows_of(it) - 1) / group + 1 - p.shape.window) : 0;
+  };
+
+  if (!works) {
+  } else if (warp == 8) {
+    if (lane == 0) {
+      prefetch_tmap(&kmap);
+      prefetch_tmap(&vmap);
+    }
+    constexpr int kBox = S8 ? D : 128, kBoxes = S8 ? 1 : D / 64;  // bytes of a row in a box, boxes of a row
+    const int page = 1 << p.seqs.page_log2, box_rows = min(kTileKeys, page), per_block = kTileKeys / box_rows;
+    int64_t issued = 0;
+    bool ok = true;
+    while (ok && walk.next(p.seqs, p.shape, item)) {
+      for (int i = 0; ok && i < item.blocks; ++i) {
+        const int key0 = (item.block + i) * kTileKeys;
+        // Boxes behind the sequence's end are not fetched: their table entries may be anything.
+        const int live = max(0, min(per_block, (item.s.length - key0 + box_rows - 1) / box_rows));
+        int id = p.seqs.pages;  // (outside the map: zeros)
+        if (lane < live) {
+          const int of = page_of(p.seqs, item.b, key0 + lane * box_rows);
+          if (of >= 0) id = of;
+        }
+        for (int which = 0; which < 2; ++which) {
+          const int slot = static_cast<int>(issued % NF);
+          const int64_t round = issued / NF;
+          if (round > 0 && !warp_wait(S8 ? &raw_empty[slot] : &empty[slot], (round - 1) & 1, kStatusAttnLoadWait)) {
+            ok = false;
+            break;
+          }
+          uint8_t *dst = S8 ? raw + slot * T::kRaw : ring + slot * T::kBlock;
+          if (lane == 0) mbar_expect_tx(&full[slot], live * box_rows * kBox * kBoxes);
+          __syncwarp();
+          const int part = lane / per_block, at = lane % per_block;  // (at most 8 x 2 boxes)
+          const int of = __shfl_sync(0xffffffffu, id, at);
+          if (part < kBoxes && at < live)
+            asm volatile(
+                "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                ::"r"(smem_u32(dst + part * 16384 + at * box_rows * kBox)), "l"(reinterpret_cast<uint64_t>(which ? &vmap : &kmap)),
+                "r"(smem_u32(&full[slot])), "r"(part * 64), "r"((key0 + at * box_rows) & (page - 1)), "r"(item.head), "r"(of)
+                : "memory");
+          ++issued;
+        }
+      }
+    }
+    // Leave no copy in flight.
+    if (lane == 0)
+      for (int64_t i = issued > NF ? issued - NF : 0; i < issued; ++i) mbar_wait(&full[i % NF], (i / NF) & 1);
+  } else if (warp == 9) {
+    if (lane == 0) {
+      constexpr uint32_t qk = idesc_16(128, kTileKeys, BF, false), pv = idesc_16(128, D, BF, true);
+      int64_t n = 0;  // slots used: keys and values in turn
+      int items = 0;
+      uint32_t p_phase[2] = {0, 0};
+      bool ok = true;
+      auto slot_of = [&](int64_t i) { return static_cast<int>(i % NS); };
+      auto scores = [&](int g, int slot) {
+        const uint32_t a = smem_u32(q_tile) + g * (T::kQ / 2), b = smem_u32(ring + slot * T::kBlock);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16(tmem + g * 128, umma_desc_sw128(a + (k / 4) * 16384) + 2 * (k % 4), umma_desc_sw128(b + (k / 4) * 16384) + 2 * (k % 4),
+                   qk, k != 0);
+        umma_commit(&s_full[g]);
+      };
+      auto values = [&](int g, int slot, bool first) {
+        const uint64_t b = umma_desc_mn128(smem_u32(ring + slot * T::kBlock));
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k)
+          umma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, b + k * (2048 >> 4), pv, !first || k != 0);
+      };
+      while (ok && walk.next(p.seqs, p.shape, item)) {
+        const int tiles = rows_of(item) > 128 ? 2 : 1;
+        ok = wait(&q_full, items & 1, kStatusAttnMmaWait) && wait(&ready[slot_of(n)], (n / NS) & 1, kStatusAttnMmaWait);
+        if (!ok) break;
+        tc_fence_after();
+        for (int g = 0; g < tiles; ++g) scores(g, slot_of(n));
+        umma_commit(&empty[slot_of(n)]);
+        if (item.blocks == 1) umma_commit(&q_empty);
+        for (int j = 0; ok && j < item.blocks; ++j, n += 2) {
+          const bool more = j + 1 < item.blocks;
+          const int64_t v = n + 1, k = n + 2;
+          ok = wait(&ready[slot_of(v)], (v / NS) & 1, kStatusAttnMmaWait);
+          for (int g = 0; ok && g < tiles; ++g) {
+            ok = wait(&p_full[g], p_phase[g], kStatusAttnMmaWait);
+            if (!ok) break;
+            p_phase[g] ^= 1;
+            tc_fence_after();
+            values(g, slot_of(v), j == 0);
+            if (g == tiles - 1) umma_commit(&empty[slot_of(v)]);
+            if (more) {
+              if (g == 0 && !(ok = wait(&ready[slot_of(k)], (k / NS) & 1, kStatusAttnMmaWait))) break;
+              tc_fence_after();
+              scores(g, slot_of(k));
+            } else {
+              umma_commit(&o_full[g]);
+            }
+          }
+          if (ok && more) {
+            umma_commit(&empty[slot_of(k)]);
+            if (j + 2 == item.blocks) umma_commit(&q_empty);
+          }
+        }
+        ++items;
+      }
+      if (!ok) {  // what was issued ends before TMEM goes
+        umma_commit(&drained);
+        mbar_wait(&drained, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 10) {
+    const int at = tid - 320;  // 0 .. 63
+    int64_t n = 0;
+    int items = 0;
+    bool ok = true;
+    while (ok && walk.next(p.seqs, p.shape, item)) {
+      const int rows = rows_of(item), row0 = item.tile * kTileRows;
+      if (items > 0 && !warp_wait(&q_empty, (items - 1) & 1, kStatusAttnLoadWait)) break;
+      auto q_row = [&](int row) {
+        const int r = row0 + row, i = r / group;
+        return static_cast<const uint16_t *>(p.q) + static_cast<int64_t>(item.s.first + i) * p.q_token +
+               static_cast<int64_t>(item.head * group + (r - i * group)) * p.q_head;
+      };
+      if constexpr (S8) {
+        for (int row = at; row < kTileRows; row += 64) {
+          uint4 w[D / 8];
+          const uint16_t *src = q_row(min(row, rows - 1));
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            w[c] = row < rows && 8 * c < p.o.dim ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+          uint32_t big = 0;  // the largest |q|'s bits, of either half
+          const uint32_t *x = reinterpret_cast<const uint32_t *>(w);
+#pragma unroll
+          for (int e = 0; e < D / 2; ++e) big = __vmaxu2(big, x[e] & 0x7fff7fffu);
+          const uint16_t top = static_cast<uint16_t>(max(big & 0xffff, big >> 16));
+          const bool f16 = p.q_dtype == MQ_F16;
+          const float most = f16 ? __half2float(__ushort_as_half(top)) : __uint_as_float(static_cast<uint32_t>(top) << 16);
+          const uint32_t e2 = min(max(__float_as_uint(most) >> 23, 27u), 227u);
+          const float down = __uint_as_float((254 - e2) << 23);
+          row_factor[items & 1][row] = __uint_as_float(e2 << 23) * p.scale;
+          uint8_t *dst = q_tile + (row / 128) * (T::kQ / 2);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t y = x[4 * c + e];
+              const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2 *>(&y))
+                                   : make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u));
+              o[e] = pack_half2(f.x * down, f.y * down);
+            }
+            *reinterpret_cast<uint4 *>(dst + swizzled(row % 128, c)) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+      } else {
+        for (int e = at; e < kTileRows * (D / 8); e += 64) {
+          const int row = e / (D / 8), c = e % (D / 8);
+          const bool real = row < rows && 8 * c < p.o.dim;
+          const uint16_t *src = q_row(min(row, rows - 1)) + (real ? 8 * c : 0);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           smem_u32(q_tile + (row / 128) * (T::kQ / 2) + swizzled(row % 128, c))),
+                       "l"(src), "r"(real ? 16 : 0)
+                       : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+      ++items;
+
+      const int part_hi = least_hi(item), part_lo = most_lo(item);
+      for (int j = 0; ok && j < item.blocks; ++j) {
+        const int key0 = (item.block + j) * kTileKeys;
+        float sk[2], sv[2];
+        if (S8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = key0 + at + 64 * h;
+            sk[h] = sv[h] = 0.f;
+            if (key < item.s.length) {
+              const int of = page_of(p.seqs, item.b, key), row = key & ((1 << p.seqs.page_log2) - 1);
+              if (of >= 0) {
+                sk[h] = p.k_scale[of * p.ks_stride[0] + item.head * p.ks_stride[1] + row * p.ks_stride[2]];
+                sv[h] = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
+              }
+            }
+          }
+        }
+        for (int which = 0; which < 2; ++which, ++n) {
+          const int src = static_cast<int>(n % NF), slot = static_cast<int>(n % NS);
+          ok = warp_wait(&full[src], (n / NF) & 1, kStatusAttnLoadWait);
+          if (ok && S8 && n >= NS) ok = warp_wait(&empty[slot], (n / NS - 1) & 1, kStatusAttnLoadWait);
+          if (!ok) break;
+          uint8_t *dst = ring + slot * T::kBlock;
+          if constexpr (S8) {
+            const uint8_t *from = raw + src * T::kRaw;
+            for (int h = 0; h < 2; ++h) {
+              const int r = at + 64 * h;
+              uint4 w[D / 16];
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c)
+                w[c] = *reinterpret_cast<const uint4 *>(from + (D == 128 ? r * 128 + ((c ^ r) & 7) * 16 : r * 64 + ((c ^ (r >> 1)) & 3) * 16));
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                const uint32_t x[4] = {w[c].x ^ 0x80808080u, w[c].y ^ 0x80808080u, w[c].z ^ 0x80808080u, w[c].w ^ 0x80808080u};
+                uint32_t o[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[2 * e] = bytes_to_half2<0x4140>(x[e]), o[2 * e + 1] = bytes_to_half2<0x4342>(x[e]);
+                *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+              }
+              if (which == 0) {
+                // (the softmax has read block n / 2 - 2's by now: the slot just waited for came behind its weights)
+                const float vs = sv[h] < kLeastScale ? kLeastScale : sv[h];
+                float (&sc)[3][S8 ? kTileKeys : 1] = scales[(n >> 1) & 1];
+                sc[0][r] = sk[h], sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&raw_empty[src]);
+          } else if (which == 1 && (key0 + kTileKeys > part_hi || key0 < part_lo)) {
+            for (int h = 0; h < 2; ++h) {
+              const int r = at + 64 * h;
+              bool bad = false;
+              const bool gone = key0 + r >= item.s.length;  // what lies there was never copied, or is another's
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c) {
+                uint4 *v = reinterpret_cast<uint4 *>(dst + swizzled(r, c));
+                uint4 x = *v;
+                const uint4 m = {not_finite2<BF>(x.x), not_finite2<BF>(x.y), not_finite2<BF>(x.z), not_finite2<BF>(x.w)};
+                if (m.x | m.y | m.z | m.w) {
+                  bad = true;
+                  x.x &= ~m.x, x.y &= ~m.y, x.z &= ~m.z, x.w &= ~m.w;
+                  *v = x;
+                }
+              }
+              const uint32_t bits = __ballot_sync(0xffffffffu, bad && !gone);
+              if (lane == 0) bad_keys[slot][(warp - 10) + 2 * h] = bits;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&ready[slot]);
+        }
+      }
+    }
+  } else {
+    const int g = warp / 4, r = tid % 128;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + g * 128, o_at = tmem + lanes + 256 + g * D;
+    int64_t n = 0;
+    int items = -1;
+    uint32_t s_phase = 0, o_phase = 0;
+    bool ok = true;
+    while (ok && walk.next(p.seqs, p.shape, item)) {
+      ++items;
+      const int rows = rows_of(item), row = g * 128 + r;
+      const bool goes_on = item.before > 0, whole = !goes_on && item.blocks == item.whole;
+      if (items == 0 && tid == 0)
+        p.parts.cuts[blockIdx.x] = Cut{item.b, item.head, item.tile, goes_on, share.begin - item.before, share.begin - item.before + item.whole};
+      if (rows <= g * 128) {  // the item has no second tile
+        n += 2 * item.blocks;
+        continue;
+      }
+      const int index = item.tile * kTileRows + min(row, rows - 1), i = index / group;
+      const int hi = row < rows ? max(item.s.pos0 + i + 1, 0) : 0;
+      const int lo = p.shape.window ? max(0, item.s.pos0 + i + 1 - p.shape.window) : 0;
+      const int part_hi = least_hi(item), part_lo = most_lo(item);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < item.blocks; ++j, n += 2) {
+        const int key0 = (item.block + j) * kTileKeys;
+        ok = warp_wait(&s_full[g], s_phase, kStatusAttnSoftmaxWait);
+        if (!ok) break;
+        s_phase ^= 1;
+        tc_fence_after();
+        float v[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_async(s_at + 32 * c, v[c]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_loaded(v[c]);
+        float scale = p.scale;
+        if constexpr (S8) {
+          scale = 1.f;
+          const float factor = row_factor[items & 1][row];
+          const float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][32 * c + e]), l4 = *reinterpret_cast<const float4 *>(&sc[1][32 * c + e]);
+              v[c][e] = fmaf(v[c][e] * factor, k4.x, l4.x), v[c][e + 1] = fmaf(v[c][e + 1] * factor, k4.y, l4.y);
+              v[c][e + 2] = fmaf(v[c][e + 2] * factor, k4.z, l4.z), v[c][e + 3] = fmaf(v[c][e + 3] * factor, k4.w, l4.w);
+            }
+        }
+        if (key0 + kTileKeys > part_hi || key0 < part_lo) {
+          if constexpr (!S8) {
+            const int slot = static_cast<int>((n + 1) % NS);
+            ok = warp_wait(&ready[slot], ((n + 1) / NS) & 1, kStatusAttnSoftmaxWait);
+            if (!ok) break;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t bits = bad_keys[slot][c];
+              if (bits)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (bits >> e & 1) v[c][e] = NAN;
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (key0 + 32 * c + e >= hi || key0 + 32 * c + e < lo) v[c][e] = -INFINITY;
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = v[c][0];
+#pragma unroll
+          for (int e = 1; e < 32; ++e) top[c] = fmaxf(top[c], v[c][e]);
+        }
+        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+        const bool grows = most > m + 8.f;
+        if (__any_sync(0xffffffffu, grows)) {
+          const float next = grows ? most : m;
+          const float a = m == next ? 1.f : ex2(m - next);
+          l *= a;
+          m = next;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              tmem_ld32(o_at + c, o);
+              uint32_t w[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * a);
+              tmem_st32(o_at + c, w);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float a = ex2(fmaf(v[c][e], scale, -ref)), b = ex2(fmaf(v[c][e + 1], scale, -ref));
+            w[e / 2] = pack16<BF>(a, b);
+            if constexpr (S8) {
+              const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][32 * c + e]);
+              l += (a == 0.f ? 0.f : a * iv.x) + (b == 0.f ? 0.f : b * iv.y);
+            } else if (BF) {  // as they were rounded: the roundings cancel where one key has most of the weight
+              l += __uint_as_float(w[e / 2] << 16) + __uint_as_float(w[e / 2] & 0xffff0000u);
+            } else {
+              l += a + b;
+            }
+          }
+          tmem_st16(s_at + 16 * c, w);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
+      }
+      if (!ok) break;
+      ok = warp_wait(&o_full[g], o_phase, kStatusAttnSoftmaxWait);
+      if (!ok) break;
+      o_phase ^= 1;
+      tc_fence_after();
+      const float inv = whole ? inverse_sum(l) : 1.f;
+      const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (goes_on ? 0 : 1)) * kTileRows + row;
+      if (!whole && row < rows) p.parts.stats[part] = make_float2(m, l);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        tmem_ld32(o_at + c, o);
+        if (row < rows) {
+          if (whole) {
+            const int64_t at = static_cast<int64_t>(item.s.first + i) * p.o.token_stride +
+                               static_cast<int64_t>(item.head * group + (index - i * group)) * p.o.head_stride + c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                w[u] = p.o.dtype == MQ_F16 ? pack16<false>(o[e + 2 * u] * inv, o[e + 2 * u + 1] * inv)
+                                           : pack16<true>(o[e + 2 * u] * inv, o[e + 2 * u + 1] * inv);
+              if (c + e < p.o.dim) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.o.out) + at + e) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4 *>(p.parts.sums + part * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, int KIND>
+int launch_tile(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, cudaStream_t stream, const char *what) {
+  using T = Tile<D, KIND>;
+  CUtensorMap kmap, vmap;
+  const int box_rows = std::min(kTileKeys, c->page), box = KIND == MQ_S8 ? D : 128;
+  const CUtensorMapSwizzle swizzle = box == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  if (int rc = encode_pages(&kmap, c->k, KIND, c, c->k_stride, box, box_rows, swizzle, what)) return rc;
+  if (int rc = encode_pages(&vmap, c->v, KIND, c, c->v_stride, box, box_rows, swizzle, what)) return rc;
+  p.parts = parts_at(workspace, ctas, kTileRows);
+  static size_t configured[64] = {};
+  auto kern = attn_tile_kernel<D, KIND>;
+  if (int rc = ensure_smem(kern, T::kSmem, configured, what)) return rc;
+  if (int rc = launch_overlapped(kern, dim3(ctas), dim3(kTileThreads), T::kSmem, stream, what, kmap, vmap, p)) return rc;
+  JoinParams j{p.seqs, p.shape, p.o, p.parts, kTileRows};
+  return launch_overlapped(attn_join_kernel<D, kTileRows>, dim3(ctas, kTileRows / 16), dim3(128), 0, stream, what, j);
+}
+
+// The rows of a kv head above which a sequence goes to the tensor core's tiles; at most kFewRows.
+constexpr int kRowsForTiles = kFewRows;
+
+struct Plan {
+  int few, few_ctas, tile_ctas;  // few: 16-row tiles per item, 0 without that launch; tile_ctas: 0 without that launch
+  int d, most_rows;
+  size_t bytes;
+};
+// Which launches a call needs: sequences may have from one to max_new new tokens.
+inline int plan_for(Plan *plan, const mq_kv_pages *c, int64_t heads, int64_t batch, int64_t tokens, int64_t max_new, int starts,
+                    int sms, const char *what) {
+  const int64_t group = heads / c->heads;
+  MQ_REQUIRE(tokens * group < (1LL << 31) - 512, MQ_EUNSUPPORTED, "%s: too many rows", what);
+  int64_t most = starts ? std::min(tokens, max_new > 0 ? max_new : tokens) : 1;
+  plan->most_rows = static_cast<int>(most * group);
+  plan->d = c->dim <= 64 ? 64 : 128;
+  plan->few = group > kRowsForTiles ? 0 : plan->most_rows <= 16 ? 1 : plan->most_rows <= 32 ? 2 : 4;
+  // One sequence has all the tokens.
+  if (batch == 1 && tokens * group > kRowsForTiles && most == tokens) plan->few = 0;
+  const bool tile = plan->most_rows > kRowsForTiles || plan->few == 0;
+  plan->few_ctas = plan->few == 0 ? 0 : sms * (c->dtype != MQ_S8 && plan->d == 128 ? 2 : plan->few == 4 && plan->d == 128 ? 2 : 3);
+  plan->tile_ctas = tile ? sms : 0;
+  plan->bytes = 0;
+  if (plan->few) plan->bytes = parts_bytes(plan->few_ctas, 16 * plan->few, plan->d);
+  if (tile) plan->bytes = std::max(plan->bytes, parts_bytes(sms, kTileRows, plan->d));
+  return MQ_OK;
+}
+
+template <int D, int KIND>
+int launch_attention(const Plan &plan, const mq_kv_pages *c, AttnParams p, void *workspace, cudaStream_t s, const char *what) {
+  p.shape.rows_most = plan.most_rows;
+  if (plan.few) {
+    p.shape.rows_from = 0, p.shape.rows_to = std::min(kRowsForTiles, 16 * plan.few);
+    int rc;
+    if (plan.few == 1)
+      rc = launch_few<D, 1, KIND>(c, p, plan.few_ctas, workspace, s, what);
+    else if (plan.few == 2)
+      rc = launch_few<D, 2, KIND>(c, p, plan.few_ctas, workspace, s, what);
+    else
+      rc = launch_few<D, 4, KIND>(c, p, plan.few_ctas, workspace, s, what);
+    if (rc) return rc;
+  }
+  if (plan.tile_ctas) {
+    p.shape.rows_from = plan.few ? kRowsForTiles : 0, p.shape.rows_to = plan.most_rows;
+    return launch_tile<D, KIND>(c, p, plan.tile_ctas, workspace, s, what);
+  }
+  return MQ_OK;
+}
+
+}  // namespace paged
+}  // namespace mq
+
+extern "C" size_t mq_paged_attention_workspace_size(const mq_kv_pages *cache, int64_t heads, int64_t batch, int64_t tokens,
+                                                    int64_t max_new) {
+  using namespace mq::paged;
+  if (check_cache(cache, "mq_paged_attention_workspace_size") || heads <= 0 || heads % cache->heads || heads > 65535 || batch <= 0 ||
+      tokens <= 0 || tokens >= (1LL << 30))
+    return 0;
+  mq::DeviceInfo dev;
+  if (mq::device_info(&dev)) return 0;
+  Plan plan;
+  if (plan_for(&plan, cache, heads, batch, tokens, max_new, 1, dev.sms, "mq_paged_attention_workspace_size")) return 0;
+  return plan.bytes;
+}
+
+extern "C" int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, int64_t q_head, const mq_kv_pages *cache,
+                                  const int32_t *table, int64_t ldt, int64_t width, const int32_t *lengths,
+                                  const int32_t *starts, int64_t batch, int64_t tokens, int64_t heads, float scale, int64_t window,
+                                  int64_t max_new, void *out, int64_t o_token, int64_t o_head, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
+  using namespace mq::paged;
+  const char *what = "mq_paged_attention";
+  if (int rc = check_cache(cache, what)) return rc;
+  AttnParams p{};
+  if (int rc = check_seqs(&p.seqs, cache, table, ldt, width, lengths, starts, batch, tokens, what)) return rc;
+  MQ_REQUIRE(heads > 0 && heads % cache->heads == 0, MQ_EINVAL, "%s: the heads must be a multiple of the cache's", what);
+  MQ_REQUIRE(heads <= 65535, MQ_EUNSUPPORTED, "%s: too many heads", what);
+  MQ_REQUIRE(q_dtype == MQ_F16 || q_dtype == MQ_BF16, MQ_EINVAL, "%s: q must be MQ_F16 or MQ_BF16", what);
+  MQ_REQUIRE(cache->dtype == MQ_S8 || cache->dtype == q_dtype, MQ_EINVAL, "%s: q must have the type of a 16-bit cache", what);
+  MQ_REQUIRE(scale > 0.f && scale < INFINITY, MQ_EINVAL, "%s: the scale must be positive and finite", what);
+  MQ_REQUIRE(window >= 0 && max_new >= 0, MQ_EINVAL, "%s: bad window or number of new tokens", what);
+  MQ_REQUIRE(window <= (1 << 30), MQ_EUNSUPPORTED, "%s: the window is above 2^30", what);
+  if (batch == 0 || tokens == 0) return MQ_OK;
+  if (int rc = check_rows(q, q_dtype, q_token, q_head, "q", what)) return rc;
+  if (int rc = check_rows_out(out, q_dtype, tokens, heads, cache->dim, o_token, o_head, "out", what)) return rc;
+  mq::DeviceInfo dev;
+  if (int rc = mq::device_info(&dev)) return rc;
+  Plan plan;
+  if (int rc = plan_for(&plan, cache, heads, batch, tokens, max_new, starts != nullptr, dev.sms, what)) return rc;
+  MQ_REQUIRE(workspace && mq::aligned(workspace, 16), MQ_EALIGN, "%s: the workspace must be 16-byte aligned", what);
+  MQ_REQUIRE(workspace_bytes >= plan.bytes, MQ_EINVAL, "%s: the workspace is too small", what);
+  p.shape.group = static_cast<int>(heads / cache->heads), p.shape.kv_heads = cache->heads, p.shape.window = static_cast<int>(window);
+  p.q = q, p.q_token = q_token, p.q_head = q_head, p.q_dtype = q_dtype;
+  p.k_scale = cache->k_scale, p.v_scale = cache->v_scale;
+  for (int i = 0; i < 3; ++i) p.ks_stride[i] = cache->ks_stride[i], p.vs_stride[i] = cache->vs_stride[i];
+  p.o = Output{out, o_token, o_head, q_dtype, cache->dim};
+  p.scale = scale * 1.44269504088896340736f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool wide = plan.d == 128;
+  if (cache->dtype == MQ_F16)
+    return wide ? launch_attention<128, MQ_F16>(plan, cache, p, workspace, s, what) : launch_attention<64, MQ_F16>(plan, cache, p, workspace, s, what);
+  if (cache->dtype == MQ_BF16)
+    return wide ? launch_attention<128, MQ_BF16>(plan, cache, p, workspace, s, what) : launch_attention<64, MQ_BF16>(plan, cache, p, workspace, s, what);
+  return wide ? launch_attention<128, MQ_S8>(plan, cache, p, workspace, s, what) : launch_attention<64, MQ_S8>(plan, cache, p, workspace, s, what);
+}

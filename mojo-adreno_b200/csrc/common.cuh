@@ -98,6 +98,10 @@ int encode_tmap_3d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype
                    uint32_t box_cols, uint32_t box_rows, uint32_t box_planes, CUtensorMapSwizzle swizzle,
                    const char *what);
 
+// A 4-D map: strides (of dimensions 1 to 3, in bytes) in any order.
+int encode_tmap_4d(CUtensorMap *map, const void *base, CUtensorMapDataType dtype, const cuuint64_t (&dims)[4],
+                   const cuuint64_t (&strides)[3], const cuuint32_t (&box)[4], CUtensorMapSwizzle swizzle, const char *what);
+
 // Raises kern's dynamic shared-memory limit to at least `smem` on the current device: the attribute belongs to the
 // device's context, so a process that drives several GPUs sets it on each. `seen` is the kernel's own table of the
 // limits already set, by device. A call that raises the limit compares, sets and notes it under a lock, so that the
@@ -160,6 +164,14 @@ enum : int {
   kStatusBeamLoadWait = 17,
   kStatusNormLoadWait = 18,
   kStatusBeamBadParent = 16,  // a parent outside [0, beams): its beam kept its own state
+  kStatusKvBadPage = 19,      // a table entry outside the pool: its rows were not written, or read as zeros
+  kStatusKvBadLength = 20,    // a length below 0 or beyond its row of the table: cut to that
+  kStatusAttnLoadWait = 21,
+  kStatusAttnMmaWait = 22,
+  kStatusAttnSoftmaxWait = 23,
+  kStatusAttnTooManyRows = 26,  // a sequence with more new tokens than the call said: its rows were left as they were
+  kStatusVerifyBadRow = 24,   // a row of logits that is no distribution (a NaN, +infinity, all -infinity)
+  kStatusVerifyBadToken = 25, // a drafted token or a number of drafts out of range
 };
 
 // Waits until the kernels this grid depends on (earlier work on its stream) have completed and

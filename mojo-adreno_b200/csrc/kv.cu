@@ -1,0 +1,222 @@
+// A paged cache's rows: the new tokens' keys and values into their pages (mq_kv_store), and what the pages hold back into
+// rows (mq_kv_load).
+//
+// A row is the keys (or values) of one token and head. Rows go in rounded once to a 16-bit cache's type; an int8
+// cache takes a = max |x| of the row, q = rint(x * (127 / a)) and the scale a / 127 (mq_quantize_s8's
+// arithmetic, bit for bit). Rows come back as q * scale in fp32, rounded once.
+//
+// Both are a copy: what bounds them is the bandwidth, or for a few tokens the launch and the chain of loads that finds a
+// token's page. A CTA takes a few tokens: their sequences are looked up once, then its threads
+// move 8 values each, 8 or 16 lanes to a row, a row's maximum being a shuffle over them.
+#include "paged.cuh"
+
+namespace mq {
+namespace paged {
+
+constexpr int kCopyThreads = 256, kMostTokens = 32;
+
+struct CopyParams {
+  Seqs seqs;
+  void *pages[2];  // keys, values
+  float *scales[2];
+  int64_t stride[2][3], scale_stride[2][3];
+  void *rows[2];
+  int64_t token_stride[2], head_stride[2];
+  int heads, dim, tokens_per_cta;
+};
+
+// Eight values of a row.
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+  constexpr int N = sizeof(T) * 8 / 16 > 0 ? sizeof(T) * 8 / 16 : 1;
+  if constexpr (sizeof(T) == 1) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    const uint32_t x[2] = {w.x, w.y};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(static_cast<int8_t>(x[i / 4] >> (8 * (i % 4))));
+  } else {
+    struct alignas(16) Vec {
+      T t[16 / sizeof(T)];
+    };
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const Vec x = reinterpret_cast<const Vec *>(p)[u];
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) v[u * (16 / sizeof(T)) + i] = static_cast<float>(x.t[i]);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+  struct alignas(16) Vec {
+    T t[16 / sizeof(T)];
+  };
+#pragma unroll
+  for (int u = 0; u < static_cast<int>(sizeof(T) / 2); ++u) {
+    Vec x;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) x.t[i] = T(v[u * (16 / sizeof(T)) + i]);
+    reinterpret_cast<Vec *>(p)[u] = x;
+  }
+}
+
+// STORE: rows of type X into pages of type C; else the other way.
+template <bool STORE, typename C, typename X, int LANES>
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_constant__ CopyParams p) {
+  __shared__ int page[kMostTokens], row[kMostTokens];  // page -1: nothing to do; -2: reads as zeros
+  griddep_launch_dependents();
+  griddep_wait();
+  const int token0 = blockIdx.x * p.tokens_per_cta, tokens = min(p.tokens_per_cta, p.seqs.tokens - token0);
+  if (static_cast<int>(threadIdx.x) < tokens) {
+    const int token = token0 + threadIdx.x;
+    int b = token;
+    page[threadIdx.x] = -1;
+    if (p.seqs.starts) {
+      // The last sequence that starts at the token or before it (empty ones end there too, and come before).
+      int lo = 0, hi = p.seqs.batch;  // starts[lo] <= token < starts[hi], if the starts rise
+      if (p.seqs.starts[0] <= token && token < p.seqs.starts[hi]) {
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (p.seqs.starts[mid] <= token)
+            lo = mid;
+          else
+            hi = mid;
+        }
+        b = lo;
+      } else {
+        b = -1;  // before the first sequence or behind the last
+      }
+    }
+    if (b >= 0) {
+      const Seq s = sequence(p.seqs, b);
+      const int i = token - s.first, position = s.pos0 + i;
+      if (i < 0 || i >= s.n) {  // starts that do not rise
+      } else if (position >= 0 && position < s.length) {
+        const int id = page_of(p.seqs, b, position);
+        page[threadIdx.x] = id >= 0 ? id : STORE ? -1 : -2;
+        row[threadIdx.x] = position & ((1 << p.seqs.page_log2) - 1);
+      } else if (!STORE) {
+        page[threadIdx.x] = -2;
+      }
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x % LANES, per_token = 2 * p.heads;
+  const bool in = lane * 8 < p.dim;
+  for (int base = threadIdx.x / LANES; base < tokens * per_token; base += kCopyThreads / LANES) {
+    const int i = base / per_token, rest = base - i * per_token, which = rest >= p.heads, head = rest - which * p.heads;
+    const int id = page[i];
+    if (id == -1) continue;  // (a row's lanes go together)
+    X *const x = static_cast<X *>(p.rows[which]) + (token0 + i) * p.token_stride[which] + head * p.head_stride[which] + lane * 8;
+    const int64_t *const st = p.stride[which], *const ss = p.scale_stride[which];
+    C *const c = static_cast<C *>(p.pages[which]) + id * st[0] + head * st[1] + row[i] * st[2] + lane * 8;
+    float v[8];
+    if constexpr (STORE) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      if (in) load8(x, v);
+      if constexpr (sizeof(C) == 1) {
+        float a = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e])), bad |= !(fabsf(v[e]) < INFINITY);
+        const unsigned mine = LANES == 32 ? ~0u : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mine, a, o));
+        bad = __ballot_sync(mine, bad) != 0;
+        if (lane == 0) p.scales[which][id * ss[0] + head * ss[1] + row[i] * ss[2]] = bad ? NAN : a / 127.f;
+        // A maximum below 1e-30 is lifted by 2^80 (exact) first, so 127 / a stays finite.
+        const float lift = a < 1e-30f ? 0x1p80f : 1.f;
+        const float f = bad || a == 0.f ? 0.f : 127.f / (a * lift);
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int n = bad ? 0 : __float2int_rn((v[e] * lift) * f);
+          w[e / 4] |= (static_cast<uint32_t>(n) & 0xff) << (8 * (e % 4));
+        }
+        if (in) *reinterpret_cast<uint2 *>(c) = make_uint2(w[0], w[1]);
+      } else {
+        if (in) store8(c, v);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      if (in && id >= 0) {
+        load8(c, v);
+        if constexpr (sizeof(C) == 1) {
+          const float s = p.scales[which][id * ss[0] + head * ss[1] + row[i] * ss[2]];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= s;
+        }
+      }
+      if (in) store8(x, v);
+    }
+  }
+}
+
+template <bool STORE, typename C, typename X>
+int launch_copy(CopyParams &p, cudaStream_t s, const char *what) {
+  const int lanes = p.dim <= 64 ? 8 : 16;
+  // Four rows a thread: enough loads on their way where there are many tokens.
+  const int64_t threads = 2LL * p.heads * lanes;  // of a token
+  p.tokens_per_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostTokens, 4 * kCopyThreads / threads)));
+  const dim3 grid((p.seqs.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta);
+  if (lanes == 8) return launch_overlapped(kv_copy_kernel<STORE, C, X, 8>, grid, dim3(kCopyThreads), 0, s, what, p);
+  return launch_overlapped(kv_copy_kernel<STORE, C, X, 16>, grid, dim3(kCopyThreads), 0, s, what, p);
+}
+template <bool STORE, typename C>
+int copy_by_rows(CopyParams &p, int dtype, cudaStream_t s, const char *what) {
+  if (dtype == MQ_F32) return launch_copy<STORE, C, float>(p, s, what);
+  if (dtype == MQ_F16) return launch_copy<STORE, C, __half>(p, s, what);
+  return launch_copy<STORE, C, __nv_bfloat16>(p, s, what);
+}
+
+template <bool STORE>
+int kv_copy(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_token, int64_t v_head, int dtype, const mq_kv_pages *c,
+            const int32_t *table, int64_t ldt, int64_t width, const int32_t *lengths, const int32_t *starts, int64_t batch,
+            int64_t tokens, void *stream, const char *what) {
+  if (int rc = check_cache(c, what)) return rc;
+  CopyParams p{};
+  if (int rc = check_seqs(&p.seqs, c, table, ldt, width, lengths, starts, batch, tokens, what)) return rc;
+  MQ_REQUIRE(dtype == MQ_F32 || dtype == MQ_F16 || dtype == MQ_BF16, MQ_EINVAL, "%s: rows must be MQ_F32, MQ_F16 or MQ_BF16", what);
+  if (batch == 0 || tokens == 0) return MQ_OK;
+  MQ_REQUIRE(tokens * c->heads < (1LL << 31), MQ_EUNSUPPORTED, "%s: too many rows", what);
+  if (STORE) {
+    if (int rc = check_rows(k, dtype, k_token, k_head, "k", what)) return rc;
+    if (int rc = check_rows(v, dtype, v_token, v_head, "v", what)) return rc;
+  } else {
+    if (int rc = check_rows_out(k, dtype, tokens, c->heads, c->dim, k_token, k_head, "k", what)) return rc;
+    if (int rc = check_rows_out(v, dtype, tokens, c->heads, c->dim, v_token, v_head, "v", what)) return rc;
+  }
+  mq::DeviceInfo dev;
+  if (int rc = device_info(&dev)) return rc;
+  p.pages[0] = c->k, p.pages[1] = c->v, p.scales[0] = c->k_scale, p.scales[1] = c->v_scale;
+  for (int i = 0; i < 3; ++i) {
+    p.stride[0][i] = c->k_stride[i], p.stride[1][i] = c->v_stride[i];
+    p.scale_stride[0][i] = c->ks_stride[i], p.scale_stride[1][i] = c->vs_stride[i];
+  }
+  p.rows[0] = k, p.rows[1] = v;
+  p.token_stride[0] = k_token, p.token_stride[1] = v_token, p.head_stride[0] = k_head, p.head_stride[1] = v_head;
+  p.heads = c->heads, p.dim = c->dim;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c->dtype == MQ_S8) return copy_by_rows<STORE, int8_t>(p, dtype, s, what);
+  if (c->dtype == MQ_F16) return copy_by_rows<STORE, __half>(p, dtype, s, what);
+  return copy_by_rows<STORE, __nv_bfloat16>(p, dtype, s, what);
+}
+
+}  // namespace paged
+}  // namespace mq
+
+extern "C" int mq_kv_store(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
+                           int dtype, const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width,
+                           const int32_t *lengths, const int32_t *starts, int64_t batch, int64_t tokens, void *stream) {
+  return mq::paged::kv_copy<true>(const_cast<void *>(k), k_token, k_head, const_cast<void *>(v), v_token, v_head, dtype, cache,
+                                  table, ldt, width, lengths, starts, batch, tokens, stream, "mq_kv_store");
+}
+
+extern "C" int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width, const int32_t *lengths,
+                          const int32_t *starts, int64_t batch, int64_t tokens, void *k, int64_t k_token, int64_t k_head, void *v,
+                          int64_t v_token, int64_t v_head, int dtype, void *stream) {
+  return mq::paged::kv_copy<false>(k, k_token, k_head, v, v_token, v_head, dtype, cache, table, ldt, width, lengths, starts,
+                                   batch, tokens, stream, "mq_kv_load");
+}

@@ -14,3 +14,7 @@
 #include "gemm_w8a8.cu"
 #include "norm.cu"
 #include "beam.cu"
+#include "kv.cu"
+#include "attn.cu"
+#include "attn_tile.cu"
+#include "verify.cu"

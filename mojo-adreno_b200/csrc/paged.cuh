@@ -1,0 +1,313 @@
+// What the operators on a paged cache share: the host's checks of a cache and its tensor maps, and the device's view of
+// sequences, their pages and the split of a launch's work.
+//
+// Sequence b has rows starts[b] .. starts[b + 1] of the tokens (row b where starts is NULL) and lengths[b] positions in
+// the cache, its new tokens' among them: row i of n is position lengths[b] - n + i. Position p lies in page
+// table[b][p / page], row p % page.
+#pragma once
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace mq {
+namespace paged {
+
+constexpr int kMaxDim = 128, kMinPage = 16, kMaxPage = 256;
+
+struct Seqs {
+  const int32_t *table, *lengths, *starts;
+  int64_t ldt;
+  int batch, tokens, width, page_log2;
+  int pages;  // of the pool
+};
+
+struct Seq {
+  int first, n;  // its rows
+  int length;    // positions in the cache
+  int pos0;      // position of its first row; negative where it has more rows than positions
+};
+
+// starts that fall or pass the tokens and lengths that pass the table are cut to what is there.
+__device__ __forceinline__ Seq sequence(const Seqs &s, int b) {
+  Seq q;
+  q.first = b, q.n = 1;
+  if (s.starts) {
+    q.first = min(max(s.starts[b], 0), s.tokens);
+    q.n = min(max(s.starts[b + 1], q.first), s.tokens) - q.first;
+  }
+  const int length = s.lengths[b], most = s.width << s.page_log2;
+  q.length = min(max(length, 0), most);
+  if (q.length != length) raise_status(kStatusKvBadLength);
+  q.pos0 = q.length - q.n;
+  return q;
+}
+
+// The page that holds a position of sequence b: -1 (reported) where the table names none of the pool's.
+__device__ __forceinline__ int page_of(const Seqs &s, int b, int position) {
+  const int id = s.table[b * s.ldt + (position >> s.page_log2)];
+  if (static_cast<unsigned>(id) < static_cast<unsigned>(s.pages)) return id;
+  raise_status(kStatusKvBadPage);
+  return -1;
+}
+
+// ---- host: checks -----------------------------------------------------------------------------------
+
+inline int element_size(int dtype) { return dtype == MQ_F32 ? 4 : dtype == MQ_S8 ? 1 : 2; }
+inline int log2_of(int v) { return 31 - __builtin_clz(static_cast<unsigned>(v)); }
+
+// Every (page, head, position) row needs bytes of its own: by rising stride, each dimension steps over all that the
+// ones before cover. `row`: elements of a row.
+inline bool rows_apart(const int64_t *stride, int64_t pages, int64_t heads, int64_t page, int64_t row) {
+  int64_t size[3] = {pages, heads, page};
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return stride[a] < stride[b]; });
+  int64_t extent = row;
+  for (int d : order) {
+    if (size[d] == 1) continue;
+    if (stride[d] < extent || stride[d] >= (1LL << 40) / size[d]) return false;
+    extent += stride[d] * (size[d] - 1);
+  }
+  return true;
+}
+
+inline int check_cache(const mq_kv_pages *c, const char *what) {
+  MQ_REQUIRE(c && c->k && c->v, MQ_EINVAL, "%s: null pointer", what);
+  MQ_REQUIRE(c->dtype == MQ_F16 || c->dtype == MQ_BF16 || c->dtype == MQ_S8, MQ_EINVAL,
+             "%s: the cache's type must be MQ_F16, MQ_BF16 or MQ_S8", what);
+  MQ_REQUIRE(c->pages > 0 && c->pages < (1LL << 31) && c->heads > 0 && c->heads <= 65535, MQ_EINVAL, "%s: bad number of pages or heads",
+             what);
+  MQ_REQUIRE(c->page >= kMinPage && c->page <= kMaxPage && (c->page & (c->page - 1)) == 0, MQ_EUNSUPPORTED,
+             "%s: a page must hold 16, 32, 64, 128 or 256 positions", what);
+  MQ_REQUIRE(c->dim >= 16 && c->dim <= kMaxDim && c->dim % 16 == 0, MQ_EUNSUPPORTED,
+             "%s: dim must be a multiple of 16 up to %d", what, kMaxDim);
+  const int es = element_size(c->dtype);
+  for (int i = 0; i < 3; ++i)
+    MQ_REQUIRE(c->k_stride[i] * es % 16 == 0 && c->v_stride[i] * es % 16 == 0, MQ_EALIGN,
+               "%s: every row of the cache must start 16-byte aligned", what);
+  MQ_REQUIRE(aligned(c->k, 16) && aligned(c->v, 16), MQ_EALIGN, "%s: every row of the cache must start 16-byte aligned", what);
+  MQ_REQUIRE(rows_apart(c->k_stride, c->pages, c->heads, c->page, c->dim) &&
+                 rows_apart(c->v_stride, c->pages, c->heads, c->page, c->dim),
+             MQ_EINVAL, "%s: rows of the cache overlap", what);
+  if (c->dtype == MQ_S8) {
+    MQ_REQUIRE(c->k_scale && c->v_scale, MQ_EINVAL, "%s: an int8 cache needs its scales", what);
+    MQ_REQUIRE(aligned(c->k_scale, 4) && aligned(c->v_scale, 4), MQ_EALIGN, "%s: scales must be 4-byte aligned", what);
+    MQ_REQUIRE(rows_apart(c->ks_stride, c->pages, c->heads, c->page, 1) && rows_apart(c->vs_stride, c->pages, c->heads, c->page, 1),
+               MQ_EINVAL, "%s: scales of the cache overlap", what);
+  }
+  return MQ_OK;
+}
+
+inline int check_seqs(Seqs *s, const mq_kv_pages *c, const int32_t *table, int64_t ldt, int64_t width, const int32_t *lengths,
+                      const int32_t *starts, int64_t batch, int64_t tokens, const char *what) {
+  MQ_REQUIRE(batch >= 0 && tokens >= 0 && width >= 0, MQ_EINVAL, "%s: bad shape", what);
+  MQ_REQUIRE(batch < (1LL << 22) && tokens < (1LL << 30), MQ_EUNSUPPORTED, "%s: too many sequences or tokens", what);
+  MQ_REQUIRE(width <= ((1LL << 31) - 1024) / c->page, MQ_EUNSUPPORTED, "%s: the table's rows name too many positions", what);
+  MQ_REQUIRE(starts || tokens == batch, MQ_EINVAL, "%s: without starts every sequence has one row", what);
+  if (batch > 0 && tokens > 0) {
+    MQ_REQUIRE(lengths && (table || width == 0), MQ_EINVAL, "%s: null pointer", what);
+    MQ_REQUIRE(aligned(table, 4) && aligned(lengths, 4) && aligned(starts, 4), MQ_EALIGN, "%s: the table, lengths and starts must be 4-byte aligned",
+               what);
+    MQ_REQUIRE(ldt >= width || batch == 1, MQ_EINVAL, "%s: the table's row stride is less than its width", what);
+  }
+  *s = Seqs{table, lengths, starts, ldt, static_cast<int>(batch), static_cast<int>(tokens), static_cast<int>(width),
+            log2_of(c->page), static_cast<int>(c->pages)};
+  return MQ_OK;
+}
+
+// Rows [tokens][heads][dim] of a strided tensor (strides in elements), each 16-byte aligned.
+inline int check_rows(const void *p, int dtype, int64_t token_stride, int64_t head_stride, const char *name, const char *what) {
+  MQ_REQUIRE(p, MQ_EINVAL, "%s: null pointer", what);
+  const int es = element_size(dtype);
+  MQ_REQUIRE(aligned(p, 16) && token_stride * es % 16 == 0 && head_stride * es % 16 == 0, MQ_EALIGN,
+             "%s: every row of %s must start 16-byte aligned", what, name);
+  MQ_REQUIRE(token_stride >= 0 && head_stride >= 0, MQ_EINVAL, "%s: %s has a negative stride", what, name);
+  return MQ_OK;
+}
+// The same of rows that are written: none may share bytes with another.
+inline int check_rows_out(const void *p, int dtype, int64_t tokens, int64_t heads, int64_t dim, int64_t token_stride,
+                          int64_t head_stride, const char *name, const char *what) {
+  if (int rc = check_rows(p, dtype, token_stride, head_stride, name, what)) return rc;
+  const int64_t stride[3] = {token_stride, head_stride, 0};
+  MQ_REQUIRE(rows_apart(stride, tokens, heads, 1, dim), MQ_EINVAL, "%s: rows of %s overlap", what, name);
+  return MQ_OK;
+}
+
+// ---- attention: items, units and shares --------------------------------------------------------------
+
+// The rows of one kv head of a sequence are its tokens' `group` query heads, token by token: row r is head r % group of
+// token r / group. An item is ROWS of them and the blocks of KEYS positions that any of them sees; a unit is one block
+// of one item. Units are numbered by sequence, kv head, row tile and block, and the launch's CTAs take equal shares of
+// them, whatever the sequences' lengths: an item may be cut between CTAs, which then leave its parts to be joined.
+struct Shape {
+  int group, kv_heads, window;
+  int rows_from, rows_to;  // the sequences of this launch: those with rows_from < rows <= rows_to
+  int rows_most;           // a sequence with more was not announced: reported, and left out by every launch
+};
+
+template <int ROWS, int KEYS>
+struct Range {
+  int lo, blocks;  // the first block, how many (one, with nothing in it, where no row sees a key)
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ Range<ROWS, KEYS> tile_range(const Seq &s, const Shape &a, int t) {
+  const int rows = s.n * a.group;
+  const int i0 = t * ROWS / a.group, i1 = (min(rows, (t + 1) * ROWS) - 1) / a.group;
+  const int hi = min(max(s.pos0 + i1 + 1, 0), s.length), lo = a.window ? max(0, s.pos0 + i0 + 1 - a.window) : 0;
+  const int b0 = min(lo, max(hi - 1, 0)) / KEYS;
+  return {b0, max(1, (hi + KEYS - 1) / KEYS - b0)};
+}
+__device__ __forceinline__ bool takes_part(const Seq &s, const Shape &a) {
+  const int64_t rows = static_cast<int64_t>(s.n) * a.group;
+  return rows > a.rows_from && rows <= a.rows_to;
+}
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int64_t units_per_head(const Seq &s, const Shape &a) {
+  const int tiles = (s.n * a.group + ROWS - 1) / ROWS;
+  int64_t units = 0;
+  for (int t = 0; t < tiles; ++t) units += tile_range<ROWS, KEYS>(s, a, t).blocks;
+  return units;
+}
+
+struct Share {
+  int64_t total, begin, end;  // units of the launch, and of this CTA
+  int64_t offset;             // of `begin` within sequence b's
+  int b, parts;               // parts: CTAs with a share
+};
+template <int THREADS>
+struct ShareScratch {
+  int64_t sums[THREADS / 32];
+  int64_t offset;
+  int b;
+};
+
+// This CTA's share; called by all THREADS threads. parts <= blockIdx.x: none.
+template <int THREADS, int ROWS, int KEYS>
+__device__ __forceinline__ Share find_share(const Seqs &s, const Shape &a, ShareScratch<THREADS> &sm) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  auto cost_of = [&](int b) -> int64_t {
+    if (b >= s.batch) return 0;
+    const Seq q = sequence(s, b);
+    if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
+    return takes_part(q, a) ? units_per_head<ROWS, KEYS>(q, a) * a.kv_heads : 0;
+  };
+  const int64_t first = cost_of(tid);
+  int64_t mine = first;
+  for (int b = tid + THREADS; b < s.batch; b += THREADS) mine += cost_of(b);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sm.sums[warp] = mine;
+  __syncthreads();
+  Share share{};
+  for (int w = 0; w < THREADS / 32; ++w) share.total += sm.sums[w];
+  share.parts = static_cast<int>(share.total < gridDim.x ? share.total : gridDim.x);
+  __syncthreads();
+  if (static_cast<int>(blockIdx.x) >= share.parts) return share;
+  share.begin = share.total * blockIdx.x / share.parts;
+  share.end = share.total * (blockIdx.x + 1) / share.parts;
+  int64_t before = 0;
+  for (int base = 0; base < s.batch; base += THREADS) {
+    const int64_t cost = base == 0 ? first : cost_of(base + tid);
+    int64_t incl = cost;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) sm.sums[warp] = incl;
+    __syncthreads();
+    int64_t ahead = before;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) ahead += sm.sums[w];
+      before += sm.sums[w];
+    }
+    const int64_t start = ahead + incl - cost;
+    if (start <= share.begin && share.begin < start + cost) sm.b = base + tid, sm.offset = share.begin - start;
+    __syncthreads();
+    if (before > share.begin) break;
+  }
+  share.b = sm.b, share.offset = sm.offset;
+  return share;
+}
+
+struct Item {
+  Seq s;
+  int b, head, tile;
+  int block, blocks;  // of this CTA
+  int before, whole;  // blocks of the item before them, blocks of the item
+};
+
+// Walks through a share's items. Every role of a CTA walks by itself.
+template <int ROWS, int KEYS>
+struct Walk {
+  Seq s;
+  int b, head, tile, tiles, skip;
+  int64_t left;
+  __device__ __forceinline__ void start(const Seqs &q, const Shape &a, const Share &share) {
+    b = share.b, left = share.end - share.begin;
+    s = sequence(q, b);
+    tiles = (s.n * a.group + ROWS - 1) / ROWS;
+    const int64_t per_head = units_per_head<ROWS, KEYS>(s, a);
+    head = static_cast<int>(share.offset / per_head);
+    int64_t rest = share.offset - head * per_head;
+    for (tile = 0;; ++tile) {
+      const int blocks = tile_range<ROWS, KEYS>(s, a, tile).blocks;
+      if (rest < blocks) break;
+      rest -= blocks;
+    }
+    skip = static_cast<int>(rest);
+  }
+  __device__ __forceinline__ bool next(const Seqs &q, const Shape &a, Item &item) {
+    if (left <= 0) return false;
+    if (tile == tiles) {
+      tile = 0;
+      if (++head == a.kv_heads) {
+        head = 0;
+        do s = sequence(q, ++b);
+        while (!takes_part(s, a));  // (units are left, so such a sequence follows)
+        tiles = (s.n * a.group + ROWS - 1) / ROWS;
+      }
+    }
+    const auto r = tile_range<ROWS, KEYS>(s, a, tile);
+    item.s = s, item.b = b, item.head = head, item.tile = tile;
+    item.before = skip, item.whole = r.blocks, item.block = r.lo + skip;
+    item.blocks = static_cast<int>(left < r.blocks - skip ? left : r.blocks - skip);
+    left -= item.blocks;
+    skip = 0;
+    ++tile;
+    return true;
+  }
+};
+
+// A CTA leaves at most two parts of items that others share: one that it goes on with (slot 0) and one that it
+// begins and does not end (slot 1). `cut` says which item the CTA goes on with.
+struct Cut {
+  int32_t b, head, tile, goes_on;
+  int64_t first, end;  // the item's units
+};
+struct Parts {
+  int64_t *counts;  // units, CTAs with a share
+  Cut *cuts;        // [ctas]
+  float2 *stats;    // [ctas][2][rows]: the maximum that the part's sums are relative to (log2), the sum of weights
+  float *sums;      // [ctas][2][rows][D]
+};
+inline size_t parts_bytes(int ctas, int rows, int d) {
+  return 256 + static_cast<size_t>(ctas) * (sizeof(Cut) + 2ull * rows * (sizeof(float2) + 4ull * d));
+}
+inline Parts parts_at(void *workspace, int ctas, int rows) {
+  char *p = static_cast<char *>(workspace);
+  Parts parts;
+  parts.counts = reinterpret_cast<int64_t *>(p);
+  parts.cuts = reinterpret_cast<Cut *>(p + 256);
+  parts.stats = reinterpret_cast<float2 *>(parts.cuts + ctas);
+  parts.sums = reinterpret_cast<float *>(parts.stats + 2ull * ctas * rows);
+  return parts;
+}
+
+struct Output {
+  void *out;
+  int64_t token_stride, head_stride;
+  int dtype, dim;
+};
+
+}  // namespace paged
+}  // namespace mq

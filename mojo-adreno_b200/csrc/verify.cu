@@ -1,0 +1,484 @@
+// Drafted tokens against the target's distribution (mq_verify_drafts): beam.cu's and mq_head_argmax's place where a
+// drafter proposes several tokens at once.
+//
+// p_i = softmax(target row i / T), q_i = softmax(draft row i / T) (without draft logits: all on the drafted token). Drafted
+// token d_i is kept while u_i q_i(d_i) < p_i(d_i). At the first that is not, i = n, one token is drawn from max(p_n - q_n, 0), where
+// all are kept from p_n: the first v whose running sum exceeds u times the whole, u the number behind the drafts' (one that was
+// looked at for a token that it rejected is no longer uniform). At T = 0 p is all on the largest logit, the
+// lowest index among equal ones.
+//
+// verify_scan_kernel reads every logit once: `splits` CTAs per row keep a maximum and a sum of exponentials, in fp32:
+// a comparison of u q with p is off by some 1e-7, so it decides otherwise once in 10^7 times. It is bound by the bandwidth.
+//
+// verify_draw_kernel, a cluster per request, decides, and goes through the chosen row again for the draw. There fp32 does not do:
+// the running sum passes some 10^5 borders between tokens, and a relative error of 1e-8 in it would move the drawn token
+// to its neighbour once in a thousand draws. So the sums and the exponentials in them are fp64: 2^y with
+// y = n / 32 + r, |r| <= 1/64, is 2^(n / 32) from a table of 32 times a Taylor polynomial of degree 5 (2e-15), nine
+// fp64 instructions. Each warp has a stretch of the row of its own; only the warp whose stretch holds the drawn
+// token looks for it, in order.
+#include "common.cuh"
+
+namespace mq {
+namespace verify {
+
+constexpr int kScan = 256, kVecs = 4;        // threads of a scan CTA, 16-byte vectors per thread and step
+constexpr int kDraw = 512, kCluster = 8;     // threads of a drawing CTA, CTAs of a request
+constexpr int kMaxDrafts = 32, kMaxSplits = 64;
+constexpr float kLeastTemperature = 1e-5f;   // below: 0
+constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
+
+// As many CTAs as run at once, a step of each at least.
+__host__ __device__ constexpr int splits_for(int64_t rows, int64_t vocab) {
+  const int64_t steps = (vocab * 4 + kScan * kVecs * 16 - 1) / (kScan * kVecs * 16);
+  int64_t s = 148 * 8 / rows;
+  if (s > kMaxSplits) s = kMaxSplits;
+  if (s > steps) s = steps;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+struct Params {
+  const void *target, *draft;  // draft may be null
+  int64_t ld_target, ld_draft;
+  const int32_t *drafted, *counts;  // counts may be null
+  const float *uniform, *temperature;  // temperature may be null: 1
+  float2 *parts;  // [batch][2 drafts + 1][splits]: the largest logit, and the sum relative to it (T = 0: its index's bits)
+  int32_t *tokens, *accepted;
+  float *logprobs;
+  int batch, drafts, vocab, splits, dtype;
+};
+
+__device__ __forceinline__ int rows_per_request(const Params &p) { return p.draft ? 2 * p.drafts + 1 : p.drafts + 1; }
+__device__ __forceinline__ float temperature_of(const Params &p, int b) {
+  const float t = p.temperature ? p.temperature[b] : 1.f;
+  return t >= kLeastTemperature ? t : 0.f;
+}
+__device__ __forceinline__ int count_of(const Params &p, int b) {
+  const int n = p.counts ? p.counts[b] : p.drafts;
+  if (n < 0 || n > p.drafts) raise_status(kStatusVerifyBadToken);
+  return min(max(n, 0), p.drafts);
+}
+// Row i of a request: target rows 0 .. drafts, then the draft's.
+__device__ __forceinline__ const char *row_at(const Params &p, int b, int i) {
+  const int es = p.dtype == MQ_F32 ? 4 : 2;
+  if (i <= p.drafts) return static_cast<const char *>(p.target) + (static_cast<int64_t>(b) * (p.drafts + 1) + i) * p.ld_target * es;
+  return static_cast<const char *>(p.draft) + (static_cast<int64_t>(b) * p.drafts + i - p.drafts - 1) * p.ld_draft * es;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kScan) verify_scan_kernel(const Params p) {
+  constexpr int V = 16 / sizeof(T), kElems = V * kVecs;
+  __shared__ float red[kScan / 32];
+  __shared__ float sums[kScan / 32];
+  __shared__ int index_red[kScan / 32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, per = rows_per_request(p);
+  const int split = blockIdx.x % p.splits, i = blockIdx.x / p.splits % per, b = blockIdx.x / p.splits / per;
+  const float hot = temperature_of(p, b);
+  const int n = count_of(p, b);
+  if (i <= p.drafts ? i > n : i - p.drafts - 1 >= n || hot == 0.f) return;  // nobody asks for that row
+  const T *x = reinterpret_cast<const T *>(row_at(p, b, i));
+  // The row's 16-byte aligned vectors, dealt to the splits; the elements before and behind them (at most V - 1 each) are
+  // split 0's.
+  const int head = min(p.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+  const int nvec = (p.vocab - head) / V, body_end = head + nvec * V, edges = head + p.vocab - body_end;
+  const int v0 = static_cast<int>(static_cast<int64_t>(nvec) * split / p.splits);
+  const int v1 = static_cast<int>(static_cast<int64_t>(nvec) * (split + 1) / p.splits);
+  const float k = static_cast<float>(kLog2e / (hot > 0.f ? static_cast<double>(hot) : 1.0));
+  float m = -INFINITY, s = 0.f;
+  int at = p.vocab;  // T = 0: the first place of m
+  auto take = [&](const float (&v)[kElems], const int (&first)[kVecs]) {
+    float big = v[0];
+#pragma unroll
+    for (int e = 1; e < kElems; ++e) big = fmaxf(big, v[e]);
+    if (hot > 0.f) {
+      if (big > m) s *= exp2f((m - big) * k), m = big;
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        float y;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((v[e] - ref) * k));
+        s += y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) s += v[e] < INFINITY ? 0.f : NAN;
+      if (big > m) {
+        m = big;
+#pragma unroll
+        for (int e = kElems - 1; e >= 0; --e)
+          if (v[e] == big) at = first[e / V] + e % V;
+      }
+    }
+  };
+  const uint4 *body = reinterpret_cast<const uint4 *>(x + head);
+#pragma unroll 1
+  for (int base = v0; base < v1; base += kScan * kVecs) {
+    float v[kElems];
+    int first[kVecs];
+    uint4 q[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int g = base + u * kScan + tid;
+      first[u] = head + g * V;
+      if (g < v1) q[u] = ldg_stream_v4(body + g);
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const bool in = base + u * kScan + tid < v1;
+      const T *e = reinterpret_cast<const T *>(&q[u]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[u * V + j] = in ? static_cast<float>(e[j]) : -INFINITY;
+    }
+    take(v, first);
+  }
+  if (split == 0 && tid < edges) {
+    float v[kElems];
+    int first[kVecs] = {};
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) v[e] = -INFINITY;
+    first[0] = tid < head ? tid : body_end + tid - head;
+    v[0] = static_cast<float>(x[first[0]]);
+    if (hot == 0.f && v[0] == m && first[0] < at) at = first[0];  // (an edge before the body)
+    take(v, first);
+  }
+  // Join the threads', in one fixed order.
+  float top = m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+  top = red[0];
+  for (int w = 1; w < kScan / 32; ++w) top = fmaxf(top, red[w]);
+  if (hot > 0.f) s = m == -INFINITY ? s : s * exp2f((m - top) * k);  // (an empty thread's sum is 0, or NaN)
+  int where = m == top ? at : p.vocab;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    where = min(where, __shfl_xor_sync(0xffffffffu, where, o));
+  }
+  if (lane == 0) sums[warp] = s, index_red[warp] = where;
+  __syncthreads();
+  if (tid == 0) {
+    s = 0.f;
+    where = p.vocab;
+    for (int w = 0; w < kScan / 32; ++w) s += sums[w], where = min(where, index_red[w]);
+    if (hot == 0.f) s = s == s ? __int_as_float(where) : __int_as_float(-1);
+    p.parts[blockIdx.x] = make_float2(top, s);
+  }
+}
+
+__device__ __forceinline__ float read(const Params &p, const char *row, int v) {
+  if (p.dtype == MQ_F32) return reinterpret_cast<const float *>(row)[v];
+  if (p.dtype == MQ_F16) return __half2float(reinterpret_cast<const __half *>(row)[v]);
+  return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(row)[v]);
+}
+
+// 2^((x - top) k / 32) in fp64, relative error below 1e-14 (k: 32 log2(e) / T). The sum with 1.5 * 2^52 rounds to an integer.
+struct Exp {
+  double k, magic;
+  float least;
+  const double *table;  // 2^(i / 32)
+  __device__ __forceinline__ void start(float top, float hot, const double *t) {
+    k = 32.0 * kLog2e / hot;
+    // (Logits so large that the next one below is 2^-10000 of the largest: only that one counts.)
+    if (!(fabs(top * k) < 1e15)) k = 0;
+    magic = 6755399441055744.0 - rint(top * k);
+    least = fmaxf(top - 600.f * hot, -3.402823466e38f);  // below: 0 (2^-865 of the largest)
+    table = t;
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    if (!(x >= least)) return 0.0;
+    const double y = x, t = fma(y, k, magic), n = t - magic, r = fma(y, k, -n);
+    constexpr double a = kLn2 / 32;
+    double e = fma(r, a * a * a * a * a / 120, a * a * a * a / 24);
+    e = fma(e, r, a * a * a / 6);
+    e = fma(e, r, a * a / 2);
+    e = fma(e, r, a);
+    e = fma(e, r, 1.0);
+    const int low = __double2loint(t);
+    const double z = table[low & 31];
+    return e * __hiloint2double(__double2hiint(z) + ((low >> 5) << 20), __double2loint(z));
+  }
+};
+
+__device__ __forceinline__ uint32_t rank_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void sync_cluster() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
+  constexpr int kWarps = kDraw / 32;
+  __shared__ double table[32];
+  __shared__ float top[2 * kMaxDrafts + 1], total[2 * kMaxDrafts + 1];  // of the request's rows; T = 0: total holds the index
+  __shared__ int kept_s, bad_s;
+  __shared__ double warp_sums[3][kWarps];    // p, q; then the weights
+  __shared__ double all_sums[3][kCluster][kWarps];
+  griddep_launch_dependents();
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, rank = rank_in_cluster(), b = blockIdx.x / kCluster;
+  if (tid < 32) table[tid] = exp2(tid / 32.0);
+  griddep_wait();
+  const int per = rows_per_request(p), n = count_of(p, b);
+  const float hot = temperature_of(p, b);
+  for (int i = warp; i < per; i += kWarps) {
+    if (i <= p.drafts ? i > n : i - p.drafts - 1 >= n || hot == 0.f) continue;
+    const float2 *parts = p.parts + (static_cast<int64_t>(b) * per + i) * p.splits;
+    float m = -INFINITY;
+    for (int j = lane; j < p.splits; j += 32) m = fmaxf(m, parts[j].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (hot > 0.f) {
+      double s = 0;
+      for (int j = lane; j < p.splits; j += 32) {
+        const float2 q = parts[j];
+        s += q.x == -INFINITY ? static_cast<double>(q.y) : q.y * exp2((static_cast<double>(q.x) - m) * kLog2e / hot);
+      }
+      s = warp_sum(s);
+      if (lane == 0) top[i] = m, total[i] = static_cast<float>(s);
+    } else {
+      int where = p.vocab;
+      bool bad = false;
+      for (int j = lane; j < p.splits; j += 32) {
+        const int at = __float_as_int(parts[j].y);
+        bad |= at < 0;
+        if (parts[j].x == m && at >= 0) where = min(where, at);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) where = min(where, __shfl_xor_sync(0xffffffffu, where, o));
+      bad = __any_sync(0xffffffffu, bad) || !(m > -INFINITY);
+      if (lane == 0) top[i] = m, total[i] = __int_as_float(bad ? -1 : where);
+    }
+  }
+  __syncthreads();
+  auto good = [&](int i) { return hot > 0.f ? total[i] > 0.f && total[i] < INFINITY && fabsf(top[i]) < INFINITY : __float_as_int(total[i]) >= 0; };
+  if (warp == 0) {  // lane i: drafted token i
+    const int64_t at = static_cast<int64_t>(b) * (p.drafts + 1) + lane;
+    bool keep = false;
+    int status = 0;
+    float logprob = 0.f;
+    if (lane <= n && !good(lane)) {
+      status = kStatusVerifyBadRow;
+    } else if (lane < n) {
+      const int d = p.drafted[static_cast<int64_t>(b) * p.drafts + lane], j = p.drafts + 1 + lane;
+      if (d < 0 || d >= p.vocab) {
+        status = kStatusVerifyBadToken;
+      } else if (hot == 0.f) {
+        keep = d == __float_as_int(total[lane]);
+      } else if (p.draft && !good(j)) {
+        status = kStatusVerifyBadRow;
+      } else {
+        const double z = (static_cast<double>(read(p, row_at(p, b, lane), d)) - top[lane]) / hot;
+        const double pd = exp(z) / total[lane];
+        const double qd = p.draft ? exp((static_cast<double>(read(p, row_at(p, b, j), d)) - top[j]) / hot) / total[j] : 1.0;
+        keep = p.uniform[at] * qd < pd;
+        logprob = static_cast<float>(z - log(static_cast<double>(total[lane])));
+      }
+    }
+    const unsigned not_kept = ~__ballot_sync(0xffffffffu, keep);  // (at most 32 drafts: lane 31 may be a kept one)
+    const int first = not_kept ? __ffs(not_kept) - 1 : 32;
+    if (lane < first && rank == 0) p.logprobs[at] = logprob;
+    if (lane == first && status) raise_status(status);
+    if (lane == 0) {
+      kept_s = first, bad_s = !good(first);
+      if (first == 32 && bad_s) raise_status(kStatusVerifyBadRow);
+    }
+  }
+  __syncthreads();
+  const int kept = kept_s, bad = bad_s;
+  const int64_t out0 = static_cast<int64_t>(b) * (p.drafts + 1);
+  if (rank == 0) {
+    if (tid == 0) p.accepted[b] = kept;
+    for (int i = tid; i <= p.drafts; i += kDraw) {
+      if (i < kept)
+        p.tokens[out0 + i] = p.drafted[static_cast<int64_t>(b) * p.drafts + i];
+      else if (i > kept || bad || hot == 0.f) {
+        p.tokens[out0 + i] = i == kept && !bad ? __float_as_int(total[kept]) : -1;
+        p.logprobs[out0 + i] = 0.f;
+      }
+    }
+  }
+  if (bad || hot == 0.f) return;  // (the whole cluster)
+
+  // The draw. This warp's stretch of the row:
+  const int stretch = kCluster * kWarps, mine = rank * kWarps + warp;
+  const int v0 = static_cast<int>(static_cast<int64_t>(p.vocab) * mine / stretch);
+  const int v1 = static_cast<int>(static_cast<int64_t>(p.vocab) * (mine + 1) / stretch);
+  const char *pr = row_at(p, b, kept);
+  const int d = kept < n ? p.drafted[static_cast<int64_t>(b) * p.drafts + kept] : -1;
+  const bool two = p.draft && kept < n && d >= 0 && d < p.vocab && good(p.drafts + 1 + kept);
+  const char *qr = two ? row_at(p, b, p.drafts + 1 + kept) : nullptr;
+  // Without draft logits the drafted token has all of q, so nothing of it is left.
+  const int without = !p.draft ? d : -1;
+  Exp ep, eq;
+  ep.start(top[kept], hot, table);
+  eq.start(two ? top[p.drafts + 1 + kept] : 0.f, hot, table);
+
+  // Sums over the cluster of what every warp has; all_sums keeps each warp's, in the row's order.
+  auto gather = [&](int which, double v) {
+    v = warp_sum(v);
+    if (lane == 0) warp_sums[which][warp] = v;
+    sync_cluster();
+    for (int e = tid; e < stretch; e += kDraw) {
+      uint32_t from;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(smem_u32(&warp_sums[which][e % kWarps])), "r"(e / kWarps));
+      double x;
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(from) : "memory");
+      all_sums[which][e / kWarps][e % kWarps] = x;
+    }
+    __syncthreads();
+    const double *all = &all_sums[which][0][0];
+    return warp_sum(all[lane] + all[lane + 32] + all[lane + 64] + all[lane + 96]);
+  };
+  double ip = 1, iq = 0;
+  bool rest = two;
+  if (two) {
+    double sp = 0, sq = 0;
+#pragma unroll 4
+    for (int v = v0 + lane; v < v1; v += 32) sp += ep(read(p, pr, v)), sq += eq(read(p, qr, v));
+    ip = 1 / gather(0, sp);
+    iq = 1 / gather(1, sq);
+  }
+  auto weight = [&](int v) -> double {
+    if (v == without) return 0;
+    const double w = ep(read(p, pr, v)) * ip;
+    return rest ? fmax(w - eq(read(p, qr, v)) * iq, 0.0) : w;
+  };
+  double whole = 0;
+  for (int round = 0; round < 2; ++round) {
+    double w = 0;
+#pragma unroll 4
+    for (int v = v0 + lane; v < v1; v += 32) w += weight(v);
+    if (round) sync_cluster();  // (everybody has read the first round's sums)
+    whole = gather(2, w);
+    if (whole > 0 || !rest) break;
+    rest = false;  // p and q are one: what is left is rounding, so the draw is from p
+  }
+  const double goal = p.uniform[out0 + p.drafts] * whole;
+  // The first stretch whose running sum passes the goal, else the last that has any weight.
+  static_assert(kCluster * kWarps == 128, "a lane has four stretches");
+  double before = 0;  // of lane's first stretch; then of the one that was found
+  int found = -1;
+  {
+    const double *all = &all_sums[2][0][0] + 4 * lane;
+    double incl = all[0] + all[1] + all[2] + all[3];
+    const double own = incl;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    double run = incl - own;
+    int over = -1, last = -1;
+    double over_at = 0, last_at = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (all[e] > 0) {
+        last = 4 * lane + e, last_at = run;
+        if (over < 0 && run + all[e] > goal) over = last, over_at = run;
+      }
+      run += all[e];
+    }
+    const unsigned overs = __ballot_sync(0xffffffffu, over >= 0), lasts = __ballot_sync(0xffffffffu, last >= 0);
+    const int from = overs ? __ffs(overs) - 1 : lasts ? 31 - __clz(lasts) : 0;
+    found = __shfl_sync(0xffffffffu, overs ? over : last, from);
+    before = __shfl_sync(0xffffffffu, overs ? over_at : last_at, from);
+  }
+  if (found == mine) {
+    double run = before;
+    int token = -1, last = -1;
+    for (int base = v0; base < v1 && token < 0; base += 32) {
+      const int v = base + lane;
+      const double w = v < v1 ? weight(v) : 0.0;
+      double incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, w > 0 && run + incl > goal), any = __ballot_sync(0xffffffffu, w > 0);
+      if (over) token = base + __ffs(over) - 1;
+      if (any) last = base + 31 - __clz(any);
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (token < 0) token = last;  // (rounding)
+    if (lane == 0) {
+      p.tokens[out0 + kept] = token;
+      const double z = (static_cast<double>(read(p, pr, token)) - top[kept]) / hot;
+      p.logprobs[out0 + kept] = static_cast<float>(z - log(static_cast<double>(total[kept])));
+    }
+  }
+  if (found < 0 && mine == 0 && lane == 0) {  // (no token has weight: the only one was drafted and is not kept)
+    p.tokens[out0 + kept] = -1;
+    p.logprobs[out0 + kept] = 0.f;
+  }
+  sync_cluster();  // no CTA's sums go away while another reads them
+}
+
+template <typename T>
+int scan(const Params &p, int64_t ctas, cudaStream_t s, const char *what) {
+  return launch_overlapped(verify_scan_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(kScan), 0, s, what, p);
+}
+
+inline bool sizes_fit(int64_t batch, int64_t drafts, int64_t vocab) {
+  return batch >= 0 && batch <= (1LL << 20) && drafts >= 0 && drafts <= kMaxDrafts && vocab > 0 && vocab <= (1LL << 30);
+}
+
+}  // namespace verify
+}  // namespace mq
+
+extern "C" size_t mq_verify_workspace_size(int64_t batch, int64_t drafts, int64_t vocab) {
+  using namespace mq::verify;
+  if (batch <= 0 || !sizes_fit(batch, drafts, vocab)) return 0;
+  const int64_t rows = batch * (2 * drafts + 1);  // (without draft logits there are fewer rows, with more splits)
+  return sizeof(float2) * std::max(rows * splits_for(rows, vocab), batch * (drafts + 1) * splits_for(batch * (drafts + 1), vocab));
+}
+
+extern "C" int mq_verify_drafts(const void *target, int64_t ld_target, const void *draft, int64_t ld_draft, int dtype,
+                                const int32_t *drafted, const int32_t *counts, const float *uniform, const float *temperature,
+                                int32_t *tokens, int32_t *accepted, float *logprobs, int64_t batch, int64_t drafts, int64_t vocab,
+                                void *workspace, size_t workspace_bytes, void *stream) {
+  using namespace mq::verify;
+  const char *what = "mq_verify_drafts";
+  MQ_REQUIRE(batch >= 0 && drafts >= 0 && vocab > 0, MQ_EINVAL, "%s: bad shape", what);
+  MQ_REQUIRE(sizes_fit(batch, drafts, vocab), MQ_EUNSUPPORTED, "%s: batch is above 2^20, drafts above %d or vocab above 2^30", what,
+             kMaxDrafts);
+  MQ_REQUIRE(dtype == MQ_F32 || dtype == MQ_F16 || dtype == MQ_BF16, MQ_EINVAL, "%s: the logits' type must be MQ_F32, MQ_F16 or MQ_BF16",
+             what);
+  MQ_REQUIRE(ld_target >= vocab && (!draft || ld_draft >= vocab), MQ_EINVAL, "%s: the logits' row stride is less than vocab", what);
+  if (batch == 0) return MQ_OK;
+  MQ_REQUIRE(target && uniform && tokens && accepted && logprobs && workspace && (drafted || drafts == 0), MQ_EINVAL, "%s: null pointer",
+             what);
+  const int es = dtype == MQ_F32 ? 4 : 2;
+  MQ_REQUIRE(mq::aligned(target, es) && mq::aligned(draft, es) && mq::aligned(drafted, 4) && mq::aligned(counts, 4) &&
+                 mq::aligned(uniform, 4) && mq::aligned(temperature, 4) && mq::aligned(tokens, 4) && mq::aligned(accepted, 4) &&
+                 mq::aligned(logprobs, 4) && mq::aligned(workspace, 16),
+             MQ_EALIGN, "%s: the workspace must be 16-byte aligned, the others aligned to their elements", what);
+  MQ_REQUIRE(workspace_bytes >= mq_verify_workspace_size(batch, drafts, vocab), MQ_EINVAL, "%s: the workspace is too small", what);
+  mq::DeviceInfo dev;
+  if (int rc = mq::device_info(&dev)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (drafts == 0) draft = nullptr;
+  const int64_t rows = batch * (draft ? 2 * drafts + 1 : drafts + 1);
+  Params p{target, draft, ld_target, ld_draft, drafted, counts, uniform, temperature, static_cast<float2 *>(workspace), tokens, accepted,
+           logprobs, static_cast<int>(batch), static_cast<int>(drafts), static_cast<int>(vocab), splits_for(rows, vocab), dtype};
+  int rc;
+  if (dtype == MQ_F32)
+    rc = scan<float>(p, rows * p.splits, s, what);
+  else if (dtype == MQ_F16)
+    rc = scan<__half>(p, rows * p.splits, s, what);
+  else
+    rc = scan<__nv_bfloat16>(p, rows * p.splits, s, what);
+  if (rc) return rc;
+  return mq::launch_overlapped_clusters(verify_draw_kernel, dim3(static_cast<unsigned>(batch * kCluster)), dim3(kDraw), kCluster, 0, s,
+                                        what, p);
+}

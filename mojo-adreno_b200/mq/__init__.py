@@ -14,4 +14,6 @@ from .pack import *  # noqa: F401,F403
 from .int8 import *  # noqa: F401,F403
 from .norm import *  # noqa: F401,F403
 from .beam import *  # noqa: F401,F403
+from .paged import *  # noqa: F401,F403
+from .verify import *  # noqa: F401,F403
 from .formats import GGUF, Manifest, read_file_to_device, read_gguf  # noqa: F401

@@ -67,6 +67,16 @@ SIGNATURES = {
                                c_size, c_vp]),
     "mq_beam_reorder": (c_int, [c_vp, c_int, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_i64, c_vp]),
     "mq_beam_reorder_check": (c_int, [c_vp, c_int, c_vp, c_i64, c_int, c_i64, c_vp, c_vp, c_i64]),
+    "mq_kv_store": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64,
+                            c_vp]),
+    "mq_kv_load": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int,
+                           c_vp]),
+    "mq_paged_attention_workspace_size": (c_size, [c_vp, c_i64, c_i64, c_i64, c_i64]),
+    "mq_paged_attention": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
+                                   c_f32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_size, c_vp]),
+    "mq_verify_workspace_size": (c_size, [c_i64, c_i64, c_i64]),
+    "mq_verify_drafts": (c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
+                                 c_i64, c_vp, c_size, c_vp]),
     "mq_read_file_to_device": (c_int, [c_vp, c_i64, c_char_p, c_i64, c_vp]),
     "mq_pack_half": (c_int, [c_vp, c_vp, c_i64, c_vp]),
 }

@@ -17,6 +17,7 @@ MQ_S8 = 3
 
 
 _device = getattr(torch._C, "_cuda_getDevice", None)
+_current_device = _device or torch.cuda.current_device
 
 
 def _stream():

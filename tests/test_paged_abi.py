@@ -1,0 +1,126 @@
+"""The refusals of the paged cache, the attention over it and the verification of drafted tokens, without a GPU: arguments are
+checked before a device is touched."""
+import ctypes
+
+import pytest
+
+P = ctypes.c_void_p
+OK = 1 << 20  # never dereferenced: validation fails first
+
+
+def pages(**kw):
+    from mq.paged import _Pages, _Three
+
+    p = _Pages(k=OK, v=OK, k_scale=OK, v_scale=OK, k_stride=_Three(2 * 16 * 64, 16 * 64, 64), v_stride=_Three(2 * 16 * 64, 16 * 64, 64),
+               ks_stride=_Three(32, 16, 1), vs_stride=_Three(32, 16, 1), pages=8, dtype=1, heads=2, page=16, dim=64)
+    for name, value in kw.items():
+        setattr(p, name, _Three(*value) if isinstance(value, tuple) else value)
+    return p
+
+
+def status(name, *args):
+    from mq._lib import lib
+
+    rc = getattr(lib, name)(*args)
+    return rc, lib.mq_last_error().decode()
+
+
+def attention(cache=None, **kw):
+    a = dict(q=OK, q_dtype=1, q_token=512, q_head=64, table=OK, ldt=4, width=4, lengths=OK, starts=OK, batch=2, tokens=5, heads=8,
+             scale=0.125, window=0, max_new=0, out=OK, o_token=512, o_head=64, workspace=OK, size=16)
+    a.update(kw)
+    c = pages() if cache is None else cache
+    return status("mq_paged_attention", a["q"], a["q_dtype"], a["q_token"], a["q_head"], ctypes.addressof(c), a["table"], a["ldt"],
+                  a["width"], a["lengths"], a["starts"], a["batch"], a["tokens"], a["heads"], a["scale"], a["window"], a["max_new"],
+                  a["out"], a["o_token"], a["o_head"], a["workspace"], a["size"], None)
+
+
+@pytest.mark.parametrize("cache,code,match", [
+    (dict(k=None), -1, "null"), (dict(dtype=0), -1, "type"), (dict(dtype=4), -1, "type"), (dict(pages=0), -1, "pages"),
+    (dict(heads=0), -1, "heads"), (dict(page=8), -4, "page"), (dict(page=48), -4, "page"), (dict(page=512), -4, "page"),
+    (dict(dim=8), -4, "dim"), (dict(dim=72), -4, "dim"), (dict(dim=144), -4, "dim"), (dict(k=OK + 8), -2, "aligned"),
+    (dict(v_stride=(2 * 16 * 64, 16 * 64, 68)), -2, "aligned"), (dict(k_stride=(2 * 16 * 64, 16 * 64, 56)), -1, "overlap"),
+    (dict(k_stride=(0, 16 * 64, 64)), -1, "overlap"), (dict(k_stride=(-2048, 16 * 64, 64)), -1, "overlap"),
+    (dict(k_stride=(1 << 40, 16 * 64, 64)), -1, "overlap"), (dict(dtype=3, v_scale=None), -1, "scales"),
+    (dict(dtype=3, ks_stride=(32, 16, 0)), -1, "overlap"), (dict(dtype=3, k_scale=OK + 2), -2, "aligned"),
+])
+def test_caches(cache, code, match):
+    c = pages(**cache)
+    for rc, msg in (attention(c), status("mq_kv_store", OK, 128, 64, OK, 128, 64, 1, ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, None),
+                    status("mq_kv_load", ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, OK, 128, 64, OK, 128, 64, 1, None)):
+        assert rc == code and match in msg
+
+
+@pytest.mark.parametrize("args,code,match", [
+    (dict(batch=-1), -1, "shape"), (dict(tokens=-1), -1, "shape"), (dict(width=-1), -1, "shape"), (dict(batch=1 << 22), -4, "too many"),
+    (dict(tokens=1 << 30), -4, "too many"), (dict(width=1 << 40), -4, "positions"), (dict(width=1 << 27, ldt=1 << 27), -4, "positions"),
+    (dict(starts=None), -1, "one row"), (dict(lengths=None), -1, "null"), (dict(table=None), -1, "null"),
+    (dict(lengths=OK + 2), -2, "aligned"), (dict(ldt=3), -1, "stride"), (dict(heads=0), -1, "multiple"), (dict(heads=7), -1, "multiple"),
+    (dict(heads=1 << 17), -4, "heads"), (dict(q_dtype=0), -1, "q must"), (dict(q_dtype=2), -1, "16-bit cache"), (dict(scale=0.0), -1, "scale"),
+    (dict(scale=-1.0), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(scale=float("nan")), -1, "scale"),
+    (dict(window=-1), -1, "window"), (dict(window=1 << 31), -4, "window"), (dict(max_new=-1), -1, "new tokens"), (dict(q=None), -1, "null"),
+    (dict(q=OK + 2), -2, "q must start"), (dict(q_token=500), -2, "q must start"), (dict(q_head=-64), -1, "negative"),
+    (dict(out=None), -1, "null"), (dict(out=OK + 8), -2, "out must start"), (dict(o_token=448), -1, "overlap"), (dict(o_head=0), -1, "overlap"),
+])
+def test_attention(args, code, match):
+    rc, msg = attention(**args)
+    assert rc == code and match in msg, msg
+
+
+def test_attention_of_nothing():
+    assert attention(tokens=0)[0] == 0 and attention(batch=0, tokens=0, starts=None)[0] == 0
+
+
+@pytest.mark.parametrize("args,code,match", [(dict(dtype=3), -1, "rows must"), (dict(k=None), -1, "null"), (dict(k=OK + 4), -2, "k must start"),
+                                           (dict(vt=100), -2, "v must start"), (dict(kh=-64), -1, "negative")])
+def test_copies(args, code, match):
+    a = dict(k=OK, kt=128, kh=64, v=OK, vt=128, vh=64, dtype=1)
+    a.update(args)
+    c = pages()
+    rows = (a["k"], a["kt"], a["kh"], a["v"], a["vt"], a["vh"])
+    where = (ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5)
+    for rc, msg in (status("mq_kv_store", *rows, a["dtype"], *where, None), status("mq_kv_load", *where, *rows, a["dtype"], None)):
+        assert rc == code and match in msg, msg
+
+
+def test_load_into_rows_that_overlap():
+    rc, msg = status("mq_kv_load", ctypes.addressof(pages()), OK, 4, 4, OK, OK, 2, 5, OK, 64, 64, OK, 128, 64, 1, None)
+    assert rc == -1 and "overlap" in msg
+
+
+@pytest.mark.parametrize("args,code,match", [
+    (dict(batch=-1), -1, "shape"), (dict(vocab=0), -1, "shape"), (dict(drafts=-1), -1, "shape"), (dict(drafts=33), -4, "drafts above"),
+    (dict(batch=1 << 21), -4, "batch"), (dict(vocab=1 << 31, ld=1 << 31), -4, "vocab"), (dict(dtype=3), -1, "type"), (dict(ld=99), -1, "stride"),
+    (dict(ld_draft=99), -1, "stride"), (dict(target=None), -1, "null"), (dict(drafted=None), -1, "null"), (dict(uniform=None), -1, "null"),
+    (dict(tokens=None), -1, "null"), (dict(target=OK + 2), -2, "aligned"), (dict(workspace=OK + 8), -2, "aligned"), (dict(size=16), -1, "too small"),
+])
+def test_verify(args, code, match):
+    a = dict(target=OK, ld=100, draft=OK, ld_draft=100, dtype=0, drafted=OK, counts=None, uniform=OK, temperature=None, tokens=OK, accepted=OK,
+             logprobs=OK, batch=2, drafts=3, vocab=100, workspace=OK, size=1 << 20)
+    a.update(args)
+    rc, msg = status("mq_verify_drafts", *a.values(), None)
+    assert rc == code and match in msg, msg
+    assert status("mq_verify_drafts", *{**a, **dict(batch=0, drafts=3, vocab=100, dtype=0, ld=100, ld_draft=100)}.values(), None)[0] == 0
+
+
+def test_workspace_sizes_of_what_is_refused():
+    from mq._lib import lib
+
+    assert lib.mq_verify_workspace_size(1 << 21, 3, 100) == 0 and lib.mq_verify_workspace_size(2, 33, 100) == 0
+    assert lib.mq_verify_workspace_size(2, 3, 100) > 0
+    assert lib.mq_paged_attention_workspace_size(ctypes.addressof(pages(dim=8)), 8, 2, 5, 0) == 0
+    assert lib.mq_paged_attention_workspace_size(ctypes.addressof(pages()), 7, 2, 5, 0) == 0
+
+
+def test_python_operators_refuse_cpu_tensors():
+    import torch
+
+    import mq
+
+    x = torch.zeros(2, 2, 16, 64, dtype=torch.float16)
+    with pytest.raises(mq.MQError, match="CUDA"):
+        mq.PagedCache(x, x)
+    with pytest.raises(mq.MQError, match="CUDA"):
+        mq.verify_drafts(torch.zeros(4, 10), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, 4))
+    with pytest.raises(mq.MQError, match="PagedCache"):
+        mq.kv_store(x[0], x[0], None, None, None)

@@ -1,0 +1,593 @@
+"""The paged cache and the attention over it, against the oracle in 64 bits.
+
+Bound of an output, from the roundings on its way (u = eps / 2 of a type): the output's own, u |o|; the weights', u of the
+cache's type (int8: fp16) each, in the sum over the values and in the sum of weights, 2 u sum_j p_j |v_j|; the scores', whose
+absolute error e in the exponent changes a weight by a factor 1 + e, in both sums: e <= (dim + 16) 2^-23 times the
+largest scale sum_d |q_d k_jd| (fp32 products and sums in any order, and the scaling), and int8's q, exact down to 2^-25 of its
+largest, 2^-25 max|q| scale sum_d |k_jd|; 2^-19 for the exponentials, the rescaling and the division.
+A weight of an fp16 product below 2^-14 is subnormal there: its error is up to 2^-25 absolute, not relative to it. The largest
+weight is 1 or more there, so in units of the sums that is 2^-25 max_j p_j times each |v_j|; int8's weights are p_j t_j, with t_j the
+value's scale, and meet the integers v_j / t_j: 2^-25 max_j (p_j t_j) sum_j |v_j| / t_j. It counts where the keys that have the weight
+have values near 0."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged, serving
+
+import mq
+
+pytestmark = pytest.mark.gpu
+F16, BF16, S8, F32 = torch.float16, torch.bfloat16, torch.int8, torch.float32
+UNIT = {F16: 2.0 ** -11, BF16: 2.0 ** -8, F32: 2.0 ** -24}
+
+
+def host(t):
+    return t.double().cpu().numpy()
+
+
+class Batch:
+    """Sequences of (new tokens, length), their table and starts. The pool's other positions hold NaN (int8: NaN scales),
+    the table's other entries nonsense; order "position" lays a page's rows out position by position."""
+
+    def __init__(self, cuda, sizes, kv_heads, page, dim, dtype, order="head", seed=0, spare=2, gap=0, scale_v=1.0):
+        self.g = torch.Generator(device=cuda).manual_seed(seed)
+        rng = np.random.default_rng(seed)
+        self.sizes, self.cuda, self.dtype = sizes, cuda, dtype
+        need = [-(-max(length, 0) // page) for _, length in sizes]
+        pages = sum(need) + spare
+        shape = (pages, kv_heads, page, dim) if order == "head" else (pages, page, kv_heads, dim)
+        self.ints = dtype == S8
+
+        def pool():
+            if self.ints:
+                t = torch.randint(-128, 128, shape, generator=self.g, device=cuda, dtype=torch.int32).to(S8)
+            else:
+                t = torch.full(shape, float("nan"), device=cuda, dtype=dtype)
+            return t if order == "head" else t.transpose(1, 2)
+
+        self.k, self.v = pool(), pool()
+        self.scales = [torch.full((pages, kv_heads, page), float("nan"), device=cuda) for _ in range(2)] if self.ints else [None, None]
+        ids = rng.permutation(pages)
+        table = np.full((len(sizes), max(max(need), 1) + 1), -7, np.int32)
+        table[:, -1] = 1 << 30
+        at = 0
+        for b, n in enumerate(need):
+            table[b, :n] = ids[at:at + n]
+            at += n
+        self.np_table = table
+        self.table = torch.from_numpy(table).to(cuda)
+        self.lengths = torch.tensor([length for _, length in sizes], dtype=torch.int32, device=cuda)
+        starts = [gap]
+        for n, _ in sizes:
+            starts.append(starts[-1] + n)
+        self.np_starts, self.tokens = starts, starts[-1] + gap
+        self.starts = torch.tensor(starts, dtype=torch.int32, device=cuda)
+        self.page, self.kv_heads, self.dim = page, kv_heads, dim
+        for b, (_, length) in enumerate(sizes):
+            if length <= 0:
+                continue
+            j = torch.arange(length, device=cuda)
+            of, row = self.table[b][j // page].long(), j % page
+            for t, sc in zip((self.k, self.v), self.scales):
+                x = torch.randn(length, kv_heads, dim, generator=self.g, device=cuda)
+                if self.ints:
+                    t[of, :, row] = (x * 40).round().clamp(-127, 127).to(S8)
+                    sc[of, :, row] = torch.rand(length, kv_heads, generator=self.g, device=cuda) * 0.05 + 0.001
+                else:
+                    t[of, :, row] = x.to(dtype)
+        if self.ints:
+            self.scales[1] *= scale_v
+
+    def cache(self):
+        return mq.PagedCache(self.k, self.v, *self.scales)
+
+    def where(self):
+        return self.table, self.lengths, self.starts
+
+    def held(self, b, length):
+        """keys, values [kv_heads, length, dim] in 64 bits, and the values' scales [kv_heads, length] (None: 16-bit)."""
+        out, steps = [], None
+        for t, sc in zip((self.k, self.v), self.scales):
+            j = torch.arange(max(length, 0), device=self.cuda)
+            of, row = self.table[b][j // self.page].long(), j % self.page
+            x = t[of, :, row].double()
+            if self.ints:
+                x = x * sc[of, :, row].double()[..., None]
+                steps = host(sc[of, :, row].transpose(0, 1))
+            out.append(host(x.transpose(0, 1)))
+        return *out, steps
+
+    def check(self, out, q, scale, window=0):
+        got, qh = host(out), host(q)
+        unit, unit_w = UNIT[q.dtype], UNIT[F16 if self.ints else self.dtype]
+        for b, (n, length) in enumerate(self.sizes):
+            if n == 0:
+                continue
+            s0 = self.np_starts[b]
+            keys, values, steps = self.held(b, length)
+            rows = qh[s0:s0 + n]
+            ref, size, tiny = paged.attention(rows, keys, values, range(length - n, length), scale, window, steps)
+            group = rows.shape[1] // self.kv_heads
+            if keys.shape[1]:
+                big = scale * np.einsum("thd,hjd->thj", np.abs(rows), np.repeat(np.abs(keys), group, 0)).max(-1)
+                small = 2.0 ** -25 * scale * np.abs(rows).max(-1) * np.repeat(np.abs(keys).sum(-1).max(-1), group)[None] if self.ints else 0
+            else:
+                big = small = np.zeros(rows.shape[:2])
+            e = (self.dim + 16) * 2.0 ** -23 * big + small
+            bound = unit * np.abs(ref) + (2 * unit_w + 2 * e + 2.0 ** -19)[..., None] * size + 2.0 ** -24 * (q.dtype == F16) + \
+                2.0 ** -25 * tiny * (self.dtype != BF16)
+            bad = ~(np.abs(got[s0:s0 + n] - ref) <= bound)
+            assert not bad.any(), (b, n, length, int(bad.sum()), np.argwhere(bad)[:3], np.nanmax(np.abs(got[s0:s0 + n] - ref) / bound))
+
+
+def attend(batch, heads, dtype, scale=None, window=0, max_new=0, **kw):
+    q = (torch.randn(batch.tokens, heads, batch.dim, generator=batch.g, device=batch.cuda) * 2).to(dtype)
+    out = torch.full_like(q, 7.0)
+    mq.device_status()
+    got = mq.paged_attention(q, batch.cache(), *batch.where(), out=out, scale=scale, window=window, max_new=max_new, **kw)
+    assert mq.device_status() == 0
+    assert got is out
+    lo, hi = batch.np_starts[0], batch.np_starts[-1]
+    assert (out[:lo] == 7).all() and (out[hi:] == 7).all(), "rows of no sequence are left as they are"
+    batch.check(out, q, batch.dim ** -0.5 if scale is None else scale, window)
+    return q, out
+
+
+CACHES = [(F16, F16), (BF16, BF16), (S8, F16), (S8, BF16)]
+ONE = [(1, 1), (1, 2), (1, 63), (1, 64), (1, 65), (1, 333)]
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("kv_heads,group,page,dim,order", [(1, 1, 16, 64, "head"), (2, 4, 16, 128, "position"), (3, 5, 64, 96, "head"),
+                                                         (8, 8, 128, 64, "position"), (1, 16, 256, 128, "head"), (2, 3, 32, 16, "head")])
+def test_one_token_each(cuda, cache, x, kv_heads, group, page, dim, order):
+    attend(Batch(cuda, ONE, kv_heads, page, dim, cache, order, gap=2), kv_heads * group, x)
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+def test_one_token_each_without_starts(cuda, cache, x):
+    batch = Batch(cuda, ONE, 2, 16, 64, cache)
+    q = torch.randn(len(ONE), 8, 64, generator=batch.g, device=cuda).to(x)
+    out = mq.paged_attention(q, batch.cache(), batch.table, batch.lengths)
+    batch.check(out, q, 64 ** -0.5)
+
+
+FEW = [(5, 5), (1, 300), (0, 40), (3, 64), (7, 65), (4, 2), (1, 0), (6, 200)]
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("kv_heads,group,page,dim,max_new", [(2, 2, 16, 128, 7), (1, 4, 32, 128, 7), (2, 8, 64, 64, 7), (2, 1, 16, 112, 0),
+                                                           (1, 9, 16, 128, 7)])
+def test_few_tokens(cuda, cache, x, kv_heads, group, page, dim, max_new):
+    attend(Batch(cuda, FEW, kv_heads, page, dim, cache, gap=1), kv_heads * group, x, max_new=max_new)
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("window", [1, 2, 64, 100])
+def test_window(cuda, cache, x, window):
+    attend(Batch(cuda, FEW + [(40, 400), (129, 129)], 2, 16, 64, cache), 8, x, window=window)
+
+
+MANY = [(65, 65), (1, 77), (128, 128), (129, 700), (0, 9), (300, 300), (17, 17)]
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("kv_heads,group,page,dim,order", [(1, 1, 16, 64, "head"), (2, 4, 32, 128, "position"), (2, 3, 128, 96, "head"),
+                                                         (1, 8, 256, 128, "head"), (2, 5, 64, 32, "position")])
+def test_many_tokens(cuda, cache, x, kv_heads, group, page, dim, order):
+    attend(Batch(cuda, MANY, kv_heads, page, dim, cache, order, gap=3), kv_heads * group, x)
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+def test_more_heads_than_a_tile_of_rows(cuda, cache, x):
+    attend(Batch(cuda, [(1, 70), (3, 90)], 1, 16, 64, cache), 71, x)
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_context_split_over_the_gpu(cuda, cache, x, dim):
+    attend(Batch(cuda, [(1, 20011)], 1, 64, dim, cache), 4, x)
+    attend(Batch(cuda, [(3, 5000), (1, 3), (2, 9001)], 1, 16, dim, cache), 8, x, max_new=3)
+    attend(Batch(cuda, [(40, 6011)], 1, 64, dim, cache), 4, x)
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+def test_more_positions_than_new_tokens_and_fewer(cuda, cache, x):
+    """Rows at positions below 0 see nothing and give zeros."""
+    sizes = [(4, 2), (100, 37), (3, 0), (90, 0)]
+    batch = Batch(cuda, sizes, 2, 16, 64, cache)
+    _, out = attend(batch, 8, x)
+    assert (out[:2] == 0).all() and (out[2:4] != 0).any()
+    assert (out[4:67] == 0).all() and (out[104:] == 0).all()
+
+
+@pytest.mark.parametrize("cache", [F16, BF16])
+@pytest.mark.parametrize("n,length", [(6, 70), (200, 260)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_what_a_row_does_not_see_does_not_matter(cuda, cache, n, length, which, value):
+    """A value that is no number at a new position, and one at an old position behind the window."""
+    batch = Batch(cuda, [(n, length), (1, 40)], 2, 16, 64, cache)
+    q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).to(cache)
+    window = 50
+    clean = mq.paged_attention(q, batch.cache(), *batch.where(), window=window)
+    at = length - n // 2
+    pool = batch.k if which == "k" else batch.v
+    for j in (at, 3):
+        pool[batch.table[0, j // 16].long(), :, j % 16, 5] = value
+    got = mq.paged_attention(q, batch.cache(), *batch.where(), window=window)
+    pos = torch.arange(length - n, length)
+    sees = torch.zeros(n, dtype=torch.bool)
+    for j in (at, 3):
+        sees |= (pos >= j) & (pos - window < j)
+    assert torch.equal(got[:n][~sees].nan_to_num(9.0), clean[:n][~sees])
+    assert torch.equal(got[n:], clean[n:])
+    if value != value or which == "v":
+        assert not got[:n][sees][..., 5].isfinite().any()
+
+
+def test_int8_scales_that_are_no_numbers(cuda):
+    batch = Batch(cuda, [(6, 70), (200, 260)], 2, 16, 64, S8)
+    q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).bfloat16()
+    clean = mq.paged_attention(q, batch.cache(), *batch.where())
+    for b, (n, length) in enumerate(batch.sizes):
+        j = length - 3
+        batch.scales[1][batch.table[b, j // 16].long(), :, j % 16] = float("nan")
+    got = mq.paged_attention(q, batch.cache(), *batch.where())
+    for first, n in ((0, 6), (6, 200)):
+        assert torch.equal(got[first:first + n - 3], clean[first:first + n - 3])
+        assert got[first + n - 3:first + n].isnan().all()
+
+
+@pytest.mark.parametrize("scale_v", [1e-12, 1e-3, 1e4])
+def test_int8_value_scales_of_any_size(cuda, scale_v):
+    attend(Batch(cuda, [(1, 200), (5, 80), (100, 200)], 2, 16, 64, S8, scale_v=scale_v), 8, BF16)
+
+
+def test_int8_values_of_zero(cuda):
+    """Rows that were quantised from zeros have scale 0: they count with their weight and add nothing."""
+    batch = Batch(cuda, [(1, 200), (100, 200)], 2, 16, 64, S8)
+    for b, (n, length) in enumerate(batch.sizes):
+        for j in range(0, length, 2):
+            batch.v[batch.table[b, j // 16].long(), :, j % 16] = 0
+            batch.scales[1][batch.table[b, j // 16].long(), :, j % 16] = 0
+    attend(batch, 8, F16)
+
+
+def test_int8_queries_of_any_size(cuda):
+    batch = Batch(cuda, [(2, 100), (90, 150)], 1, 16, 64, S8)
+    q = (torch.randn(batch.tokens, 4, 64, generator=batch.g, device=cuda) * 10.0 ** torch.linspace(-6, 6, batch.tokens, device=cuda)[:, None, None])
+    q = q.bfloat16()
+    out = mq.paged_attention(q, batch.cache(), *batch.where(), scale=1e-5)
+    batch.check(out, q, 1e-5)
+
+
+@pytest.mark.parametrize("cache", [F16, BF16])
+def test_peaked_and_growing_scores(cuda, cache):
+    """Scores that grow along the sequence, so that the maximum keeps moving, and large ones."""
+    for n, length in ((1, 700), (130, 700)):
+        batch = Batch(cuda, [(n, length)], 1, 16, 64, cache)
+        j = torch.arange(length, device=cuda)
+        of, row = batch.table[0][j // 16].long(), j % 16
+        batch.k[of, :, row] = (batch.k[of, :, row].float() * (j / 30.0)[:, None, None]).to(cache)
+        attend(batch, 4, cache, scale=0.5)
+
+
+def test_strided_rows_and_in_place(cuda):
+    """q as a slice of a fused projection, out its own buffer; tables with a stride."""
+    batch = Batch(cuda, MANY, 2, 32, 64, BF16)
+    fused = torch.randn(batch.tokens, 12, 64, generator=batch.g, device=cuda).bfloat16()
+    q = fused[:, :8]
+    keep = fused.clone()
+    wide = torch.full((len(MANY), batch.table.shape[1] + 5), 99999, dtype=torch.int32, device=cuda)
+    wide[:, 2:2 + batch.table.shape[1]] = batch.table
+    table = wide[:, 2:2 + batch.table.shape[1]]
+    plain = mq.paged_attention(q.contiguous(), batch.cache(), *batch.where())
+    out = mq.paged_attention(q, batch.cache(), table, batch.lengths, batch.starts, out=q)
+    assert torch.equal(out, plain)
+    assert torch.equal(fused[:, 8:], keep[:, 8:])
+    heads_first = keep[:, :8].transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(mq.paged_attention(heads_first, batch.cache(), *batch.where()), plain)
+
+
+def test_results_do_not_vary(cuda):
+    batch = Batch(cuda, [(1, 3000), (5, 700), (300, 2000)], 2, 16, 128, BF16)
+    q = torch.randn(batch.tokens, 8, 128, generator=batch.g, device=cuda).bfloat16()
+    first = mq.paged_attention(q, batch.cache(), *batch.where())
+    for _ in range(5):
+        assert torch.equal(mq.paged_attention(q, batch.cache(), *batch.where()), first)
+
+
+def test_bad_pages_are_reported_and_read_as_zeros(cuda):
+    for n in (1, 90):
+        batch = Batch(cuda, [(n, 100), (1, 30)], 2, 16, 64, F16)
+        zero = Batch(cuda, [(n, 100), (1, 30)], 2, 16, 64, F16)
+        bad = zero.table[0, 2].long()
+        zero.k[bad] = 0
+        zero.v[bad] = 0
+        q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).half()
+        want = mq.paged_attention(q, zero.cache(), *zero.where())
+        mq.device_status()
+        for entry in (-1, batch.k.shape[0], 2 ** 31 - 1, -2 ** 31):
+            batch.table[0, 2] = entry
+            got = mq.paged_attention(q, batch.cache(), *batch.where())
+            assert mq.device_status() == 19
+            assert torch.equal(got, want)
+
+
+def test_bad_lengths_starts_and_counts_are_cut(cuda):
+    batch = Batch(cuda, [(2, 48), (70, 96)], 2, 16, 64, F16)
+    q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).half()
+    table = batch.table[:, :3].contiguous()
+    mq.device_status()
+    got = mq.paged_attention(q, batch.cache(), table, batch.lengths, batch.starts)
+    assert mq.device_status() == 20
+    shorter = batch.lengths.clamp(max=48)
+    assert torch.equal(got, mq.paged_attention(q, batch.cache(), table, shorter, batch.starts))
+    batch.lengths[0] = -5
+    got = mq.paged_attention(q, batch.cache(), *batch.where())
+    assert mq.device_status() == 20 and (got[:2] == 0).all()
+    batch.lengths[0] = 48
+    out = torch.full_like(q, 7.0)
+    mq.paged_attention(q, batch.cache(), *batch.where(), out=out, max_new=16)
+    assert mq.device_status() == 26 and (out[2:] == 7).all() and (out[:2] != 7).any()
+    starts = torch.tensor([-9, 2, 10 ** 6], dtype=torch.int32, device=cuda)
+    got = mq.paged_attention(q, batch.cache(), batch.table, batch.lengths, starts)
+    assert torch.equal(got, mq.paged_attention(q, batch.cache(), *batch.where()))
+    starts = torch.tensor([5, 3, 1], dtype=torch.int32, device=cuda)
+    mq.paged_attention(q, batch.cache(), batch.table, batch.lengths, starts)  # (no sequence has a row)
+    assert mq.device_status() == 0
+
+
+def test_nothing_to_do(cuda):
+    cache = mq.paged_cache(4, 2, 16, 64)
+    empty = torch.empty(0, 8, 64, device=cuda, dtype=F16)
+    table = torch.empty(0, 3, dtype=torch.int32, device=cuda)
+    none = torch.empty(0, dtype=torch.int32, device=cuda)
+    assert mq.paged_attention(empty, cache, table, none).shape == (0, 8, 64)
+    kv = torch.empty(0, 2, 64, device=cuda, dtype=F16)
+    mq.kv_store(kv, kv, cache, table, none)
+    mq.kv_load(cache, table, none)
+    # A table without entries, sequences of length 0.
+    table, lengths = torch.empty(3, 0, dtype=torch.int32, device=cuda), torch.zeros(3, dtype=torch.int32, device=cuda)
+    q = torch.randn(3, 8, 64, device=cuda).half()
+    assert (mq.paged_attention(q, cache, table, lengths) == 0).all()
+
+
+# ---- the cache's rows -------------------------------------------------------------------------------------
+
+STORED = [(5, 5), (1, 300), (0, 40), (31, 64), (7, 65), (4, 2), (1, 0), (60, 200)]
+
+
+def sources(batch, dtype):
+    k, v = (torch.randn(batch.tokens, batch.kv_heads, batch.dim, generator=batch.g, device=batch.cuda) for _ in range(2))
+    v[3::7] = 0
+    k *= 10.0 ** torch.randint(-3, 4, k.shape[:2], generator=batch.g, device=batch.cuda)[..., None]
+    if dtype == F32:
+        k[::5] *= 1e-35  # (rows below 1e-30 are quantised through a power of two)
+    return k.to(dtype), v.to(dtype)
+
+
+@pytest.mark.parametrize("x", [F32, F16, BF16])
+@pytest.mark.parametrize("cache", [F16, BF16, S8])
+@pytest.mark.parametrize("kv_heads,page,dim,order", [(1, 16, 64, "head"), (8, 16, 128, "position"), (3, 64, 96, "head"), (2, 256, 16, "position"),
+                                                   (40, 32, 48, "head")])
+def test_store_and_load(cuda, x, cache, kv_heads, page, dim, order):
+    batch = Batch(cuda, STORED, kv_heads, page, dim, cache, order, gap=2)
+    k, v = sources(batch, x)
+    before = [t.clone() for t in (batch.k, batch.v, *[s for s in batch.scales if s is not None])]
+    mq.device_status()
+    assert mq.kv_store(k, v, batch.cache(), *batch.where()).k is batch.k
+    assert mq.device_status() == 0
+    places = paged.places(batch.np_starts, batch.lengths.tolist(), batch.tokens)
+    after = (batch.k, batch.v, *[s for s in batch.scales if s is not None])
+    want = [t.clone() for t in before]
+    for i, t in enumerate((k, v)):
+        rows, scales = (torch.from_numpy(a).to(cuda) for a in serving.quantize_s8(t.float().cpu().numpy())) if cache == S8 else (t.to(cache), None)
+        for token, (b, p) in enumerate(places):
+            if b >= 0 and p >= 0:
+                of = int(batch.np_table[b, p // page])
+                want[i][of, :, p % page] = rows[token]
+                if cache == S8:
+                    want[2 + i][of, :, p % page] = scales[token]
+    for a, w in zip(after, want):
+        assert torch.equal(a.nan_to_num(nan=123.0) if a.is_floating_point() else a, w.nan_to_num(nan=123.0) if w.is_floating_point() else w)
+
+    for out in (F32, F16, BF16):
+        got = [torch.full((batch.tokens, kv_heads, dim), 7.0, device=cuda, dtype=out) for _ in range(2)]
+        mq.kv_load(batch.cache(), *batch.where(), k=got[0], v=got[1])
+        assert mq.device_status() == 0
+        for i, t in enumerate(got):
+            ref = torch.full_like(t, 7.0)
+            for token, (b, p) in enumerate(places):
+                if b >= 0:
+                    ref[token] = 0
+                    if p >= 0:
+                        of = int(batch.np_table[b, p // page])
+                        row = after[i][of, :, p % page].float()
+                        ref[token] = (row * after[2 + i][of, :, p % page][:, None] if cache == S8 else row).to(out)
+            assert torch.equal(t, ref)
+
+
+def test_store_not_numbers(cuda):
+    for cache in (S8, F16):
+        batch = Batch(cuda, [(9, 20)], 2, 16, 64, cache)
+        k, v = sources(batch, F32)
+        k[2, 1, 3], k[4, 0, 0], v[5, 1, 63] = float("nan"), float("inf"), float("-inf")
+        mq.kv_store(k, v, batch.cache(), *batch.where())
+        lk, lv = mq.kv_load(batch.cache(), *batch.where(), tokens=9, dtype=F32)
+        if cache == S8:
+            assert lk[2, 1].isnan().all() and lk[4, 0].isnan().all() and lv[5, 1].isnan().all()
+            assert lk[2, 0].isfinite().all() and lk[4, 1].isfinite().all()
+        else:
+            assert torch.equal(lk.isfinite(), k.half().isfinite()) and torch.equal(lv.isfinite(), v.half().isfinite())
+
+
+def test_store_strided_sources(cuda):
+    batch, same = (Batch(cuda, STORED, 2, 16, 64, S8) for _ in range(2))
+    fused = torch.randn(batch.tokens, 8 + 2 + 2, 64, generator=batch.g, device=cuda).bfloat16()
+    mq.kv_store(fused[:, 8:10], fused[:, 10:], batch.cache(), *batch.where())
+    mq.kv_store(fused[:, 8:10].contiguous(), fused[:, 10:].contiguous(), same.cache(), *same.where())
+    assert torch.equal(batch.k, same.k) and torch.equal(batch.v, same.v)
+    assert torch.equal(batch.scales[0].nan_to_num(), same.scales[0].nan_to_num())
+
+
+def test_store_and_load_bad_pages(cuda):
+    batch = Batch(cuda, [(40, 40), (3, 3)], 2, 16, 64, F16)
+    k, v = sources(batch, F16)
+    before = batch.k.clone()
+    missing = int(batch.table[0, 1])
+    mq.device_status()
+    for entry in (-1, batch.k.shape[0], 2 ** 31 - 1, -2 ** 31):
+        batch.table[0, 1] = entry
+        mq.kv_store(k, v, batch.cache(), *batch.where())
+        assert mq.device_status() == 19
+        assert torch.equal(batch.k[missing].nan_to_num(), before[missing].nan_to_num())
+        lk, lv = mq.kv_load(batch.cache(), *batch.where(), tokens=43)
+        assert mq.device_status() == 19
+        assert (lk[16:32] == 0).all() and torch.equal(lk[:16], k[:16]) and torch.equal(lk[32:], k[32:]) and torch.equal(lv[40:], v[40:])
+
+
+def test_store_then_attend_as_used(cuda):
+    """Prompt, chunk, single tokens: the int8 cache is written and read step by step, and the outputs are those of the
+    whole sequence at once."""
+    heads, kv_heads, dim, page = 8, 2, 64, 16
+    g = torch.Generator(device=cuda).manual_seed(5)
+    total = 150
+    q, k, v = (torch.randn(total, h, dim, generator=g, device=cuda).bfloat16() for h in (heads, kv_heads, kv_heads))
+    for dtype in (S8, BF16):
+        cache = mq.paged_cache(total // page + 2, kv_heads, page, dim, dtype)
+        table = torch.arange(total // page + 1, -1, -1, dtype=torch.int32, device=cuda)[None, :total // page + 1].contiguous()
+        outs, at = [], 0
+        for n in (100, 30, 5, 1, 1, 13):
+            lengths = torch.tensor([at + n], dtype=torch.int32, device=cuda)
+            starts = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+            mq.kv_store(k[at:at + n], v[at:at + n], cache, table, lengths, starts)
+            outs.append(mq.paged_attention(q[at:at + n], cache, table, lengths, starts))
+            at += n
+        starts = torch.tensor([0, total], dtype=torch.int32, device=cuda)
+        whole = mq.paged_attention(q, cache, table, lengths, starts)
+        unit = UNIT[BF16]
+        size = 8 * unit * v.float().abs().max()  # (two results, each within half of this of the exact one)
+        assert (torch.cat(outs).float() - whole.float()).abs().max() <= size
+        assert mq.device_status() == 0
+
+
+# ---- streams, graphs, refusals ----------------------------------------------------------------------------------
+
+
+def test_two_streams_at_once(cuda):
+    sizes = [(1, 900), (80, 300)]
+    batches = [Batch(cuda, sizes, 2, 16, 128, d, seed=i) for i, d in enumerate((BF16, S8))]
+    qs = [torch.randn(81, 8, 128, generator=b.g, device=cuda).bfloat16() for b in batches]
+    want = [mq.paged_attention(q, b.cache(), *b.where()) for q, b in zip(qs, batches)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(10):
+        for s, q, b in zip(streams, qs, batches):
+            with torch.cuda.stream(s):
+                got.append(mq.paged_attention(q, b.cache(), *b.where()))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g, want[i % 2])
+
+
+def test_captured_step(cuda):
+    """Store and attention in one graph, replayed as the lengths grow on the device."""
+    heads, kv_heads, dim, page, most = 8, 2, 64, 16, 64
+    g = torch.Generator(device=cuda).manual_seed(1)
+    for dtype in (F16, S8):
+        cache = mq.paged_cache(2 * most // page, kv_heads, page, dim, dtype)
+        table = torch.randperm(2 * most // page, generator=g, device=cuda).int().view(2, -1).contiguous()
+        lengths = torch.zeros(2, dtype=torch.int32, device=cuda)
+        q, k, v = (torch.empty(2, h, dim, device=cuda, dtype=F16) for h in (heads, kv_heads, kv_heads))
+        out = torch.empty_like(q)
+        work = torch.empty(mq.paged_attention_workspace(cache, heads, 2, 2, 1), dtype=torch.uint8, device=cuda)
+
+        def step():
+            lengths.add_(1)
+            mq.kv_store(k, v, cache, table, lengths)
+            mq.paged_attention(q, cache, table, lengths, out=out, workspace=work)
+
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.synchronize()
+        lengths.zero_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        lengths.zero_()
+        ks, vs = [], []
+        for i in range(20):
+            for t in (q, k, v):
+                t.copy_(torch.randn(t.shape, generator=g, device=cuda))
+            ks.append(k.clone())
+            vs.append(v.clone())
+            graph.replay()
+            want = mq.paged_attention(q, cache, table, lengths)
+            assert torch.equal(out, want)
+            if dtype == F16:
+                lk, lv = mq.kv_load(cache, table, lengths)
+                assert torch.equal(lk, k) and torch.equal(lv, v)
+                z = torch.einsum("bkgd,lbkd->bkgl", q.double().view(2, kv_heads, -1, dim), torch.stack(ks).double()) * dim ** -0.5
+                ref = torch.einsum("bkgl,lbkd->bkgd", z.softmax(-1), torch.stack(vs).double()).reshape(2, heads, dim)
+                # (fp16 output and weights: 3 units of the largest value; scores below 2^-17)
+                assert (out.double() - ref).abs().max() <= (3 * 2.0 ** -11 + 2.0 ** -16) * torch.stack(vs).abs().max()
+        assert mq.device_status() == 0
+
+
+def test_workspace_serves_smaller_calls(cuda):
+    batch = Batch(cuda, [(1, 900), (80, 300)], 2, 16, 128, BF16)
+    cache = batch.cache()
+    work = torch.empty(mq.paged_attention_workspace(cache, 8, 8, 4096), dtype=torch.uint8, device=cuda)
+    attend(batch, 8, BF16, workspace=work)
+    attend(Batch(cuda, ONE, 2, 16, 128, BF16), 8, BF16, workspace=work, max_new=1)
+
+
+def test_refusals(cuda):
+    cache = mq.paged_cache(4, 2, 16, 64)
+    table = torch.zeros(1, 4, dtype=torch.int32, device=cuda)
+    lengths = torch.ones(1, dtype=torch.int32, device=cuda)
+    q = torch.zeros(1, 8, 64, device=cuda, dtype=F16)
+    kv = torch.zeros(1, 2, 64, device=cuda, dtype=F16)
+
+    def refuses(match, call):
+        with pytest.raises(mq.MQError, match=match):
+            call()
+
+    refuses("type in", lambda: mq.paged_attention(q.float(), cache, table, lengths))
+    refuses("16-bit cache", lambda: mq.paged_attention(q.bfloat16(), cache, table, lengths))
+    refuses("multiple of the cache", lambda: mq.paged_attention(q[:, :3], cache, table, lengths))
+    refuses("does not go with", lambda: mq.paged_attention(q[..., :32].contiguous(), cache, table, lengths))
+    refuses("scale must be positive", lambda: mq.paged_attention(q, cache, table, lengths, scale=0.0))
+    refuses("scale must be positive", lambda: mq.paged_attention(q, cache, table, lengths, scale=float("nan")))
+    refuses("bad window", lambda: mq.paged_attention(q, cache, table, lengths, window=-1))
+    refuses("need starts", lambda: mq.paged_attention(q.expand(2, 8, 64).contiguous(), cache, table, lengths))
+    refuses("overlap", lambda: mq.paged_attention(q.expand(2, 8, 64).contiguous(), cache, table, lengths, torch.tensor([0, 2], dtype=torch.int32, device=cuda),
+                                                  out=torch.empty(1, 8, 64, device=cuda, dtype=F16).expand(2, 8, 64)))
+    refuses("workspace is too small", lambda: mq.paged_attention(q, cache, table, lengths, workspace=torch.empty(64, dtype=torch.uint8, device=cuda)))
+    refuses("16-byte aligned", lambda: mq.paged_attention(torch.zeros(1 * 8 * 64 + 4, device=cuda, dtype=F16)[4:].view(1, 8, 64), cache, table, lengths))
+    refuses("int32", lambda: mq.paged_attention(q, cache, table.long(), lengths))
+    refuses("lengths", lambda: mq.paged_attention(q, cache, table, lengths.long()))
+    refuses("lengths", lambda: mq.paged_attention(q, cache, table, lengths.expand(2).contiguous()))
+    refuses("starts", lambda: mq.paged_attention(q, cache, table, lengths, lengths))
+    refuses("CUDA|device", lambda: mq.paged_attention(q.cpu(), cache, table, lengths))
+    refuses("device", lambda: mq.paged_attention(q, cache, table.cpu(), lengths))
+    refuses("does not go with", lambda: mq.kv_store(kv[:, :1], kv[:, :1], cache, table, lengths))
+    refuses("k's type", lambda: mq.kv_store(kv, kv.float(), cache, table, lengths))
+    refuses("rows", lambda: mq.kv_load(cache, table, lengths, k=kv, v=kv, tokens=2))
+    refuses("PagedCache", lambda: mq.kv_store(kv, kv, None, table, lengths))
+    refuses("scales", lambda: mq.PagedCache(cache.k, cache.v, lengths, lengths))
+    refuses("int8 cache needs", lambda: mq.PagedCache(cache.k.to(S8), cache.v.to(S8)))
+    refuses("the same for keys", lambda: mq.PagedCache(cache.k, cache.v[:2]))
+    refuses("positions", lambda: mq.kv_store(kv, kv, mq.paged_cache(4, 2, 24, 64), table, lengths))
+    refuses("multiple of 16", lambda: mq.paged_attention(q[..., :40].contiguous(), mq.paged_cache(4, 2, 16, 40), table, lengths))
+    refuses("multiple of 16", lambda: mq.paged_attention(torch.zeros(1, 8, 256, device=cuda, dtype=F16), mq.paged_cache(4, 2, 16, 256), table, lengths))
+    wide = torch.zeros(4, 2, 16, 68, device=cuda, dtype=F16)[..., :64]
+    refuses("16-byte", lambda: mq.kv_store(kv, kv, mq.PagedCache(wide, wide.clone()), table, lengths))
+    flat = torch.zeros(1, 2, 16, 64, device=cuda, dtype=F16).expand(4, 2, 16, 64)
+    refuses("overlap", lambda: mq.kv_store(kv, kv, mq.PagedCache(flat, cache.v), table, lengths))
