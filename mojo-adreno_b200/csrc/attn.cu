@@ -30,6 +30,7 @@ namespace paged {
 
 constexpr int kFewKeys = 64, kFewRows = 64;  // keys of a block; the most rows of an item
 constexpr int kFewWarps = 4, kFewThreads = 32 * (kFewWarps + 1);
+using FewGrain = Grain<kFewRows, kFewKeys, 2>;
 constexpr int kPadCols = 72;                 // floats between rows of the joining buffer: no bank conflicts
 
 __device__ __forceinline__ float ex2(float x) {
@@ -162,11 +163,12 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
   }
   __syncthreads();
   griddep_wait();
-  const Share share = find_share<kFewThreads, kFewRows, kFewKeys>(p.seqs, p.shape, scratch);
+  const Share share = find_share<kFewThreads, FewGrain>(p.seqs, p.shape, scratch);
   if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = share.total, p.parts.counts[1] = share.parts;
   if (static_cast<int>(blockIdx.x) >= share.parts) return;
-  Walk<kFewRows, kFewKeys> walk;
+  Walk<FewGrain> walk;
   walk.start(p.seqs, p.shape, share);
+  if (tid == 0) p.parts.cuts[blockIdx.x] = cut_at(walk, p.shape, share);
   Item item;
 
   if (warp == kFewWarps) {
@@ -241,7 +243,6 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
   const int heads = p.shape.group;
   int s = 0;
   uint32_t phase = 0;
-  bool first_item = true;
   while (walk.next(p.seqs, p.shape, item)) {
     const int rows = item.s.n * heads;
     // A thread's rows are g and g + 8 of its warp's 16; q as the MMA's A, in registers.
@@ -250,12 +251,12 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
     int lo[2], hi[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = mt * 16 + g + 8 * r, i = min(row, rows - 1) / heads;
+      const int row = mt * 16 + g + 8 * r, i = over_group(p.shape, min(row, rows - 1));
       const int pos = item.s.pos0 + i;
       hi[r] = max(pos + 1, 0);
       lo[r] = p.shape.window ? max(0, pos + 1 - p.shape.window) : 0;
       row_scale[r] = p.scale;
-      const int64_t at = static_cast<int64_t>(item.s.first + i) * p.q_token + static_cast<int64_t>(item.head * heads + row % heads) * p.q_head;
+      const int64_t at = static_cast<int64_t>(item.s.first + i) * p.q_token + static_cast<int64_t>(item.head * heads + row - i * heads) * p.q_head;
       const bool real = row < rows;
       if constexpr (S8) {
         float v[D / 4];  // d = 64 h + 16 t + 0 .. 15: bytes that a 16-byte load of the keys brings to this thread
@@ -515,11 +516,6 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
       for (int j = 0; j < D / 8; ++j) o[j][2 * r] *= a, o[j][2 * r + 1] *= a;
     }
     const bool goes_on = item.before > 0, whole = !goes_on && item.blocks == item.whole;
-    if (first_item && tid == 0) {
-      Cut cut{item.b, item.head, item.tile, goes_on, share.begin - item.before, share.begin - item.before + item.whole};
-      p.parts.cuts[blockIdx.x] = cut;
-    }
-    first_item = false;
     const int64_t part0 = (2 * static_cast<int64_t>(blockIdx.x) + (goes_on ? 0 : 1)) * (16 * MT);
 #pragma unroll
     for (int h = 0; h < D / 64; ++h) {
@@ -558,9 +554,9 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
         if (row < rows) {
           if (whole) {
             const float inv = inverse_sum(sum);
+            const int i = over_group(p.shape, row);
             if (64 * h + col < p.o.dim)
-              store_out4(p.o, item.s.first + row / heads, item.head * heads + row % heads, 64 * h + col, v.x * inv, v.y * inv, v.z * inv,
-                         v.w * inv);
+              store_out4(p.o, item.s.first + i, item.head * heads + row - i * heads, 64 * h + col, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
           } else {
             *reinterpret_cast<float4 *>(p.parts.sums + (part0 + row) * D + 64 * h + col) = v;
             if (h == 0 && col == 0) p.parts.stats[part0 + row] = make_float2(top, sum);
@@ -622,11 +618,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const JoinParams p) {
   }
   if (row >= rows) return;
   const float inv = inverse_sum(sum);
-  const int r = cut.tile * TILE_ROWS + row;
+  const int r = cut.tile * TILE_ROWS + row, i = over_group(p.shape, r);
 #pragma unroll
   for (int k = 0; k < D / 32; ++k)
     if ((k * 8 + u) * 4 < p.o.dim)
-      store_out4(p.o, s.first + r / p.shape.group, cut.head * p.shape.group + r % p.shape.group, (k * 8 + u) * 4, v[k].x * inv,
+      store_out4(p.o, s.first + i, cut.head * p.shape.group + r - i * p.shape.group, (k * 8 + u) * 4, v[k].x * inv,
                  v[k].y * inv, v[k].z * inv, v[k].w * inv);
 }
 

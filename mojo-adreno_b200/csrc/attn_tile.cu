@@ -18,6 +18,11 @@ namespace paged {
 
 constexpr int kTileKeys = 128, kTileRows = 256;
 constexpr int kTileThreads = 384, kAuxWarps = 2;
+using TileGrain = Grain<kTileRows, kTileKeys, 2>;
+// Registers of a thread at launch, of a softmax thread (a row of scores is 128 of them) and of the others.
+constexpr int kTileRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 104;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kTileThreads * kTileRegs, "more registers than the block was launched with");
+constexpr int kStageBytes = 2048;  // per softmax warp: 64 bytes of each of its rows on their way out
 
 template <int D, int KIND>
 struct Tile {
@@ -28,7 +33,7 @@ struct Tile {
   static constexpr int kQ = kTileRows * D * 2;
   // All of shared memory, since it takes all of TMEM: no other CTA that wants TMEM then fits beside it.
   static constexpr int kSmem = 220 * 1024;
-  static_assert(kQ + kSlots * kBlock + 2 * kRaw + 1024 <= kSmem, "shared memory");
+  static_assert(kQ + kSlots * kBlock + 2 * kRaw + 8 * kStageBytes + 1024 <= kSmem, "shared memory");
 };
 
 // Row-major rows of 128 bytes, 128 of them to a 64-column part: where 16-byte chunk c of row r lies.
@@ -55,6 +60,15 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float (&v)[32]) 
         "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_loaded(float (&v)[32]) {
 #pragma unroll
@@ -65,6 +79,29 @@ __device__ __forceinline__ void tmem_loaded(float (&v)[32]) {
                    "+f"(v[i + 13]), "+f"(v[i + 14]), "+f"(v[i + 15]));
 }
 
+// (x, y) = (x, y) * a + b, and (x, y) = (x, y) + (a, b): two fp32 operations of one instruction.
+__device__ __forceinline__ void fma2(float &x, float &y, float ax, float ay, float bx, float by) {
+  asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%0, %1};\n mov.b64 q, {%2, %3};\n mov.b64 r, {%4, %5};\n"
+      " fma.rn.f32x2 p, p, q, r;\n mov.b64 {%0, %1}, p;\n}"
+      : "+f"(x), "+f"(y)
+      : "f"(ax), "f"(ay), "f"(bx), "f"(by));
+}
+__device__ __forceinline__ void add2(float &x, float &y, float ax, float ay) {
+  asm("{\n .reg .b64 p, q;\n mov.b64 p, {%0, %1};\n mov.b64 q, {%2, %3};\n add.rn.f32x2 p, p, q;\n mov.b64 {%0, %1}, p;\n}"
+      : "+f"(x), "+f"(y)
+      : "f"(ax), "f"(ay));
+}
+__device__ __forceinline__ void mul2(float &x, float &y, float ax, float ay) {
+  asm("{\n .reg .b64 p, q;\n mov.b64 p, {%0, %1};\n mov.b64 q, {%2, %3};\n mul.rn.f32x2 p, p, q;\n mov.b64 {%0, %1}, p;\n}"
+      : "+f"(x), "+f"(y)
+      : "f"(ax), "f"(ay));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <int D, int KIND>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attn_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
@@ -73,9 +110,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   constexpr int NS = T::kSlots, NF = S8 ? 2 : NS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock;
-  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full, q_empty, drained, s_full[2], p_full[2], o_full[2];
-  __shared__ ShareScratch<kTileThreads> scratch;
+  uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock, *stages = raw + 2 * T::kRaw;
+  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained, s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t bad_keys[NS][4];
   __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
   __shared__ uint32_t tmem_slot;
@@ -88,13 +124,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&q_full[i], kAuxWarps);
+      mbar_init(&q_empty[i], 1);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&ready[i], kAuxWarps);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(&q_full, kAuxWarps);
-    mbar_init(&q_empty, 1);
     mbar_init(&drained, 1);
     abort_flag = 0;
     fence_mbar_init();
@@ -106,13 +142,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_after();
   griddep_launch_dependents();
   const uint32_t tmem = tmem_slot;
-  const Share share = find_share<kTileThreads, kTileRows, kTileKeys>(p.seqs, p.shape, scratch);
+  ShareScratch<kTileThreads> &scratch = *reinterpret_cast<ShareScratch<kTileThreads> *>(ring);  // (nothing has been copied yet)
+  const Share share = find_share<kTileThreads, TileGrain>(p.seqs, p.shape, scratch);
+  __syncthreads();
   if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = share.total, p.parts.counts[1] = share.parts;
   const bool works = static_cast<int>(blockIdx.x) < share.parts;
   const int group = p.shape.group;
-  Walk<kTileRows, kTileKeys> walk;
+  Walk<TileGrain> walk;
   Item item;
-  if (works) walk.start(p.seqs, p.shape, share);
+  if (works) {
+    walk.start(p.seqs, p.shape, share);
+    if (tid == 0) p.parts.cuts[blockIdx.x] = cut_at(walk, p.shape, share);
+  }
   // Waits that give up set the flag, and everybody leaves at the next wait.
   auto wait = [&](uint64_t *bar, uint32_t parity, int code) -> bool {
     if (!abort_flag && mbar_wait(bar, parity)) return true;
@@ -124,13 +165,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   };
   // Rows of an item's two tiles; whether some row of the item sees a block only in part.
   auto rows_of = [&](const Item &it) { return min(kTileRows, it.s.n * group - it.tile * kTileRows); };
-  auto least_hi = [&](const Item &it) { return max(it.s.pos0 + it.tile * kTileRows / group + 1, 0); };
+  auto least_hi = [&](const Item &it) { return max(it.s.pos0 + over_group(p.shape, it.tile * kTileRows) + 1, 0); };
   auto most_lo = [&](const Item &it) {
-    return p.shape.window ? max(0, it.s.pos0 + (it.tile * kTileRows + rows_of(it) - 1) / group + 1 - p.shape.window) : 0;
+    return p.shape.window ? max(0, it.s.pos0 + over_group(p.shape, it.tile * kTileRows + rows_of(it) - 1) + 1 - p.shape.window) : 0;
   };
 
   if (!works) {
-  } else if (warp == 8) {
+  } else if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp == 8) {
     if (lane == 0) {
       prefetch_tmap(&kmap);
       prefetch_tmap(&vmap);
@@ -178,8 +221,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (lane == 0) {
       constexpr uint32_t qk = idesc_16(128, kTileKeys, BF, false), pv = idesc_16(128, D, BF, true);
       int64_t n = 0;  // slots used: keys and values in turn
-      int items = 0;
-      uint32_t p_phase[2] = {0, 0};
+      uint32_t p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
       bool ok = true;
       auto slot_of = [&](int64_t i) { return static_cast<int>(i % NS); };
       auto scores = [&](int g, int slot) {
@@ -198,12 +240,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       };
       while (ok && walk.next(p.seqs, p.shape, item)) {
         const int tiles = rows_of(item) > 128 ? 2 : 1;
-        ok = wait(&q_full, items & 1, kStatusAttnMmaWait) && wait(&ready[slot_of(n)], (n / NS) & 1, kStatusAttnMmaWait);
+        ok = wait(&ready[slot_of(n)], (n / NS) & 1, kStatusAttnMmaWait);
+        for (int g = 0; ok && g < tiles; ++g) {
+          ok = wait(&q_full[g], q_phase[g], kStatusAttnMmaWait);
+          if (!ok) break;
+          q_phase[g] ^= 1;
+          tc_fence_after();
+          scores(g, slot_of(n));
+          if (item.blocks == 1) umma_commit(&q_empty[g]);
+        }
         if (!ok) break;
-        tc_fence_after();
-        for (int g = 0; g < tiles; ++g) scores(g, slot_of(n));
         umma_commit(&empty[slot_of(n)]);
-        if (item.blocks == 1) umma_commit(&q_empty);
         for (int j = 0; ok && j < item.blocks; ++j, n += 2) {
           const bool more = j + 1 < item.blocks;
           const int64_t v = n + 1, k = n + 2;
@@ -219,16 +266,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               if (g == 0 && !(ok = wait(&ready[slot_of(k)], (k / NS) & 1, kStatusAttnMmaWait))) break;
               tc_fence_after();
               scores(g, slot_of(k));
+              if (j + 2 == item.blocks) umma_commit(&q_empty[g]);
             } else {
               umma_commit(&o_full[g]);
             }
           }
-          if (ok && more) {
-            umma_commit(&empty[slot_of(k)]);
-            if (j + 2 == item.blocks) umma_commit(&q_empty);
-          }
+          if (ok && more) umma_commit(&empty[slot_of(k)]);
         }
-        ++items;
       }
       if (!ok) {  // what was issued ends before TMEM goes
         umma_commit(&drained);
@@ -236,65 +280,79 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp >= 10) {
+  } else {
     const int at = tid - 320;  // 0 .. 63
     int64_t n = 0;
-    int items = 0;
+    int items = 0, q_uses[2] = {0, 0};
     bool ok = true;
     while (ok && walk.next(p.seqs, p.shape, item)) {
       const int rows = rows_of(item), row0 = item.tile * kTileRows;
-      if (items > 0 && !warp_wait(&q_empty, (items - 1) & 1, kStatusAttnLoadWait)) break;
       auto q_row = [&](int row) {
-        const int r = row0 + row, i = r / group;
+        const int r = row0 + row, i = over_group(p.shape, r);
         return static_cast<const uint16_t *>(p.q) + static_cast<int64_t>(item.s.first + i) * p.q_token +
                static_cast<int64_t>(item.head * group + (r - i * group)) * p.q_head;
       };
-      if constexpr (S8) {
-        for (int row = at; row < kTileRows; row += 64) {
-          uint4 w[D / 8];
-          const uint16_t *src = q_row(min(row, rows - 1));
+      const int tiles = rows > 128 ? 2 : 1;
+      for (int g = 0; g < tiles; ++g) {
+        uint8_t *dst = q_tile + g * (T::kQ / 2);
+        if (q_uses[g] > 0) ok = warp_wait(&q_empty[g], (q_uses[g] - 1) & 1, kStatusAttnLoadWait);
+        if (!ok) break;
+        ++q_uses[g];
+        if constexpr (S8) {
+          for (int r = at; r < 128; r += 64) {
+            const int row = g * 128 + r;
+            uint4 w[D / 8];
+            const uint16_t *src = q_row(min(row, rows - 1));
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            w[c] = row < rows && 8 * c < p.o.dim ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-          uint32_t big = 0;  // the largest |q|'s bits, of either half
-          const uint32_t *x = reinterpret_cast<const uint32_t *>(w);
+            for (int c = 0; c < D / 8; ++c)
+              w[c] = row < rows && 8 * c < p.o.dim ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+            uint32_t big = 0;  // the largest |q|'s bits, of either half
+            const uint32_t *x = reinterpret_cast<const uint32_t *>(w);
 #pragma unroll
-          for (int e = 0; e < D / 2; ++e) big = __vmaxu2(big, x[e] & 0x7fff7fffu);
-          const uint16_t top = static_cast<uint16_t>(max(big & 0xffff, big >> 16));
-          const bool f16 = p.q_dtype == MQ_F16;
-          const float most = f16 ? __half2float(__ushort_as_half(top)) : __uint_as_float(static_cast<uint32_t>(top) << 16);
-          const uint32_t e2 = min(max(__float_as_uint(most) >> 23, 27u), 227u);
-          const float down = __uint_as_float((254 - e2) << 23);
-          row_factor[items & 1][row] = __uint_as_float(e2 << 23) * p.scale;
-          uint8_t *dst = q_tile + (row / 128) * (T::kQ / 2);
+            for (int e = 0; e < D / 2; ++e) big = __vmaxu2(big, x[e] & 0x7fff7fffu);
+            const uint16_t top = static_cast<uint16_t>(max(big & 0xffff, big >> 16));
+            const bool f16 = p.q_dtype == MQ_F16;
+            const float most = f16 ? __half2float(__ushort_as_half(top)) : __uint_as_float(static_cast<uint32_t>(top) << 16);
+            const uint32_t e2 = min(max(__float_as_uint(most) >> 23, 27u), 227u);
+            const float down = __uint_as_float((254 - e2) << 23);
+            row_factor[items & 1][row] = __uint_as_float(e2 << 23) * p.scale;
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            uint32_t o[4];
+            for (int c = 0; c < D / 8; ++c) {
+              uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t y = x[4 * c + e];
-              const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2 *>(&y))
-                                   : make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u));
-              o[e] = pack_half2(f.x * down, f.y * down);
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t y = x[4 * c + e];
+                const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2 *>(&y))
+                                     : make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u));
+                o[e] = pack_half2(f.x * down, f.y * down);
+              }
+              *reinterpret_cast<uint4 *>(dst + swizzled(r, c)) = make_uint4(o[0], o[1], o[2], o[3]);
             }
-            *reinterpret_cast<uint4 *>(dst + swizzled(row % 128, c)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
+        } else {
+          constexpr int kLanes = D / 8;  // of a row
+          const int c = at % kLanes;
+#pragma unroll 4
+          for (int r = at / kLanes; r < 128; r += 64 / kLanes) {
+            const int row = g * 128 + r;
+            const bool real = row < rows && 8 * c < p.o.dim;
+            const uint16_t *src = q_row(min(row, rows - 1)) + (real ? 8 * c : 0);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + swizzled(r, c))), "l"(src), "r"(real ? 16 : 0)
+                         : "memory");
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
         }
-      } else {
-        for (int e = at; e < kTileRows * (D / 8); e += 64) {
-          const int row = e / (D / 8), c = e % (D / 8);
-          const bool real = row < rows && 8 * c < p.o.dim;
-          const uint16_t *src = q_row(min(row, rows - 1)) + (real ? 8 * c : 0);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                           smem_u32(q_tile + (row / 128) * (T::kQ / 2) + swizzled(row % 128, c))),
-                       "l"(src), "r"(real ? 16 : 0)
-                       : "memory");
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
+      if (!ok) break;
+      for (int g = 0; g < tiles; ++g) {
+        if (g + 1 < tiles)
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[g]);
+      }
       ++items;
 
       const int part_hi = least_hi(item), part_lo = most_lo(item);
@@ -374,10 +432,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int g = warp / 4, r = tid % 128;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + g * 128, o_at = tmem + lanes + 256 + g * D;
+    uint8_t *const stage = stages + warp * kStageBytes;
     int64_t n = 0;
     int items = -1;
     uint32_t s_phase = 0, o_phase = 0;
@@ -385,14 +446,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     while (ok && walk.next(p.seqs, p.shape, item)) {
       ++items;
       const int rows = rows_of(item), row = g * 128 + r;
-      const bool goes_on = item.before > 0, whole = !goes_on && item.blocks == item.whole;
-      if (items == 0 && tid == 0)
-        p.parts.cuts[blockIdx.x] = Cut{item.b, item.head, item.tile, goes_on, share.begin - item.before, share.begin - item.before + item.whole};
       if (rows <= g * 128) {  // the item has no second tile
         n += 2 * item.blocks;
         continue;
       }
-      const int index = item.tile * kTileRows + min(row, rows - 1), i = index / group;
+      const int index = item.tile * kTileRows + min(row, rows - 1), i = over_group(p.shape, index);
       const int hi = row < rows ? max(item.s.pos0 + i + 1, 0) : 0;
       const int lo = p.shape.window ? max(0, item.s.pos0 + i + 1 - p.shape.window) : 0;
       const int part_hi = least_hi(item), part_lo = most_lo(item);
@@ -409,6 +467,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_loaded(v[c]);
+        const bool edge = key0 + kTileKeys > part_hi || key0 < part_lo;
         float scale = p.scale;
         if constexpr (S8) {
           scale = 1.f;
@@ -418,12 +477,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][32 * c + e]), l4 = *reinterpret_cast<const float4 *>(&sc[1][32 * c + e]);
-              v[c][e] = fmaf(v[c][e] * factor, k4.x, l4.x), v[c][e + 1] = fmaf(v[c][e + 1] * factor, k4.y, l4.y);
-              v[c][e + 2] = fmaf(v[c][e + 2] * factor, k4.z, l4.z), v[c][e + 3] = fmaf(v[c][e + 3] * factor, k4.w, l4.w);
+              float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][32 * c + e]);
+              const float4 l4 = *reinterpret_cast<const float4 *>(&sc[1][32 * c + e]);
+              mul2(k4.x, k4.y, factor, factor);
+              mul2(k4.z, k4.w, factor, factor);
+              fma2(v[c][e], v[c][e + 1], k4.x, k4.y, l4.x, l4.y);
+              fma2(v[c][e + 2], v[c][e + 3], k4.z, k4.w, l4.z, l4.w);
             }
         }
-        if (key0 + kTileKeys > part_hi || key0 < part_lo) {
+        if (edge) {
           if constexpr (!S8) {
             const int slot = static_cast<int>((n + 1) % NS);
             ok = warp_wait(&ready[slot], ((n + 1) / NS) & 1, kStatusAttnSoftmaxWait);
@@ -446,9 +508,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         float top[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          top[c] = v[c][0];
+          top[c] = fmaxf(v[c][0], v[c][1]);
 #pragma unroll
-          for (int e = 1; e < 32; ++e) top[c] = fmaxf(top[c], v[c][e]);
+          for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], v[c][e], v[c][e + 1]);
         }
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
         const bool grows = most > m + 8.f;
@@ -458,36 +520,45 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           l *= a;
           m = next;
           if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tmem_ld16(o_at + c, o);
+              uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              float o[32];
-              tmem_ld32(o_at + c, o);
-              uint32_t w[32];
-#pragma unroll
-              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * a);
-              tmem_st32(o_at + c, w);
+              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * a);
+              tmem_st16(o_at + c, w);
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float ref = m == -INFINITY ? 0.f : -m;
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float a = ex2(fmaf(v[c][e], scale, -ref)), b = ex2(fmaf(v[c][e + 1], scale, -ref));
+            if (S8)
+              add2(v[c][e], v[c][e + 1], ref, ref);
+            else
+              fma2(v[c][e], v[c][e + 1], scale, scale, ref, ref);
+            const float a = ex2(v[c][e]), b = ex2(v[c][e + 1]);
             w[e / 2] = pack16<BF>(a, b);
             if constexpr (S8) {
               const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][32 * c + e]);
-              l += (a == 0.f ? 0.f : a * iv.x) + (b == 0.f ? 0.f : b * iv.y);
+              if (edge)  // (a key that the row does not see may have any scale)
+                add2(sum[0], sum[1], a == 0.f ? 0.f : a * iv.x, b == 0.f ? 0.f : b * iv.y);
+              else
+                sum[0] = fmaf(a, iv.x, sum[0]), sum[1] = fmaf(b, iv.y, sum[1]);
             } else if (BF) {  // as they were rounded: the roundings cancel where one key has most of the weight
-              l += __uint_as_float(w[e / 2] << 16) + __uint_as_float(w[e / 2] & 0xffff0000u);
+              add2(sum[0], sum[1], __uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xffff0000u));
             } else {
-              l += a + b;
+              add2(sum[0], sum[1], a, b);
             }
           }
           tmem_st16(s_at + 16 * c, w);
         }
+        l += sum[0] + sum[1];
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -498,31 +569,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!ok) break;
       o_phase ^= 1;
       tc_fence_after();
+      const bool goes_on = item.before > 0, whole = !goes_on && item.blocks == item.whole;
       const float inv = whole ? inverse_sum(l) : 1.f;
       const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (goes_on ? 0 : 1)) * kTileRows + row;
       if (!whole && row < rows) p.parts.stats[part] = make_float2(m, l);
-#pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      // 64 bytes of each of the warp's rows at a time: through shared memory, so that eight rows leave with one store
+      // instead of each lane's own (six times the cycles).
+      const int64_t out_at = static_cast<int64_t>(item.s.first + i) * p.o.token_stride +
+                             static_cast<int64_t>(item.head * group + (index - i * group)) * p.o.head_stride;
+      char *const base = whole ? static_cast<char *>(p.o.out) : reinterpret_cast<char *>(p.parts.sums);
+      const int64_t mine = whole ? 2 * out_at : 4 * part * D;
+      const int pieces = whole ? (p.o.dim + 31) / 32 : D / 16, width = whole ? 2 * p.o.dim : 4 * D;
+#pragma unroll 1
+      for (int c = 0; c < pieces; ++c) {
         float o[32];
-        tmem_ld32(o_at + c, o);
-        if (row < rows) {
-          if (whole) {
-            const int64_t at = static_cast<int64_t>(item.s.first + i) * p.o.token_stride +
-                               static_cast<int64_t>(item.head * group + (index - i * group)) * p.o.head_stride + c;
+        if (whole)
+          tmem_ld32(o_at + 32 * c, o);
+        else
+          tmem_ld16(o_at + 16 * c, reinterpret_cast<float(&)[16]>(o));
+        uint4 w[4];
+        uint32_t *words = reinterpret_cast<uint32_t *>(w);
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t w[4];
+        for (int e = 0; e < 16; ++e)
+          words[e] = !whole                  ? __float_as_uint(o[e])
+                     : p.o.dtype == MQ_F16 ? pack16<false>(o[2 * e] * inv, o[2 * e + 1] * inv)
+                                            : pack16<true>(o[2 * e] * inv, o[2 * e + 1] * inv);
+        __syncwarp();
 #pragma unroll
-              for (int u = 0; u < 4; ++u)
-                w[u] = p.o.dtype == MQ_F16 ? pack16<false>(o[e + 2 * u] * inv, o[e + 2 * u + 1] * inv)
-                                           : pack16<true>(o[e + 2 * u] * inv, o[e + 2 * u + 1] * inv);
-              if (c + e < p.o.dim) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.o.out) + at + e) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
+        for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4 *>(stage + lane * 64 + ((u ^ (lane >> 1)) & 3) * 16) = w[u];
+        __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4 *>(p.parts.sums + part * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
+        for (int it = 0; it < 4; ++it) {
+          const int from = it * 8 + lane / 4, u = lane % 4;
+          const int64_t to = __shfl_sync(0xffffffffu, mine, from) + 64 * c + 16 * u;
+          if (g * 128 + (warp & 3) * 32 + from < rows && 64 * c + 16 * u < width)
+            *reinterpret_cast<uint4 *>(base + to) = *reinterpret_cast<const uint4 *>(stage + from * 64 + ((u ^ (from >> 1)) & 3) * 16);
         }
       }
       tc_fence_before();
@@ -548,6 +629,12 @@ int launch_tile(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, c
   static size_t configured[64] = {};
   auto kern = attn_tile_kernel<D, KIND>;
   if (int rc = ensure_smem(kern, T::kSmem, configured, what)) return rc;
+  // The kernel deals its registers out anew, which waits for good where a block has fewer of them.
+  static const int regs = [&] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
+  }();
+  MQ_REQUIRE(regs == kTileRegs, MQ_ECUDA, "%s: the kernel was built with %d registers, not %d", what, regs, kTileRegs);
   if (int rc = launch_overlapped(kern, dim3(ctas), dim3(kTileThreads), T::kSmem, stream, what, kmap, vmap, p)) return rc;
   JoinParams j{p.seqs, p.shape, p.o, p.parts, kTileRows};
   return launch_overlapped(attn_join_kernel<D, kTileRows>, dim3(ctas, kTileRows / 16), dim3(128), 0, stream, what, j);
@@ -644,7 +731,8 @@ extern "C" int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, i
   if (int rc = plan_for(&plan, cache, heads, batch, tokens, max_new, starts != nullptr, dev.sms, what)) return rc;
   MQ_REQUIRE(workspace && mq::aligned(workspace, 16), MQ_EALIGN, "%s: the workspace must be 16-byte aligned", what);
   MQ_REQUIRE(workspace_bytes >= plan.bytes, MQ_EINVAL, "%s: the workspace is too small", what);
-  p.shape.group = static_cast<int>(heads / cache->heads), p.shape.kv_heads = cache->heads, p.shape.window = static_cast<int>(window);
+  set_group(&p.shape, static_cast<int>(heads / cache->heads));
+  p.shape.kv_heads = cache->heads, p.shape.window = static_cast<int>(window);
   p.q = q, p.q_token = q_token, p.q_head = q_head, p.q_dtype = q_dtype;
   p.k_scale = cache->k_scale, p.v_scale = cache->v_scale;
   for (int i = 0; i < 3; ++i) p.ks_stride[i] = cache->ks_stride[i], p.vs_stride[i] = cache->vs_stride[i];

@@ -135,97 +135,172 @@ inline int check_rows_out(const void *p, int dtype, int64_t tokens, int64_t head
 // ---- attention: items, units and shares --------------------------------------------------------------
 
 // The rows of one kv head of a sequence are its tokens' `group` query heads, token by token: row r is head r % group of
-// token r / group. An item is ROWS of them and the blocks of KEYS positions that any of them sees; a unit is one block
-// of one item. Units are numbered by sequence, kv head, row tile and block, and the launch's CTAs take equal shares of
-// them, whatever the sequences' lengths: an item may be cut between CTAs, which then leave its parts to be joined.
+// token r / group. An item is ROWS of them and the blocks of KEYS positions that any of them sees. Its units are its blocks
+// and EXTRA more before them, for what an item costs beside its blocks. Units are numbered by sequence, kv head, row tile and
+// block, and the launch's CTAs take equal shares of them, whatever the sequences' lengths: an item may be cut between CTAs, which
+// then leave its parts to be joined.
 struct Shape {
   int group, kv_heads, window;
   int rows_from, rows_to;  // the sequences of this launch: those with rows_from < rows <= rows_to
   int rows_most;           // a sequence with more was not announced: reported, and left out by every launch
+  uint32_t by_group, by_group_shift;
 };
+// x / group for 0 <= x < 2^31: with k = 31 + ceil(log2(group)), ceil(2^k / group) x >> k is exact.
+inline void set_group(Shape *a, int group) {
+  int log = 0;
+  while ((1 << log) < group) ++log;
+  a->group = group, a->by_group_shift = 31 + log;
+  a->by_group = static_cast<uint32_t>(((1ull << a->by_group_shift) + group - 1) / group);
+}
+__device__ __forceinline__ int over_group(const Shape &a, int x) {
+  return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * a.by_group >> a.by_group_shift);
+}
 
-template <int ROWS, int KEYS>
+template <int R, int K, int E>
+struct Grain {
+  static constexpr int ROWS = R, KEYS = K, EXTRA = E;
+};
 struct Range {
   int lo, blocks;  // the first block, how many (one, with nothing in it, where no row sees a key)
 };
-template <int ROWS, int KEYS>
-__device__ __forceinline__ Range<ROWS, KEYS> tile_range(const Seq &s, const Shape &a, int t) {
+template <typename G>
+__device__ __forceinline__ Range tile_range(const Seq &s, const Shape &a, int t) {
   const int rows = s.n * a.group;
-  const int i0 = t * ROWS / a.group, i1 = (min(rows, (t + 1) * ROWS) - 1) / a.group;
+  const int i0 = over_group(a, t * G::ROWS), i1 = over_group(a, min(rows, (t + 1) * G::ROWS) - 1);
   const int hi = min(max(s.pos0 + i1 + 1, 0), s.length), lo = a.window ? max(0, s.pos0 + i0 + 1 - a.window) : 0;
-  const int b0 = min(lo, max(hi - 1, 0)) / KEYS;
-  return {b0, max(1, (hi + KEYS - 1) / KEYS - b0)};
+  const int b0 = min(lo, max(hi - 1, 0)) / G::KEYS;
+  return {b0, max(1, (hi + G::KEYS - 1) / G::KEYS - b0)};
 }
 __device__ __forceinline__ bool takes_part(const Seq &s, const Shape &a) {
   const int64_t rows = static_cast<int64_t>(s.n) * a.group;
   return rows > a.rows_from && rows <= a.rows_to;
 }
-template <int ROWS, int KEYS>
-__device__ __forceinline__ int64_t units_per_head(const Seq &s, const Shape &a) {
-  const int tiles = (s.n * a.group + ROWS - 1) / ROWS;
-  int64_t units = 0;
-  for (int t = 0; t < tiles; ++t) units += tile_range<ROWS, KEYS>(s, a, t).blocks;
-  return units;
+template <typename G>
+__device__ __forceinline__ int tiles_of(const Seq &s, const Shape &a) {
+  return (s.n * a.group + G::ROWS - 1) / G::ROWS;
 }
 
 struct Share {
   int64_t total, begin, end;  // units of the launch, and of this CTA
-  int64_t offset;             // of `begin` within sequence b's
-  int b, parts;               // parts: CTAs with a share
+  int parts;                  // CTAs with a share
+  int b, head, tile, rest;    // where it begins: `rest` units into that item
 };
 template <int THREADS>
 struct ShareScratch {
+  int64_t costs[THREADS];  // units of THREADS sequences
   int64_t sums[THREADS / 32];
-  int64_t offset;
-  int b;
+  Share found;
 };
 
 // This CTA's share; called by all THREADS threads. parts <= blockIdx.x: none.
-template <int THREADS, int ROWS, int KEYS>
+template <int THREADS, typename G>
 __device__ __forceinline__ Share find_share(const Seqs &s, const Shape &a, ShareScratch<THREADS> &sm) {
+  constexpr int kWarps = THREADS / 32;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  auto cost_of = [&](int b) -> int64_t {
-    if (b >= s.batch) return 0;
-    const Seq q = sequence(s, b);
-    if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
-    return takes_part(q, a) ? units_per_head<ROWS, KEYS>(q, a) * a.kv_heads : 0;
+  // Units of sequences base + 0 .. THREADS - 1 into sm.costs: a thread each where a sequence has one tile at most, else a
+  // warp each, its lanes on the tiles.
+  auto fill_costs = [&](int base) {
+    if (G::ROWS <= 64) {
+      int64_t cost = 0;
+      if (base + tid < s.batch) {
+        const Seq q = sequence(s, base + tid);
+        if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
+        if (takes_part(q, a)) cost = static_cast<int64_t>(G::EXTRA + tile_range<G>(q, a, 0).blocks) * a.kv_heads;
+      }
+      sm.costs[tid] = cost;
+    } else {
+      for (int b = warp; b < THREADS; b += kWarps) {
+        if (base + b >= s.batch) {
+          if (lane == 0) sm.costs[b] = 0;
+          continue;
+        }
+        const Seq q = sequence(s, base + b);
+        int64_t cost = 0;
+        if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
+        if (takes_part(q, a))
+          for (int t = lane, tiles = tiles_of<G>(q, a); t < tiles; t += 32) cost += G::EXTRA + tile_range<G>(q, a, t).blocks;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+        if (lane == 0) sm.costs[b] = cost * a.kv_heads;
+      }
+    }
+    __syncthreads();
   };
-  const int64_t first = cost_of(tid);
-  int64_t mine = first;
-  for (int b = tid + THREADS; b < s.batch; b += THREADS) mine += cost_of(b);
+  int64_t mine = 0;
+  for (int base = 0; base < s.batch; base += THREADS) {
+    fill_costs(base);
+    mine += sm.costs[tid];
+    if (base + THREADS < s.batch) __syncthreads();
+  }
+  const bool many = s.batch > THREADS;  // (else sm.costs holds all)
 #pragma unroll
   for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) sm.sums[warp] = mine;
   __syncthreads();
   Share share{};
-  for (int w = 0; w < THREADS / 32; ++w) share.total += sm.sums[w];
+  for (int w = 0; w < kWarps; ++w) share.total += sm.sums[w];
   share.parts = static_cast<int>(share.total < gridDim.x ? share.total : gridDim.x);
-  __syncthreads();
   if (static_cast<int>(blockIdx.x) >= share.parts) return share;
   share.begin = share.total * blockIdx.x / share.parts;
   share.end = share.total * (blockIdx.x + 1) / share.parts;
   int64_t before = 0;
   for (int base = 0; base < s.batch; base += THREADS) {
-    const int64_t cost = base == 0 ? first : cost_of(base + tid);
+    if (many) {
+      __syncthreads();
+      fill_costs(base);
+    }
+    const int64_t cost = sm.costs[tid];
     int64_t incl = cost;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
+    __syncthreads();
     if (lane == 31) sm.sums[warp] = incl;
     __syncthreads();
     int64_t ahead = before;
-    for (int w = 0; w < THREADS / 32; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) ahead += sm.sums[w];
       before += sm.sums[w];
     }
+    // The warp with the sequence in which the share begins finds the tile.
     const int64_t start = ahead + incl - cost;
-    if (start <= share.begin && share.begin < start + cost) sm.b = base + tid, sm.offset = share.begin - start;
-    __syncthreads();
+    const unsigned here = __ballot_sync(0xffffffffu, start <= share.begin && share.begin < start + cost);
+    if (here) {
+      const int from = __ffs(here) - 1, b = base + warp * 32 + from;
+      const int64_t offset = share.begin - __shfl_sync(0xffffffffu, start, from);
+      const int64_t per_head = __shfl_sync(0xffffffffu, cost, from) / a.kv_heads;
+      const int head = static_cast<int>(offset / per_head);
+      int64_t rest = offset - head * per_head;
+      int tile = 0;
+      if (G::ROWS > 64) {
+        const Seq q = sequence(s, b);
+        for (const int tiles = tiles_of<G>(q, a);; tile += 32) {
+          const int t = tile + lane;
+          const int64_t units = t < tiles ? G::EXTRA + tile_range<G>(q, a, t).blocks : 0;
+          int64_t sum = units;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+          }
+          const unsigned in = __ballot_sync(0xffffffffu, rest < sum);
+          if (in) {  // (the units of all tiles are more than `rest`, so some lane's is)
+            const int l = __ffs(in) - 1;
+            rest -= __shfl_sync(0xffffffffu, sum - units, l);
+            tile += l;
+            break;
+          }
+          rest -= __shfl_sync(0xffffffffu, sum, 31);
+        }
+      }
+      if (lane == 0) sm.found.b = b, sm.found.head = head, sm.found.tile = tile, sm.found.rest = static_cast<int>(rest);
+    }
     if (before > share.begin) break;
   }
-  share.b = sm.b, share.offset = sm.offset;
+  __syncthreads();
+  share.b = sm.found.b, share.head = sm.found.head, share.tile = sm.found.tile, share.rest = sm.found.rest;
   return share;
 }
 
@@ -237,24 +312,15 @@ struct Item {
 };
 
 // Walks through a share's items. Every role of a CTA walks by itself.
-template <int ROWS, int KEYS>
+template <typename G>
 struct Walk {
   Seq s;
-  int b, head, tile, tiles, skip;
+  int b, head, tile, tiles, rest;
   int64_t left;
   __device__ __forceinline__ void start(const Seqs &q, const Shape &a, const Share &share) {
-    b = share.b, left = share.end - share.begin;
+    b = share.b, head = share.head, tile = share.tile, rest = share.rest, left = share.end - share.begin;
     s = sequence(q, b);
-    tiles = (s.n * a.group + ROWS - 1) / ROWS;
-    const int64_t per_head = units_per_head<ROWS, KEYS>(s, a);
-    head = static_cast<int>(share.offset / per_head);
-    int64_t rest = share.offset - head * per_head;
-    for (tile = 0;; ++tile) {
-      const int blocks = tile_range<ROWS, KEYS>(s, a, tile).blocks;
-      if (rest < blocks) break;
-      rest -= blocks;
-    }
-    skip = static_cast<int>(rest);
+    tiles = tiles_of<G>(s, a);
   }
   __device__ __forceinline__ bool next(const Seqs &q, const Shape &a, Item &item) {
     if (left <= 0) return false;
@@ -264,17 +330,18 @@ struct Walk {
         head = 0;
         do s = sequence(q, ++b);
         while (!takes_part(s, a));  // (units are left, so such a sequence follows)
-        tiles = (s.n * a.group + ROWS - 1) / ROWS;
+        tiles = tiles_of<G>(s, a);
       }
     }
-    const auto r = tile_range<ROWS, KEYS>(s, a, tile);
+    const Range r = tile_range<G>(s, a, tile);
+    const int take = static_cast<int>(left < G::EXTRA + r.blocks - rest ? left : G::EXTRA + r.blocks - rest);
     item.s = s, item.b = b, item.head = head, item.tile = tile;
-    item.before = skip, item.whole = r.blocks, item.block = r.lo + skip;
-    item.blocks = static_cast<int>(left < r.blocks - skip ? left : r.blocks - skip);
-    left -= item.blocks;
-    skip = 0;
+    item.before = max(rest - G::EXTRA, 0), item.whole = r.blocks, item.block = r.lo + item.before;
+    item.blocks = rest + take - G::EXTRA - item.before;
+    left -= take;
+    rest = 0;
     ++tile;
-    return true;
+    return item.blocks > 0;  // (a share may end before the first block of its last item)
   }
 };
 
@@ -282,8 +349,14 @@ struct Walk {
 // begins and does not end (slot 1). `cut` says which item the CTA goes on with.
 struct Cut {
   int32_t b, head, tile, goes_on;
-  int64_t first, end;  // the item's units
+  int64_t first, end;  // the units of the item's blocks
 };
+// Of a walk that has just started.
+template <typename G>
+__device__ __forceinline__ Cut cut_at(const Walk<G> &w, const Shape &a, const Share &share) {
+  const int64_t first = share.begin - share.rest + G::EXTRA;
+  return {w.b, w.head, w.tile, share.rest > G::EXTRA, first, first + tile_range<G>(w.s, a, w.tile).blocks};
+}
 struct Parts {
   int64_t *counts;  // units, CTAs with a share
   Cut *cuts;        // [ctas]
