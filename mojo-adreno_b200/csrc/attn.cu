@@ -147,8 +147,9 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   float *join = reinterpret_cast<float *>(ring + S * F::kStageBytes);  // [WK][16 MT][kPadCols]
-  __shared__ uint64_t full[S], empty[S];
+  __shared__ uint64_t full[S], empty[S], meeting;
   __shared__ ShareScratch<kFewThreads> scratch;
+  __shared__ ItemRing items;
   __shared__ float2 row_stats[WK][16 * MT];
   __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -158,17 +159,16 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
       mbar_init(&full[i], S8 ? 33 : 1);  // the copies' bytes; the lanes whose scales have come
       mbar_init(&empty[i], kFewWarps);
     }
+    items.init(kFewWarps);
+    mbar_init(&meeting, kFewWarps);
     abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
   griddep_wait();
-  const Share share = find_share<kFewThreads, FewGrain>(p.seqs, p.shape, scratch);
-  if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = share.total, p.parts.counts[1] = share.parts;
-  if (static_cast<int>(blockIdx.x) >= share.parts) return;
-  Walk<FewGrain> walk;
-  walk.start(p.seqs, p.shape, share);
-  if (tid == 0) p.parts.cuts[blockIdx.x] = cut_at(walk, p.shape, share);
+  find_share<kFewThreads, FewGrain>(p.seqs, p.shape, scratch);
+  if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = scratch.found.total, p.parts.counts[1] = scratch.found.parts;
+  if (static_cast<int>(blockIdx.x) >= scratch.found.parts) return;
   Item item;
 
   if (warp == kFewWarps) {
@@ -178,10 +178,19 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
     }
     const int box_rows = min(kFewKeys, 1 << p.seqs.page_log2), per_block = kFewKeys / box_rows;
     const int boxes = per_block * F::kBoxes;  // of keys, and as many of values
-    int s = 0, round = 0;
-    int64_t issued = 0;
+    Walk<FewGrain> walk;
+    walk.start(p.seqs, p.shape, scratch.found);
+    if (lane == 0) p.parts.cuts[blockIdx.x] = cut_at(walk, p.shape, scratch.found);
+    int s = 0, round = 0, k = 0;
+    uint32_t issued = 0;
     bool ok = true;
-    while (ok && walk.next(p.seqs, p.shape, item)) {
+    while (ok) {
+      if (!walk.next(p.seqs, p.shape, item)) item.blocks = 0;
+      if (!items.put(k++, item)) {
+        if (lane == 0) raise_status(kStatusAttnLoadWait), abort_flag = 1;
+        break;
+      }
+      if (item.blocks == 0) break;
       for (int i = 0; i < item.blocks; ++i) {
         const int key0 = (item.block + i) * kFewKeys;
         // Boxes behind the sequence's end are not fetched: their table entries may be anything.
@@ -235,15 +244,33 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
     }
     // Leave no copy in flight.
     if (lane == 0)
-      for (int64_t i = issued > S ? issued - S : 0; i < issued; ++i) mbar_wait(&full[i % S], (i / S) & 1);
+      for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i) mbar_wait(&full[i % S], (i / S) & 1);
     return;
   }
 
   const int mt = warp % MT, wk = warp / MT, g = lane / 4, t = lane % 4;
   const int heads = p.shape.group;
   int s = 0;
-  uint32_t phase = 0;
-  while (walk.next(p.seqs, p.shape, item)) {
+  uint32_t phase = 0, meetings = 0;
+  // All four warps, or false for those that waited in vain.
+  auto meet = [&]() -> bool {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&meeting);
+    const bool met = !abort_flag && mbar_wait(&meeting, meetings++ & 1);
+    if (__all_sync(0xffffffffu, met)) return true;
+    if (lane == 0 && !abort_flag) raise_status(kStatusAttnSoftmaxWait), abort_flag = 1;
+    return false;
+  };
+  for (int k = 0;; ++k) {
+    const bool told = mbar_wait(&items.full[k % kItems], (k / kItems) & 1);
+    if (!__all_sync(0xffffffffu, told)) {
+      if (lane == 0 && !abort_flag) raise_status(kStatusAttnSoftmaxWait), abort_flag = 1;
+      break;  // (what the others wait for next does not come either)
+    }
+    item = items.item[k % kItems];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&items.empty[k % kItems]);
+    if (item.blocks == 0) break;
     const int rows = item.s.n * heads;
     // A thread's rows are g and g + 8 of its warp's 16; q as the MMA's A, in registers.
     uint32_t qa[D / 16][4];
@@ -402,11 +429,14 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
               bad[0] |= __shfl_xor_sync(0xffffffffu, bad[0], x);
               bad[1] |= __shfl_xor_sync(0xffffffffu, bad[1], x);
             }
+            if (bad[0] | bad[1])  // (rare: a row that sees one of them ends as NaN)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+              for (int u = 0; u < 2; ++u)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (bad[u] >> (e & 1 ? 16 : 0) & 1) c[2 * kk + u][e] = NAN;
+                for (int e = 0; e < 4; ++e) {
+                  const int key = key0 + 16 * kk + 8 * u + 2 * t + (e & 1);
+                  if ((bad[u] >> (e & 1 ? 16 : 0) & 1) && key < hi[e >> 1] && key >= lo[e >> 1]) l[e >> 1] = NAN;
+                }
           }
         }
 #pragma unroll
@@ -504,8 +534,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       if (t == 0) row_stats[wk][mt * 16 + g + 8 * r] = make_float2(m[r], l[r]);
     }
-    named_bar_sync(1, 32 * kFewWarps);
-    if (abort_flag) break;
+    if (!meet()) break;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       float top = -INFINITY;
@@ -535,7 +564,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
             *reinterpret_cast<float2 *>(at + 8 * c + 2 * t) = make_float2(o[8 * h + c][2 * r], o[8 * h + c][2 * r + 1]);
         }
       }
-      named_bar_sync(1, 32 * kFewWarps);
+      if (!meet()) return;
       for (int e = tid; e < 16 * MT * 16; e += 32 * kFewWarps) {
         const int row = e / 16, col = e % 16 * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -563,7 +592,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
           }
         }
       }
-      named_bar_sync(1, 32 * kFewWarps);
+      if (!meet()) return;
     }
   }
 }

@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained, s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t bad_keys[NS][4];
   __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
+  __shared__ ItemRing items;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -132,6 +133,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&empty[i], 1);
     }
     mbar_init(&drained, 1);
+    items.init(1 + kAuxWarps + 8);
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -143,17 +145,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   griddep_launch_dependents();
   const uint32_t tmem = tmem_slot;
   ShareScratch<kTileThreads> &scratch = *reinterpret_cast<ShareScratch<kTileThreads> *>(ring);  // (nothing has been copied yet)
-  const Share share = find_share<kTileThreads, TileGrain>(p.seqs, p.shape, scratch);
-  __syncthreads();
+  find_share<kTileThreads, TileGrain>(p.seqs, p.shape, scratch);
+  const Share share = scratch.found;
+  __syncthreads();  // (the ring is free again)
   if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = share.total, p.parts.counts[1] = share.parts;
   const bool works = static_cast<int>(blockIdx.x) < share.parts;
   const int group = p.shape.group;
-  Walk<TileGrain> walk;
   Item item;
-  if (works) {
-    walk.start(p.seqs, p.shape, share);
-    if (tid == 0) p.parts.cuts[blockIdx.x] = cut_at(walk, p.shape, share);
-  }
   // Waits that give up set the flag, and everybody leaves at the next wait.
   auto wait = [&](uint64_t *bar, uint32_t parity, int code) -> bool {
     if (!abort_flag && mbar_wait(bar, parity)) return true;
@@ -162,6 +160,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   };
   auto warp_wait = [&](uint64_t *bar, uint32_t parity, int code) -> bool {
     return __all_sync(0xffffffffu, wait(bar, parity, code));
+  };
+  // The next item, by a whole warp; false behind the last.
+  int k_item = 0;
+  auto next_item = [&](int code) -> bool {
+    if (!warp_wait(&items.full[k_item % kItems], (k_item / kItems) & 1, code)) return false;
+    item = items.item[k_item % kItems];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&items.empty[k_item % kItems]);
+    ++k_item;
+    return item.blocks > 0;
   };
   // Rows of an item's two tiles; whether some row of the item sees a block only in part.
   auto rows_of = [&](const Item &it) { return min(kTileRows, it.s.n * group - it.tile * kTileRows); };
@@ -180,9 +188,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     constexpr int kBox = S8 ? D : 128, kBoxes = S8 ? 1 : D / 64;  // bytes of a row in a box, boxes of a row
     const int page = 1 << p.seqs.page_log2, box_rows = min(kTileKeys, page), per_block = kTileKeys / box_rows;
-    int64_t issued = 0;
+    Walk<TileGrain> walk;
+    walk.start(p.seqs, p.shape, share);
+    if (lane == 0) p.parts.cuts[blockIdx.x] = cut_at(walk, p.shape, share);
+    uint32_t issued = 0;
     bool ok = true;
-    while (ok && walk.next(p.seqs, p.shape, item)) {
+    while (ok) {
+      if (!walk.next(p.seqs, p.shape, item)) item.blocks = 0;
+      if (!items.put(k_item++, item)) {
+        if (lane == 0) raise_status(kStatusAttnLoadWait), abort_flag = 1;
+        break;
+      }
+      if (item.blocks == 0) break;
       for (int i = 0; ok && i < item.blocks; ++i) {
         const int key0 = (item.block + i) * kTileKeys;
         // Boxes behind the sequence's end are not fetched: their table entries may be anything.
@@ -193,8 +210,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (of >= 0) id = of;
         }
         for (int which = 0; which < 2; ++which) {
-          const int slot = static_cast<int>(issued % NF);
-          const int64_t round = issued / NF;
+          const uint32_t slot = issued % NF, round = issued / NF;
           if (round > 0 && !warp_wait(S8 ? &raw_empty[slot] : &empty[slot], (round - 1) & 1, kStatusAttnLoadWait)) {
             ok = false;
             break;
@@ -216,14 +232,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     // Leave no copy in flight.
     if (lane == 0)
-      for (int64_t i = issued > NF ? issued - NF : 0; i < issued; ++i) mbar_wait(&full[i % NF], (i / NF) & 1);
+      for (uint32_t i = issued > NF ? issued - NF : 0; i < issued; ++i) mbar_wait(&full[i % NF], (i / NF) & 1);
   } else if (warp == 9) {
-    if (lane == 0) {
+    {
       constexpr uint32_t qk = idesc_16(128, kTileKeys, BF, false), pv = idesc_16(128, D, BF, true);
-      int64_t n = 0;  // slots used: keys and values in turn
+      uint32_t n = 0;  // slots used: keys and values in turn
       uint32_t p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
       bool ok = true;
-      auto slot_of = [&](int64_t i) { return static_cast<int>(i % NS); };
+      auto slot_of = [&](uint32_t i) { return static_cast<int>(i % NS); };
       auto scores = [&](int g, int slot) {
         const uint32_t a = smem_u32(q_tile) + g * (T::kQ / 2), b = smem_u32(ring + slot * T::kBlock);
 #pragma unroll
@@ -238,7 +254,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int k = 0; k < kTileKeys / 16; ++k)
           umma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, b + k * (2048 >> 4), pv, !first || k != 0);
       };
-      while (ok && walk.next(p.seqs, p.shape, item)) {
+      while (next_item(kStatusAttnMmaWait)) {
+        if (lane == 0) {
         const int tiles = rows_of(item) > 128 ? 2 : 1;
         ok = wait(&ready[slot_of(n)], (n / NS) & 1, kStatusAttnMmaWait);
         for (int g = 0; ok && g < tiles; ++g) {
@@ -249,11 +266,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           scores(g, slot_of(n));
           if (item.blocks == 1) umma_commit(&q_empty[g]);
         }
-        if (!ok) break;
-        umma_commit(&empty[slot_of(n)]);
+        if (ok) umma_commit(&empty[slot_of(n)]);
         for (int j = 0; ok && j < item.blocks; ++j, n += 2) {
           const bool more = j + 1 < item.blocks;
-          const int64_t v = n + 1, k = n + 2;
+          const uint32_t v = n + 1, k = n + 2;
           ok = wait(&ready[slot_of(v)], (v / NS) & 1, kStatusAttnMmaWait);
           for (int g = 0; ok && g < tiles; ++g) {
             ok = wait(&p_full[g], p_phase[g], kStatusAttnMmaWait);
@@ -273,8 +289,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           if (ok && more) umma_commit(&empty[slot_of(k)]);
         }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
       }
-      if (!ok) {  // what was issued ends before TMEM goes
+      if (!ok && lane == 0) {  // what was issued ends before TMEM goes
         umma_commit(&drained);
         mbar_wait(&drained, 0);
       }
@@ -282,10 +301,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncwarp();
   } else {
     const int at = tid - 320;  // 0 .. 63
-    int64_t n = 0;
-    int items = 0, q_uses[2] = {0, 0};
+    uint32_t n = 0;
+    int at_item = 0, q_uses[2] = {0, 0};
     bool ok = true;
-    while (ok && walk.next(p.seqs, p.shape, item)) {
+    while (ok && next_item(kStatusAttnLoadWait)) {
       const int rows = rows_of(item), row0 = item.tile * kTileRows;
       auto q_row = [&](int row) {
         const int r = row0 + row, i = over_group(p.shape, r);
@@ -315,7 +334,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const float most = f16 ? __half2float(__ushort_as_half(top)) : __uint_as_float(static_cast<uint32_t>(top) << 16);
             const uint32_t e2 = min(max(__float_as_uint(most) >> 23, 27u), 227u);
             const float down = __uint_as_float((254 - e2) << 23);
-            row_factor[items & 1][row] = __uint_as_float(e2 << 23) * p.scale;
+            row_factor[at_item & 1][row] = __uint_as_float(e2 << 23) * p.scale;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
               uint32_t o[4];
@@ -353,7 +372,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[g]);
       }
-      ++items;
+      ++at_item;
 
       const int part_hi = least_hi(item), part_lo = most_lo(item);
       for (int j = 0; ok && j < item.blocks; ++j) {
@@ -411,7 +430,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               const int r = at + 64 * h;
               bool bad = false;
               const bool gone = key0 + r >= item.s.length;  // what lies there was never copied, or is another's
-#pragma unroll
+#pragma unroll 4
               for (int c = 0; c < D / 8; ++c) {
                 uint4 *v = reinterpret_cast<uint4 *>(dst + swizzled(r, c));
                 uint4 x = *v;
@@ -439,12 +458,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + g * 128, o_at = tmem + lanes + 256 + g * D;
     uint8_t *const stage = stages + warp * kStageBytes;
-    int64_t n = 0;
-    int items = -1;
+    uint32_t n = 0;
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
-    while (ok && walk.next(p.seqs, p.shape, item)) {
-      ++items;
+    while (ok && next_item(kStatusAttnSoftmaxWait)) {
       const int rows = rows_of(item), row = g * 128 + r;
       if (rows <= g * 128) {  // the item has no second tile
         n += 2 * item.blocks;
@@ -471,7 +488,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         float scale = p.scale;
         if constexpr (S8) {
           scale = 1.f;
-          const float factor = row_factor[items & 1][row];
+          const float factor = row_factor[(k_item - 1) & 1][row];
           const float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -486,24 +503,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         }
         if (edge) {
+          // The columns that this row sees, a bit each: from lo - key0 up to hi - key0.
+          uint32_t sees[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int to = min(max(hi - key0 - 32 * c, 0), 32), from = min(max(lo - key0 - 32 * c, 0), 32);
+            sees[c] = (to == 32 ? ~0u : (1u << to) - 1) & ~(from == 32 ? ~0u : (1u << from) - 1);
+          }
           if constexpr (!S8) {
             const int slot = static_cast<int>((n + 1) % NS);
             ok = warp_wait(&ready[slot], ((n + 1) / NS) & 1, kStatusAttnSoftmaxWait);
             if (!ok) break;
+            uint32_t bad = 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t bits = bad_keys[slot][c];
-              if (bits)
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (bits >> e & 1) v[c][e] = NAN;
-            }
+            for (int c = 0; c < 4; ++c) bad |= bad_keys[slot][c] & sees[c];
+            if (bad) l = NAN;  // (a row that sees a value that is no number ends as NaN)
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (key0 + 32 * c + e >= hi || key0 + 32 * c + e < lo) v[c][e] = -INFINITY;
+              if (!(sees[c] >> e & 1)) v[c][e] = -INFINITY;
         }
         float top[4];
 #pragma unroll

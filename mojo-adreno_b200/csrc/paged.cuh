@@ -192,116 +192,101 @@ struct ShareScratch {
   Share found;
 };
 
-// This CTA's share; called by all THREADS threads. parts <= blockIdx.x: none.
+// This CTA's share, in sm.found; called by all THREADS threads. parts <= blockIdx.x: none.
 template <int THREADS, typename G>
-__device__ __forceinline__ Share find_share(const Seqs &s, const Shape &a, ShareScratch<THREADS> &sm) {
+__device__ __forceinline__ void find_share(const Seqs &s, const Shape &a, ShareScratch<THREADS> &sm) {
   constexpr int kWarps = THREADS / 32;
+  constexpr bool kOneTile = G::ROWS <= 64;  // a sequence has one tile at most
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  // Units of sequences base + 0 .. THREADS - 1 into sm.costs: a thread each where a sequence has one tile at most, else a
-  // warp each, its lanes on the tiles.
-  auto fill_costs = [&](int base) {
-    if (G::ROWS <= 64) {
+  int64_t total = 0;
+  // Twice through the sequences, THREADS at a time: for the total, and for the one in which the share begins. Once where
+  // one step takes all.
+  for (int pass = s.batch <= THREADS ? 1 : 0; pass < 2; ++pass) {
+    int64_t before = 0;
+    for (int base = 0; base < s.batch; base += THREADS) {
       int64_t cost = 0;
-      if (base + tid < s.batch) {
-        const Seq q = sequence(s, base + tid);
-        if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
-        if (takes_part(q, a)) cost = static_cast<int64_t>(G::EXTRA + tile_range<G>(q, a, 0).blocks) * a.kv_heads;
-      }
-      sm.costs[tid] = cost;
-    } else {
-      for (int b = warp; b < THREADS; b += kWarps) {
-        if (base + b >= s.batch) {
-          if (lane == 0) sm.costs[b] = 0;
-          continue;
+      if (kOneTile) {
+        if (base + tid < s.batch) {
+          const Seq q = sequence(s, base + tid);
+          if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
+          if (takes_part(q, a)) cost = static_cast<int64_t>(G::EXTRA + tile_range<G>(q, a, 0).blocks) * a.kv_heads;
         }
-        const Seq q = sequence(s, base + b);
-        int64_t cost = 0;
-        if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
-        if (takes_part(q, a))
-          for (int t = lane, tiles = tiles_of<G>(q, a); t < tiles; t += 32) cost += G::EXTRA + tile_range<G>(q, a, t).blocks;
+      } else {  // a warp for a sequence, its lanes for the tiles
+        for (int b = warp; b < min(THREADS, s.batch - base); b += kWarps) {
+          const Seq q = sequence(s, base + b);
+          int64_t units = 0;
+          if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
+          if (takes_part(q, a))
+            for (int t = lane, tiles = tiles_of<G>(q, a); t < tiles; t += 32) units += G::EXTRA + tile_range<G>(q, a, t).blocks;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
-        if (lane == 0) sm.costs[b] = cost * a.kv_heads;
+          for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+          if (lane == 0) sm.costs[b] = units * a.kv_heads;
+        }
+        __syncthreads();
+        if (base + tid < s.batch) cost = sm.costs[tid];
       }
-    }
-    __syncthreads();
-  };
-  int64_t mine = 0;
-  for (int base = 0; base < s.batch; base += THREADS) {
-    fill_costs(base);
-    mine += sm.costs[tid];
-    if (base + THREADS < s.batch) __syncthreads();
-  }
-  const bool many = s.batch > THREADS;  // (else sm.costs holds all)
+      int64_t incl = cost;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sm.sums[warp] = mine;
-  __syncthreads();
-  Share share{};
-  for (int w = 0; w < kWarps; ++w) share.total += sm.sums[w];
-  share.parts = static_cast<int>(share.total < gridDim.x ? share.total : gridDim.x);
-  if (static_cast<int>(blockIdx.x) >= share.parts) return share;
-  share.begin = share.total * blockIdx.x / share.parts;
-  share.end = share.total * (blockIdx.x + 1) / share.parts;
-  int64_t before = 0;
-  for (int base = 0; base < s.batch; base += THREADS) {
-    if (many) {
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      if (lane == 31) sm.sums[warp] = incl;
       __syncthreads();
-      fill_costs(base);
-    }
-    const int64_t cost = sm.costs[tid];
-    int64_t incl = cost;
+      int64_t start = before + incl - cost;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    __syncthreads();
-    if (lane == 31) sm.sums[warp] = incl;
-    __syncthreads();
-    int64_t ahead = before;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) ahead += sm.sums[w];
-      before += sm.sums[w];
-    }
-    // The warp with the sequence in which the share begins finds the tile.
-    const int64_t start = ahead + incl - cost;
-    const unsigned here = __ballot_sync(0xffffffffu, start <= share.begin && share.begin < start + cost);
-    if (here) {
-      const int from = __ffs(here) - 1, b = base + warp * 32 + from;
-      const int64_t offset = share.begin - __shfl_sync(0xffffffffu, start, from);
-      const int64_t per_head = __shfl_sync(0xffffffffu, cost, from) / a.kv_heads;
-      const int head = static_cast<int>(offset / per_head);
-      int64_t rest = offset - head * per_head;
-      int tile = 0;
-      if (G::ROWS > 64) {
-        const Seq q = sequence(s, b);
-        for (const int tiles = tiles_of<G>(q, a);; tile += 32) {
-          const int t = tile + lane;
-          const int64_t units = t < tiles ? G::EXTRA + tile_range<G>(q, a, t).blocks : 0;
-          int64_t sum = units;
+      for (int w = 0; w < kWarps; ++w) {
+        const int64_t sum = sm.sums[w];
+        if (w < warp) start += sum;
+        before += sum;
+      }
+      if (s.batch <= THREADS) total = before;
+      if (pass == 1) {
+        const int parts = static_cast<int>(total < gridDim.x ? total : gridDim.x);
+        if (base == 0 && tid == 0) sm.found.total = total, sm.found.parts = parts;
+        if (static_cast<int>(blockIdx.x) < parts) {
+          const int64_t begin = total * blockIdx.x / parts;
+          // The warp with the sequence in which the share begins finds the tile.
+          const unsigned here = __ballot_sync(0xffffffffu, start <= begin && begin < start + cost);
+          if (here) {
+            const int from = __ffs(here) - 1, b = base + warp * 32 + from;
+            const int64_t per_head = __shfl_sync(0xffffffffu, cost, from) / a.kv_heads;
+            int64_t rest = begin - __shfl_sync(0xffffffffu, start, from);
+            const int head = static_cast<int>(rest / per_head);
+            rest -= head * per_head;
+            int tile = 0;
+            if (!kOneTile) {
+              const Seq q = sequence(s, b);
+              for (const int tiles = tiles_of<G>(q, a);; tile += 32) {
+                const int t = tile + lane;
+                const int64_t units = t < tiles ? G::EXTRA + tile_range<G>(q, a, t).blocks : 0;
+                int64_t sum = units;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += up;
+                for (int o = 1; o < 32; o <<= 1) {
+                  const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+                  if (lane >= o) sum += up;
+                }
+                const unsigned in = __ballot_sync(0xffffffffu, rest < sum);
+                if (in) {  // (the units of all tiles are more than `rest`, so some lane's is)
+                  const int l = __ffs(in) - 1;
+                  rest -= __shfl_sync(0xffffffffu, sum - units, l);
+                  tile += l;
+                  break;
+                }
+                rest -= __shfl_sync(0xffffffffu, sum, 31);
+              }
+            }
+            if (lane == 0) {
+              sm.found.begin = begin, sm.found.end = total * (blockIdx.x + 1) / parts;
+              sm.found.b = b, sm.found.head = head, sm.found.tile = tile, sm.found.rest = static_cast<int>(rest);
+            }
           }
-          const unsigned in = __ballot_sync(0xffffffffu, rest < sum);
-          if (in) {  // (the units of all tiles are more than `rest`, so some lane's is)
-            const int l = __ffs(in) - 1;
-            rest -= __shfl_sync(0xffffffffu, sum - units, l);
-            tile += l;
-            break;
-          }
-          rest -= __shfl_sync(0xffffffffu, sum, 31);
         }
       }
-      if (lane == 0) sm.found.b = b, sm.found.head = head, sm.found.tile = tile, sm.found.rest = static_cast<int>(rest);
+      __syncthreads();
     }
-    if (before > share.begin) break;
+    total = before;
   }
-  __syncthreads();
-  share.b = sm.found.b, share.head = sm.found.head, share.tile = sm.found.tile, share.rest = sm.found.rest;
-  return share;
 }
 
 struct Item {
@@ -311,7 +296,7 @@ struct Item {
   int before, whole;  // blocks of the item before them, blocks of the item
 };
 
-// Walks through a share's items. Every role of a CTA walks by itself.
+// Walks through a share's items: the warp that brings keys and values does, and tells the others.
 template <typename G>
 struct Walk {
   Seq s;
@@ -342,6 +327,26 @@ struct Walk {
     rest = 0;
     ++tile;
     return item.blocks > 0;  // (a share may end before the first block of its last item)
+  }
+};
+
+// Where it does: the next item is in item[k % kItems] when its `full` barrier says so; an item without blocks ends it.
+constexpr int kItems = 4;
+struct ItemRing {
+  Item item[kItems];
+  uint64_t full[kItems], empty[kItems];
+  __device__ __forceinline__ void init(int readers) {
+    for (int i = 0; i < kItems; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], readers);
+  }
+  // By a whole warp.
+  __device__ __forceinline__ bool put(int k, const Item &it) {
+    if (k >= kItems && !__all_sync(0xffffffffu, mbar_wait(&empty[k % kItems], (k / kItems - 1) & 1))) return false;
+    if (threadIdx.x % 32 == 0) {
+      item[k % kItems] = it;
+      mbar_arrive(&full[k % kItems]);
+    }
+    __syncwarp();
+    return true;
   }
 };
 
