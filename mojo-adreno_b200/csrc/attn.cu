@@ -11,8 +11,7 @@
 //
 //  * A producer warp brings blocks of 64 keys and values through a ring, one tiled copy per page (or part of one) and
 //    128 (int8: 64) bytes of a row, a lane each; the ring's barriers are the only ones between producer and consumers.
-//  * Four consumer warps: MT of them take 16 rows each, the others share the block's keys. Each keeps its own
-//    running maximum, sum and accumulators, in fp32, and they meet once, when an item ends.
+//  * Four consumer warps share a block's keys. Each keeps its own running maximum, sum and accumulators, in fp32, and they meet once, when an item ends.
 //  * All CTAs take equal shares of all blocks (paged.cuh), so lengths need not be known on the host and a long
 //    sequence takes as many SMs as it has work for. Parts of cut items are joined by a kernel behind this one, in a fixed
 //    order: results do not vary from run to run.
@@ -20,6 +19,8 @@
 //    1024 + it), the rows' q to fp16 after a power of two that its largest |q| fixes (exact but below 2^-24 of that). s_j scales
 //    the scores; t_j goes into the exponent: w_j t_j = 2^(score + log2 t_j - m) with m the maximum of that, so the
 //    weights that meet the integers are at most 2^8 whatever the scales, and the sum of w is that of (w t) (1 / t).
+//  * Neither kernel lets the next one start early: its CTAs would sit on the SMs with room for some, and one of this grid's,
+//    which is exactly as many as run at once, would begin when all others end (64x1 int8: 210 us instead of 146).
 //  * The maximum may lag by 2^8 before accumulators are rescaled: weights up to 2^8 are as exact in fp16 and bf16.
 //  * Blocks that some row sees only in part: scores are replaced, not added to, so no masked key's value matters; a
 //    value that is no number is taken out of the product and makes the score of its key NaN for the rows that see it.
@@ -28,7 +29,7 @@
 namespace mq {
 namespace paged {
 
-constexpr int kFewKeys = 64, kFewRows = 64;  // keys of a block; the most rows of an item
+constexpr int kFewKeys = 64, kFewRows = 16;  // keys of a block; the most rows of an item
 constexpr int kFewWarps = 4, kFewThreads = 32 * (kFewWarps + 1);
 using FewGrain = Grain<kFewRows, kFewKeys, 2>;
 constexpr int kPadCols = 72;                 // floats between rows of the joining buffer: no bank conflicts
@@ -120,40 +121,38 @@ __device__ __forceinline__ void store_out4(const Output &o, int64_t token, int64
 // What a row's accumulators are multiplied by: 0 for a row that sees nothing, NaN where its sum is.
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-template <int D, int MT, int KIND>
+template <int D, int KIND>
 struct Few {
   static constexpr int kBytes = KIND == MQ_S8 ? 1 : 2;
   static constexpr int kBox = KIND == MQ_S8 ? 64 : 128;                 // bytes of a row in a box
   static constexpr int kBoxes = D * kBytes / kBox;
   static constexpr int kTile = kFewKeys * D * kBytes;                   // of keys, or of values
-  static constexpr int kScales = KIND == MQ_S8 ? 2 * kFewKeys * 4 : 0;  // of keys and of values
+  static constexpr int kScales = KIND == MQ_S8 ? 3 * kFewKeys * 4 : 0;  // keys' scales, values': log2 and inverse
   static constexpr int kStageBytes = 2 * kTile + 1024 * (kScales > 0);
-  // Two CTAs on an SM where a stage has 32 KB or a warp works on 64 keys of 128 dim (204 registers), else three; as
-  // many stages, up to four, as fit beside the joining buffer.
-  static constexpr int kCtas = kTile == 16384 || (MT == 4 && D == 128) ? 2 : 3;
-  static constexpr int kJoin = kFewRows * kPadCols * 4;
+  // Two CTAs on an SM where a stage has 32 KB, else three; as many stages, up to four, as fit beside the joining buffer.
+  static constexpr int kCtas = kTile == 16384 ? 2 : 3;
+  static constexpr int kJoin = kFewWarps * kFewRows * kPadCols * 4;
   static constexpr int kRoom = (227 * 1024 / kCtas - 1024 - kJoin - 2048) / kStageBytes;
   static constexpr int kStages = kRoom > 4 ? 4 : kRoom;
   static constexpr int kSmem = kStages * kStageBytes + kJoin + 1024;
 };
 
-template <int D, int MT, int KIND>
-__global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
+template <int D, int KIND>
+__global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
     attn_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
-  using F = Few<D, MT, KIND>;
+  using F = Few<D, KIND>;
   constexpr bool BF = KIND == MQ_BF16, S8 = KIND == MQ_S8;
-  constexpr int WK = kFewWarps / MT, KW = kFewKeys / WK;  // warps that share a block's keys; keys of a warp
+  constexpr int WK = kFewWarps, KW = kFewKeys / WK;  // the warps share a block's keys
   constexpr int NT = KW / 8, S = F::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float *join = reinterpret_cast<float *>(ring + S * F::kStageBytes);  // [WK][16 MT][kPadCols]
+  float *join = reinterpret_cast<float *>(ring + S * F::kStageBytes);  // [WK][kFewRows][kPadCols]
   __shared__ uint64_t full[S], empty[S], meeting;
   __shared__ ShareScratch<kFewThreads> scratch;
   __shared__ ItemRing items;
-  __shared__ float2 row_stats[WK][16 * MT];
+  __shared__ float2 row_stats[WK][kFewRows];
   __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  griddep_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], S8 ? 33 : 1);  // the copies' bytes; the lanes whose scales have come
@@ -208,6 +207,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
               sk[h] = p.k_scale[of * p.ks_stride[0] + item.head * p.ks_stride[1] + row * p.ks_stride[2]];
               sv[h] = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
             }
+            if (sv[h] < kLeastScale) sv[h] = kLeastScale;  // (fmaxf would drop a NaN)
           }
         }
         if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[s], (round - 1) & 1))) {
@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
         if (S8) {
           float *sc = reinterpret_cast<float *>(stage + 2 * F::kTile);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) sc[lane + 32 * h] = sk[h], sc[kFewKeys + lane + 32 * h] = sv[h];
+          for (int h = 0; h < 2; ++h)
+            sc[lane + 32 * h] = sk[h], sc[kFewKeys + lane + 32 * h] = lg2(sv[h]), sc[2 * kFewKeys + lane + 32 * h] = __frcp_rn(sv[h]);
         }
         if (lane == 0) mbar_expect_tx(&full[s], 2 * live * F::kBoxes * box_rows * F::kBox);
         __syncwarp();
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
     return;
   }
 
-  const int mt = warp % MT, wk = warp / MT, g = lane / 4, t = lane % 4;
+  const int wk = warp, g = lane / 4, t = lane % 4;
   const int heads = p.shape.group;
   int s = 0;
   uint32_t phase = 0, meetings = 0;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
     int lo[2], hi[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = mt * 16 + g + 8 * r, i = over_group(p.shape, min(row, rows - 1));
+      const int row = g + 8 * r, i = over_group(p.shape, min(row, rows - 1));
       const int pos = item.s.pos0 + i;
       hi[r] = max(pos + 1, 0);
       lo[r] = p.shape.window ? max(0, pos + 1 - p.shape.window) : 0;
@@ -401,12 +402,9 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
       for (int j = 0; j < NT; ++j) {
         if (S8) {
           const float2 ks = *reinterpret_cast<const float2 *>(scales + wk * KW + 8 * j + 2 * t);
-          float2 vs = *reinterpret_cast<const float2 *>(scales + kFewKeys + wk * KW + 8 * j + 2 * t);
-          // (fmaxf would drop a NaN)
-          vs.x = vs.x < kLeastScale ? kLeastScale : vs.x, vs.y = vs.y < kLeastScale ? kLeastScale : vs.y;
-          const float lx = lg2(vs.x), ly = lg2(vs.y);
-          c[j][0] = fmaf(c[j][0] * row_scale[0], ks.x, lx), c[j][1] = fmaf(c[j][1] * row_scale[0], ks.y, ly);
-          c[j][2] = fmaf(c[j][2] * row_scale[1], ks.x, lx), c[j][3] = fmaf(c[j][3] * row_scale[1], ks.y, ly);
+          const float2 lv = *reinterpret_cast<const float2 *>(scales + kFewKeys + wk * KW + 8 * j + 2 * t);
+          c[j][0] = fmaf(c[j][0] * row_scale[0], ks.x, lv.x), c[j][1] = fmaf(c[j][1] * row_scale[0], ks.y, lv.y);
+          c[j][2] = fmaf(c[j][2] * row_scale[1], ks.x, lv.x), c[j][3] = fmaf(c[j][3] * row_scale[1], ks.y, lv.y);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[j][e] *= p.scale;
@@ -473,11 +471,14 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
       if (S8) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float2 vs = *reinterpret_cast<const float2 *>(scales + kFewKeys + wk * KW + 8 * j + 2 * t);
-          const float ix = __frcp_rn(vs.x < kLeastScale ? kLeastScale : vs.x), iy = __frcp_rn(vs.y < kLeastScale ? kLeastScale : vs.y);
-          // (a masked key's scale may be anything, its weight is 0)
-          l[0] += (c[j][0] == 0.f ? 0.f : c[j][0] * ix) + (c[j][1] == 0.f ? 0.f : c[j][1] * iy);
-          l[1] += (c[j][2] == 0.f ? 0.f : c[j][2] * ix) + (c[j][3] == 0.f ? 0.f : c[j][3] * iy);
+          const float2 iv = *reinterpret_cast<const float2 *>(scales + 2 * kFewKeys + wk * KW + 8 * j + 2 * t);
+          if (edge) {  // (a key that the row does not see may have any scale; its weight is 0)
+            l[0] += (c[j][0] == 0.f ? 0.f : c[j][0] * iv.x) + (c[j][1] == 0.f ? 0.f : c[j][1] * iv.y);
+            l[1] += (c[j][2] == 0.f ? 0.f : c[j][2] * iv.x) + (c[j][3] == 0.f ? 0.f : c[j][3] * iv.y);
+          } else {
+            l[0] += c[j][0] * iv.x + c[j][1] * iv.y;
+            l[1] += c[j][2] * iv.x + c[j][3] * iv.y;
+          }
         }
       }
       // Weights become the MMA's A; 16-bit caches sum them as they were rounded, so that the two roundings cancel where
@@ -532,23 +533,23 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t == 0) row_stats[wk][mt * 16 + g + 8 * r] = make_float2(m[r], l[r]);
+      if (t == 0) row_stats[wk][g + 8 * r] = make_float2(m[r], l[r]);
     }
     if (!meet()) break;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < WK; ++w) top = fmaxf(top, row_stats[w][mt * 16 + g + 8 * r].x);
+      for (int w = 0; w < WK; ++w) top = fmaxf(top, row_stats[w][g + 8 * r].x);
       const float a = m[r] == top ? 1.f : ex2(m[r] - top);
 #pragma unroll
       for (int j = 0; j < D / 8; ++j) o[j][2 * r] *= a, o[j][2 * r + 1] *= a;
     }
     const bool goes_on = item.before > 0, whole = !goes_on && item.blocks == item.whole;
-    const int64_t part0 = (2 * static_cast<int64_t>(blockIdx.x) + (goes_on ? 0 : 1)) * (16 * MT);
+    const int64_t part0 = (2 * static_cast<int64_t>(blockIdx.x) + (goes_on ? 0 : 1)) * (kFewRows);
 #pragma unroll
     for (int h = 0; h < D / 64; ++h) {
-      float *mine = join + (wk * 16 * MT + mt * 16) * kPadCols;
+      float *mine = join + (wk * kFewRows) * kPadCols;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float *at = mine + (g + 8 * r) * kPadCols;
@@ -565,13 +566,13 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
         }
       }
       if (!meet()) return;
-      for (int e = tid; e < 16 * MT * 16; e += 32 * kFewWarps) {
+      for (int e = tid; e < kFewRows * 16; e += 32 * kFewWarps) {
         const int row = e / 16, col = e % 16 * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < WK; ++w) {
-          const float4 x = *reinterpret_cast<const float4 *>(join + (w * 16 * MT + row) * kPadCols + col);
+          const float4 x = *reinterpret_cast<const float4 *>(join + (w * kFewRows + row) * kPadCols + col);
           v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
           top = fmaxf(top, row_stats[w][row].x);
         }
@@ -598,61 +599,56 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, MT, KIND>::kCtas)
 }
 
 // Joins the parts of the items that CTAs of the launch before shared. CTA c (of x) takes the item that c goes on with
-// where c is the first to do so; y: 16 rows each.
+// where c is the first to do so; a warp a row. What a row needs is known after one load (the cut), so that the
+// parts' statistics and sums come together: a few CTAs' parts of a short call take 3 us, most of it the launch.
 struct JoinParams {
-  Seqs seqs;
   Shape shape;
   Output o;
   Parts parts;
   int rows;  // of an item's parts
 };
+constexpr int kJoinRows = 8;
 template <int D, int TILE_ROWS>
-__global__ void __launch_bounds__(128) attn_join_kernel(const JoinParams p) {
-  griddep_launch_dependents();
+__global__ void __launch_bounds__(32 * kJoinRows) attn_join_kernel(const JoinParams p) {
   griddep_wait();
+  const int c = blockIdx.x, lane = threadIdx.x % 32;
+  if (c == 0) return;
   const int64_t total = p.parts.counts[0], ctas = p.parts.counts[1];
-  const int c = blockIdx.x;
-  if (c == 0 || c >= ctas) return;
-  const Cut cut = p.parts.cuts[c];
-  if (!cut.goes_on || total * (c - 1) / ctas > cut.first) return;
-  const Seq s = sequence(p.seqs, cut.b);
-  const int rows = min(TILE_ROWS, s.n * p.shape.group - cut.tile * TILE_ROWS);
-  const int row = blockIdx.y * 16 + threadIdx.x / 8, u = threadIdx.x % 8;
-  if (static_cast<int>(blockIdx.y) * 16 >= rows) return;
-  int last = c;  // the item's last CTA
-  while (last + 1 < ctas && total * (last + 1) / ctas < cut.end) ++last;
-  const int from = row < rows ? row : 0;
-  // Part 0 is CTA c - 1's, which began the item (its slot 1), the others what CTAs c .. last went on with (slot 0).
-  const int n = last - c + 2;
-  auto at = [&](int i) { return (2 * static_cast<int64_t>(c - 1 + i) + (i == 0 ? 1 : 0)) * p.rows + from; };
+  const Cut cut = p.parts.cuts[c];  // (there is one, used or not)
+  if (c >= ctas || !cut.goes_on || total * (c - 1) / ctas > cut.first) return;
+  const int rows = min(TILE_ROWS, cut.n * p.shape.group - cut.tile * TILE_ROWS);
+  const int row = blockIdx.y * kJoinRows + threadIdx.x / 32;
+  if (row >= rows) return;
+  // Part 0 is CTA c - 1's, which began the item (its slot 1), the others what CTAs c .. last went on with (slot 0); CTA `last`
+  // is the last whose share begins before the item's end.
+  const int last = static_cast<int>((cut.end * ctas + total - 1) / total) - 1, n = last - c + 2;
+  auto at = [&](int i) { return (2 * static_cast<int64_t>(c - 1 + i) + (i == 0 ? 1 : 0)) * p.rows + row; };
   float top = -INFINITY;
-  for (int i = u; i < n; i += 8) top = fmaxf(top, p.parts.stats[at(i)].x);
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, p.parts.stats[at(i)].x);
 #pragma unroll
-  for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  constexpr int kLanes = D / 4, kTurns = 32 / kLanes;  // lanes of a part, parts at a time
+  const int u = lane % kLanes;
   float sum = 0.f;
-  float4 v[D / 32];
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (int i = 0; i < n; ++i) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = lane / kLanes; i < n; i += kTurns) {
     const int64_t a = at(i);
     const float2 st = p.parts.stats[a];
+    const float4 x = *reinterpret_cast<const float4 *>(p.parts.sums + a * D + u * 4);
     const float w = st.x == top ? 1.f : ex2(st.x - top);
     sum += st.y * w;
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      const float4 x = *reinterpret_cast<const float4 *>(p.parts.sums + a * D + (k * 8 + u) * 4);
-      v[k].x += x.x * w, v[k].y += x.y * w, v[k].z += x.z * w, v[k].w += x.w * w;
-    }
+    v.x += x.x * w, v.y += x.y * w, v.z += x.z * w, v.w += x.w * w;
   }
-  if (row >= rows) return;
+  if (kTurns == 2) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, 16), v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+    v.z += __shfl_xor_sync(0xffffffffu, v.z, 16), v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+  }
   const float inv = inverse_sum(sum);
   const int r = cut.tile * TILE_ROWS + row, i = over_group(p.shape, r);
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k)
-    if ((k * 8 + u) * 4 < p.o.dim)
-      store_out4(p.o, s.first + i, cut.head * p.shape.group + r - i * p.shape.group, (k * 8 + u) * 4, v[k].x * inv,
-                 v[k].y * inv, v[k].z * inv, v[k].w * inv);
+  if (lane < kLanes && u * 4 < p.o.dim)
+    store_out4(p.o, cut.token + i, cut.head * p.shape.group + r - i * p.shape.group, u * 4, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
 }
 
 // A map of a pool's rows: (dim, row of the page, head, page), boxes of `box_bytes` of `box_rows` rows.
@@ -670,21 +666,21 @@ inline int encode_pages(CUtensorMap *map, void *base, int dtype, const mq_kv_pag
                         dims, strides, box, swizzle, what);
 }
 
-template <int D, int MT, int KIND>
+template <int D, int KIND>
 int launch_few(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, cudaStream_t stream, const char *what) {
-  using F = Few<D, MT, KIND>;
+  using F = Few<D, KIND>;
   CUtensorMap kmap, vmap;
   const int box_rows = std::min(kFewKeys, c->page);
   const CUtensorMapSwizzle swizzle = KIND == MQ_S8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   if (int rc = encode_pages(&kmap, c->k, KIND, c, c->k_stride, F::kBox, box_rows, swizzle, what)) return rc;
   if (int rc = encode_pages(&vmap, c->v, KIND, c, c->v_stride, F::kBox, box_rows, swizzle, what)) return rc;
-  p.parts = parts_at(workspace, ctas, 16 * MT);
+  p.parts = parts_at(workspace, ctas, kFewRows);
   static size_t configured[64] = {};
-  auto kern = attn_few_kernel<D, MT, KIND>;
+  auto kern = attn_few_kernel<D, KIND>;
   if (int rc = ensure_smem(kern, F::kSmem, configured, what)) return rc;
   if (int rc = launch_overlapped(kern, dim3(ctas), dim3(kFewThreads), F::kSmem, stream, what, kmap, vmap, p)) return rc;
-  JoinParams j{p.seqs, p.shape, p.o, p.parts, 16 * MT};
-  return launch_overlapped(attn_join_kernel<D, kFewRows>, dim3(ctas, MT), dim3(128), 0, stream, what, j);
+  JoinParams j{p.shape, p.o, p.parts, kFewRows};
+  return launch_overlapped(attn_join_kernel<D, kFewRows>, dim3(ctas, kFewRows / kJoinRows), dim3(32 * kJoinRows), 0, stream, what, j);
 }
 
 }  // namespace paged

@@ -111,10 +111,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock, *stages = raw + 2 * T::kRaw;
-  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained, s_full[2], p_full[2], o_full[2];
+  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained, s_full[2], p_full[2], o_full[2], half_done, half_read;
   __shared__ uint32_t bad_keys[NS][4];
   __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
   __shared__ ItemRing items;
+  __shared__ float2 half_stats[128];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -133,6 +134,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&empty[i], 1);
     }
     mbar_init(&drained, 1);
+    mbar_init(&half_done, 4);
+    mbar_init(&half_read, 4);
     items.init(1 + kAuxWarps + 8);
     abort_flag = 0;
     fence_mbar_init();
@@ -240,8 +243,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       uint32_t p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
       bool ok = true;
       auto slot_of = [&](uint32_t i) { return static_cast<int>(i % NS); };
-      auto scores = [&](int g, int slot) {
-        const uint32_t a = smem_u32(q_tile) + g * (T::kQ / 2), b = smem_u32(ring + slot * T::kBlock);
+      // S of accumulator g from q tile `q` and the keys in a slot; O of accumulator g from its weights and the values there.
+      auto scores = [&](int g, int q, int slot) {
+        const uint32_t a = smem_u32(q_tile) + q * (T::kQ / 2), b = smem_u32(ring + slot * T::kBlock);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           umma_f16(tmem + g * 128, umma_desc_sw128(a + (k / 4) * 16384) + 2 * (k % 4), umma_desc_sw128(b + (k / 4) * 16384) + 2 * (k % 4),
@@ -254,41 +258,48 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int k = 0; k < kTileKeys / 16; ++k)
           umma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, b + k * (2048 >> 4), pv, !first || k != 0);
       };
+      auto await = [&](uint64_t *bar, uint32_t parity) {
+        if (ok) ok = wait(bar, parity, kStatusAttnMmaWait);
+        tc_fence_after();
+        return ok;
+      };
+      auto await_slot = [&](uint32_t i) { return await(&ready[slot_of(i)], (i / NS) & 1); };
       while (next_item(kStatusAttnMmaWait)) {
         if (lane == 0) {
-        const int tiles = rows_of(item) > 128 ? 2 : 1;
-        ok = wait(&ready[slot_of(n)], (n / NS) & 1, kStatusAttnMmaWait);
-        for (int g = 0; ok && g < tiles; ++g) {
-          ok = wait(&q_full[g], q_phase[g], kStatusAttnMmaWait);
-          if (!ok) break;
-          q_phase[g] ^= 1;
-          tc_fence_after();
-          scores(g, slot_of(n));
-          if (item.blocks == 1) umma_commit(&q_empty[g]);
-        }
-        if (ok) umma_commit(&empty[slot_of(n)]);
-        for (int j = 0; ok && j < item.blocks; ++j, n += 2) {
-          const bool more = j + 1 < item.blocks;
-          const uint32_t v = n + 1, k = n + 2;
-          ok = wait(&ready[slot_of(v)], (v / NS) & 1, kStatusAttnMmaWait);
-          for (int g = 0; ok && g < tiles; ++g) {
-            ok = wait(&p_full[g], p_phase[g], kStatusAttnMmaWait);
-            if (!ok) break;
-            p_phase[g] ^= 1;
-            tc_fence_after();
-            values(g, slot_of(v), j == 0);
-            if (g == tiles - 1) umma_commit(&empty[slot_of(v)]);
-            if (more) {
-              if (g == 0 && !(ok = wait(&ready[slot_of(k)], (k / NS) & 1, kStatusAttnMmaWait))) break;
-              tc_fence_after();
-              scores(g, slot_of(k));
-              if (j + 2 == item.blocks) umma_commit(&q_empty[g]);
-            } else {
-              umma_commit(&o_full[g]);
+          // Step j works on accumulator j & 1: of the two tiles, block by block, or of a narrow item's blocks in turn. Scores run
+          // two steps ahead of the values.
+          const bool narrow = rows_of(item) <= 128;
+          const int steps = narrow ? item.blocks : 2 * item.blocks;
+          auto score = [&](int j) {
+            const int g = j & 1, block = narrow ? j : j >> 1;
+            const uint32_t k = n + 2 * block;
+            if (narrow || g == 0) await_slot(k);
+            if (j < (narrow ? 1 : 2)) {
+              await(&q_full[g], q_phase[g]);
+              q_phase[g] ^= 1;
             }
+            if (!ok) return;
+            scores(g, narrow ? 0 : g, slot_of(k));
+            if (narrow || g == 1) umma_commit(&empty[slot_of(k)]);
+            if (block == item.blocks - 1) umma_commit(&q_empty[narrow ? 0 : g]);
+          };
+          score(0);
+          if (ok && steps > 1) score(1);
+#pragma unroll 1
+          for (int j = 0; ok && j < steps; ++j) {
+            const int g = j & 1;
+            const uint32_t v = n + 2 * (narrow ? j : j >> 1) + 1;
+            if (narrow || g == 0) await_slot(v);
+            if (!await(&p_full[g], p_phase[g])) break;
+            p_phase[g] ^= 1;
+            values(g, slot_of(v), j < 2);
+            if (narrow || g == 1) umma_commit(&empty[slot_of(v)]);
+            if (j + 2 < steps)
+              score(j + 2);
+            else
+              umma_commit(&o_full[g]);
           }
-          if (ok && more) umma_commit(&empty[slot_of(k)]);
-        }
+          n += 2 * item.blocks;
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
@@ -458,26 +469,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + g * 128, o_at = tmem + lanes + 256 + g * D;
     uint8_t *const stage = stages + warp * kStageBytes;
-    uint32_t n = 0;
-    uint32_t s_phase = 0, o_phase = 0;
+    uint32_t n0 = 0, s_phase = 0, o_phase[2] = {0, 0}, half_phase = 0;
     bool ok = true;
     while (ok && next_item(kStatusAttnSoftmaxWait)) {
-      const int rows = rows_of(item), row = g * 128 + r;
-      if (rows <= g * 128) {  // the item has no second tile
-        n += 2 * item.blocks;
-        continue;
-      }
+      // An item of two tiles: each group has one. A narrow one: the groups take its blocks in turn, and group 0 joins the two.
+      const int rows = rows_of(item);
+      const bool narrow = rows <= 128, halves = narrow && item.blocks > 1;
+      const int row = (narrow ? 0 : g * 128) + r;
       const int index = item.tile * kTileRows + min(row, rows - 1), i = over_group(p.shape, index);
       const int hi = row < rows ? max(item.s.pos0 + i + 1, 0) : 0;
       const int lo = p.shape.window ? max(0, item.s.pos0 + i + 1 - p.shape.window) : 0;
       const int part_hi = least_hi(item), part_lo = most_lo(item);
+      const bool idle = row - lane >= rows;  // no row of this warp is one: its weights may be anything
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < item.blocks; ++j, n += 2) {
+      const int first = narrow ? g : 0, step = narrow ? 2 : 1;
+      for (int j = first; j < item.blocks; j += step) {
+        const uint32_t n = n0 + 2 * j;
         const int key0 = (item.block + j) * kTileKeys;
         ok = warp_wait(&s_full[g], s_phase, kStatusAttnSoftmaxWait);
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after();
+        if (idle) {
+          if (lane == 0) mbar_arrive(&p_full[g]);
+          continue;
+        }
         float v[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32_async(s_at + 32 * c, v[c]);
@@ -539,7 +555,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const float a = m == next ? 1.f : ex2(m - next);
           l *= a;
           m = next;
-          if (j > 0) {
+          if (j != first) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               float o[16];
@@ -585,12 +601,40 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[g]);
       }
       if (!ok) break;
-      ok = warp_wait(&o_full[g], o_phase, kStatusAttnSoftmaxWait);
+      n0 += 2 * item.blocks;
+      const uint32_t done[2] = {o_phase[0], o_phase[1]};
+      o_phase[0] ^= 1;
+      if (!narrow || halves) o_phase[1] ^= 1;
+      if (narrow && g == 1) {
+        if (halves) {
+          half_stats[r] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&half_done);
+          ok = warp_wait(&half_read, half_phase, kStatusAttnSoftmaxWait);  // then this accumulator is free again
+          half_phase ^= 1;
+        }
+        continue;
+      }
+      ok = warp_wait(&o_full[g], done[g], kStatusAttnSoftmaxWait);
+      if (ok && halves) {
+        ok = warp_wait(&o_full[1], done[1], kStatusAttnSoftmaxWait) && warp_wait(&half_done, half_phase, kStatusAttnSoftmaxWait);
+        half_phase ^= 1;
+      }
       if (!ok) break;
-      o_phase ^= 1;
       tc_fence_after();
+      float a0 = 1.f, a1 = 0.f;
+      if (halves) {
+        const float2 other = half_stats[r];
+        const float most = fmaxf(m, other.x);
+        a0 = m == most ? 1.f : ex2(m - most), a1 = other.x == most ? 1.f : ex2(other.x - most);
+        l = l * a0 + other.y * a1;
+        m = most;
+      }
       const bool goes_on = item.before > 0, whole = !goes_on && item.blocks == item.whole;
-      const float inv = whole ? inverse_sum(l) : 1.f;
+      if (whole) {
+        const float inv = inverse_sum(l);
+        a0 *= inv, a1 *= inv;
+      }
       const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (goes_on ? 0 : 1)) * kTileRows + row;
       if (!whole && row < rows) p.parts.stats[part] = make_float2(m, l);
       // 64 bytes of each of the warp's rows at a time: through shared memory, so that eight rows leave with one store
@@ -607,13 +651,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_ld32(o_at + 32 * c, o);
         else
           tmem_ld16(o_at + 16 * c, reinterpret_cast<float(&)[16]>(o));
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] *= a0;
+        if (halves) {
+          float x[32];
+          if (whole)
+            tmem_ld32(o_at + D + 32 * c, x);
+          else
+            tmem_ld16(o_at + D + 16 * c, reinterpret_cast<float(&)[16]>(x));
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] += x[e] * a1;
+        }
         uint4 w[4];
         uint32_t *words = reinterpret_cast<uint32_t *>(w);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           words[e] = !whole                  ? __float_as_uint(o[e])
-                     : p.o.dtype == MQ_F16 ? pack16<false>(o[2 * e] * inv, o[2 * e + 1] * inv)
-                                            : pack16<true>(o[2 * e] * inv, o[2 * e + 1] * inv);
+                     : p.o.dtype == MQ_F16 ? pack16<false>(o[2 * e], o[2 * e + 1])
+                                            : pack16<true>(o[2 * e], o[2 * e + 1]);
         __syncwarp();
 #pragma unroll
         for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4 *>(stage + lane * 64 + ((u ^ (lane >> 1)) & 3) * 16) = w[u];
@@ -622,11 +677,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int it = 0; it < 4; ++it) {
           const int from = it * 8 + lane / 4, u = lane % 4;
           const int64_t to = __shfl_sync(0xffffffffu, mine, from) + 64 * c + 16 * u;
-          if (g * 128 + (warp & 3) * 32 + from < rows && 64 * c + 16 * u < width)
+          if (row - lane + from < rows && 64 * c + 16 * u < width)
             *reinterpret_cast<uint4 *>(base + to) = *reinterpret_cast<const uint4 *>(stage + from * 64 + ((u ^ (from >> 1)) & 3) * 16);
         }
       }
       tc_fence_before();
+      if (halves) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&half_read);
+      }
     }
   }
   tc_fence_before();
@@ -656,15 +715,15 @@ int launch_tile(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, c
   }();
   MQ_REQUIRE(regs == kTileRegs, MQ_ECUDA, "%s: the kernel was built with %d registers, not %d", what, regs, kTileRegs);
   if (int rc = launch_overlapped(kern, dim3(ctas), dim3(kTileThreads), T::kSmem, stream, what, kmap, vmap, p)) return rc;
-  JoinParams j{p.seqs, p.shape, p.o, p.parts, kTileRows};
-  return launch_overlapped(attn_join_kernel<D, kTileRows>, dim3(ctas, kTileRows / 16), dim3(128), 0, stream, what, j);
+  JoinParams j{p.shape, p.o, p.parts, kTileRows};
+  return launch_overlapped(attn_join_kernel<D, kTileRows>, dim3(ctas, kTileRows / kJoinRows), dim3(32 * kJoinRows), 0, stream, what, j);
 }
 
-// The rows of a kv head above which a sequence goes to the tensor core's tiles; at most kFewRows.
+// The rows of a kv head above which a sequence goes to the tensor core's tiles.
 constexpr int kRowsForTiles = kFewRows;
 
 struct Plan {
-  int few, few_ctas, tile_ctas;  // few: 16-row tiles per item, 0 without that launch; tile_ctas: 0 without that launch
+  int few_ctas, tile_ctas;  // 0 without that launch
   int d, most_rows;
   size_t bytes;
 };
@@ -676,14 +735,13 @@ inline int plan_for(Plan *plan, const mq_kv_pages *c, int64_t heads, int64_t bat
   int64_t most = starts ? std::min(tokens, max_new > 0 ? max_new : tokens) : 1;
   plan->most_rows = static_cast<int>(most * group);
   plan->d = c->dim <= 64 ? 64 : 128;
-  plan->few = group > kRowsForTiles ? 0 : plan->most_rows <= 16 ? 1 : plan->most_rows <= 32 ? 2 : 4;
-  // One sequence has all the tokens.
-  if (batch == 1 && tokens * group > kRowsForTiles && most == tokens) plan->few = 0;
-  const bool tile = plan->most_rows > kRowsForTiles || plan->few == 0;
-  plan->few_ctas = plan->few == 0 ? 0 : sms * (c->dtype != MQ_S8 && plan->d == 128 ? 2 : plan->few == 4 && plan->d == 128 ? 2 : 3);
+  // One sequence may have all the tokens.
+  const bool few = group <= kRowsForTiles && !(batch == 1 && most == tokens && tokens * group > kRowsForTiles);
+  const bool tile = plan->most_rows > kRowsForTiles || !few;
+  plan->few_ctas = !few ? 0 : sms * (c->dtype != MQ_S8 && plan->d == 128 ? 2 : 3);
   plan->tile_ctas = tile ? sms : 0;
   plan->bytes = 0;
-  if (plan->few) plan->bytes = parts_bytes(plan->few_ctas, 16 * plan->few, plan->d);
+  if (few) plan->bytes = parts_bytes(plan->few_ctas, kFewRows, plan->d);
   if (tile) plan->bytes = std::max(plan->bytes, parts_bytes(sms, kTileRows, plan->d));
   return MQ_OK;
 }
@@ -691,19 +749,12 @@ inline int plan_for(Plan *plan, const mq_kv_pages *c, int64_t heads, int64_t bat
 template <int D, int KIND>
 int launch_attention(const Plan &plan, const mq_kv_pages *c, AttnParams p, void *workspace, cudaStream_t s, const char *what) {
   p.shape.rows_most = plan.most_rows;
-  if (plan.few) {
-    p.shape.rows_from = 0, p.shape.rows_to = std::min(kRowsForTiles, 16 * plan.few);
-    int rc;
-    if (plan.few == 1)
-      rc = launch_few<D, 1, KIND>(c, p, plan.few_ctas, workspace, s, what);
-    else if (plan.few == 2)
-      rc = launch_few<D, 2, KIND>(c, p, plan.few_ctas, workspace, s, what);
-    else
-      rc = launch_few<D, 4, KIND>(c, p, plan.few_ctas, workspace, s, what);
-    if (rc) return rc;
+  if (plan.few_ctas) {
+    p.shape.rows_from = 0, p.shape.rows_to = kRowsForTiles;
+    if (int rc = launch_few<D, KIND>(c, p, plan.few_ctas, workspace, s, what)) return rc;
   }
   if (plan.tile_ctas) {
-    p.shape.rows_from = plan.few ? kRowsForTiles : 0, p.shape.rows_to = plan.most_rows;
+    p.shape.rows_from = plan.few_ctas ? kRowsForTiles : 0, p.shape.rows_to = plan.most_rows;
     return launch_tile<D, KIND>(c, p, plan.tile_ctas, workspace, s, what);
   }
   return MQ_OK;

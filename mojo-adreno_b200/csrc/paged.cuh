@@ -353,14 +353,15 @@ struct ItemRing {
 // A CTA leaves at most two parts of items that others share: one that it goes on with (slot 0) and one that it
 // begins and does not end (slot 1). `cut` says which item the CTA goes on with.
 struct Cut {
-  int32_t b, head, tile, goes_on;
+  int32_t token, n;  // the sequence's first row, its rows
+  int32_t head, tile, goes_on, unused[3];
   int64_t first, end;  // the units of the item's blocks
 };
 // Of a walk that has just started.
 template <typename G>
 __device__ __forceinline__ Cut cut_at(const Walk<G> &w, const Shape &a, const Share &share) {
   const int64_t first = share.begin - share.rest + G::EXTRA;
-  return {w.b, w.head, w.tile, share.rest > G::EXTRA, first, first + tile_range<G>(w.s, a, w.tile).blocks};
+  return {w.s.first, w.s.n, w.head, w.tile, share.rest > G::EXTRA, {}, first, first + tile_range<G>(w.s, a, w.tile).blocks};
 }
 struct Parts {
   int64_t *counts;  // units, CTAs with a share
@@ -369,6 +370,7 @@ struct Parts {
   float *sums;      // [ctas][2][rows][D]
 };
 inline size_t parts_bytes(int ctas, int rows, int d) {
+  static_assert(sizeof(Cut) % 16 == 0, "the sums are read 16 bytes at a time");
   return 256 + static_cast<size_t>(ctas) * (sizeof(Cut) + 2ull * rows * (sizeof(float2) + 4ull * d));
 }
 inline Parts parts_at(void *workspace, int ctas, int rows) {
