@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
             if (sv[h] < kLeastScale) sv[h] = kLeastScale;  // (fmaxf would drop a NaN)
           }
         }
-        if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[s], (round - 1) & 1))) {
+        if (round > 0 && !__all_sync(0xffffffffu, wait_for(&empty[s], (round - 1) & 1))) {
           if (lane == 0) raise_status(kStatusAttnLoadWait), abort_flag = 1;
           ok = false;
           break;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
     }
     // Leave no copy in flight.
     if (lane == 0)
-      for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i) mbar_wait(&full[i % S], (i / S) & 1);
+      for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i) wait_for(&full[i % S], (i / S) & 1);
     return;
   }
 
@@ -257,13 +257,13 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
   auto meet = [&]() -> bool {
     __syncwarp();
     if (lane == 0) mbar_arrive(&meeting);
-    const bool met = !abort_flag && mbar_wait(&meeting, meetings++ & 1);
+    const bool met = !abort_flag && wait_for(&meeting, meetings++ & 1);
     if (__all_sync(0xffffffffu, met)) return true;
     if (lane == 0 && !abort_flag) raise_status(kStatusAttnSoftmaxWait), abort_flag = 1;
     return false;
   };
   for (int k = 0;; ++k) {
-    const bool told = mbar_wait(&items.full[k % kItems], (k / kItems) & 1);
+    const bool told = wait_for(&items.full[k % kItems], (k / kItems) & 1);
     if (!__all_sync(0xffffffffu, told)) {
       if (lane == 0 && !abort_flag) raise_status(kStatusAttnSoftmaxWait), abort_flag = 1;
       break;  // (what the others wait for next does not come either)
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // l: this thread's columns
 
     for (int b = 0; b < item.blocks; ++b) {
-      const bool came = !abort_flag && mbar_wait(&full[s], phase);
+      const bool came = !abort_flag && wait_for(&full[s], phase);
       if (!__all_sync(0xffffffffu, came)) {
         if (lane == 0 && !abort_flag) raise_status(kStatusAttnSoftmaxWait), abort_flag = 1;
         break;

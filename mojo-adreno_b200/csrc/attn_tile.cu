@@ -11,6 +11,8 @@
 //    between the copies and the MMAs: of an int8 cache they make fp16 of every block; of a 16-bit one they take what is
 //    no number out of the values of the blocks that some row sees only in part, and say which keys had any.
 //  * One persistent CTA per SM, all of TMEM, equal shares of the blocks: causal or ragged, no SM waits for another.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace mq {
@@ -111,19 +113,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock, *stages = raw + 2 * T::kRaw;
-  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained, s_full[2], p_full[2], o_full[2], half_done, half_read;
+  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained, s_full[2], p_half[2], p_full[2], o_full[2], half_done, half_read;
   __shared__ uint32_t bad_keys[NS][4];
   __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
   __shared__ ItemRing items;
   __shared__ float2 half_stats[128];
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) {
     for (int i = 0; i < NF; ++i) mbar_init(&full[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&raw_empty[i], kAuxWarps);
       mbar_init(&s_full[i], 1);
+      mbar_init(&p_half[i], 4);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&q_full[i], kAuxWarps);
@@ -137,7 +139,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(&half_done, 4);
     mbar_init(&half_read, 4);
     items.init(1 + kAuxWarps + 8);
-    abort_flag = 0;
     fence_mbar_init();
   }
   griddep_wait();  // (before TMEM is taken: the kernels before this one have returned theirs)
@@ -155,10 +156,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const bool works = static_cast<int>(blockIdx.x) < share.parts;
   const int group = p.shape.group;
   Item item;
-  // Waits that give up set the flag, and everybody leaves at the next wait.
+  // A role whose wait gives up leaves; so do then those that wait for it.
   auto wait = [&](uint64_t *bar, uint32_t parity, int code) -> bool {
-    if (!abort_flag && mbar_wait(bar, parity)) return true;
-    if (!abort_flag) raise_status(code), abort_flag = 1;
+    if (wait_for(bar, parity)) return true;
+    raise_status(code);
     return false;
   };
   auto warp_wait = [&](uint64_t *bar, uint32_t parity, int code) -> bool {
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     while (ok) {
       if (!walk.next(p.seqs, p.shape, item)) item.blocks = 0;
       if (!items.put(k_item++, item)) {
-        if (lane == 0) raise_status(kStatusAttnLoadWait), abort_flag = 1;
+        if (lane == 0) raise_status(kStatusAttnLoadWait);
         break;
       }
       if (item.blocks == 0) break;
@@ -235,78 +236,99 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     // Leave no copy in flight.
     if (lane == 0)
-      for (uint32_t i = issued > NF ? issued - NF : 0; i < issued; ++i) mbar_wait(&full[i % NF], (i / NF) & 1);
+      for (uint32_t i = issued > NF ? issued - NF : 0; i < issued; ++i) wait_for(&full[i % NF], (i / NF) & 1);
   } else if (warp == 9) {
     {
       constexpr uint32_t qk = idesc_16(128, kTileKeys, BF, false), pv = idesc_16(128, D, BF, true);
-      uint32_t n = 0;  // slots used: keys and values in turn
+      // Keys and values take the ring's slots in turn: where the next scores' keys are, and the next product's values.
+      struct At {
+        int slot;
+        uint32_t phase;
+        __device__ void next() {
+          if ((slot += 2) >= NS) slot -= NS, phase ^= 1;
+        }
+      } at_k{0, 0}, at_v{1, 0};
       uint32_t p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
       bool ok = true;
-      auto slot_of = [&](uint32_t i) { return static_cast<int>(i % NS); };
-      // S of accumulator g from q tile `q` and the keys in a slot; O of accumulator g from its weights and the values there.
+      // Descriptors' low words; the high ones are constant. 64 columns of a K-major operand are 16 KB apart, its 16-column
+      // steps 32 bytes; the 16-key steps of the values 2 KB.
+      const uint32_t q_low = (smem_u32(q_tile) >> 4) & 0x3FFF, ring_low = (smem_u32(ring) >> 4) & 0x3FFF;
+      constexpr uint32_t kHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+      auto desc = [](uint32_t low) { return static_cast<uint64_t>(kHigh) << 32 | low; };
+      // S of accumulator g from q tile `q` and the keys in a slot; O of accumulator g from half of its weights and the
+      // values there.
       auto scores = [&](int g, int q, int slot) {
-        const uint32_t a = smem_u32(q_tile) + q * (T::kQ / 2), b = smem_u32(ring + slot * T::kBlock);
+        const uint32_t a = q_low + q * (T::kQ / 2 >> 4) + (1u << 16), b = ring_low + slot * (T::kBlock >> 4) + (1u << 16);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_f16(tmem + g * 128, umma_desc_sw128(a + (k / 4) * 16384) + 2 * (k % 4), umma_desc_sw128(b + (k / 4) * 16384) + 2 * (k % 4),
-                   qk, k != 0);
+          umma_f16(tmem + g * 128, desc(a + (k / 4) * 1024 + 2 * (k % 4)), desc(b + (k / 4) * 1024 + 2 * (k % 4)), qk, k != 0);
         umma_commit(&s_full[g]);
       };
-      auto values = [&](int g, int slot, bool first) {
-        const uint64_t b = umma_desc_mn128(smem_u32(ring + slot * T::kBlock));
+      auto values = [&](int g, int slot, int half, bool first) {
+        const uint32_t b = ring_low + slot * (T::kBlock >> 4) + (1024u << 16);
 #pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k)
-          umma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, b + k * (2048 >> 4), pv, !first || k != 0);
+        for (int k = 4 * half; k < 4 * half + 4; ++k)
+          umma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, desc(b + k * 128), pv, !first || k != 0);
       };
       auto await = [&](uint64_t *bar, uint32_t parity) {
         if (ok) ok = wait(bar, parity, kStatusAttnMmaWait);
         tc_fence_after();
         return ok;
       };
-      auto await_slot = [&](uint32_t i) { return await(&ready[slot_of(i)], (i / NS) & 1); };
       while (next_item(kStatusAttnMmaWait)) {
         if (lane == 0) {
           // Step j works on accumulator j & 1: of the two tiles, block by block, or of a narrow item's blocks in turn. Scores run
           // two steps ahead of the values.
           const bool narrow = rows_of(item) <= 128;
           const int steps = narrow ? item.blocks : 2 * item.blocks;
-          auto score = [&](int j) {
-            const int g = j & 1, block = narrow ? j : j >> 1;
-            const uint32_t k = n + 2 * block;
-            if (narrow || g == 0) await_slot(k);
+          auto score = [&](auto gc, int j) {
+            constexpr int g = decltype(gc)::value;
+            if (narrow || g == 0) await(&ready[at_k.slot], at_k.phase);
             if (j < (narrow ? 1 : 2)) {
               await(&q_full[g], q_phase[g]);
               q_phase[g] ^= 1;
             }
             if (!ok) return;
-            scores(g, narrow ? 0 : g, slot_of(k));
-            if (narrow || g == 1) umma_commit(&empty[slot_of(k)]);
-            if (block == item.blocks - 1) umma_commit(&q_empty[narrow ? 0 : g]);
+            scores(g, narrow ? 0 : g, at_k.slot);
+            if (narrow || g == 1) {
+              umma_commit(&empty[at_k.slot]);
+              at_k.next();
+            }
+            if (j + (narrow ? 1 : 2) >= steps) umma_commit(&q_empty[narrow ? 0 : g]);
           };
-          score(0);
-          if (ok && steps > 1) score(1);
-#pragma unroll 1
-          for (int j = 0; ok && j < steps; ++j) {
-            const int g = j & 1;
-            const uint32_t v = n + 2 * (narrow ? j : j >> 1) + 1;
-            if (narrow || g == 0) await_slot(v);
-            if (!await(&p_full[g], p_phase[g])) break;
+          auto turn = [&](auto gc, int j) {
+            constexpr int g = decltype(gc)::value;
+            if (narrow || g == 0) await(&ready[at_v.slot], at_v.phase);
+            if (!await(&p_half[g], p_phase[g])) return;
+            values(g, at_v.slot, 0, j < 2);
+            if (!await(&p_full[g], p_phase[g])) return;
             p_phase[g] ^= 1;
-            values(g, slot_of(v), j < 2);
-            if (narrow || g == 1) umma_commit(&empty[slot_of(v)]);
+            values(g, at_v.slot, 1, false);
+            if (narrow || g == 1) {
+              umma_commit(&empty[at_v.slot]);
+              at_v.next();
+            }
             if (j + 2 < steps)
-              score(j + 2);
+              score(gc, j + 2);
             else
               umma_commit(&o_full[g]);
+          };
+          const std::integral_constant<int, 0> zero;
+          const std::integral_constant<int, 1> one;
+          score(zero, 0);
+          if (ok && steps > 1) score(one, 1);
+#pragma unroll 1
+          for (int j = 0; ok && j < steps; j += 2) {
+            turn(zero, j);
+            if (ok && j + 1 < steps) turn(one, j + 1);
           }
-          n += 2 * item.blocks;
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
       }
       if (!ok && lane == 0) {  // what was issued ends before TMEM goes
         umma_commit(&drained);
-        mbar_wait(&drained, 0);
+        wait_for(&drained, 0);
       }
     }
     __syncwarp();
@@ -491,15 +513,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         s_phase ^= 1;
         tc_fence_after();
         if (idle) {
-          if (lane == 0) mbar_arrive(&p_full[g]);
+          if (lane == 0) mbar_arrive(&p_half[g]), mbar_arrive(&p_full[g]);
           continue;
         }
         float v[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_async(s_at + 32 * c, v[c]);
+        tmem_ld32_async(s_at, v[0]);
+        tmem_ld32_async(s_at + 32, v[1]);
         tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_loaded(v[c]);
+        tmem_ld32_async(s_at + 64, v[2]);
+        tmem_ld32_async(s_at + 96, v[3]);
+        tmem_loaded(v[0]);
+        tmem_loaded(v[1]);
+        tmem_wait_ld();
+        tmem_loaded(v[2]);
+        tmem_loaded(v[3]);
         const bool edge = key0 + kTileKeys > part_hi || key0 < part_lo;
         float scale = p.scale;
         if constexpr (S8) {
@@ -593,12 +620,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
           }
           tmem_st16(s_at + 16 * c, w);
+          if (c & 1) {  // the first half's product starts while the second is made
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c == 1 ? &p_half[g] : &p_full[g]);
+          }
         }
         l += sum[0] + sum[1];
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g]);
       }
       if (!ok) break;
       n0 += 2 * item.blocks;
@@ -646,29 +675,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int pieces = whole ? (p.o.dim + 31) / 32 : D / 16, width = whole ? 2 * p.o.dim : 4 * D;
 #pragma unroll 1
       for (int c = 0; c < pieces; ++c) {
-        float o[32];
-        if (whole)
-          tmem_ld32(o_at + 32 * c, o);
-        else
-          tmem_ld16(o_at + 16 * c, reinterpret_cast<float(&)[16]>(o));
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] *= a0;
-        if (halves) {
-          float x[32];
-          if (whole)
-            tmem_ld32(o_at + D + 32 * c, x);
-          else
-            tmem_ld16(o_at + D + 16 * c, reinterpret_cast<float(&)[16]>(x));
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] += x[e] * a1;
-        }
         uint4 w[4];
         uint32_t *words = reinterpret_cast<uint32_t *>(w);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          words[e] = !whole                  ? __float_as_uint(o[e])
-                     : p.o.dtype == MQ_F16 ? pack16<false>(o[2 * e], o[2 * e + 1])
-                                            : pack16<true>(o[2 * e], o[2 * e + 1]);
+        for (int half = 0; half < 2; ++half) {  // 16 columns a time: 8 words of a 16-bit row, or all 16 of a part's
+          if (half == 1 && !whole) break;
+          const int col = whole ? 32 * c + 16 * half : 16 * c;
+          float o[16];
+          tmem_ld16(o_at + col, o);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] *= a0;
+          if (halves) {
+            float x[16];
+            tmem_ld16(o_at + D + col, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] += x[e] * a1;
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              words[8 * half + e] = p.o.dtype == MQ_F16 ? pack16<false>(o[2 * e], o[2 * e + 1]) : pack16<true>(o[2 * e], o[2 * e + 1]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) words[e] = __float_as_uint(o[e]);
+          }
+        }
         __syncwarp();
 #pragma unroll
         for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4 *>(stage + lane * 64 + ((u ^ (lane >> 1)) & 3) * 16) = w[u];

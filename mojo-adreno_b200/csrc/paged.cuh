@@ -50,6 +50,17 @@ __device__ __forceinline__ int page_of(const Seqs &s, int b, int position) {
   return -1;
 }
 
+// mbar_wait in fewer instructions: a role waits in many places, and code that is not in the instruction cache yet costs
+// a short call more than the waiting.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  do {
+    if (mbar_try_wait(bar, parity)) return true;
+  } while (globaltimer() - t0 < kWaitTimeoutNs);
+  return false;
+}
+
 // ---- host: checks -----------------------------------------------------------------------------------
 
 inline int element_size(int dtype) { return dtype == MQ_F32 ? 4 : dtype == MQ_S8 ? 1 : 2; }
@@ -340,7 +351,7 @@ struct ItemRing {
   }
   // By a whole warp.
   __device__ __forceinline__ bool put(int k, const Item &it) {
-    if (k >= kItems && !__all_sync(0xffffffffu, mbar_wait(&empty[k % kItems], (k / kItems - 1) & 1))) return false;
+    if (k >= kItems && !__all_sync(0xffffffffu, wait_for(&empty[k % kItems], (k / kItems - 1) & 1))) return false;
     if (threadIdx.x % 32 == 0) {
       item[k % kItems] = it;
       mbar_arrive(&full[k % kItems]);
