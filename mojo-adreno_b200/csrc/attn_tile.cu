@@ -7,7 +7,8 @@
 //    rescaled there only when a row's maximum has grown by 2^8 since the last time.
 //  * V is used as it lies, [keys][dim], as an MN-major B operand: nothing is transposed.
 //  * Warps 0-3 and 4-7: softmax and output of the two tiles. Warp 8: the copies of keys and values, a lane per page (or part
-//    of one) and 128 bytes of row. Warp 9: one thread issues the MMAs. Warps 10 and 11: bring q, and stand
+//    of one) and 128 bytes of row. Warps 9 and 10: a
+//    thread each issues the MMAs of an accumulator. Warps 12 to 15: bring q, and stand
 //    between the copies and the MMAs: of an int8 cache they make fp16 of every block; of a 16-bit one they take what is
 //    no number out of the values of the blocks that some row sees only in part, and say which keys had any.
 //  * One persistent CTA per SM, all of TMEM, equal shares of the blocks: causal or ragged, no SM waits for another.
@@ -19,11 +20,11 @@ namespace mq {
 namespace paged {
 
 constexpr int kTileKeys = 128, kTileRows = 256;
-constexpr int kTileThreads = 384, kAuxWarps = 2;
+constexpr int kTileThreads = 512, kAuxWarps = 4;
 using TileGrain = Grain<kTileRows, kTileKeys, 2>;
-// Registers of a thread at launch, of a softmax thread (a row of scores is 128 of them) and of the others.
-constexpr int kTileRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 104;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kTileThreads * kTileRegs, "more registers than the block was launched with");
+// Registers of a thread at launch, of a softmax thread (half a row of scores is 64 of them) and of the others.
+constexpr int kTileRegs = 128, kSoftmaxRegs = 152, kOtherRegs = 104;
+static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kTileThreads * kTileRegs, "more registers than the block was launched with");
 constexpr int kStageBytes = 2048;  // per softmax warp: 64 bytes of each of its rows on their way out
 
 template <int D, int KIND>
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock, *stages = raw + 2 * T::kRaw;
-  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained, s_full[2], p_half[2], p_full[2], o_full[2], half_done, half_read;
+  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained[2], s_full[2][2], p_full[2][2], o_step[2], o_full[2], half_done, half_read;
   __shared__ uint32_t bad_keys[NS][4];
   __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
   __shared__ ItemRing items;
@@ -124,21 +125,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     for (int i = 0; i < NF; ++i) mbar_init(&full[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&raw_empty[i], kAuxWarps);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_half[i], 4);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&o_step[i], 1);
       mbar_init(&o_full[i], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[i][b], 1);
+        mbar_init(&p_full[i][b], 4);
+      }
       mbar_init(&q_full[i], kAuxWarps);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_empty[i], 2);  // of both MMA threads, or twice of the one that used it
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&ready[i], kAuxWarps);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], 2);  // of both MMA threads
     }
-    mbar_init(&drained, 1);
+    mbar_init(&drained[0], 1);
+    mbar_init(&drained[1], 1);
     mbar_init(&half_done, 4);
     mbar_init(&half_read, 4);
-    items.init(1 + kAuxWarps + 8);
+    items.init(2 + kAuxWarps + 8);
     fence_mbar_init();
   }
   griddep_wait();  // (before TMEM is taken: the kernels before this one have returned theirs)
@@ -237,9 +241,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // Leave no copy in flight.
     if (lane == 0)
       for (uint32_t i = issued > NF ? issued - NF : 0; i < issued; ++i) wait_for(&full[i % NF], (i / NF) & 1);
-  } else if (warp == 9) {
+  } else if (warp == 9 || warp == 10) {
     {
-      constexpr uint32_t qk = idesc_16(128, kTileKeys, BF, false), pv = idesc_16(128, D, BF, true);
+      // A thread for each accumulator: what it waits for and what it commits takes as long as its MMAs, so one thread for both
+      // left the tensor core idle half of the time (8192 tokens: MMA MMA_TIME).
+      constexpr uint32_t qk = idesc_16(128, 64, BF, false), pv = idesc_16(128, D, BF, true);
+      const int g = warp - 9;
       // Keys and values take the ring's slots in turn: where the next scores' keys are, and the next product's values.
       struct At {
         int slot;
@@ -248,92 +255,78 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if ((slot += 2) >= NS) slot -= NS, phase ^= 1;
         }
       } at_k{0, 0}, at_v{1, 0};
-      uint32_t p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+      uint32_t p_phase = 0, q_phase[2] = {0, 0};  // p_phase: a bit for each buffer
       bool ok = true;
       // Descriptors' low words; the high ones are constant. 64 columns of a K-major operand are 16 KB apart, its 16-column
-      // steps 32 bytes; the 16-key steps of the values 2 KB.
+      // steps 32 bytes, 64 keys 8 KB; the 16-key steps of the values 2 KB.
       const uint32_t q_low = (smem_u32(q_tile) >> 4) & 0x3FFF, ring_low = (smem_u32(ring) >> 4) & 0x3FFF;
+      const uint32_t s_tmem = tmem + g * 128, o_tmem = tmem + 256 + g * D;
       constexpr uint32_t kHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
       auto desc = [](uint32_t low) { return static_cast<uint64_t>(kHigh) << 32 | low; };
-      // S of accumulator g from q tile `q` and the keys in a slot; O of accumulator g from half of its weights and the
-      // values there.
-      auto scores = [&](int g, int q, int slot) {
-        const uint32_t a = q_low + q * (T::kQ / 2 >> 4) + (1u << 16), b = ring_low + slot * (T::kBlock >> 4) + (1u << 16);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_f16(tmem + g * 128, desc(a + (k / 4) * 1024 + 2 * (k % 4)), desc(b + (k / 4) * 1024 + 2 * (k % 4)), qk, k != 0);
-        umma_commit(&s_full[g]);
-      };
-      auto values = [&](int g, int slot, int half, bool first) {
-        const uint32_t b = ring_low + slot * (T::kBlock >> 4) + (1024u << 16);
-#pragma unroll
-        for (int k = 4 * half; k < 4 * half + 4; ++k)
-          umma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + k * 8, desc(b + k * 128), pv, !first || k != 0);
-      };
       auto await = [&](uint64_t *bar, uint32_t parity) {
         if (ok) ok = wait(bar, parity, kStatusAttnMmaWait);
-        tc_fence_after();
         return ok;
       };
       while (next_item(kStatusAttnMmaWait)) {
         if (lane == 0) {
-          // Step j works on accumulator j & 1: of the two tiles, block by block, or of a narrow item's blocks in turn. Scores run
-          // two steps ahead of the values.
+          // A step is 64 keys. An item of two tiles: both halves of each block for this one's rows. A narrow one: half g of
+          // each block. Scores run two steps ahead of the values, in the two halves of the accumulator in turn.
           const bool narrow = rows_of(item) <= 128;
-          const int steps = narrow ? item.blocks : 2 * item.blocks;
-          auto score = [&](auto gc, int j) {
-            constexpr int g = decltype(gc)::value;
-            if (narrow || g == 0) await(&ready[at_k.slot], at_k.phase);
-            if (j < (narrow ? 1 : 2)) {
-              await(&q_full[g], q_phase[g]);
-              q_phase[g] ^= 1;
-            }
-            if (!ok) return;
-            scores(g, narrow ? 0 : g, at_k.slot);
-            if (narrow || g == 1) {
+          const int q = narrow ? 0 : g, steps = narrow ? item.blocks : 2 * item.blocks;
+          auto score = [&](int i) {
+            const int half = narrow ? g : i & 1;
+            if ((narrow || half == 0) && !await(&ready[at_k.slot], at_k.phase)) return;
+            const uint32_t a = q_low + q * (T::kQ / 2 >> 4) + (1u << 16);
+            const uint32_t b = ring_low + at_k.slot * (T::kBlock >> 4) + half * (8192 >> 4) + (1u << 16);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_f16(s_tmem + (i & 1) * 64, desc(a + (k / 4) * 1024 + 2 * (k % 4)), desc(b + (k / 4) * 1024 + 2 * (k % 4)), qk, k != 0);
+            umma_commit(&s_full[g][i & 1]);
+            if (narrow || half == 1) {
               umma_commit(&empty[at_k.slot]);
               at_k.next();
             }
-            if (j + (narrow ? 1 : 2) >= steps) umma_commit(&q_empty[narrow ? 0 : g]);
+            if (i == steps - 1) {
+              umma_commit(&q_empty[q]);
+              if (!narrow) umma_commit(&q_empty[q]);
+            }
           };
-          auto turn = [&](auto gc, int j) {
-            constexpr int g = decltype(gc)::value;
-            if (narrow || g == 0) await(&ready[at_v.slot], at_v.phase);
-            if (!await(&p_half[g], p_phase[g])) return;
-            values(g, at_v.slot, 0, j < 2);
-            if (!await(&p_full[g], p_phase[g])) return;
-            p_phase[g] ^= 1;
-            values(g, at_v.slot, 1, false);
-            if (narrow || g == 1) {
-              umma_commit(&empty[at_v.slot]);
+          await(&q_full[q], q_phase[q]);
+          q_phase[0] ^= 1;
+          if (!narrow) q_phase[1] ^= 1;
+          if (ok) score(0);
+          if (ok && steps > 1) score(1);
+#pragma unroll 1
+          for (int i = 0; ok && i < steps; ++i) {
+            const int half = narrow ? g : i & 1, buffer = i & 1;
+            if (narrow || half == 0) await(&ready[at_v.slot], at_v.phase);
+            if (!await(&p_full[g][buffer], p_phase >> buffer & 1)) break;
+            p_phase ^= 1u << buffer;
+            tc_fence_after();
+            const uint32_t b = ring_low + at_v.slot * (T::kBlock >> 4) + half * (8192 >> 4) + (1024u << 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16_ts(o_tmem, s_tmem + buffer * 64 + k * 8, desc(b + k * 128), pv, i != 0 || k != 0);
+            umma_commit(&o_step[g]);
+            if (i == steps - 1) umma_commit(&o_full[g]);
+            if (narrow || half == 1) {
+              umma_commit(&empty[at_v.slot]);  // (before the next keys are waited for, which may need this slot)
               at_v.next();
             }
-            if (j + 2 < steps)
-              score(gc, j + 2);
-            else
-              umma_commit(&o_full[g]);
-          };
-          const std::integral_constant<int, 0> zero;
-          const std::integral_constant<int, 1> one;
-          score(zero, 0);
-          if (ok && steps > 1) score(one, 1);
-#pragma unroll 1
-          for (int j = 0; ok && j < steps; j += 2) {
-            turn(zero, j);
-            if (ok && j + 1 < steps) turn(one, j + 1);
+            if (i + 2 < steps) score(i + 2);
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
       }
       if (!ok && lane == 0) {  // what was issued ends before TMEM goes
-        umma_commit(&drained);
-        wait_for(&drained, 0);
+        umma_commit(&drained[g]);
+        wait_for(&drained[g], 0);
       }
     }
     __syncwarp();
-  } else {
-    const int at = tid - 320;  // 0 .. 63
+  } else if (warp >= 12) {
+    const int at = tid - 384;  // 0 .. 127
     uint32_t n = 0;
     int at_item = 0, q_uses[2] = {0, 0};
     bool ok = true;
@@ -351,41 +344,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!ok) break;
         ++q_uses[g];
         if constexpr (S8) {
-          for (int r = at; r < 128; r += 64) {
-            const int row = g * 128 + r;
-            uint4 w[D / 8];
-            const uint16_t *src = q_row(min(row, rows - 1));
+          const int r = at, row = g * 128 + r;
+          const uint16_t *src = q_row(min(row, rows - 1));
+          const bool f16 = p.q_dtype == MQ_F16;
+          auto chunk = [&](int c) {
+            return row < rows && 8 * c < p.o.dim ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+          };
+          uint32_t big = 0;  // the largest |q|'s bits, of either half
+#pragma unroll 8
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 w = chunk(c);
+            big = __vmaxu2(__vmaxu2(big, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+          }
+          const uint16_t top = static_cast<uint16_t>(max(big & 0xffff, big >> 16));
+          const float most = f16 ? __half2float(__ushort_as_half(top)) : __uint_as_float(static_cast<uint32_t>(top) << 16);
+          const uint32_t e2 = min(max(__float_as_uint(most) >> 23, 27u), 227u);
+          const float down = __uint_as_float((254 - e2) << 23);
+          row_factor[at_item & 1][row] = __uint_as_float(e2 << 23) * p.scale;
+#pragma unroll 4
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 w = chunk(c);
+            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+            uint32_t o[4];
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-              w[c] = row < rows && 8 * c < p.o.dim ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-            uint32_t big = 0;  // the largest |q|'s bits, of either half
-            const uint32_t *x = reinterpret_cast<const uint32_t *>(w);
-#pragma unroll
-            for (int e = 0; e < D / 2; ++e) big = __vmaxu2(big, x[e] & 0x7fff7fffu);
-            const uint16_t top = static_cast<uint16_t>(max(big & 0xffff, big >> 16));
-            const bool f16 = p.q_dtype == MQ_F16;
-            const float most = f16 ? __half2float(__ushort_as_half(top)) : __uint_as_float(static_cast<uint32_t>(top) << 16);
-            const uint32_t e2 = min(max(__float_as_uint(most) >> 23, 27u), 227u);
-            const float down = __uint_as_float((254 - e2) << 23);
-            row_factor[at_item & 1][row] = __uint_as_float(e2 << 23) * p.scale;
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              uint32_t o[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t y = x[4 * c + e];
-                const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2 *>(&y))
-                                     : make_float2(__uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u));
-                o[e] = pack_half2(f.x * down, f.y * down);
-              }
-              *reinterpret_cast<uint4 *>(dst + swizzled(r, c)) = make_uint4(o[0], o[1], o[2], o[3]);
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = f16 ? __half22float2(*reinterpret_cast<const __half2 *>(&x[e]))
+                                   : make_float2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u));
+              o[e] = pack_half2(f.x * down, f.y * down);
             }
+            *reinterpret_cast<uint4 *>(dst + swizzled(r, c)) = make_uint4(o[0], o[1], o[2], o[3]);
           }
         } else {
           constexpr int kLanes = D / 8;  // of a row
           const int c = at % kLanes;
 #pragma unroll 4
-          for (int r = at / kLanes; r < 128; r += 64 / kLanes) {
+          for (int r = at / kLanes; r < 128; r += 128 / kLanes) {
             const int row = g * 128 + r;
             const bool real = row < rows && 8 * c < p.o.dim;
             const uint16_t *src = q_row(min(row, rows - 1)) + (real ? 8 * c : 0);
@@ -410,19 +403,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int part_hi = least_hi(item), part_lo = most_lo(item);
       for (int j = 0; ok && j < item.blocks; ++j) {
         const int key0 = (item.block + j) * kTileKeys;
-        float sk[2], sv[2];
-        if (S8) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int key = key0 + at + 64 * h;
-            sk[h] = sv[h] = 0.f;
-            if (key < item.s.length) {
-              const int of = page_of(p.seqs, item.b, key), row = key & ((1 << p.seqs.page_log2) - 1);
-              if (of >= 0) {
-                sk[h] = p.k_scale[of * p.ks_stride[0] + item.head * p.ks_stride[1] + row * p.ks_stride[2]];
-                sv[h] = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
-              }
-            }
+        const int r = at, key = key0 + r;  // this thread's
+        float sk = 0.f, sv = 0.f;
+        if (S8 && key < item.s.length) {
+          const int of = page_of(p.seqs, item.b, key), row = key & ((1 << p.seqs.page_log2) - 1);
+          if (of >= 0) {
+            sk = p.k_scale[of * p.ks_stride[0] + item.head * p.ks_stride[1] + row * p.ks_stride[2]];
+            sv = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
           }
         }
         for (int which = 0; which < 2; ++which, ++n) {
@@ -433,50 +420,44 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           uint8_t *dst = ring + slot * T::kBlock;
           if constexpr (S8) {
             const uint8_t *from = raw + src * T::kRaw;
-            for (int h = 0; h < 2; ++h) {
-              const int r = at + 64 * h;
-              uint4 w[D / 16];
+            uint4 w[D / 16];
 #pragma unroll
-              for (int c = 0; c < D / 16; ++c)
-                w[c] = *reinterpret_cast<const uint4 *>(from + (D == 128 ? r * 128 + ((c ^ r) & 7) * 16 : r * 64 + ((c ^ (r >> 1)) & 3) * 16));
+            for (int c = 0; c < D / 16; ++c)
+              w[c] = *reinterpret_cast<const uint4 *>(from + (D == 128 ? r * 128 + ((c ^ r) & 7) * 16 : r * 64 + ((c ^ (r >> 1)) & 3) * 16));
 #pragma unroll
-              for (int c = 0; c < D / 16; ++c) {
-                const uint32_t x[4] = {w[c].x ^ 0x80808080u, w[c].y ^ 0x80808080u, w[c].z ^ 0x80808080u, w[c].w ^ 0x80808080u};
-                uint32_t o[8];
+            for (int c = 0; c < D / 16; ++c) {
+              const uint32_t x[4] = {w[c].x ^ 0x80808080u, w[c].y ^ 0x80808080u, w[c].z ^ 0x80808080u, w[c].w ^ 0x80808080u};
+              uint32_t o[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[2 * e] = bytes_to_half2<0x4140>(x[e]), o[2 * e + 1] = bytes_to_half2<0x4342>(x[e]);
-                *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
-              }
-              if (which == 0) {
-                // (the softmax has read block n / 2 - 2's by now: the slot just waited for came behind its weights)
-                const float vs = sv[h] < kLeastScale ? kLeastScale : sv[h];
-                float (&sc)[3][S8 ? kTileKeys : 1] = scales[(n >> 1) & 1];
-                sc[0][r] = sk[h], sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
-              }
+              for (int e = 0; e < 4; ++e) o[2 * e] = bytes_to_half2<0x4140>(x[e]), o[2 * e + 1] = bytes_to_half2<0x4342>(x[e]);
+              *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            if (which == 0) {
+              // (the softmax has read block n / 2 - 2's by now: the slot just waited for came behind its weights)
+              const float vs = sv < kLeastScale ? kLeastScale : sv;
+              float (&sc)[3][S8 ? kTileKeys : 1] = scales[(n >> 1) & 1];
+              sc[0][r] = sk, sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&raw_empty[src]);
           } else if (which == 1 && (key0 + kTileKeys > part_hi || key0 < part_lo)) {
-            for (int h = 0; h < 2; ++h) {
-              const int r = at + 64 * h;
-              bool bad = false;
-              const bool gone = key0 + r >= item.s.length;  // what lies there was never copied, or is another's
+            bool bad = false;
+            const bool gone = key >= item.s.length;  // what lies there was never copied, or is another's
 #pragma unroll 4
-              for (int c = 0; c < D / 8; ++c) {
-                uint4 *v = reinterpret_cast<uint4 *>(dst + swizzled(r, c));
-                uint4 x = *v;
-                const uint4 m = {not_finite2<BF>(x.x), not_finite2<BF>(x.y), not_finite2<BF>(x.z), not_finite2<BF>(x.w)};
-                if (m.x | m.y | m.z | m.w) {
-                  bad = true;
-                  x.x &= ~m.x, x.y &= ~m.y, x.z &= ~m.z, x.w &= ~m.w;
-                  *v = x;
-                }
+            for (int c = 0; c < D / 8; ++c) {
+              uint4 *v = reinterpret_cast<uint4 *>(dst + swizzled(r, c));
+              uint4 x = *v;
+              const uint4 m = {not_finite2<BF>(x.x), not_finite2<BF>(x.y), not_finite2<BF>(x.z), not_finite2<BF>(x.w)};
+              if (m.x | m.y | m.z | m.w) {
+                bad = true;
+                x.x &= ~m.x, x.y &= ~m.y, x.z &= ~m.z, x.w &= ~m.w;
+                *v = x;
               }
-              const uint32_t bits = __ballot_sync(0xffffffffu, bad && !gone);
-              if (lane == 0) bad_keys[slot][(warp - 10) + 2 * h] = bits;
             }
+            const uint32_t bits = __ballot_sync(0xffffffffu, bad && !gone);
+            if (lane == 0) bad_keys[slot][warp - 12] = bits;
             fence_proxy_async_smem();
             __syncwarp();
           }
@@ -491,12 +472,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + g * 128, o_at = tmem + lanes + 256 + g * D;
     uint8_t *const stage = stages + warp * kStageBytes;
-    uint32_t n0 = 0, s_phase = 0, o_phase[2] = {0, 0}, half_phase = 0;
+    uint32_t n0 = 0, s_phase = 0, o_steps = 0, half_phase = 0;  // s_phase: a bit for each buffer; o_steps: products so far
     bool ok = true;
     while (ok && next_item(kStatusAttnSoftmaxWait)) {
-      // An item of two tiles: each group has one. A narrow one: the groups take its blocks in turn, and group 0 joins the two.
+      // An item of two tiles: each group has one, half a block a step. A narrow one: each group has half of every block, and
+      // group 0 joins the two.
       const int rows = rows_of(item);
-      const bool narrow = rows <= 128, halves = narrow && item.blocks > 1;
+      const bool narrow = rows <= 128;
       const int row = (narrow ? 0 : g * 128) + r;
       const int index = item.tile * kTileRows + min(row, rows - 1), i = over_group(p.shape, index);
       const int hi = row < rows ? max(item.s.pos0 + i + 1, 0) : 0;
@@ -504,41 +486,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int part_hi = least_hi(item), part_lo = most_lo(item);
       const bool idle = row - lane >= rows;  // no row of this warp is one: its weights may be anything
       float m = -INFINITY, l = 0.f;
-      const int first = narrow ? g : 0, step = narrow ? 2 : 1;
-      for (int j = first; j < item.blocks; j += step) {
-        const uint32_t n = n0 + 2 * j;
-        const int key0 = (item.block + j) * kTileKeys;
-        ok = warp_wait(&s_full[g], s_phase, kStatusAttnSoftmaxWait);
+      const int steps = narrow ? item.blocks : 2 * item.blocks;
+      for (int step = 0; step < steps; ++step) {
+        const int buffer = step & 1, half = narrow ? g : buffer;
+        const uint32_t n = n0 + 2 * (narrow ? step : step >> 1);
+        const int block0 = (item.block + (narrow ? step : step >> 1)) * kTileKeys, key0 = block0 + 64 * half;
+        ok = warp_wait(&s_full[g][buffer], s_phase >> buffer & 1, kStatusAttnSoftmaxWait);
         if (!ok) break;
-        s_phase ^= 1;
+        s_phase ^= 1u << buffer;
         tc_fence_after();
         if (idle) {
-          if (lane == 0) mbar_arrive(&p_half[g]), mbar_arrive(&p_full[g]);
+          if (lane == 0) mbar_arrive(&p_full[g][buffer]);
           continue;
         }
-        float v[4][32];
-        tmem_ld32_async(s_at, v[0]);
-        tmem_ld32_async(s_at + 32, v[1]);
+        const uint32_t at = s_at + buffer * 64;
+        float v[2][32];
+        tmem_ld32_async(at, v[0]);
+        tmem_ld32_async(at + 32, v[1]);
         tmem_wait_ld();
-        tmem_ld32_async(s_at + 64, v[2]);
-        tmem_ld32_async(s_at + 96, v[3]);
         tmem_loaded(v[0]);
         tmem_loaded(v[1]);
-        tmem_wait_ld();
-        tmem_loaded(v[2]);
-        tmem_loaded(v[3]);
-        const bool edge = key0 + kTileKeys > part_hi || key0 < part_lo;
+        const bool edge = block0 + kTileKeys > part_hi || block0 < part_lo;
         float scale = p.scale;
         if constexpr (S8) {
           scale = 1.f;
           const float factor = row_factor[(k_item - 1) & 1][row];
           const float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][32 * c + e]);
-              const float4 l4 = *reinterpret_cast<const float4 *>(&sc[1][32 * c + e]);
+              float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][64 * half + 32 * c + e]);
+              const float4 l4 = *reinterpret_cast<const float4 *>(&sc[1][64 * half + 32 * c + e]);
               mul2(k4.x, k4.y, factor, factor);
               mul2(k4.z, k4.w, factor, factor);
               fma2(v[c][e], v[c][e + 1], k4.x, k4.y, l4.x, l4.y);
@@ -547,9 +526,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (edge) {
           // The columns that this row sees, a bit each: from lo - key0 up to hi - key0.
-          uint32_t sees[4];
+          uint32_t sees[2];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             const int to = min(max(hi - key0 - 32 * c, 0), 32), from = min(max(lo - key0 - 32 * c, 0), 32);
             sees[c] = (to == 32 ? ~0u : (1u << to) - 1) & ~(from == 32 ? ~0u : (1u << from) - 1);
           }
@@ -557,13 +536,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const int slot = static_cast<int>((n + 1) % NS);
             ok = warp_wait(&ready[slot], ((n + 1) / NS) & 1, kStatusAttnSoftmaxWait);
             if (!ok) break;
-            uint32_t bad = 0;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) bad |= bad_keys[slot][c] & sees[c];
+            const uint32_t bad = (bad_keys[slot][2 * half] & sees[0]) | (bad_keys[slot][2 * half + 1] & sees[1]);
             if (bad) l = NAN;  // (a row that sees a value that is no number ends as NaN)
           }
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(sees[c] >> e & 1)) v[c][e] = -INFINITY;
@@ -571,18 +548,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         float top[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          top[c] = fmaxf(v[c][0], v[c][1]);
+          const float *x = &v[c / 2][16 * (c & 1)];
+          top[c] = fmaxf(x[0], x[1]);
 #pragma unroll
-          for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], v[c][e], v[c][e + 1]);
+          for (int e = 2; e < 16; e += 2) top[c] = max3(top[c], x[e], x[e + 1]);
         }
-        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+        const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * scale;
         const bool grows = most > m + 8.f;
         if (__any_sync(0xffffffffu, grows)) {
           const float next = grows ? most : m;
           const float a = m == next ? 1.f : ex2(m - next);
           l *= a;
           m = next;
-          if (j != first) {
+          if (step > 0) {
+            // Behind the product of the step before. (That of the one before it was done when these scores came, so the parity
+            // is this one's.)
+            ok = warp_wait(&o_step[g], (o_steps + step - 1) & 1, kStatusAttnSoftmaxWait);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               float o[16];
@@ -597,7 +580,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float ref = m == -INFINITY ? 0.f : -m;
         float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
@@ -608,7 +591,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const float a = ex2(v[c][e]), b = ex2(v[c][e + 1]);
             w[e / 2] = pack16<BF>(a, b);
             if constexpr (S8) {
-              const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][32 * c + e]);
+              const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][64 * half + 32 * c + e]);
               if (edge)  // (a key that the row does not see may have any scale)
                 add2(sum[0], sum[1], a == 0.f ? 0.f : a * iv.x, b == 0.f ? 0.f : b * iv.y);
               else
@@ -619,40 +602,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               add2(sum[0], sum[1], a, b);
             }
           }
-          tmem_st16(s_at + 16 * c, w);
-          if (c & 1) {  // the first half's product starts while the second is made
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(c == 1 ? &p_half[g] : &p_full[g]);
-          }
+          tmem_st16(at + 16 * c, w);
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g][buffer]);
         l += sum[0] + sum[1];
       }
       if (!ok) break;
       n0 += 2 * item.blocks;
-      const uint32_t done[2] = {o_phase[0], o_phase[1]};
-      o_phase[0] ^= 1;
-      if (!narrow || halves) o_phase[1] ^= 1;
+      o_steps += steps;
       if (narrow && g == 1) {
-        if (halves) {
-          half_stats[r] = make_float2(m, l);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&half_done);
-          ok = warp_wait(&half_read, half_phase, kStatusAttnSoftmaxWait);  // then this accumulator is free again
-          half_phase ^= 1;
-        }
+        half_stats[r] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&half_done);
+        ok = warp_wait(&half_read, half_phase, kStatusAttnSoftmaxWait);  // then this accumulator is free again
+        half_phase ^= 1;
         continue;
       }
-      ok = warp_wait(&o_full[g], done[g], kStatusAttnSoftmaxWait);
-      if (ok && halves) {
-        ok = warp_wait(&o_full[1], done[1], kStatusAttnSoftmaxWait) && warp_wait(&half_done, half_phase, kStatusAttnSoftmaxWait);
+      const uint32_t done = (k_item - 1) & 1;
+      ok = warp_wait(&o_full[g], done, kStatusAttnSoftmaxWait);
+      if (ok && narrow) {
+        ok = warp_wait(&half_done, half_phase, kStatusAttnSoftmaxWait) && warp_wait(&o_full[1], done, kStatusAttnSoftmaxWait);
         half_phase ^= 1;
       }
       if (!ok) break;
       tc_fence_after();
       float a0 = 1.f, a1 = 0.f;
-      if (halves) {
+      if (narrow) {
         const float2 other = half_stats[r];
         const float most = fmaxf(m, other.x);
         a0 = m == most ? 1.f : ex2(m - most), a1 = other.x == most ? 1.f : ex2(other.x - most);
@@ -685,7 +663,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tmem_ld16(o_at + col, o);
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] *= a0;
-          if (halves) {
+          if (narrow) {
             float x[16];
             tmem_ld16(o_at + D + col, x);
 #pragma unroll
@@ -713,7 +691,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
       }
       tc_fence_before();
-      if (halves) {
+      if (narrow) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&half_read);
       }
