@@ -27,9 +27,15 @@ constexpr int kTileRegs = 128, kSoftmaxRegs = 152, kOtherRegs = 104;
 static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kTileThreads * kTileRegs, "more registers than the block was launched with");
 constexpr int kStageBytes = 2048;  // per softmax warp: 64 bytes of each of its rows on their way out
 
+// An int8 cache's kinds here. Exact: the integers are the operands, the keys' and values' scales meet the scores and weights
+// (attn.cu). Folded, for bf16 rows: the operands are fp16, integer * scale / (the largest scale of 32 keys), rounded (2^-11 twice, a
+// quarter of what bf16 rounds), so the softmax has one factor for 32 scores and one for their weights where the exact one reads
+// three numbers per key and row from shared memory (2048 of 30000 tokens: 1140 us instead of 1440). A block that some row sees
+// only in part is exact there too: a scale that a row does not see does not touch what it sees.
+constexpr int kFolded = 16;
 template <int D, int KIND>
 struct Tile {
-  static constexpr bool kS8 = KIND == MQ_S8;
+  static constexpr bool kFold = KIND == kFolded, kS8 = KIND == MQ_S8 || kFold;
   static constexpr int kBlock = kTileKeys * D * 2;          // of keys or values, as operands
   static constexpr int kSlots = kS8 ? 3 : 4;                // keys and values in turn
   static constexpr int kRaw = kS8 ? kTileKeys * D : 0;      // int8 as it was copied, two of them
@@ -109,12 +115,12 @@ template <int D, int KIND>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attn_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
   using T = Tile<D, KIND>;
-  constexpr bool BF = KIND == MQ_BF16, S8 = T::kS8;
+  constexpr bool BF = KIND == MQ_BF16, S8 = T::kS8, Fold = T::kFold, Exact = S8 && !Fold;  // (both int8 kinds multiply fp16)
   constexpr int NS = T::kSlots, NF = S8 ? 2 : NS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock, *stages = raw + 2 * T::kRaw;
-  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained[2], s_full[2][2], p_full[2][2], o_step[2], o_full[2], half_done, half_read;
+  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained[2], s_full[2][2], p_full[2][2], o_step[2], o_full[2], half_done, half_read, turn[2][4];
   __shared__ uint32_t bad_keys[NS][4];
   __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
   __shared__ ItemRing items;
@@ -140,6 +146,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     mbar_init(&drained[0], 1);
     mbar_init(&drained[1], 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&turn[i / 4][i % 4], 1);
     mbar_init(&half_done, 4);
     mbar_init(&half_read, 4);
     items.init(2 + kAuxWarps + 8);
@@ -244,7 +251,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   } else if (warp == 9 || warp == 10) {
     {
       // A thread for each accumulator: what it waits for and what it commits takes as long as its MMAs, so one thread for both
-      // left the tensor core idle half of the time (8192 tokens: MMA MMA_TIME).
+      // left the tensor core idle half of the time.
       constexpr uint32_t qk = idesc_16(128, 64, BF, false), pv = idesc_16(128, D, BF, true);
       const int g = warp - 9;
       // Keys and values take the ring's slots in turn: where the next scores' keys are, and the next product's values.
@@ -412,6 +419,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             sv = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
           }
         }
+        float most_k = fabsf(sk) < INFINITY ? sk : 0.f, most_v = fabsf(sv) < INFINITY ? sv : 0.f;  // of the warp's 32 keys
+        const bool edge = key0 + kTileKeys > part_hi || key0 < part_lo, exact = Exact || (Fold && edge);
+        if (Fold && !edge) {
+#pragma unroll
+          for (int o = 16; o; o >>= 1) {
+            most_k = fmaxf(most_k, __shfl_xor_sync(0xffffffffu, most_k, o));
+            most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, o));
+          }
+          if (!(most_k > 0.f)) most_k = 1.f;
+          most_v = fmaxf(most_v, kLeastScale);
+        }
         for (int which = 0; which < 2; ++which, ++n) {
           const int src = static_cast<int>(n % NF), slot = static_cast<int>(n % NS);
           ok = warp_wait(&full[src], (n / NF) & 1, kStatusAttnLoadWait);
@@ -420,6 +438,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           uint8_t *dst = ring + slot * T::kBlock;
           if constexpr (S8) {
             const uint8_t *from = raw + src * T::kRaw;
+            __half2 f2 = __float2half2_rn(1.f);
+            if (which == 0) {
+              // (the softmax has read block n / 2 - 2's by now: the slot just waited for came behind its weights)
+              float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
+              if (exact) {
+                const float vs = sv < kLeastScale ? kLeastScale : sv;
+                sc[0][r] = sk, sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
+              } else if (lane == 0) {  // one for the warp's 32 keys
+                sc[0][warp - 12] = most_k, sc[1][warp - 12] = lg2(most_v), sc[2][warp - 12] = __frcp_rn(most_v);
+              }
+            }
+            if (!exact) f2 = __float2half2_rn(which == 0 ? sk / most_k : (sv < kLeastScale ? kLeastScale : sv) / most_v);
             uint4 w[D / 16];
 #pragma unroll
             for (int c = 0; c < D / 16; ++c)
@@ -430,19 +460,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               uint32_t o[8];
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[2 * e] = bytes_to_half2<0x4140>(x[e]), o[2 * e + 1] = bytes_to_half2<0x4342>(x[e]);
+              if (!exact)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&o[e]), f2);
+                  o[e] = *reinterpret_cast<const uint32_t *>(&h);
+                }
               *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
               *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
-            }
-            if (which == 0) {
-              // (the softmax has read block n / 2 - 2's by now: the slot just waited for came behind its weights)
-              const float vs = sv < kLeastScale ? kLeastScale : sv;
-              float (&sc)[3][S8 ? kTileKeys : 1] = scales[(n >> 1) & 1];
-              sc[0][r] = sk, sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&raw_empty[src]);
-          } else if (which == 1 && (key0 + kTileKeys > part_hi || key0 < part_lo)) {
+          } else if (which == 1 && edge) {
             bool bad = false;
             const bool gone = key >= item.s.length;  // what lies there was never copied, or is another's
 #pragma unroll 4
@@ -472,7 +502,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + g * 128, o_at = tmem + lanes + 256 + g * D;
     uint8_t *const stage = stages + warp * kStageBytes;
-    uint32_t n0 = 0, s_phase = 0, o_steps = 0, half_phase = 0;  // s_phase: a bit for each buffer; o_steps: products so far
+    uint32_t n0 = 0, s_phase = 0, o_steps = 0, half_phase = 0, turn_phase = g ^ 1;  // s_phase: a bit for each buffer; o_steps: products so far
     bool ok = true;
     while (ok && next_item(kStatusAttnSoftmaxWait)) {
       // An item of two tiles: each group has one, half a block a step. A narrow one: each group has half of every block, and
@@ -496,7 +526,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         s_phase ^= 1u << buffer;
         tc_fence_after();
         if (idle) {
-          if (lane == 0) mbar_arrive(&p_full[g][buffer]);
+          ok = warp_wait(&turn[g][warp & 3], turn_phase, kStatusAttnSoftmaxWait);
+          if (!ok) break;
+          turn_phase ^= 1;
+          if (lane == 0) mbar_arrive(&turn[g ^ 1][warp & 3]), mbar_arrive(&p_full[g][buffer]);
           continue;
         }
         const uint32_t at = s_at + buffer * 64;
@@ -507,22 +540,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_loaded(v[0]);
         tmem_loaded(v[1]);
         const bool edge = block0 + kTileKeys > part_hi || block0 < part_lo;
-        float scale = p.scale;
+        // A score's log2 is scale * s + shift, for each 32 keys: the scale is the row's and, folded, the keys'; the shift the
+        // values'. (Exact: both go into v.)
+        float scale[2] = {p.scale, p.scale}, shift[2] = {0.f, 0.f};
         if constexpr (S8) {
-          scale = 1.f;
           const float factor = row_factor[(k_item - 1) & 1][row];
           const float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
+          if (Exact || edge) {
+            scale[0] = scale[1] = 1.f;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][64 * half + 32 * c + e]);
-              const float4 l4 = *reinterpret_cast<const float4 *>(&sc[1][64 * half + 32 * c + e]);
-              mul2(k4.x, k4.y, factor, factor);
-              mul2(k4.z, k4.w, factor, factor);
-              fma2(v[c][e], v[c][e + 1], k4.x, k4.y, l4.x, l4.y);
-              fma2(v[c][e + 2], v[c][e + 3], k4.z, k4.w, l4.z, l4.w);
-            }
+              for (int e = 0; e < 32; e += 4) {
+                float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][64 * half + 32 * c + e]);
+                const float4 l4 = *reinterpret_cast<const float4 *>(&sc[1][64 * half + 32 * c + e]);
+                mul2(k4.x, k4.y, factor, factor);
+                mul2(k4.z, k4.w, factor, factor);
+                fma2(v[c][e], v[c][e + 1], k4.x, k4.y, l4.x, l4.y);
+                fma2(v[c][e + 2], v[c][e + 3], k4.z, k4.w, l4.z, l4.w);
+              }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) scale[c] = factor * sc[0][2 * half + c], shift[c] = sc[1][2 * half + c];
+          }
         }
         if (edge) {
           // The columns that this row sees, a bit each: from lo - key0 up to hi - key0.
@@ -553,7 +593,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int e = 2; e < 16; e += 2) top[c] = max3(top[c], x[e], x[e + 1]);
         }
-        const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * scale;
+        const float most = Fold ? fmaxf(fmaf(fmaxf(top[0], top[1]), scale[0], shift[0]), fmaf(fmaxf(top[2], top[3]), scale[1], shift[1]))
+                                : max3(fmaxf(top[0], top[1]), top[2], top[3]) * scale[0];
         const bool grows = most > m + 8.f;
         if (__any_sync(0xffffffffu, grows)) {
           const float next = grows ? most : m;
@@ -578,31 +619,54 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.f : -m;
+        // The exponentials of the two warps that share a scheduler take turns, half a step apart: side by side they would also
+        // wait for their scores side by side (8192 tokens: 541 us without turns, 548 with whole ones, 536 with halves).
+        ok = warp_wait(&turn[g][warp & 3], turn_phase, kStatusAttnSoftmaxWait);
+        if (!ok) break;
+        turn_phase ^= 1;
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
+          auto weigh = [&](auto exactly) {
+            constexpr bool kExactly = decltype(exactly)::value;
+            const float from = ref + shift[c];
+            float part[2] = {0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            if (S8)
-              add2(v[c][e], v[c][e + 1], ref, ref);
-            else
-              fma2(v[c][e], v[c][e + 1], scale, scale, ref, ref);
-            const float a = ex2(v[c][e]), b = ex2(v[c][e + 1]);
-            w[e / 2] = pack16<BF>(a, b);
-            if constexpr (S8) {
-              const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][64 * half + 32 * c + e]);
-              if (edge)  // (a key that the row does not see may have any scale)
-                add2(sum[0], sum[1], a == 0.f ? 0.f : a * iv.x, b == 0.f ? 0.f : b * iv.y);
+            for (int e = 0; e < 32; e += 2) {
+              if (kExactly)
+                add2(v[c][e], v[c][e + 1], ref, ref);
               else
-                sum[0] = fmaf(a, iv.x, sum[0]), sum[1] = fmaf(b, iv.y, sum[1]);
-            } else if (BF) {  // as they were rounded: the roundings cancel where one key has most of the weight
-              add2(sum[0], sum[1], __uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xffff0000u));
-            } else {
-              add2(sum[0], sum[1], a, b);
+                fma2(v[c][e], v[c][e + 1], scale[c], scale[c], from, from);
+              const float a = ex2(v[c][e]), b = ex2(v[c][e + 1]);
+              w[e / 2] = pack16<BF>(a, b);
+              if constexpr (kExactly) {
+                const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][64 * half + 32 * c + e]);
+                if (Fold || edge)  // (a key that the row does not see may have any scale)
+                  add2(part[0], part[1], a == 0.f ? 0.f : a * iv.x, b == 0.f ? 0.f : b * iv.y);
+                else
+                  part[0] = fmaf(a, iv.x, part[0]), part[1] = fmaf(b, iv.y, part[1]);
+              } else if (BF) {  // as they were rounded: the roundings cancel where one key has most of the weight
+                add2(part[0], part[1], __uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xffff0000u));
+              } else {
+                add2(part[0], part[1], a, b);
+              }
             }
+            if (S8 && !kExactly) part[0] *= scales[(n >> 1) & 1][2][2 * half + c], part[1] *= scales[(n >> 1) & 1][2][2 * half + c];
+            sum[0] += part[0], sum[1] += part[1];
+          };
+          if constexpr (Exact) {
+            weigh(std::true_type());
+          } else if constexpr (Fold) {
+            if (edge)
+              weigh(std::true_type());
+            else
+              weigh(std::false_type());
+          } else {
+            weigh(std::false_type());
           }
           tmem_st16(at + 16 * c, w);
+          if (c == 0 && lane == 0) mbar_arrive(&turn[g ^ 1][warp & 3]);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -709,10 +773,10 @@ template <int D, int KIND>
 int launch_tile(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, cudaStream_t stream, const char *what) {
   using T = Tile<D, KIND>;
   CUtensorMap kmap, vmap;
-  const int box_rows = std::min(kTileKeys, c->page), box = KIND == MQ_S8 ? D : 128;
+  const int box_rows = std::min(kTileKeys, c->page), box = T::kS8 ? D : 128;
   const CUtensorMapSwizzle swizzle = box == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-  if (int rc = encode_pages(&kmap, c->k, KIND, c, c->k_stride, box, box_rows, swizzle, what)) return rc;
-  if (int rc = encode_pages(&vmap, c->v, KIND, c, c->v_stride, box, box_rows, swizzle, what)) return rc;
+  if (int rc = encode_pages(&kmap, c->k, c->dtype, c, c->k_stride, box, box_rows, swizzle, what)) return rc;
+  if (int rc = encode_pages(&vmap, c->v, c->dtype, c, c->v_stride, box, box_rows, swizzle, what)) return rc;
   p.parts = parts_at(workspace, ctas, kTileRows);
   static size_t configured[64] = {};
   auto kern = attn_tile_kernel<D, KIND>;
@@ -764,6 +828,7 @@ int launch_attention(const Plan &plan, const mq_kv_pages *c, AttnParams p, void 
   }
   if (plan.tile_ctas) {
     p.shape.rows_from = plan.few_ctas ? kRowsForTiles : 0, p.shape.rows_to = plan.most_rows;
+    if (KIND == MQ_S8 && p.q_dtype == MQ_BF16) return launch_tile<D, KIND == MQ_S8 ? kFolded : KIND>(c, p, plan.tile_ctas, workspace, s, what);
     return launch_tile<D, KIND>(c, p, plan.tile_ctas, workspace, s, what);
   }
   return MQ_OK;
