@@ -8,12 +8,14 @@
 // Both are a copy: what bounds them is the bandwidth, or for a few tokens the launch and the chain of loads that finds a
 // token's page. A CTA takes a few tokens: their sequences are looked up once, then its threads
 // move 8 values each, 8 or 16 lanes to a row, a row's maximum being a shuffle over them.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace mq {
 namespace paged {
 
-constexpr int kCopyThreads = 256, kMostTokens = 32;
+constexpr int kCopyThreads = 256, kMostTokens = 64, kAhead = 4;
 
 struct CopyParams {
   Seqs seqs;
@@ -25,27 +27,38 @@ struct CopyParams {
   int heads, dim, tokens_per_cta;
 };
 
-// Eight values of a row.
+// Eight values of a row, as they come.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-  constexpr int N = sizeof(T) * 8 / 16 > 0 ? sizeof(T) * 8 / 16 : 1;
-  if constexpr (sizeof(T) == 1) {
-    const uint2 w = *reinterpret_cast<const uint2 *>(p);
-    const uint32_t x[2] = {w.x, w.y};
+struct Eight {
+  static constexpr int kWords = sizeof(T) * 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (sizeof(T) == 1) {
+      const uint2 a = *reinterpret_cast<const uint2 *>(p);
+      w[0] = a.x, w[1] = a.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(static_cast<int8_t>(x[i / 4] >> (8 * (i % 4))));
-  } else {
-    struct alignas(16) Vec {
-      T t[16 / sizeof(T)];
-    };
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const Vec x = reinterpret_cast<const Vec *>(p)[u];
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) v[u * (16 / sizeof(T)) + i] = static_cast<float>(x.t[i]);
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 a = reinterpret_cast<const uint4 *>(p)[i / 4];
+        w[i] = a.x, w[i + 1] = a.y, w[i + 2] = a.z, w[i + 3] = a.w;
+      }
     }
   }
-}
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 1) {
+      // A biased byte beside 0x4b0000 is 2^23 + it.
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t b = w[i / 4] ^ 0x80808080u;
+        v[i] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7650 + i % 4)) - 8388736.f;
+      }
+    } else {
+      const T *t = reinterpret_cast<const T *>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(t[i]);
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
   struct alignas(16) Vec {
@@ -63,7 +76,8 @@ __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
 // STORE: rows of type X into pages of type C; else the other way.
 template <bool STORE, typename C, typename X, int LANES>
 __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_constant__ CopyParams p) {
-  __shared__ int page[kMostTokens], row[kMostTokens];  // page -1: nothing to do; -2: reads as zeros
+  __shared__ int page[kMostTokens];         // -1: nothing to do; -2: reads as zeros
+  __shared__ int64_t at[kMostTokens][4];    // where the token's rows begin in the pages of keys and values, and the scales'
   griddep_launch_dependents();
   griddep_wait();
   const int token0 = blockIdx.x * p.tokens_per_cta, tokens = min(p.tokens_per_cta, p.seqs.tokens - token0);
@@ -94,81 +108,105 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
       } else if (position >= 0 && position < s.length) {
         const int id = page_of(p.seqs, b, position);
         page[threadIdx.x] = id >= 0 ? id : STORE ? -1 : -2;
-        row[threadIdx.x] = position & ((1 << p.seqs.page_log2) - 1);
+        const int row = position & ((1 << p.seqs.page_log2) - 1);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          at[threadIdx.x][w] = id * p.stride[w][0] + row * p.stride[w][2];
+          at[threadIdx.x][2 + w] = id * p.scale_stride[w][0] + row * p.scale_stride[w][2];
+        }
       } else if (!STORE) {
         page[threadIdx.x] = -2;
       }
     }
   }
   __syncthreads();
-  const int lane = threadIdx.x % LANES, per_token = 2 * p.heads;
+  // A thread has one piece of a token's rows, the same for each of its tokens, so that a token costs it one addition per
+  // address; kAhead of them are fetched before the first is written.
+  const int pieces = 2 * p.heads * LANES, side = pieces < kCopyThreads ? kCopyThreads / pieces : 1;  // side: tokens side by side
+  const int mine = side > 1 ? threadIdx.x / pieces : 0, lane = threadIdx.x % LANES;
+  if (mine >= side) return;
   const bool in = lane * 8 < p.dim;
-  for (int base = threadIdx.x / LANES; base < tokens * per_token; base += kCopyThreads / LANES) {
-    const int i = base / per_token, rest = base - i * per_token, which = rest >= p.heads, head = rest - which * p.heads;
-    const int id = page[i];
-    if (id == -1) continue;  // (a row's lanes go together)
-    X *const x = static_cast<X *>(p.rows[which]) + (token0 + i) * p.token_stride[which] + head * p.head_stride[which] + lane * 8;
-    const int64_t *const st = p.stride[which], *const ss = p.scale_stride[which];
-    C *const c = static_cast<C *>(p.pages[which]) + id * st[0] + head * st[1] + row[i] * st[2] + lane * 8;
-    float v[8];
-    if constexpr (STORE) {
+  for (int piece = side > 1 ? threadIdx.x - mine * pieces : threadIdx.x; piece < pieces; piece += kCopyThreads) {
+    const int r = piece / LANES, which = r >= p.heads, head = r - which * p.heads;
+    const int64_t xs = p.token_stride[which];
+    X *const x = static_cast<X *>(p.rows[which]) + token0 * xs + head * p.head_stride[which] + lane * 8;
+    C *const c = static_cast<C *>(p.pages[which]) + head * p.stride[which][1] + lane * 8;
+    float *const s = sizeof(C) == 1 ? p.scales[which] + head * p.scale_stride[which][1] : nullptr;
+    for (int base = mine; base < tokens; base += side * kAhead) {
+      Eight<typename std::conditional<STORE, X, C>::type> raw[kAhead];
+      float scale[kAhead];
+      int id[kAhead];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (in) load8(x, v);
-      if constexpr (sizeof(C) == 1) {
-        float a = 0.f;
-        bool bad = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e])), bad |= !(fabsf(v[e]) < INFINITY);
-        const unsigned mine = LANES == 32 ? ~0u : ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
-#pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mine, a, o));
-        bad = __ballot_sync(mine, bad) != 0;
-        if (lane == 0) p.scales[which][id * ss[0] + head * ss[1] + row[i] * ss[2]] = bad ? NAN : a / 127.f;
-        // A maximum below 1e-30 is lifted by 2^80 (exact) first, so 127 / a stays finite.
-        const float lift = a < 1e-30f ? 0x1p80f : 1.f;
-        const float f = bad || a == 0.f ? 0.f : 127.f / (a * lift);
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int n = bad ? 0 : __float2int_rn((v[e] * lift) * f);
-          w[e / 4] |= (static_cast<uint32_t>(n) & 0xff) << (8 * (e % 4));
-        }
-        if (in) *reinterpret_cast<uint2 *>(c) = make_uint2(w[0], w[1]);
-      } else {
-        if (in) store8(c, v);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (in && id >= 0) {
-        load8(c, v);
-        if constexpr (sizeof(C) == 1) {
-          const float s = p.scales[which][id * ss[0] + head * ss[1] + row[i] * ss[2]];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= s;
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = base + u * side;
+        id[u] = i < tokens ? page[i] : -1;
+        if (STORE ? id[u] == -1 : id[u] < 0) continue;
+        if constexpr (STORE) {
+          if (in) raw[u].load(x + i * xs);
+        } else {
+          if (in) raw[u].load(c + at[i][which]);
+          if (sizeof(C) == 1) scale[u] = s[at[i][2 + which]];
         }
       }
-      if (in) store8(x, v);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (id[u] == -1) continue;  // (a row's lanes go together)
+        const int i = base + u * side;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        if (in && (STORE || id[u] >= 0)) raw[u].get(v);
+        if constexpr (!STORE) {
+          if (sizeof(C) == 1 && id[u] >= 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= scale[u];
+          }
+          if (in) store8(x + i * xs, v);
+        } else if constexpr (sizeof(C) == 1) {
+          float a = 0.f;
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e])), bad |= !(fabsf(v[e]) < INFINITY);
+          const unsigned lanes = ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
+#pragma unroll
+          for (int o = LANES / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(lanes, a, o));
+          bad = __ballot_sync(lanes, bad) != 0;
+          if (lane == 0) s[at[i][2 + which]] = bad ? NAN : a / 127.f;
+          // A maximum below 1e-30 is lifted by 2^80 (exact) first, so 127 / a stays finite.
+          const float lift = a < 1e-30f ? 0x1p80f : 1.f;
+          const float f = bad || a == 0.f ? 0.f : 127.f / (a * lift);
+          uint32_t w[2] = {0, 0};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int n = bad ? 0 : __float2int_rn((v[e] * lift) * f);
+            w[e / 4] |= (static_cast<uint32_t>(n) & 0xff) << (8 * (e % 4));
+          }
+          if (in) *reinterpret_cast<uint2 *>(c + at[i][which]) = make_uint2(w[0], w[1]);
+        } else {
+          if (in) store8(c + at[i][which], v);
+        }
+      }
     }
   }
 }
 
 template <bool STORE, typename C, typename X>
-int launch_copy(CopyParams &p, cudaStream_t s, const char *what) {
+int launch_copy(CopyParams &p, int sms, cudaStream_t s, const char *what) {
   const int lanes = p.dim <= 64 ? 8 : 16;
-  // Four rows a thread: enough loads on their way where there are many tokens.
+  // A token's place takes a chain of loads, so a CTA looks up many at once, as long as there are CTAs for every SM: four or so
+  // of 16-byte pieces a thread for few tokens.
   const int64_t threads = 2LL * p.heads * lanes;  // of a token
-  p.tokens_per_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostTokens, 4 * kCopyThreads / threads)));
+  const int64_t least = std::max<int64_t>(1, 4 * kCopyThreads / threads), fill = p.seqs.tokens / (16LL * sms);
+  p.tokens_per_cta = static_cast<int>(std::min<int64_t>(kMostTokens, std::max(least, fill)));
   const dim3 grid((p.seqs.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta);
   if (lanes == 8) return launch_overlapped(kv_copy_kernel<STORE, C, X, 8>, grid, dim3(kCopyThreads), 0, s, what, p);
   return launch_overlapped(kv_copy_kernel<STORE, C, X, 16>, grid, dim3(kCopyThreads), 0, s, what, p);
 }
 template <bool STORE, typename C>
-int copy_by_rows(CopyParams &p, int dtype, cudaStream_t s, const char *what) {
-  if (dtype == MQ_F32) return launch_copy<STORE, C, float>(p, s, what);
-  if (dtype == MQ_F16) return launch_copy<STORE, C, __half>(p, s, what);
-  return launch_copy<STORE, C, __nv_bfloat16>(p, s, what);
+int copy_by_rows(CopyParams &p, int dtype, int sms, cudaStream_t s, const char *what) {
+  if (dtype == MQ_F32) return launch_copy<STORE, C, float>(p, sms, s, what);
+  if (dtype == MQ_F16) return launch_copy<STORE, C, __half>(p, sms, s, what);
+  return launch_copy<STORE, C, __nv_bfloat16>(p, sms, s, what);
 }
 
 template <bool STORE>
@@ -199,9 +237,9 @@ int kv_copy(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_token, 
   p.token_stride[0] = k_token, p.token_stride[1] = v_token, p.head_stride[0] = k_head, p.head_stride[1] = v_head;
   p.heads = c->heads, p.dim = c->dim;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (c->dtype == MQ_S8) return copy_by_rows<STORE, int8_t>(p, dtype, s, what);
-  if (c->dtype == MQ_F16) return copy_by_rows<STORE, __half>(p, dtype, s, what);
-  return copy_by_rows<STORE, __nv_bfloat16>(p, dtype, s, what);
+  if (c->dtype == MQ_S8) return copy_by_rows<STORE, int8_t>(p, dtype, dev.sms, s, what);
+  if (c->dtype == MQ_F16) return copy_by_rows<STORE, __half>(p, dtype, dev.sms, s, what);
+  return copy_by_rows<STORE, __nv_bfloat16>(p, dtype, dev.sms, s, what);
 }
 
 }  // namespace paged

@@ -16,13 +16,18 @@
 // y = n / 32 + r, |r| <= 1/64, is 2^(n / 32) from a table of 32 times a Taylor polynomial of degree 5 (2e-15), nine
 // fp64 instructions. Each warp has a stretch of the row of its own; only the warp whose stretch holds the drawn
 // token looks for it, in order.
+#include <algorithm>
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mq {
 namespace verify {
 
 constexpr int kScan = 256, kVecs = 4;        // threads of a scan CTA, 16-byte vectors per thread and step
-constexpr int kDraw = 512, kCluster = 8;     // threads of a drawing CTA, CTAs of a request
+constexpr int kCluster = 8;                  // drawing CTAs of a request
+// Their threads: many for the latency of a few requests, fewer where that lets all CTAs run at once (four on an SM).
+constexpr int kDrawFew = 512, kDrawMany = 256, kManyRequests = 148 * 2 / kCluster;
 constexpr int kMaxDrafts = 32, kMaxSplits = 64;
 constexpr float kLeastTemperature = 1e-5f;   // below: 0
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
@@ -168,10 +173,9 @@ __global__ void __launch_bounds__(kScan) verify_scan_kernel(const Params p) {
   }
 }
 
-__device__ __forceinline__ float read(const Params &p, const char *row, int v) {
-  if (p.dtype == MQ_F32) return reinterpret_cast<const float *>(row)[v];
-  if (p.dtype == MQ_F16) return __half2float(reinterpret_cast<const __half *>(row)[v]);
-  return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(row)[v]);
+template <typename T>
+__device__ __forceinline__ float read(const char *row, int v) {
+  return static_cast<float>(reinterpret_cast<const T *>(row)[v]);
 }
 
 // 2^((x - top) k / 32) in fp64, relative error below 1e-14 (k: 32 log2(e) / T). The sum with 1.5 * 2^52 rounds to an integer.
@@ -188,8 +192,7 @@ struct Exp {
     table = t;
   }
   __device__ __forceinline__ double operator()(float x) const {
-    if (!(x >= least)) return 0.0;
-    const double y = x, t = fma(y, k, magic), n = t - magic, r = fma(y, k, -n);
+    const double y = fmaxf(x, least), t = fma(y, k, magic), n = t - magic, r = fma(y, k, -n);
     constexpr double a = kLn2 / 32;
     double e = fma(r, a * a * a * a * a / 120, a * a * a * a / 24);
     e = fma(e, r, a * a * a / 6);
@@ -198,7 +201,8 @@ struct Exp {
     e = fma(e, r, 1.0);
     const int low = __double2loint(t);
     const double z = table[low & 31];
-    return e * __hiloint2double(__double2hiint(z) + ((low >> 5) << 20), __double2loint(z));
+    e *= __hiloint2double(__double2hiint(z) + ((low >> 5) << 20), __double2loint(z));
+    return x >= least ? e : 0.0;  // (no branch: several are computed side by side)
   }
 };
 
@@ -217,11 +221,12 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
-  constexpr int kWarps = kDraw / 32;
+template <typename T, int kDraw>
+__global__ void __launch_bounds__(kDraw, 1024 / kDraw) verify_draw_kernel(const Params p) {
+  constexpr int kWarps = kDraw / 32, stretch = kCluster * kWarps, kPer = stretch / 32;  // stretches of a row; of a lane
   __shared__ double table[32];
   __shared__ float top[2 * kMaxDrafts + 1], total[2 * kMaxDrafts + 1];  // of the request's rows; T = 0: total holds the index
-  __shared__ int kept_s, bad_s;
+  __shared__ int kept_s, bad_s, last_s;
   __shared__ double warp_sums[3][kWarps];    // p, q; then the weights
   __shared__ double all_sums[3][kCluster][kWarps];
   griddep_launch_dependents();
@@ -277,9 +282,9 @@ __global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
       } else if (p.draft && !good(j)) {
         status = kStatusVerifyBadRow;
       } else {
-        const double z = (static_cast<double>(read(p, row_at(p, b, lane), d)) - top[lane]) / hot;
+        const double z = (static_cast<double>(read<T>(row_at(p, b, lane), d)) - top[lane]) / hot;
         const double pd = exp(z) / total[lane];
-        const double qd = p.draft ? exp((static_cast<double>(read(p, row_at(p, b, j), d)) - top[j]) / hot) / total[j] : 1.0;
+        const double qd = p.draft ? exp((static_cast<double>(read<T>(row_at(p, b, j), d)) - top[j]) / hot) / total[j] : 1.0;
         keep = p.uniform[at] * qd < pd;
         logprob = static_cast<float>(z - log(static_cast<double>(total[lane])));
       }
@@ -310,7 +315,7 @@ __global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
   if (bad || hot == 0.f) return;  // (the whole cluster)
 
   // The draw. This warp's stretch of the row:
-  const int stretch = kCluster * kWarps, mine = rank * kWarps + warp;
+  const int mine = rank * kWarps + warp;
   const int v0 = static_cast<int>(static_cast<int64_t>(p.vocab) * mine / stretch);
   const int v1 = static_cast<int>(static_cast<int64_t>(p.vocab) * (mine + 1) / stretch);
   const char *pr = row_at(p, b, kept);
@@ -337,27 +342,46 @@ __global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
     }
     __syncthreads();
     const double *all = &all_sums[which][0][0];
-    return warp_sum(all[lane] + all[lane + 32] + all[lane + 64] + all[lane + 96]);
+    double sum = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum += all[lane + 32 * e];
+    return warp_sum(sum);
+  };
+  // f(token, its logit in p, in q) of this warp's stretch, a lane every 32nd: kAhead of them are fetched before any is used.
+  constexpr int kAhead = 8;
+  auto sweep = [&](auto both, auto f) {
+    constexpr bool kBoth = decltype(both)::value;
+#pragma unroll 1
+    for (int base = v0 + lane; base < v1; base += 32 * kAhead) {
+      float x[kAhead], y[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int v = base + 32 * u;
+        x[u] = v < v1 ? read<T>(pr, v) : -INFINITY;
+        y[u] = kBoth && v < v1 ? read<T>(qr, v) : -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) f(base + 32 * u, x[u], y[u]);
+    }
   };
   double ip = 1, iq = 0;
   bool rest = two;
   if (two) {
     double sp = 0, sq = 0;
-#pragma unroll 4
-    for (int v = v0 + lane; v < v1; v += 32) sp += ep(read(p, pr, v)), sq += eq(read(p, qr, v));
+    sweep(std::true_type(), [&](int, float x, float y) { sp += ep(x), sq += eq(y); });
     ip = 1 / gather(0, sp);
     iq = 1 / gather(1, sq);
   }
-  auto weight = [&](int v) -> double {
-    if (v == without) return 0;
-    const double w = ep(read(p, pr, v)) * ip;
-    return rest ? fmax(w - eq(read(p, qr, v)) * iq, 0.0) : w;
-  };
   double whole = 0;
   for (int round = 0; round < 2; ++round) {
     double w = 0;
-#pragma unroll 4
-    for (int v = v0 + lane; v < v1; v += 32) w += weight(v);
+    if (rest)
+      sweep(std::true_type(), [&](int, float x, float y) {
+        const double left = fma(eq(y), -iq, ep(x) * ip);
+        w += left > 0 ? left : 0.0;
+      });
+    else
+      sweep(std::false_type(), [&](int v, float x, float) { w += v == without ? 0.0 : ep(x); });
     if (round) sync_cluster();  // (everybody has read the first round's sums)
     whole = gather(2, w);
     if (whole > 0 || !rest) break;
@@ -365,12 +389,13 @@ __global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
   }
   const double goal = p.uniform[out0 + p.drafts] * whole;
   // The first stretch whose running sum passes the goal, else the last that has any weight.
-  static_assert(kCluster * kWarps == 128, "a lane has four stretches");
   double before = 0;  // of lane's first stretch; then of the one that was found
   int found = -1;
   {
-    const double *all = &all_sums[2][0][0] + 4 * lane;
-    double incl = all[0] + all[1] + all[2] + all[3];
+    const double *all = &all_sums[2][0][0] + kPer * lane;
+    double incl = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) incl += all[e];
     const double own = incl;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -381,9 +406,9 @@ __global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
     int over = -1, last = -1;
     double over_at = 0, last_at = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kPer; ++e) {
       if (all[e] > 0) {
-        last = 4 * lane + e, last_at = run;
+        last = kPer * lane + e, last_at = run;
         if (over < 0 && run + all[e] > goal) over = last, over_at = run;
       }
       run += all[e];
@@ -393,40 +418,94 @@ __global__ void __launch_bounds__(kDraw, 2) verify_draw_kernel(const Params p) {
     found = __shfl_sync(0xffffffffu, overs ? over : last, from);
     before = __shfl_sync(0xffffffffu, overs ? over_at : last_at, from);
   }
-  if (found == mine) {
-    double run = before;
-    int token = -1, last = -1;
-    for (int base = v0; base < v1 && token < 0; base += 32) {
-      const int v = base + lane;
-      const double w = v < v1 ? weight(v) : 0.0;
-      double incl = w;
+  sync_cluster();  // (nobody reads another's sums from here on: who is done may leave)
+  if (found < 0) {  // no token has weight: the only one was drafted and is not kept
+    if (rank == 0 && tid == 0) p.tokens[out0 + kept] = -1, p.logprobs[out0 + kept] = 0.f;
+    return;
+  }
+  if (found / kWarps != static_cast<int>(rank)) return;
+  // The CTA whose stretch it is looks for the token: each warp takes a part, and has its weights in registers when it is known
+  // which part the goal lies in. (One warp alone took 50 us, 32 tokens after 32.)
+  const int f0 = static_cast<int>(static_cast<int64_t>(p.vocab) * found / stretch);
+  const int f1 = static_cast<int>(static_cast<int64_t>(p.vocab) * (found + 1) / stretch);
+  double run = before;
+  if (tid == 0) last_s = -1;  // the last token with any weight so far
+  for (int first = f0; first < f1; first += 32 * kAhead * kWarps) {  // (once, up to vocabularies of 131072)
+    const int part = (min(f1 - first, 32 * kAhead * kWarps) + kWarps - 1) / kWarps, g0 = first + warp * part, g1 = min(g0 + part, f1);
+    float x[kAhead], y[kAhead];
+    double w[kAhead], own = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
+    for (int u = 0; u < kAhead; ++u) {
+      const int v = g0 + 32 * u + lane;
+      x[u] = v < g1 ? read<T>(pr, v) : -INFINITY;
+      y[u] = rest && v < g1 ? read<T>(qr, v) : -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int v = g0 + 32 * u + lane;
+      const double e = v >= g1 || v == without ? 0.0 : ep(x[u]);
+      const double left = rest && v < g1 ? fma(eq(y[u]), -iq, e * ip) : e;
+      w[u] = left > 0 ? left : 0.0;
+      own += w[u];
+    }
+    own = warp_sum(own);
+    __syncthreads();
+    if (lane == 0) warp_sums[0][warp] = own;
+#pragma unroll
+    for (int u = kAhead - 1; u >= 0; --u) {
+      const unsigned any = __ballot_sync(0xffffffffu, w[u] > 0);
+      if (any) {
+        if (lane == 0) atomicMax(&last_s, g0 + 32 * u + 31 - __clz(any));
+        break;
       }
-      const unsigned over = __ballot_sync(0xffffffffu, w > 0 && run + incl > goal), any = __ballot_sync(0xffffffffu, w > 0);
-      if (over) token = base + __ffs(over) - 1;
-      if (any) last = base + 31 - __clz(any);
-      run += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (token < 0) token = last;  // (rounding)
-    if (lane == 0) {
-      p.tokens[out0 + kept] = token;
-      const double z = (static_cast<double>(read(p, pr, token)) - top[kept]) / hot;
-      p.logprobs[out0 + kept] = static_cast<float>(z - log(static_cast<double>(total[kept])));
+    __syncthreads();
+    double ahead = run, at_part = 0;
+    int holds = -1;  // the warp whose part holds the goal
+    for (int v = 0; v < kWarps; ++v) {
+      const double s = warp_sums[0][v];
+      if (s > 0 && holds < 0 && ahead + s > goal) holds = v, at_part = ahead;
+      ahead += s;
     }
+    const bool ends = first + 32 * kAhead * kWarps >= f1;
+    // (Rounding may leave the goal beyond the last weight, of the stretch or of the part.)
+    if (warp == (holds >= 0 ? holds : 0) && (holds >= 0 || ends)) {
+      double sum = at_part;
+      int token = holds < 0 ? last_s : -1, last = -1;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        double incl = w[u];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += up;
+        }
+        const unsigned over = __ballot_sync(0xffffffffu, w[u] > 0 && sum + incl > goal), any = __ballot_sync(0xffffffffu, w[u] > 0);
+        if (token < 0 && over) token = g0 + 32 * u + __ffs(over) - 1;
+        if (any) last = g0 + 32 * u + 31 - __clz(any);
+        sum += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (token < 0) token = last;
+      if (lane == 0) {
+        p.tokens[out0 + kept] = token;
+        const double z = (static_cast<double>(read<T>(pr, token)) - top[kept]) / hot;
+        p.logprobs[out0 + kept] = static_cast<float>(z - log(static_cast<double>(total[kept])));
+      }
+    }
+    if (holds >= 0) return;
+    run = ahead;
   }
-  if (found < 0 && mine == 0 && lane == 0) {  // (no token has weight: the only one was drafted and is not kept)
-    p.tokens[out0 + kept] = -1;
-    p.logprobs[out0 + kept] = 0.f;
-  }
-  sync_cluster();  // no CTA's sums go away while another reads them
 }
 
 template <typename T>
 int scan(const Params &p, int64_t ctas, cudaStream_t s, const char *what) {
   return launch_overlapped(verify_scan_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(kScan), 0, s, what, p);
+}
+
+template <typename T>
+int draw(const Params &p, dim3 grid, cudaStream_t s, const char *what) {
+  if (p.batch > kManyRequests) return launch_overlapped_clusters(verify_draw_kernel<T, kDrawMany>, grid, dim3(kDrawMany), kCluster, 0, s, what, p);
+  return launch_overlapped_clusters(verify_draw_kernel<T, kDrawFew>, grid, dim3(kDrawFew), kCluster, 0, s, what, p);
 }
 
 inline bool sizes_fit(int64_t batch, int64_t drafts, int64_t vocab) {
@@ -479,6 +558,8 @@ extern "C" int mq_verify_drafts(const void *target, int64_t ld_target, const voi
   else
     rc = scan<__nv_bfloat16>(p, rows * p.splits, s, what);
   if (rc) return rc;
-  return mq::launch_overlapped_clusters(verify_draw_kernel, dim3(static_cast<unsigned>(batch * kCluster)), dim3(kDraw), kCluster, 0, s,
-                                        what, p);
+  const dim3 draws(static_cast<unsigned>(batch * kCluster));
+  if (dtype == MQ_F32) return draw<float>(p, draws, s, what);
+  if (dtype == MQ_F16) return draw<__half>(p, draws, s, what);
+  return draw<__nv_bfloat16>(p, draws, s, what);
 }
