@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
     const int box_rows = min(kFewKeys, 1 << p.seqs.page_log2), per_block = kFewKeys / box_rows;
     const int boxes = per_block * F::kBoxes;  // of keys, and as many of values
     Walk<FewGrain> walk;
-    walk.start(p.seqs, p.shape, scratch.found);
-    if (lane == 0) p.parts.cuts[blockIdx.x] = cut_at(walk, p.shape, scratch.found);
+    walk.start(p.shape, scratch.found);
+    const Walk<FewGrain> begin = walk;
     int s = 0, round = 0, k = 0;
     uint32_t issued = 0;
     bool ok = true;
@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
         if (++s == S) s = 0, ++round;
       }
     }
+    if (lane == 0) p.parts.cuts[blockIdx.x] = cut_at(begin, p.shape, scratch.found);
     // Leave no copy in flight.
     if (lane == 0)
       for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i) wait_for(&full[i % S], (i / S) & 1);
@@ -607,9 +608,9 @@ struct JoinParams {
   Parts parts;
   int rows;  // of an item's parts
 };
-constexpr int kJoinRows = 8;
+constexpr int kJoinWarps = 8;
 template <int D, int TILE_ROWS>
-__global__ void __launch_bounds__(32 * kJoinRows) attn_join_kernel(const JoinParams p) {
+__global__ void __launch_bounds__(32 * kJoinWarps) attn_join_kernel(const JoinParams p) {
   griddep_wait();
   const int c = blockIdx.x, lane = threadIdx.x % 32;
   if (c == 0) return;
@@ -617,38 +618,38 @@ __global__ void __launch_bounds__(32 * kJoinRows) attn_join_kernel(const JoinPar
   const Cut cut = p.parts.cuts[c];  // (there is one, used or not)
   if (c >= ctas || !cut.goes_on || total * (c - 1) / ctas > cut.first) return;
   const int rows = min(TILE_ROWS, cut.n * p.shape.group - cut.tile * TILE_ROWS);
-  const int row = blockIdx.y * kJoinRows + threadIdx.x / 32;
-  if (row >= rows) return;
   // Part 0 is CTA c - 1's, which began the item (its slot 1), the others what CTAs c .. last went on with (slot 0); CTA `last`
   // is the last whose share begins before the item's end.
   const int last = static_cast<int>((cut.end * ctas + total - 1) / total) - 1, n = last - c + 2;
-  auto at = [&](int i) { return (2 * static_cast<int64_t>(c - 1 + i) + (i == 0 ? 1 : 0)) * p.rows + row; };
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, p.parts.stats[at(i)].x);
+  for (int row = blockIdx.y * kJoinWarps + threadIdx.x / 32; row < rows; row += gridDim.y * kJoinWarps) {
+    auto at = [&](int i) { return (2 * static_cast<int64_t>(c - 1 + i) + (i == 0 ? 1 : 0)) * p.rows + row; };
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.parts.stats[at(i)].x);
 #pragma unroll
-  for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  constexpr int kLanes = D / 4, kTurns = 32 / kLanes;  // lanes of a part, parts at a time
-  const int u = lane % kLanes;
-  float sum = 0.f;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    constexpr int kLanes = D / 4, kTurns = 32 / kLanes;  // lanes of a part, parts at a time
+    const int u = lane % kLanes;
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = lane / kLanes; i < n; i += kTurns) {
-    const int64_t a = at(i);
-    const float2 st = p.parts.stats[a];
-    const float4 x = *reinterpret_cast<const float4 *>(p.parts.sums + a * D + u * 4);
-    const float w = st.x == top ? 1.f : ex2(st.x - top);
-    sum += st.y * w;
-    v.x += x.x * w, v.y += x.y * w, v.z += x.z * w, v.w += x.w * w;
+    for (int i = lane / kLanes; i < n; i += kTurns) {
+      const int64_t a = at(i);
+      const float2 st = p.parts.stats[a];
+      const float4 x = *reinterpret_cast<const float4 *>(p.parts.sums + a * D + u * 4);
+      const float w = st.x == top ? 1.f : ex2(st.x - top);
+      sum += st.y * w;
+      v.x += x.x * w, v.y += x.y * w, v.z += x.z * w, v.w += x.w * w;
+    }
+    if (kTurns == 2) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, 16), v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+      v.z += __shfl_xor_sync(0xffffffffu, v.z, 16), v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+    }
+    const float inv = inverse_sum(sum);
+    const int r = cut.tile * TILE_ROWS + row, i = over_group(p.shape, r);
+    if (lane < kLanes && u * 4 < p.o.dim)
+      store_out4(p.o, cut.token + i, cut.head * p.shape.group + r - i * p.shape.group, u * 4, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
   }
-  if (kTurns == 2) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, 16), v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
-    v.z += __shfl_xor_sync(0xffffffffu, v.z, 16), v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
-  }
-  const float inv = inverse_sum(sum);
-  const int r = cut.tile * TILE_ROWS + row, i = over_group(p.shape, r);
-  if (lane < kLanes && u * 4 < p.o.dim)
-    store_out4(p.o, cut.token + i, cut.head * p.shape.group + r - i * p.shape.group, u * 4, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
 }
 
 // A map of a pool's rows: (dim, row of the page, head, page), boxes of `box_bytes` of `box_rows` rows.
@@ -680,7 +681,7 @@ int launch_few(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, cu
   if (int rc = ensure_smem(kern, F::kSmem, configured, what)) return rc;
   if (int rc = launch_overlapped(kern, dim3(ctas), dim3(kFewThreads), F::kSmem, stream, what, kmap, vmap, p)) return rc;
   JoinParams j{p.shape, p.o, p.parts, kFewRows};
-  return launch_overlapped(attn_join_kernel<D, kFewRows>, dim3(ctas, kFewRows / kJoinRows), dim3(32 * kJoinRows), 0, stream, what, j);
+  return launch_overlapped(attn_join_kernel<D, kFewRows>, dim3(ctas, kFewRows / kJoinWarps), dim3(32 * kJoinWarps), 0, stream, what, j);
 }
 
 }  // namespace paged

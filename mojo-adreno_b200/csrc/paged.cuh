@@ -195,7 +195,13 @@ struct Share {
   int64_t total, begin, end;  // units of the launch, and of this CTA
   int parts;                  // CTAs with a share
   int b, head, tile, rest;    // where it begins: `rest` units into that item
+  Seq s;                      // sequence b
 };
+// total * i / parts, without a 64-bit division where none is needed (they are a subroutine of a hundred instructions).
+__device__ __forceinline__ int64_t portion(int64_t total, int i, int parts) {
+  if (total < (1 << 21) && i <= 1023) return static_cast<uint32_t>(total) * static_cast<uint32_t>(i) / static_cast<uint32_t>(parts);
+  return total * i / parts;
+}
 template <int THREADS>
 struct ShareScratch {
   int64_t costs[THREADS];  // units of THREADS sequences
@@ -210,6 +216,7 @@ __device__ __forceinline__ void find_share(const Seqs &s, const Shape &a, ShareS
   constexpr bool kOneTile = G::ROWS <= 64;  // a sequence has one tile at most
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   int64_t total = 0;
+  Seq own{};  // the last sequence this thread (with one tile each) or its warp looked at
   // Twice through the sequences, THREADS at a time: for the total, and for the one in which the share begins. Once where
   // one step takes all.
   for (int pass = s.batch <= THREADS ? 1 : 0; pass < 2; ++pass) {
@@ -218,7 +225,7 @@ __device__ __forceinline__ void find_share(const Seqs &s, const Shape &a, ShareS
       int64_t cost = 0;
       if (kOneTile) {
         if (base + tid < s.batch) {
-          const Seq q = sequence(s, base + tid);
+          const Seq q = own = sequence(s, base + tid);
           if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
           if (takes_part(q, a)) cost = static_cast<int64_t>(G::EXTRA + tile_range<G>(q, a, 0).blocks) * a.kv_heads;
         }
@@ -256,18 +263,28 @@ __device__ __forceinline__ void find_share(const Seqs &s, const Shape &a, ShareS
         const int parts = static_cast<int>(total < gridDim.x ? total : gridDim.x);
         if (base == 0 && tid == 0) sm.found.total = total, sm.found.parts = parts;
         if (static_cast<int>(blockIdx.x) < parts) {
-          const int64_t begin = total * blockIdx.x / parts;
+          const int64_t begin = portion(total, blockIdx.x, parts);
           // The warp with the sequence in which the share begins finds the tile.
           const unsigned here = __ballot_sync(0xffffffffu, start <= begin && begin < start + cost);
           if (here) {
             const int from = __ffs(here) - 1, b = base + warp * 32 + from;
-            const int64_t per_head = __shfl_sync(0xffffffffu, cost, from) / a.kv_heads;
-            int64_t rest = begin - __shfl_sync(0xffffffffu, start, from);
-            const int head = static_cast<int>(rest / per_head);
+            const int64_t all = __shfl_sync(0xffffffffu, cost, from);
+            int64_t rest = begin - __shfl_sync(0xffffffffu, start, from), per_head;
+            int head;
+            if (all < (1LL << 31)) {
+              per_head = static_cast<uint32_t>(all) / static_cast<uint32_t>(a.kv_heads);
+              head = static_cast<uint32_t>(rest) / static_cast<uint32_t>(per_head);
+            } else {
+              per_head = all / a.kv_heads;
+              head = static_cast<int>(rest / per_head);
+            }
             rest -= head * per_head;
+            Seq q = own;
+            q.first = __shfl_sync(0xffffffffu, q.first, from), q.n = __shfl_sync(0xffffffffu, q.n, from);
+            q.length = __shfl_sync(0xffffffffu, q.length, from), q.pos0 = q.length - q.n;
             int tile = 0;
             if (!kOneTile) {
-              const Seq q = sequence(s, b);
+              q = sequence(s, b);
               for (const int tiles = tiles_of<G>(q, a);; tile += 32) {
                 const int t = tile + lane;
                 const int64_t units = t < tiles ? G::EXTRA + tile_range<G>(q, a, t).blocks : 0;
@@ -288,7 +305,8 @@ __device__ __forceinline__ void find_share(const Seqs &s, const Shape &a, ShareS
               }
             }
             if (lane == 0) {
-              sm.found.begin = begin, sm.found.end = total * (blockIdx.x + 1) / parts;
+              sm.found.begin = begin, sm.found.end = portion(total, blockIdx.x + 1, parts);
+              sm.found.s = q;
               sm.found.b = b, sm.found.head = head, sm.found.tile = tile, sm.found.rest = static_cast<int>(rest);
             }
           }
@@ -313,9 +331,9 @@ struct Walk {
   Seq s;
   int b, head, tile, tiles, rest;
   int64_t left;
-  __device__ __forceinline__ void start(const Seqs &q, const Shape &a, const Share &share) {
+  __device__ __forceinline__ void start(const Shape &a, const Share &share) {
     b = share.b, head = share.head, tile = share.tile, rest = share.rest, left = share.end - share.begin;
-    s = sequence(q, b);
+    s = share.s;
     tiles = tiles_of<G>(s, a);
   }
   __device__ __forceinline__ bool next(const Seqs &q, const Shape &a, Item &item) {
