@@ -29,9 +29,8 @@
 namespace mq {
 namespace paged {
 
-constexpr int kFewKeys = 64, kFewRows = 16;  // keys of a block; the most rows of an item
+constexpr int kFewRows = 16;  // the most rows of an item
 constexpr int kFewWarps = 4, kFewThreads = 32 * (kFewWarps + 1);
-using FewGrain = Grain<kFewRows, kFewKeys, 2>;
 constexpr int kPadCols = 72;                 // floats between rows of the joining buffer: no bank conflicts
 
 __device__ __forceinline__ float ex2(float x) {
@@ -124,13 +123,17 @@ __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 
 template <int D, int KIND>
 struct Few {
   static constexpr int kBytes = KIND == MQ_S8 ? 1 : 2;
+  // Keys of a block: 32 KB of keys and values either way at 128 dim (int8 64x1: 144 us with two CTAs and 128 keys, 148 with three
+  // and 64, 186 with two and 64).
+  static constexpr int kKeys = KIND == MQ_S8 ? 128 : 64;
+  using Units = Grain<kFewRows, kKeys, 2>;
   static constexpr int kBox = KIND == MQ_S8 ? 64 : 128;                 // bytes of a row in a box
   static constexpr int kBoxes = D * kBytes / kBox;
-  static constexpr int kTile = kFewKeys * D * kBytes;                   // of keys, or of values
-  static constexpr int kScales = KIND == MQ_S8 ? 3 * kFewKeys * 4 : 0;  // keys' scales, values': log2 and inverse
-  static constexpr int kStageBytes = 2 * kTile + 1024 * (kScales > 0);
+  static constexpr int kTile = kKeys * D * kBytes;                   // of keys, or of values
+  static constexpr int kScales = KIND == MQ_S8 ? 3 * kKeys * 4 : 0;  // keys' scales, values': log2 and inverse
+  static constexpr int kStageBytes = 2 * kTile + (kScales + 1023) / 1024 * 1024;
   // Two CTAs on an SM where a stage has 32 KB, else three; as many stages, up to four, as fit beside the joining buffer.
-  static constexpr int kCtas = kTile == 16384 ? 2 : 3;
+  static constexpr int kCtas = D == 128 ? 2 : 3;
   static constexpr int kJoin = kFewWarps * kFewRows * kPadCols * 4;
   static constexpr int kRoom = (227 * 1024 / kCtas - 1024 - kJoin - 2048) / kStageBytes;
   static constexpr int kStages = kRoom > 4 ? 4 : kRoom;
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
     attn_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
   using F = Few<D, KIND>;
   constexpr bool BF = KIND == MQ_BF16, S8 = KIND == MQ_S8;
-  constexpr int WK = kFewWarps, KW = kFewKeys / WK;  // the warps share a block's keys
+  constexpr int kFewKeys = F::kKeys, WK = kFewWarps, KW = kFewKeys / WK;  // the warps share a block's keys
   constexpr int NT = KW / 8, S = F::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
   }
   __syncthreads();
   griddep_wait();
-  find_share<kFewThreads, FewGrain>(p.seqs, p.shape, scratch);
+  find_share<kFewThreads, typename F::Units>(p.seqs, p.shape, scratch);
   if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = scratch.found.total, p.parts.counts[1] = scratch.found.parts;
   if (static_cast<int>(blockIdx.x) >= scratch.found.parts) return;
   Item item;
@@ -177,9 +180,9 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
     }
     const int box_rows = min(kFewKeys, 1 << p.seqs.page_log2), per_block = kFewKeys / box_rows;
     const int boxes = per_block * F::kBoxes;  // of keys, and as many of values
-    Walk<FewGrain> walk;
+    Walk<typename F::Units> walk;
     walk.start(p.shape, scratch.found);
-    const Walk<FewGrain> begin = walk;
+    const Walk<typename F::Units> begin = walk;
     int s = 0, round = 0, k = 0;
     uint32_t issued = 0;
     bool ok = true;
@@ -196,10 +199,10 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
         const int live = max(0, min(per_block, (item.s.length - key0 + box_rows - 1) / box_rows));
         int page = -1;  // lane l knows the page of box l of the block
         if (lane < live) page = page_of(p.seqs, item.b, key0 + lane * box_rows);
-        float sk[2], sv[2];  // scales of keys lane and lane + 32
+        float sk[kFewKeys / 32], sv[kFewKeys / 32];  // scales of keys lane, lane + 32 ..
         if (S8) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < kFewKeys / 32; ++h) {
             const int key = lane + 32 * h, of = __shfl_sync(0xffffffffu, page, key / box_rows);
             sk[h] = 0.f, sv[h] = 0.f;
             if (of >= 0 && key0 + key < item.s.length) {
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
         if (S8) {
           float *sc = reinterpret_cast<float *>(stage + 2 * F::kTile);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < kFewKeys / 32; ++h)
             sc[lane + 32 * h] = sk[h], sc[kFewKeys + lane + 32 * h] = lg2(sv[h]), sc[2 * kFewKeys + lane + 32 * h] = __frcp_rn(sv[h]);
         }
         if (lane == 0) mbar_expect_tx(&full[s], 2 * live * F::kBoxes * box_rows * F::kBox);
@@ -671,7 +674,7 @@ template <int D, int KIND>
 int launch_few(const mq_kv_pages *c, AttnParams p, int ctas, void *workspace, cudaStream_t stream, const char *what) {
   using F = Few<D, KIND>;
   CUtensorMap kmap, vmap;
-  const int box_rows = std::min(kFewKeys, c->page);
+  const int box_rows = std::min(F::kKeys, c->page);
   const CUtensorMapSwizzle swizzle = KIND == MQ_S8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   if (int rc = encode_pages(&kmap, c->k, KIND, c, c->k_stride, F::kBox, box_rows, swizzle, what)) return rc;
   if (int rc = encode_pages(&vmap, c->v, KIND, c, c->v_stride, F::kBox, box_rows, swizzle, what)) return rc;

@@ -814,7 +814,7 @@ inline int plan_for(Plan *plan, const mq_kv_pages *c, int64_t heads, int64_t bat
   const bool few = group <= kRowsForTiles && !(batch == 1 && most == tokens && tokens * group > kRowsForTiles) &&
                    !(plan->most_rows <= 128 && tokens * group >= 2 * kRowsForTiles * batch);
   const bool tile = plan->most_rows > kRowsForTiles || !few;
-  plan->few_ctas = !few ? 0 : sms * (c->dtype != MQ_S8 && plan->d == 128 ? 2 : 3);
+  plan->few_ctas = !few ? 0 : sms * (plan->d == 128 ? 2 : 3);
   plan->tile_ctas = tile ? sms : 0;
   plan->bytes = 0;
   if (few) plan->bytes = parts_bytes(plan->few_ctas, kFewRows, plan->d);
