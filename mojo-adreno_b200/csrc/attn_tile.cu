@@ -812,7 +812,7 @@ inline int plan_for(Plan *plan, const mq_kv_pages *c, int64_t heads, int64_t bat
   // One sequence may have all the tokens; and where sequences have some drafted tokens each, a launch for the few that may have one
   // or two costs more than they do among the others (16 x 5 tokens, 8 heads to a kv head: 36.0 us with it, 32.7 without).
   const bool few = group <= kRowsForTiles && !(batch == 1 && most == tokens && tokens * group > kRowsForTiles) &&
-                   !(plan->most_rows <= 128 && tokens * group >= 2 * kRowsForTiles * batch);
+                   !(plan->most_rows > kRowsForTiles && plan->most_rows <= 128 && tokens * group >= 2 * kRowsForTiles * batch);
   const bool tile = plan->most_rows > kRowsForTiles || !few;
   plan->few_ctas = !few ? 0 : sms * (plan->d == 128 ? 2 : 3);
   plan->tile_ctas = tile ? sms : 0;

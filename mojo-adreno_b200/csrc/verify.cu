@@ -55,7 +55,7 @@ struct Params {
 __device__ __forceinline__ int rows_per_request(const Params &p) { return p.draft ? 2 * p.drafts + 1 : p.drafts + 1; }
 __device__ __forceinline__ float temperature_of(const Params &p, int b) {
   const float t = p.temperature ? p.temperature[b] : 1.f;
-  return t >= kLeastTemperature ? t : 0.f;
+  return t >= kLeastTemperature ? fminf(t, 1e30f) : 0.f;  // (an infinite one would make -infinity / T no number)
 }
 __device__ __forceinline__ int count_of(const Params &p, int b) {
   const int n = p.counts ? p.counts[b] : p.drafts;

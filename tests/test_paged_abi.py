@@ -83,6 +83,22 @@ def test_copies(args, code, match):
         assert rc == code and match in msg, msg
 
 
+@pytest.mark.parametrize("shift,refused", [(0, True), (128, True), (64 * 2 * 16 * 2 - 16, True), (64 * 2 * 16 * 2 * 8, False), (-64 * 2 * 16 * 2 * 8, False)])
+def test_store_where_keys_and_values_share_memory(shift, refused):
+    """v `shift` bytes behind k, both of 8 pages of 2 x 16 rows of 128 bytes."""
+    c = pages(v=OK + shift)
+    rc, msg = status("mq_kv_store", OK, 128, 64, OK, 128, 64, 1, ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, None)
+    assert ("share memory" in msg and rc == -1) if refused else rc != -1  # (without a device the call ends behind the checks)
+
+
+def test_store_of_interleaved_pages_is_not_refused():
+    """One tensor [pages, 2, heads, page, dim]: keys and values lie between one another's pages."""
+    stride = (2 * 2 * 16 * 64, 16 * 64, 64)
+    c = pages(k_stride=stride, v_stride=stride, v=OK + 2 * 16 * 64 * 2)
+    rc, msg = status("mq_kv_store", OK, 128, 64, OK, 128, 64, 1, ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, None)
+    assert rc != -1, msg
+
+
 def test_load_into_rows_that_overlap():
     rc, msg = status("mq_kv_load", ctypes.addressof(pages()), OK, 4, 4, OK, OK, 2, 5, OK, 64, 64, OK, 128, 64, 1, None)
     assert rc == -1 and "overlap" in msg

@@ -549,6 +549,48 @@ def test_captured_step(cuda):
         assert mq.device_status() == 0
 
 
+@pytest.mark.parametrize("cache,x", [(S8, BF16), (F16, F16)])
+def test_pages_beyond_32_bits(cuda, cache, x):
+    """A pool of more than 2^32 bytes (fp16: 2^32 elements): the pages in use are its first and its last ones."""
+    page, kv_heads, dim = 64, 8, 128
+    pages = 2 ** 32 // (page * kv_heads * dim) + 9
+    k, v = (torch.empty(pages, kv_heads, page, dim, dtype=cache, device=cuda) for _ in range(2))
+    scales = [torch.zeros(pages, kv_heads, page, device=cuda) for _ in range(2)] if cache == S8 else []
+    pool = mq.PagedCache(k, v, *scales)
+    ids = [pages - 1, 0, pages - 3, pages // 2 + 1, 2, pages - 2]
+    small = mq.paged_cache(len(ids), kv_heads, page, dim, cache)
+    g = torch.Generator(device=cuda).manual_seed(2)
+    table = torch.tensor([ids[:3], ids[3:]], dtype=torch.int32, device=cuda)
+    near = torch.arange(6, dtype=torch.int32, device=cuda).view(2, 3)
+    lengths = torch.tensor([180, 130], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, 180, 310], dtype=torch.int32, device=cuda)
+    rows = [torch.randn(310, kv_heads, dim, generator=g, device=cuda).to(x) for _ in range(2)]
+    q = torch.randn(310, 16, dim, generator=g, device=cuda).to(x)
+    for c, t in ((pool, table), (small, near)):
+        mq.kv_store(*rows, c, t, lengths, starts)
+    for a, b in zip(mq.kv_load(pool, table, lengths, starts, tokens=310, dtype=x), mq.kv_load(small, near, lengths, starts, tokens=310, dtype=x)):
+        assert torch.equal(a, b)
+    assert torch.equal(mq.paged_attention(q, pool, table, lengths, starts), mq.paged_attention(q, small, near, lengths, starts))
+    assert torch.equal(mq.paged_attention(q[:2], pool, table, lengths), mq.paged_attention(q[:2], small, near, lengths))
+    assert mq.device_status() == 0
+
+
+def test_workspace_of_a_larger_call_is_enough(cuda):
+    """Sizes never fall when a call has more sequences, tokens or new tokens."""
+    for dim, dtype in ((64, F16), (128, S8)):
+        cache = mq.paged_cache(2, 2, 16, dim, dtype)
+        for heads in (2, 8, 16, 64):
+            size = {}
+            for batch in (1, 2, 4, 9):
+                for tokens in (1, 2, 4, 9, 40):
+                    for most in (1, 2, 5, 40):
+                        size[batch, tokens, most] = mq.paged_attention_workspace(cache, heads, batch, tokens, most)
+            for a, sa in size.items():
+                for b, sb in size.items():
+                    if all(i <= j for i, j in zip(a, b)):
+                        assert sa <= sb, (heads, a, b)
+
+
 def test_workspace_serves_smaller_calls(cuda):
     batch = Batch(cuda, [(1, 900), (80, 300)], 2, 16, 128, BF16)
     cache = batch.cache()

@@ -120,6 +120,22 @@ def test_counts(cuda):
     case.check(got)
 
 
+def test_temperatures_at_the_ends(cuda):
+    """An infinite temperature: all tokens that are not masked alike; one that is no number: greedy."""
+    case = Case(cuda, 4, 2, 301, F32, True, [1.0])
+    case.temperature[:] = torch.tensor([float("inf"), 1e38, float("nan"), -1.0], device=cuda)
+    mq.device_status()
+    tokens, accepted, logprobs = case.call()
+    assert mq.device_status() == 0
+    z = case.target.view(4, 3, 301)
+    for b in range(2):  # 1 / (tokens that are not masked) each
+        for i in range(int(accepted[b]) + 1):
+            assert abs(float(logprobs[b, i]) + math.log(int(z[b, i].isfinite().sum()))) < 1e-4
+            assert z[b, i, tokens[b, i]].isfinite()
+    for b in range(2, 4):
+        assert tokens[b, 0] == z[b, 0].argmax()
+
+
 def test_identical_distributions_keep_all(cuda):
     """Draft and target the same: every token that the draft gives any weight is kept."""
     case = Case(cuda, 16, 5, 3001, F32, True)
