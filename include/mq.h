@@ -66,8 +66,10 @@ MQ_API int mq_version(void);
  * (0 = none, else the code of the first wait that gave up). Synchronises `stream`. When `reset`
  * is nonzero the word is cleared afterwards. Returns the word (>= 0) or a negative MQ_E* code.
  * Waits: 1-4 int4 and ternary GEMM, 5-7 GEMVs, 10 and 11 a peer's rows or returns, 12-14 int8 products, 17 beam
- * selection, 18 norms. Four codes report data instead: 8 an expert id out of range, 9 more pairs than a rank's capacity,
- * 15 a beam with a NaN or +inf logit, 16 a parent out of range. The first code of either kind stays until it is reset,
+ * selection, 18 norms, 21-23 attention. Others report data instead: 8 an expert id out of range, 9 more pairs than a rank's
+ * capacity, 15 a beam with a NaN or +inf logit, 16 a parent out of range, 19 a page outside its pool, 20 a length out of range,
+ * 24 a row of logits that is no distribution, 25 a drafted token or number of drafts out of range, 26 a sequence with more new
+ * tokens than the call said. The first code of either kind stays until it is reset,
  * so a caller who expects such data resets the word to see what comes later. */
 MQ_API int mq_device_status(int reset, void *stream);
 
@@ -448,8 +450,9 @@ typedef struct mq_kv_pages {
 
 /* k[t][h], v[t][h] -> the pages, rounded to their type; int8 as mq_quantize_s8 makes it, row by row (a row with a NaN or an
  * infinity: zeros and scale NaN). k, v: fp32, fp16 or bf16 (dtype), [tokens][heads][dim] with strides in elements, rows
- * 16-byte aligned. A position that two rows name gets either's values, or a mix of the two. Keys and values, and the rows that
- * are read, must not share memory with one another's pages. */
+ * 16-byte aligned. A position that two rows name (of sequences that share a page) gets either's
+ * values, or a mix of the two, unless they are equal. Keys' and values' pages must not share memory (refused where they have one
+ * layout), nor the rows with the pages. */
 MQ_API int mq_kv_store(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
                        int dtype, const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width,
                        const int32_t *lengths, const int32_t *starts, int64_t batch, int64_t tokens, void *stream);
@@ -464,7 +467,9 @@ MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ld
  * q's own buffer with q's strides. A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
  * row does not see have no influence on it, whatever they hold; one that it sees and whose row holds a NaN or an infinity (int8: whose scale is one) makes
  * it NaN or infinite. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they
- * meet the values; an int8 cache's scales must not be negative, and a value scale below 1e-30 counts as 1e-30.
+ * meet the values; bf16 rows of more than 16 per kv head and sequence (or of drafted tokens) meet an int8 cache as fp16 operands,
+ * each integer times its scale over the largest of 32 keys, rounded. An int8 cache's scales must not be negative, and a value
+ * scale below 1e-30 counts as 1e-30.
  * max_new: no sequence has more new tokens (0: unknown); one that has is reported (26) and its rows are left as they are.
  * scale > 0. Reproducible bit for bit. workspace: mq_paged_attention_workspace_size() bytes, 16-byte aligned (0 for sizes that
  * are refused); calls that may overlap in time need one each. tokens == 0 does nothing. */
@@ -484,7 +489,7 @@ MQ_API int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, int64
  * exceeds uniform[b][drafts] times the whole (sums in fp64). A temperature below 1e-5 (or NaN): p_i is all on the largest logit, the
  * lowest index among equal ones, and the draft's logits and the uniforms do not count.
  * tokens[b]: the kept ones, the drawn one, then -1; accepted[b] = n; logprobs[b][i] = log p_i(tokens[b][i]), 0 behind.
- * temperature: fp32 [batch] or NULL (1). counts: int32 [batch] or NULL, how many drafts request b has (<= drafts; outside
+ * temperature: fp32 [batch] or NULL (1); above 1e30 it counts as 1e30. counts: int32 [batch] or NULL, how many drafts request b has (<= drafts; outside
  * [0, drafts] reported, 25, and cut); rows behind are not read. A drafted token outside the vocabulary is reported (25) and not kept. A target row that is
  * no distribution (a NaN, +infinity, all -infinity) is reported (24), and its request ends there with token -1; such a draft row is
  * reported, its token is not kept and q counts as 0. Logits: fp32, fp16 or bf16, rows ld elements apart. drafts <= 32.
