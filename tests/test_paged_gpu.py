@@ -483,6 +483,104 @@ def test_store_then_attend_as_used(cuda):
         assert mq.device_status() == 0
 
 
+class Drafted(Batch):
+    """Steps with drafted tokens, as they are used: qkv product, kv_store, paged_attention, head product, verify_drafts, and the
+    lengths that follow from what was accepted, all on the device. Three requests, one of them greedy, one that begins empty."""
+
+    heads, kv_heads, dim, page, drafts, vocab = 8, 2, 64, 16, 3, 203
+    temperatures, before = [1.0, 0.0, 0.7], [0, 5, 33]
+
+    def __init__(self, cuda, dtype, x):
+        g = torch.Generator(device=cuda).manual_seed(9)
+        self.g, self.cuda, self.dtype, self.x, self.ints = g, cuda, dtype, x, dtype == S8
+        wide, self.n, b = self.heads * self.dim, self.drafts + 1, 3
+        self.np_starts = [self.n * i for i in range(b + 1)]
+        self.tokens, self.starts = self.n * b, torch.tensor(self.np_starts, dtype=torch.int32, device=cuda)
+        self.table = torch.randperm(6 * b, generator=g, device=cuda).int().view(b, 6).contiguous()
+        self.pool = mq.paged_cache(6 * b, self.kv_heads, self.page, self.dim, dtype)
+        self.k, self.v, self.scales = self.pool.k, self.pool.v, [self.pool.k_scale, self.pool.v_scale]
+        self.qkv = mq.quantize_s8(torch.randn(wide + 2 * self.kv_heads * self.dim, wide, generator=g, device=cuda) * wide ** -0.5)
+        self.head = mq.quantize_s8(torch.randn(self.vocab, wide, generator=g, device=cuda) * 3 * wide ** -0.5)
+        self.temperature = torch.tensor(self.temperatures, device=cuda)
+        self.h = torch.empty(self.tokens, wide, dtype=F16, device=cuda)
+        self.draft = torch.empty(b * self.drafts, self.vocab, device=cuda)
+        self.drafted = torch.empty(b, self.drafts, dtype=torch.int32, device=cuda)
+        self.uniform = torch.empty(b, self.n, device=cuda)
+        self.lengths = torch.empty(b, dtype=torch.int32, device=cuda)
+        self.work = torch.empty(mq.paged_attention_workspace(self.pool, self.heads, b, self.tokens, self.n), dtype=torch.uint8, device=cuda)
+        self.verify_work = torch.empty(mq.verify_workspace(b, self.drafts, self.vocab), dtype=torch.uint8, device=cuda)
+        self.past = [[torch.randn(m, self.kv_heads, self.dim, generator=g, device=cuda).to(x) for _ in range(2)] for m in self.before]
+        self.inputs = [self.draw() for _ in range(6)]
+
+    def draw(self):
+        draft = torch.randn(self.draft.shape, generator=self.g, device=self.cuda)
+        drafted = torch.multinomial(draft.softmax(-1), 1, generator=self.g).int().view(self.drafted.shape)
+        return (torch.randn(self.h.shape, generator=self.g, device=self.cuda).half(), draft, drafted,
+                torch.rand(self.uniform.shape, generator=self.g, device=self.cuda))
+
+    def begin(self):
+        for b, (k, v) in enumerate(self.past):
+            if len(k):
+                m = torch.tensor([len(k)], dtype=torch.int32, device=self.cuda)
+                mq.kv_store(k, v, self.pool, self.table[b:b + 1], m, torch.tensor([0, len(k)], dtype=torch.int32, device=self.cuda))
+        self.lengths.copy_(torch.tensor(self.before, device=self.cuda) + self.n)
+
+    def feed(self, i):
+        for t, new in zip((self.h, self.draft, self.drafted, self.uniform), self.inputs[i]):
+            t.copy_(new)
+
+    def step(self):
+        at = self.lengths.clone()
+        wide, kv = self.heads * self.dim, self.kv_heads * self.dim
+        y = mq.gemm_w8a8(*mq.quantize_s8(self.h), *self.qkv, dtype=self.x)
+        q, k, v = (p.view(self.tokens, -1, self.dim) for p in y.split([wide, kv, kv], 1))
+        mq.kv_store(k, v, self.pool, self.table, self.lengths, self.starts)
+        o = mq.paged_attention(q, self.pool, self.table, self.lengths, self.starts, max_new=self.n, workspace=self.work)
+        logits = mq.gemm_w8a8(*mq.quantize_s8(o.view(self.tokens, -1)), *self.head, dtype=F32)
+        got = mq.verify_drafts(logits, self.drafted, self.uniform, draft=self.draft, temperature=self.temperature, workspace=self.verify_work)
+        self.lengths.add_(got[1] + 1)
+        return [at, q, k, v, o, logits, *got, self.lengths]
+
+
+@pytest.mark.parametrize("dtype,x", CACHES)
+def test_drafted_steps_as_used(cuda, dtype, x):
+    """Each operator against the oracle on what it was given, step after step as the lengths follow from the tokens that were
+    accepted; then the same steps as one captured graph, with the same bits."""
+    d = Drafted(cuda, dtype, x)
+    d.begin()
+    want, seen = [], set()
+    for i in range(len(d.inputs)):
+        d.feed(i)
+        at, q, k, v, o, logits, tokens, accepted, logprobs, after = got = d.step()
+        assert mq.device_status() == 0
+        d.sizes = [(d.n, length) for length in at.tolist()]
+        if dtype != S8:
+            held = mq.kv_load(d.pool, d.table, at, d.starts, tokens=d.tokens, dtype=x)
+            assert torch.equal(held[0], k) and torch.equal(held[1], v)
+        d.check(o, q, d.dim ** -0.5)
+        for b, t in enumerate(d.temperatures):
+            rows, theirs = host(logits.view(3, d.n, -1)[b]), host(d.draft.view(3, d.drafts, -1)[b])
+            # (temperatures as the device holds them)
+            ref = paged.verify(rows, host(d.drafted[b]), host(d.uniform[b]), theirs, float(d.temperature[b]))
+            assert tokens[b].tolist() == ref[0] and int(accepted[b]) == ref[1]
+            unit = 2.0 ** -24 * (2 * (np.log2(d.vocab) + 2) + 4 + d.vocab / 256 + 24)  # as the verification's own tests derive it
+            assert (np.abs(host(logprobs[b]) - ref[2]) <= unit + 2.0 ** -24 * np.abs(ref[2])).all()
+            seen.add(ref[1])
+        assert torch.equal(after, at + accepted + 1)
+        want.append([t.clone() for t in got])
+    assert 0 in seen and len(seen) > 1, "the steps keep different numbers of drafted tokens"
+    d.begin()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = d.step()
+    for i in range(len(d.inputs)):
+        d.feed(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want[i])), i
+    assert mq.device_status() == 0
+
+
 # ---- streams, graphs, refusals ----------------------------------------------------------------------------------
 
 
