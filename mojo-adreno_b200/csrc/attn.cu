@@ -9,8 +9,8 @@
 // arithmetic goes to the warp-level mma.m16n8k16, which has the rate for it (64 keys x 128 dim x 16 rows: 128 of them, 280 cycles,
 // against the 1400 that an SM's share of the bandwidth needs for the 16-bit rows) and takes its operands without a detour through
 // TMEM. 64 sequences of 4000 positions on average, 8 kv heads of 128: bf16 163 us (6.5 TB/s, the copy bandwidth), int8 144 us
-// (3.8 TB/s: conversions and their latency, a third of the cycles issue). One sequence of 1001: 8.5 us with the joining
-// kernel, latency: 1.3 for the shares, 0.7 until an item is known, 1.2 for the first copy, 2 for joining the warps, 3 for the parts.
+// (3.8 TB/s: conversions and their latency, a third of the cycles issue). One sequence of 1001: 8.7 us with the joining
+// kernel, latency: a traced run had 1.3 for the shares, 0.6 until an item is known and 5.1 for the whole launch.
 //
 //  * A producer warp walks through the CTA's items and brings blocks of 64 keys and values (int8: 128) through a ring, one tiled
 //    copy per page (or part of one) and 128 (int8: 64) bytes of a row, a lane each. Only an item's end joins the consumers.
@@ -25,8 +25,8 @@
 //    weights that meet the integers are at most 2^8 whatever the scales, and the sum of w is that of (w t) (1 / t).
 //  * Weights are rounded to the MMA's 16 bits (scores, maxima, sums and accumulators are fp32). A 16-bit cache's are summed as
 //    they were rounded, which takes the error back where one key has most of the weight.
-//  * Neither kernel lets the next one start early: its CTAs would sit on the SMs with room for some, and one of this grid's,
-//    which is exactly as many as run at once, would begin when all others end (64x1 int8: 210 us instead of 146).
+//  * Neither kernel lets the next one start early (64x1 int8: 210 us with both doing so, 146 with either or neither). Why is not
+//    traced; early CTAs taking places of a grid that is as many CTAs as run at once would explain it.
 //  * The maximum may lag by 2^8 before accumulators are rescaled: weights up to 2^8 are as exact in fp16 and bf16.
 //  * Blocks that some row sees only in part: scores are replaced, not added to, so no hidden key's value matters; a
 //    value that is no number is taken out of the product and makes the sum, so the result, of the rows that see it NaN.
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
 
 // Joins the parts of the items that CTAs of the launch before shared. CTA c (of x) takes the item that c goes on with
 // where c is the first to do so; a warp a row. What a row needs is known after one load (the cut), so that the
-// parts' statistics and sums come together: a few CTAs' parts of a short call take 3 us, most of it the launch.
+// parts' statistics and sums come together: with nothing to join the launch took 3 us (profiled, cold).
 struct JoinParams {
   Shape shape;
   Output o;

@@ -16,8 +16,8 @@
 //
 // 8192 tokens, 32 heads on 8 of 128, bf16: 535-620 us, 0.9-1.03 PFLOP/s (0.53-0.61 of the measured burst, 0.63-0.72 of the
 // sustained rate; power caps the clock). A step of both accumulators takes some 2000 cycles where its MMAs take 1280 and its
-// exponentials 1024: what is left over is waiting between the two. Short calls are latency: 431 tokens 21 us, of which 3 for the
-// shares, 3 until the first scores, 3 for one to four steps, 2 for the output and 5 for joining the parts.
+// exponentials 1024: what is left over is waiting between the two. Short calls are latency: 431 tokens 22 us; a traced
+// run had 2.8 for the shares, 3.8 more until the first scores, 3.0 for one to four steps, 2.6 for the output, then the join.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -36,7 +36,7 @@ constexpr int kStageBytes = 2048;  // per softmax warp: 64 bytes of each of its 
 // An int8 cache's kinds here. Exact: the integers are the operands, the keys' and values' scales meet the scores and weights
 // (attn.cu). Folded, for bf16 rows: the operands are fp16, integer * scale / (the largest scale of 32 keys), rounded (2^-11 twice, a
 // quarter of what bf16 rounds), so the softmax has one factor for 32 scores and one for their weights where the exact one reads
-// three numbers per key and row from shared memory (2048 of 30000 tokens: 1240 us instead of 1440). A block that some row sees
+// three numbers per key and row from shared memory (2048 of 30000 tokens: 1200-1270 us instead of 1440). A block that some row sees
 // only in part is exact there too: a scale that a row does not see does not touch what it sees.
 constexpr int kFolded = 16;
 template <int D, int KIND>

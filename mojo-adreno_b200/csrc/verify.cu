@@ -9,16 +9,15 @@
 //
 // verify_scan_kernel reads every logit once: `splits` CTAs per row keep a maximum and a sum of exponentials, in fp32:
 // a comparison of u q with p is off by some 1e-7, so it decides otherwise once in 10^7 times. It is bound by the bandwidth
-// (64 requests x 9 rows x 128256 fp32: 45-47 us, 6.3-6.6 TB/s).
+// (64 requests of 128256 fp32 and 4 drafts, 21 of them greedy, so 252 MB: 47 us, 5.4 TB/s, 0.82 of a copy's).
 //
 // verify_draw_kernel, a cluster per request, decides, and goes through the chosen row again for the draw. There fp32 does not do:
 // the running sum passes some 10^5 borders between tokens, and a relative error of 1e-8 in it would move the drawn token
 // to its neighbour once in a thousand draws. So the sums and the exponentials in them are fp64: 2^y with
 // y = n / 32 + r, |r| <= 1/64, is 2^(n / 32) from a table of 32 times a Taylor polynomial of degree 5 (2e-15), nine
 // fp64 instructions. Each warp has a stretch of the row of its own; the CTA whose stretch holds the drawn token looks for it.
-// It goes through the row twice where q is taken off (first for the two sums): 58 us for the 48 of those 64 requests that draw
-// by chance, bound by the latency of the fetches and of the cluster's three exchanges. A greedy request needs neither (1 x 9 rows
-// of 151669: 5.9 us in all).
+// It goes through the row twice where q is taken off (first for the two sums): 60 us for the 43 of those 64 requests that sample, bound by the latency of the fetches and of the cluster's three exchanges. A greedy request needs neither (4 drafts of
+// 151669: 6 us in all, 31 where it samples).
 #include <algorithm>
 #include <type_traits>
 
