@@ -17,8 +17,9 @@
 // y = n / 32 + r, |r| <= 1/64, is 2^(n / 32) from a table of 32 times a Taylor polynomial of degree 5 (2e-15), nine
 // fp64 instructions. Each warp has a stretch of the row of its own; the CTA whose stretch holds the drawn token looks for it.
 // It goes through the row twice where q is taken off (first for the two sums): 60 us for the 43 of those 64 requests that sample, bound by the latency of the fetches and of the cluster's three exchanges. A greedy request needs neither (4 drafts of
-// 151669: 6 us in all, 31 where it samples).
+// 151669: 6 us in all, 27 where it samples).
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -27,9 +28,12 @@ namespace mq {
 namespace verify {
 
 constexpr int kScan = 256, kVecs = 4;        // threads of a scan CTA, 16-byte vectors per thread and step
-constexpr int kCluster = 8;                  // drawing CTAs of a request
-// Their threads: many for the latency of a few requests, fewer where that lets all CTAs run at once (four on an SM).
-constexpr int kDrawFew = 512, kDrawMany = 256, kManyRequests = 148 * 2 / kCluster;
+// The drawing CTAs of a request and their threads: many for the latency of a few requests, fewer where that lets all CTAs run at
+// once (four of 256 on an SM). Sixteen CTAs against eight, requests of 4 drafts and 151669 fp32 that all sample, scan and draw:
+// 1: 26.7 us (31.1), 4: 32.5 (37.4), 9: 44.2 (46.9), 12: 48.1 (53.8), but 18: 69.8 (62.9), 37: 120 (100). (With an SM to each of
+// the sixteen, and registers for it, 1: 25.8, 4: 30.4, but 9: 49.1.)
+constexpr int kClusterFew = 16, kCluster = 8;
+constexpr int kDrawFew = 512, kDrawMany = 256, kFewRequests = 12, kManyRequests = 148 * 2 / kCluster;
 constexpr int kMaxDrafts = 32, kMaxSplits = 64;
 constexpr float kLeastTemperature = 1e-5f;   // below: 0
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
@@ -223,7 +227,7 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-template <typename T, int kDraw>
+template <typename T, int kDraw, int kCluster>
 __global__ void __launch_bounds__(kDraw, 1024 / kDraw) verify_draw_kernel(const Params p) {
   constexpr int kWarps = kDraw / 32, stretch = kCluster * kWarps, kPer = stretch / 32;  // stretches of a row; of a lane
   __shared__ double table[32];
@@ -504,10 +508,43 @@ int scan(const Params &p, int64_t ctas, cudaStream_t s, const char *what) {
   return launch_overlapped(verify_scan_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(kScan), 0, s, what, p);
 }
 
+// Whether this device runs clusters of kClusterFew, which are more than every device of the architecture has to take: asked
+// once per kernel and device. Two threads that ask at once get the same answer.
 template <typename T>
-int draw(const Params &p, dim3 grid, cudaStream_t s, const char *what) {
-  if (p.batch > kManyRequests) return launch_overlapped_clusters(verify_draw_kernel<T, kDrawMany>, grid, dim3(kDrawMany), kCluster, 0, s, what, p);
-  return launch_overlapped_clusters(verify_draw_kernel<T, kDrawFew>, grid, dim3(kDrawFew), kCluster, 0, s, what, p);
+bool wide_clusters_run() {
+  static std::atomic<int> known[64];  // 0 not asked, 1 yes, 2 no
+  auto *kern = verify_draw_kernel<T, kDrawFew, kClusterFew>;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return false;
+  int yes = known[device].load(std::memory_order_acquire);
+  if (yes == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kClusterFew);
+    cfg.blockDim = dim3(kDrawFew);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kClusterFew;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    const bool ok = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters > 0;
+    if (!ok) cudaGetLastError();  // (the answer is no, not an error of this call)
+    yes = ok ? 1 : 2;
+    known[device].store(yes, std::memory_order_release);
+  }
+  return yes == 1;
+}
+
+template <typename T>
+int draw(const Params &p, cudaStream_t s, const char *what) {
+  auto go = [&](auto kern, int threads, int cluster) {
+    return launch_overlapped_clusters(kern, dim3(static_cast<unsigned>(p.batch * cluster)), dim3(threads), cluster, 0, s, what, p);
+  };
+  if (p.batch > kManyRequests) return go(verify_draw_kernel<T, kDrawMany, kCluster>, kDrawMany, kCluster);
+  if (p.batch <= kFewRequests && wide_clusters_run<T>()) return go(verify_draw_kernel<T, kDrawFew, kClusterFew>, kDrawFew, kClusterFew);
+  return go(verify_draw_kernel<T, kDrawFew, kCluster>, kDrawFew, kCluster);
 }
 
 inline bool sizes_fit(int64_t batch, int64_t drafts, int64_t vocab) {
@@ -560,8 +597,7 @@ extern "C" int mq_verify_drafts(const void *target, int64_t ld_target, const voi
   else
     rc = scan<__nv_bfloat16>(p, rows * p.splits, s, what);
   if (rc) return rc;
-  const dim3 draws(static_cast<unsigned>(batch * kCluster));
-  if (dtype == MQ_F32) return draw<float>(p, draws, s, what);
-  if (dtype == MQ_F16) return draw<__half>(p, draws, s, what);
-  return draw<__nv_bfloat16>(p, draws, s, what);
+  if (dtype == MQ_F32) return draw<float>(p, s, what);
+  if (dtype == MQ_F16) return draw<__half>(p, s, what);
+  return draw<__nv_bfloat16>(p, s, what);
 }

@@ -74,6 +74,13 @@ def test_verify(cuda, dtype, batch, drafts, vocab, pad, draft):
         case.check(got)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch", [12, 13, 37, 38])
+def test_batches_where_the_draw_is_split_otherwise(cuda, dtype, batch):
+    case = Case(cuda, batch, 2, 1501, dtype, True, [1.0, 0.0, 0.7], batch)
+    case.check(case.call())
+
+
 @pytest.mark.parametrize("draft", [True, False])
 def test_without_temperature_and_given_outputs(cuda, draft):
     case = Case(cuda, 6, 3, 2003, F32, draft)
