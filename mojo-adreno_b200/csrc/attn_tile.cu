@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t *ring = q_tile + T::kQ, *raw = ring + NS * T::kBlock, *stages = raw + 2 * T::kRaw;
-  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained[2], s_full[2][2], p_full[2][2], o_step[2], o_full[2], half_done, half_read, turn[2][4];
+  __shared__ uint64_t full[NF], raw_empty[2], ready[NS], empty[NS], q_full[2], q_empty[2], drained[2], s_full[2][2], p_full[2][2], o_step[2], o_full[2], half_done, half_read, turn[2][4], factors_read[2];
   __shared__ uint32_t bad_keys[NS][4];
   __shared__ __align__(16) float scales[S8 ? 2 : 1][3][S8 ? kTileKeys : 1], row_factor[2][S8 ? kTileRows : 1];
   __shared__ ItemRing items;
@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     for (int i = 0; i < 8; ++i) mbar_init(&turn[i / 4][i % 4], 1);
     mbar_init(&half_done, 4);
     mbar_init(&half_read, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&factors_read[i], 8);
     items.init(2 + kAuxWarps + 8);
     fence_mbar_init();
   }
@@ -352,7 +353,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                static_cast<int64_t>(item.head * group + (r - i * group)) * p.q_head;
       };
       const int tiles = rows > 128 ? 2 : 1;
-      for (int g = 0; g < tiles; ++g) {
+      // The rows' factors take the place of those of the item before last. q_empty does not say that both accumulators' softmax
+      // warps are through with them: a narrow item's are read by both, and behind an item of one block and two tiles only the
+      // first one's MMA thread has spoken.
+      if (S8 && at_item >= 2) ok = warp_wait(&factors_read[at_item & 1], (at_item / 2 - 1) & 1, kStatusAttnLoadWait);
+      for (int g = 0; ok && g < tiles; ++g) {
         uint8_t *dst = q_tile + g * (T::kQ / 2);
         if (q_uses[g] > 0) ok = warp_wait(&q_empty[g], (q_uses[g] - 1) & 1, kStatusAttnLoadWait);
         if (!ok) break;
@@ -684,6 +689,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!ok) break;
       n0 += 2 * item.blocks;
       o_steps += steps;
+      if (S8) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&factors_read[(k_item - 1) & 1]);
+      }
       if (narrow && g == 1) {
         half_stats[r] = make_float2(m, l);
         __syncwarp();

@@ -740,3 +740,20 @@ def test_refusals(cuda):
     refuses("16-byte", lambda: mq.kv_store(kv, kv, mq.PagedCache(wide, wide.clone()), table, lengths))
     flat = torch.zeros(1, 2, 16, 64, device=cuda, dtype=F16).expand(4, 2, 16, 64)
     refuses("overlap", lambda: mq.kv_store(kv, kv, mq.PagedCache(flat, cache.v), table, lengths))
+
+
+@pytest.mark.parametrize("x", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_int8_narrow_and_wide_items_in_turn(cuda, x, dim):
+    """Items of at most 128 rows and items of more, of one block each, several in turn for every CTA: the rows' factors (which
+    differ from row to row) change while the accumulators are not equally far."""
+    sizes = [(n, n + extra) for n, extra in ((9, 40), (40, 60), (64, 0), (30, 98), (64, 64), (33, 0))] * 60
+    batch = Batch(cuda, sizes, 2, 16, dim, S8)
+    q = torch.randn(batch.tokens, 8, dim, generator=batch.g, device=cuda) * 2.0 ** torch.randint(-6, 3, (batch.tokens, 8, 1), generator=batch.g, device=cuda)
+    q = q.to(x)
+    mq.device_status()
+    out = mq.paged_attention(q, batch.cache(), *batch.where(), max_new=64)
+    for _ in range(20):
+        assert torch.equal(mq.paged_attention(q, batch.cache(), *batch.where(), max_new=64), out)
+    assert mq.device_status() == 0
+    batch.check(out, q, dim ** -0.5)
