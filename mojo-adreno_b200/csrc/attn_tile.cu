@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   ShareScratch<kTileThreads> &scratch = *reinterpret_cast<ShareScratch<kTileThreads> *>(ring);  // (nothing has been copied yet)
   find_share<kTileThreads, TileGrain>(p.seqs, p.shape, scratch);
   const Share share = scratch.found;
-  __syncthreads();  // (the ring is free again)
+  fence_proxy_async_smem();  // (copies into the ring come behind what was written there by ordinary stores)
+  __syncthreads();           // (the ring is free again)
   if (blockIdx.x == 0 && tid == 0) p.parts.counts[0] = share.total, p.parts.counts[1] = share.parts;
   const bool works = static_cast<int>(blockIdx.x) < share.parts;
   const int group = p.shape.group;

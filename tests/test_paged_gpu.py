@@ -757,3 +757,14 @@ def test_int8_narrow_and_wide_items_in_turn(cuda, x, dim):
         assert torch.equal(mq.paged_attention(q, batch.cache(), *batch.where(), max_new=64), out)
     assert mq.device_status() == 0
     batch.check(out, q, dim ** -0.5)
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("batch,new", [(161, 1), (320, 1), (321, 3), (512, 6), (513, 40), (1025, 9)])
+def test_more_sequences_than_threads_that_find_the_shares(cuda, cache, x, batch, new):
+    """Shares are found by 160 threads (few rows) or 512 (tiles), which go through the sequences in turns, and twice through more
+    of them than threads; what they leave in shared memory is where a CTA's first keys come to lie."""
+    rng = np.random.default_rng(batch)
+    sizes = [(n, n + int(rng.integers(0, 90))) for n in (int(rng.integers(0, new + 1)) for _ in range(batch))]
+    sizes[0], sizes[batch // 2], sizes[-1] = (new, new + 700), (0, 50), (new, new + 900)
+    attend(Batch(cuda, sizes, 2, 16, 64, cache), 8, x, max_new=new)
