@@ -69,7 +69,7 @@ MQ_API int mq_version(void);
  * selection, 18 norms, 21-23 attention. Others report data instead: 8 an expert id out of range, 9 more pairs than a rank's
  * capacity, 15 a beam with a NaN or +inf logit, 16 a parent out of range, 19 a page outside its pool, 20 a length out of range,
  * 24 a row of logits that is no distribution, 25 a drafted token or number of drafts out of range, 26 a sequence with more new
- * tokens than the call said. The first code of either kind stays until it is reset,
+ * tokens than the call said, 27 starts that pass the rows. The first code of either kind stays until it is reset,
  * so a caller who expects such data resets the word to see what comes later. */
 MQ_API int mq_device_status(int reset, void *stream);
 
@@ -444,7 +444,9 @@ typedef struct mq_kv_pages {
  * (starts: int32 [batch + 1], rising; NULL: row b, one each) and lengths[b] positions in the cache, the new ones among them, so
  * that its row i of n is position lengths[b] - n + i. table: int32 [batch][width], ldt elements from row to row; only the
  * entries of positions below lengths[b] are read. All of these are device memory, read when the kernels run. Rows before
- * starts[0] and behind starts[batch] are left as they are. A table entry outside the pool is reported (mq_device_status 19): its
+ * starts[0] and behind starts[batch] are left as they are. Starts that pass the tokens are reported (mq_device_status 27): the rows that
+ * are there keep their positions, the others are left out. (mq_paged_attention alone takes an end so far behind the rows that
+ * none of them would have a position, as 2^31 - 1, for theirs, and does not report it.) A table entry outside the pool is reported (19): its
  * rows are not written, and read as zeros. A length below 0 or above width * page is reported (20) and cut. A position below 0
  * (more rows than positions) is not stored, loads as zeros and sees nothing. */
 

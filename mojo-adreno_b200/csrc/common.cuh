@@ -166,6 +166,7 @@ enum : int {
   kStatusBeamBadParent = 16,  // a parent outside [0, beams): its beam kept its own state
   kStatusKvBadPage = 19,      // a table entry outside the pool: its rows were not written, or read as zeros
   kStatusKvBadLength = 20,    // a length below 0 or beyond its row of the table: cut to that
+  kStatusKvBadStarts = 27,    // starts that pass the rows: those that are there kept their positions
   kStatusAttnLoadWait = 21,
   kStatusAttnMmaWait = 22,
   kStatusAttnSoftmaxWait = 23,

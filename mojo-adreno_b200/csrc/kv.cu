@@ -90,7 +90,9 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
     if (p.seqs.starts) {
       // The last sequence that starts at the token or before it (empty ones end there too, and come before).
       int lo = 0, hi = p.seqs.batch;  // starts[lo] <= token < starts[hi], if the starts rise
-      if (p.seqs.starts[0] <= token && token < p.seqs.starts[hi]) {
+      const int end = p.seqs.starts[hi];
+      if (end > p.seqs.tokens) raise_status(kStatusKvBadStarts);
+      if (p.seqs.starts[0] <= token && token < end) {
         while (hi - lo > 1) {
           const int mid = (lo + hi) / 2;
           if (p.seqs.starts[mid] <= token)
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
       }
     }
     if (b >= 0) {
-      const Seq s = sequence(p.seqs, b);
+      const Seq s = sequence<false>(p.seqs, b);
       const int i = token - s.first, position = s.pos0 + i;
       if (i < 0 || i >= s.n) {  // starts that do not rise
       } else if (position >= 0 && position < s.length) {

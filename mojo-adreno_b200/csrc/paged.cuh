@@ -2,8 +2,8 @@
 // sequences, their pages and the split of a launch's work.
 //
 // Sequence b has rows starts[b] .. starts[b + 1] of the tokens (row b where starts is NULL) and lengths[b] positions in
-// the cache, its new tokens' among them: row i of n is position lengths[b] - n + i. Position p lies in page
-// table[b][p / page], row p % page.
+// the cache, its new tokens' among them: row r is position lengths[b] - (starts[b + 1] - r), whether or not all of these rows
+// are there. Position p lies in page table[b][p / page], row p % page.
 #pragma once
 #include <algorithm>
 
@@ -27,18 +27,29 @@ struct Seq {
   int pos0;      // position of its first row; negative where it has more rows than positions
 };
 
-// starts that fall or pass the tokens and lengths that pass the table are cut to what is there.
+// Rows that are not there (before the first, behind the last: reported) are left out, the others keep their positions. FAR_END:
+// an end so far behind the rows that none of them would have a position counts as theirs. Starts that fall make an
+// empty sequence; lengths that pass the table are cut to it (reported).
+template <bool FAR_END>
 __device__ __forceinline__ Seq sequence(const Seqs &s, int b) {
   Seq q;
-  q.first = b, q.n = 1;
-  if (s.starts) {
-    q.first = min(max(s.starts[b], 0), s.tokens);
-    q.n = min(max(s.starts[b + 1], q.first), s.tokens) - q.first;
-  }
   const int length = s.lengths[b], most = s.width << s.page_log2;
   q.length = min(max(length, 0), most);
   if (q.length != length) raise_status(kStatusKvBadLength);
-  q.pos0 = q.length - q.n;
+  q.first = b, q.n = 1, q.pos0 = q.length - 1;
+  if (s.starts) {
+    q.first = min(max(s.starts[b], 0), s.tokens);
+    int end = max(s.starts[b + 1], q.first);
+    q.n = min(end, s.tokens) - q.first;
+    if (end > s.tokens) {
+      if (FAR_END && q.n > 0 && end - s.tokens >= q.length)
+        end = s.tokens;
+      else
+        raise_status(kStatusKvBadStarts);
+    }
+    // (The bound keeps what is added to and taken from it in range; it is below 0 as far as there are rows.)
+    q.pos0 = max(q.length - (end - q.first), -(1 << 30));
+  }
   return q;
 }
 
@@ -225,13 +236,13 @@ __device__ __forceinline__ void find_share(const Seqs &s, const Shape &a, ShareS
       int64_t cost = 0;
       if (kOneTile) {
         if (base + tid < s.batch) {
-          const Seq q = own = sequence(s, base + tid);
+          const Seq q = own = sequence<true>(s, base + tid);
           if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
           if (takes_part(q, a)) cost = static_cast<int64_t>(G::EXTRA + tile_range<G>(q, a, 0).blocks) * a.kv_heads;
         }
       } else {  // a warp for a sequence, its lanes for the tiles
         for (int b = warp; b < min(THREADS, s.batch - base); b += kWarps) {
-          const Seq q = sequence(s, base + b);
+          const Seq q = sequence<true>(s, base + b);
           int64_t units = 0;
           if (static_cast<int64_t>(q.n) * a.group > a.rows_most) raise_status(kStatusAttnTooManyRows);
           if (takes_part(q, a))
@@ -281,10 +292,10 @@ __device__ __forceinline__ void find_share(const Seqs &s, const Shape &a, ShareS
             rest -= head * per_head;
             Seq q = own;
             q.first = __shfl_sync(0xffffffffu, q.first, from), q.n = __shfl_sync(0xffffffffu, q.n, from);
-            q.length = __shfl_sync(0xffffffffu, q.length, from), q.pos0 = q.length - q.n;
+            q.length = __shfl_sync(0xffffffffu, q.length, from), q.pos0 = __shfl_sync(0xffffffffu, q.pos0, from);
             int tile = 0;
             if (!kOneTile) {
-              q = sequence(s, b);
+              q = sequence<true>(s, b);
               for (const int tiles = tiles_of<G>(q, a);; tile += 32) {
                 const int t = tile + lane;
                 const int64_t units = t < tiles ? G::EXTRA + tile_range<G>(q, a, t).blocks : 0;
@@ -342,7 +353,7 @@ struct Walk {
       tile = 0;
       if (++head == a.kv_heads) {
         head = 0;
-        do s = sequence(q, ++b);
+        do s = sequence<true>(q, ++b);
         while (!takes_part(s, a));  // (units are left, so such a sequence follows)
         tiles = tiles_of<G>(s, a);
       }

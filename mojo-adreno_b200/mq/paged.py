@@ -4,7 +4,8 @@ The reference's attention reads one contiguous cache of one sequence. Here a cac
 share: sequence b keeps position p in page table[b, p // page], row p % page. The operators take a batch's
 new tokens (a prompt, a chunk of one, drafted tokens, one token each) behind one another: sequence b has rows
 starts[b] .. starts[b + 1], and lengths[b] positions in the cache with them, so that its row i of n is position
-lengths[b] - n + i. Table, lengths and starts are int32 on the device and are never read on the host.
+lengths[b] - n + i, n = starts[b + 1] - starts[b]. Starts that pass the rows are reported (device_status() 27) and those that
+are there keep their positions. Table, lengths and starts are int32 on the device and are never read on the host.
 """
 import ctypes
 

@@ -768,3 +768,83 @@ def test_more_sequences_than_threads_that_find_the_shares(cuda, cache, x, batch,
     sizes = [(n, n + int(rng.integers(0, 90))) for n in (int(rng.integers(0, new + 1)) for _ in range(batch))]
     sizes[0], sizes[batch // 2], sizes[-1] = (new, new + 700), (0, 50), (new, new + 900)
     attend(Batch(cuda, sizes, 2, 16, 64, cache), 8, x, max_new=new)
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("held,rows", [([(3, 10)], 2), ([(1, 5), (4, 40), (3, 9)], 7), ([(2, 7), (5, 60), (4, 8), (1, 3)], 4),
+                                       ([(150, 200), (40, 300)], 170), ([(90, 80), (300, 295)], 100), ([(4, 6), (9, 9)], 4)])
+def test_starts_that_pass_the_rows(cuda, cache, x, held, rows):
+    """The rows that are there keep their positions; the others are left out, and the status says so."""
+    batch = Batch(cuda, held, 2, 16, 64, cache)
+    full = [torch.randn(batch.tokens, 2, 64, generator=batch.g, device=cuda).to(x) for _ in range(2)]
+    q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).to(x)
+    before = [t.clone() for t in (batch.k, batch.v)]
+    mq.device_status()
+    got = mq.paged_attention(q[:rows].clone(), batch.cache(), *batch.where())
+    assert mq.device_status() == 27
+    want = mq.paged_attention(q, batch.cache(), *batch.where())
+    batch.check(want, q, 64 ** -0.5)
+    short = Batch.__new__(Batch)  # the rows that are there, by the oracle: each sequence's, at positions counted from its whole end
+    short.__dict__.update(batch.__dict__)
+    for b, (n, length) in enumerate(held):
+        s0, s1 = batch.np_starts[b], min(batch.np_starts[b + 1], rows)
+        if s1 > s0:
+            # (a sequence that is cut to the positions of its rows holds the same for them)
+            short.sizes, short.np_starts = [(s1 - s0, length - n + s1 - s0)], [s0, s1]
+            short.held = lambda _, upto, b=b: batch.held(b, upto)
+            if length - n + s1 - s0 > 0:
+                short.check(got, q[:rows], 64 ** -0.5)
+            else:
+                assert (got[s0:s1] == 0).all()
+    lk, lv = mq.kv_load(batch.cache(), *batch.where(), tokens=rows, dtype=x)
+    assert mq.device_status() == 27
+    ak, av = mq.kv_load(batch.cache(), *batch.where(), tokens=batch.tokens, dtype=x)
+    assert torch.equal(lk, ak[:rows]) and torch.equal(lv, av[:rows])
+    mq.kv_store(full[0][:rows], full[1][:rows], batch.cache(), *batch.where())
+    assert mq.device_status() == 27
+    lk, lv = mq.kv_load(batch.cache(), *batch.where(), tokens=batch.tokens, dtype=x)
+    assert mq.device_status() == 0
+    places = paged.places(batch.np_starts, [length for _, length in held], batch.tokens)
+    real = torch.tensor([p >= 0 for _, p in places], device=cuda)
+    if cache != S8:
+        assert torch.equal(lk[:rows][real[:rows]], full[0][:rows][real[:rows]]) and torch.equal(lv[:rows][real[:rows]], full[1][:rows][real[:rows]])
+    else:  # (half a step of the row's largest over 127, and the rounding to x)
+        for a, b in ((lk, full[0]), (lv, full[1])):
+            b = b[:rows][real[:rows]].double()
+            tol = b.abs().amax(-1, keepdim=True) / 254 * 1.001 + UNIT[x] * b.abs().amax(-1, keepdim=True)
+            assert ((a[:rows][real[:rows]].double() - b).abs() <= tol).all()
+    assert torch.equal(lk[rows:], ak[rows:]) and torch.equal(lv[rows:], av[rows:])
+    # All that no row belongs to is as it was.
+    for t, old in zip((batch.k, batch.v), before):
+        for (b, p), there in zip(places, range(batch.tokens)):
+            if there < rows and p >= 0:
+                page = int(batch.np_table[b, p // 16])
+                old[page, :, p % 16] = t[page, :, p % 16]
+        assert torch.equal(t.view(torch.uint8) if cache == S8 else t.view(torch.int16), old.view(torch.uint8) if cache == S8 else old.view(torch.int16))
+
+
+def test_starts_far_behind_the_rows(cuda):
+    """An end that would leave no row a position is the rows' end to the attention; the copies leave such rows out, and say so."""
+    batch = Batch(cuda, [(3, 40), (5, 60)], 2, 16, 64, F16)
+    q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).half()
+    for end in (8 + 60, 10 ** 6, 2 ** 31 - 1):
+        starts = torch.tensor([-2 ** 31, 3, end], dtype=torch.int32, device=cuda)
+        mq.device_status()
+        want = mq.paged_attention(q, batch.cache(), *batch.where())
+        assert torch.equal(mq.paged_attention(q, batch.cache(), batch.table, batch.lengths, starts), want)
+        assert mq.device_status() == 0
+        before = [batch.k.clone(), batch.v.clone()]
+        kv = torch.randn(8, 2, 64, generator=batch.g, device=cuda)
+        mq.kv_store(kv, kv, batch.cache(), batch.table, batch.lengths, starts)
+        assert mq.device_status() == 27
+        k, v = mq.kv_load(batch.cache(), batch.table, batch.lengths, starts, tokens=8)
+        assert mq.device_status() == 27
+        assert torch.equal(k[:3], kv[:3].half()) and torch.equal(v[:3], kv[:3].half()) and (k[3:] == 0).all() and (v[3:] == 0).all()
+        for j in range(40, 60):
+            page = int(batch.np_table[1, j // 16])
+            assert torch.equal(batch.k[page, :, j % 16], before[0][page, :, j % 16])
+    starts = torch.tensor([0, 3, 8 + 59], dtype=torch.int32, device=cuda)  # the last row's position is 0
+    got = mq.paged_attention(q, batch.cache(), batch.table, batch.lengths, starts)
+    assert mq.device_status() == 27
+    first = batch.v[int(batch.np_table[1, 0]), :, 0].repeat_interleave(4, 0)
+    assert (got[3:7] == 0).all() and torch.equal(got[7], first)
