@@ -149,13 +149,18 @@ def kv_store(k, v, cache, table, lengths, starts=None):
 
 def kv_load(cache, table, lengths, starts=None, k=None, v=None, tokens=None, dtype=torch.float16):
     """(k, v) [tokens, kv_heads, dim]: what the pages hold of the positions that kv_store would write. k, v: fp32, fp16 or
-    bf16, made of `dtype` if None, with as many rows as `tokens` (None: one per sequence)."""
+    bf16, made of `dtype` if None, with as many rows as `tokens` (None: one per sequence, and with starts, whose end is on the
+    device, to be said)."""
     device = _here(cache)
     p = cache._pages
     if k is None or v is None:
         if tokens is None:
             have = k if k is not None else v
-            tokens = have.shape[0] if have is not None else table.shape[0]
+            if have is None and starts is not None:
+                raise MQError(-1, "tokens: with starts, say how many rows there are (or give k or v)")
+            if not isinstance(table if have is None else have, torch.Tensor):
+                raise MQError(-1, "table, k, v: expected a torch.Tensor")
+            tokens = (table if have is None else have).shape[0]
         shape = (tokens, p.heads, p.dim)
         kind = k.dtype if k is not None else v.dtype if v is not None else dtype
         k = torch.empty(shape, dtype=kind, device=cache.k.device) if k is None else k

@@ -848,3 +848,18 @@ def test_starts_far_behind_the_rows(cuda):
     assert mq.device_status() == 27
     first = batch.v[int(batch.np_table[1, 0]), :, 0].repeat_interleave(4, 0)
     assert (got[3:7] == 0).all() and torch.equal(got[7], first)
+
+
+def test_load_with_starts_needs_the_number_of_rows(cuda):
+    """Without it there was one row per sequence, of positions that the starts do not mean."""
+    batch = Batch(cuda, [(3, 10), (2, 20)], 2, 16, 64, F16)
+    with pytest.raises(mq.MQError, match="tokens"):
+        mq.kv_load(batch.cache(), *batch.where())
+    with pytest.raises(mq.MQError, match="table"):
+        mq.kv_load(batch.cache(), None, batch.lengths)
+    want = mq.kv_load(batch.cache(), *batch.where(), tokens=5)
+    for kw in (dict(k=torch.empty_like(want[0])), dict(v=torch.empty_like(want[1])), dict(k=torch.empty_like(want[0]), v=torch.empty_like(want[1]))):
+        got = mq.kv_load(batch.cache(), *batch.where(), **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    k, v = mq.kv_load(batch.cache(), batch.table, batch.lengths)  # each one's last position
+    assert torch.equal(k, want[0][[2, 4]]) and torch.equal(v, want[1][[2, 4]])
