@@ -38,10 +38,12 @@ constexpr int kMaxDrafts = 32, kMaxSplits = 64;
 constexpr float kLeastTemperature = 1e-5f;   // below: 0
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
-// As many CTAs as run at once, a step of each at least.
+// CTAs of a scan that run at once: eight on each of 148 SMs.
+constexpr int kScanCtas = 148 * 8;
+// As many CTAs as run at once, a step of each at least. rows * splits is at most the larger of rows and kScanCtas.
 __host__ __device__ constexpr int splits_for(int64_t rows, int64_t vocab) {
   const int64_t steps = (vocab * 4 + kScan * kVecs * 16 - 1) / (kScan * kVecs * 16);
-  int64_t s = 148 * 8 / rows;
+  int64_t s = kScanCtas / rows;
   if (s > kMaxSplits) s = kMaxSplits;
   if (s > steps) s = steps;
   return s < 1 ? 1 : static_cast<int>(s);
@@ -557,8 +559,8 @@ inline bool sizes_fit(int64_t batch, int64_t drafts, int64_t vocab) {
 extern "C" size_t mq_verify_workspace_size(int64_t batch, int64_t drafts, int64_t vocab) {
   using namespace mq::verify;
   if (batch <= 0 || !sizes_fit(batch, drafts, vocab)) return 0;
-  const int64_t rows = batch * (2 * drafts + 1);  // (without draft logits there are fewer rows, with more splits)
-  return sizeof(float2) * std::max(rows * splits_for(rows, vocab), batch * (drafts + 1) * splits_for(batch * (drafts + 1), vocab));
+  // What rows * splits can be, not what it is: that falls and rises with the rows, and a larger call's workspace serves a smaller one.
+  return sizeof(float2) * std::max<int64_t>(batch * (2 * drafts + 1), kScanCtas);
 }
 
 extern "C" int mq_verify_drafts(const void *target, int64_t ld_target, const void *draft, int64_t ld_draft, int dtype,

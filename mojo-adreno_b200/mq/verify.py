@@ -13,7 +13,7 @@ _I32 = frozenset((torch.int32,))
 
 
 def verify_workspace(batch, drafts, vocab):
-    """The bytes of a workspace for verify_drafts."""
+    """The bytes of a workspace for verify_drafts; enough for fewer requests, drafts or tokens too."""
     return max(lib.mq_verify_workspace_size(batch, drafts, vocab), 16)
 
 

@@ -140,3 +140,22 @@ def test_python_operators_refuse_cpu_tensors():
         mq.verify_drafts(torch.zeros(4, 10), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, 4))
     with pytest.raises(mq.MQError, match="PagedCache"):
         mq.kv_store(x[0], x[0], None, None, None)
+
+
+def test_verify_workspace_of_a_larger_call_is_enough():
+    """Sizes never fall when a call has more requests, drafts or tokens, and hold a pair of fp32 for each CTA of the scan: as many per
+    row as let eight run on each of 148 SMs, 64 at most, and one step of 16 KB of fp32 each."""
+    from mq._lib import lib
+
+    def needs(rows, vocab):
+        return 8 * rows * max(1, min(64, 148 * 8 // rows, -(-vocab * 4 // (256 * 4 * 16))))
+
+    for vocab in (1, 100, 4096, 32000, 128256, 151669, 262144, 1 << 20):
+        for drafts in (0, 1, 2, 4, 8, 32):
+            largest = 0
+            for batch in list(range(1, 140)) + [250, 591, 592, 593, 1183, 1184, 1185, 5000, 1 << 20]:
+                size = lib.mq_verify_workspace_size(batch, drafts, vocab)
+                assert size >= largest and size >= needs(batch * (2 * drafts + 1), vocab) and size >= needs(batch * (drafts + 1), vocab)
+                assert size >= lib.mq_verify_workspace_size(batch, max(drafts - 1, 0), vocab)
+                assert size >= lib.mq_verify_workspace_size(batch, drafts, max(vocab // 3, 1))
+                largest = size

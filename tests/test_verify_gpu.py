@@ -310,3 +310,14 @@ def test_refusals(cuda):
             target=torch.zeros(68, 100, device=cuda), draft=None)
     with pytest.raises(mq.MQError, match="CUDA"):
         mq.verify_drafts(case.target.cpu(), case.drafted, case.uniform)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+def test_workspace_of_a_larger_batch_serves(cuda, draft):
+    """A server has one of its largest batch. What the call leaves alone behind it stays as it was."""
+    work = torch.empty(mq.verify_workspace(64, 4, 40009) + 64, dtype=torch.uint8, device=cuda)
+    for batch in (1, 5, 7, 8, 9, 10, 11, 13, 18, 21, 64):
+        case = Case(cuda, batch, 4, 40009, F16, draft, [1.0, 0.0], seed=batch)
+        work.fill_(0x5a)
+        case.check(case.call(workspace=work[:-64]))
+        assert (work[-64:] == 0x5a).all()
