@@ -487,8 +487,9 @@ MQ_API int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, int64
  * Which of a request's drafted tokens stay, so that the tokens are distributed as the target's own samples. p_i and q_i:
  * softmax(logits / temperature[b]) of row i of the request's target rows [drafts + 1] and draft rows [drafts] (draft NULL: q_i is
  * all on the drafted token). Token i is kept while uniform[b][i] * q_i(token) < p_i(token). At the first that is not, i = n, a token is
- * drawn from max(p_n - q_n, 0) (where all are kept, from p_n; where nothing is left of it, from p_n): the first v whose running sum
- * exceeds uniform[b][drafts] times the whole (sums in fp64). A temperature below 1e-5 (or NaN): p_i is all on the largest logit, the
+ * drawn from max(p_n - q_n, 0) (where all are kept, from p_n; where less than 1e-13 is left of it, which is rounding, from p_n): the
+ * first v whose running sum exceeds uniform[b][drafts] times the whole (sums in fp64). Without draft logits, and with all of p_n on
+ * the drafted token, no other is left: the token is -1. A temperature below 1e-5 (or NaN): p_i is all on the largest logit, the
  * lowest index among equal ones, and the draft's logits and the uniforms do not count.
  * tokens[b]: the kept ones, the drawn one, then -1; accepted[b] = n; logprobs[b][i] = log p_i(tokens[b][i]), 0 behind.
  * temperature: fp32 [batch] or NULL (1); above 1e30 it counts as 1e30. counts: int32 [batch] or NULL, how many drafts request b has (<= drafts; outside

@@ -36,6 +36,9 @@ constexpr int kClusterFew = 16, kCluster = 8;
 constexpr int kDrawFew = 512, kDrawMany = 256, kFewRequests = 12, kManyRequests = 148 * 2 / kCluster;
 constexpr int kMaxDrafts = 32, kMaxSplits = 64;
 constexpr float kLeastTemperature = 1e-5f;   // below: 0
+// Less than this of p - q is nothing: equal distributions leave the roundings of their terms, 1e-14 in all (of two rows with the
+// same bits 1e-17: one product is rounded before the other is taken off it, in one operation).
+constexpr double kNothingLeft = 1e-13;
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
 // CTAs of a scan that run at once: eight on each of 148 SMs.
@@ -392,8 +395,8 @@ __global__ void __launch_bounds__(kDraw, 1024 / kDraw) verify_draw_kernel(const 
       sweep(std::false_type(), [&](int v, float x, float) { w += v == without ? 0.0 : ep(x); });
     if (round) sync_cluster();  // (everybody has read the first round's sums)
     whole = gather(2, w);
-    if (whole > 0 || !rest) break;
-    rest = false;  // p and q are one: what is left is rounding, so the draw is from p
+    if (whole > kNothingLeft || !rest) break;
+    rest = false;  // p and q are one, so the draw is from p
   }
   const double goal = p.uniform[out0 + p.drafts] * whole;
   // The first stretch whose running sum passes the goal, else the last that has any weight.

@@ -321,3 +321,30 @@ def test_workspace_of_a_larger_batch_serves(cuda, draft):
         work.fill_(0x5a)
         case.check(case.call(workspace=work[:-64]))
         assert (work[-64:] == 0x5a).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch", [2, 20, 40])
+@pytest.mark.parametrize("shift", [0.0, 64.0, -32.0])
+def test_equal_distributions_draw_from_the_target(cuda, dtype, batch, shift):
+    """A token that neither can give is drafted, so it is not kept, and nothing is left of p - q: the draw is from p. The logits are whole
+    numbers, and the draft's a constant above them (the same probabilities)."""
+    vocab = 20000
+    case = Case(cuda, batch, 2, vocab, dtype, True, [1.0, 0.7], seed=batch)
+    z = case.target.view(batch, 3, vocab)
+    z.copy_((z.float() * 2).round().clamp(-INF, 12))
+    z[..., 3] = -INF
+    case.draft = (z[:, :2].float() + shift).to(dtype).reshape(batch * 2, vocab).contiguous()
+    case.drafted[:, 0] = 3
+    got = case.call()
+    assert (got[1] == 0).all()
+    case.check(got)
+
+
+def test_equal_distributions_and_a_uniform_of_one(cuda):
+    case = Case(cuda, 8, 1, 4000, F32, True)
+    case.draft = case.target.view(8, 2, 4000)[:, 0].contiguous()
+    case.uniform[:, 0] = 1.0
+    got = case.call()
+    assert (got[1] == 0).all()
+    case.check(got)
