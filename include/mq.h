@@ -453,8 +453,8 @@ typedef struct mq_kv_pages {
 /* k[t][h], v[t][h] -> the pages, rounded to their type; int8 as mq_quantize_s8 makes it, row by row (a row with a NaN or an
  * infinity: zeros and scale NaN). k, v: fp32, fp16 or bf16 (dtype), [tokens][heads][dim] with strides in elements, rows
  * 16-byte aligned. A position that two rows name (of sequences that share a page) gets either's
- * values, or a mix of the two, unless they are equal. Keys' and values' pages must not share memory (refused where they have one
- * layout), nor the rows with the pages. */
+ * values, or a mix of the two, unless they are equal. Keys' and values' pages must not share memory, nor their scales (refused where
+ * they have one layout), nor the rows with the pages. */
 MQ_API int mq_kv_store(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
                        int dtype, const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width,
                        const int32_t *lengths, const int32_t *starts, int64_t batch, int64_t tokens, void *stream);

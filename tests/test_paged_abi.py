@@ -25,6 +25,14 @@ def status(name, *args):
     return rc, lib.mq_last_error().decode()
 
 
+def without_device():
+    """For calls that the checks let pass: with a device they would go on to addresses that are none."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("needs a machine without a GPU")
+
+
 def attention(cache=None, **kw):
     a = dict(q=OK, q_dtype=1, q_token=512, q_head=64, table=OK, ldt=4, width=4, lengths=OK, starts=OK, batch=2, tokens=5, heads=8,
              scale=0.125, window=0, max_new=0, out=OK, o_token=512, o_head=64, workspace=OK, size=16)
@@ -159,3 +167,19 @@ def test_verify_workspace_of_a_larger_call_is_enough():
                 assert size >= lib.mq_verify_workspace_size(batch, max(drafts - 1, 0), vocab)
                 assert size >= lib.mq_verify_workspace_size(batch, drafts, max(vocab // 3, 1))
                 largest = size
+
+
+@pytest.mark.parametrize("shift,stride,refused", [(0, (32, 16, 1), True), (4, (32, 16, 1), True), (4 * 255, (32, 16, 1), True), (4 * 256, (32, 16, 1), False),
+                                                  (-4 * 255, (32, 16, 1), True), (-4 * 256, (32, 16, 1), False), (64, (64, 32, 1), False),
+                                                  (68, (64, 32, 1), True), (4, (64, 32, 2), False), (8, (64, 32, 2), True), (0, (1, 8, 16), True)])
+def test_store_where_scales_share_memory(shift, stride, refused):
+    """v_scale `shift` bytes behind k_scale, both of 8 pages of 2 x 16 fp32: side by side or between one another they may lie."""
+    without_device()
+
+    def store(dtype):
+        c = pages(v=OK + (1 << 16), dtype=dtype, k_scale=OK, v_scale=OK + shift, ks_stride=stride, vs_stride=stride)
+        return status("mq_kv_store", OK, 128, 64, OK, 128, 64, 1, ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, None)
+
+    rc, msg = store(3)
+    assert ("share memory" in msg and rc == -1) if refused else rc != -1, msg
+    assert store(1)[0] != -1  # (a 16-bit cache has none)
