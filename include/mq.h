@@ -469,8 +469,7 @@ MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ld
  * q's own buffer with q's strides. A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
  * row does not see have no influence on it, whatever they hold; one that it sees and whose row holds a NaN or an infinity (int8: whose scale is one) makes
  * it NaN or infinite. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they
- * meet the values; bf16 rows of more than 16 per kv head and sequence (or of drafted tokens) meet an int8 cache as fp16 operands,
- * each integer times its scale over the largest of 32 keys, rounded. An int8 cache's scales must not be negative, and a value
+ * meet the values; an int8 cache's integers are multiplied as they are, its scales in fp32. An int8 cache's scales must not be negative, and a value
  * scale below 1e-30 counts as 1e-30.
  * max_new: no sequence has more new tokens (0: unknown); one that has is reported (26) and its rows are left as they are.
  * scale > 0. Reproducible bit for bit. workspace: mq_paged_attention_workspace_size() bytes, 16-byte aligned (0 for sizes that

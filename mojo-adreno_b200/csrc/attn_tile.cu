@@ -12,14 +12,16 @@
 //    lane per page (or part of one) and 128 bytes of row. Warps 9 and 10: a thread each issues the MMAs of an accumulator. Warps
 //    12 to 15: bring q, and stand between the copies and the MMAs: of an int8 cache they make fp16 of every block; of a 16-bit one
 //    they take what is no number out of the values of the blocks that some row sees only in part, and say which keys had any.
+//  * An int8 cache's scales meet the scores and weights in fp32 (attn.cu), three numbers per key and row from shared memory. In the
+//    operands, as fp16(integer * scale / the largest of 32 keys), they would take less (2048 of 30,001 tokens: 1244 us, 1340 here;
+//    2048 of 2048: 125, 119 here), but a ratio's rounding is common to all terms of a score, and a scale far above its neighbours'
+//    takes their bits. Error beside the bf16 output's own rounding: 0.0012 so, 0.00015 here.
 //  * One persistent CTA per SM, all of TMEM, equal shares of the blocks: causal or ragged, no SM waits for another.
 //
 // 8192 tokens, 32 heads on 8 of 128, bf16: 535-620 us, 0.9-1.03 PFLOP/s (0.53-0.61 of the measured burst, 0.63-0.72 of the
 // sustained rate; power caps the clock). A step of both accumulators takes some 2000 cycles where its MMAs take 1280 and its
 // exponentials 1024: what is left over is waiting between the two. Short calls are latency: 431 tokens 22 us; a traced
 // run had 2.8 for the shares, 3.8 more until the first scores, 3.0 for one to four steps, 2.6 for the output, then the join.
-#include <type_traits>
-
 #include "paged.cuh"
 
 namespace mq {
@@ -33,15 +35,9 @@ constexpr int kTileRegs = 128, kSoftmaxRegs = 152, kOtherRegs = 104;
 static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kTileThreads * kTileRegs, "more registers than the block was launched with");
 constexpr int kStageBytes = 2048;  // per softmax warp: 64 bytes of each of its rows on their way out
 
-// An int8 cache's kinds here. Exact: the integers are the operands, the keys' and values' scales meet the scores and weights
-// (attn.cu). Folded, for bf16 rows: the operands are fp16, integer * scale / (the largest scale of 32 keys), rounded (2^-11 twice, a
-// quarter of what bf16 rounds), so the softmax has one factor for 32 scores and one for their weights where the exact one reads
-// three numbers per key and row from shared memory (2048 of 30000 tokens: 1200-1270 us instead of 1440). A block that some row sees
-// only in part is exact there too: a scale that a row does not see does not touch what it sees.
-constexpr int kFolded = 16;
 template <int D, int KIND>
 struct Tile {
-  static constexpr bool kFold = KIND == kFolded, kS8 = KIND == MQ_S8 || kFold;
+  static constexpr bool kS8 = KIND == MQ_S8;
   static constexpr int kBlock = kTileKeys * D * 2;          // of keys or values, as operands
   static constexpr int kSlots = kS8 ? 3 : 4;                // keys and values in turn
   static constexpr int kRaw = kS8 ? kTileKeys * D : 0;      // int8 as it was copied, two of them
@@ -121,7 +117,7 @@ template <int D, int KIND>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attn_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
   using T = Tile<D, KIND>;
-  constexpr bool BF = KIND == MQ_BF16, S8 = T::kS8, Fold = T::kFold, Exact = S8 && !Fold;  // (both int8 kinds multiply fp16)
+  constexpr bool BF = KIND == MQ_BF16, S8 = T::kS8;
   constexpr int NS = T::kSlots, NF = S8 ? 2 : NS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *q_tile = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -432,17 +428,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             sv = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
           }
         }
-        float most_k = fabsf(sk) < INFINITY ? sk : 0.f, most_v = fabsf(sv) < INFINITY ? sv : 0.f;  // of the warp's 32 keys
-        const bool edge = key0 + kTileKeys > part_hi || key0 < part_lo, exact = Exact || (Fold && edge);
-        if (Fold && !edge) {
-#pragma unroll
-          for (int o = 16; o; o >>= 1) {
-            most_k = fmaxf(most_k, __shfl_xor_sync(0xffffffffu, most_k, o));
-            most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, o));
-          }
-          if (!(most_k > 0.f)) most_k = 1.f;
-          most_v = fmaxf(most_v, kLeastScale);
-        }
+        const bool edge = key0 + kTileKeys > part_hi || key0 < part_lo;
         for (int which = 0; which < 2; ++which, ++n) {
           const int src = static_cast<int>(n % NF), slot = static_cast<int>(n % NS);
           ok = warp_wait(&full[src], (n / NF) & 1, kStatusAttnLoadWait);
@@ -451,18 +437,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           uint8_t *dst = ring + slot * T::kBlock;
           if constexpr (S8) {
             const uint8_t *from = raw + src * T::kRaw;
-            __half2 f2 = __float2half2_rn(1.f);
             if (which == 0) {
               // (the softmax has read block n / 2 - 2's by now: the slot just waited for came behind its weights)
               float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
-              if (exact) {
-                const float vs = sv < kLeastScale ? kLeastScale : sv;
-                sc[0][r] = sk, sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
-              } else if (lane == 0) {  // one for the warp's 32 keys
-                sc[0][warp - 12] = most_k, sc[1][warp - 12] = lg2(most_v), sc[2][warp - 12] = __frcp_rn(most_v);
-              }
+              const float vs = sv < kLeastScale ? kLeastScale : sv;
+              sc[0][r] = sk, sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
             }
-            if (!exact) f2 = __float2half2_rn(which == 0 ? sk / most_k : (sv < kLeastScale ? kLeastScale : sv) / most_v);
             uint4 w[D / 16];
 #pragma unroll
             for (int c = 0; c < D / 16; ++c)
@@ -473,12 +453,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               uint32_t o[8];
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[2 * e] = bytes_to_half2<0x4140>(x[e]), o[2 * e + 1] = bytes_to_half2<0x4342>(x[e]);
-              if (!exact)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&o[e]), f2);
-                  o[e] = *reinterpret_cast<const uint32_t *>(&h);
-                }
               *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
               *reinterpret_cast<uint4 *>(dst + swizzled(r, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
             }
@@ -553,29 +527,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_loaded(v[0]);
         tmem_loaded(v[1]);
         const bool edge = block0 + kTileKeys > part_hi || block0 < part_lo;
-        // A score's log2 is scale * s + shift, for each 32 keys: the scale is the row's and, folded, the keys'; the shift the
-        // values'. (Exact: both go into v.)
-        float scale[2] = {p.scale, p.scale}, shift[2] = {0.f, 0.f};
+        // int8: a score's log2, with the values' (attn.cu), from the row's factor and the keys' and values' scales. A 16-bit cache's is
+        // p.scale times it, which the maximum and the exponents apply.
         if constexpr (S8) {
           const float factor = row_factor[(k_item - 1) & 1][row];
           const float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
-          if (Exact || edge) {
-            scale[0] = scale[1] = 1.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][64 * half + 32 * c + e]);
-                const float4 l4 = *reinterpret_cast<const float4 *>(&sc[1][64 * half + 32 * c + e]);
-                mul2(k4.x, k4.y, factor, factor);
-                mul2(k4.z, k4.w, factor, factor);
-                fma2(v[c][e], v[c][e + 1], k4.x, k4.y, l4.x, l4.y);
-                fma2(v[c][e + 2], v[c][e + 3], k4.z, k4.w, l4.z, l4.w);
-              }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) scale[c] = factor * sc[0][2 * half + c], shift[c] = sc[1][2 * half + c];
-          }
+            for (int e = 0; e < 32; e += 4) {
+              float4 k4 = *reinterpret_cast<const float4 *>(&sc[0][64 * half + 32 * c + e]);
+              const float4 l4 = *reinterpret_cast<const float4 *>(&sc[1][64 * half + 32 * c + e]);
+              mul2(k4.x, k4.y, factor, factor);
+              mul2(k4.z, k4.w, factor, factor);
+              fma2(v[c][e], v[c][e + 1], k4.x, k4.y, l4.x, l4.y);
+              fma2(v[c][e + 2], v[c][e + 3], k4.z, k4.w, l4.z, l4.w);
+            }
         }
         if (edge) {
           // The columns that this row sees, a bit each: from lo - key0 up to hi - key0.
@@ -606,8 +573,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int e = 2; e < 16; e += 2) top[c] = max3(top[c], x[e], x[e + 1]);
         }
-        const float most = Fold ? fmaxf(fmaf(fmaxf(top[0], top[1]), scale[0], shift[0]), fmaf(fmaxf(top[2], top[3]), scale[1], shift[1]))
-                                : max3(fmaxf(top[0], top[1]), top[2], top[3]) * scale[0];
+        const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * (S8 ? 1.f : p.scale);
         const bool grows = most > m + 8.f;
         if (__any_sync(0xffffffffu, grows)) {
           const float next = grows ? most : m;
@@ -641,43 +607,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
-          auto weigh = [&](auto exactly) {
-            constexpr bool kExactly = decltype(exactly)::value;
-            const float from = ref + shift[c];
-            float part[2] = {0.f, 0.f};
+          float part[2] = {0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              if (kExactly)
-                add2(v[c][e], v[c][e + 1], ref, ref);
-              else
-                fma2(v[c][e], v[c][e + 1], scale[c], scale[c], from, from);
-              const float a = ex2(v[c][e]), b = ex2(v[c][e + 1]);
-              w[e / 2] = pack16<BF>(a, b);
-              if constexpr (kExactly) {
-                const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][64 * half + 32 * c + e]);
-                if (Fold || edge)  // (a key that the row does not see may have any scale)
-                  add2(part[0], part[1], a == 0.f ? 0.f : a * iv.x, b == 0.f ? 0.f : b * iv.y);
-                else
-                  part[0] = fmaf(a, iv.x, part[0]), part[1] = fmaf(b, iv.y, part[1]);
-              } else if (BF) {  // as they were rounded: the roundings cancel where one key has most of the weight
-                add2(part[0], part[1], __uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xffff0000u));
-              } else {
-                add2(part[0], part[1], a, b);
-              }
-            }
-            if (S8 && !kExactly) part[0] *= scales[(n >> 1) & 1][2][2 * half + c], part[1] *= scales[(n >> 1) & 1][2][2 * half + c];
-            sum[0] += part[0], sum[1] += part[1];
-          };
-          if constexpr (Exact) {
-            weigh(std::true_type());
-          } else if constexpr (Fold) {
-            if (edge)
-              weigh(std::true_type());
+          for (int e = 0; e < 32; e += 2) {
+            if (S8)
+              add2(v[c][e], v[c][e + 1], ref, ref);
             else
-              weigh(std::false_type());
-          } else {
-            weigh(std::false_type());
+              fma2(v[c][e], v[c][e + 1], p.scale, p.scale, ref, ref);
+            const float a = ex2(v[c][e]), b = ex2(v[c][e + 1]);
+            w[e / 2] = pack16<BF>(a, b);
+            if constexpr (S8) {
+              const float2 iv = *reinterpret_cast<const float2 *>(&scales[(n >> 1) & 1][2][64 * half + 32 * c + e]);
+              if (edge)  // (a key that the row does not see may have any scale)
+                add2(part[0], part[1], a == 0.f ? 0.f : a * iv.x, b == 0.f ? 0.f : b * iv.y);
+              else
+                part[0] = fmaf(a, iv.x, part[0]), part[1] = fmaf(b, iv.y, part[1]);
+            } else if (BF) {  // as they were rounded: the roundings cancel where one key has most of the weight
+              add2(part[0], part[1], __uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xffff0000u));
+            } else {
+              add2(part[0], part[1], a, b);
+            }
           }
+          sum[0] += part[0], sum[1] += part[1];
           tmem_st16(at + 16 * c, w);
           if (c == 0 && lane == 0) mbar_arrive(&turn[g ^ 1][warp & 3]);
         }
@@ -847,7 +798,6 @@ int launch_attention(const Plan &plan, const mq_kv_pages *c, AttnParams p, void 
   }
   if (plan.tile_ctas) {
     p.shape.rows_from = plan.few_ctas ? kRowsForTiles : 0, p.shape.rows_to = plan.most_rows;
-    if (KIND == MQ_S8 && p.q_dtype == MQ_BF16) return launch_tile<D, KIND == MQ_S8 ? kFolded : KIND>(c, p, plan.tile_ctas, workspace, s, what);
     return launch_tile<D, KIND>(c, p, plan.tile_ctas, workspace, s, what);
   }
   return MQ_OK;

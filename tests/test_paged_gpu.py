@@ -863,3 +863,75 @@ def test_load_with_starts_needs_the_number_of_rows(cuda):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     k, v = mq.kv_load(batch.cache(), batch.table, batch.lengths)  # each one's last position
     assert torch.equal(k, want[0][[2, 4]]) and torch.equal(v, want[1][[2, 4]])
+
+
+def test_int8_operands_are_the_integers(cuda):
+    """Scores of many terms of one sign, where an error that a key's terms share would show (bf16 rows, most blocks seen by every row).
+    Weights are rounded to fp16, u = 2^-11 at most, u / sqrt(3) in the mean; a score is off by dim 2^-24 of itself, for the fp32
+    sums; an output by those of its terms p_j v_j, root of the sum of squares, within six standard deviations, and by 2^-8 of itself."""
+    n, length, dim, heads = 64, 1000, 128, 8
+    batch = Batch(cuda, [(n, length)], 2, 16, dim, S8)
+    batch.k.copy_(torch.randint(32, 128, batch.k.shape, generator=batch.g, device=cuda, dtype=torch.int32).to(S8))
+    batch.scales[0].uniform_(0.00097, 0.001, generator=batch.g)
+    batch.scales[1].uniform_(0.01, 0.02, generator=batch.g)
+    q = (torch.rand(n, heads, dim, generator=batch.g, device=cuda) + 0.5).bfloat16()
+    scale = 6.0  # scores of 60 or so
+    out = mq.paged_attention(q, batch.cache(), *batch.where(), scale=scale)
+    keys, values, _ = batch.held(0, length)
+    got, rows, u = host(out), host(q), 2.0 ** -11
+    for h in range(heads):
+        k, v = keys[h // 4], values[h // 4]
+        z = scale * rows[:, h] @ k.T
+        assert 40 < z.mean() < 80
+        e2 = (dim * 2.0 ** -24 * z) ** 2
+        z[np.arange(length) > np.arange(length - n, length)[:, None]] = -np.inf
+        p = np.exp(z - z.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        ref = p @ v
+        # (the sum of weights carries the scores' errors as well)
+        sigma = np.sqrt((p ** 2 * (e2 + u * u / 3)) @ v ** 2 + (p ** 2 * e2).sum(1, keepdims=True) * ref ** 2)
+        bad = np.abs(got[:, h] - ref) > 6 * sigma + 2.0 ** -8 * np.abs(ref)
+        assert not bad.any(), (h, int(bad.sum()), float((np.abs(got[:, h] - ref) / sigma).max()))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spike", [4096.0, 2.0 ** 20])
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+def test_int8_one_scale_far_above_its_neighbours(cuda, dim, spike, which):
+    """One key of 32 has a scale `spike` times the others', and (its row being against q) no weight: what the others give must not
+    suffer from it. bf16 rows; the bound is that of an int8 cache at the head of this file, q's conversion being exact here."""
+    n, length, heads = 64, 500, 8
+    batch = Batch(cuda, [(n, length)], 2, 16, dim, S8)
+    q = (torch.rand(n, heads, dim, generator=batch.g, device=cuda) + 0.5).bfloat16()
+    for j in range(5, length, 32):
+        of, row = batch.table[0, j // 16].long(), j % 16
+        batch.k[of, :, row] = -100
+        batch.scales[0][of, :, row] = 0.05 * (spike if "k" in which else 40)
+        if "v" in which:
+            batch.scales[1][of, :, row] = 0.05 * spike
+    scale = dim ** -0.5
+    mq.device_status()
+    got = host(mq.paged_attention(q, batch.cache(), *batch.where()))
+    assert mq.device_status() == 0
+    keys, values, steps = batch.held(0, length)
+    rows = host(q)
+    ref, size, tiny = paged.attention(rows, keys, values, range(length - n, length), scale, 0, steps[1])
+    near = np.ones(length, bool)
+    near[5::32] = False
+    big = scale * np.einsum("thd,hjd->thj", np.abs(rows), np.repeat(np.abs(keys[:, near]), 4, 0)).max(-1)
+    e = (dim + 16) * 2.0 ** -23 * big
+    bound = 2.0 ** -8 * np.abs(ref) + (2 * 2.0 ** -11 + 2 * e + 2.0 ** -19)[..., None] * size + 2.0 ** -25 * tiny
+    assert (np.abs(got - ref) <= bound).all(), float((np.abs(got - ref) / bound).max())
+
+
+@pytest.mark.parametrize("x", [F16, BF16])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_int8_scales_of_zero(cuda, x, which):
+    """Rows that were quantised from zeros, alone and 64 in a row, in blocks that every row sees and in others."""
+    batch = Batch(cuda, [(1, 400), (100, 400), (7, 300)], 2, 16, 64, S8)
+    for b, (n, length) in enumerate(batch.sizes):
+        for j in sorted({*range(1, length, 7), *range(128, 192)}):
+            of = batch.table[b, j // 16].long()
+            (batch.k if which == "k" else batch.v)[of, :, j % 16] = 0
+            batch.scales["kv".index(which)][of, :, j % 16] = 0
+    attend(batch, 8, x)
