@@ -467,8 +467,9 @@ MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ld
  * those before it, the last `window` of them (0: all). Query head h uses kv head h / (heads / cache->heads). q and out: fp16
  * or bf16 (q_dtype; a 16-bit cache's own type), [tokens][heads][dim] with strides in elements, rows 16-byte aligned; out may be
  * q's own buffer with q's strides. A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
- * row does not see have no influence on it, whatever they hold; one that it sees and whose row holds a NaN or an infinity (int8: whose scale is one) makes
- * it NaN or infinite. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they
+ * row does not see have no influence on it, whatever they hold; one that it sees and whose key or value holds a NaN, or its value an
+ * infinity (int8: whose scale is either), makes it NaN or infinite. An infinity in a 16-bit key makes the score one: +infinity makes
+ * the row NaN, a key of score -infinity has no weight. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they
  * meet the values; an int8 cache's integers are multiplied as they are, its scales in fp32. An int8 cache's scales must not be negative, and a value
  * scale below 1e-30 counts as 1e-30.
  * max_new: no sequence has more new tokens (0: unknown); one that has is reported (26) and its rows are left as they are.

@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<D, KIND>::kCtas)
               sk[h] = p.k_scale[of * p.ks_stride[0] + item.head * p.ks_stride[1] + row * p.ks_stride[2]];
               sv[h] = p.v_scale[of * p.vs_stride[0] + item.head * p.vs_stride[1] + row * p.vs_stride[2]];
             }
+            // (An infinite key scale would make a score of minus infinity, so no weight, where the product is negative.)
+            if (!(sk[h] < INFINITY)) sk[h] = NAN;
             if (sv[h] < kLeastScale) sv[h] = kLeastScale;  // (fmaxf would drop a NaN)
           }
         }

@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               // (the softmax has read block n / 2 - 2's by now: the slot just waited for came behind its weights)
               float (&sc)[3][kTileKeys] = scales[(n >> 1) & 1];
               const float vs = sv < kLeastScale ? kLeastScale : sv;
-              sc[0][r] = sk, sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
+              sc[0][r] = sk < INFINITY ? sk : NAN, sc[1][r] = lg2(vs), sc[2][r] = __frcp_rn(vs);
             }
             uint4 w[D / 16];
 #pragma unroll

@@ -935,3 +935,22 @@ def test_int8_scales_of_zero(cuda, x, which):
             (batch.k if which == "k" else batch.v)[of, :, j % 16] = 0
             batch.scales["kv".index(which)][of, :, j % 16] = 0
     attend(batch, 8, x)
+
+
+@pytest.mark.parametrize("x", [F16, BF16])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [5, 200, -3])
+def test_int8_scales_that_are_no_numbers_anywhere(cuda, x, which, value, at):
+    """In blocks that every row sees and in others: the rows that see such a scale are no numbers, the others as without it."""
+    batch = Batch(cuda, [(6, 400), (1, 400), (100, 400), (40, 500)], 2, 16, 64, S8)
+    q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).to(x)
+    clean = mq.paged_attention(q, batch.cache(), *batch.where())
+    for b, (n, length) in enumerate(batch.sizes):
+        j = at % length
+        batch.scales["kv".index(which)][batch.table[b, j // 16].long(), :, j % 16] = value
+    got = mq.paged_attention(q, batch.cache(), *batch.where())
+    for b, (n, length) in enumerate(batch.sizes):
+        first, sees = batch.np_starts[b], torch.arange(length - n, length) >= at % length
+        assert torch.equal(got[first:first + n][~sees], clean[first:first + n][~sees])
+        assert not got[first:first + n][sees].isfinite().any(), b
