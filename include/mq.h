@@ -447,7 +447,8 @@ typedef struct mq_kv_pages {
  * starts[0] and behind starts[batch] are left as they are. Starts that pass the tokens are reported (mq_device_status 27): the rows that
  * are there keep their positions, the others are left out. (mq_paged_attention alone takes an end so far behind the rows that
  * none of them would have a position, as 2^31 - 1, for theirs, and does not report it.) A table entry outside the pool is reported (19): its
- * rows are not written, and read as zeros. A length below 0 or above width * page is reported (20) and cut. A position below 0
+ * rows are not written, and read as zeros. A length below 0 or above width * page is reported (20): mq_paged_attention cuts it, the
+ * copies leave out the positions that the table does not name (not stored, loaded as zeros). A position below 0
  * (more rows than positions) is not stored, loads as zeros and sees nothing. */
 
 /* k[t][h], v[t][h] -> the pages, rounded to their type; int8 as mq_quantize_s8 makes it, row by row (a row with a NaN or an

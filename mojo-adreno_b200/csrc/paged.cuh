@@ -27,28 +27,30 @@ struct Seq {
   int pos0;      // position of its first row; negative where it has more rows than positions
 };
 
-// Rows that are not there (before the first, behind the last: reported) are left out, the others keep their positions. FAR_END:
-// an end so far behind the rows that none of them would have a position counts as theirs. Starts that fall make an
-// empty sequence; lengths that pass the table are cut to it (reported).
-template <bool FAR_END>
+// Rows that are not there (before the first, behind the last: reported) are left out, the others keep their positions. Starts that
+// fall make an empty sequence. Lengths that pass the table are reported and cut; the copies' rows keep their positions, beyond
+// the table for some, which are then left out. The attention's (ATTEND) count from the cut length, and an end so far behind
+// the rows that none of them would have a position counts as theirs.
+template <bool ATTEND>
 __device__ __forceinline__ Seq sequence(const Seqs &s, int b) {
   Seq q;
   const int length = s.lengths[b], most = s.width << s.page_log2;
   q.length = min(max(length, 0), most);
   if (q.length != length) raise_status(kStatusKvBadLength);
-  q.first = b, q.n = 1, q.pos0 = q.length - 1;
+  const int last = ATTEND ? q.length : max(length, 0);
+  q.first = b, q.n = 1, q.pos0 = last - 1;
   if (s.starts) {
     q.first = min(max(s.starts[b], 0), s.tokens);
     int end = max(s.starts[b + 1], q.first);
     q.n = min(end, s.tokens) - q.first;
     if (end > s.tokens) {
-      if (FAR_END && q.n > 0 && end - s.tokens >= q.length)
+      if (ATTEND && q.n > 0 && end - s.tokens >= q.length)
         end = s.tokens;
       else
         raise_status(kStatusKvBadStarts);
     }
     // (The bound keeps what is added to and taken from it in range; it is below 0 as far as there are rows.)
-    q.pos0 = max(q.length - (end - q.first), -(1 << 30));
+    q.pos0 = max(last - (end - q.first), -(1 << 30));
   }
   return q;
 }

@@ -954,3 +954,33 @@ def test_int8_scales_that_are_no_numbers_anywhere(cuda, x, which, value, at):
         first, sees = batch.np_starts[b], torch.arange(length - n, length) >= at % length
         assert torch.equal(got[first:first + n][~sees], clean[first:first + n][~sees])
         assert not got[first:first + n][sees].isfinite().any(), b
+
+
+@pytest.mark.parametrize("cache", [F16, S8])
+def test_positions_beyond_the_table_are_not_copied(cuda, cache):
+    """They were stored over the last positions that the table names."""
+    batch = Batch(cuda, [(2, 30), (5, 32), (1, 32)], 2, 16, 64, cache)
+    table = batch.table[:, :2].contiguous()
+    lengths = torch.tensor([33, 35, 2 ** 31 - 1], dtype=torch.int32, device=cuda)  # 31 and 32; 30 .. 34; 2^31 - 2
+    kv = torch.randn(8, 2, 64, generator=batch.g, device=cuda).half()
+    before = [batch.k.clone(), batch.v.clone()]
+    mq.device_status()
+    mq.kv_store(kv, kv, batch.cache(), table, lengths, batch.starts)
+    assert mq.device_status() == 20
+    for t, old in zip((batch.k, batch.v), before):
+        changed = {(int(p), int(r)) for p, _, r, _ in (t.view(torch.uint8) != old.view(torch.uint8)).nonzero()}
+        assert changed == {(int(table[0, 1]), 15), (int(table[1, 1]), 14), (int(table[1, 1]), 15)}
+    k, v = mq.kv_load(batch.cache(), table, lengths, batch.starts, tokens=8)
+    assert mq.device_status() == 20
+    there = torch.tensor([True, False, True, True, False, False, False, False], device=cuda)
+    assert (k[~there] == 0).all() and (v[~there] == 0).all()
+    k2, v2 = mq.kv_load(batch.cache(), table, torch.tensor([32, 32, 32], dtype=torch.int32, device=cuda),
+                        torch.tensor([0, 1, 3, 3], dtype=torch.int32, device=cuda), tokens=3)
+    assert mq.device_status() == 0
+    assert torch.equal(k[there], k2) and torch.equal(v[there], v2)
+    if cache == F16:
+        assert torch.equal(k[there], kv[there])
+    mq.kv_store(kv[:3], kv[:3], batch.cache(), table, lengths)  # without starts: positions 32, 34, 2^31 - 2
+    assert mq.device_status() == 20
+    k, v = mq.kv_load(batch.cache(), table, torch.full_like(lengths, 32))
+    assert torch.equal(k[:2], k2[[0, 2]]) and torch.equal(v[:2], v2[[0, 2]])
