@@ -454,12 +454,13 @@ typedef struct mq_kv_pages {
 /* k[t][h], v[t][h] -> the pages, rounded to their type; int8 as mq_quantize_s8 makes it, row by row (a row with a NaN or an
  * infinity: zeros and scale NaN). k, v: fp32, fp16 or bf16 (dtype), [tokens][heads][dim] with strides in elements, rows
  * 16-byte aligned. A position that two rows name (of sequences that share a page) gets either's
- * values, or a mix of the two, unless they are equal. Keys' and values' pages must not share memory, nor their scales (refused where
- * they have one layout), nor the rows with the pages. */
+ * values, or a mix of the two, unless they are equal. Keys, values and scales must not share memory with one another (refused), nor
+ * the rows with the pages. */
 MQ_API int mq_kv_store(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
                        int dtype, const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width,
                        const int32_t *lengths, const int32_t *starts, int64_t batch, int64_t tokens, void *stream);
-/* The other way: what the pages hold of those positions -> k, v (an int8 row times its scale), rounded once. */
+/* The other way: what the pages hold of those positions -> k, v (an int8 row times its scale), rounded once. k and v must not share
+ * memory with one another or with the pages (refused). */
 MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width, const int32_t *lengths,
                       const int32_t *starts, int64_t batch, int64_t tokens, void *k, int64_t k_token, int64_t k_head, void *v,
                       int64_t v_token, int64_t v_head, int dtype, void *stream);
@@ -467,7 +468,7 @@ MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ld
 /* out[t][h] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * q[t][h].k_j), over the positions j that row t sees: its own and
  * those before it, the last `window` of them (0: all). Query head h uses kv head h / (heads / cache->heads). q and out: fp16
  * or bf16 (q_dtype; a 16-bit cache's own type), [tokens][heads][dim] with strides in elements, rows 16-byte aligned; out may be
- * q's own buffer with q's strides. A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
+ * q's own buffer with q's strides; else it must not share memory with q, nor with the pages (refused). A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
  * row does not see have no influence on it, whatever they hold; one that it sees and whose key or value holds a NaN, or its value an
  * infinity (int8: whose scale is either), makes it NaN or infinite. An infinity in a 16-bit key makes the score one: +infinity makes
  * the row NaN, a key of score -infinity has no weight. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they

@@ -839,6 +839,13 @@ extern "C" int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, i
   if (batch == 0 || tokens == 0) return MQ_OK;
   if (int rc = check_rows(q, q_dtype, q_token, q_head, "q", what)) return rc;
   if (int rc = check_rows_out(out, q_dtype, tokens, heads, cache->dim, o_token, o_head, "out", what)) return rc;
+  // (out may be q: an item's rows are read before any of them is written)
+  if (!(out == q && (tokens == 1 || o_token == q_token) && (heads == 1 || o_head == q_head)))
+    MQ_REQUIRE(!share_bytes(area_of_rows(q, 2, tokens, heads, cache->dim, q_token, q_head), area_of_rows(out, 2, tokens, heads, cache->dim, o_token, o_head)),
+               MQ_EINVAL, "%s: out shares memory with q, and is not q", what);
+  Area held[4];
+  for (int i = areas_of(cache, held) - 1; i >= 0; --i)
+    MQ_REQUIRE(!share_bytes(held[i], area_of_rows(out, 2, tokens, heads, cache->dim, o_token, o_head)), MQ_EINVAL, "%s: out shares memory with the pages", what);
   mq::DeviceInfo dev;
   if (int rc = mq::device_info(&dev)) return rc;
   Plan plan;

@@ -213,27 +213,14 @@ int copy_by_rows(CopyParams &p, int dtype, int sms, cudaStream_t s, const char *
   return launch_copy<STORE, C, __nv_bfloat16>(p, sms, s, what);
 }
 
-// Whether keys and values of one layout (rows of `row` bytes, strides in elements of `es`) share a byte; of two layouts: not looked at.
-inline bool share_bytes(const mq_kv_pages *c, const void *k, const void *v, const int64_t *k_stride, const int64_t *v_stride, int64_t es,
-                        int64_t row) {
-  const int64_t size[3] = {c->pages, c->heads, c->page};
-  beam::Dim dims[3];
-  int n = 0;
-  for (int i = 0; i < 3; ++i) {
-    if (size[i] == 1) continue;
-    if (k_stride[i] != v_stride[i]) return false;
-    dims[n++] = {k_stride[i] * es, size[i]};
-  }
-  std::sort(dims, dims + n, [](const beam::Dim &a, const beam::Dim &b) { return a.stride > b.stride; });
-  int64_t extents[4] = {};
-  extents[n] = row;
-  for (int i = n - 1; i >= 0; --i) extents[i] = extents[i + 1] + dims[i].stride * (dims[i].size - 1);
-  return beam::share_bytes(dims, extents, n, static_cast<const char *>(v) - static_cast<const char *>(k));
-}
-inline bool keys_touch_values(const mq_kv_pages *c) {
-  const int64_t es = element_size(c->dtype);
-  return share_bytes(c, c->k, c->v, c->k_stride, c->v_stride, es, c->dim * es) ||
-         (c->dtype == MQ_S8 && share_bytes(c, c->k_scale, c->v_scale, c->ks_stride, c->vs_stride, 4, 4));
+// Whether a cache's keys, values and scales share a byte with one another.
+inline bool cache_overlaps(const mq_kv_pages *c) {
+  Area a[4];
+  const int n = areas_of(c, a);
+  for (int i = 0; i < n; ++i)
+    for (int j = 0; j < i; ++j)
+      if (share_bytes(a[i], a[j])) return true;
+  return false;
 }
 
 template <bool STORE>
@@ -249,10 +236,16 @@ int kv_copy(void *k, int64_t k_token, int64_t k_head, void *v, int64_t v_token, 
   if (STORE) {
     if (int rc = check_rows(k, dtype, k_token, k_head, "k", what)) return rc;
     if (int rc = check_rows(v, dtype, v_token, v_head, "v", what)) return rc;
-    MQ_REQUIRE(!keys_touch_values(c), MQ_EINVAL, "%s: keys and values, or their scales, share memory", what);
+    MQ_REQUIRE(!cache_overlaps(c), MQ_EINVAL, "%s: keys and values, or their scales, share memory", what);
   } else {
     if (int rc = check_rows_out(k, dtype, tokens, c->heads, c->dim, k_token, k_head, "k", what)) return rc;
     if (int rc = check_rows_out(v, dtype, tokens, c->heads, c->dim, v_token, v_head, "v", what)) return rc;
+    const int64_t es = element_size(dtype);
+    const Area rows_k = area_of_rows(k, es, tokens, c->heads, c->dim, k_token, k_head), rows_v = area_of_rows(v, es, tokens, c->heads, c->dim, v_token, v_head);
+    MQ_REQUIRE(!share_bytes(rows_k, rows_v), MQ_EINVAL, "%s: k and v share memory", what);
+    Area held[4];
+    for (int i = areas_of(c, held) - 1; i >= 0; --i)
+      MQ_REQUIRE(!share_bytes(rows_k, held[i]) && !share_bytes(rows_v, held[i]), MQ_EINVAL, "%s: k or v shares memory with the pages", what);
   }
   mq::DeviceInfo dev;
   if (int rc = device_info(&dev)) return rc;

@@ -156,6 +156,107 @@ inline int check_rows_out(const void *p, int dtype, int64_t tokens, int64_t head
   return MQ_OK;
 }
 
+// ---- host: what shares memory ------------------------------------------------------------------------
+
+// Rows of `row` bytes, [size[0]][size[1]][size[2]] of them, strides in bytes (0 or more).
+struct Area {
+  const char *base;
+  __int128 row, stride[3];
+  int64_t size[3];
+  __int128 extent() const {
+    __int128 e = row;
+    for (int i = 0; i < 3; ++i) e += stride[i] * (size[i] - 1);
+    return e;
+  }
+  // The same bytes, dimensions by falling stride and as few as will do: the others have size 1 and stride 0.
+  Area plain() const {
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return stride[a] > stride[b]; });
+    Area a{base, row, {0, 0, 0}, {1, 1, 1}};
+    int n = 0;
+    for (int d : order) {
+      if (size[d] == 1 || stride[d] == 0) continue;
+      if (n > 0 && a.stride[n - 1] == stride[d] * size[d])  // one dimension of both
+        a.stride[n - 1] = stride[d], a.size[n - 1] *= size[d];
+      else
+        a.stride[n] = stride[d], a.size[n++] = size[d];
+    }
+    if (n > 0 && a.stride[n - 1] == row) a.row = row * a.size[n - 1], a.stride[n - 1] = 0, a.size[n - 1] = 1;
+    return a;
+  }
+  // Whether a row, of a plain area whose rows lie apart, has a byte in [at, at + bytes) behind the base. Rows rise in the
+  // order of their dimensions, so the last row that starts before the end is the only one to look at.
+  bool has(__int128 at, __int128 bytes) const {
+    __int128 rest = at + bytes - 1;
+    if (rest < 0) return false;
+    for (int i = 0; i < 3; ++i)
+      if (stride[i] > 0) rest -= stride[i] * std::min<__int128>(size[i] - 1, rest / stride[i]);
+    return rest - (bytes - 1) < row;
+  }
+};
+// The dimensions of two areas by falling stride, with the size that each has there (1: not one of its own).
+struct Both {
+  int n;
+  __int128 stride[6], rest[7];  // rest[d]: the larger extent of what lies within dimension d - 1
+  int64_t a[6], b[6];
+};
+// Whether a row of a and one of b, `delta` bytes behind it so far, share a byte. A stride is at least the extent of what follows, so
+// only the two multiples of it around what is left can bring them together.
+inline bool rows_meet(const Both &p, __int128 row_a, __int128 row_b, int d, __int128 delta) {
+  if (d == p.n) return delta < row_a && -delta < row_b;
+  __int128 i = delta / p.stride[d];
+  if (i * p.stride[d] > delta) --i;
+  for (int k = 0; k < 2; ++k, ++i) {
+    const __int128 left = delta - i * p.stride[d];
+    if (i < p.a[d] && -i < p.b[d] && left < p.rest[d + 1] && -left < p.rest[d + 1] && rows_meet(p, row_a, row_b, d + 1, left)) return true;
+  }
+  return false;
+}
+// Whether two areas share a byte. The rows of `apart` lie apart (rows_apart); those of the other need not. Two that lie between one
+// another in strides that do not go together are compared row by row, as far as kMostCompared: beyond, they count as apart.
+constexpr int64_t kMostCompared = 4096;
+inline bool share_bytes(const Area &any, const Area &apart) {
+  const __int128 delta = static_cast<__int128>(reinterpret_cast<intptr_t>(apart.base)) - reinterpret_cast<intptr_t>(any.base);
+  if (delta >= any.extent() || -delta >= apart.extent()) return false;  // (nearly always)
+  const Area a = any.plain(), b = apart.plain();
+  Both p{};
+  for (int i = 0, j = 0; (i < 3 && a.stride[i] > 0) || (j < 3 && b.stride[j] > 0); ++p.n) {
+    const __int128 x = i < 3 ? a.stride[i] : 0, y = j < 3 ? b.stride[j] : 0;
+    p.stride[p.n] = std::max(x, y);
+    p.a[p.n] = x == p.stride[p.n] ? a.size[i++] : 1;
+    p.b[p.n] = y == p.stride[p.n] ? b.size[j++] : 1;
+  }
+  bool regular = true;
+  p.rest[p.n] = std::max(a.row, b.row);
+  for (int d = p.n - 1; d >= 0; --d) {
+    regular = regular && p.stride[d] >= p.rest[d + 1];
+    p.rest[d] = p.rest[d + 1] + p.stride[d] * (std::max(p.a[d], p.b[d]) - 1);
+  }
+  if (regular) return rows_meet(p, a.row, b.row, 0, delta);
+  int64_t left = kMostCompared;
+  for (int64_t x = 0; x < a.size[0] && left > 0; ++x)
+    for (int64_t y = 0; y < a.size[1] && left > 0; ++y)
+      for (int64_t z = 0; z < a.size[2] && left > 0; ++z, --left)
+        if (b.has(x * a.stride[0] + y * a.stride[1] + z * a.stride[2] - delta, a.row)) return true;
+  return false;
+}
+
+inline Area area_of_pages(const mq_kv_pages *c, const void *base, const int64_t *stride, int64_t es, int64_t row) {
+  return {static_cast<const char *>(base), row * es, {static_cast<__int128>(stride[0]) * es, static_cast<__int128>(stride[1]) * es, static_cast<__int128>(stride[2]) * es},
+          {c->pages, c->heads, c->page}};
+}
+// A cache's keys, values and, int8, their scales: how many areas.
+inline int areas_of(const mq_kv_pages *c, Area (&a)[4]) {
+  const int64_t es = element_size(c->dtype);
+  a[0] = area_of_pages(c, c->k, c->k_stride, es, c->dim), a[1] = area_of_pages(c, c->v, c->v_stride, es, c->dim);
+  if (c->dtype != MQ_S8) return 2;
+  a[2] = area_of_pages(c, c->k_scale, c->ks_stride, 4, 1), a[3] = area_of_pages(c, c->v_scale, c->vs_stride, 4, 1);
+  return 4;
+}
+inline Area area_of_rows(const void *base, int64_t es, int64_t tokens, int64_t heads, int64_t dim, int64_t token_stride, int64_t head_stride) {
+  return {static_cast<const char *>(base), dim * es, {static_cast<__int128>(token_stride) * es, static_cast<__int128>(head_stride) * es, 0}, {tokens, heads, 1}};
+}
+
 // ---- attention: items, units and shares --------------------------------------------------------------
 
 // The rows of one kv head of a sequence are its tokens' `group` query heads, token by token: row r is head r % group of

@@ -177,9 +177,75 @@ def test_store_where_scales_share_memory(shift, stride, refused):
     without_device()
 
     def store(dtype):
-        c = pages(v=OK + (1 << 16), dtype=dtype, k_scale=OK, v_scale=OK + shift, ks_stride=stride, vs_stride=stride)
+        c = pages(v=OK + (1 << 16), dtype=dtype, k_scale=OK << 2, v_scale=(OK << 2) + shift, ks_stride=stride, vs_stride=stride)
         return status("mq_kv_store", OK, 128, 64, OK, 128, 64, 1, ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, None)
 
     rc, msg = store(3)
     assert ("share memory" in msg and rc == -1) if refused else rc != -1, msg
     assert store(1)[0] != -1  # (a 16-bit cache has none)
+
+
+# ---- calls that overlap: the pages of `pages()` are 8 x 2 x 16 rows of 128 bytes, 32768 in all --------------------
+
+FAR = OK + (1 << 24)
+
+
+def apart(**kw):
+    return pages(**{**dict(k=OK, v=OK + 32768, k_scale=OK + 65536, v_scale=OK + 65536 + 1024), **kw})
+
+
+@pytest.mark.parametrize("args,refused", [
+    (dict(out=FAR), None), (dict(out=FAR, o_head=128, o_token=1024), "q"), (dict(out=FAR + 16), "q"), (dict(out=FAR + 512), "q"),
+    (dict(out=FAR + 5 * 1024), None), (dict(out=FAR - 5 * 1024), None), (dict(out=FAR - 5 * 1024 + 16), "q"),
+    # A fused projection's buffer: q's 8 of 12 heads, out in the 4 (of 4 heads of 64, 2 kv heads) behind them or over q's last.
+    (dict(q_token=768, out=FAR + 1024, o_token=768, heads=4), None), (dict(q_token=768, out=FAR + 256, o_token=768, heads=4), "q"),
+    (dict(q_token=768, out=FAR + 1024, o_token=760, heads=4), None), (dict(q_token=768, out=FAR + 1024, o_token=776, heads=4), "q"), (dict(q_token=768, out=FAR + 512, o_token=760, heads=4), "q"),
+    # Heads behind one another instead of tokens: the same bytes in another order.
+    (dict(out=FAR, o_token=64, o_head=5 * 64), "q"), (dict(q=FAR, q_token=0, q_head=0, out=FAR + 128), None), (dict(q_token=0, q_head=0, out=FAR), "q"),
+    (dict(out=OK), "pages"), (dict(out=OK + 32768 + 32752), "pages"), (dict(out=OK + 65536), None), (dict(out=OK - 5 * 1024), None),
+])
+def test_attention_into_memory_that_is_read(args, refused):
+    without_device()
+    rc, msg = attention(apart(), **{**dict(q=FAR), **args})
+    if refused:
+        assert rc == -1 and "shares memory with " + ("q" if refused == "q" else "the pages") in msg, msg
+    else:
+        assert rc not in (-1, 0) and "memory" not in msg, msg
+
+
+def test_attention_into_scales():
+    without_device()
+    for at, refused in ((65536, True), (65536 + 2047 // 16 * 16, True), (65536 + 2048, False)):
+        rc, msg = attention(apart(dtype=3), q=FAR, out=OK + at)
+        assert (rc == -1 and "with the pages" in msg) if refused else rc not in (-1, 0), msg
+
+
+@pytest.mark.parametrize("k,kt,v,vt,match", [
+    (FAR, 128, FAR, 128, "k and v"), (FAR, 128, FAR + 1280, 128, None), (FAR, 128, FAR + 1280 - 16, 128, "k and v"), (FAR, 256, FAR + 256, 256, None),
+    (FAR, 256, FAR + 240, 256, "k and v"), (FAR, 256, FAR + 256, 384, "k and v"), (OK, 128, FAR, 128, "pages"), (FAR, 128, OK + 65536 - 16, 128, "pages"),
+    (FAR, 128, OK + 65536, 128, None)])
+def test_load_into_memory_that_is_read(k, kt, v, vt, match):
+    without_device()
+    c = apart()
+    rc, msg = status("mq_kv_load", ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, k, kt, 64, v, vt, 64, 1, None)
+    assert (rc == -1 and match in msg and "memory" in msg) if match else rc not in (-1, 0), msg
+
+
+@pytest.mark.parametrize("cache,refused", [
+    (dict(), False), (dict(v=OK), True), (dict(v=OK + 32768 - 16), True),
+    # Pages of keys head by head and of values position by position, one behind the other in each block of 8192 bytes.
+    (dict(k_stride=(4096, 1024, 64), v=OK + 4096, v_stride=(4096, 64, 128)), False),
+    (dict(k_stride=(4096, 1024, 64), v=OK + 4096 - 128, v_stride=(4096, 64, 128)), True),
+    # Keys, values and scales of a page in one block of 8448 bytes.
+    (dict(dtype=3, k_stride=(8448, 1024, 64), v=OK + 2048, v_stride=(8448, 1024, 64), k_scale=OK + 4096, v_scale=OK + 4224, ks_stride=(2112, 16, 1),
+          vs_stride=(2112, 16, 1)), False),
+    (dict(dtype=3, k_stride=(8448, 1024, 64), v=OK + 2048, v_stride=(8448, 1024, 64), k_scale=OK + 4092, v_scale=OK + 4224, ks_stride=(2112, 16, 1),
+          vs_stride=(2112, 16, 1)), True),
+    (dict(dtype=3, k_stride=(8448, 1024, 64), v=OK + 2048, v_stride=(8448, 1024, 64), k_scale=OK + 4096, v_scale=OK + 4096, ks_stride=(2112, 32, 2),
+          vs_stride=(2112, 32, 1)), True),
+])
+def test_store_into_caches_of_two_layouts(cache, refused):
+    without_device()
+    c = apart(**cache)
+    rc, msg = status("mq_kv_store", FAR, 128, 64, FAR, 128, 64, 1, ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, None)
+    assert (rc == -1 and "share memory" in msg) if refused else rc not in (-1, 0), msg
