@@ -499,7 +499,7 @@ MQ_API int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, int64
  * no distribution (a NaN, +infinity, all -infinity) is reported (24), and its request ends there with token -1; such a draft row is
  * reported, its token is not kept and q counts as 0. Logits: fp32, fp16 or bf16, rows ld elements apart. drafts <= 32.
  * workspace: mq_verify_workspace_size() bytes, 16-byte aligned, or a larger call's; calls that may overlap in time need one each.
- * batch == 0 does nothing. */
+ * Outputs and workspace must not share memory with one another or the inputs (refused). batch == 0 does nothing. */
 MQ_API size_t mq_verify_workspace_size(int64_t batch, int64_t drafts, int64_t vocab);
 MQ_API int mq_verify_drafts(const void *target, int64_t ld_target, const void *draft, int64_t ld_draft, int dtype,
                             const int32_t *drafted, const int32_t *counts, const float *uniform, const float *temperature,

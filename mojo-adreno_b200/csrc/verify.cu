@@ -587,11 +587,31 @@ extern "C" int mq_verify_drafts(const void *target, int64_t ld_target, const voi
                  mq::aligned(logprobs, 4) && mq::aligned(workspace, 16),
              MQ_EALIGN, "%s: the workspace must be 16-byte aligned, the others aligned to their elements", what);
   MQ_REQUIRE(workspace_bytes >= mq_verify_workspace_size(batch, drafts, vocab), MQ_EINVAL, "%s: the workspace is too small", what);
+  if (drafts == 0) draft = nullptr;
+  const int64_t rows = batch * (draft ? 2 * drafts + 1 : drafts + 1), given = 4 * batch * (drafts + 1);
+  {
+    // Some CTAs of a request write while others still read.
+    struct Range {
+      const void *at;
+      __int128 bytes;
+    };
+    const Range written[] = {{tokens, given}, {accepted, 4 * batch}, {logprobs, given}, {workspace, static_cast<int64_t>(mq_verify_workspace_size(batch, drafts, vocab))}};
+    const Range read[] = {{target, (static_cast<__int128>(batch * (drafts + 1) - 1) * ld_target + vocab) * es},
+                          {draft, (static_cast<__int128>(batch * drafts - 1) * ld_draft + vocab) * es},
+                          {drafted, 4 * batch * drafts}, {counts, 4 * batch}, {uniform, given}, {temperature, 4 * batch}};
+    auto meet = [](const Range &a, const Range &b) {
+      return a.at && b.at && a.bytes > 0 && b.bytes > 0 &&
+             (a.at <= b.at ? static_cast<const char *>(b.at) - static_cast<const char *>(a.at) < a.bytes
+                           : static_cast<const char *>(a.at) - static_cast<const char *>(b.at) < b.bytes);
+    };
+    for (int i = 0; i < 4; ++i) {
+      for (const Range &r : read) MQ_REQUIRE(!meet(written[i], r), MQ_EINVAL, "%s: an output or the workspace shares memory with an input", what);
+      for (int j = 0; j < i; ++j) MQ_REQUIRE(!meet(written[i], written[j]), MQ_EINVAL, "%s: outputs or the workspace share memory", what);
+    }
+  }
   mq::DeviceInfo dev;
   if (int rc = mq::device_info(&dev)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (drafts == 0) draft = nullptr;
-  const int64_t rows = batch * (draft ? 2 * drafts + 1 : drafts + 1);
   Params p{target, draft, ld_target, ld_draft, drafted, counts, uniform, temperature, static_cast<float2 *>(workspace), tokens, accepted,
            logprobs, static_cast<int>(batch), static_cast<int>(drafts), static_cast<int>(vocab), splits_for(rows, vocab), dtype};
   int rc;

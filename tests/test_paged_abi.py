@@ -249,3 +249,30 @@ def test_store_into_caches_of_two_layouts(cache, refused):
     c = apart(**cache)
     rc, msg = status("mq_kv_store", FAR, 128, 64, FAR, 128, 64, 1, ctypes.addressof(c), OK, 4, 4, OK, OK, 2, 5, None)
     assert (rc == -1 and "share memory" in msg) if refused else rc not in (-1, 0), msg
+
+
+def test_verify_into_memory_that_is_read():
+    without_device()
+    n, rows = 2 * 4 * 4, 2 * 4 * 100 * 4
+    inputs = dict(target=OK, draft=OK + rows, drafted=FAR, counts=FAR + 64, uniform=FAR + 128, temperature=FAR + 192)
+    outputs = dict(tokens=FAR + 256, accepted=FAR + 320, logprobs=FAR + 384, workspace=FAR + 448)
+    size = dict(target=rows, draft=rows * 3 // 4, drafted=24, counts=8, uniform=n, temperature=8, tokens=n, accepted=8, logprobs=n, workspace=9472)
+
+    def verify(**kw):
+        a = dict(target=0, ld=100, draft=0, ld_draft=100, dtype=0, drafted=0, counts=0, uniform=0, temperature=0, tokens=0, accepted=0,
+                 logprobs=0, batch=2, drafts=3, vocab=100, workspace=0, size=1 << 20)
+        a.update(**inputs, **outputs)
+        a.update(kw)
+        return status("mq_verify_drafts", *a.values(), None)
+
+    assert verify()[0] not in (-1, 0), verify()
+    assert verify(draft=None, counts=None, temperature=None)[0] not in (-1, 0)
+    for out in outputs:
+        for other in [*inputs, *outputs]:
+            if other == out:
+                continue
+            at = {**inputs, **outputs}[other]
+            for shift in (0, size[other] // 16 * 16 - 16):  # its first and one of its last bytes
+                if shift >= 0:
+                    rc, msg = verify(**{out: at + shift})
+                    assert rc == -1 and ("shares memory" in msg or "share memory" in msg), (out, other, msg)
