@@ -984,3 +984,35 @@ def test_positions_beyond_the_table_are_not_copied(cuda, cache):
     assert mq.device_status() == 20
     k, v = mq.kv_load(batch.cache(), table, torch.full_like(lengths, 32))
     assert torch.equal(k[:2], k2[[0, 2]]) and torch.equal(v[:2], v2[[0, 2]])
+
+
+@pytest.mark.parametrize("batch,new,group", [(300, 1, 1), (520, 5, 4)])
+def test_shares_of_more_units_than_32_bits_divide(cuda, batch, new, group):
+    """Sequences of 131072 positions or so that share one table's pages: more than 2^21 units (a block of 64 keys for few rows, of 128
+    for more, and two for each item), whose shares take 64-bit products. A sample of the sequences against the formula."""
+    page, kv_heads, dim, most = 256, 4, 16, 131072
+    cache = mq.paged_cache(most // page, kv_heads, page, dim, F16)
+    g = torch.Generator(device=cuda).manual_seed(batch)
+    for t in (cache.k, cache.v):
+        t.normal_(generator=g)
+    table = torch.randperm(most // page, generator=g, device=cuda).int().repeat(batch, 1)
+    lengths = most - 3 * torch.arange(batch, dtype=torch.int32, device=cuda).flip(0).contiguous()
+    assert batch * kv_heads * (2 + (most - 3 * batch) // (64 if new * group <= 16 else 128)) > 2 ** 21
+    starts = torch.arange(0, (batch + 1) * new, new, dtype=torch.int32, device=cuda)
+    q = (torch.randn(batch * new, kv_heads * group, dim, generator=g, device=cuda) * 4).half()
+    mq.device_status()
+    out = mq.paged_attention(q, cache, table, lengths, starts, max_new=new)
+    assert mq.device_status() == 0
+    k, v = (t[table[0].long()].transpose(0, 1).reshape(kv_heads, most, dim).double() for t in (cache.k, cache.v))
+    for b in {0, 1, batch // 3, batch // 2, batch - 2, batch - 1}:
+        rows = q[b * new:(b + 1) * new].double().view(new, kv_heads, group, dim)
+        z = torch.einsum("tkgd,kld->tkgl", rows, k) * dim ** -0.5
+        end = int(lengths[b])
+        z = z.masked_fill(torch.arange(most, device=cuda) > torch.arange(end - new, end, device=cuda)[:, None, None, None], -float("inf"))
+        p = z.softmax(-1)
+        ref, size = torch.einsum("tkgl,kld->tkgd", p, v), torch.einsum("tkgl,kld->tkgd", p, v.abs())
+        big = dim ** -0.5 * torch.einsum("tkgd,kd->tkg", rows.abs(), k.abs().amax(1))
+        bound = 2.0 ** -11 * ref.abs() + (2 * 2.0 ** -11 + 2 * (dim + 16) * 2.0 ** -23 * big + 2.0 ** -19)[..., None] * size + 2.0 ** -24 + \
+            2.0 ** -25 * p.amax(-1)[..., None] * v.abs().sum(1)[:, None]
+        err = (out[b * new:(b + 1) * new].double().view_as(ref) - ref).abs()
+        assert (err <= bound).all(), (b, float((err / bound).max()))
