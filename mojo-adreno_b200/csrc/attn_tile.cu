@@ -776,10 +776,16 @@ inline int plan_for(Plan *plan, const mq_kv_pages *c, int64_t heads, int64_t bat
   int64_t most = starts ? std::min(tokens, max_new > 0 ? max_new : tokens) : 1;
   plan->most_rows = static_cast<int>(most * group);
   plan->d = c->dim <= 64 ? 64 : 128;
-  // One sequence may have all the tokens; and where sequences have some drafted tokens each, a launch for the few that may have one
-  // or two costs more than they do among the others (16 x 5 tokens, 8 heads to a kv head: 36.0 us with it, 32.7 without).
-  const bool few = group <= kRowsForTiles && !(batch == 1 && most == tokens && tokens * group > kRowsForTiles) &&
-                   !(plan->most_rows > kRowsForTiles && plan->most_rows <= 128 && tokens * group >= 2 * kRowsForTiles * batch);
+  // One sequence may have all the tokens. And where sequences have some drafted tokens each, a launch for those that may have one
+  // or two costs more than they do among the others. Without it and with it, us: 16 sequences of 5 tokens, 8 heads to a kv head,
+  // up to 4100 positions: 34.7 and 39.3; 64 of 1 to 8 tokens: 85.5 and 97.7; 64 of which 16 have 13 and the others one, up to 8000:
+  // 132 and 138. From int8 the tiles are slower for single tokens (the last: 187 and 145; of 16 sequences 65 and 66), so more than
+  // 16 sequences go there only where at most a quarter can have few rows, by their mean and the most that one may have (64 of 5
+  // tokens: 122 and 127; but of 1 to 8, which are so many by that: 122 and, as it is, 127).
+  const int64_t rows = tokens * group;
+  const bool drafts = plan->most_rows > kRowsForTiles && plan->most_rows <= 128 && rows >= 2 * kRowsForTiles * batch;
+  const bool singles = c->dtype == MQ_S8 && batch > 16 && 4 * (plan->most_rows * batch - rows) > (plan->most_rows - kRowsForTiles) * batch;
+  const bool few = group <= kRowsForTiles && !(batch == 1 && most == tokens && rows > kRowsForTiles) && !(drafts && !singles);
   const bool tile = plan->most_rows > kRowsForTiles || !few;
   plan->few_ctas = !few ? 0 : sms * (plan->d == 128 ? 2 : 3);
   plan->tile_ctas = tile ? sms : 0;

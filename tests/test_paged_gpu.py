@@ -1016,3 +1016,13 @@ def test_shares_of_more_units_than_32_bits_divide(cuda, batch, new, group):
             2.0 ** -25 * p.amax(-1)[..., None] * v.abs().sum(1)[:, None]
         err = (out[b * new:(b + 1) * new].double().view_as(ref) - ref).abs()
         assert (err <= bound).all(), (b, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("cache,x", CACHES)
+@pytest.mark.parametrize("batch", [16, 17, 40])
+@pytest.mark.parametrize("new", [(5,), (13, 1, 1, 1), (8, 1), (8, 7, 6, 5), (1, 2, 3, 4, 5, 6, 7, 8)])
+def test_drafted_and_single_tokens_in_one_batch(cuda, cache, x, batch, new):
+    """Mixes for which the plan takes one launch or two."""
+    rng = np.random.default_rng(batch)
+    sizes = [(new[b % len(new)], new[b % len(new)] + int(rng.integers(0, 300))) for b in range(batch)]
+    attend(Batch(cuda, sizes, 2, 16, 64, cache), 16, x, max_new=max(new))
