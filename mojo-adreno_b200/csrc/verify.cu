@@ -28,12 +28,15 @@ namespace mq {
 namespace verify {
 
 constexpr int kScan = 256, kVecs = 4;        // threads of a scan CTA, 16-byte vectors per thread and step
-// The drawing CTAs of a request and their threads: many for the latency of a few requests, fewer where that lets all CTAs run at
-// once (four of 256 on an SM). Sixteen CTAs against eight, requests of 4 drafts and 151669 fp32 that all sample, scan and draw:
-// 1: 26.7 us (31.1), 4: 32.5 (37.4), 9: 44.2 (46.9), 12: 48.1 (53.8), but 18: 69.8 (62.9), 37: 120 (100). (With an SM to each of
-// the sixteen, and registers for it, 1: 25.8, 4: 30.4, but 9: 49.1.)
+// The drawing CTAs of a request and their threads: many for the latency of a few requests with a long row, fewer where that lets all
+// CTAs run at once (four of 256 on an SM). Sixteen CTAs against eight, requests of 4 drafts that all sample, scan and draw, us:
+//   fp32  151669: 1: 25.4 (28.5), 4: 34.8 (37.4), 12: 49.6 (54.6), but 18: 69.8 (62.9), 37: 120 (100); 100352: 1: 21.5 (24.4),
+//         12: 39.8 (44.0); but 48000: 4: 26.3 (23.2), 32000: 1: 18.4 (17.3), 4: 25.1 (20.1), 12: 27.8 (23.8); 80000: about equal.
+//   bf16  151669: 1: 26.0 (29.5), 6: 34.1 (38.1), but 8: 44.9 (42.2), 12: 46.6 (43.0); 100352: 6: 29.8 (33.4), but 12: 39.7 (37.4).
 constexpr int kClusterFew = 16, kCluster = 8;
-constexpr int kDrawFew = 512, kDrawMany = 256, kFewRequests = 12, kManyRequests = 148 * 2 / kCluster;
+constexpr int kDrawFew = 512, kDrawMany = 256, kManyRequests = 148 * 2 / kCluster;
+constexpr int kFewRequests = 12, kFewRequests16 = 6;  // of fp32, of 16-bit logits
+constexpr int64_t kLongRow = 100000;
 constexpr int kMaxDrafts = 32, kMaxSplits = 64;
 constexpr float kLeastTemperature = 1e-5f;   // below: 0
 // Less than this of p - q is nothing: equal distributions leave the roundings of their terms, 1e-14 in all (of two rows with the
@@ -548,7 +551,7 @@ int draw(const Params &p, cudaStream_t s, const char *what) {
     return launch_overlapped_clusters(kern, dim3(static_cast<unsigned>(p.batch * cluster)), dim3(threads), cluster, 0, s, what, p);
   };
   if (p.batch > kManyRequests) return go(verify_draw_kernel<T, kDrawMany, kCluster>, kDrawMany, kCluster);
-  if (p.batch <= kFewRequests && wide_clusters_run<T>()) return go(verify_draw_kernel<T, kDrawFew, kClusterFew>, kDrawFew, kClusterFew);
+  if (p.batch <= (sizeof(T) == 4 ? kFewRequests : kFewRequests16) && p.vocab >= kLongRow && wide_clusters_run<T>()) return go(verify_draw_kernel<T, kDrawFew, kClusterFew>, kDrawFew, kClusterFew);
   return go(verify_draw_kernel<T, kDrawFew, kCluster>, kDrawFew, kCluster);
 }
 

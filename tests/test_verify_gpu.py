@@ -348,3 +348,11 @@ def test_equal_distributions_and_a_uniform_of_one(cuda):
     got = case.call()
     assert (got[1] == 0).all()
     case.check(got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("batch", [1, 6, 7, 12, 13])
+@pytest.mark.parametrize("vocab", [99999, 100003])
+def test_long_rows_where_the_draw_is_split_otherwise(cuda, dtype, batch, vocab):
+    case = Case(cuda, batch, 1, vocab, dtype, True, [1.0, 0.0, 0.7], batch)
+    case.check(case.call())
