@@ -135,7 +135,8 @@ def _rows3(t, name, dtypes, heads, dim, device):
 def kv_store(k, v, cache, table, lengths, starts=None):
     """Writes the new tokens' keys and values into their pages, rounded to the cache's type or, int8, quantised row by
     row as quantize_s8 does. k, v: fp32, fp16 or bf16 [tokens, kv_heads, dim], rows 16-byte aligned. A table entry
-    outside the pool is skipped and reported (device_status() 19). Returns the cache."""
+    outside the pool is skipped and reported (device_status() 19), and so are positions beyond the table (20). k and v must not lie in
+    the pages. Returns the cache."""
     device = _here(cache)
     p = cache._pages
     tokens, _, kt, kh = _rows3(k, "k", _DT, p.heads, p.dim, device)
@@ -186,7 +187,8 @@ def paged_attention(q, cache, table, lengths, starts=None, out=None, scale=None,
     """Attention of the new tokens over what their sequences have in the cache, themselves included: out[t, h] =
     softmax(scale * q[t, h] . k_j) v_j over the positions j up to the token's own, the last `window` of them if that is
     not 0. q fp16 or bf16 (a 16-bit cache's type) [tokens, heads, dim], heads a multiple of the cache's (query head h
-    uses kv head h // (heads // kv_heads)); out likewise, made if None, may be q. scale: dim ** -0.5 if None. A row that sees
+    uses kv head h // (heads // kv_heads)); out likewise, made if None, may be q
+    (but not share memory with it in another way). scale: dim ** -0.5 if None. A row that sees
     nothing gives zeros; positions that a row does not see do not matter, whatever they hold. max_new: no sequence has
     more new tokens than this (0: unknown); said, it spares a launch where all have few. Calls that may overlap in time
     need a workspace each."""

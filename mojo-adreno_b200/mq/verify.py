@@ -24,9 +24,9 @@ def verify_drafts(target, drafted, uniform, draft=None, temperature=None, counts
     draft: the drafter's logits [batch * drafts, vocab] of target's type (None: its tokens came without a distribution);
     temperature fp32 [batch] (None: 1; 0: greedy); counts int32 [batch]: how many drafts each request has (None: all).
     Token i is kept while uniform * q(token) < p(token), with p and q the softmax of the logits / temperature; at the
-    first that is not, one is drawn from max(p - q, 0), from p where all are kept, with the last uniform. Returns (tokens
+    first that is not, one is drawn from max(p - q, 0), from p where all are kept or the two are the same, with the last uniform. Returns (tokens
     int32 [batch, drafts + 1]: the kept ones, the drawn one, then -1; accepted int32 [batch]; logprobs fp32 [batch,
-    drafts + 1]: the target's log-probability of each, 0 behind)."""
+    drafts + 1]: the target's log-probability of each, 0 behind). Outputs and workspace may not share memory with the inputs."""
     if not isinstance(drafted, torch.Tensor) or drafted.dim() != 2:
         raise MQError(-1, "drafted: expected a [batch, drafts] tensor")
     batch, drafts = drafted.shape
