@@ -8,7 +8,7 @@
 // Both are a copy: what bounds them is the bandwidth, or for a few tokens the launch and the chain of loads that finds a
 // token's page. A CTA looks up the places of its tokens (up to 64) at once; then each of its threads has one piece of 8 values of
 // a token's rows, 8 or 16 lanes to a row, and takes it from token to token, four on their way (two: 75 and 183 us, eight: 79 and
-// 200). 53,223 tokens of 2 x 8 x 128 bf16 into pages: 74 us (5.9 TB/s); 137,835 of int8 back as bf16: 168 us (5.1 TB/s: the
+// 200). 53,223 tokens of 2 x 8 x 128 bf16 into pages: 74 us (5.9 TB/s), into int8 pages 115 (2.9); 137,835 of int8 back as bf16: 168 us (5.1 TB/s: the
 // conversions); one token: 2 us.
 #include <type_traits>
 
