@@ -468,7 +468,8 @@ MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ld
 /* out[t][h] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * q[t][h].k_j), over the positions j that row t sees: its own and
  * those before it, the last `window` of them (0: all). Query head h uses kv head h / (heads / cache->heads). q and out: fp16
  * or bf16 (q_dtype; a 16-bit cache's own type), [tokens][heads][dim] with strides in elements, rows 16-byte aligned; out may be
- * q's own buffer with q's strides; else it must not share memory with q, nor with the pages (refused). A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
+ * q's own buffer with q's strides; else it must not share memory with q, nor with the pages, nor
+ * the workspace with any of these (refused). A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
  * row does not see have no influence on it, whatever they hold; one that it sees and whose key or value holds a NaN, or its value an
  * infinity (int8: whose scale is either), makes it NaN or infinite. An infinity in a 16-bit key makes the score one: +infinity makes
  * the row NaN, a key of score -infinity has no weight. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they

@@ -847,18 +847,23 @@ extern "C" int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, i
   if (int rc = check_rows(q, q_dtype, q_token, q_head, "q", what)) return rc;
   if (int rc = check_rows_out(out, q_dtype, tokens, heads, cache->dim, o_token, o_head, "out", what)) return rc;
   // (out may be q: an item's rows are read before any of them is written)
+  const Area rows_q = area_of_rows(q, 2, tokens, heads, cache->dim, q_token, q_head);
+  const Area rows_out = area_of_rows(out, 2, tokens, heads, cache->dim, o_token, o_head);
   if (!(out == q && (tokens == 1 || o_token == q_token) && (heads == 1 || o_head == q_head)))
-    MQ_REQUIRE(!share_bytes(area_of_rows(q, 2, tokens, heads, cache->dim, q_token, q_head), area_of_rows(out, 2, tokens, heads, cache->dim, o_token, o_head)),
-               MQ_EINVAL, "%s: out shares memory with q, and is not q", what);
+    MQ_REQUIRE(!share_bytes(rows_q, rows_out), MQ_EINVAL, "%s: out shares memory with q, and is not q", what);
   Area held[4];
-  for (int i = areas_of(cache, held) - 1; i >= 0; --i)
-    MQ_REQUIRE(!share_bytes(held[i], area_of_rows(out, 2, tokens, heads, cache->dim, o_token, o_head)), MQ_EINVAL, "%s: out shares memory with the pages", what);
+  const int nheld = areas_of(cache, held);
+  for (int i = 0; i < nheld; ++i) MQ_REQUIRE(!share_bytes(held[i], rows_out), MQ_EINVAL, "%s: out shares memory with the pages", what);
   mq::DeviceInfo dev;
   if (int rc = mq::device_info(&dev)) return rc;
   Plan plan;
   if (int rc = plan_for(&plan, cache, heads, batch, tokens, max_new, starts != nullptr, dev.sms, what)) return rc;
   MQ_REQUIRE(workspace && mq::aligned(workspace, 16), MQ_EALIGN, "%s: the workspace must be 16-byte aligned", what);
   MQ_REQUIRE(workspace_bytes >= plan.bytes, MQ_EINVAL, "%s: the workspace is too small", what);
+  const Area work = {static_cast<const char *>(workspace), static_cast<__int128>(plan.bytes), {0, 0, 0}, {1, 1, 1}};
+  bool meets = share_bytes(rows_q, work) || share_bytes(rows_out, work);
+  for (int i = 0; i < nheld; ++i) meets = meets || share_bytes(held[i], work);
+  MQ_REQUIRE(!meets, MQ_EINVAL, "%s: the workspace shares memory with q, out or the pages", what);
   set_group(&p.shape, static_cast<int>(heads / cache->heads));
   p.shape.kv_heads = cache->heads, p.shape.window = static_cast<int>(window);
   p.q = q, p.q_token = q_token, p.q_head = q_head, p.q_dtype = q_dtype;

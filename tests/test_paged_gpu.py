@@ -1026,3 +1026,21 @@ def test_drafted_and_single_tokens_in_one_batch(cuda, cache, x, batch, new):
     rng = np.random.default_rng(batch)
     sizes = [(new[b % len(new)], new[b % len(new)] + int(rng.integers(0, 300))) for b in range(batch)]
     attend(Batch(cuda, sizes, 2, 16, 64, cache), 16, x, max_new=max(new))
+
+
+def test_workspace_that_shares_memory(cuda):
+    cache = mq.paged_cache(4, 2, 16, 64)
+    table = torch.zeros(1, 4, dtype=torch.int32, device=cuda)
+    lengths = torch.ones(1, dtype=torch.int32, device=cuda)
+    nbytes = mq.paged_attention_workspace(cache, 8, 1, 1)
+    buf = torch.zeros(nbytes + 2048, dtype=torch.uint8, device=cuda)
+    inside, behind = (buf[at:at + 1024].view(F16).view(1, 8, 64) for at in (nbytes // 2 // 16 * 16, (nbytes + 15) // 16 * 16))
+    clear = torch.zeros(1, 8, 64, device=cuda, dtype=F16)
+    for q, out in ((inside, clear), (clear, inside), (inside, inside)):
+        with pytest.raises(mq.MQError, match="workspace shares memory"):
+            mq.paged_attention(q, cache, table, lengths, out=out, workspace=buf)
+    pool = buf[:4 * 2 * 16 * 64 * 2].view(F16).view(4, 2, 16, 64)
+    with pytest.raises(mq.MQError, match="workspace shares memory"):
+        mq.paged_attention(clear, mq.PagedCache(pool, cache.v), table, lengths, workspace=buf)
+    mq.device_status()
+    assert (mq.paged_attention(behind, cache, table, lengths, workspace=buf[:nbytes]) == 0).all() and mq.device_status() == 0
