@@ -445,8 +445,8 @@ typedef struct mq_kv_pages {
  * that its row i of n is position lengths[b] - n + i. table: int32 [batch][width], ldt elements from row to row; only the
  * entries of positions below lengths[b] are read. All of these are device memory, read when the kernels run. Rows before
  * starts[0] and behind starts[batch] are left as they are. Starts that pass the tokens are reported (mq_device_status 27): the rows that
- * are there keep their positions, the others are left out. (mq_paged_attention alone takes an end so far behind the rows that
- * none of them would have a position, as 2^31 - 1, for theirs, and does not report it.) A table entry outside the pool is reported (19): its
+ * are there keep their positions, the others are left out. (mq_paged_attention alone takes an end that can be none, as 2^31 - 1, for
+ * the rows' end, and does not report it: one that means more rows than width * page, and leaves no row that is there a position.) A table entry outside the pool is reported (19): its
  * rows are not written, and read as zeros. A length below 0 or above width * page is reported (20): mq_paged_attention cuts it, the
  * copies leave out the positions that the table does not name (not stored, loaded as zeros). A position below 0
  * (more rows than positions) is not stored, loads as zeros and sees nothing. */

@@ -29,8 +29,8 @@ struct Seq {
 
 // Rows that are not there (before the first, behind the last: reported) are left out, the others keep their positions. Starts that
 // fall make an empty sequence. Lengths that pass the table are reported and cut; the copies' rows keep their positions, beyond
-// the table for some, which are then left out. The attention's (ATTEND) count from the cut length, and an end so far behind
-// the rows that none of them would have a position counts as theirs.
+// the table for some, which are then left out. The attention's (ATTEND) count from the cut length, and an end that can be none,
+// with more rows than the table has positions and none of those that are there at one of them, counts as the rows' end.
 template <bool ATTEND>
 __device__ __forceinline__ Seq sequence(const Seqs &s, int b) {
   Seq q;
@@ -44,7 +44,7 @@ __device__ __forceinline__ Seq sequence(const Seqs &s, int b) {
     int end = max(s.starts[b + 1], q.first);
     q.n = min(end, s.tokens) - q.first;
     if (end > s.tokens) {
-      if (ATTEND && q.n > 0 && end - s.tokens >= q.length)
+      if (ATTEND && q.n > 0 && end - q.first > most && end - s.tokens >= q.length)
         end = s.tokens;
       else
         raise_status(kStatusKvBadStarts);

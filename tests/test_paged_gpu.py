@@ -824,10 +824,11 @@ def test_starts_that_pass_the_rows(cuda, cache, x, held, rows):
 
 
 def test_starts_far_behind_the_rows(cuda):
-    """An end that would leave no row a position is the rows' end to the attention; the copies leave such rows out, and say so."""
+    """An end that can be none (more rows than the table has positions, none of those that are there at one) is the rows' end to the
+    attention; the copies leave such rows out, and say so. One that can be makes rows without positions, which see nothing."""
     batch = Batch(cuda, [(3, 40), (5, 60)], 2, 16, 64, F16)
     q = torch.randn(batch.tokens, 8, 64, generator=batch.g, device=cuda).half()
-    for end in (8 + 60, 10 ** 6, 2 ** 31 - 1):
+    for end in (3 + 5 * 16 + 1, 10 ** 6, 2 ** 31 - 1):
         starts = torch.tensor([-2 ** 31, 3, end], dtype=torch.int32, device=cuda)
         mq.device_status()
         want = mq.paged_attention(q, batch.cache(), *batch.where())
@@ -843,6 +844,11 @@ def test_starts_far_behind_the_rows(cuda):
         for j in range(40, 60):
             page = int(batch.np_table[1, j // 16])
             assert torch.equal(batch.k[page, :, j % 16], before[0][page, :, j % 16])
+    want = mq.paged_attention(q, batch.cache(), *batch.where())
+    for end in (8 + 60, 3 + 5 * 16):
+        starts = torch.tensor([0, 3, end], dtype=torch.int32, device=cuda)
+        got = mq.paged_attention(q, batch.cache(), batch.table, batch.lengths, starts)
+        assert mq.device_status() == 27 and (got[3:] == 0).all() and torch.equal(got[:3], want[:3])
     starts = torch.tensor([0, 3, 8 + 59], dtype=torch.int32, device=cuda)  # the last row's position is 0
     got = mq.paged_attention(q, batch.cache(), batch.table, batch.lengths, starts)
     assert mq.device_status() == 27
