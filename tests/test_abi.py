@@ -144,3 +144,15 @@ def test_router_chain_and_layer_reject_bad_arguments_before_launch():
     rc, msg = _status("mq_moe_layer", ok, ok, ok, ok, ok, ok, ok, ok, ok, None, 4, 128, 8, 2048, 768, 32, 0, ok, 16,
                       None)
     assert rc == -1 and "workspace" in msg
+
+
+def test_build_without_the_reference_sources(tmp_path, monkeypatch):
+    """An empty reference folder is no reason to fail: only the oracle's converters need its sources."""
+    import __graft_entry__
+    import build
+
+    monkeypatch.setattr(build, "build", lambda: None)  # (the library is there)
+    monkeypatch.setenv("MQ_REFERENCE", str(tmp_path))
+    __graft_entry__.build()
+    monkeypatch.setenv("MQ_REFERENCE", str(tmp_path / "none"))
+    __graft_entry__.build()
