@@ -441,21 +441,22 @@ typedef struct mq_kv_pages {
 } mq_kv_pages;
 
 /* The new tokens of a call, [tokens] rows, belong to `batch` sequences: sequence b has rows starts[b] .. starts[b + 1] - 1
- * (starts: int32 [batch + 1], rising; NULL: row b, one each) and lengths[b] positions in the cache, the new ones among them, so
- * that its row i of n is position lengths[b] - n + i. table: int32 [batch][width], ldt elements from row to row; only the
- * entries of positions below lengths[b] are read. All of these are device memory, read when the kernels run. Rows before
- * starts[0] and behind starts[batch] are left as they are. Starts that pass the tokens are reported (mq_device_status 27): the rows that
- * are there keep their positions, the others are left out. (mq_paged_attention alone takes an end that can be none, as 2^31 - 1, for
- * the rows' end, and does not report it: one that means more rows than width * page, and leaves no row that is there a position.) A table entry outside the pool is reported (19): its
- * rows are not written, and read as zeros. A length below 0 or above width * page is reported (20): mq_paged_attention cuts it, the
- * copies leave out the positions that the table does not name (not stored, loaded as zeros). A position below 0
- * (more rows than positions) is not stored, loads as zeros and sees nothing. */
+ * (starts: int32 [batch + 1], rising; NULL: row b, one each) and lengths[b] positions in the cache, the new ones among
+ * them, so that its row i of n, starts[b + 1] - starts[b], is position lengths[b] - n + i. table: int32 [batch][width],
+ * ldt elements from row to row; only the entries of positions below lengths[b] are read. All of these are device memory,
+ * read when the kernels run. Rows before starts[0] and behind starts[batch] are left as they are. Starts that pass the
+ * tokens are reported (mq_device_status 27): the rows that are there keep their positions, the others are left out.
+ * (mq_paged_attention alone takes an end that can be none, as 2^31 - 1, for the rows' end, and does not report it: one
+ * that means more rows than width * page, and leaves no row that is there a position.) A table entry outside the pool is
+ * reported (19): its rows are not written, and read as zeros. A length below 0 or above width * page is reported (20):
+ * mq_paged_attention cuts it, the copies leave out the positions that the table does not name (not stored, loaded as
+ * zeros). A position below 0 (more rows than positions) is not stored, loads as zeros and sees nothing. */
 
-/* k[t][h], v[t][h] -> the pages, rounded to their type; int8 as mq_quantize_s8 makes it, row by row (a row with a NaN or an
- * infinity: zeros and scale NaN). k, v: fp32, fp16 or bf16 (dtype), [tokens][heads][dim] with strides in elements, rows
- * 16-byte aligned. A position that two rows name (of sequences that share a page) gets either's
- * values, or a mix of the two, unless they are equal. Keys, values and scales must not share memory with one another (refused), nor
- * the rows with the pages. */
+/* k[t][h], v[t][h] -> the pages, rounded to their type; int8 as mq_quantize_s8 makes it, row by row (a row with a NaN or
+ * an infinity: zeros and scale NaN). k, v: fp32, fp16 or bf16 (dtype), [tokens][heads][dim] with strides in elements, rows
+ * 16-byte aligned. A position that two rows name (of sequences that share a page) gets either's values, or a mix of the
+ * two, unless they are equal. Keys, values and scales must not share memory with one another (refused), nor the rows with
+ * the pages. */
 MQ_API int mq_kv_store(const void *k, int64_t k_token, int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
                        int dtype, const mq_kv_pages *cache, const int32_t *table, int64_t ldt, int64_t width,
                        const int32_t *lengths, const int32_t *starts, int64_t batch, int64_t tokens, void *stream);
@@ -466,18 +467,18 @@ MQ_API int mq_kv_load(const mq_kv_pages *cache, const int32_t *table, int64_t ld
                       int64_t v_token, int64_t v_head, int dtype, void *stream);
 
 /* out[t][h] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale * q[t][h].k_j), over the positions j that row t sees: its own and
- * those before it, the last `window` of them (0: all). Query head h uses kv head h / (heads / cache->heads). q and out: fp16
- * or bf16 (q_dtype; a 16-bit cache's own type), [tokens][heads][dim] with strides in elements, rows 16-byte aligned; out may be
- * q's own buffer with q's strides; else it must not share memory with q, nor with the pages, nor
- * the workspace with any of these (refused). A row that sees no position, or only scores of -infinity, gives zeros. Positions that a
- * row does not see have no influence on it, whatever they hold; one that it sees and whose key or value holds a NaN, or its value an
- * infinity (int8: whose scale is either), makes it NaN or infinite. An infinity in a 16-bit key makes the score one: +infinity makes
- * the row NaN, a key of score -infinity has no weight. Scores, maxima and sums are fp32; the weights are rounded to the cache's type (int8: fp16) before they
- * meet the values; an int8 cache's integers are multiplied as they are, its scales in fp32. An int8 cache's scales must not be negative, and a value
- * scale below 1e-30 counts as 1e-30.
- * max_new: no sequence has more new tokens (0: unknown); one that has is reported (26) and its rows are left as they are.
- * scale > 0. Reproducible bit for bit. workspace: mq_paged_attention_workspace_size() bytes, 16-byte aligned (0 for sizes that
- * are refused); calls that may overlap in time need one each. tokens == 0 does nothing. */
+ * those before it, the last `window` of them (0: all). Query head h uses kv head h / (heads / cache->heads). q and out:
+ * fp16 or bf16 (q_dtype; a 16-bit cache's own type), [tokens][heads][dim] with strides in elements, rows 16-byte aligned;
+ * out may be q's own buffer with q's strides; else it must not share memory with q, nor with the pages, nor the workspace
+ * with any of these (refused). A row that sees no position, or only scores of -infinity, gives zeros. Positions that a row
+ * does not see have no influence on it, whatever they hold; one that it sees and whose key or value holds a NaN, or its
+ * value an infinity (int8: whose scale is either), makes it NaN or infinite. An infinity in a 16-bit key makes the score
+ * one: +infinity makes the row NaN, a key of score -infinity has no weight. Scores, maxima and sums are fp32; the weights
+ * are rounded to the cache's type (int8: fp16) before they meet the values; an int8 cache's integers are multiplied as
+ * they are, its scales in fp32. An int8 cache's scales must not be negative, and a value scale below 1e-30 counts as
+ * 1e-30. max_new: no sequence has more new tokens (0: unknown); one that has is reported (26) and its rows are left as
+ * they are. scale > 0. Reproducible bit for bit. workspace: mq_paged_attention_workspace_size() bytes, 16-byte aligned (0
+ * for sizes that are refused); calls that may overlap in time need one each. tokens == 0 does nothing. */
 MQ_API size_t mq_paged_attention_workspace_size(const mq_kv_pages *cache, int64_t heads, int64_t batch, int64_t tokens,
                                                 int64_t max_new);
 MQ_API int mq_paged_attention(const void *q, int q_dtype, int64_t q_token, int64_t q_head, const mq_kv_pages *cache,

@@ -242,8 +242,8 @@ inline bool share_bytes(const Area &any, const Area &apart) {
 }
 
 inline Area area_of_pages(const mq_kv_pages *c, const void *base, const int64_t *stride, int64_t es, int64_t row) {
-  return {static_cast<const char *>(base), row * es, {static_cast<__int128>(stride[0]) * es, static_cast<__int128>(stride[1]) * es, static_cast<__int128>(stride[2]) * es},
-          {c->pages, c->heads, c->page}};
+  const __int128 bytes = es;
+  return {static_cast<const char *>(base), row * es, {stride[0] * bytes, stride[1] * bytes, stride[2] * bytes}, {c->pages, c->heads, c->page}};
 }
 // A cache's keys, values and, int8, their scales: how many areas.
 inline int areas_of(const mq_kv_pages *c, Area (&a)[4]) {
@@ -254,7 +254,8 @@ inline int areas_of(const mq_kv_pages *c, Area (&a)[4]) {
   return 4;
 }
 inline Area area_of_rows(const void *base, int64_t es, int64_t tokens, int64_t heads, int64_t dim, int64_t token_stride, int64_t head_stride) {
-  return {static_cast<const char *>(base), dim * es, {static_cast<__int128>(token_stride) * es, static_cast<__int128>(head_stride) * es, 0}, {tokens, heads, 1}};
+  const __int128 bytes = es;
+  return {static_cast<const char *>(base), dim * es, {token_stride * bytes, head_stride * bytes, 0}, {tokens, heads, 1}};
 }
 
 // ---- attention: items, units and shares --------------------------------------------------------------
